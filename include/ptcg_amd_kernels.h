@@ -209,6 +209,56 @@ int ptcg_kernel_attention_bwd_ws(const float* qkv, const float* keep, const floa
  * recomputing S and dP per query stripe (longer rows); -1 unsupported.     */
 int ptcg_kernel_attention_path(int L, int Dh);
 
+/* Cross attention to an encoder's states of another length.  A sample's lq
+ * query rows of `heads` heads attend to its lk key / value rows of kv_heads
+ * heads (a divisor: query head h reads kv head h / (heads / kv_heads)), dh
+ * elements each (a multiple of 8, up to 128):
+ *   s_ij = scale q_i . k_j over the kept keys, P = softmax_j(s),
+ *   out_i = sum_j P_ij v_j, lse_i = log sum_j exp(s_ij).
+ * Element (sample, row, head, e) of q lies at q[sn sample + sl row + sh head +
+ * e]; the same for k, v and o (strides in elements, multiples of 16 bytes, 0
+ * allowed in inputs: a broadcast; buffers 16 B aligned).  Gradients lie as
+ * their tensors do, dout as out.
+ * q_off (device, n + 1 ascending ints): packed queries, sample i owns rows
+ * q_off[i] .. q_off[i + 1] - 1 of one long matrix (sn unused), at most lq of
+ * them; k_off the same for k, v and keep.  k_len (device, n ints, padded keys
+ * only): rows past k_len[i] are not read.  keep: 0 masks the key, padded at
+ * keep[keep_sn sample + row], packed at keep[row].  NULL each: all rows, all
+ * kept.  Masked rows may hold anything, NaN too; their dk and dv are zeros.
+ * Rows outside every packed sample stay as they were.
+ * A query that keeps no key gives out = 0, lse = -inf and no gradient.
+ * bf16: products of bf16 operands (P and dS rounded to bf16 for them),
+ * softmax, statistics and sums fp32.                                        */
+typedef struct PtcgHeadLayout {
+    int64_t sn, sl, sh;   /* strides of sample, row, head */
+} PtcgHeadLayout;
+typedef struct PtcgCrossAttn {
+    int n, lq, lk, heads, kv_heads, dh;
+    int bf16;      /* element type of q, k, v, out and their gradients: 0 fp32, 1 bf16 */
+    float scale;   /* of the scores, positive */
+    PtcgHeadLayout q, k, v, o;
+    const int32_t* q_off;
+    const int32_t* k_off;
+    const int32_t* k_len;
+    const float* keep;
+    int64_t keep_sn;
+} PtcgCrossAttn;
+/* bytes of scratch a call takes (backward = 0 / 1; 16 B aligned; 0: none;
+ * -1: the descriptor is refused).  Calls that may run at the same time need
+ * scratch of their own.                                                    */
+int64_t ptcg_kernel_cross_attention_ws_bytes(const PtcgCrossAttn* desc, int backward);
+/* lse (nullable: acting needs none) (n, heads, lq) fp32.  Few rows against
+ * many keys (a single token) split the keys over workgroups and join.
+ * No reference counterpart: its trunk attends to itself only.              */
+int ptcg_kernel_cross_attention_fwd(const PtcgCrossAttn* desc, const void* q, const void* k, const void* v,
+                                    void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                    void* stream);
+/* dq, dk, dv overwritten; dk and dv summed over the heads that share them, in
+ * a fixed order.                                                           */
+int ptcg_kernel_cross_attention_bwd(const PtcgCrossAttn* desc, const void* q, const void* k, const void* v,
+                                    const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                                    void* dv, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Launch timing: between begin and end, every GEMM, LayerNorm and Adam
  * launch (up to max_launches in all) is bracketed by a HIP event pair on its
  * own stream.  end waits for the events and returns the GEMM launches'

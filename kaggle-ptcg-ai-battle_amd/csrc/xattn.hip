@@ -1,0 +1,999 @@
+// Cross attention: query rows against an encoder's key / value rows of another
+// length, shared kv heads, key masks, padded or packed samples; fp32 or bf16.
+//
+// Forward, per (sample, query head), over the kept keys j:
+//   s_ij = scale q_i . k_j,  m_i = max_j s_ij,  l_i = sum_j exp(s_ij - m_i),
+//   o_i = sum_j exp(s_ij - m_i) v_j / l_i,  lse_i = m_i + log l_i,
+// in one pass over the keys: a tile's larger maximum rescales what is summed.
+// Backward, with P_ij = exp(s_ij - lse_i) and D_i = do_i . o_i:
+//   dv_j = sum_i P_ij do_i,  dS_ij = P_ij (do_i . v_j - D_i),
+//   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,
+// dk and dv summed over the query heads that share the kv head, in row order.
+// A query that keeps no key: o = 0, lse = -inf, and it adds to no gradient.
+//
+// Layout.  The G = heads / kv_heads query heads of a kv head are one matrix of
+// lq * G rows (row r is query r / G, head r % G), so a single token's heads
+// fill one tile and a gradient's sum over the heads is a sum over rows.  All
+// products run as 32 x 32 tiles of v_mfma_f32_32x32x16_bf16 or
+// v_mfma_f32_32x32x2_f32, computed transposed: S^T = K Q^T leaves query
+// lane % 32 of keys {8 (r / 4) + 4 (lane / 32) + r % 4} in register r, which is
+// a B operand of O^T = V^T P^T over the same order of the keys, so P goes from
+// accumulators to the next product without passing through LDS, and a
+// query's maximum and sum are in-lane but for one exchange of the halves.  The
+// A operand V^T comes from row-major LDS by ds_read_b64_tr_b16 (4 keys of 16
+// columns to a lane's 4 values); in fp32 by plain 32-bit reads.
+// LDS row strides: 32 bytes of padding in bf16 keep both the row reads (8 lanes
+// of 16 bytes) and the transposed reads (4 rows of 32 bytes) free of bank
+// conflicts; 16 bytes in fp32.
+#include "common.h"
+#include "../../include/ptcg_amd_kernels.h"
+
+#include <type_traits>
+
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// the descriptor as the kernels take it
+struct XArgs {
+    int n, lq, lk, H, KV, G, dh;
+    unsigned gmagic;              // r / G = umulhi(r, gmagic) for r G < 2^32 (G > 1)
+    float scale, scale2;          // scale2 = scale * log2(e): exponentials are exp2
+    PtcgHeadLayout q, k, v, o;
+    const int *q_off, *k_off, *k_len;
+    const float* keep;
+    long keep_sn;
+};
+
+struct Sample { long q, k, v, o, keep; int ql, kl; };   // element offsets of row 0, and row counts
+
+// Row counts come from device memory: they are held to the host's bounds.
+__device__ __forceinline__ Sample sample_of(const XArgs& a, int i) {
+    Sample s;
+    s.ql = a.lq; s.kl = a.lk;
+    if (a.q_off) {
+        const int r0 = a.q_off[i];
+        s.ql = max(0, min(a.lq, a.q_off[i + 1] - r0));
+        s.q = r0 * a.q.sl; s.o = r0 * a.o.sl;
+    } else {
+        s.q = i * a.q.sn; s.o = i * a.o.sn;
+    }
+    if (a.k_off) {
+        const int r0 = a.k_off[i];
+        s.kl = max(0, min(a.lk, a.k_off[i + 1] - r0));
+        s.k = r0 * a.k.sl; s.v = r0 * a.v.sl; s.keep = r0;
+    } else {
+        s.k = i * a.k.sn; s.v = i * a.v.sn; s.keep = i * a.keep_sn;
+        if (a.k_len) s.kl = max(0, min(a.lk, a.k_len[i]));
+    }
+    return s;
+}
+
+__device__ __forceinline__ int head_div(const XArgs& a, int r) {
+    return a.G == 1 ? r : (int)__umulhi((unsigned)r, a.gmagic);
+}
+// element offset of flattened query row r of kv head kvh (before the sample's)
+__device__ __forceinline__ long row_off(const XArgs& a, const PtcgHeadLayout& l, int kvh, int r) {
+    const int qi = head_div(a, r), g = r - qi * a.G;
+    return (long)qi * l.sl + (long)(kvh * a.G + g) * l.sh;
+}
+
+// Workgroups go to the 8 XCDs in turn; consecutive logical indexes on one XCD
+// share a sample's keys in its L2.
+__device__ __forceinline__ int xcd_block(int nblk) {
+    const int x = blockIdx.x & 7, per = nblk >> 3, rem = nblk & 7;
+    return x * per + min(x, rem) + (blockIdx.x >> 3);
+}
+
+__device__ __forceinline__ float half_swap(float v) { return __shfl_xor(v, 32, 64); }
+
+// ------------------------------------------------------------- fragments
+// A row operand's chunk c holds dims 2 EL c + EL (lane / 32) + e, e < EL.
+template <typename T> struct Frag;
+template <> struct Frag<__bf16> { typedef bf16x8 V; static constexpr int EL = 8, PAD = 16; };
+template <> struct Frag<float> { typedef floatx4 V; static constexpr int EL = 4, PAD = 4; };
+
+__device__ __forceinline__ void mma_row(bf16x8 a, bf16x8 b, floatx16& c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_row(floatx4 a, floatx4 b, floatx16& c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+}
+
+// 16-byte load of a row chunk
+template <typename T> __device__ __forceinline__ typename Frag<T>::V ldv(const T* p) {
+    return *reinterpret_cast<const typename Frag<T>::V*>(p);
+}
+template <typename T> __device__ __forceinline__ typename Frag<T>::V zerov() {
+    typename Frag<T>::V z;
+#pragma unroll
+    for (int e = 0; e < Frag<T>::EL; ++e) z[e] = (T)0.f;
+    return z;
+}
+
+// row fragments of one lane's global row (dims past dh, or no row: zeros)
+template <typename T, int DH>
+__device__ __forceinline__ void load_row(typename Frag<T>::V (&f)[DH / (2 * Frag<T>::EL)], const T* row, bool ok,
+                                         int dh, int h) {
+    constexpr int EL = Frag<T>::EL;
+#pragma unroll
+    for (int c = 0; c < DH / (2 * EL); ++c) {
+        const int d = 2 * EL * c + EL * h;
+        f[c] = ok && d < dh ? ldv<T>(row + d) : zerov<T>();
+    }
+}
+
+// c += X^T P over 32 rows of X (row-major in LDS from xs, stride ST): c[dt] is
+// columns 32 dt .. of X; P's register r stands for row 8 (r / 4) + 4 h + r % 4.
+// bf16: P is rounded to bf16 for the product (relative 2^-9 each, as the
+// stored operands are); its fp32 values make the softmax's sum.
+template <int DH, int ST>
+__device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floatx16 (&c)[DH / 32], int lane) {
+    typedef __attribute__((address_space(3))) bf16x4* lds4;
+    const int i = lane & 15, h = lane >> 5;
+    const __bf16* a0 = xs + (4 * h + (i >> 2)) * ST + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        bf16x8 b;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) b[e] = (__bf16)p[8 * kb + e];
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt) {
+            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(a0 + 16 * kb * ST + 32 * dt));
+            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(a0 + (16 * kb + 8) * ST + 32 * dt));
+            const bf16x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            c[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c[dt], 0, 0, 0);
+        }
+    }
+}
+template <int DH, int ST>
+__device__ __forceinline__ void mma_tr(const float* xs, const floatx16& p, floatx16 (&c)[DH / 32], int lane) {
+    const float* a0 = xs + 4 * (lane >> 5) * ST + (lane & 31);
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt)
+            c[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a0[(8 * (r / 4) + r % 4) * ST + 32 * dt], p[r], c[dt], 0, 0,
+                                                         0);
+}
+
+// s = X Y^T of 32 LDS rows against a lane's row fragments
+template <typename T, int DH, int ST>
+__device__ __forceinline__ floatx16 mma_rows(const T* xs, const typename Frag<T>::V (&f)[DH / (2 * Frag<T>::EL)],
+                                             int lane) {
+    constexpr int EL = Frag<T>::EL;
+    floatx16 s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+    const T* x = xs + (lane & 31) * ST + EL * (lane >> 5);
+#pragma unroll
+    for (int c = 0; c < DH / (2 * EL); ++c) mma_row(ldv<T>(x + 2 * EL * c), f[c], s);
+    return s;
+}
+
+// A tile of BR rows on its way through registers into LDS: 16-byte chunks,
+// thread t takes chunks t, t + NTH, ...  Loads are issued a tile ahead of the
+// barrier that publishes them.
+template <typename T, int DH, int BR, int NTH> struct Stage {
+    static constexpr int E = Frag<T>::EL, CPR = DH / E, NCH = BR * CPR / NTH, ST = DH + Frag<T>::PAD;
+    static_assert(BR * CPR % NTH == 0, "whole chunks per thread");
+    typename Frag<T>::V r[NCH];
+    // rows row0 + [0, BR) of a matrix at base (row stride sl), rows < len
+    __device__ __forceinline__ void load(const T* base, long sl, int row0, int len, int dh, int tid) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = tid + i * NTH, row = row0 + c / CPR, col = (c % CPR) * E;
+            r[i] = row < len && col < dh ? ldv<T>(base + row * sl + col) : zerov<T>();
+        }
+    }
+    // rows of the flattened query matrix of kv head kvh
+    __device__ __forceinline__ void load_q(const XArgs& a, const PtcgHeadLayout& l, const T* base, int kvh, int row0,
+                                           int len, int tid) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = tid + i * NTH, row = row0 + c / CPR, col = (c % CPR) * E;
+            r[i] = row < len && col < a.dh ? ldv<T>(base + row_off(a, l, kvh, row) + col) : zerov<T>();
+        }
+    }
+    // whether each chunk's row is kept (masked rows enter LDS as zeros, so
+    // that what they hold, NaN too, reaches no product)
+    __device__ __forceinline__ void keeps(bool (&kp)[NCH], const float* keep, int row0, int len, int tid) const {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int row = row0 + (tid + i * NTH) / CPR;
+            kp[i] = !keep || (row < len && keep[row] != 0.f);
+        }
+    }
+    __device__ __forceinline__ void store(T* s, int tid, const bool (&kp)[NCH]) const {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = tid + i * NTH;
+            *reinterpret_cast<typename Frag<T>::V*>(s + (c / CPR) * ST + (c % CPR) * E) = kp[i] ? r[i] : zerov<T>();
+        }
+    }
+    __device__ __forceinline__ void store(T* s, int tid) const {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int c = tid + i * NTH;
+            *reinterpret_cast<typename Frag<T>::V*>(s + (c / CPR) * ST + (c % CPR) * E) = r[i];
+        }
+    }
+};
+
+// the last kept key of [k0, kend), plus one (k0 if none): keys behind a
+// sample's valid prefix are not read.  Every thread of the workgroup calls it.
+__device__ __forceinline__ int last_kept(const float* keep, int k0, int kend, int nth, int* sh) {
+    if (threadIdx.x == 0) *sh = k0;
+    __syncthreads();
+    int last = k0;
+    for (int j = k0 + threadIdx.x; j < kend; j += nth)
+        if (keep[j] != 0.f) last = j + 1;
+    if (last > k0) atomicMax(sh, last);
+    __syncthreads();
+    return *sh;
+}
+
+// a lane's 4 consecutive output values
+__device__ __forceinline__ void st4(float* p, float a, float b, float c, float d) {
+    *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+__device__ __forceinline__ void st4(__bf16* p, float a, float b, float c, float d) {
+    *reinterpret_cast<bf16x4*>(p) = bf16x4{(__bf16)a, (__bf16)b, (__bf16)c, (__bf16)d};
+}
+// row (lane % 32) of a transposed accumulator, times f
+template <typename T, int DH>
+__device__ __forceinline__ void store_row(T* row, const floatx16 (&o)[DH / 32], float f, int dh, int h) {
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int d = 32 * dt + 8 * b + 4 * h;
+            if (d < dh)
+                st4(row + d, o[dt][4 * b] * f, o[dt][4 * b + 1] * f, o[dt][4 * b + 2] * f, o[dt][4 * b + 3] * f);
+        }
+}
+
+template <typename T, int DH, int BR> constexpr int tile_elems() { return BR * (DH + Frag<T>::PAD); }
+
+// ---------------------------------------------------------------- forward
+// A workgroup owns 32 NW query rows; KS waves share a row block and split each
+// tile of KS * KT keys (few rows against many keys), joined in LDS at the end.
+// nsplit > 1: workgroups also split the keys, each leaving an unnormalised
+// partial with its maximum and sum for xattn_join_kernel.
+template <typename T, int DH, int NW, int KS, int KT> struct FwdCfg {
+    static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
+    static constexpr size_t TILES = 2 * (size_t)tile_elems<T, DH, BK>() * sizeof(T);
+    static constexpr size_t JOIN = (size_t)NW * (KS - 1) * (DH * 32 + 64) * sizeof(float);
+    static constexpr size_t LDS = (TILES > JOIN ? TILES : JOIN) + BK * sizeof(float) + 16;
+};
+
+template <typename T, int DH, int NW, int KS, int KT>
+__global__ __launch_bounds__(64 * NW * KS) void xattn_fwd_kernel(const XArgs a, const T* __restrict__ q,
+        const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
+        float* __restrict__ part, int qtiles, int nsplit, int split_keys) {
+    typedef FwdCfg<T, DH, NW, KS, KT> C;
+    typedef Stage<T, DH, C::BK, C::NTH> St;
+    extern __shared__ __align__(16) char smem[];
+    T* Ks = reinterpret_cast<T*>(smem);
+    T* Vs = Ks + tile_elems<T, DH, C::BK>();
+    float* kf = reinterpret_cast<float*>(smem + C::LDS - 16 - C::BK * sizeof(float));
+    int* sh = reinterpret_cast<int*>(smem + C::LDS - 16);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int qw = wave % NW, kw = wave / NW;
+    int b = xcd_block(gridDim.x);
+    const int qt = b % qtiles; b /= qtiles;
+    const int sp = b % nsplit; b /= nsplit;
+    const int kvh = b % a.KV, i = b / a.KV;
+    const Sample s = sample_of(a, i);
+    const int rows = s.ql * a.G;
+    if (qt * C::BQ >= rows) return;
+    const int r = qt * C::BQ + 32 * qw + (lane & 31);
+    const bool rok = r < rows;
+
+    const T* kb = k + s.k + (long)kvh * a.k.sh;
+    const T* vb = v + s.v + (long)kvh * a.v.sh;
+    const float* keep = a.keep ? a.keep + s.keep : nullptr;
+    const int k0 = sp * split_keys;
+    int kend = min(s.kl, k0 + split_keys);
+    if (keep && k0 < kend) kend = last_kept(keep, k0, kend, C::NTH, sh);
+    const int nt = kend > k0 ? (kend - k0 + C::BK - 1) / C::BK : 0;
+
+    typename Frag<T>::V qf[DH / (2 * Frag<T>::EL)];
+    load_row<T, DH>(qf, q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
+
+    float m2 = -INFINITY, l = 0.f;   // running maximum (of s scale2) and this half's sum
+    floatx16 o[DH / 32];
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
+
+    St ks, vs;
+    bool kp[St::NCH];
+    float kfr = 0.f;
+    auto fetch = [&](int t) {
+        const int row0 = k0 + t * C::BK;
+        ks.load(kb, a.k.sl, row0, kend, a.dh, tid);
+        vs.load(vb, a.v.sl, row0, kend, a.dh, tid);
+        ks.keeps(kp, keep, row0, kend, tid);
+        if (tid < C::BK) {
+            const int j = row0 + tid;
+            kfr = j < kend && (!keep || keep[j] != 0.f) ? 0.f : -INFINITY;
+        }
+    };
+    if (nt > 0) fetch(0);
+    for (int t = 0; t < nt; ++t) {
+        __syncthreads();
+        ks.store(Ks, tid, kp);
+        vs.store(Vs, tid, kp);
+        if (tid < C::BK) kf[tid] = kfr;
+        __syncthreads();
+        if (t + 1 < nt) fetch(t + 1);
+        const int row0 = k0 + t * C::BK + kw * KT;
+        if (row0 >= kend) continue;
+        const bool masked = keep || row0 + KT > kend;
+        floatx16 sc[KT / 32];
+        float mt = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j) {
+            sc[j] = mma_rows<T, DH, St::ST>(Ks + (kw * KT + 32 * j) * St::ST, qf, lane);
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 f = *reinterpret_cast<const float4*>(kf + kw * KT + 32 * j + 8 * e + 4 * h);
+                    sc[j][4 * e] += f.x; sc[j][4 * e + 1] += f.y; sc[j][4 * e + 2] += f.z; sc[j][4 * e + 3] += f.w;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, sc[j][e]);
+        }
+        mt = fmaxf(mt, half_swap(mt));
+        const float mn = fmaxf(m2, mt * a.scale2);
+        if (__any(mn > m2)) {
+            const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m2 - mn);
+            l *= al;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] *= al;
+            m2 = mn;
+        }
+        const float ms = m2 == -INFINITY ? 0.f : m2;
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[j][e] = __builtin_amdgcn_exp2f(fmaf(sc[j][e], a.scale2, -ms));
+                l += sc[j][e];
+            }
+            mma_tr<DH, St::ST>(Vs + (kw * KT + 32 * j) * St::ST, sc[j], o, lane);
+        }
+    }
+    l += half_swap(l);
+
+    // the key waves' results join in LDS, in wave order
+    if constexpr (KS > 1) {
+        __syncthreads();
+        float* jb = reinterpret_cast<float*>(smem);
+        constexpr int JS = DH * 32 + 64;
+        if (kw > 0) {
+            float* p = jb + (size_t)((kw - 1) * NW + qw) * JS;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) p[(dt * 16 + e) * 64 + lane] = o[dt][e];
+            if (h == 0) {
+                p[DH * 32 + lane] = m2;
+                p[DH * 32 + 32 + lane] = l;
+            }
+        }
+        __syncthreads();
+        if (kw > 0) return;
+        for (int w = 1; w < KS; ++w) {
+            const float* p = jb + (size_t)((w - 1) * NW + qw) * JS;
+            const float mw = p[DH * 32 + (lane & 31)], lw = p[DH * 32 + 32 + (lane & 31)];
+            const float mn = fmaxf(m2, mw), ms = mn == -INFINITY ? 0.f : mn;
+            const float f0 = __builtin_amdgcn_exp2f(m2 - ms), f1 = __builtin_amdgcn_exp2f(mw - ms);
+            l = l * f0 + lw * f1;
+            m2 = mn;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * f0 + p[(dt * 16 + e) * 64 + lane] * f1;
+        }
+    }
+    if (!rok) return;
+    const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
+    const long row = ((long)i * a.H + head) * a.lq + qi;
+    if (nsplit > 1) {
+        const long R = (long)a.n * a.H * a.lq;
+        float* p = part + ((long)sp * R + row) * a.dh;
+        store_row<float, DH>(p, o, 1.f, a.dh, h);
+        if (h == 0) {
+            float* ml = part + (long)nsplit * R * a.dh + ((long)sp * R + row) * 2;
+            ml[0] = m2;
+            ml[1] = l;
+        }
+        return;
+    }
+    // no key kept: no tile was read and the sum is 0 (scores of NaN leave the
+    // maximum at -inf too, but a sum of NaN), whatever the query holds
+    const bool none = m2 == -INFINITY && l == 0.f;
+    if (none) {
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
+    }
+    store_row<T, DH>(out + s.o + row_off(a, a.o, kvh, r), o, none ? 0.f : 1.f / l, a.dh, h);
+    if (lse && h == 0) lse[row] = none ? -INFINITY : m2 * LN2 + logf(l);
+}
+
+// joins the key splits of one row per wave, in split order
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_join_kernel(const XArgs a, const float* __restrict__ part,
+        T* __restrict__ out, float* __restrict__ lse, int nsplit) {
+    const int lane = threadIdx.x & 63;
+    const long R = (long)a.n * a.H * a.lq, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= R) return;
+    const int qi = (int)(row % a.lq), head = (int)(row / a.lq % a.H), i = (int)(row / a.lq / a.H);
+    const Sample s = sample_of(a, i);
+    if (qi >= s.ql) return;
+    const float* ml = part + (long)nsplit * R * a.dh;
+    float m = -INFINITY;
+    for (int p = lane; p < nsplit; p += 64) m = fmaxf(m, ml[((long)p * R + row) * 2]);
+    m = wave_max(m);
+    const float ms = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    for (int p = lane; p < nsplit; p += 64) {
+        const float* e = ml + ((long)p * R + row) * 2;
+        l += e[1] * __builtin_amdgcn_exp2f(e[0] - ms);
+    }
+    l = wave_sum(l);
+    const bool none = m == -INFINITY && l == 0.f;
+    T* orow = out + s.o + (long)qi * a.o.sl + (long)head * a.o.sh;
+    for (int d = lane; d < a.dh; d += 64) {
+        float acc = 0.f;
+        if (!none)
+#pragma unroll 4
+            for (int p = 0; p < nsplit; ++p) {
+                const long e = (long)p * R + row;
+                acc += part[e * a.dh + d] * __builtin_amdgcn_exp2f(ml[e * 2] - ms);
+            }
+        orow[d] = (T)(none ? 0.f : acc / l);
+    }
+    if (lse && lane == 0) lse[row] = none ? -INFINITY : m * LN2 + logf(l);
+}
+
+// --------------------------------------------------------------- backward
+// dQ: the forward's shape.  Per 32 keys S^T and dP^T = V dO^T with queries on
+// lanes, dS^T in registers, dQ^T += K^T dS^T.  Also leaves D_i (from the
+// stored o: in bf16 its rounding moves D by 2^-9 of terms that average out)
+// for the dK / dV kernel, in row order of lse.
+template <typename T, int DH, int NW, int KS, int KT> struct DqCfg {
+    static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
+    static constexpr size_t TILES = 2 * (size_t)tile_elems<T, DH, BK>() * sizeof(T);
+    static constexpr size_t JOIN = (size_t)NW * (KS - 1) * DH * 32 * sizeof(float);
+    static constexpr size_t LDS = (TILES > JOIN ? TILES : JOIN) + BK * sizeof(float) + 16;
+};
+
+template <typename T, int DH, int NW, int KS, int KT>
+__global__ __launch_bounds__(64 * NW * KS) void xattn_dq_kernel(const XArgs a, const T* __restrict__ q,
+        const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ out,
+        const float* __restrict__ lse, const T* __restrict__ dout, T* __restrict__ dq,
+        float* __restrict__ delta, int qtiles) {
+    typedef DqCfg<T, DH, NW, KS, KT> C;
+    typedef Stage<T, DH, C::BK, C::NTH> St;
+    constexpr int EL = Frag<T>::EL, NF = DH / (2 * EL);
+    extern __shared__ __align__(16) char smem[];
+    T* Ks = reinterpret_cast<T*>(smem);
+    T* Vs = Ks + tile_elems<T, DH, C::BK>();
+    float* kf = reinterpret_cast<float*>(smem + C::LDS - 16 - C::BK * sizeof(float));
+    int* sh = reinterpret_cast<int*>(smem + C::LDS - 16);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int qw = wave % NW, kw = wave / NW;
+    int b = xcd_block(gridDim.x);
+    const int qt = b % qtiles; b /= qtiles;
+    const int kvh = b % a.KV, i = b / a.KV;
+    const Sample s = sample_of(a, i);
+    const int rows = s.ql * a.G;
+    if (qt * C::BQ >= rows) return;
+    const int r = qt * C::BQ + 32 * qw + (lane & 31);
+    const bool rok = r < rows;
+
+    typename Frag<T>::V qf[NF], df[NF];
+    load_row<T, DH>(qf, q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
+    const long oo = s.o + (rok ? row_off(a, a.o, kvh, r) : 0);
+    load_row<T, DH>(df, dout + oo, rok, a.dh, h);
+    const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
+    const long lrow = ((long)i * a.H + head) * a.lq + qi;
+    const float lr = rok ? lse[lrow] : -INFINITY;
+    const bool none = lr == -INFINITY;
+    const float l2 = none ? INFINITY : lr * LOG2E;
+    float D = 0.f;
+    {
+        typename Frag<T>::V of[NF];
+        load_row<T, DH>(of, out + oo, rok, a.dh, h);
+#pragma unroll
+        for (int c = 0; c < NF; ++c)
+#pragma unroll
+            for (int e = 0; e < EL; ++e) D += (float)of[c][e] * (float)df[c][e];
+    }
+    D += half_swap(D);
+    if (rok && kw == 0 && h == 0) delta[lrow] = D;
+
+    const T* kb = k + s.k + (long)kvh * a.k.sh;
+    const T* vb = v + s.v + (long)kvh * a.v.sh;
+    const float* keep = a.keep ? a.keep + s.keep : nullptr;
+    int kend = s.kl;
+    if (keep && kend > 0) kend = last_kept(keep, 0, kend, C::NTH, sh);
+    const int nt = (kend + C::BK - 1) / C::BK;
+
+    floatx16 g[DH / 32];
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) g[dt][e] = 0.f;
+    St ks, vs;
+    bool kp[St::NCH];
+    float kfr = 0.f;
+    auto fetch = [&](int t) {
+        const int row0 = t * C::BK;
+        ks.load(kb, a.k.sl, row0, kend, a.dh, tid);
+        vs.load(vb, a.v.sl, row0, kend, a.dh, tid);
+        ks.keeps(kp, keep, row0, kend, tid);
+        if (tid < C::BK) {
+            const int j = row0 + tid;
+            kfr = j < kend && (!keep || keep[j] != 0.f) ? 0.f : -INFINITY;
+        }
+    };
+    if (nt > 0) fetch(0);
+    for (int t = 0; t < nt; ++t) {
+        __syncthreads();
+        ks.store(Ks, tid, kp);
+        vs.store(Vs, tid, kp);
+        if (tid < C::BK) kf[tid] = kfr;
+        __syncthreads();
+        if (t + 1 < nt) fetch(t + 1);
+#pragma unroll 1
+        for (int j = 0; j < KT / 32; ++j) {
+            const int kr = kw * KT + 32 * j, row0 = t * C::BK + kr;
+            if (row0 >= kend) break;
+            const bool masked = keep || row0 + 32 > kend;
+            floatx16 sc = mma_rows<T, DH, St::ST>(Ks + kr * St::ST, qf, lane);
+            const floatx16 dp = mma_rows<T, DH, St::ST>(Vs + kr * St::ST, df, lane);
+            if (masked) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float4 f = *reinterpret_cast<const float4*>(kf + kr + 8 * e + 4 * h);
+                    sc[4 * e] += f.x; sc[4 * e + 1] += f.y; sc[4 * e + 2] += f.z; sc[4 * e + 3] += f.w;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -l2)) * (dp[e] - D);
+            mma_tr<DH, St::ST>(Ks + kr * St::ST, sc, g, lane);
+        }
+    }
+    if constexpr (KS > 1) {
+        __syncthreads();
+        float* jb = reinterpret_cast<float*>(smem);
+        if (kw > 0) {
+            float* p = jb + (size_t)((kw - 1) * NW + qw) * DH * 32;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) p[(dt * 16 + e) * 64 + lane] = g[dt][e];
+        }
+        __syncthreads();
+        if (kw > 0) return;
+        for (int w = 1; w < KS; ++w) {
+            const float* p = jb + (size_t)((w - 1) * NW + qw) * DH * 32;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) g[dt][e] += p[(dt * 16 + e) * 64 + lane];
+        }
+    }
+    if (!rok) return;
+    if (none) {
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) g[dt][e] = 0.f;
+    }
+    store_row<T, DH>(dq + s.q + row_off(a, a.q, kvh, r), g, a.scale, a.dh, h);
+}
+
+// dK and dV: a workgroup owns 32 NK keys of one kv head, a wave 32 of them, and
+// walks the flattened query rows in tiles of QS * QT (QS waves share a key
+// block and split each tile).  S = Q K^T and dP = dO V^T with keys on lanes;
+// dV^T += dO^T P and dK^T += Q^T dS read dO and Q transposed from LDS.
+template <typename T, int DH, int NK, int QS, int QT> struct DkvCfg {
+    static constexpr int NTH = 64 * NK * QS, BKEY = 32 * NK, BQ = QT * QS;
+    static constexpr size_t TILES = 2 * (size_t)tile_elems<T, DH, BQ>() * sizeof(T);
+    static constexpr size_t JOIN = (size_t)NK * (QS - 1) * 2 * DH * 32 * sizeof(float);
+    static constexpr size_t LDS = (TILES > JOIN ? TILES : JOIN) + 2 * BQ * sizeof(float) + 16;
+};
+
+template <typename T, int DH, int NK, int QS, int QT>
+__global__ __launch_bounds__(64 * NK * QS) void xattn_dkv_kernel(const XArgs a, const T* __restrict__ q,
+        const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ lse,
+        const T* __restrict__ dout, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
+        int ktiles) {
+    typedef DkvCfg<T, DH, NK, QS, QT> C;
+    typedef Stage<T, DH, C::BQ, C::NTH> St;
+    constexpr int NF = DH / (2 * Frag<T>::EL);
+    extern __shared__ __align__(16) char smem[];
+    T* Qs = reinterpret_cast<T*>(smem);
+    T* Ds = Qs + tile_elems<T, DH, C::BQ>();
+    float* ls = reinterpret_cast<float*>(smem + C::LDS - 16 - 2 * C::BQ * sizeof(float));
+    float* dl = ls + C::BQ;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int kwv = wave % NK, qs = wave / NK;
+    int b = xcd_block(gridDim.x);
+    const int kt = b % ktiles; b /= ktiles;
+    const int kvh = b % a.KV, i = b / a.KV;
+    const Sample s = sample_of(a, i);
+    const int kall = a.k_off ? s.kl : a.lk;   // padded rows past k_len get zeros
+    if (kt * C::BKEY >= kall) return;
+    const int key = kt * C::BKEY + 32 * kwv + (lane & 31);
+    const bool kin = key < kall;
+    const bool kok = key < s.kl && (!a.keep || a.keep[s.keep + key] != 0.f);
+
+    typename Frag<T>::V kfr[NF], vfr[NF];
+    const long ko = s.k + (kin ? (long)key * a.k.sl + (long)kvh * a.k.sh : 0);
+    const long vo = s.v + (kin ? (long)key * a.v.sl + (long)kvh * a.v.sh : 0);
+    load_row<T, DH>(kfr, k + ko, kok, a.dh, h);
+    load_row<T, DH>(vfr, v + vo, kok, a.dh, h);
+    floatx16 gk[DH / 32], gv[DH / 32];
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
+
+    const int rows = __syncthreads_or(kok) ? s.ql * a.G : 0;   // a block that keeps no key has no gradient
+    const int nt = (rows + C::BQ - 1) / C::BQ;
+    St qs_, ds_;
+    float lr = 0.f, dr = 0.f;
+    auto fetch = [&](int t) {
+        const int row0 = t * C::BQ;
+        qs_.load_q(a, a.q, q + s.q, kvh, row0, rows, tid);
+        ds_.load_q(a, a.o, dout + s.o, kvh, row0, rows, tid);
+        if (tid < C::BQ) {
+            const int r = row0 + tid;
+            lr = INFINITY;   // exp2(s - inf) = 0: rows past the end add nothing
+            dr = 0.f;
+            if (r < rows) {
+                const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
+                const long lrow = ((long)i * a.H + head) * a.lq + qi;
+                lr = lse[lrow];
+                lr = lr == -INFINITY ? INFINITY : lr * LOG2E;
+                dr = delta[lrow];
+            }
+        }
+    };
+    if (nt > 0) fetch(0);
+    for (int t = 0; t < nt; ++t) {
+        __syncthreads();
+        qs_.store(Qs, tid);
+        ds_.store(Ds, tid);
+        if (tid < C::BQ) {
+            ls[tid] = lr;
+            dl[tid] = dr;
+        }
+        __syncthreads();
+        if (t + 1 < nt) fetch(t + 1);
+#pragma unroll 1
+        for (int j = 0; j < QT / 32; ++j) {
+            const int qr = qs * QT + 32 * j;
+            if (t * C::BQ + qr >= rows) break;
+            floatx16 p = mma_rows<T, DH, St::ST>(Qs + qr * St::ST, kfr, lane);
+            floatx16 d = mma_rows<T, DH, St::ST>(Ds + qr * St::ST, vfr, lane);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float4 lf = *reinterpret_cast<const float4*>(ls + qr + 8 * e + 4 * h);
+                const float4 df = *reinterpret_cast<const float4*>(dl + qr + 8 * e + 4 * h);
+                const float lv[4] = {lf.x, lf.y, lf.z, lf.w}, dv4[4] = {df.x, df.y, df.z, df.w};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float pe = __builtin_amdgcn_exp2f(fmaf(p[4 * e + x], a.scale2, -lv[x]));
+                    p[4 * e + x] = kok ? pe : 0.f;
+                    d[4 * e + x] = kok ? pe * (d[4 * e + x] - dv4[x]) : 0.f;
+                }
+            }
+            mma_tr<DH, St::ST>(Ds + qr * St::ST, p, gv, lane);
+            mma_tr<DH, St::ST>(Qs + qr * St::ST, d, gk, lane);
+        }
+    }
+    if constexpr (QS > 1) {
+        __syncthreads();
+        float* jb = reinterpret_cast<float*>(smem);
+        if (qs > 0) {
+            float* p = jb + (size_t)((qs - 1) * NK + kwv) * 2 * DH * 32;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    p[(dt * 16 + e) * 64 + lane] = gk[dt][e];
+                    p[DH * 32 + (dt * 16 + e) * 64 + lane] = gv[dt][e];
+                }
+        }
+        __syncthreads();
+        if (qs > 0) return;
+        for (int w = 1; w < QS; ++w) {
+            const float* p = jb + (size_t)((w - 1) * NK + kwv) * 2 * DH * 32;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    gk[dt][e] += p[(dt * 16 + e) * 64 + lane];
+                    gv[dt][e] += p[DH * 32 + (dt * 16 + e) * 64 + lane];
+                }
+        }
+    }
+    if (!kin) return;
+    if (!kok) {   // a masked key's gradient is zero, whatever the rows hold
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
+    }
+    store_row<T, DH>(dk + ko, gk, a.scale, a.dh, h);
+    store_row<T, DH>(dv + vo, gv, 1.f, a.dh, h);
+}
+
+// ------------------------------------------------------------------- host
+int cu_count() {
+    int dev = 0, cu = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&cu, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cu <= 0)
+        return 256;
+    return cu;
+}
+
+// rows (or keys) a workgroup covers: waves along them, the rest of the four
+// split the other axis
+int waves_for(long rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+
+struct Plan { int nw, qtiles, nsplit, split_keys; };
+
+// Key splits (forward): where the rows' workgroups leave CUs idle, enough
+// workgroups for two per CU, at least four tiles of keys in each.
+Plan fwd_plan(const PtcgCrossAttn* d) {
+    Plan p;
+    const long rows = (long)d->lq * (d->heads / d->kv_heads);
+    p.nw = waves_for(rows);
+    p.qtiles = pt_cdiv(rows, 32 * p.nw);
+    const int bk = p.nw == 1 ? 128 : 64;
+    const long blocks = (long)d->n * d->kv_heads * p.qtiles;
+    const int cu = cu_count();
+    p.nsplit = 1;
+    p.split_keys = d->lk;
+    if (blocks < cu && d->lk >= 8 * bk) {
+        const long want = (2 * cu + blocks - 1) / blocks, most = d->lk / (4 * bk);
+        const int tiles = pt_cdiv(d->lk, bk);
+        const int sp = (int)(want < most ? want : most);
+        const int per = pt_cdiv(tiles, sp);
+        p.split_keys = per * bk;
+        p.nsplit = pt_cdiv(d->lk, p.split_keys);
+    }
+    return p;
+}
+
+bool layout_ok(const PtcgHeadLayout& l, int e) { return l.sn >= 0 && l.sl >= 0 && l.sh >= 0 && l.sn % e == 0 && l.sl % e == 0 && l.sh % e == 0; }
+
+// whether no two elements of an output share an address (offsets: the sample
+// stride is unused)
+bool layout_apart(const PtcgHeadLayout& l, int n, int rows, int heads, int dh) {
+    int64_t st[3] = {n > 1 ? l.sn : -1, rows > 1 ? l.sl : -1, heads > 1 ? l.sh : -1};
+    int64_t ex[3] = {n, rows, heads};
+    for (int i = 0; i < 3; ++i)
+        for (int j = i + 1; j < 3; ++j)
+            if (st[j] < st[i]) {
+                const int64_t t = st[i]; st[i] = st[j]; st[j] = t;
+                const int64_t u = ex[i]; ex[i] = ex[j]; ex[j] = u;
+            }
+    int64_t span = dh;
+    for (int i = 0; i < 3; ++i) {
+        if (st[i] < 0) continue;
+        if (st[i] < span) return false;
+        span = st[i] * (ex[i] - 1) + span;
+    }
+    return true;
+}
+
+int check_desc(const PtcgCrossAttn* d, const char* who) {
+    PT_REQUIRE(d, "%s: null descriptor", who);
+    PT_REQUIRE(d->n >= 0 && d->lq >= 0 && d->lk >= 0, "%s: negative size n=%d lq=%d lk=%d", who, d->n, d->lq, d->lk);
+    PT_REQUIRE(d->heads >= 1 && d->kv_heads >= 1 && d->heads % d->kv_heads == 0,
+               "%s: %d heads over %d kv heads", who, d->heads, d->kv_heads);
+    PT_REQUIRE(d->dh >= 8 && d->dh <= 128 && d->dh % 8 == 0, "%s: head width %d is not a multiple of 8 up to 128", who,
+               d->dh);
+    PT_REQUIRE(d->bf16 == 0 || d->bf16 == 1, "%s: bf16=%d", who, d->bf16);
+    PT_REQUIRE(d->scale > 0.f && d->scale < 1e30f, "%s: scale must be positive and finite", who);
+    PT_REQUIRE(!(d->k_off && d->k_len), "%s: packed keys (k_off) take no k_len", who);
+    PT_REQUIRE(!d->keep || d->k_off || d->n <= 1 || d->keep_sn >= 0, "%s: negative keep stride", who);
+    const int e = d->bf16 ? 8 : 4;
+    PT_REQUIRE(layout_ok(d->q, e) && layout_ok(d->k, e) && layout_ok(d->v, e) && layout_ok(d->o, e),
+               "%s: strides must be non-negative multiples of 16 bytes", who);
+    const int64_t G = d->heads / d->kv_heads, rows = (int64_t)d->lq * G;
+    PT_REQUIRE(rows * G < (1LL << 32) && rows < (1LL << 31) - 256 && d->lk < (1 << 30),
+               "%s: lq=%d lk=%d with %d heads a kv head is too long", who, d->lq, d->lk, (int)G);
+    PT_REQUIRE((int64_t)d->n * d->kv_heads * (rows / 32 + 1) < (1LL << 30) &&
+                   (int64_t)d->n * d->kv_heads * (d->lk / 32 + 1) < (1LL << 30) &&
+                   (int64_t)d->n * d->heads * d->lq < (1LL << 32),
+               "%s: too many tiles", who);
+    return PTCG_OK;
+}
+
+XArgs to_args(const PtcgCrossAttn* d) {
+    XArgs a;
+    a.n = d->n; a.lq = d->lq; a.lk = d->lk; a.H = d->heads; a.KV = d->kv_heads;
+    a.G = d->heads / d->kv_heads; a.dh = d->dh;
+    a.gmagic = (unsigned)((1ULL << 32) / a.G + 1);
+    a.scale = d->scale; a.scale2 = d->scale * LOG2E;
+    a.q = d->q; a.k = d->k; a.v = d->v; a.o = d->o;
+    a.q_off = d->q_off; a.k_off = d->k_off; a.k_len = d->k_len;
+    a.keep = d->keep; a.keep_sn = d->keep_sn;
+    return a;
+}
+
+bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <typename K> int lds_attr(K kernel, size_t bytes) {
+    if (bytes > 64 * 1024)
+        PT_HIP(hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    return PTCG_OK;
+}
+
+template <typename T, int DH, int NW, int KS, int KT>
+int launch_fwd(const XArgs& a, const Plan& p, const void* q, const void* k, const void* v, void* out, float* lse,
+               float* part, hipStream_t s) {
+    typedef FwdCfg<T, DH, NW, KS, KT> C;
+    auto kern = xattn_fwd_kernel<T, DH, NW, KS, KT>;
+    PT_TRY(lds_attr(kern, C::LDS));
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.n * a.KV * (long)p.qtiles * p.nsplit)), dim3(C::NTH), C::LDS, s, a,
+                       static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                       static_cast<T*>(out), lse, part, p.qtiles, p.nsplit, p.split_keys);
+    PT_LAUNCH_CHECK();
+    if (p.nsplit > 1) {
+        hipLaunchKernelGGL(xattn_join_kernel<T>, dim3(pt_cdiv((long)a.n * a.H * a.lq, 4)), dim3(256), 0, s, a, part,
+                           static_cast<T*>(out), lse, p.nsplit);
+        PT_LAUNCH_CHECK();
+    }
+    return PTCG_OK;
+}
+
+template <typename T, int DH>
+int fwd_nw(const XArgs& a, const Plan& p, const void* q, const void* k, const void* v, void* out, float* lse,
+           float* part, hipStream_t s) {
+    if (p.nw == 1) return launch_fwd<T, DH, 1, 4, 32>(a, p, q, k, v, out, lse, part, s);
+    if (p.nw == 2) return launch_fwd<T, DH, 2, 2, 32>(a, p, q, k, v, out, lse, part, s);
+    return launch_fwd<T, DH, 4, 1, 64>(a, p, q, k, v, out, lse, part, s);
+}
+
+template <typename T, int DH, int NW, int KS, int KT>
+int launch_dq(const XArgs& a, const void* q, const void* k, const void* v, const void* out, const float* lse,
+              const void* dout, void* dq, float* delta, hipStream_t s) {
+    typedef DqCfg<T, DH, NW, KS, KT> C;
+    auto kern = xattn_dq_kernel<T, DH, NW, KS, KT>;
+    PT_TRY(lds_attr(kern, C::LDS));
+    const int qtiles = pt_cdiv((long)a.lq * a.G, C::BQ);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * qtiles)), dim3(C::NTH), C::LDS, s, a,
+                       static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                       static_cast<const T*>(out), lse, static_cast<const T*>(dout), static_cast<T*>(dq), delta,
+                       qtiles);
+    PT_LAUNCH_CHECK();
+    return PTCG_OK;
+}
+
+template <typename T, int DH, int NK, int QS, int QT>
+int launch_dkv(const XArgs& a, const void* q, const void* k, const void* v, const float* lse, const void* dout,
+               const float* delta, void* dk, void* dv, hipStream_t s) {
+    typedef DkvCfg<T, DH, NK, QS, QT> C;
+    auto kern = xattn_dkv_kernel<T, DH, NK, QS, QT>;
+    PT_TRY(lds_attr(kern, C::LDS));
+    const int ktiles = pt_cdiv(a.lk, C::BKEY);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * ktiles)), dim3(C::NTH), C::LDS, s, a,
+                       static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), lse,
+                       static_cast<const T*>(dout), delta, static_cast<T*>(dk), static_cast<T*>(dv), ktiles);
+    PT_LAUNCH_CHECK();
+    return PTCG_OK;
+}
+
+template <typename T, int DH>
+int bwd(const XArgs& a, const void* q, const void* k, const void* v, const void* out, const float* lse,
+        const void* dout, void* dq, void* dk, void* dv, float* delta, hipStream_t s) {
+    if (a.lq > 0) {
+        const int nw = waves_for((long)a.lq * a.G);
+        PT_TRY(nw == 1   ? (launch_dq<T, DH, 1, 4, 32>(a, q, k, v, out, lse, dout, dq, delta, s))
+               : nw == 2 ? (launch_dq<T, DH, 2, 2, 32>(a, q, k, v, out, lse, dout, dq, delta, s))
+                         : (launch_dq<T, DH, 4, 1, 64>(a, q, k, v, out, lse, dout, dq, delta, s)));
+    }
+    if (a.lk > 0) {
+        const int nk = waves_for(a.lk);
+        return nk == 1   ? launch_dkv<T, DH, 1, 4, 32>(a, q, k, v, lse, dout, delta, dk, dv, s)
+               : nk == 2 ? launch_dkv<T, DH, 2, 2, 32>(a, q, k, v, lse, dout, delta, dk, dv, s)
+                         : launch_dkv<T, DH, 4, 1, 64>(a, q, k, v, lse, dout, delta, dk, dv, s);
+    }
+    return PTCG_OK;
+}
+
+int64_t ws_need(const PtcgCrossAttn* d, int backward) {
+    const int64_t R = (int64_t)d->n * d->heads * d->lq;
+    if (backward) return R * 4;
+    if (R == 0) return 0;
+    const Plan p = fwd_plan(d);
+    return p.nsplit > 1 ? (int64_t)p.nsplit * R * (d->dh + 2) * 4 : 0;
+}
+
+}  // namespace
+
+extern "C" int64_t ptcg_kernel_cross_attention_ws_bytes(const PtcgCrossAttn* d, int backward) {
+    if (check_desc(d, "cross_attention_ws_bytes") != PTCG_OK) return -1;
+    return ws_need(d, backward);
+}
+
+extern "C" int ptcg_kernel_cross_attention_fwd(const PtcgCrossAttn* d, const void* q, const void* k, const void* v,
+                                               void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                               void* stream) {
+    PT_TRY(check_desc(d, "cross_attention_fwd"));
+    if ((int64_t)d->n * d->lq == 0) return PTCG_OK;
+    PT_REQUIRE(q && out && (d->lk == 0 || (k && v)), "cross_attention_fwd: null buffer");
+    PT_REQUIRE(al16(q) && al16(k) && al16(v) && al16(out), "cross_attention_fwd: buffers must be 16 B aligned");
+    PT_REQUIRE(layout_apart(d->o, d->q_off ? 1 : d->n, d->lq, d->heads, d->dh),
+               "cross_attention_fwd: rows of the output overlap");
+    const int64_t need = ws_need(d, 0);
+    PT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && al16(workspace)),
+               "cross_attention_fwd: workspace of %lld bytes, need %lld (16 B aligned)", (long long)workspace_bytes,
+               (long long)need);
+    const XArgs a = to_args(d);
+    const Plan p = fwd_plan(d);
+    float* part = static_cast<float*>(workspace);
+    const hipStream_t s = (hipStream_t)stream;
+    if (d->bf16)
+        return d->dh <= 32   ? fwd_nw<__bf16, 32>(a, p, q, k, v, out, lse, part, s)
+               : d->dh <= 64 ? fwd_nw<__bf16, 64>(a, p, q, k, v, out, lse, part, s)
+                             : fwd_nw<__bf16, 128>(a, p, q, k, v, out, lse, part, s);
+    return d->dh <= 32   ? fwd_nw<float, 32>(a, p, q, k, v, out, lse, part, s)
+           : d->dh <= 64 ? fwd_nw<float, 64>(a, p, q, k, v, out, lse, part, s)
+                         : fwd_nw<float, 128>(a, p, q, k, v, out, lse, part, s);
+}
+
+extern "C" int ptcg_kernel_cross_attention_bwd(const PtcgCrossAttn* d, const void* q, const void* k, const void* v,
+                                               const void* out, const float* lse, const void* dout, void* dq,
+                                               void* dk, void* dv, void* workspace, int64_t workspace_bytes,
+                                               void* stream) {
+    PT_TRY(check_desc(d, "cross_attention_bwd"));
+    if (d->n == 0 || (d->lq == 0 && d->lk == 0)) return PTCG_OK;
+    PT_REQUIRE(d->lq == 0 || (q && out && lse && dout && dq), "cross_attention_bwd: null buffer");
+    PT_REQUIRE(d->lk == 0 || (k && v && dk && dv), "cross_attention_bwd: null buffer");
+    PT_REQUIRE(al16(q) && al16(k) && al16(v) && al16(out) && al16(dout) && al16(dq) && al16(dk) && al16(dv),
+               "cross_attention_bwd: buffers must be 16 B aligned");
+    PT_REQUIRE(layout_apart(d->q, d->q_off ? 1 : d->n, d->lq, d->heads, d->dh),
+               "cross_attention_bwd: rows of dq overlap (a broadcast q has no gradient layout)");
+    PT_REQUIRE(layout_apart(d->k, d->k_off ? 1 : d->n, d->lk, d->kv_heads, d->dh) &&
+                   layout_apart(d->v, d->k_off ? 1 : d->n, d->lk, d->kv_heads, d->dh),
+               "cross_attention_bwd: rows of dk or dv overlap (broadcast keys have no gradient layout)");
+    const int64_t need = ws_need(d, 1);
+    PT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && al16(workspace)),
+               "cross_attention_bwd: workspace of %lld bytes, need %lld (16 B aligned)", (long long)workspace_bytes,
+               (long long)need);
+    const XArgs a = to_args(d);
+    float* delta = static_cast<float*>(workspace);
+    const hipStream_t s = (hipStream_t)stream;
+    if (d->bf16)
+        return d->dh <= 32   ? bwd<__bf16, 32>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s)
+               : d->dh <= 64 ? bwd<__bf16, 64>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s)
+                             : bwd<__bf16, 128>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s);
+    return d->dh <= 32   ? bwd<float, 32>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s)
+           : d->dh <= 64 ? bwd<float, 64>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s)
+                         : bwd<float, 128>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s);
+}

@@ -35,6 +35,18 @@ class CPtcgLog(ctypes.Structure):
          ("vram_total_gb", ctypes.c_double), ("global_step", ctypes.c_int64), ("epoch", ctypes.c_int64)]
 
 
+class CPtcgHeadLayout(ctypes.Structure):
+    """struct PtcgHeadLayout: strides of sample, row and head, in elements."""
+    _fields_ = [(n, ctypes.c_int64) for n in ("sn", "sl", "sh")]
+
+
+class CPtcgCrossAttn(ctypes.Structure):
+    """struct PtcgCrossAttn of include/ptcg_amd_kernels.h."""
+    _fields_ = [(n, ctypes.c_int) for n in ("n", "lq", "lk", "heads", "kv_heads", "dh", "bf16")] + \
+        [("scale", ctypes.c_float)] + [(n, CPtcgHeadLayout) for n in ("q", "k", "v", "o")] + \
+        [(n, c_void_p) for n in ("q_off", "k_off", "k_len", "keep")] + [("keep_sn", ctypes.c_int64)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "ptcg_last_error": (ctypes.c_char_p, []),
@@ -269,6 +281,11 @@ _SIGS = {
                                                     c_void_p, c_void_p, ctypes.c_int, ctypes.c_int,
                                                     ctypes.c_int, ctypes.c_int, ctypes.c_int, c_void_p,
                                                     ctypes.c_int64, c_void_p]),
+    "ptcg_kernel_cross_attention_ws_bytes": (ctypes.c_int64, [ctypes.POINTER(CPtcgCrossAttn), ctypes.c_int]),
+    "ptcg_kernel_cross_attention_fwd": (ctypes.c_int, [ctypes.POINTER(CPtcgCrossAttn)] + [c_void_p] * 6
+                                        + [ctypes.c_int64, c_void_p]),
+    "ptcg_kernel_cross_attention_bwd": (ctypes.c_int, [ctypes.POINTER(CPtcgCrossAttn)] + [c_void_p] * 10
+                                        + [ctypes.c_int64, c_void_p]),
 }
 
 _lib = None

@@ -259,6 +259,53 @@ int ptcg_kernel_cross_attention_bwd(const PtcgCrossAttn* desc, const void* q, co
                                     const void* out, const float* lse, const void* dout, void* dq, void* dk,
                                     void* dv, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* Embedding lookup with scaling: out[t] = scale table[ids[t]], rows t of d
+ * values at row strides ldt, ldo (elements); table and out fp32, or bf16 where
+ * their flag is 1 (products and sums fp32).  An id outside [0, vocab) is
+ * padding: a row of zeros, and no gradient.
+ * bwd: dtable (vocab, d) fp32, overwritten, [v] = scale sum of dout[t] over the
+ * tokens of id v in token order (the tokens are sorted: no atomics, the same
+ * sums in every run); dout bf16 where bf16 = 1; workspace of _bwd_ws_bytes
+ * (-1: refused), 16 B aligned.  rows < 2^30, d <= 65536.
+ * Replaces the lookups of the reference's k_tok_cat and their scatter with
+ * atomics (native/model/ptcg_model.cu:289, ptcg_model2.cu:36) for tables of
+ * any size.                                                                */
+int ptcg_kernel_embedding_fwd(const int32_t* ids, int64_t rows, const void* table, int64_t ldt, int table_bf16,
+                              int vocab, int d, float scale, void* out, int64_t ldo, int out_bf16, void* stream);
+int64_t ptcg_kernel_embedding_bwd_ws_bytes(int64_t rows, int vocab, int d);
+int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const void* dout, int64_t ldo, int bf16, int vocab,
+                              int d, float scale, float* dtable, int64_t ldt, void* workspace,
+                              int64_t workspace_bytes, void* stream);
+
+/* Activation checkpoints in 8 bits: rows of d values kept as e4m3 codes (row
+ * stride ldq >= d) with one scale byte per 32 consecutive values of a row (row
+ * stride lds >= ceil(d / 32)): x8 = code 2^(byte - 127), the scale the least
+ * power of two that keeps the group's largest value within 448 of it
+ * (bytes 17 .. 246), codes rounded to nearest even; values past 448 2^119
+ * saturate, NaN and infinities are kept as NaN.  Any d and strides; 8-value
+ * pieces move as vectors where d and the code stride are multiples of 8 and
+ * rows are 16 B (codes 8 B) aligned.
+ * pack: x (fp32, or bf16 where bf16 = 1) to codes and scales; unpack: x8 back.
+ * gelu_bwd: the backward of a GELU layer from its pre-activation z8: dz = dy
+ * gelu'(z8) and, where act is given, act = gelu(z8) (the next layer's input);
+ * dy, dz, act fp32 or bf16; dz may be dy.
+ * dw: a linear layer's dW (out, in) = dY^T x8 and db = column sums of dY
+ * (nullable), fp32, overwritten, summed in a fixed order; dY (rows, out) fp32
+ * (split into three bf16 terms: fp32 products; an infinity becomes NaN) or bf16; workspace of
+ * _dw_ws_bytes (0: none, -1: refused), 16 B aligned.
+ * No reference counterpart: it keeps activations in fp32 or bf16.            */
+int ptcg_kernel_ckpt8_pack(const void* x, int64_t ldx, int bf16, int rows, int d, uint8_t* q, int64_t ldq,
+                           uint8_t* scales, int64_t lds, void* stream);
+int ptcg_kernel_ckpt8_unpack(const uint8_t* q, int64_t ldq, const uint8_t* scales, int64_t lds, int rows, int d,
+                             void* x, int64_t ldx, int bf16, void* stream);
+int ptcg_kernel_ckpt8_gelu_bwd(const uint8_t* q, int64_t ldq, const uint8_t* scales, int64_t lds, int rows, int d,
+                               const void* dy, int64_t lddy, void* dz, int64_t lddz, void* act, int64_t lda,
+                               int bf16, void* stream);
+int64_t ptcg_kernel_ckpt8_dw_ws_bytes(int rows, int in, int out, int bf16);
+int ptcg_kernel_ckpt8_dw(int rows, int in, int out, const void* dY, int64_t lddy, int bf16, const uint8_t* q,
+                         int64_t ldq, const uint8_t* scales, int64_t lds, float* dW, float* db, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
 /* Launch timing: between begin and end, every GEMM, LayerNorm and Adam
  * launch (up to max_launches in all) is bracketed by a HIP event pair on its
  * own stream.  end waits for the events and returns the GEMM launches'

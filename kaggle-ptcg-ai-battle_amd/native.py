@@ -286,6 +286,26 @@ _SIGS = {
                                         + [ctypes.c_int64, c_void_p]),
     "ptcg_kernel_cross_attention_bwd": (ctypes.c_int, [ctypes.POINTER(CPtcgCrossAttn)] + [c_void_p] * 10
                                         + [ctypes.c_int64, c_void_p]),
+    "ptcg_kernel_embedding_fwd": (ctypes.c_int, [
+        c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float,
+        c_void_p, ctypes.c_int64, ctypes.c_int, c_void_p]),
+    "ptcg_kernel_embedding_bwd_ws_bytes": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
+    "ptcg_kernel_embedding_bwd": (ctypes.c_int, [
+        c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float,
+        c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int64, c_void_p]),
+    "ptcg_kernel_ckpt8_pack": (ctypes.c_int, [
+        c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, c_void_p, ctypes.c_int64, c_void_p,
+        ctypes.c_int64, c_void_p]),
+    "ptcg_kernel_ckpt8_unpack": (ctypes.c_int, [
+        c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, c_void_p, ctypes.c_int64,
+        ctypes.c_int, c_void_p]),
+    "ptcg_kernel_ckpt8_gelu_bwd": (ctypes.c_int, [
+        c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_int, c_void_p, ctypes.c_int64,
+        c_void_p, ctypes.c_int64, c_void_p, ctypes.c_int64, ctypes.c_int, c_void_p]),
+    "ptcg_kernel_ckpt8_dw_ws_bytes": (ctypes.c_int64, [ctypes.c_int] * 4),
+    "ptcg_kernel_ckpt8_dw": (ctypes.c_int, [
+        ctypes.c_int, ctypes.c_int, ctypes.c_int, c_void_p, ctypes.c_int64, ctypes.c_int, c_void_p, ctypes.c_int64,
+        c_void_p, ctypes.c_int64, c_void_p, c_void_p, c_void_p, ctypes.c_int64, c_void_p]),
 }
 
 _lib = None

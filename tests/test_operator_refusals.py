@@ -81,3 +81,73 @@ def test_cross_attention_of_nothing_is_done():
     _fwd(_desc(n=0), q=None, k=None, v=None, out=None)
     _fwd(_desc(lq=0), q=None, k=None, v=None, out=None)
     _bwd(_desc(n=0), *[None] * 9, ws=None, nb=0)
+
+
+def _emb_fwd(ids=P, rows=10, table=P, ldt=8, vocab=5, d=8, out=P, ldo=8):
+    return native.check(native.lib().ptcg_kernel_embedding_fwd(ids, rows, table, ldt, 0, vocab, d, 1.0, out, ldo, 0,
+                                                               None))
+
+
+def _emb_bwd(ids=P, rows=10, dout=P, ldo=8, vocab=5, d=8, dtable=P, ldt=8, ws=P, nb=1 << 20):
+    return native.check(native.lib().ptcg_kernel_embedding_bwd(ids, rows, dout, ldo, 0, vocab, d, 1.0, dtable, ldt, ws,
+                                                               nb, None))
+
+
+@pytest.mark.parametrize("call", [_emb_fwd, _emb_bwd])
+@pytest.mark.parametrize("kw,match", [
+    (dict(rows=-1), "rows"), (dict(rows=1 << 30), "rows"), (dict(vocab=0), "vocab"), (dict(d=0), "d=0"),
+    (dict(d=65537, ldt=65537, ldo=65537), "d=65537"), (dict(ldt=7), "row strides"), (dict(ldo=4), "row strides"),
+    (dict(ids=None), "null buffer"),
+])
+def test_embedding_refuses(call, kw, match):
+    with pytest.raises(native.PtcgError, match=match):
+        call(**kw)
+
+
+def test_embedding_refuses_buffers():
+    L = native.lib()
+    for kw in (dict(table=None), dict(out=None)):
+        with pytest.raises(native.PtcgError, match="null buffer"):
+            _emb_fwd(**kw)
+    for kw in (dict(dout=None), dict(dtable=None)):
+        with pytest.raises(native.PtcgError, match="null buffer"):
+            _emb_bwd(**kw)
+    need = L.ptcg_kernel_embedding_bwd_ws_bytes(10, 5, 8)
+    assert need > 0 and L.ptcg_kernel_embedding_bwd_ws_bytes(10, 0, 8) == -1
+    for kw in (dict(ws=None), dict(nb=need - 1), dict(ws=P + 4)):
+        with pytest.raises(native.PtcgError, match="workspace"):
+            _emb_bwd(**kw)
+    _emb_fwd(rows=0, ids=None, table=None, out=None)     # nothing to look up
+
+
+def test_ckpt8_refuses():
+    L, check = native.lib(), native.check
+    bad = lambda match: pytest.raises(native.PtcgError, match=match)
+    for rows, d, ldx, ldq, lds, match in ((-1, 8, 8, 8, 1, "rows"), (4, 0, 8, 8, 1, "d=0"), (4, 8, 7, 8, 1, "stride"),
+                                          (4, 8, 8, 7, 1, "strides"), (4, 40, 40, 40, 1, "strides"),
+                                          (2 ** 31 - 1, 2 ** 20, 2 ** 20, 2 ** 20, 2 ** 15, "too many")):
+        with bad(match):
+            check(L.ptcg_kernel_ckpt8_pack(P, ldx, 0, rows, d, P, ldq, P, lds, None))
+        with bad(match):
+            check(L.ptcg_kernel_ckpt8_unpack(P, ldq, P, lds, rows, d, P, ldx, 0, None))
+        with bad(match):
+            check(L.ptcg_kernel_ckpt8_gelu_bwd(P, ldq, P, lds, rows, d, P, ldx, P, ldx, None, 0, 0, None))
+    with bad("stride"):
+        check(L.ptcg_kernel_ckpt8_gelu_bwd(P, 8, P, 1, 4, 8, P, 8, P, 8, P, 4, 0, None))
+    for k in range(3):
+        a = [None if i == k else P for i in range(3)]
+        with bad("null buffer"):
+            check(L.ptcg_kernel_ckpt8_pack(a[0], 8, 0, 4, 8, a[1], 8, a[2], 1, None))
+        with bad("null buffer"):
+            check(L.ptcg_kernel_ckpt8_unpack(a[0], 8, a[1], 1, 4, 8, a[2], 8, 0, None))
+    dw = lambda rows=4000, k=32, n=16, dy=P, lddy=16, q=P, ldq=32, sc=P, lds=1, dW=P, ws=P, nb=1 << 30: check(
+        L.ptcg_kernel_ckpt8_dw(rows, k, n, dy, lddy, 0, q, ldq, sc, lds, dW, P, ws, nb, None))
+    need = L.ptcg_kernel_ckpt8_dw_ws_bytes(4000, 32, 16, 0)
+    assert need > 0 and L.ptcg_kernel_ckpt8_dw_ws_bytes(4000, 0, 16, 0) == -1
+    for kw, match in ((dict(rows=-1), "rows"), (dict(k=0), "in=0"), (dict(n=0), "out=0"), (dict(lddy=15), "stride"),
+                      (dict(ldq=31), "strides"), (dict(lds=0), "strides"), (dict(dy=None), "null"),
+                      (dict(q=None), "null"), (dict(sc=None), "null"), (dict(dW=None), "null"),
+                      (dict(ws=None), "workspace"), (dict(nb=need - 1), "workspace"), (dict(ws=P + 2), "workspace"),
+                      (dict(k=1 << 20, n=1 << 20, ldq=1 << 20, lds=1 << 15, lddy=1 << 20), "too large")):
+        with bad(match):
+            dw(**kw)

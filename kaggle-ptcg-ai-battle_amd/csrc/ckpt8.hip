@@ -9,7 +9,8 @@
 // value, or 2^-10 2^e for small ones) is the only one.  e >= -110 keeps every x8
 // a normal bf16; e <= 119 a finite fp32 (values past 448 2^119 saturate).  NaN
 // and infinities are kept as NaN and leave the group's scale to the others.
-#include "common.h"
+#include "rowbuf.h"
+#include <type_traits>
 #include "../../include/ptcg_amd_kernels.h"
 
 namespace {
@@ -181,17 +182,20 @@ __global__ __launch_bounds__(256) void gelu_bwd_kernel(const uint8_t* __restrict
 // into three bf16 terms (8 bits each, by truncation, together exact above
 // 2^-102): 3 products against an x8 that needs no splitting, where two fp32
 // operands take 6.
-// A workgroup of 4 waves owns a TM x TN tile of dW and a range of the rows
-// (splits leave partial tiles, added in split order by dw_reduce_kernel);
-// splits also make the partial column sums.
-constexpr int TM = 128, TN = 128, TK = 32, PADB = 16;
+// A workgroup owns a TM x TN tile of dW and a range of the rows (splits leave
+// partial tiles, added in split order by dw_reduce_kernel); its waves own
+// TM / 2 x 64 each.  Steps of TK rows go through registers, two steps ahead of
+// their use, into the half of a double buffer that the products left a barrier
+// ago.  Splits also make the partial column sums.
+constexpr int TK = 32, PADB = 16;
 
 struct DwArgs {
     const void* dy; long lddy;
     const uint8_t* q; long ldq;
     const uint8_t* sc; long lds;
     float* dw; float* db;
-    float* part;          // [splits][n][k], then [splits][n] column sums
+    float* part;          // [splits][pstride]: dW (n, k), then the n column sums
+    long pstride;
     int rows, k, n, splits, chunk, tn, tm;
 };
 
@@ -207,66 +211,114 @@ __device__ __forceinline__ bf16x8 frag_tr(const __bf16* s, int st, int lane) {
 
 __device__ __forceinline__ float trunc_bf16(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 
+// 8 values of dY as they were loaded, 8 codes; single values where rows are not
+// aligned
+template <typename T> struct Raw8;
+template <> struct Raw8<float> {
+    pt_uintx4 w[2];
+    template <bool VEC> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off) {
+        if constexpr (VEC) {
+            w[0] = ld_buf16(rs, off);
+            w[1] = ld_buf16(rs, off + 16);
+        } else
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = ld_buf4(rs, off + 4 * i);
+    }
+    __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i / 4][i % 4]); }
+};
+template <> struct Raw8<__bf16> {
+    pt_uintx4 w;
+    template <bool VEC> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off) {
+        if constexpr (VEC) w = ld_buf16(rs, off);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = ld_buf2(rs, off + 4 * i) | ld_buf2(rs, off + 4 * i + 2) << 16;
+    }
+    __device__ __forceinline__ float at(int i) const {
+        return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+};
+template <bool VEC> __device__ __forceinline__ pt_uintx2 codes8(__amdgpu_buffer_rsrc_t rs, int off) {
+    if constexpr (VEC) return ld_buf8(rs, off);
+    pt_uintx2 r = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i / 4] |= ld_buf1(rs, off + i) << (8 * (i % 4));
+    return r;
+}
+
+template <typename T, int TM, int TN> struct DwCfg {
+    static constexpr int NP = sizeof(T) == 4 ? 3 : 1;          // bf16 terms of dY
+    static constexpr int NTH = 2 * TN;                         // 2 x TN / 64 waves
+    static constexpr int SA = TM + PADB, SB = TN + PADB;
+    static constexpr int BUF = NP * TK * SA + TK * SB;         // one half of the double buffer
+    static constexpr int RA = NTH / (TM / 8), RB = NTH / (TN / 8);   // rows of a staging pass
+    static constexpr int PA = TK / RA, PB = TK / RB;
+    static constexpr size_t LDS = 2 * (size_t)BUF * 2;
+    static_assert(TK % RA == 0 && TK % RB == 0 && LDS >= (size_t)RA * TM * 4, "staging passes, column sums");
+};
+
 // VEC: rows of dy and q are 16 / 8 B aligned with n, k multiples of 8
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void dw_kernel(const DwArgs g) {
-    constexpr int NP = sizeof(T) == 4 ? 3 : 1;          // bf16 terms of dY
-    constexpr int SA = TM + PADB, SB = TN + PADB;
+template <typename T, bool VEC, int TM, int TN>
+__global__ __launch_bounds__(2 * TN) void dw_kernel(const DwArgs g) {
+    typedef DwCfg<T, TM, TN> C;
+    constexpr int NP = C::NP, SA = C::SA, SB = C::SB, MT = TM / 64;
     extern __shared__ __align__(16) char smem[];
-    __bf16* As = reinterpret_cast<__bf16*>(smem);       // [NP][TK][SA]
-    __bf16* Bs = As + NP * TK * SA;                     // [TK][SB]
+    __bf16* lds = reinterpret_cast<__bf16*>(smem);      // [2] of A [NP][TK][SA], B [TK][SB]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int b = blockIdx.x;
+    // consecutive tiles of one row range on one XCD: its L2 serves their shared operands
+    int b;
+    {
+        const int nblk = gridDim.x, x = blockIdx.x & 7, per = nblk >> 3, rem = nblk & 7;
+        b = x * per + min(x, rem) + (blockIdx.x >> 3);
+    }
     const int it = b % g.tn; b /= g.tn;
     const int ot = b % g.tm, sp = b / g.tm;
     const int o0 = ot * TM, i0 = it * TN;
     const int r0 = sp * g.chunk, r1 = min(g.rows, r0 + g.chunk);
-    const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-    const T* dy = static_cast<const T*>(g.dy);
-    const bool sums = it == 0;
+    const int wm = (wave & 1) * (TM / 2), wn = (wave >> 1) * 64;
+    const bool sums = it == 0 && g.db;
 
-    // staging: thread owns column piece pc (8 columns) of rows pr, pr + 16
-    const int pc = (tid & 15) * 8, pr = tid >> 4;
-    float a[2][8], csum[8];
-    uint2 xb[2];
-    int xe[2];
+    // staging: a thread owns 8 columns of rows ra + RA u of dY and rb + RB u of
+    // x8.  What it reads of a row past column n (k) reaches only outputs that
+    // are not stored; rows past the range come as zeros.
+    const int ca = tid % (TM / 8) * 8, ra = tid / (TM / 8);
+    const int cb = tid % (TN / 8) * 8, rb = tid / (TN / 8);
+    const RowBuf ya = {static_cast<const char*>(g.dy) + (long)o0 * sizeof(T), (int)g.lddy * (int)sizeof(T),
+                       (g.n - o0) * (int)sizeof(T)};
+    const RowBuf xq = {reinterpret_cast<const char*>(g.q) + i0, (int)g.ldq, g.k - i0};
+    const RowBuf xs = {reinterpret_cast<const char*>(g.sc) + i0 / GRP, (int)g.lds, (g.k - i0 + GRP - 1) / GRP};
+    int offa[C::PA], offq[C::PB], offs[C::PB];
+#pragma unroll
+    for (int u = 0; u < C::PA; ++u)
+        offa[u] = o0 + ca < g.n ? (ra + C::RA * u) * ya.ld + ca * (int)sizeof(T) : PT_NOWHERE;
+#pragma unroll
+    for (int u = 0; u < C::PB; ++u) {
+        offq[u] = i0 + cb < g.k ? (rb + C::RB * u) * xq.ld + cb : PT_NOWHERE;
+        offs[u] = i0 + cb < g.k ? (rb + C::RB * u) * xs.ld + cb / GRP : PT_NOWHERE;
+    }
+    struct Set { Raw8<T> a[C::PA]; pt_uintx2 xb[C::PB]; unsigned xe[C::PB]; } set[2];
+    float csum[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) csum[i] = 0.f;
-    auto fetch = [&](int r) {
+    auto fetch = [&](int r, Set& f) {
+        const auto ry = ya.rows(r, r1, TK), rq = xq.rows(r, r1, TK), rs = xs.rows(r, r1, TK);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = r + pr + 16 * u;
-            const bool ok = row < r1;
-            const int la = ok ? g.n - (o0 + pc) : 0, lb = ok ? g.k - (i0 + pc) : 0;
+        for (int u = 0; u < C::PA; ++u) f.a[u].template load<VEC>(ry, offa[u]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) a[u][i] = 0.f;
-            xb[u] = make_uint2(0u, 0u);
-            xe[u] = 127;
-            if (la > 0) ld8<VEC>(dy + (long)row * g.lddy + o0 + pc, la, a[u]);
-            if (lb > 0) {
-                xb[u] = ldq8<VEC>(g.q + (long)row * g.ldq + i0 + pc, lb);
-                xe[u] = g.sc[(long)row * g.lds + (i0 + pc) / GRP];
-            }
+        for (int u = 0; u < C::PB; ++u) {
+            f.xb[u] = codes8<VEC>(rq, offq[u]);
+            f.xe[u] = ld_buf1(rs, offs[u]);
         }
     };
-    floatx16 acc[2][2];
+    auto put = [&](auto sum, __bf16* As, const Set& f) {
+        __bf16* Bs = As + NP * TK * SA;
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[m][n][e] = 0.f;
-    if (r0 < r1) fetch(r0);
-    for (int r = r0; r < r1; r += TK) {
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int row = pr + 16 * u;
+        for (int u = 0; u < C::PA; ++u) {
             bf16x8 h[NP];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float v = a[u][i];
-                if (sums) csum[i] += v;
+                float v = f.a[u].at(i);
+                if constexpr (sum) csum[i] += v;
                 if constexpr (NP == 1) h[0][i] = (__bf16)v;
                 else {
                     const float t0 = trunc_bf16(v);
@@ -278,35 +330,92 @@ __global__ __launch_bounds__(256) void dw_kernel(const DwArgs g) {
                 }
             }
 #pragma unroll
-            for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(As + (p * TK + row) * SA + pc) = h[p];
-            const float w = scale_of(xe[u] - 127);
-            const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xb[u].x, w, false);
-            const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xb[u].x, w, true);
-            const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xb[u].y, w, false);
-            const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(xb[u].y, w, true);
-            *reinterpret_cast<bf16x8*>(Bs + row * SB + pc) = bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+            for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(As + (p * TK + ra + C::RA * u) * SA + ca) = h[p];
         }
-        __syncthreads();
-        if (r + TK < r1) fetch(r + TK);
 #pragma unroll
-        for (int kk = 0; kk < TK; kk += 16) {
-            bf16x8 bf[2];
+        for (int u = 0; u < C::PB; ++u) {
+            const float w = scale_of((int)f.xe[u] - 127);   // rows past the range: 0 times 0
+            const bf16x2 x0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f.xb[u][0], w, false);
+            const bf16x2 x1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f.xb[u][0], w, true);
+            const bf16x2 x2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f.xb[u][1], w, false);
+            const bf16x2 x3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(f.xb[u][1], w, true);
+            *reinterpret_cast<bf16x8*>(Bs + (rb + C::RB * u) * SB + cb) =
+                bf16x8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+        }
+    };
+    floatx16 acc[MT][2];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) bf[n] = frag_tr(Bs + kk * SB + wn + 32 * n, SB, lane);
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[m][n][e] = 0.f;
+    // One step: the products of buffer `cur`, with step `set` going into buffer
+    // `nxt` and step r on its way into `set` between them: products, LDS traffic,
+    // loads and the operands' conversion take turns in one wave's instruction
+    // stream (the groups below), where phase by phase the products would stand
+    // still in the others (all waves meet at the same barrier).
+    auto step = [&](auto sum, const __bf16* cur, __bf16* nxt, Set& f, int r) {
+        const __bf16* Bs = cur + NP * TK * SA;
+        bf16x8 af[TK / 16][NP][MT], bf[TK / 16][2];
+        auto read = [&](int k) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) bf[k][n] = frag_tr(Bs + 16 * k * SB + wn + 32 * n, SB, lane);
+#pragma unroll
+            for (int p = NP - 1; p >= 0; --p)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) af[k][p][m] = frag_tr(cur + (p * TK + 16 * k) * SA + wm + 32 * m, SA, lane);
+        };
+        read(0);
+        put(sum, nxt, f);
+        fetch(r, f);
+        read(1);
+#pragma unroll
+        for (int k = 0; k < TK / 16; ++k)
 #pragma unroll
             for (int p = NP - 1; p >= 0; --p)     // small terms first
 #pragma unroll
-                for (int m = 0; m < 2; ++m) {
-                    const bf16x8 af = frag_tr(As + (p * TK + kk) * SA + wm + 32 * m, SA, lane);
+                for (int m = 0; m < MT; ++m)
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
-                        acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af, bf[n], acc[m][n], 0, 0, 0);
-                }
-        }
-    }
-    float* out = g.splits > 1 ? g.part + (long)sp * g.n * g.k : g.dw;
+                        acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(af[k][p][m], bf[k][n], acc[m][n], 0, 0, 0);
+        constexpr int FR = 2 * (2 + NP * MT), MF = NP * MT * 2;   // LDS reads and products of 16 rows
+        __builtin_amdgcn_sched_group_barrier(0x100, FR, 0);
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+        for (int i = 0; i < MF; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, (FR + MF - 1) / MF, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+        }
+        __syncthreads();
+    };
+    // step t sits in buffer t % 2 while steps t + 1 and t + 2 are on their way
+    auto walk = [&](auto sum) {
+        fetch(r0, set[0]);
+        put(sum, lds, set[0]);
+        fetch(r0 + TK, set[1]);
+        fetch(r0 + 2 * TK, set[0]);
+        __syncthreads();
+        for (int r = r0; r < r1; r += 2 * TK) {
+            step(sum, lds, lds + C::BUF, set[1], r + 3 * TK);
+            step(sum, lds + C::BUF, lds, set[0], r + 4 * TK);   // past the range: zeros
+        }
+    };
+    if (r0 < r1) {
+        if (sums) walk(std::true_type());
+        else walk(std::false_type());
+    }
+    float* out = g.splits > 1 ? g.part + sp * g.pstride : g.dw;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const int col = i0 + wn + 32 * n + (lane & 31);
@@ -317,33 +426,57 @@ __global__ __launch_bounds__(256) void dw_kernel(const DwArgs g) {
                 if (row < g.n) out[(long)row * g.k + col] = acc[m][n][e];
             }
         }
-    if (!sums || !g.db) return;
-    // column sums: the 16 threads of a column piece add in row order
-    __syncthreads();
-    float* cs = reinterpret_cast<float*>(smem);     // [16][TM]
+    if (!sums) return;
+    // column sums: the RA threads of a column piece add in row order
+    float* cs = reinterpret_cast<float*>(smem);     // [RA][TM]; the loop ended in a barrier
 #pragma unroll
-    for (int i = 0; i < 8; ++i) cs[pr * TM + pc + i] = csum[i];
+    for (int i = 0; i < 8; ++i) cs[ra * TM + ca + i] = csum[i];
     __syncthreads();
-    if (tid < TM && o0 + tid < g.n) {
+    for (int c = tid; c < TM && o0 + c < g.n; c += C::NTH) {
         float s = 0.f;
-        for (int i = 0; i < 16; ++i) s += cs[i * TM + tid];
-        if (g.splits > 1) g.part[(long)g.splits * g.n * g.k + (long)sp * g.n + o0 + tid] = s;
-        else g.db[o0 + tid] = s;
+        for (int i = 0; i < C::RA; ++i) s += cs[i * TM + c];
+        if (g.splits > 1) g.part[sp * g.pstride + (long)g.n * g.k + o0 + c] = s;
+        else g.db[o0 + c] = s;
     }
 }
 
-__global__ __launch_bounds__(256) void dw_reduce_kernel(const DwArgs g) {
-    const long nk = (long)g.n * g.k, i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i < nk) {
-        float s = 0.f;
+// Adds the splits' partials (dW, then db): a thread takes 4 consecutive values
+// of every SG-th split, SG groups of a workgroup meet in LDS, in order.  Few
+// outputs with many splits need the groups (one thread walking 200 splits of a
+// 128 x 128 dW waits 200 loads in line: 60 us against 12 with 16 groups).
+template <int SG> __global__ __launch_bounds__(256) void dw_reduce_kernel(const DwArgs g) {
+    __shared__ float4 sh[256];
+    constexpr int CW = 256 / SG;
+    const int c = threadIdx.x % CW, grp = threadIdx.x / CW;
+    const long i = ((long)blockIdx.x * CW + c) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < g.pstride) {
 #pragma unroll 8
-        for (int p = 0; p < g.splits; ++p) s += g.part[p * nk + i];
-        g.dw[i] = s;
-    } else if (g.db && i < nk + g.n) {
-        const float* c = g.part + g.splits * nk + (i - nk);
-        float s = 0.f;
-        for (int p = 0; p < g.splits; ++p) s += c[(long)p * g.n];
-        g.db[i - nk] = s;
+        for (int p = grp; p < g.splits; p += SG) {
+            const float4 x = *reinterpret_cast<const float4*>(g.part + p * g.pstride + i);
+            s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+        }
+    }
+    if constexpr (SG > 1) {
+        sh[threadIdx.x] = s;
+        __syncthreads();
+        if (grp > 0) return;
+#pragma unroll
+        for (int k = 1; k < SG; ++k) {
+            const float4 x = sh[k * CW + c];
+            s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+        }
+    }
+    const long nk = (long)g.n * g.k;
+    if (i + 4 <= nk && ((uintptr_t)g.dw & 15) == 0) {
+        *reinterpret_cast<float4*>(g.dw + i) = s;
+        return;
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (i + e < nk) g.dw[i + e] = v[e];
+        else if (g.db && i + e < nk + g.n) g.db[i + e - nk] = v[e];
     }
 }
 
@@ -356,19 +489,31 @@ int cu_count() {
     return cu;
 }
 
-// splits of the rows: two workgroups per CU, at least 8 steps each
-struct DwPlan { int tm, tn, splits, chunk; };
-DwPlan dw_plan(int rows, int k, int n) {
+// Tiles and splits of the rows.  One workgroup per CU (a second one shares its
+// matrix cores and doubles the partials: 37 391 x 256 x 1 024 fp32 77 us with
+// one, 95 with two).  128 x 256 tiles read the narrower operand half as often as
+// 128 x 128 ones (62 us against 72, 20 000 x 1 024 x 1 024 bf16); a dW of few
+// tiles takes 128 x 128, whose partials are half as many bytes (60 000 x 256 x
+// 256 bf16: 40 us against 50).  256 x 256 in bf16 (16 products of 12 LDS reads a
+// step) gains 14% of the products and costs another 33 MB of partials: from
+// rows * in * out = 4e10 on (65 539 x 4 096 x 1 024: 537 us against 625;
+// 20 000 x 1 024 x 1 024: 70 against 63).  In fp32 its accumulators leave too
+// few registers for the three terms.  At least 8 steps a split.
+struct DwPlan { int big_m, big_n, tm, tn, splits, chunk; long pstride; };
+DwPlan dw_plan(int rows, int k, int n, int bf16) {
     DwPlan p;
-    p.tm = pt_cdiv(n, TM);
-    p.tn = pt_cdiv(k, TN);
+    p.big_n = k > 128 && (long)n * k > 256 * 256;
+    p.big_m = bf16 && p.big_n && n > 128 && (double)rows * n * k > 4e10;
+    p.tm = pt_cdiv(n, p.big_m ? 256 : 128);
+    p.tn = pt_cdiv(k, p.big_n ? 256 : 128);
     const long tiles = (long)p.tm * p.tn;
-    long sp = (2 * cu_count()) / tiles;
+    long sp = cu_count() / tiles;
     const long most = rows / (8 * TK);
     if (sp > most) sp = most;
     if (sp < 1) sp = 1;
     p.chunk = rows > 0 ? pt_cdiv(pt_cdiv(rows, sp), TK) * TK : TK;
     p.splits = rows > 0 ? pt_cdiv(rows, p.chunk) : 1;
+    p.pstride = ((long)n * k + n + 3) / 4 * 4;
     return p;
 }
 
@@ -422,16 +567,32 @@ int gelu(const uint8_t* q, long ldq, const uint8_t* sc, long lds, int rows, int 
     PT_LAUNCH_CHECK();
     return PTCG_OK;
 }
-template <typename T> int dw(const DwArgs& g, const DwPlan& p, hipStream_t s) {
-    constexpr int NP = sizeof(T) == 4 ? 3 : 1;
-    constexpr size_t lds = (size_t)(NP * TK * (TM + PADB) + TK * (TN + PADB)) * 2;
-    static_assert(lds >= 16 * TM * 4 && lds <= 64 * 1024, "the column sums reuse the tiles");
-    const bool vec = vecq(g.q, g.ldq, g.k) && vec8<T>(g.dy, g.lddy) && g.n % 8 == 0;
-    auto kern = vec ? dw_kernel<T, true> : dw_kernel<T, false>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((long)p.tm * p.tn * p.splits)), dim3(256), lds, s, g);
+template <typename T, bool VEC, int TM, int TN> int launch_dw(const DwArgs& g, hipStream_t s) {
+    typedef DwCfg<T, TM, TN> C;
+    auto kern = dw_kernel<T, VEC, TM, TN>;
+    if (C::LDS > 64 * 1024)
+        PT_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)C::LDS));
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)g.tm * g.tn * g.splits)), dim3(C::NTH), C::LDS, s, g);
     PT_LAUNCH_CHECK();
+    return PTCG_OK;
+}
+template <typename T, bool VEC> int dw_tiles(const DwArgs& g, const DwPlan& p, hipStream_t s) {
+    if constexpr (sizeof(T) == 2)
+        if (p.big_m) return launch_dw<T, VEC, 256, 256>(g, s);
+    return p.big_n ? launch_dw<T, VEC, 128, 256>(g, s) : launch_dw<T, VEC, 128, 128>(g, s);
+}
+template <typename T> int dw(const DwArgs& g, const DwPlan& p, hipStream_t s) {
+    const bool vec = vecq(g.q, g.ldq, g.k) && vec8<T>(g.dy, g.lddy) && g.n % 8 == 0;
+    PT_TRY(vec ? (dw_tiles<T, true>(g, p, s)) : (dw_tiles<T, false>(g, p, s)));
     if (p.splits > 1) {
-        hipLaunchKernelGGL(dw_reduce_kernel, dim3(pt_cdiv((long)g.n * g.k + g.n, 256)), dim3(256), 0, s, g);
+        // enough workgroups for two per CU or so
+        const long quads = g.pstride / 4;
+        if (quads >= 512 * 256 || g.splits < 8)
+            hipLaunchKernelGGL(dw_reduce_kernel<1>, dim3(pt_cdiv(quads, 256)), dim3(256), 0, s, g);
+        else if (quads >= 128 * 256 || g.splits < 32)
+            hipLaunchKernelGGL(dw_reduce_kernel<4>, dim3(pt_cdiv(quads, 64)), dim3(256), 0, s, g);
+        else
+            hipLaunchKernelGGL(dw_reduce_kernel<16>, dim3(pt_cdiv(quads, 16)), dim3(256), 0, s, g);
         PT_LAUNCH_CHECK();
     }
     return PTCG_OK;
@@ -439,13 +600,13 @@ template <typename T> int dw(const DwArgs& g, const DwPlan& p, hipStream_t s) {
 
 int check_dw(const char* who, int rows, int in, int out) {
     PT_REQUIRE(rows >= 0 && rows < (1 << 30) && in >= 1 && out >= 1, "%s: rows=%d in=%d out=%d", who, rows, in, out);
-    PT_REQUIRE((long)in * out < (1LL << 36) && (long)pt_cdiv(in, TN) * pt_cdiv(out, TM) < (1LL << 22),
+    PT_REQUIRE((long)in * out < (1LL << 36) && (long)pt_cdiv(in, 128) * pt_cdiv(out, 128) < (1LL << 22),
                "%s: in=%d out=%d are too large", who, in, out);
     return PTCG_OK;
 }
-int64_t dw_need(int rows, int in, int out) {
-    const DwPlan p = dw_plan(rows, in, out);
-    return p.splits > 1 ? (int64_t)p.splits * ((int64_t)in * out + out) * 4 : 0;
+int64_t dw_need(int rows, int in, int out, int bf16) {
+    const DwPlan p = dw_plan(rows, in, out, bf16);
+    return p.splits > 1 ? (int64_t)p.splits * p.pstride * 4 : 0;
 }
 
 }  // namespace
@@ -483,7 +644,7 @@ extern "C" int ptcg_kernel_ckpt8_gelu_bwd(const uint8_t* q, int64_t ldq, const u
 
 extern "C" int64_t ptcg_kernel_ckpt8_dw_ws_bytes(int rows, int in, int out, int bf16) {
     if (check_dw("ckpt8_dw_ws_bytes", rows, in, out) != PTCG_OK) return -1;
-    return dw_need(rows, in, out);
+    return dw_need(rows, in, out, bf16);
 }
 
 extern "C" int ptcg_kernel_ckpt8_dw(int rows, int in, int out, const void* dY, int64_t lddy, int bf16,
@@ -492,15 +653,17 @@ extern "C" int ptcg_kernel_ckpt8_dw(int rows, int in, int out, const void* dY, i
     PT_TRY(check_dw("ckpt8_dw", rows, in, out));
     PT_TRY(check_rows("ckpt8_dw", rows, in, ldq, lds));
     PT_REQUIRE(lddy >= out, "ckpt8_dw: row stride %lld below out=%d", (long long)lddy, out);
+    PT_REQUIRE(lddy < (1 << 23) && ldq < (1 << 23) && lds < (1 << 23), "ckpt8_dw: a row stride is 2^23 or more");
     PT_REQUIRE(dW && (rows == 0 || (dY && q && scales)), "ckpt8_dw: null buffer");
-    const int64_t need = dw_need(rows, in, out);
+    const int64_t need = dw_need(rows, in, out, bf16);
     PT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && al(workspace, 16)),
                "ckpt8_dw: workspace of %lld bytes, need %lld (16 B aligned)", (long long)workspace_bytes,
                (long long)need);
-    const DwPlan p = dw_plan(rows, in, out);
+    const DwPlan p = dw_plan(rows, in, out, bf16);
     DwArgs g{};
     g.dy = dY; g.lddy = lddy; g.q = q; g.ldq = ldq; g.sc = scales; g.lds = lds;
     g.dw = dW; g.db = db; g.part = static_cast<float*>(workspace);
     g.rows = rows; g.k = in; g.n = out; g.splits = p.splits; g.chunk = p.chunk; g.tm = p.tm; g.tn = p.tn;
+    g.pstride = p.pstride;
     return bf16 ? dw<__bf16>(g, p, (hipStream_t)stream) : dw<float>(g, p, (hipStream_t)stream);
 }

@@ -189,7 +189,7 @@ def _ws(rows, k, n, bf16):
 @pytest.mark.parametrize("rows,k,n,pad", [
     (1, 1, 1, 0), (5, 33, 7, 0), (32, 128, 128, 0), (33, 130, 129, 3), (1000, 256, 64, 0), (700, 634, 136, 0),
     (2047, 200, 300, 8), (9000, 128, 128, 0), (513, 1024, 256, 0), (40, 256, 1024, 0), (4000, 40, 24, 16),
-    (100003, 64, 32, 0),
+    (100003, 64, 32, 0), (300, 520, 264, 0), (36001, 1100, 1040, 0), (36001, 1088, 1032, 5),
 ])
 def test_weight_gradient(rows, k, n, pad, bf16, cuda):
     """Each product is exact (bf16 terms) and sums of m of them are fp32: off by

@@ -25,7 +25,7 @@
 // LDS row strides: 32 bytes of padding in bf16 keep both the row reads (8 lanes
 // of 16 bytes) and the transposed reads (4 rows of 32 bytes) free of bank
 // conflicts; 16 bytes in fp32.
-#include "common.h"
+#include "rowbuf.h"
 #include "../../include/ptcg_amd_kernels.h"
 
 #include <type_traits>
@@ -178,65 +178,103 @@ __device__ __forceinline__ floatx16 mma_rows(const T* xs, const typename Frag<T>
 }
 
 // A tile of BR rows on its way through registers into LDS: 16-byte chunks,
-// thread t takes chunks t, t + NTH, ...  Loads are issued a tile ahead of the
+// thread t takes chunks t, t + NTH, ...  Loads are issued well before the
 // barrier that publishes them.
 template <typename T, int DH, int BR, int NTH> struct Stage {
-    static constexpr int E = Frag<T>::EL, CPR = DH / E, NCH = BR * CPR / NTH, ST = DH + Frag<T>::PAD;
-    static_assert(BR * CPR % NTH == 0, "whole chunks per thread");
-    typename Frag<T>::V r[NCH];
-    // rows row0 + [0, BR) of a matrix at base (row stride sl), rows < len
-    __device__ __forceinline__ void load(const T* base, long sl, int row0, int len, int dh, int tid) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = tid + i * NTH, row = row0 + c / CPR, col = (c % CPR) * E;
-            r[i] = row < len && col < dh ? ldv<T>(base + row * sl + col) : zerov<T>();
-        }
+    static constexpr int E = Frag<T>::EL, CPR = DH / E, NCH = BR * CPR / NTH, RPP = NTH / CPR;
+    static constexpr int ST = DH + Frag<T>::PAD;
+    static_assert(BR * CPR % NTH == 0 && NTH % CPR == 0, "whole chunks per thread");
+    pt_uintx4 r[NCH];
+    // byte offset of the thread's first chunk; chunk i is i * RPP rows on
+    static __device__ __forceinline__ int first(int ld, int dh, int tid) {
+        return tid % CPR * E < dh ? tid / CPR * ld + tid % CPR * 16 : PT_NOWHERE;
     }
-    // rows of the flattened query matrix of kv head kvh
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off, int ld) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) r[i] = ld_buf16(rs, off + i * (RPP * ld));
+    }
+    // rows of the flattened query matrix of kv head kvh, from row0; the last
+    // row stands in for rows past it (zeroed on the way into LDS)
     __device__ __forceinline__ void load_q(const XArgs& a, const PtcgHeadLayout& l, const T* base, int kvh, int row0,
                                            int len, int tid) {
+        const int col = min(tid % CPR * E, a.dh - E);
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = tid + i * NTH, row = row0 + c / CPR, col = (c % CPR) * E;
-            r[i] = row < len && col < a.dh ? ldv<T>(base + row_off(a, l, kvh, row) + col) : zerov<T>();
-        }
+        for (int i = 0; i < NCH; ++i)
+            r[i] = *reinterpret_cast<const pt_uintx4*>(
+                base + row_off(a, l, kvh, min(row0 + tid / CPR + i * RPP, len - 1)) + col);
     }
-    // whether each chunk's row is kept (masked rows enter LDS as zeros, so
-    // that what they hold, NaN too, reaches no product)
-    __device__ __forceinline__ void keeps(bool (&kp)[NCH], const float* keep, int row0, int len, int tid) const {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int row = row0 + (tid + i * NTH) / CPR;
-            kp[i] = !keep || (row < len && keep[row] != 0.f);
-        }
-    }
-    __device__ __forceinline__ void store(T* s, int tid, const bool (&kp)[NCH]) const {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = tid + i * NTH;
-            *reinterpret_cast<typename Frag<T>::V*>(s + (c / CPR) * ST + (c % CPR) * E) = kp[i] ? r[i] : zerov<T>();
-        }
+    __device__ __forceinline__ void put(T* s, int tid, int i, bool ok) const {
+        *reinterpret_cast<pt_uintx4*>(s + (tid / CPR + i * RPP) * ST + tid % CPR * E) = ok ? r[i] : pt_uintx4{0, 0, 0, 0};
     }
     __device__ __forceinline__ void store(T* s, int tid) const {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const int c = tid + i * NTH;
-            *reinterpret_cast<typename Frag<T>::V*>(s + (c / CPR) * ST + (c % CPR) * E) = r[i];
-        }
+        for (int i = 0; i < NCH; ++i) put(s, tid, i, true);
+    }
+    // rows below `rows`, columns below dh
+    __device__ __forceinline__ void store_q(T* s, int tid, int rows, int dh) const {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) put(s, tid, i, tid / CPR + i * RPP < rows && tid % CPR * E < dh);
     }
 };
 
-// the last kept key of [k0, kend), plus one (k0 if none): keys behind a
-// sample's valid prefix are not read.  Every thread of the workgroup calls it.
-__device__ __forceinline__ int last_kept(const float* keep, int k0, int kend, int nth, int* sh) {
-    if (threadIdx.x == 0) *sh = k0;
-    __syncthreads();
+// A tile of keys and values on its way: masked rows enter LDS as zeros, so that
+// what they hold, NaN too, reaches no product; kf holds 0 or -inf per key.
+template <typename T, int DH, int BK, int NTH> struct KvTile {
+    typedef Stage<T, DH, BK, NTH> St;
+    static_assert(BK <= NTH, "a thread per key flag");
+    St k, v;
+    float kp[St::NCH], kfr;
+    RowBuf kb, vb, keep;
+    int ko, vo, kend;
+    bool masks;
+    __device__ __forceinline__ void init(const XArgs& a, const Sample& s, const T* kp_, const T* vp, int kvh,
+                                         int kend_, int tid) {
+        constexpr int es = sizeof(T);
+        kb = {reinterpret_cast<const char*>(kp_ + s.k + (long)kvh * a.k.sh), (int)a.k.sl * es, a.dh * es};
+        vb = {reinterpret_cast<const char*>(vp + s.v + (long)kvh * a.v.sh), (int)a.v.sl * es, a.dh * es};
+        keep = {reinterpret_cast<const char*>(a.keep + s.keep), 4, 4};
+        masks = a.keep != nullptr;
+        ko = St::first(kb.ld, a.dh, tid);
+        vo = St::first(vb.ld, a.dh, tid);
+        kend = kend_;
+    }
+    __device__ __forceinline__ void fetch(int row0, int tid) {
+        const auto rk = kb.rows(row0, kend, BK), rv = vb.rows(row0, kend, BK);
+        k.load(rk, ko, kb.ld);
+        v.load(rv, vo, vb.ld);
+        kfr = row0 + tid < kend ? 1.f : 0.f;
+        if (masks) {
+            const auto rm = keep.rows(row0, kend, BK);
+#pragma unroll
+            for (int i = 0; i < St::NCH; ++i) kp[i] = __uint_as_float(ld_buf4(rm, 4 * (tid / St::CPR + i * St::RPP)));
+            kfr = __uint_as_float(ld_buf4(rm, 4 * tid));
+        }
+    }
+    __device__ __forceinline__ void store(T* Ks, T* Vs, float* kf, int tid) const {
+        if (masks) {
+#pragma unroll
+            for (int i = 0; i < St::NCH; ++i) {
+                k.put(Ks, tid, i, kp[i] != 0.f);
+                v.put(Vs, tid, i, kp[i] != 0.f);
+            }
+        } else {
+            k.store(Ks, tid);
+            v.store(Vs, tid);
+        }
+        if (tid < BK) kf[tid] = kfr != 0.f ? 0.f : -INFINITY;
+    }
+};
+
+// the last kept key of [k0, kend), plus one (k0 if none): tiles behind a
+// sample's valid prefix are not read.  A wave's part; the workgroup's is the
+// largest of its waves'.
+__device__ __forceinline__ int last_kept(const float* keep, int k0, int kend, int nth) {
     int last = k0;
-    for (int j = k0 + threadIdx.x; j < kend; j += nth)
-        if (keep[j] != 0.f) last = j + 1;
-    if (last > k0) atomicMax(sh, last);
-    __syncthreads();
-    return *sh;
+    for (int j = k0 + (int)threadIdx.x; j - (int)(threadIdx.x & 63) < kend; j += nth) {
+        const unsigned long long m = __ballot(j < kend && keep[min(j, kend - 1)] != 0.f);
+        if (m) last = j - (int)(threadIdx.x & 63) + 64 - __builtin_clzll(m);
+    }
+    return last;
 }
 
 // a lane's 4 consecutive output values
@@ -259,6 +297,40 @@ __device__ __forceinline__ void store_row(T* row, const floatx16 (&o)[DH / 32], 
         }
 }
 
+// A wave's 32 rows of a transposed accumulator to memory, times each row's f, by
+// way of LDS (ws: 32 rows of DH + PAD): whole rows of 16 bytes a lane instead of
+// 8 bytes here and there.  Rows r0 .. of kv head kvh, those below `rows`.
+template <typename T, int DH>
+__device__ __forceinline__ void write_q_rows(const XArgs& a, const PtcgHeadLayout& l, T* out, int kvh, int r0,
+                                             int rows, const floatx16 (&o)[DH / 32], float f, T* ws, int lane) {
+    constexpr int E = Frag<T>::EL, CPR = DH / E, ST = DH + Frag<T>::PAD;
+    store_row<T, DH>(ws + (lane & 31) * ST, o, f, DH, lane >> 5);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < 32 * CPR / 64; ++i) {
+        const int c = i * 64 + lane, row = c / CPR, col = c % CPR * E;
+        if (r0 + row < rows && col < a.dh)
+            *reinterpret_cast<pt_uintx4*>(out + row_off(a, l, kvh, r0 + row) + col) =
+                *reinterpret_cast<const pt_uintx4*>(ws + row * ST + col);
+    }
+}
+// the same for key rows key0 .. of a matrix at base, row stride sl
+template <typename T, int DH>
+__device__ __forceinline__ void write_k_rows(T* base, long sl, int key0, int keys, int dh,
+                                             const floatx16 (&o)[DH / 32], float f, T* ws, int lane) {
+    constexpr int E = Frag<T>::EL, CPR = DH / E, ST = DH + Frag<T>::PAD;
+    store_row<T, DH>(ws + (lane & 31) * ST, o, f, DH, lane >> 5);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int i = 0; i < 32 * CPR / 64; ++i) {
+        const int c = i * 64 + lane, row = c / CPR, col = c % CPR * E;
+        if (key0 + row < keys && col < dh)
+            *reinterpret_cast<pt_uintx4*>(base + (long)(key0 + row) * sl + col) =
+                *reinterpret_cast<const pt_uintx4*>(ws + row * ST + col);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+
 template <typename T, int DH, int BR> constexpr int tile_elems() { return BR * (DH + Frag<T>::PAD); }
 
 // ---------------------------------------------------------------- forward
@@ -268,22 +340,30 @@ template <typename T, int DH, int BR> constexpr int tile_elems() { return BR * (
 // partial with its maximum and sum for xattn_join_kernel.
 template <typename T, int DH, int NW, int KS, int KT> struct FwdCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
-    static constexpr size_t TILES = 2 * (size_t)tile_elems<T, DH, BK>() * sizeof(T);
+    static constexpr int TILE = tile_elems<T, DH, BK>();
+    // two buffers (one barrier a tile) where they leave room for another
+    // workgroup, or at all; else one
+    static constexpr size_t PAIR = 2 * (size_t)TILE * sizeof(T);
+    static constexpr int NB = 2 * PAIR <= 144 * 1024 ? 2 : 1;
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * (DH * 32 + 64) * sizeof(float);
-    static constexpr size_t LDS = (TILES > JOIN ? TILES : JOIN) + BK * sizeof(float) + 16;
+    static constexpr size_t BUFS = NB * PAIR > JOIN ? NB * PAIR : JOIN;
+    static constexpr size_t LDS = BUFS + NB * BK * sizeof(float) + 64;
 };
+// Waves a SIMD holds, for the register allocator: two (of 256 registers each)
+// let one wave's softmax run beside the other's products.
+template <typename T, int DH> constexpr int min_waves() { return sizeof(T) == 2 || DH <= 64 ? 2 : 1; }
 
 template <typename T, int DH, int NW, int KS, int KT>
-__global__ __launch_bounds__(64 * NW * KS) void xattn_fwd_kernel(const XArgs a, const T* __restrict__ q,
-        const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
-        float* __restrict__ part, int qtiles, int nsplit, int split_keys) {
+__global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_kernel(const XArgs a,
+        const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,
+        float* __restrict__ lse, float* __restrict__ part, int qtiles, int nsplit, int split_keys) {
     typedef FwdCfg<T, DH, NW, KS, KT> C;
-    typedef Stage<T, DH, C::BK, C::NTH> St;
+    typedef KvTile<T, DH, C::BK, C::NTH> Kv;
+    constexpr int ST = Kv::St::ST;
     extern __shared__ __align__(16) char smem[];
-    T* Ks = reinterpret_cast<T*>(smem);
-    T* Vs = Ks + tile_elems<T, DH, C::BK>();
-    float* kf = reinterpret_cast<float*>(smem + C::LDS - 16 - C::BK * sizeof(float));
-    int* sh = reinterpret_cast<int*>(smem + C::LDS - 16);
+    T* tiles = reinterpret_cast<T*>(smem);
+    float* kfs = reinterpret_cast<float*>(smem + C::BUFS);
+    int* sh = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int qw = wave % NW, kw = wave / NW;
     int b = xcd_block(gridDim.x);
@@ -296,13 +376,11 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_fwd_kernel(const XArgs a, 
     const int r = qt * C::BQ + 32 * qw + (lane & 31);
     const bool rok = r < rows;
 
-    const T* kb = k + s.k + (long)kvh * a.k.sh;
-    const T* vb = v + s.v + (long)kvh * a.v.sh;
-    const float* keep = a.keep ? a.keep + s.keep : nullptr;
     const int k0 = sp * split_keys;
     int kend = min(s.kl, k0 + split_keys);
-    if (keep && k0 < kend) kend = last_kept(keep, k0, kend, C::NTH, sh);
-    const int nt = kend > k0 ? (kend - k0 + C::BK - 1) / C::BK : 0;
+    Kv kv;
+    kv.init(a, s, k, v, kvh, kend, tid);
+    if (k0 < kend) kv.fetch(k0, tid);       // on its way while the masks are looked through
 
     typename Frag<T>::V qf[DH / (2 * Frag<T>::EL)];
     load_row<T, DH>(qf, q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
@@ -314,45 +392,40 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_fwd_kernel(const XArgs a, 
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
 
-    St ks, vs;
-    bool kp[St::NCH];
-    float kfr = 0.f;
-    auto fetch = [&](int t) {
-        const int row0 = k0 + t * C::BK;
-        ks.load(kb, a.k.sl, row0, kend, a.dh, tid);
-        vs.load(vb, a.v.sl, row0, kend, a.dh, tid);
-        ks.keeps(kp, keep, row0, kend, tid);
-        if (tid < C::BK) {
-            const int j = row0 + tid;
-            kfr = j < kend && (!keep || keep[j] != 0.f) ? 0.f : -INFINITY;
-        }
-    };
-    if (nt > 0) fetch(0);
-    for (int t = 0; t < nt; ++t) {
+    if (a.keep && k0 < kend) {
+        const int last = last_kept(a.keep + s.keep, k0, kend, C::NTH);
+        if (lane == 0) sh[wave] = last;
         __syncthreads();
-        ks.store(Ks, tid, kp);
-        vs.store(Vs, tid, kp);
-        if (tid < C::BK) kf[tid] = kfr;
-        __syncthreads();
-        if (t + 1 < nt) fetch(t + 1);
+        kend = k0;
+#pragma unroll
+        for (int w = 0; w < NW * KS; ++w) kend = max(kend, sh[w]);
+        kend = __builtin_amdgcn_readfirstlane(kend);
+        kv.kend = kend;
+    }
+    const int nt = kend > k0 ? (kend - k0 + C::BK - 1) / C::BK : 0;
+
+    auto tile = [&](int t, const T* Ks, const float* kf) {
+        const T* Vs = Ks + C::TILE;
         const int row0 = k0 + t * C::BK + kw * KT;
-        if (row0 >= kend) continue;
-        const bool masked = keep || row0 + KT > kend;
+        if (row0 >= kend) return;
+        const bool masked = a.keep || row0 + KT > kend;
         floatx16 sc[KT / 32];
         float mt = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < KT / 32; ++j) {
-            sc[j] = mma_rows<T, DH, St::ST>(Ks + (kw * KT + 32 * j) * St::ST, qf, lane);
-            if (masked) {
+        for (int j = 0; j < KT / 32; ++j) sc[j] = mma_rows<T, DH, ST>(Ks + (kw * KT + 32 * j) * ST, qf, lane);
+        if (masked) {
+#pragma unroll
+            for (int j = 0; j < KT / 32; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float4 f = *reinterpret_cast<const float4*>(kf + kw * KT + 32 * j + 8 * e + 4 * h);
                     sc[j][4 * e] += f.x; sc[j][4 * e + 1] += f.y; sc[j][4 * e + 2] += f.z; sc[j][4 * e + 3] += f.w;
                 }
-            }
+        }
+#pragma unroll
+        for (int j = 0; j < KT / 32; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mt = fmaxf(mt, sc[j][e]);
-        }
         mt = fmaxf(mt, half_swap(mt));
         const float mn = fmaxf(m2, mt * a.scale2);
         if (__any(mn > m2)) {
@@ -372,14 +445,33 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_fwd_kernel(const XArgs a, 
                 sc[j][e] = __builtin_amdgcn_exp2f(fmaf(sc[j][e], a.scale2, -ms));
                 l += sc[j][e];
             }
-            mma_tr<DH, St::ST>(Vs + (kw * KT + 32 * j) * St::ST, sc[j], o, lane);
+            mma_tr<DH, ST>(Vs + (kw * KT + 32 * j) * ST, sc[j], o, lane);
+        }
+    };
+    if (nt > 0) {
+        kv.store(tiles, tiles + C::TILE, kfs, tid);
+        if (nt > 1) kv.fetch(k0 + C::BK, tid);
+        __syncthreads();
+    }
+    for (int t = 0; t < nt; ++t) {
+        const int cur = C::NB == 2 ? t & 1 : 0;
+        if (C::NB == 2 && t + 1 < nt) {
+            T* nx = tiles + (cur ^ 1) * 2 * C::TILE;
+            kv.store(nx, nx + C::TILE, kfs + (cur ^ 1) * C::BK, tid);
+            if (t + 2 < nt) kv.fetch(k0 + (t + 2) * C::BK, tid);
+        }
+        tile(t, tiles + cur * 2 * C::TILE, kfs + cur * C::BK);
+        __syncthreads();
+        if (C::NB == 1 && t + 1 < nt) {
+            kv.store(tiles, tiles + C::TILE, kfs, tid);
+            if (t + 2 < nt) kv.fetch(k0 + (t + 2) * C::BK, tid);
+            __syncthreads();
         }
     }
     l += half_swap(l);
 
     // the key waves' results join in LDS, in wave order
     if constexpr (KS > 1) {
-        __syncthreads();
         float* jb = reinterpret_cast<float*>(smem);
         constexpr int JS = DH * 32 + 64;
         if (kw > 0) {
@@ -394,8 +486,7 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_fwd_kernel(const XArgs a, 
             }
         }
         __syncthreads();
-        if (kw > 0) return;
-        for (int w = 1; w < KS; ++w) {
+        for (int w = 1; w < KS && kw == 0; ++w) {
             const float* p = jb + (size_t)((w - 1) * NW + qw) * JS;
             const float mw = p[DH * 32 + (lane & 31)], lw = p[DH * 32 + 32 + (lane & 31)];
             const float mn = fmaxf(m2, mw), ms = mn == -INFINITY ? 0.f : mn;
@@ -408,10 +499,14 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_fwd_kernel(const XArgs a, 
                 for (int e = 0; e < 16; ++e) o[dt][e] = o[dt][e] * f0 + p[(dt * 16 + e) * 64 + lane] * f1;
         }
     }
-    if (!rok) return;
-    const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
+    if constexpr (KS > 1) {
+        __syncthreads();     // the joined buffers become the rows' way out
+        if (kw > 0) return;
+    }
+    const int qi = head_div(a, rok ? r : 0), head = kvh * a.G + (rok ? r : 0) - qi * a.G;
     const long row = ((long)i * a.H + head) * a.lq + qi;
     if (nsplit > 1) {
+        if (!rok) return;
         const long R = (long)a.n * a.H * a.lq;
         float* p = part + ((long)sp * R + row) * a.dh;
         store_row<float, DH>(p, o, 1.f, a.dh, h);
@@ -431,8 +526,9 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_fwd_kernel(const XArgs a, 
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
     }
-    store_row<T, DH>(out + s.o + row_off(a, a.o, kvh, r), o, none ? 0.f : 1.f / l, a.dh, h);
-    if (lse && h == 0) lse[row] = none ? -INFINITY : m2 * LN2 + logf(l);
+    if (lse && rok && h == 0) lse[row] = none ? -INFINITY : m2 * LN2 + logf(l);
+    write_q_rows<T, DH>(a, a.o, out + s.o, kvh, qt * C::BQ + 32 * qw, rows, o, none ? 0.f : 1.f / l,
+                        tiles + qw * 32 * ST, lane);
 }
 
 // joins the key splits of one row per wave, in split order
@@ -478,24 +574,26 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const XArgs a, const fl
 // for the dK / dV kernel, in row order of lse.
 template <typename T, int DH, int NW, int KS, int KT> struct DqCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
-    static constexpr size_t TILES = 2 * (size_t)tile_elems<T, DH, BK>() * sizeof(T);
+    static constexpr int TILE = tile_elems<T, DH, BK>();
+    static constexpr size_t PAIR = 2 * (size_t)TILE * sizeof(T);
+    static constexpr int NB = 2 * PAIR <= 144 * 1024 ? 2 : 1;
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * DH * 32 * sizeof(float);
-    static constexpr size_t LDS = (TILES > JOIN ? TILES : JOIN) + BK * sizeof(float) + 16;
+    static constexpr size_t BUFS = NB * PAIR > JOIN ? NB * PAIR : JOIN;
+    static constexpr size_t LDS = BUFS + NB * BK * sizeof(float) + 64;
 };
 
 template <typename T, int DH, int NW, int KS, int KT>
-__global__ __launch_bounds__(64 * NW * KS) void xattn_dq_kernel(const XArgs a, const T* __restrict__ q,
-        const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ out,
+__global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_kernel(const XArgs a,
+        const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ out,
         const float* __restrict__ lse, const T* __restrict__ dout, T* __restrict__ dq,
         float* __restrict__ delta, int qtiles) {
     typedef DqCfg<T, DH, NW, KS, KT> C;
-    typedef Stage<T, DH, C::BK, C::NTH> St;
-    constexpr int EL = Frag<T>::EL, NF = DH / (2 * EL);
+    typedef KvTile<T, DH, C::BK, C::NTH> Kv;
+    constexpr int EL = Frag<T>::EL, NF = DH / (2 * EL), ST = Kv::St::ST;
     extern __shared__ __align__(16) char smem[];
-    T* Ks = reinterpret_cast<T*>(smem);
-    T* Vs = Ks + tile_elems<T, DH, C::BK>();
-    float* kf = reinterpret_cast<float*>(smem + C::LDS - 16 - C::BK * sizeof(float));
-    int* sh = reinterpret_cast<int*>(smem + C::LDS - 16);
+    T* tiles = reinterpret_cast<T*>(smem);
+    float* kfs = reinterpret_cast<float*>(smem + C::BUFS);
+    int* sh = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int qw = wave % NW, kw = wave / NW;
     int b = xcd_block(gridDim.x);
@@ -507,11 +605,16 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_dq_kernel(const XArgs a, c
     const int r = qt * C::BQ + 32 * qw + (lane & 31);
     const bool rok = r < rows;
 
+    int kend = s.kl;
+    Kv kv;
+    kv.init(a, s, k, v, kvh, kend, tid);
+    if (kend > 0) kv.fetch(0, tid);
+
     typename Frag<T>::V qf[NF], df[NF];
     load_row<T, DH>(qf, q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
     const long oo = s.o + (rok ? row_off(a, a.o, kvh, r) : 0);
     load_row<T, DH>(df, dout + oo, rok, a.dh, h);
-    const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
+    const int qi = head_div(a, rok ? r : 0), head = kvh * a.G + (rok ? r : 0) - qi * a.G;
     const long lrow = ((long)i * a.H + head) * a.lq + qi;
     const float lr = rok ? lse[lrow] : -INFINITY;
     const bool none = lr == -INFINITY;
@@ -528,11 +631,16 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_dq_kernel(const XArgs a, c
     D += half_swap(D);
     if (rok && kw == 0 && h == 0) delta[lrow] = D;
 
-    const T* kb = k + s.k + (long)kvh * a.k.sh;
-    const T* vb = v + s.v + (long)kvh * a.v.sh;
-    const float* keep = a.keep ? a.keep + s.keep : nullptr;
-    int kend = s.kl;
-    if (keep && kend > 0) kend = last_kept(keep, 0, kend, C::NTH, sh);
+    if (a.keep && kend > 0) {
+        const int last = last_kept(a.keep + s.keep, 0, kend, C::NTH);
+        if (lane == 0) sh[wave] = last;
+        __syncthreads();
+        kend = 0;
+#pragma unroll
+        for (int w = 0; w < NW * KS; ++w) kend = max(kend, sh[w]);
+        kend = __builtin_amdgcn_readfirstlane(kend);
+        kv.kend = kend;
+    }
     const int nt = (kend + C::BK - 1) / C::BK;
 
     floatx16 g[DH / 32];
@@ -540,34 +648,15 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_dq_kernel(const XArgs a, c
     for (int dt = 0; dt < DH / 32; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) g[dt][e] = 0.f;
-    St ks, vs;
-    bool kp[St::NCH];
-    float kfr = 0.f;
-    auto fetch = [&](int t) {
-        const int row0 = t * C::BK;
-        ks.load(kb, a.k.sl, row0, kend, a.dh, tid);
-        vs.load(vb, a.v.sl, row0, kend, a.dh, tid);
-        ks.keeps(kp, keep, row0, kend, tid);
-        if (tid < C::BK) {
-            const int j = row0 + tid;
-            kfr = j < kend && (!keep || keep[j] != 0.f) ? 0.f : -INFINITY;
-        }
-    };
-    if (nt > 0) fetch(0);
-    for (int t = 0; t < nt; ++t) {
-        __syncthreads();
-        ks.store(Ks, tid, kp);
-        vs.store(Vs, tid, kp);
-        if (tid < C::BK) kf[tid] = kfr;
-        __syncthreads();
-        if (t + 1 < nt) fetch(t + 1);
+    auto tile = [&](int t, const T* Ks, const float* kf) {
+        const T* Vs = Ks + C::TILE;
 #pragma unroll 1
         for (int j = 0; j < KT / 32; ++j) {
             const int kr = kw * KT + 32 * j, row0 = t * C::BK + kr;
             if (row0 >= kend) break;
-            const bool masked = keep || row0 + 32 > kend;
-            floatx16 sc = mma_rows<T, DH, St::ST>(Ks + kr * St::ST, qf, lane);
-            const floatx16 dp = mma_rows<T, DH, St::ST>(Vs + kr * St::ST, df, lane);
+            const bool masked = a.keep || row0 + 32 > kend;
+            floatx16 sc = mma_rows<T, DH, ST>(Ks + kr * ST, qf, lane);
+            const floatx16 dp = mma_rows<T, DH, ST>(Vs + kr * ST, df, lane);
             if (masked) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -578,11 +667,30 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_dq_kernel(const XArgs a, c
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -l2)) * (dp[e] - D);
-            mma_tr<DH, St::ST>(Ks + kr * St::ST, sc, g, lane);
+            mma_tr<DH, ST>(Ks + kr * ST, sc, g, lane);
+        }
+    };
+    if (nt > 0) {
+        kv.store(tiles, tiles + C::TILE, kfs, tid);
+        if (nt > 1) kv.fetch(C::BK, tid);
+        __syncthreads();
+    }
+    for (int t = 0; t < nt; ++t) {
+        const int cur = C::NB == 2 ? t & 1 : 0;
+        if (C::NB == 2 && t + 1 < nt) {
+            T* nx = tiles + (cur ^ 1) * 2 * C::TILE;
+            kv.store(nx, nx + C::TILE, kfs + (cur ^ 1) * C::BK, tid);
+            if (t + 2 < nt) kv.fetch((t + 2) * C::BK, tid);
+        }
+        tile(t, tiles + cur * 2 * C::TILE, kfs + cur * C::BK);
+        __syncthreads();
+        if (C::NB == 1 && t + 1 < nt) {
+            kv.store(tiles, tiles + C::TILE, kfs, tid);
+            if (t + 2 < nt) kv.fetch((t + 2) * C::BK, tid);
+            __syncthreads();
         }
     }
     if constexpr (KS > 1) {
-        __syncthreads();
         float* jb = reinterpret_cast<float*>(smem);
         if (kw > 0) {
             float* p = jb + (size_t)((kw - 1) * NW + qw) * DH * 32;
@@ -592,23 +700,23 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_dq_kernel(const XArgs a, c
                 for (int e = 0; e < 16; ++e) p[(dt * 16 + e) * 64 + lane] = g[dt][e];
         }
         __syncthreads();
-        if (kw > 0) return;
-        for (int w = 1; w < KS; ++w) {
+        for (int w = 1; w < KS && kw == 0; ++w) {
             const float* p = jb + (size_t)((w - 1) * NW + qw) * DH * 32;
 #pragma unroll
             for (int dt = 0; dt < DH / 32; ++dt)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) g[dt][e] += p[(dt * 16 + e) * 64 + lane];
         }
+        __syncthreads();
+        if (kw > 0) return;
     }
-    if (!rok) return;
     if (none) {
 #pragma unroll
         for (int dt = 0; dt < DH / 32; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) g[dt][e] = 0.f;
     }
-    store_row<T, DH>(dq + s.q + row_off(a, a.q, kvh, r), g, a.scale, a.dh, h);
+    write_q_rows<T, DH>(a, a.q, dq + s.q, kvh, qt * C::BQ + 32 * qw, rows, g, a.scale, tiles + qw * 32 * ST, lane);
 }
 
 // dK and dV: a workgroup owns 32 NK keys of one kv head, a wave 32 of them, and
@@ -617,24 +725,25 @@ __global__ __launch_bounds__(64 * NW * KS) void xattn_dq_kernel(const XArgs a, c
 // dV^T += dO^T P and dK^T += Q^T dS read dO and Q transposed from LDS.
 template <typename T, int DH, int NK, int QS, int QT> struct DkvCfg {
     static constexpr int NTH = 64 * NK * QS, BKEY = 32 * NK, BQ = QT * QS;
-    static constexpr size_t TILES = 2 * (size_t)tile_elems<T, DH, BQ>() * sizeof(T);
+    static constexpr int TILE = tile_elems<T, DH, BQ>();
+    static constexpr size_t PAIR = 2 * (size_t)TILE * sizeof(T);
+    static constexpr int NB = 2 * PAIR <= 144 * 1024 ? 2 : 1;
     static constexpr size_t JOIN = (size_t)NK * (QS - 1) * 2 * DH * 32 * sizeof(float);
-    static constexpr size_t LDS = (TILES > JOIN ? TILES : JOIN) + 2 * BQ * sizeof(float) + 16;
+    static constexpr size_t BUFS = NB * PAIR > JOIN ? NB * PAIR : JOIN;
+    static constexpr size_t LDS = BUFS + NB * 2 * BQ * sizeof(float) + 16;
 };
 
 template <typename T, int DH, int NK, int QS, int QT>
-__global__ __launch_bounds__(64 * NK * QS) void xattn_dkv_kernel(const XArgs a, const T* __restrict__ q,
-        const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ lse,
+__global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_kernel(const XArgs a,
+        const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ lse,
         const T* __restrict__ dout, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
         int ktiles) {
     typedef DkvCfg<T, DH, NK, QS, QT> C;
     typedef Stage<T, DH, C::BQ, C::NTH> St;
     constexpr int NF = DH / (2 * Frag<T>::EL);
     extern __shared__ __align__(16) char smem[];
-    T* Qs = reinterpret_cast<T*>(smem);
-    T* Ds = Qs + tile_elems<T, DH, C::BQ>();
-    float* ls = reinterpret_cast<float*>(smem + C::LDS - 16 - 2 * C::BQ * sizeof(float));
-    float* dl = ls + C::BQ;
+    T* tiles = reinterpret_cast<T*>(smem);
+    float* lss = reinterpret_cast<float*>(smem + C::BUFS);   // log-sum-exp and D of each buffer's rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int kwv = wave % NK, qs = wave / NK;
     int b = xcd_block(gridDim.x);
@@ -662,34 +771,33 @@ __global__ __launch_bounds__(64 * NK * QS) void xattn_dkv_kernel(const XArgs a, 
     const int nt = (rows + C::BQ - 1) / C::BQ;
     St qs_, ds_;
     float lr = 0.f, dr = 0.f;
+    int rown = 0;     // rows of the fetched tile
     auto fetch = [&](int t) {
         const int row0 = t * C::BQ;
+        rown = rows - row0;
         qs_.load_q(a, a.q, q + s.q, kvh, row0, rows, tid);
         ds_.load_q(a, a.o, dout + s.o, kvh, row0, rows, tid);
         if (tid < C::BQ) {
-            const int r = row0 + tid;
-            lr = INFINITY;   // exp2(s - inf) = 0: rows past the end add nothing
-            dr = 0.f;
-            if (r < rows) {
-                const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
-                const long lrow = ((long)i * a.H + head) * a.lq + qi;
-                lr = lse[lrow];
-                lr = lr == -INFINITY ? INFINITY : lr * LOG2E;
-                dr = delta[lrow];
-            }
+            const int r = min(row0 + tid, rows - 1);
+            const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
+            const long lrow = ((long)i * a.H + head) * a.lq + qi;
+            lr = lse[lrow];
+            dr = delta[lrow];
         }
     };
-    if (nt > 0) fetch(0);
-    for (int t = 0; t < nt; ++t) {
-        __syncthreads();
-        qs_.store(Qs, tid);
-        ds_.store(Ds, tid);
+    auto store = [&](T* Qs, float* ls) {
+        qs_.store_q(Qs, tid, rown, a.dh);
+        ds_.store_q(Qs + C::TILE, tid, rown, a.dh);
         if (tid < C::BQ) {
-            ls[tid] = lr;
-            dl[tid] = dr;
+            // exp2(s - inf) = 0: rows past the end, and rows that keep no key, add nothing
+            const bool live = tid < rown;
+            ls[tid] = live && lr != -INFINITY ? lr * LOG2E : INFINITY;
+            ls[C::BQ + tid] = live ? dr : 0.f;
         }
-        __syncthreads();
-        if (t + 1 < nt) fetch(t + 1);
+    };
+    auto tile = [&](int t, const T* Qs, const float* ls) {
+        const T* Ds = Qs + C::TILE;
+        const float* dl = ls + C::BQ;
 #pragma unroll 1
         for (int j = 0; j < QT / 32; ++j) {
             const int qr = qs * QT + 32 * j;
@@ -711,10 +819,30 @@ __global__ __launch_bounds__(64 * NK * QS) void xattn_dkv_kernel(const XArgs a, 
             mma_tr<DH, St::ST>(Ds + qr * St::ST, p, gv, lane);
             mma_tr<DH, St::ST>(Qs + qr * St::ST, d, gk, lane);
         }
+    };
+    if (nt > 0) {
+        fetch(0);
+        store(tiles, lss);
+        if (nt > 1) fetch(1);
+        __syncthreads();
+    }
+    for (int t = 0; t < nt; ++t) {
+        const int cur = C::NB == 2 ? t & 1 : 0;
+        if (C::NB == 2 && t + 1 < nt) {
+            store(tiles + (cur ^ 1) * 2 * C::TILE, lss + (cur ^ 1) * 2 * C::BQ);
+            if (t + 2 < nt) fetch(t + 2);
+        }
+        tile(t, tiles + cur * 2 * C::TILE, lss + cur * 2 * C::BQ);
+        __syncthreads();
+        if (C::NB == 1 && t + 1 < nt) {
+            store(tiles, lss);
+            if (t + 2 < nt) fetch(t + 2);
+            __syncthreads();
+        }
     }
     if constexpr (QS > 1) {
-        __syncthreads();
         float* jb = reinterpret_cast<float*>(smem);
+        __syncthreads();
         if (qs > 0) {
             float* p = jb + (size_t)((qs - 1) * NK + kwv) * 2 * DH * 32;
 #pragma unroll
@@ -726,8 +854,7 @@ __global__ __launch_bounds__(64 * NK * QS) void xattn_dkv_kernel(const XArgs a, 
                 }
         }
         __syncthreads();
-        if (qs > 0) return;
-        for (int w = 1; w < QS; ++w) {
+        for (int w = 1; w < QS && qs == 0; ++w) {
             const float* p = jb + (size_t)((w - 1) * NK + kwv) * 2 * DH * 32;
 #pragma unroll
             for (int dt = 0; dt < DH / 32; ++dt)
@@ -737,16 +864,19 @@ __global__ __launch_bounds__(64 * NK * QS) void xattn_dkv_kernel(const XArgs a, 
                     gv[dt][e] += p[DH * 32 + (dt * 16 + e) * 64 + lane];
                 }
         }
+        __syncthreads();
+        if (qs > 0) return;
     }
-    if (!kin) return;
     if (!kok) {   // a masked key's gradient is zero, whatever the rows hold
 #pragma unroll
         for (int dt = 0; dt < DH / 32; ++dt)
 #pragma unroll
             for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
     }
-    store_row<T, DH>(dk + ko, gk, a.scale, a.dh, h);
-    store_row<T, DH>(dv + vo, gv, 1.f, a.dh, h);
+    const int key0 = kt * C::BKEY + 32 * kwv;
+    T* ws = tiles + kwv * 32 * St::ST;
+    write_k_rows<T, DH>(dk + s.k + (long)kvh * a.k.sh, a.k.sl, key0, kall, a.dh, gk, a.scale, ws, lane);
+    write_k_rows<T, DH>(dv + s.v + (long)kvh * a.v.sh, a.v.sl, key0, kall, a.dh, gv, 1.f, ws, lane);
 }
 
 // ------------------------------------------------------------------- host
@@ -823,6 +953,7 @@ int check_desc(const PtcgCrossAttn* d, const char* who) {
     const int e = d->bf16 ? 8 : 4;
     PT_REQUIRE(layout_ok(d->q, e) && layout_ok(d->k, e) && layout_ok(d->v, e) && layout_ok(d->o, e),
                "%s: strides must be non-negative multiples of 16 bytes", who);
+    PT_REQUIRE((d->k.sl | d->v.sl) < (1 << 22), "%s: key rows 2^22 elements apart or more", who);
     const int64_t G = d->heads / d->kv_heads, rows = (int64_t)d->lq * G;
     PT_REQUIRE(rows * G < (1LL << 32) && rows < (1LL << 31) - 256 && d->lk < (1 << 30),
                "%s: lq=%d lk=%d with %d heads a kv head is too long", who, d->lq, d->lk, (int)G);

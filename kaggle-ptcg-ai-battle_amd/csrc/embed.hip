@@ -29,7 +29,7 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int CHUNK = 64;        // tokens a group adds on its own
-constexpr int MAXB = 256;        // workgroups of a sort pass (tiles grow past it)
+constexpr int MAXB = 1024;        // workgroups of a sort pass (tiles grow past it)
 constexpr int BITS1 = 11, BITS2 = 9;
 
 // VW values of a row, as floats
@@ -78,6 +78,15 @@ template <int VW> __device__ __forceinline__ void st(__bf16* p, const Vals<VW>& 
     }
 }
 
+// the same as it lies in memory, so that a load in flight takes no more
+// registers than its bytes
+template <typename T, int VW> struct Raw {
+    T v[VW] __attribute__((aligned(sizeof(T) * VW < 16 ? sizeof(T) * VW : 16)));
+};
+template <typename T, int VW> __device__ __forceinline__ Raw<T, VW> ldraw(const T* p) {
+    return *reinterpret_cast<const Raw<T, VW>*>(p);
+}
+
 // ---------------------------------------------------------------- forward
 // A workgroup moves FWD_U * 256 consecutive VW-wide pieces of out, FWD_U of
 // them in flight per thread.
@@ -122,7 +131,7 @@ struct SortPass {
     const int* keys; const int* pos;
     const int* n_dev;
     int n, vocab, shift, bits, tile, nb;
-    int* cnt;     // [bins][nb]
+    int* cnt;     // [nb][bins]
     int* tot;     // [bins]
     int* out_keys; int* out_pos;
     int* starts;  // one-digit sorts: first sorted position of each id, [vocab + 1] (else null)
@@ -150,27 +159,36 @@ __global__ __launch_bounds__(256) void sort_count_kernel(const SortPass p) {
         if (d >= 0) atomicAdd(&hist[d], 1);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < bins; i += 256) p.cnt[(long)i * p.nb + blockIdx.x] = hist[i];
+    for (int i = threadIdx.x; i < bins; i += 256) p.cnt[(long)blockIdx.x * bins + i] = hist[i];
 }
 
-// one wave per digit: exclusive scan over the workgroups' counts
-__global__ __launch_bounds__(256) void sort_scan_kernel(const SortPass p) {
-    const int lane = threadIdx.x & 63, bin = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (bin >= 1 << p.bits) return;
-    int* c = p.cnt + (long)bin * p.nb;
+// exclusive scan over the workgroups' counts of each digit: a workgroup takes 64
+// digits, 16 waves a run of the counting workgroups each
+__global__ __launch_bounds__(1024) void sort_scan_kernel(const SortPass p) {
+    __shared__ int sums[16][64];
+    const int bins = 1 << p.bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6, d = blockIdx.x * 64 + lane;
+    const int per = (p.nb + 15) / 16, b0 = min(w * per, p.nb), b1 = min(b0 + per, p.nb);
+    int* c = p.cnt + d;
     int run = 0;
-    for (int b0 = 0; b0 < p.nb; b0 += 64) {
-        const int v = b0 + lane < p.nb ? c[b0 + lane] : 0;
-        int s = v;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(s, o, 64);
-            if (lane >= o) s += x;
-        }
-        if (b0 + lane < p.nb) c[b0 + lane] = run + s - v;
-        run += __shfl(s, 63, 64);
+    if (d < bins) {
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) run += c[(long)b * bins];
     }
-    if (lane == 0) p.tot[bin] = run;
+    sums[w][lane] = run;
+    __syncthreads();
+    int base = 0;
+    for (int k = 0; k < 16; ++k) {
+        if (k == w) run = base;
+        base += sums[k][lane];
+    }
+    if (d >= bins) return;
+#pragma unroll 8
+    for (int b = b0; b < b1; ++b) {
+        const int v = c[(long)b * bins];
+        c[(long)b * bins] = run;
+        run += v;
+    }
+    if (w == 0) p.tot[d] = base;
 }
 
 // Placement.  A wave owns a quarter of the workgroup's tile and walks it 64
@@ -181,37 +199,76 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
     extern __shared__ int sm[];
     const int bins = 1 << p.bits, n = pass_n(p);
     int* cnt = sm;               // [4][bins]
-    int* part = sm + 4 * bins;   // [256]
+    int* tot = sm + 4 * bins;    // [bins]
+    int* part = tot + bins;      // [4]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int i = tid; i < 4 * bins; i += 256) cnt[i] = 0;
-    __syncthreads();
-    const int per = p.tile / 4, w0 = blockIdx.x * p.tile + wave * per;
-    for (int o = lane; o < per; o += 64) {
-        int key;
-        const int d = digit_of(p, w0 + o, n, key);
-        if (d >= 0) atomicAdd(&cnt[wave * bins + d], 1);
+    // what the previous launches left, all of it on its way before anything waits
+    constexpr int PT = (1 << BITS1) / 256;
+    int tv[PT], mv[PT];
+    const int* mine = p.cnt + (long)blockIdx.x * bins;
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+        const int d = min(tid + 256 * i, bins - 1);
+        tv[i] = p.tot[d];
+        mv[i] = mine[d];
     }
-    // exclusive scan of the digits' totals: thread t owns bpt consecutive digits
+    for (int i = tid; i < 4 * bins; i += 256) cnt[i] = 0;
+    // four batches' keys at a time (a wave's quarter is a multiple of 256 tokens)
+    const int per = p.tile / 4, w0 = blockIdx.x * p.tile + wave * per;
+    int key[4], dig[4];
+    auto load = [&](int o) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) dig[u] = digit_of(p, w0 + o + 64 * u + lane, n, key[u]);
+    };
+    load(0);
+    __syncthreads();
+    for (int o = 0; o < per; o += 256) {
+        if (o > 0) load(o);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (dig[u] >= 0) atomicAdd(&cnt[wave * bins + dig[u]], 1);
+    }
+    // exclusive scan of the digits' totals: thread t adds up bpt consecutive digits
     const int bpt = (bins + 255) / 256, d0 = tid * bpt;
+#pragma unroll
+    for (int i = 0; i < PT; ++i)
+        if (tid + 256 * i < bins) tot[tid + 256 * i] = tv[i];
+    __syncthreads();
     int sum = 0;
     for (int i = 0; i < bpt; ++i)
-        if (d0 + i < bins) sum += p.tot[d0 + i];
-    part[tid] = sum;
-    __syncthreads();
-    for (int o = 1; o < 256; o <<= 1) {
-        const int x = tid >= o ? part[tid - o] : 0;
-        __syncthreads();
-        part[tid] += x;
-        __syncthreads();
+        if (d0 + i < bins) sum += tot[d0 + i];
+    int inc = sum;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += x;
     }
-    int base = part[tid] - sum;
-    if (tid == 255 && blockIdx.x == 0 && p.live) *p.live = part[255];
+    if (lane == 63) part[wave] = inc;
+    __syncthreads();
+    int base = inc - sum, all = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < wave) base += part[w];
+        all += part[w];
+    }
     for (int i = 0; i < bpt; ++i) {
-        const int d = d0 + i;
+        if (d0 + i >= bins) break;
+        const int v = tot[d0 + i];
+        tot[d0 + i] = base;
+        base += v;
+    }
+    if (blockIdx.x == 0 && tid == 0) {
+        if (p.live) *p.live = all;
+        if (p.starts) p.starts[p.vocab] = all;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+        const int d = tid + 256 * i;
         if (d >= bins) break;
-        if (p.starts && blockIdx.x == 0 && d < p.vocab) p.starts[d] = base;
-        int run = base + p.cnt[(long)d * p.nb + blockIdx.x];
-        base += p.tot[d];
+        const int at = tot[d];
+        if (p.starts && blockIdx.x == 0 && d < p.vocab) p.starts[d] = at;
+        int run = at + mv[i];
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const int c = cnt[w * bins + d];
@@ -219,26 +276,32 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
             run += c;
         }
     }
-    if (p.starts && blockIdx.x == 0 && tid == 255) p.starts[p.vocab] = part[255];
     __syncthreads();
-    volatile int* my = cnt + wave * bins;
-    for (int o = 0; o < per; o += 64) {
-        const int t = w0 + o + lane;
-        int key = 0;
-        const int d = digit_of(p, t, n, key);
-        unsigned long long same = __ballot(d >= 0);
-        for (int i = 0; i < p.bits; ++i) {
-            const unsigned long long b = __ballot((d >> i) & 1);
-            same &= ((d >> i) & 1) ? b : ~b;
-        }
-        if (d >= 0) {
+    for (int o = 0; o < per; o += 256) {
+        if (per > 256) load(o);
+        int at[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int d = dig[u];
+            unsigned long long same = __ballot(d >= 0);
+            for (int i = 0; i < p.bits; ++i) {
+                const unsigned long long b = __ballot((d >> i) & 1);
+                same &= ((d >> i) & 1) ? b : ~b;
+            }
             const int rank = __popcll(same & ((1ull << lane) - 1));
-            const int at = my[d] + rank;
-            __builtin_amdgcn_wave_barrier();
-            if (rank == 0) my[d] = at + __popcll(same);
-            p.out_keys[at] = key;
-            p.out_pos[at] = p.pos ? p.pos[t] : t;
+            int* c = sm + wave * bins + max(d, 0);
+            at[u] = *c + rank;      // every lane reads before the digit's first lane moves it on
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (d >= 0 && rank == 0) *c = at[u] + __popcll(same);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (dig[u] >= 0) {
+                const int t = w0 + o + 64 * u + lane;
+                p.out_keys[at[u]] = key[u];
+                p.out_pos[at[u]] = p.pos ? p.pos[t] : t;
+            }
     }
 }
 
@@ -266,76 +329,96 @@ struct GradArgs {
     float* part;    // [nchunks][2][d]: a chunk's piece of the run it continues, and of the one it starts
 };
 
-// sum of dout rows of sorted tokens [a, b) at columns col.., in order, 8 in flight
-template <typename TO, int VW>
-__device__ __forceinline__ Vals<VW> run_sum(const TO* __restrict__ dout, const GradArgs& g, int a, int b, int col) {
-    Vals<VW> s;
+// sums of dout rows of sorted tokens [a, b) at CB column pieces `step` apart, in
+// order; several rows in flight (past the end the last one again, not added),
+// as many as leave eight waves a SIMD
+template <typename TO, int VW, int CB>
+__device__ __forceinline__ void run_sum(const TO* __restrict__ dout, const GradArgs& g, int a, int b,
+                                        const int (&col)[CB], Vals<VW> (&s)[CB]) {
+    constexpr int U = VW * sizeof(TO) * CB <= 16 ? 8 : 4;
 #pragma unroll
-    for (int i = 0; i < VW; ++i) s.v[i] = 0.f;
-    int t = a;
-    for (; t + 8 <= b; t += 8) {
-        int at[8];
-        Vals<VW> x[8];
+    for (int c = 0; c < CB; ++c)
 #pragma unroll
-        for (int u = 0; u < 8; ++u) at[u] = g.pos[t + u];
+        for (int i = 0; i < VW; ++i) s[c].v[i] = 0.f;
+    for (int t = a; t < b; t += U) {
+        int at[U];
+        Raw<TO, VW> x[U][CB];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = ld<VW>(dout + at[u] * g.ldo + col);
+        for (int u = 0; u < U; ++u) at[u] = g.pos[min(t + u, b - 1)];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int i = 0; i < VW; ++i) s.v[i] += x[u].v[i];
+            for (int c = 0; c < CB; ++c) x[u][c] = ldraw<TO, VW>(dout + at[u] * g.ldo + col[c]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int c = 0; c < CB; ++c)
+#pragma unroll
+                for (int i = 0; i < VW; ++i) s[c].v[i] += t + u < b ? (float)x[u][c].v[i] : 0.f;
     }
-    if (t < b) {
-        int at[8];
-        Vals<VW> x[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) at[u] = g.pos[min(t + u, b - 1)];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) x[u] = ld<VW>(dout + at[u] * g.ldo + col);
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-#pragma unroll
-            for (int i = 0; i < VW; ++i) s.v[i] += t + u < b ? x[u].v[i] : 0.f;
-    }
-    return s;
 }
 
-// One group of lpr lanes per (table row, column block), then per (chunk, column
-// block); rows whose run is longer than CHUNK are left to the chunks.
-template <typename TO, int VW>
+// One group of lpr lanes per (table row, column block of CB * lpr * VW), then per
+// (chunk, column block); rows whose run is longer than CHUNK are left to the
+// chunks.  Wide rows take two pieces a lane (CB = 2): a row of few tokens is a
+// chain of dependent loads, and half as many groups walk it (300 007 tokens of
+// 1 024 bf16 values, 100 003 ids: 269 us with one piece).
+template <typename TO, int VW, int CB>
 __global__ __launch_bounds__(256) void embed_grad_kernel(const TO* __restrict__ dout, const GradArgs g) {
     const int gl = threadIdx.x & (g.lpr - 1);
     const long item = ((long)blockIdx.x << (8 - g.lpr_shift)) + (threadIdx.x >> g.lpr_shift);
     const long cold = (long)g.vocab * g.ncc;
     const long j = item < cold ? item : item - cold;
     const long r = j / g.ncc;
-    const int col = ((int)(j - r * g.ncc) * g.lpr + gl) * VW;
-    if (col >= g.d) return;
+    int col[CB];
+    bool ok[CB];
+#pragma unroll
+    for (int c = 0; c < CB; ++c) {
+        const int x = (((int)(j - r * g.ncc) * CB + c) * g.lpr + gl) * VW;
+        ok[c] = x < g.d;
+        col[c] = ok[c] ? x : 0;
+    }
+    if (!ok[0]) return;
+    Vals<VW> s[CB];
     if (item < cold) {
         const int a = g.starts[r], b = g.starts[r + 1];
         if (b - a > CHUNK) return;
-        Vals<VW> s = run_sum<TO, VW>(dout, g, a, b, col);
+        run_sum<TO, VW, CB>(dout, g, a, b, col, s);
 #pragma unroll
-        for (int i = 0; i < VW; ++i) s.v[i] *= g.scale;
-        st<VW>(g.dtable + r * g.ldt + col, s);
+        for (int c = 0; c < CB; ++c) {
+#pragma unroll
+            for (int i = 0; i < VW; ++i) s[c].v[i] *= g.scale;
+            if (ok[c]) st<VW>(g.dtable + r * g.ldt + col[c], s[c]);
+        }
         return;
     }
     const int live = *g.live;
     if (r >= g.nchunks || r * CHUNK >= live) return;
     const int a = (int)r * CHUNK, b = min(a + CHUNK, live);
-    float* part = g.part + r * 2 * g.d + col;
+    float* part = g.part + r * 2 * g.d;
     const int v0 = g.keys[a], s0 = g.starts[v0], e0 = g.starts[v0 + 1];
-    if (e0 - s0 > CHUNK && s0 < a) st<VW>(part, run_sum<TO, VW>(dout, g, a, min(e0, b), col));
+    if (e0 - s0 > CHUNK && s0 < a) {
+        run_sum<TO, VW, CB>(dout, g, a, min(e0, b), col, s);
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+            if (ok[c]) st<VW>(part + col[c], s[c]);
+    }
     const int v1 = g.keys[b - 1], s1 = g.starts[v1], e1 = g.starts[v1 + 1];
-    if (e1 - s1 > CHUNK && s1 >= a) st<VW>(part + g.d, run_sum<TO, VW>(dout, g, s1, b, col));
+    if (e1 - s1 > CHUNK && s1 >= a) {
+        run_sum<TO, VW, CB>(dout, g, s1, b, col, s);
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+            if (ok[c]) st<VW>(part + g.d + col[c], s[c]);
+    }
 }
 
-// The chunk a long run starts in folds its pieces: groups take every 256 / lpr th
+constexpr int FOLD = 512;
+// The chunk a long run starts in folds its pieces: groups take every FOLD / lpr th
 // piece in order, then add in group order.
 template <int VW>
-__global__ __launch_bounds__(256) void embed_fold_kernel(const GradArgs g) {
-    __shared__ float sh[256 * VW];
-    const int gl = threadIdx.x & (g.lpr - 1), grp = threadIdx.x >> g.lpr_shift, ng = 256 >> g.lpr_shift;
+__global__ __launch_bounds__(FOLD) void embed_fold_kernel(const GradArgs g) {
+    __shared__ float sh[FOLD * VW];
+    const int gl = threadIdx.x & (g.lpr - 1), grp = threadIdx.x >> g.lpr_shift, ng = FOLD >> g.lpr_shift;
     const int c = blockIdx.x / g.ncc, cc = blockIdx.x - c * g.ncc;
     const int live = *g.live;
     if ((long)c * CHUNK >= live) return;
@@ -356,12 +439,12 @@ __global__ __launch_bounds__(256) void embed_fold_kernel(const GradArgs g) {
         }
     }
 #pragma unroll
-    for (int i = 0; i < VW; ++i) sh[i * 256 + threadIdx.x] = s.v[i];
+    for (int i = 0; i < VW; ++i) sh[i * FOLD + threadIdx.x] = s.v[i];
     __syncthreads();
     if (grp > 0 || col >= g.d) return;
     for (int k = 1; k < ng; ++k)
 #pragma unroll
-        for (int i = 0; i < VW; ++i) s.v[i] += sh[i * 256 + k * g.lpr + gl];
+        for (int i = 0; i < VW; ++i) s.v[i] += sh[i * FOLD + k * g.lpr + gl];
 #pragma unroll
     for (int i = 0; i < VW; ++i) s.v[i] *= g.scale;
     st<VW>(g.dtable + (long)v * g.ldt + col, s);
@@ -445,16 +528,19 @@ int launch_grad(const TO* dout, GradArgs g, long rows, hipStream_t s) {
         g.lpr <<= 1;
         ++g.lpr_shift;
     }
-    g.ncc = pt_cdiv(cpr, g.lpr);
+    g.ncc = pt_cdiv(cpr, g.lpr);      // the fold's column blocks; the sums' are cb times as wide
     g.nchunks = rows > CHUNK ? pt_cdiv(rows, CHUNK) : 0;
+    const int cb = g.ncc > 1 ? 2 : 1, fold_ncc = g.ncc;
+    g.ncc = pt_cdiv(g.ncc, cb);
     const long items = ((long)g.vocab + g.nchunks) * g.ncc, per = 256 >> g.lpr_shift;
-    PT_REQUIRE((items + per - 1) / per < (1LL << 31) && (long)g.nchunks * g.ncc < (1LL << 31),
+    PT_REQUIRE((items + per - 1) / per < (1LL << 31) && (long)g.nchunks * fold_ncc < (1LL << 31),
                "embedding_bwd: %d rows of %d are too many", g.vocab, g.d);
-    hipLaunchKernelGGL((embed_grad_kernel<TO, VW>), dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, s, dout,
-                       g);
+    auto kern = cb == 2 ? embed_grad_kernel<TO, VW, 2> : embed_grad_kernel<TO, VW, 1>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, s, dout, g);
     PT_LAUNCH_CHECK();
     if (g.nchunks) {
-        hipLaunchKernelGGL(embed_fold_kernel<VW>, dim3((unsigned)(g.nchunks * g.ncc)), dim3(256), 0, s, g);
+        g.ncc = fold_ncc;
+        hipLaunchKernelGGL(embed_fold_kernel<VW>, dim3((unsigned)(g.nchunks * g.ncc)), dim3(FOLD), 0, s, g);
         PT_LAUNCH_CHECK();
     }
     return PTCG_OK;
@@ -518,7 +604,7 @@ extern "C" int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const
     a.n = (int)rows; a.vocab = vocab; a.bits = p.bits; a.tile = p.tile; a.nb = p.nb;
     a.cnt = ws + w.cnt; a.tot = ws + w.tot;
     a.starts = p.passes == 1 ? ws + w.starts : nullptr;
-    const size_t place_lds = (4 * (size_t)p.bins + 256) * sizeof(int);
+    const size_t place_lds = (5 * (size_t)p.bins + 4) * sizeof(int);
     for (int k = 0; k < p.passes; ++k) {
         a.shift = k * p.bits;
         a.live = k == 0 ? ws + w.live : nullptr;
@@ -527,7 +613,7 @@ extern "C" int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const
         a.out_pos = ws + (odd ? w.pos2 : w.pos);
         hipLaunchKernelGGL(sort_count_kernel, dim3(a.nb), dim3(256), p.bins * sizeof(int), s, a);
         PT_LAUNCH_CHECK();
-        hipLaunchKernelGGL(sort_scan_kernel, dim3(pt_cdiv(p.bins, 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(sort_scan_kernel, dim3(pt_cdiv(p.bins, 64)), dim3(1024), 0, s, a);
         PT_LAUNCH_CHECK();
         hipLaunchKernelGGL(sort_place_kernel, dim3(a.nb), dim3(256), place_lds, s, a);
         PT_LAUNCH_CHECK();

@@ -331,6 +331,7 @@ __device__ __forceinline__ void write_k_rows(T* base, long sl, int key0, int key
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
+constexpr size_t max3(size_t a, size_t b, size_t c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
 template <typename T, int DH, int BR> constexpr int tile_elems() { return BR * (DH + Frag<T>::PAD); }
 
 // ---------------------------------------------------------------- forward
@@ -341,12 +342,16 @@ template <typename T, int DH, int BR> constexpr int tile_elems() { return BR * (
 template <typename T, int DH, int NW, int KS, int KT> struct FwdCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
     static constexpr int TILE = tile_elems<T, DH, BK>();
-    // two buffers (one barrier a tile) where they leave room for another
-    // workgroup, or at all; else one
+    // Two buffers (one barrier a tile) for full row blocks in bf16: 324 us
+    // against 333 (16 samples of up to 1 501 x 4 003, 128 wide).  One elsewhere:
+    // what few tiles gain by a second buffer they lose in workgroups a CU holds
+    // (8 192 x 64 x 97, 64 wide: 293 us against 333; a token against 50 001 keys
+    // 39 against 46).
     static constexpr size_t PAIR = 2 * (size_t)TILE * sizeof(T);
-    static constexpr int NB = 2 * PAIR <= 144 * 1024 ? 2 : 1;
+    static constexpr int NB = NW == 4 && sizeof(T) == 2 ? 2 : 1;
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * (DH * 32 + 64) * sizeof(float);
-    static constexpr size_t BUFS = NB * PAIR > JOIN ? NB * PAIR : JOIN;
+    static constexpr size_t OUT = (size_t)NW * 32 * (DH + Frag<T>::PAD) * sizeof(T);   // the rows' way out
+    static constexpr size_t BUFS = max3(NB * PAIR, JOIN, OUT);
     static constexpr size_t LDS = BUFS + NB * BK * sizeof(float) + 64;
 };
 // Waves a SIMD holds, for the register allocator: two (of 256 registers each)
@@ -531,40 +536,56 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
                         tiles + qw * 32 * ST, lane);
 }
 
-// joins the key splits of one row per wave, in split order
+// Joins the key splits: a workgroup per row; groups of 32 lanes take every 8th
+// split, 4 columns a lane, and meet in LDS in group order (one wave walking 56
+// splits waits them in line: 13.6 us for 32 rows of 128).
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(const XArgs a, const float* __restrict__ part,
         T* __restrict__ out, float* __restrict__ lse, int nsplit) {
-    const int lane = threadIdx.x & 63;
-    const long R = (long)a.n * a.H * a.lq, row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= R) return;
+    __shared__ float4 sh[256];
+    __shared__ float shl[8], shm[4];
+    const int tid = threadIdx.x, lane = tid & 63, grp = tid >> 5, c = tid & 31;
+    const long R = (long)a.n * a.H * a.lq, row = blockIdx.x;
     const int qi = (int)(row % a.lq), head = (int)(row / a.lq % a.H), i = (int)(row / a.lq / a.H);
     const Sample s = sample_of(a, i);
     if (qi >= s.ql) return;
-    const float* ml = part + (long)nsplit * R * a.dh;
+    const float2* ml = reinterpret_cast<const float2*>(part + (long)nsplit * R * a.dh);
     float m = -INFINITY;
-    for (int p = lane; p < nsplit; p += 64) m = fmaxf(m, ml[((long)p * R + row) * 2]);
+    for (int p = tid; p < nsplit; p += 256) m = fmaxf(m, ml[p * R + row].x);
     m = wave_max(m);
+    if (lane == 0) shm[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(shm[0], shm[1]), fmaxf(shm[2], shm[3]));
     const float ms = m == -INFINITY ? 0.f : m;
     float l = 0.f;
-    for (int p = lane; p < nsplit; p += 64) {
-        const float* e = ml + ((long)p * R + row) * 2;
-        l += e[1] * __builtin_amdgcn_exp2f(e[0] - ms);
-    }
-    l = wave_sum(l);
-    const bool none = m == -INFINITY && l == 0.f;
-    T* orow = out + s.o + (long)qi * a.o.sl + (long)head * a.o.sh;
-    for (int d = lane; d < a.dh; d += 64) {
-        float acc = 0.f;
-        if (!none)
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-            for (int p = 0; p < nsplit; ++p) {
-                const long e = (long)p * R + row;
-                acc += part[e * a.dh + d] * __builtin_amdgcn_exp2f(ml[e * 2] - ms);
-            }
-        orow[d] = (T)(none ? 0.f : acc / l);
+    for (int p = grp; p < nsplit; p += 8) {
+        const float2 e = ml[p * R + row];
+        const float w = __builtin_amdgcn_exp2f(e.x - ms);
+        l += e.y * w;
+        // a split without a kept key left zeros (its w is 0 as well)
+        if (4 * c < a.dh) {
+            const float4 x = *reinterpret_cast<const float4*>(part + (p * R + row) * a.dh + 4 * c);
+            acc.x += x.x * w; acc.y += x.y * w; acc.z += x.z * w; acc.w += x.w * w;
+        }
     }
-    if (lse && lane == 0) lse[row] = none ? -INFINITY : m * LN2 + logf(l);
+    sh[tid] = acc;
+    if (c == 0) shl[grp] = l;
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int g = 1; g < 8; ++g) {
+        const float4 x = sh[g * 32 + c];
+        acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+        l += shl[g];
+    }
+    const bool none = m == -INFINITY && l == 0.f;
+    const float f = none ? 0.f : 1.f / l;
+    if (none) acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (4 * c < a.dh)
+        st4(out + s.o + (long)qi * a.o.sl + (long)head * a.o.sh + 4 * c, acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+    if (lse && c == 0) lse[row] = none ? -INFINITY : m * LN2 + logf(l);
 }
 
 // --------------------------------------------------------------- backward
@@ -576,9 +597,10 @@ template <typename T, int DH, int NW, int KS, int KT> struct DqCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
     static constexpr int TILE = tile_elems<T, DH, BK>();
     static constexpr size_t PAIR = 2 * (size_t)TILE * sizeof(T);
-    static constexpr int NB = 2 * PAIR <= 144 * 1024 ? 2 : 1;
+    static constexpr int NB = NW == 4 && sizeof(T) == 2 ? 2 : 1;   // as the forward
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * DH * 32 * sizeof(float);
-    static constexpr size_t BUFS = NB * PAIR > JOIN ? NB * PAIR : JOIN;
+    static constexpr size_t OUT = (size_t)NW * 32 * (DH + Frag<T>::PAD) * sizeof(T);   // the rows' way out
+    static constexpr size_t BUFS = max3(NB * PAIR, JOIN, OUT);
     static constexpr size_t LDS = BUFS + NB * BK * sizeof(float) + 64;
 };
 
@@ -727,9 +749,10 @@ template <typename T, int DH, int NK, int QS, int QT> struct DkvCfg {
     static constexpr int NTH = 64 * NK * QS, BKEY = 32 * NK, BQ = QT * QS;
     static constexpr int TILE = tile_elems<T, DH, BQ>();
     static constexpr size_t PAIR = 2 * (size_t)TILE * sizeof(T);
-    static constexpr int NB = 2 * PAIR <= 144 * 1024 ? 2 : 1;
+    static constexpr int NB = 1;      // a second buffer's addresses cost registers: 675 us against 798
     static constexpr size_t JOIN = (size_t)NK * (QS - 1) * 2 * DH * 32 * sizeof(float);
-    static constexpr size_t BUFS = NB * PAIR > JOIN ? NB * PAIR : JOIN;
+    static constexpr size_t OUT = (size_t)NK * 32 * (DH + Frag<T>::PAD) * sizeof(T);   // the rows' way out
+    static constexpr size_t BUFS = max3(NB * PAIR, JOIN, OUT);
     static constexpr size_t LDS = BUFS + NB * 2 * BQ * sizeof(float) + 16;
 };
 
@@ -811,9 +834,10 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
                 const float lv[4] = {lf.x, lf.y, lf.z, lf.w}, dv4[4] = {df.x, df.y, df.z, df.w};
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
+                    // a masked key's lane goes along: its columns are cleared at the end
                     const float pe = __builtin_amdgcn_exp2f(fmaf(p[4 * e + x], a.scale2, -lv[x]));
-                    p[4 * e + x] = kok ? pe : 0.f;
-                    d[4 * e + x] = kok ? pe * (d[4 * e + x] - dv4[x]) : 0.f;
+                    p[4 * e + x] = pe;
+                    d[4 * e + x] = pe * (d[4 * e + x] - dv4[x]);
                 }
             }
             mma_tr<DH, St::ST>(Ds + qr * St::ST, p, gv, lane);
@@ -894,8 +918,9 @@ int waves_for(long rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
 
 struct Plan { int nw, qtiles, nsplit, split_keys; };
 
-// Key splits (forward): where the rows' workgroups leave CUs idle, enough
-// workgroups for two per CU, at least four tiles of keys in each.
+// Key splits (forward), where the rows' workgroups leave CUs idle: four
+// workgroups a CU (samples differ in length; the shorter ones' last splits have
+// nothing to do), at least two tiles of keys in each.
 Plan fwd_plan(const PtcgCrossAttn* d) {
     Plan p;
     const long rows = (long)d->lq * (d->heads / d->kv_heads);
@@ -907,7 +932,7 @@ Plan fwd_plan(const PtcgCrossAttn* d) {
     p.nsplit = 1;
     p.split_keys = d->lk;
     if (blocks < cu && d->lk >= 8 * bk) {
-        const long want = (2 * cu + blocks - 1) / blocks, most = d->lk / (4 * bk);
+        const long want = (4 * cu + blocks - 1) / blocks, most = d->lk / (2 * bk);
         const int tiles = pt_cdiv(d->lk, bk);
         const int sp = (int)(want < most ? want : most);
         const int per = pt_cdiv(tiles, sp);
@@ -995,7 +1020,7 @@ int launch_fwd(const XArgs& a, const Plan& p, const void* q, const void* k, cons
                        static_cast<T*>(out), lse, part, p.qtiles, p.nsplit, p.split_keys);
     PT_LAUNCH_CHECK();
     if (p.nsplit > 1) {
-        hipLaunchKernelGGL(xattn_join_kernel<T>, dim3(pt_cdiv((long)a.n * a.H * a.lq, 4)), dim3(256), 0, s, a, part,
+        hipLaunchKernelGGL(xattn_join_kernel<T>, dim3((unsigned)((long)a.n * a.H * a.lq)), dim3(256), 0, s, a, part,
                            static_cast<T*>(out), lse, p.nsplit);
         PT_LAUNCH_CHECK();
     }
@@ -1052,7 +1077,7 @@ int bwd(const XArgs& a, const void* q, const void* k, const void* v, const void*
         const int nk = waves_for(a.lk);
         return nk == 1   ? launch_dkv<T, DH, 1, 4, 32>(a, q, k, v, lse, dout, delta, dk, dv, s)
                : nk == 2 ? launch_dkv<T, DH, 2, 2, 32>(a, q, k, v, lse, dout, delta, dk, dv, s)
-                         : launch_dkv<T, DH, 4, 1, 64>(a, q, k, v, lse, dout, delta, dk, dv, s);
+                         : launch_dkv<T, DH, 4, 1, DH == 128 ? 32 : 64>(a, q, k, v, lse, dout, delta, dk, dv, s);
     }
     return PTCG_OK;
 }

@@ -14,17 +14,21 @@
 // Layout.  The G = heads / kv_heads query heads of a kv head are one matrix of
 // lq * G rows (row r is query r / G, head r % G), so a single token's heads
 // fill one tile and a gradient's sum over the heads is a sum over rows.  All
-// products run as 32 x 32 tiles of v_mfma_f32_32x32x16_bf16 or
-// v_mfma_f32_32x32x2_f32, computed transposed: S^T = K Q^T leaves query
-// lane % 32 of keys {8 (r / 4) + 4 (lane / 32) + r % 4} in register r, which is
-// a B operand of O^T = V^T P^T over the same order of the keys, so P goes from
-// accumulators to the next product without passing through LDS, and a
-// query's maximum and sum are in-lane but for one exchange of the halves.  The
-// A operand V^T comes from row-major LDS by ds_read_b64_tr_b16 (4 keys of 16
-// columns to a lane's 4 values); in fp32 by plain 32-bit reads.
-// LDS row strides: 32 bytes of padding in bf16 keep both the row reads (8 lanes
-// of 16 bytes) and the transposed reads (4 rows of 32 bytes) free of bank
-// conflicts; 16 bytes in fp32.
+// products run as 32 x 32 tiles of v_mfma_f32_32x32x16_bf16, computed
+// transposed: S^T = K Q^T leaves query lane % 32 of keys {8 (r / 4) +
+// 4 (lane / 32) + r % 4} in register r, which is a B operand of O^T = V^T P^T
+// over the same order of the keys, so P goes from accumulators to the next
+// product without passing through LDS, and a query's maximum and sum are
+// in-lane but for one exchange of the halves.  The A operand V^T comes from
+// row-major LDS by ds_read_b64_tr_b16 (4 keys of 16 columns to a lane's 4
+// values).
+// fp32 operands are split into three bf16 terms (x = x0 + x1 + x2, 8 bits each,
+// exact above 2^-102) that lie in LDS as three planes; a product is the six
+// term products down to 2^-26 of it, small ones first: 6 / 16 of the time of
+// v_mfma_f32_32x32x2_f32.  An infinite operand becomes NaN in the products.
+// LDS rows are unpadded; 16-byte chunk c of a row lies at c ^ swz(row), which
+// keeps both the row reads (16 rows' chunk c) and the transposed reads (4 rows'
+// 4 chunks) on 64 different banks.
 #include "rowbuf.h"
 #include "../../include/ptcg_amd_kernels.h"
 
@@ -93,127 +97,182 @@ __device__ __forceinline__ int xcd_block(int nblk) {
 __device__ __forceinline__ float half_swap(float v) { return __shfl_xor(v, 32, 64); }
 
 // ------------------------------------------------------------- fragments
-// A row operand's chunk c holds dims 2 EL c + EL (lane / 32) + e, e < EL.
-template <typename T> struct Frag;
-template <> struct Frag<__bf16> { typedef bf16x8 V; static constexpr int EL = 8, PAD = 16; };
-template <> struct Frag<float> { typedef floatx4 V; static constexpr int EL = 4, PAD = 4; };
+template <typename T> constexpr int planes() { return sizeof(T) == 4 ? 3 : 1; }
 
-__device__ __forceinline__ void mma_row(bf16x8 a, bf16x8 b, floatx16& c) {
-    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ void mma_row(floatx4 a, floatx4 b, floatx16& c) {
+// x[0..8) as bf16 terms
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[3]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-}
-
-// 16-byte load of a row chunk
-template <typename T> __device__ __forceinline__ typename Frag<T>::V ldv(const T* p) {
-    return *reinterpret_cast<const typename Frag<T>::V*>(p);
-}
-template <typename T> __device__ __forceinline__ typename Frag<T>::V zerov() {
-    typename Frag<T>::V z;
-#pragma unroll
-    for (int e = 0; e < Frag<T>::EL; ++e) z[e] = (T)0.f;
-    return z;
-}
-
-// row fragments of one lane's global row (dims past dh, or no row: zeros)
-template <typename T, int DH>
-__device__ __forceinline__ void load_row(typename Frag<T>::V (&f)[DH / (2 * Frag<T>::EL)], const T* row, bool ok,
-                                         int dh, int h) {
-    constexpr int EL = Frag<T>::EL;
-#pragma unroll
-    for (int c = 0; c < DH / (2 * EL); ++c) {
-        const int d = 2 * EL * c + EL * h;
-        f[c] = ok && d < dh ? ldv<T>(row + d) : zerov<T>();
+    for (int i = 0; i < 8; ++i) {
+        t[0][i] = (__bf16)x[i];
+        const float r = x[i] - (float)t[0][i];
+        t[1][i] = (__bf16)r;
+        t[2][i] = (__bf16)(r - (float)t[1][i]);
     }
 }
+__device__ __forceinline__ void split8(const float (&x)[8], bf16x8 (&t)[1]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[0][i] = (__bf16)x[i];
+}
 
-// c += X^T P over 32 rows of X (row-major in LDS from xs, stride ST): c[dt] is
-// columns 32 dt .. of X; P's register r stands for row 8 (r / 4) + 4 h + r % 4.
-// bf16: P is rounded to bf16 for the product (relative 2^-9 each, as the
-// stored operands are); its fp32 values make the softmax's sum.
-template <int DH, int ST>
-__device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floatx16 (&c)[DH / 32], int lane) {
-    typedef __attribute__((address_space(3))) bf16x4* lds4;
-    const int i = lane & 15, h = lane >> 5;
-    const __bf16* a0 = xs + (4 * h + (i >> 2)) * ST + 16 * ((lane >> 4) & 1) + 4 * (i & 3);
+// c += a b by terms, small ones first
+__device__ __forceinline__ void mma(const bf16x8 (&a)[1], const bf16x8 (&b)[1], floatx16& c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
+}
+__device__ __forceinline__ void mma(const bf16x8 (&a)[3], const bf16x8 (&b)[3], floatx16& c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2], b[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[2], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[0], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
+}
+
+// 8 consecutive values as they lie in memory
+template <typename T> struct Chunk;
+template <> struct Chunk<__bf16> {
+    pt_uintx4 w;
+    __device__ __forceinline__ void terms(bf16x8 (&t)[1]) const { t[0] = __builtin_bit_cast(bf16x8, w); }
+    __device__ __forceinline__ void load(const __bf16* p) { w = *reinterpret_cast<const pt_uintx4*>(p); }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off) { w = ld_buf16(rs, off); }
+    __device__ __forceinline__ void zero() { w = pt_uintx4{0, 0, 0, 0}; }
+    __device__ __forceinline__ float at(int i) const {
+        return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+};
+template <> struct Chunk<float> {
+    pt_uintx4 w[2];
+    __device__ __forceinline__ void terms(bf16x8 (&t)[3]) const {
+        float x[8];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-        bf16x8 b;
+        for (int i = 0; i < 8; ++i) x[i] = at(i);
+        split8(x, t);
+    }
+    __device__ __forceinline__ void load(const float* p) {
+        w[0] = *reinterpret_cast<const pt_uintx4*>(p);
+        w[1] = *reinterpret_cast<const pt_uintx4*>(p + 4);
+    }
+    __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off) {
+        w[0] = ld_buf16(rs, off);
+        w[1] = ld_buf16(rs, off + 16);
+    }
+    __device__ __forceinline__ void zero() { w[0] = w[1] = pt_uintx4{0, 0, 0, 0}; }
+    __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i / 4][i % 4]); }
+};
+
+// a lane's row as an operand: chunk c holds dims 16 c + 8 (lane / 32) + 0..7
+template <typename T, int DH> struct Row {
+    bf16x8 f[DH / 16][planes<T>()];
+    // dims past dh, or no row: zeros
+    __device__ __forceinline__ void load(const T* row, bool ok, int dh, int h) {
+        Chunk<T> x[DH / 16];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) b[e] = (__bf16)p[8 * kb + e];
-#pragma unroll
-        for (int dt = 0; dt < DH / 32; ++dt) {
-            const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(a0 + 16 * kb * ST + 32 * dt));
-            const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(a0 + (16 * kb + 8) * ST + 32 * dt));
-            const bf16x8 a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            c[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c[dt], 0, 0, 0);
+        for (int c = 0; c < DH / 16; ++c) {
+            x[c].zero();
+            if (ok && 16 * c + 8 * h < dh) x[c].load(row + 16 * c + 8 * h);
         }
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) x[c].terms(f[c]);
     }
-}
-template <int DH, int ST>
-__device__ __forceinline__ void mma_tr(const float* xs, const floatx16& p, floatx16 (&c)[DH / 32], int lane) {
-    const float* a0 = xs + 4 * (lane >> 5) * ST + (lane & 31);
-#pragma unroll
-    for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int dt = 0; dt < DH / 32; ++dt)
-            c[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a0[(8 * (r / 4) + r % 4) * ST + 32 * dt], p[r], c[dt], 0, 0,
-                                                         0);
+};
+
+// where chunk c of LDS row `row` lies: c ^ swz(row)
+template <int DH> __device__ __forceinline__ int swz(int row) {
+    if constexpr (DH == 128) return (row & 3) << 2 | (row >> 2 & 3);
+    else if constexpr (DH == 64) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+    else return row >> 2 & 3;
 }
 
-// s = X Y^T of 32 LDS rows against a lane's row fragments
-template <typename T, int DH, int ST>
-__device__ __forceinline__ floatx16 mma_rows(const T* xs, const typename Frag<T>::V (&f)[DH / (2 * Frag<T>::EL)],
-                                             int lane) {
-    constexpr int EL = Frag<T>::EL;
+// S = X Y^T of 32 LDS rows of X (PS elements between its planes) against the
+// lanes' rows
+template <typename T, int DH, int PS>
+__device__ __forceinline__ floatx16 mma_rows(const __bf16* xs, const Row<T, DH>& y, int lane) {
     floatx16 s;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.f;
-    const T* x = xs + (lane & 31) * ST + EL * (lane >> 5);
+    const int row = lane & 31, at = row * DH + 8 * ((lane >> 5) ^ swz<DH>(row));
 #pragma unroll
-    for (int c = 0; c < DH / (2 * EL); ++c) mma_row(ldv<T>(x + 2 * EL * c), f[c], s);
+    for (int c = 0; c < DH / 16; ++c) {
+        bf16x8 a[planes<T>()];
+#pragma unroll
+        for (int p = 0; p < planes<T>(); ++p) a[p] = *reinterpret_cast<const bf16x8*>(xs + p * PS + (at ^ 16 * c));
+        mma(a, y.f[c], s);
+    }
     return s;
 }
 
-// A tile of BR rows on its way through registers into LDS: 16-byte chunks,
+// c += X^T P over 32 LDS rows of X: c[dt] is columns 32 dt .. of X; P's register
+// r stands for row 8 (r / 4) + 4 h + r % 4.  bf16: P is rounded to bf16 for the
+// product (relative 2^-9 each, as the stored operands are); its fp32 values make
+// the softmax's sum.
+template <typename T, int DH, int PS>
+__device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floatx16 (&c)[DH / 32], int lane) {
+    typedef __attribute__((address_space(3))) bf16x4* lds4;
+    const int i = lane & 15, r0 = 4 * (lane >> 5) + (i >> 2), ch = 2 * (lane >> 4 & 1) + (i >> 1 & 1);
+    const int lo = r0 * DH + 8 * (ch ^ swz<DH>(r0)) + 4 * (i & 1);
+    const int hi = (r0 + 8) * DH + 8 * (ch ^ swz<DH>(r0 + 8)) + 4 * (i & 1);
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        float x[8];
+        bf16x8 b[planes<T>()];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = p[8 * kb + e];
+        split8(x, b);
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt) {
+            bf16x8 a[planes<T>()];
+#pragma unroll
+            for (int pl = 0; pl < planes<T>(); ++pl) {
+                const __bf16* q = xs + pl * PS + 16 * kb * DH;
+                const bf16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + (lo ^ 32 * dt)));
+                const bf16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + (hi ^ 32 * dt)));
+                a[pl] = bf16x8{u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
+            }
+            mma(a, b, c[dt]);
+        }
+    }
+}
+
+// A tile of BR rows on its way through registers into LDS: chunks of 8 values,
 // thread t takes chunks t, t + NTH, ...  Loads are issued well before the
 // barrier that publishes them.
 template <typename T, int DH, int BR, int NTH> struct Stage {
-    static constexpr int E = Frag<T>::EL, CPR = DH / E, NCH = BR * CPR / NTH, RPP = NTH / CPR;
-    static constexpr int ST = DH + Frag<T>::PAD;
-    static_assert(BR * CPR % NTH == 0 && NTH % CPR == 0, "whole chunks per thread");
-    pt_uintx4 r[NCH];
+    static constexpr int CPR = DH / 8, NCH = BR * CPR / NTH, RPP = NTH / CPR, PS = BR * DH;
+    static_assert(BR * CPR % NTH == 0 && NTH % CPR == 0 && RPP % 16 == 0, "whole chunks per thread, one swizzle");
+    Chunk<T> r[NCH];
     // byte offset of the thread's first chunk; chunk i is i * RPP rows on
     static __device__ __forceinline__ int first(int ld, int dh, int tid) {
-        return tid % CPR * E < dh ? tid / CPR * ld + tid % CPR * 16 : PT_NOWHERE;
+        return tid % CPR * 8 < dh ? tid / CPR * ld + tid % CPR * 8 * (int)sizeof(T) : PT_NOWHERE;
     }
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off, int ld) {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) r[i] = ld_buf16(rs, off + i * (RPP * ld));
+        for (int i = 0; i < NCH; ++i) r[i].load(rs, off + i * (RPP * ld));
     }
     // rows of the flattened query matrix of kv head kvh, from row0; the last
     // row stands in for rows past it (zeroed on the way into LDS)
     __device__ __forceinline__ void load_q(const XArgs& a, const PtcgHeadLayout& l, const T* base, int kvh, int row0,
                                            int len, int tid) {
-        const int col = min(tid % CPR * E, a.dh - E);
+        const int col = min(tid % CPR * 8, a.dh - 8);
 #pragma unroll
         for (int i = 0; i < NCH; ++i)
-            r[i] = *reinterpret_cast<const pt_uintx4*>(
-                base + row_off(a, l, kvh, min(row0 + tid / CPR + i * RPP, len - 1)) + col);
+            r[i].load(base + row_off(a, l, kvh, min(row0 + tid / CPR + i * RPP, len - 1)) + col);
     }
-    __device__ __forceinline__ void put(T* s, int tid, int i, bool ok) const {
-        *reinterpret_cast<pt_uintx4*>(s + (tid / CPR + i * RPP) * ST + tid % CPR * E) = ok ? r[i] : pt_uintx4{0, 0, 0, 0};
+    __device__ __forceinline__ void put(__bf16* s, int tid, int i, bool ok) const {
+        const int row = tid / CPR + i * RPP;
+        bf16x8 t[planes<T>()];
+        r[i].terms(t);
+#pragma unroll
+        for (int p = 0; p < planes<T>(); ++p)
+            *reinterpret_cast<pt_uintx4*>(s + p * PS + row * DH + 8 * (tid % CPR ^ swz<DH>(row))) =
+                ok ? __builtin_bit_cast(pt_uintx4, t[p]) : pt_uintx4{0, 0, 0, 0};
     }
-    __device__ __forceinline__ void store(T* s, int tid) const {
+    __device__ __forceinline__ void store(__bf16* s, int tid) const {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) put(s, tid, i, true);
     }
     // rows below `rows`, columns below dh
-    __device__ __forceinline__ void store_q(T* s, int tid, int rows, int dh) const {
+    __device__ __forceinline__ void store_q(__bf16* s, int tid, int rows, int dh) const {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) put(s, tid, i, tid / CPR + i * RPP < rows && tid % CPR * E < dh);
+        for (int i = 0; i < NCH; ++i) put(s, tid, i, tid / CPR + i * RPP < rows && tid % CPR * 8 < dh);
     }
 };
 
@@ -250,7 +309,7 @@ template <typename T, int DH, int BK, int NTH> struct KvTile {
             kfr = __uint_as_float(ld_buf4(rm, 4 * tid));
         }
     }
-    __device__ __forceinline__ void store(T* Ks, T* Vs, float* kf, int tid) const {
+    __device__ __forceinline__ void store(__bf16* Ks, __bf16* Vs, float* kf, int tid) const {
         if (masks) {
 #pragma unroll
             for (int i = 0; i < St::NCH; ++i) {
@@ -298,41 +357,45 @@ __device__ __forceinline__ void store_row(T* row, const floatx16 (&o)[DH / 32], 
 }
 
 // A wave's 32 rows of a transposed accumulator to memory, times each row's f, by
-// way of LDS (ws: 32 rows of DH + PAD): whole rows of 16 bytes a lane instead of
-// 8 bytes here and there.  Rows r0 .. of kv head kvh, those below `rows`.
-template <typename T, int DH>
-__device__ __forceinline__ void write_q_rows(const XArgs& a, const PtcgHeadLayout& l, T* out, int kvh, int r0,
-                                             int rows, const floatx16 (&o)[DH / 32], float f, T* ws, int lane) {
-    constexpr int E = Frag<T>::EL, CPR = DH / E, ST = DH + Frag<T>::PAD;
-    store_row<T, DH>(ws + (lane & 31) * ST, o, f, DH, lane >> 5);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int i = 0; i < 32 * CPR / 64; ++i) {
-        const int c = i * 64 + lane, row = c / CPR, col = c % CPR * E;
-        if (r0 + row < rows && col < a.dh)
-            *reinterpret_cast<pt_uintx4*>(out + row_off(a, l, kvh, r0 + row) + col) =
-                *reinterpret_cast<const pt_uintx4*>(ws + row * ST + col);
+// way of LDS (ws: 32 padded rows): whole rows of 16 bytes a lane instead of 8
+// bytes here and there (8 192 x 64 x 97 bf16: 283 us with, 300 without).
+template <typename T, int DH> struct Out {
+    static constexpr int E = 16 / sizeof(T), CPR = DH / E, ST = DH + E, WAVE = 32 * ST;
+    static __device__ __forceinline__ void turn(T* ws, const floatx16 (&o)[DH / 32], float f, int lane) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        store_row<T, DH>(ws + (lane & 31) * ST, o, f, DH, lane >> 5);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-}
-// the same for key rows key0 .. of a matrix at base, row stride sl
-template <typename T, int DH>
-__device__ __forceinline__ void write_k_rows(T* base, long sl, int key0, int keys, int dh,
-                                             const floatx16 (&o)[DH / 32], float f, T* ws, int lane) {
-    constexpr int E = Frag<T>::EL, CPR = DH / E, ST = DH + Frag<T>::PAD;
-    store_row<T, DH>(ws + (lane & 31) * ST, o, f, DH, lane >> 5);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    // rows r0 .. of kv head kvh, those below `rows`
+    static __device__ __forceinline__ void query_rows(const XArgs& a, const PtcgHeadLayout& l, T* out, int kvh, int r0,
+                                                      int rows, const floatx16 (&o)[DH / 32], float f, T* ws,
+                                                      int lane) {
+        turn(ws, o, f, lane);
 #pragma unroll
-    for (int i = 0; i < 32 * CPR / 64; ++i) {
-        const int c = i * 64 + lane, row = c / CPR, col = c % CPR * E;
-        if (key0 + row < keys && col < dh)
-            *reinterpret_cast<pt_uintx4*>(base + (long)(key0 + row) * sl + col) =
-                *reinterpret_cast<const pt_uintx4*>(ws + row * ST + col);
+        for (int i = 0; i < 32 * CPR / 64; ++i) {
+            const int c = i * 64 + lane, row = c / CPR, col = c % CPR * E;
+            if (r0 + row < rows && col < a.dh)
+                *reinterpret_cast<pt_uintx4*>(out + row_off(a, l, kvh, r0 + row) + col) =
+                    *reinterpret_cast<const pt_uintx4*>(ws + row * ST + col);
+        }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-}
+    // key rows key0 .. of a matrix at base, row stride sl
+    static __device__ __forceinline__ void key_rows(T* base, long sl, int key0, int keys, int dh,
+                                                    const floatx16 (&o)[DH / 32], float f, T* ws, int lane) {
+        turn(ws, o, f, lane);
+#pragma unroll
+        for (int i = 0; i < 32 * CPR / 64; ++i) {
+            const int c = i * 64 + lane, row = c / CPR, col = c % CPR * E;
+            if (key0 + row < keys && col < dh)
+                *reinterpret_cast<pt_uintx4*>(base + (long)(key0 + row) * sl + col) =
+                    *reinterpret_cast<const pt_uintx4*>(ws + row * ST + col);
+        }
+    }
+};
 
 constexpr size_t max3(size_t a, size_t b, size_t c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
-template <typename T, int DH, int BR> constexpr int tile_elems() { return BR * (DH + Frag<T>::PAD); }
+// elements (bf16) of a tile of BR rows
+template <typename T, int DH, int BR> constexpr int tile_elems() { return planes<T>() * BR * DH; }
 
 // ---------------------------------------------------------------- forward
 // A workgroup owns 32 NW query rows; KS waves share a row block and split each
@@ -347,10 +410,10 @@ template <typename T, int DH, int NW, int KS, int KT> struct FwdCfg {
     // what few tiles gain by a second buffer they lose in workgroups a CU holds
     // (8 192 x 64 x 97, 64 wide: 293 us against 333; a token against 50 001 keys
     // 39 against 46).
-    static constexpr size_t PAIR = 2 * (size_t)TILE * sizeof(T);
+    static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
     static constexpr int NB = NW == 4 && sizeof(T) == 2 ? 2 : 1;
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * (DH * 32 + 64) * sizeof(float);
-    static constexpr size_t OUT = (size_t)NW * 32 * (DH + Frag<T>::PAD) * sizeof(T);   // the rows' way out
+    static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);   // the rows' way out
     static constexpr size_t BUFS = max3(NB * PAIR, JOIN, OUT);
     static constexpr size_t LDS = BUFS + NB * BK * sizeof(float) + 64;
 };
@@ -364,9 +427,9 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
         float* __restrict__ lse, float* __restrict__ part, int qtiles, int nsplit, int split_keys) {
     typedef FwdCfg<T, DH, NW, KS, KT> C;
     typedef KvTile<T, DH, C::BK, C::NTH> Kv;
-    constexpr int ST = Kv::St::ST;
-    extern __shared__ __align__(16) char smem[];
-    T* tiles = reinterpret_cast<T*>(smem);
+    constexpr int PS = Kv::St::PS;
+    extern __shared__ __align__(256) char smem[];
+    __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     float* kfs = reinterpret_cast<float*>(smem + C::BUFS);
     int* sh = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
@@ -387,8 +450,8 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
     kv.init(a, s, k, v, kvh, kend, tid);
     if (k0 < kend) kv.fetch(k0, tid);       // on its way while the masks are looked through
 
-    typename Frag<T>::V qf[DH / (2 * Frag<T>::EL)];
-    load_row<T, DH>(qf, q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
+    Row<T, DH> qf;
+    qf.load(q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
 
     float m2 = -INFINITY, l = 0.f;   // running maximum (of s scale2) and this half's sum
     floatx16 o[DH / 32];
@@ -409,15 +472,15 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
     }
     const int nt = kend > k0 ? (kend - k0 + C::BK - 1) / C::BK : 0;
 
-    auto tile = [&](int t, const T* Ks, const float* kf) {
-        const T* Vs = Ks + C::TILE;
+    auto tile = [&](int t, const __bf16* Ks, const float* kf) {
+        const __bf16* Vs = Ks + C::TILE;
         const int row0 = k0 + t * C::BK + kw * KT;
         if (row0 >= kend) return;
         const bool masked = a.keep || row0 + KT > kend;
         floatx16 sc[KT / 32];
         float mt = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < KT / 32; ++j) sc[j] = mma_rows<T, DH, ST>(Ks + (kw * KT + 32 * j) * ST, qf, lane);
+        for (int j = 0; j < KT / 32; ++j) sc[j] = mma_rows<T, DH, PS>(Ks + (kw * KT + 32 * j) * DH, qf, lane);
         if (masked) {
 #pragma unroll
             for (int j = 0; j < KT / 32; ++j)
@@ -450,7 +513,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
                 sc[j][e] = __builtin_amdgcn_exp2f(fmaf(sc[j][e], a.scale2, -ms));
                 l += sc[j][e];
             }
-            mma_tr<DH, ST>(Vs + (kw * KT + 32 * j) * ST, sc[j], o, lane);
+            mma_tr<T, DH, PS>(Vs + (kw * KT + 32 * j) * DH, sc[j], o, lane);
         }
     };
     if (nt > 0) {
@@ -461,7 +524,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
     for (int t = 0; t < nt; ++t) {
         const int cur = C::NB == 2 ? t & 1 : 0;
         if (C::NB == 2 && t + 1 < nt) {
-            T* nx = tiles + (cur ^ 1) * 2 * C::TILE;
+            __bf16* nx = tiles + (cur ^ 1) * 2 * C::TILE;
             kv.store(nx, nx + C::TILE, kfs + (cur ^ 1) * C::BK, tid);
             if (t + 2 < nt) kv.fetch(k0 + (t + 2) * C::BK, tid);
         }
@@ -532,8 +595,8 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
             for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
     }
     if (lse && rok && h == 0) lse[row] = none ? -INFINITY : m2 * LN2 + logf(l);
-    write_q_rows<T, DH>(a, a.o, out + s.o, kvh, qt * C::BQ + 32 * qw, rows, o, none ? 0.f : 1.f / l,
-                        tiles + qw * 32 * ST, lane);
+    Out<T, DH>::query_rows(a, a.o, out + s.o, kvh, qt * C::BQ + 32 * qw, rows, o, none ? 0.f : 1.f / l,
+                           reinterpret_cast<T*>(smem) + qw * Out<T, DH>::WAVE, lane);
 }
 
 // Joins the key splits: a workgroup per row; groups of 32 lanes take every 8th
@@ -596,10 +659,10 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const XArgs a, const fl
 template <typename T, int DH, int NW, int KS, int KT> struct DqCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
     static constexpr int TILE = tile_elems<T, DH, BK>();
-    static constexpr size_t PAIR = 2 * (size_t)TILE * sizeof(T);
+    static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
     static constexpr int NB = NW == 4 && sizeof(T) == 2 ? 2 : 1;   // as the forward
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * DH * 32 * sizeof(float);
-    static constexpr size_t OUT = (size_t)NW * 32 * (DH + Frag<T>::PAD) * sizeof(T);   // the rows' way out
+    static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);   // the rows' way out
     static constexpr size_t BUFS = max3(NB * PAIR, JOIN, OUT);
     static constexpr size_t LDS = BUFS + NB * BK * sizeof(float) + 64;
 };
@@ -611,9 +674,9 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
         float* __restrict__ delta, int qtiles) {
     typedef DqCfg<T, DH, NW, KS, KT> C;
     typedef KvTile<T, DH, C::BK, C::NTH> Kv;
-    constexpr int EL = Frag<T>::EL, NF = DH / (2 * EL), ST = Kv::St::ST;
-    extern __shared__ __align__(16) char smem[];
-    T* tiles = reinterpret_cast<T*>(smem);
+    constexpr int PS = Kv::St::PS;
+    extern __shared__ __align__(256) char smem[];
+    __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     float* kfs = reinterpret_cast<float*>(smem + C::BUFS);
     int* sh = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
@@ -632,25 +695,29 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
     kv.init(a, s, k, v, kvh, kend, tid);
     if (kend > 0) kv.fetch(0, tid);
 
-    typename Frag<T>::V qf[NF], df[NF];
-    load_row<T, DH>(qf, q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
+    Row<T, DH> qf, df;
+    qf.load(q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
     const long oo = s.o + (rok ? row_off(a, a.o, kvh, r) : 0);
-    load_row<T, DH>(df, dout + oo, rok, a.dh, h);
+    float D = 0.f;
+#pragma unroll
+    for (int c = 0; c < DH / 16; ++c) {
+        Chunk<T> x, y;
+        x.zero();
+        y.zero();
+        if (rok && 16 * c + 8 * h < a.dh) {
+            x.load(dout + oo + 16 * c + 8 * h);
+            y.load(out + oo + 16 * c + 8 * h);
+        }
+        x.terms(df.f[c]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) D += x.at(e) * y.at(e);
+    }
+    D += half_swap(D);
     const int qi = head_div(a, rok ? r : 0), head = kvh * a.G + (rok ? r : 0) - qi * a.G;
     const long lrow = ((long)i * a.H + head) * a.lq + qi;
     const float lr = rok ? lse[lrow] : -INFINITY;
     const bool none = lr == -INFINITY;
     const float l2 = none ? INFINITY : lr * LOG2E;
-    float D = 0.f;
-    {
-        typename Frag<T>::V of[NF];
-        load_row<T, DH>(of, out + oo, rok, a.dh, h);
-#pragma unroll
-        for (int c = 0; c < NF; ++c)
-#pragma unroll
-            for (int e = 0; e < EL; ++e) D += (float)of[c][e] * (float)df[c][e];
-    }
-    D += half_swap(D);
     if (rok && kw == 0 && h == 0) delta[lrow] = D;
 
     if (a.keep && kend > 0) {
@@ -670,15 +737,15 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
     for (int dt = 0; dt < DH / 32; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) g[dt][e] = 0.f;
-    auto tile = [&](int t, const T* Ks, const float* kf) {
-        const T* Vs = Ks + C::TILE;
+    auto tile = [&](int t, const __bf16* Ks, const float* kf) {
+        const __bf16* Vs = Ks + C::TILE;
 #pragma unroll 1
         for (int j = 0; j < KT / 32; ++j) {
             const int kr = kw * KT + 32 * j, row0 = t * C::BK + kr;
             if (row0 >= kend) break;
             const bool masked = a.keep || row0 + 32 > kend;
-            floatx16 sc = mma_rows<T, DH, ST>(Ks + kr * ST, qf, lane);
-            const floatx16 dp = mma_rows<T, DH, ST>(Vs + kr * ST, df, lane);
+            floatx16 sc = mma_rows<T, DH, PS>(Ks + kr * DH, qf, lane);
+            const floatx16 dp = mma_rows<T, DH, PS>(Vs + kr * DH, df, lane);
             if (masked) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -689,7 +756,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -l2)) * (dp[e] - D);
-            mma_tr<DH, ST>(Ks + kr * ST, sc, g, lane);
+            mma_tr<T, DH, PS>(Ks + kr * DH, sc, g, lane);
         }
     };
     if (nt > 0) {
@@ -700,7 +767,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
     for (int t = 0; t < nt; ++t) {
         const int cur = C::NB == 2 ? t & 1 : 0;
         if (C::NB == 2 && t + 1 < nt) {
-            T* nx = tiles + (cur ^ 1) * 2 * C::TILE;
+            __bf16* nx = tiles + (cur ^ 1) * 2 * C::TILE;
             kv.store(nx, nx + C::TILE, kfs + (cur ^ 1) * C::BK, tid);
             if (t + 2 < nt) kv.fetch((t + 2) * C::BK, tid);
         }
@@ -738,7 +805,8 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
 #pragma unroll
             for (int e = 0; e < 16; ++e) g[dt][e] = 0.f;
     }
-    write_q_rows<T, DH>(a, a.q, dq + s.q, kvh, qt * C::BQ + 32 * qw, rows, g, a.scale, tiles + qw * 32 * ST, lane);
+    Out<T, DH>::query_rows(a, a.q, dq + s.q, kvh, qt * C::BQ + 32 * qw, rows, g, a.scale,
+                           reinterpret_cast<T*>(smem) + qw * Out<T, DH>::WAVE, lane);
 }
 
 // dK and dV: a workgroup owns 32 NK keys of one kv head, a wave 32 of them, and
@@ -748,10 +816,10 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
 template <typename T, int DH, int NK, int QS, int QT> struct DkvCfg {
     static constexpr int NTH = 64 * NK * QS, BKEY = 32 * NK, BQ = QT * QS;
     static constexpr int TILE = tile_elems<T, DH, BQ>();
-    static constexpr size_t PAIR = 2 * (size_t)TILE * sizeof(T);
+    static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
     static constexpr int NB = 1;      // a second buffer's addresses cost registers: 675 us against 798
     static constexpr size_t JOIN = (size_t)NK * (QS - 1) * 2 * DH * 32 * sizeof(float);
-    static constexpr size_t OUT = (size_t)NK * 32 * (DH + Frag<T>::PAD) * sizeof(T);   // the rows' way out
+    static constexpr size_t OUT = (size_t)NK * Out<T, DH>::WAVE * sizeof(T);   // the rows' way out
     static constexpr size_t BUFS = max3(NB * PAIR, JOIN, OUT);
     static constexpr size_t LDS = BUFS + NB * 2 * BQ * sizeof(float) + 16;
 };
@@ -763,9 +831,8 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
         int ktiles) {
     typedef DkvCfg<T, DH, NK, QS, QT> C;
     typedef Stage<T, DH, C::BQ, C::NTH> St;
-    constexpr int NF = DH / (2 * Frag<T>::EL);
-    extern __shared__ __align__(16) char smem[];
-    T* tiles = reinterpret_cast<T*>(smem);
+    extern __shared__ __align__(256) char smem[];
+    __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     float* lss = reinterpret_cast<float*>(smem + C::BUFS);   // log-sum-exp and D of each buffer's rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int kwv = wave % NK, qs = wave / NK;
@@ -779,11 +846,11 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
     const bool kin = key < kall;
     const bool kok = key < s.kl && (!a.keep || a.keep[s.keep + key] != 0.f);
 
-    typename Frag<T>::V kfr[NF], vfr[NF];
+    Row<T, DH> kfr, vfr;
     const long ko = s.k + (kin ? (long)key * a.k.sl + (long)kvh * a.k.sh : 0);
     const long vo = s.v + (kin ? (long)key * a.v.sl + (long)kvh * a.v.sh : 0);
-    load_row<T, DH>(kfr, k + ko, kok, a.dh, h);
-    load_row<T, DH>(vfr, v + vo, kok, a.dh, h);
+    kfr.load(k + ko, kok, a.dh, h);
+    vfr.load(v + vo, kok, a.dh, h);
     floatx16 gk[DH / 32], gv[DH / 32];
 #pragma unroll
     for (int dt = 0; dt < DH / 32; ++dt)
@@ -808,7 +875,7 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
             dr = delta[lrow];
         }
     };
-    auto store = [&](T* Qs, float* ls) {
+    auto store = [&](__bf16* Qs, float* ls) {
         qs_.store_q(Qs, tid, rown, a.dh);
         ds_.store_q(Qs + C::TILE, tid, rown, a.dh);
         if (tid < C::BQ) {
@@ -818,15 +885,15 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
             ls[C::BQ + tid] = live ? dr : 0.f;
         }
     };
-    auto tile = [&](int t, const T* Qs, const float* ls) {
-        const T* Ds = Qs + C::TILE;
+    auto tile = [&](int t, const __bf16* Qs, const float* ls) {
+        const __bf16* Ds = Qs + C::TILE;
         const float* dl = ls + C::BQ;
 #pragma unroll 1
         for (int j = 0; j < QT / 32; ++j) {
             const int qr = qs * QT + 32 * j;
             if (t * C::BQ + qr >= rows) break;
-            floatx16 p = mma_rows<T, DH, St::ST>(Qs + qr * St::ST, kfr, lane);
-            floatx16 d = mma_rows<T, DH, St::ST>(Ds + qr * St::ST, vfr, lane);
+            floatx16 p = mma_rows<T, DH, St::PS>(Qs + qr * DH, kfr, lane);
+            floatx16 d = mma_rows<T, DH, St::PS>(Ds + qr * DH, vfr, lane);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float4 lf = *reinterpret_cast<const float4*>(ls + qr + 8 * e + 4 * h);
@@ -840,8 +907,8 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
                     d[4 * e + x] = pe * (d[4 * e + x] - dv4[x]);
                 }
             }
-            mma_tr<DH, St::ST>(Ds + qr * St::ST, p, gv, lane);
-            mma_tr<DH, St::ST>(Qs + qr * St::ST, d, gk, lane);
+            mma_tr<T, DH, St::PS>(Ds + qr * DH, p, gv, lane);
+            mma_tr<T, DH, St::PS>(Qs + qr * DH, d, gk, lane);
         }
     };
     if (nt > 0) {
@@ -898,9 +965,9 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
             for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
     }
     const int key0 = kt * C::BKEY + 32 * kwv;
-    T* ws = tiles + kwv * 32 * St::ST;
-    write_k_rows<T, DH>(dk + s.k + (long)kvh * a.k.sh, a.k.sl, key0, kall, a.dh, gk, a.scale, ws, lane);
-    write_k_rows<T, DH>(dv + s.v + (long)kvh * a.v.sh, a.v.sl, key0, kall, a.dh, gv, 1.f, ws, lane);
+    T* ws = reinterpret_cast<T*>(smem) + kwv * Out<T, DH>::WAVE;
+    Out<T, DH>::key_rows(dk + s.k + (long)kvh * a.k.sh, a.k.sl, key0, kall, a.dh, gk, a.scale, ws, lane);
+    Out<T, DH>::key_rows(dv + s.v + (long)kvh * a.v.sh, a.v.sl, key0, kall, a.dh, gv, 1.f, ws, lane);
 }
 
 // ------------------------------------------------------------------- host
@@ -912,9 +979,10 @@ int cu_count() {
     return cu;
 }
 
-// rows (or keys) a workgroup covers: waves along them, the rest of the four
-// split the other axis
-int waves_for(long rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+// Waves along a workgroup's rows (or keys); the rest of the four split the other
+// axis.  Four along the other axis take a tile of 128 rows, which in fp32 (three
+// planes) fits LDS up to 64 wide.
+int waves_for(long rows, bool bf16, int dh) { return rows <= 32 && (bf16 || dh <= 64) ? 1 : rows <= 64 ? 2 : 4; }
 
 struct Plan { int nw, qtiles, nsplit, split_keys; };
 
@@ -924,7 +992,7 @@ struct Plan { int nw, qtiles, nsplit, split_keys; };
 Plan fwd_plan(const PtcgCrossAttn* d) {
     Plan p;
     const long rows = (long)d->lq * (d->heads / d->kv_heads);
-    p.nw = waves_for(rows);
+    p.nw = waves_for(rows, d->bf16, d->dh);
     p.qtiles = pt_cdiv(rows, 32 * p.nw);
     const int bk = p.nw == 1 ? 128 : 64;
     const long blocks = (long)d->n * d->kv_heads * p.qtiles;
@@ -1030,7 +1098,8 @@ int launch_fwd(const XArgs& a, const Plan& p, const void* q, const void* k, cons
 template <typename T, int DH>
 int fwd_nw(const XArgs& a, const Plan& p, const void* q, const void* k, const void* v, void* out, float* lse,
            float* part, hipStream_t s) {
-    if (p.nw == 1) return launch_fwd<T, DH, 1, 4, 32>(a, p, q, k, v, out, lse, part, s);
+    if constexpr (sizeof(T) == 2 || DH <= 64)
+        if (p.nw == 1) return launch_fwd<T, DH, 1, 4, 32>(a, p, q, k, v, out, lse, part, s);
     if (p.nw == 2) return launch_fwd<T, DH, 2, 2, 32>(a, p, q, k, v, out, lse, part, s);
     return launch_fwd<T, DH, 4, 1, 64>(a, p, q, k, v, out, lse, part, s);
 }
@@ -1067,17 +1136,20 @@ int launch_dkv(const XArgs& a, const void* q, const void* k, const void* v, cons
 template <typename T, int DH>
 int bwd(const XArgs& a, const void* q, const void* k, const void* v, const void* out, const float* lse,
         const void* dout, void* dq, void* dk, void* dv, float* delta, hipStream_t s) {
+    constexpr bool ONE = sizeof(T) == 2 || DH <= 64;
     if (a.lq > 0) {
-        const int nw = waves_for((long)a.lq * a.G);
-        PT_TRY(nw == 1   ? (launch_dq<T, DH, 1, 4, 32>(a, q, k, v, out, lse, dout, dq, delta, s))
-               : nw == 2 ? (launch_dq<T, DH, 2, 2, 32>(a, q, k, v, out, lse, dout, dq, delta, s))
-                         : (launch_dq<T, DH, 4, 1, 64>(a, q, k, v, out, lse, dout, dq, delta, s)));
+        const int nw = waves_for((long)a.lq * a.G, sizeof(T) == 2, DH);
+        if constexpr (ONE)
+            if (nw == 1) PT_TRY((launch_dq<T, DH, 1, 4, 32>(a, q, k, v, out, lse, dout, dq, delta, s)));
+        if (nw == 2) PT_TRY((launch_dq<T, DH, 2, 2, 32>(a, q, k, v, out, lse, dout, dq, delta, s)));
+        if (nw == 4) PT_TRY((launch_dq<T, DH, 4, 1, 64>(a, q, k, v, out, lse, dout, dq, delta, s)));
     }
     if (a.lk > 0) {
-        const int nk = waves_for(a.lk);
-        return nk == 1   ? launch_dkv<T, DH, 1, 4, 32>(a, q, k, v, lse, dout, delta, dk, dv, s)
-               : nk == 2 ? launch_dkv<T, DH, 2, 2, 32>(a, q, k, v, lse, dout, delta, dk, dv, s)
-                         : launch_dkv<T, DH, 4, 1, DH == 128 ? 32 : 64>(a, q, k, v, lse, dout, delta, dk, dv, s);
+        const int nk = waves_for(a.lk, sizeof(T) == 2, DH);
+        if constexpr (ONE)
+            if (nk == 1) return launch_dkv<T, DH, 1, 4, 32>(a, q, k, v, lse, dout, delta, dk, dv, s);
+        if (nk == 2) return launch_dkv<T, DH, 2, 2, 32>(a, q, k, v, lse, dout, delta, dk, dv, s);
+        return launch_dkv<T, DH, 4, 1, DH == 128 || (DH == 64 && sizeof(T) == 4) ? 32 : 64>(a, q, k, v, lse, dout, delta, dk, dv, s);
     }
     return PTCG_OK;
 }

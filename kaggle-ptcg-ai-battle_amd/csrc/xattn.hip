@@ -26,9 +26,6 @@
 // exact above 2^-102) that lie in LDS as three planes; a product is the six
 // term products down to 2^-26 of it, small ones first: 6 / 16 of the time of
 // v_mfma_f32_32x32x2_f32.  An infinite operand becomes NaN in the products.
-// LDS rows are unpadded; 16-byte chunk c of a row lies at c ^ swz(row), which
-// keeps both the row reads (16 rows' chunk c) and the transposed reads (4 rows'
-// 4 chunks) on 64 different banks.
 #include "rowbuf.h"
 #include "../../include/ptcg_amd_kernels.h"
 
@@ -52,6 +49,7 @@ struct XArgs {
     const int *q_off, *k_off, *k_len;
     const float* keep;
     long keep_sn;
+    bool sorted;                  // place_of
 };
 
 struct Sample { long q, k, v, o, keep; int ql, kl; };   // element offsets of row 0, and row counts
@@ -92,6 +90,35 @@ __device__ __forceinline__ long row_off(const XArgs& a, const PtcgHeadLayout& l,
 __device__ __forceinline__ int xcd_block(int nblk) {
     const int x = blockIdx.x & 7, per = nblk >> 3, rem = nblk & 7;
     return x * per + min(x, rem) + (blockIdx.x >> 3);
+}
+
+// Which (sample, rest) a workgroup works on.  Samples whose lengths only the
+// device knows (`sorted`: up to 64 of them) are taken in the order of a tile's
+// cost, longest first, without gaps: workgroups start in index order, and a long
+// one that starts last runs alone (16 packed samples of 376 .. 1 501 rows and
+// 1 001 .. 4 003 keys on 512 places).  Indexes past the last tile: i = -1.
+struct Place { int i, rest; };
+template <class Cost, class Tiles>
+__device__ __forceinline__ Place place_of(const XArgs& a, bool sorted, int per_sample, Cost cost, Tiles tiles) {
+    Place p;
+    if (!sorted) {
+        const int b = xcd_block(gridDim.x);
+        p.i = b / per_sample;
+        p.rest = b - p.i * per_sample;
+        return p;
+    }
+    const int lane = threadIdx.x & 63, b = blockIdx.x;
+    const Sample s = sample_of(a, min(lane, a.n - 1));
+    const int c = lane < a.n ? cost(s) : -1, t = lane < a.n ? tiles(s) : 0;
+    int first = 0;
+    for (int j = 0; j < a.n; ++j) {
+        const int cj = __builtin_amdgcn_readlane(c, j), tj = __builtin_amdgcn_readlane(t, j);
+        if (cj > c || (cj == c && j < lane)) first += tj;
+    }
+    const unsigned long long m = __ballot(b >= first && b < first + t);
+    p.i = m ? __builtin_ctzll(m) : -1;
+    p.rest = m ? b - __builtin_amdgcn_readlane(first, __builtin_ctzll(m)) : 0;
+    return p;
 }
 
 __device__ __forceinline__ float half_swap(float v) { return __shfl_xor(v, 32, 64); }
@@ -175,11 +202,26 @@ template <typename T, int DH> struct Row {
     }
 };
 
-// where chunk c of LDS row `row` lies: c ^ swz(row)
+// LDS rows are ST elements apart and chunk c (8 values) of a row lies at
+// c ^ swz(row).  Both keep the row reads (16 rows' chunk c) and the transposed
+// reads (4 rows' 4 chunks) on 64 different banks.  128 wide: 64 bytes of
+// padding move 4 successive rows to different quarters of the banks and only
+// the low two bits of c are turned, so that most of an operand's addresses are
+// one register and a constant.
+template <int DH> constexpr int row_st() { return DH == 128 ? 160 : DH; }
 template <int DH> __device__ __forceinline__ int swz(int row) {
-    if constexpr (DH == 128) return (row & 3) << 2 | (row >> 2 & 3);
-    else if constexpr (DH == 64) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+    if constexpr (DH == 64) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
     else return row >> 2 & 3;
+}
+// element offset of chunk 2 c + h of a row
+template <int DH> __device__ __forceinline__ int chunk_at(int row, int h, int c) {
+    if constexpr (DH == 128) return row * row_st<DH>() + 8 * ((2 * (c & 1) + h) ^ swz<DH>(row)) + 32 * (c >> 1);
+    else return row * DH + (8 * (h ^ swz<DH>(row)) ^ 16 * c);
+}
+// element offset of column group dt (32 columns), chunk ch of it
+template <int DH> __device__ __forceinline__ int group_at(int row, int ch, int dt) {
+    if constexpr (DH == 128) return row * row_st<DH>() + 8 * (ch ^ swz<DH>(row)) + 32 * dt;
+    else return row * DH + (8 * (ch ^ swz<DH>(row)) ^ 32 * dt);
 }
 
 // S = X Y^T of 32 LDS rows of X (PS elements between its planes) against the
@@ -189,12 +231,11 @@ __device__ __forceinline__ floatx16 mma_rows(const __bf16* xs, const Row<T, DH>&
     floatx16 s;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = 0.f;
-    const int row = lane & 31, at = row * DH + 8 * ((lane >> 5) ^ swz<DH>(row));
 #pragma unroll
     for (int c = 0; c < DH / 16; ++c) {
         bf16x8 a[planes<T>()];
 #pragma unroll
-        for (int p = 0; p < planes<T>(); ++p) a[p] = *reinterpret_cast<const bf16x8*>(xs + p * PS + (at ^ 16 * c));
+        for (int p = 0; p < planes<T>(); ++p) a[p] = *reinterpret_cast<const bf16x8*>(xs + p * PS + chunk_at<DH>(lane & 31, lane >> 5, c));
         mma(a, y.f[c], s);
     }
     return s;
@@ -208,8 +249,6 @@ template <typename T, int DH, int PS>
 __device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floatx16 (&c)[DH / 32], int lane) {
     typedef __attribute__((address_space(3))) bf16x4* lds4;
     const int i = lane & 15, r0 = 4 * (lane >> 5) + (i >> 2), ch = 2 * (lane >> 4 & 1) + (i >> 1 & 1);
-    const int lo = r0 * DH + 8 * (ch ^ swz<DH>(r0)) + 4 * (i & 1);
-    const int hi = (r0 + 8) * DH + 8 * (ch ^ swz<DH>(r0 + 8)) + 4 * (i & 1);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
         float x[8];
@@ -222,9 +261,9 @@ __device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floa
             bf16x8 a[planes<T>()];
 #pragma unroll
             for (int pl = 0; pl < planes<T>(); ++pl) {
-                const __bf16* q = xs + pl * PS + 16 * kb * DH;
-                const bf16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + (lo ^ 32 * dt)));
-                const bf16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + (hi ^ 32 * dt)));
+                const __bf16* q = xs + pl * PS + 16 * kb * row_st<DH>() + 4 * (i & 1);
+                const bf16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + group_at<DH>(r0, ch, dt)));
+                const bf16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + group_at<DH>(r0 + 8, ch, dt)));
                 a[pl] = bf16x8{u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
             }
             mma(a, b, c[dt]);
@@ -236,7 +275,7 @@ __device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floa
 // thread t takes chunks t, t + NTH, ...  Loads are issued well before the
 // barrier that publishes them.
 template <typename T, int DH, int BR, int NTH> struct Stage {
-    static constexpr int CPR = DH / 8, NCH = BR * CPR / NTH, RPP = NTH / CPR, PS = BR * DH;
+    static constexpr int CPR = DH / 8, NCH = BR * CPR / NTH, RPP = NTH / CPR, PS = BR * row_st<DH>();
     static_assert(BR * CPR % NTH == 0 && NTH % CPR == 0 && RPP % 16 == 0, "whole chunks per thread, one swizzle");
     Chunk<T> r[NCH];
     // byte offset of the thread's first chunk; chunk i is i * RPP rows on
@@ -262,7 +301,7 @@ template <typename T, int DH, int BR, int NTH> struct Stage {
         r[i].terms(t);
 #pragma unroll
         for (int p = 0; p < planes<T>(); ++p)
-            *reinterpret_cast<pt_uintx4*>(s + p * PS + row * DH + 8 * (tid % CPR ^ swz<DH>(row))) =
+            *reinterpret_cast<pt_uintx4*>(s + p * PS + row * row_st<DH>() + 8 * (tid % CPR ^ swz<DH>(row))) =
                 ok ? __builtin_bit_cast(pt_uintx4, t[p]) : pt_uintx4{0, 0, 0, 0};
     }
     __device__ __forceinline__ void store(__bf16* s, int tid) const {
@@ -395,7 +434,7 @@ template <typename T, int DH> struct Out {
 
 constexpr size_t max3(size_t a, size_t b, size_t c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
 // elements (bf16) of a tile of BR rows
-template <typename T, int DH, int BR> constexpr int tile_elems() { return planes<T>() * BR * DH; }
+template <typename T, int DH, int BR> constexpr int tile_elems() { return planes<T>() * BR * row_st<DH>(); }
 
 // ---------------------------------------------------------------- forward
 // A workgroup owns 32 NW query rows; KS waves share a row block and split each
@@ -405,17 +444,14 @@ template <typename T, int DH, int BR> constexpr int tile_elems() { return planes
 template <typename T, int DH, int NW, int KS, int KT> struct FwdCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
     static constexpr int TILE = tile_elems<T, DH, BK>();
-    // Two buffers (one barrier a tile) for full row blocks in bf16: 324 us
-    // against 333 (16 samples of up to 1 501 x 4 003, 128 wide).  One elsewhere:
-    // what few tiles gain by a second buffer they lose in workgroups a CU holds
-    // (8 192 x 64 x 97, 64 wide: 293 us against 333; a token against 50 001 keys
-    // 39 against 46).
+    // One buffer: what a second one saves in barriers it costs in workgroups a CU
+    // holds (8 192 x 64 x 97, 64 wide: 293 us against 333; a token against 50 001
+    // keys 39 against 46).
     static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
-    static constexpr int NB = NW == 4 && sizeof(T) == 2 ? 2 : 1;
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * (DH * 32 + 64) * sizeof(float);
     static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);   // the rows' way out
-    static constexpr size_t BUFS = max3(NB * PAIR, JOIN, OUT);
-    static constexpr size_t LDS = BUFS + NB * BK * sizeof(float) + 64;
+    static constexpr size_t BUFS = max3(PAIR, JOIN, OUT);
+    static constexpr size_t LDS = BUFS + BK * sizeof(float) + 64;
 };
 // Waves a SIMD holds, for the register allocator: two (of 256 registers each)
 // let one wave's softmax run beside the other's products.
@@ -434,11 +470,13 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
     int* sh = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int qw = wave % NW, kw = wave / NW;
-    int b = xcd_block(gridDim.x);
-    const int qt = b % qtiles; b /= qtiles;
-    const int sp = b % nsplit; b /= nsplit;
-    const int kvh = b % a.KV, i = b / a.KV;
+    const Place pl = place_of(a, a.sorted && nsplit == 1, a.KV * qtiles * nsplit, [](const Sample& x) { return x.kl; },
+                              [&](const Sample& x) { return (x.ql * a.G + C::BQ - 1) / C::BQ * a.KV; });
+    if (pl.i < 0) return;
+    const int i = pl.i;
     const Sample s = sample_of(a, i);
+    const int qtn = a.sorted && nsplit == 1 ? (s.ql * a.G + C::BQ - 1) / C::BQ : qtiles;
+    const int qt = pl.rest % qtn, sp = pl.rest / qtn % nsplit, kvh = pl.rest / qtn / nsplit;
     const int rows = s.ql * a.G;
     if (qt * C::BQ >= rows) return;
     const int r = qt * C::BQ + 32 * qw + (lane & 31);
@@ -480,7 +518,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
         floatx16 sc[KT / 32];
         float mt = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < KT / 32; ++j) sc[j] = mma_rows<T, DH, PS>(Ks + (kw * KT + 32 * j) * DH, qf, lane);
+        for (int j = 0; j < KT / 32; ++j) sc[j] = mma_rows<T, DH, PS>(Ks + (kw * KT + 32 * j) * row_st<DH>(), qf, lane);
         if (masked) {
 #pragma unroll
             for (int j = 0; j < KT / 32; ++j)
@@ -513,7 +551,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
                 sc[j][e] = __builtin_amdgcn_exp2f(fmaf(sc[j][e], a.scale2, -ms));
                 l += sc[j][e];
             }
-            mma_tr<T, DH, PS>(Vs + (kw * KT + 32 * j) * DH, sc[j], o, lane);
+            mma_tr<T, DH, PS>(Vs + (kw * KT + 32 * j) * row_st<DH>(), sc[j], o, lane);
         }
     };
     if (nt > 0) {
@@ -522,15 +560,9 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
         __syncthreads();
     }
     for (int t = 0; t < nt; ++t) {
-        const int cur = C::NB == 2 ? t & 1 : 0;
-        if (C::NB == 2 && t + 1 < nt) {
-            __bf16* nx = tiles + (cur ^ 1) * 2 * C::TILE;
-            kv.store(nx, nx + C::TILE, kfs + (cur ^ 1) * C::BK, tid);
-            if (t + 2 < nt) kv.fetch(k0 + (t + 2) * C::BK, tid);
-        }
-        tile(t, tiles + cur * 2 * C::TILE, kfs + cur * C::BK);
+        tile(t, tiles, kfs);
         __syncthreads();
-        if (C::NB == 1 && t + 1 < nt) {
+        if (t + 1 < nt) {
             kv.store(tiles, tiles + C::TILE, kfs, tid);
             if (t + 2 < nt) kv.fetch(k0 + (t + 2) * C::BK, tid);
             __syncthreads();
@@ -660,11 +692,10 @@ template <typename T, int DH, int NW, int KS, int KT> struct DqCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
     static constexpr int TILE = tile_elems<T, DH, BK>();
     static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
-    static constexpr int NB = NW == 4 && sizeof(T) == 2 ? 2 : 1;   // as the forward
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * DH * 32 * sizeof(float);
     static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);   // the rows' way out
-    static constexpr size_t BUFS = max3(NB * PAIR, JOIN, OUT);
-    static constexpr size_t LDS = BUFS + NB * BK * sizeof(float) + 64;
+    static constexpr size_t BUFS = max3(PAIR, JOIN, OUT);
+    static constexpr size_t LDS = BUFS + BK * sizeof(float) + 64;
 };
 
 template <typename T, int DH, int NW, int KS, int KT>
@@ -681,10 +712,13 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
     int* sh = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int qw = wave % NW, kw = wave / NW;
-    int b = xcd_block(gridDim.x);
-    const int qt = b % qtiles; b /= qtiles;
-    const int kvh = b % a.KV, i = b / a.KV;
+    const Place pl = place_of(a, a.sorted, a.KV * qtiles, [](const Sample& x) { return x.kl; },
+                              [&](const Sample& x) { return (x.ql * a.G + C::BQ - 1) / C::BQ * a.KV; });
+    if (pl.i < 0) return;
+    const int i = pl.i;
     const Sample s = sample_of(a, i);
+    const int qtn = a.sorted ? (s.ql * a.G + C::BQ - 1) / C::BQ : qtiles;
+    const int qt = pl.rest % qtn, kvh = pl.rest / qtn;
     const int rows = s.ql * a.G;
     if (qt * C::BQ >= rows) return;
     const int r = qt * C::BQ + 32 * qw + (lane & 31);
@@ -744,8 +778,8 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
             const int kr = kw * KT + 32 * j, row0 = t * C::BK + kr;
             if (row0 >= kend) break;
             const bool masked = a.keep || row0 + 32 > kend;
-            floatx16 sc = mma_rows<T, DH, PS>(Ks + kr * DH, qf, lane);
-            const floatx16 dp = mma_rows<T, DH, PS>(Vs + kr * DH, df, lane);
+            floatx16 sc = mma_rows<T, DH, PS>(Ks + kr * row_st<DH>(), qf, lane);
+            const floatx16 dp = mma_rows<T, DH, PS>(Vs + kr * row_st<DH>(), df, lane);
             if (masked) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -756,7 +790,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -l2)) * (dp[e] - D);
-            mma_tr<T, DH, PS>(Ks + kr * DH, sc, g, lane);
+            mma_tr<T, DH, PS>(Ks + kr * row_st<DH>(), sc, g, lane);
         }
     };
     if (nt > 0) {
@@ -765,15 +799,9 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
         __syncthreads();
     }
     for (int t = 0; t < nt; ++t) {
-        const int cur = C::NB == 2 ? t & 1 : 0;
-        if (C::NB == 2 && t + 1 < nt) {
-            __bf16* nx = tiles + (cur ^ 1) * 2 * C::TILE;
-            kv.store(nx, nx + C::TILE, kfs + (cur ^ 1) * C::BK, tid);
-            if (t + 2 < nt) kv.fetch((t + 2) * C::BK, tid);
-        }
-        tile(t, tiles + cur * 2 * C::TILE, kfs + cur * C::BK);
+        tile(t, tiles, kfs);
         __syncthreads();
-        if (C::NB == 1 && t + 1 < nt) {
+        if (t + 1 < nt) {
             kv.store(tiles, tiles + C::TILE, kfs, tid);
             if (t + 2 < nt) kv.fetch((t + 2) * C::BK, tid);
             __syncthreads();
@@ -817,11 +845,10 @@ template <typename T, int DH, int NK, int QS, int QT> struct DkvCfg {
     static constexpr int NTH = 64 * NK * QS, BKEY = 32 * NK, BQ = QT * QS;
     static constexpr int TILE = tile_elems<T, DH, BQ>();
     static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
-    static constexpr int NB = 1;      // a second buffer's addresses cost registers: 675 us against 798
     static constexpr size_t JOIN = (size_t)NK * (QS - 1) * 2 * DH * 32 * sizeof(float);
     static constexpr size_t OUT = (size_t)NK * Out<T, DH>::WAVE * sizeof(T);   // the rows' way out
-    static constexpr size_t BUFS = max3(NB * PAIR, JOIN, OUT);
-    static constexpr size_t LDS = BUFS + NB * 2 * BQ * sizeof(float) + 16;
+    static constexpr size_t BUFS = max3(PAIR, JOIN, OUT);
+    static constexpr size_t LDS = BUFS + 2 * BQ * sizeof(float) + 16;
 };
 
 template <typename T, int DH, int NK, int QS, int QT>
@@ -836,11 +863,16 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
     float* lss = reinterpret_cast<float*>(smem + C::BUFS);   // log-sum-exp and D of each buffer's rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int kwv = wave % NK, qs = wave / NK;
-    int b = xcd_block(gridDim.x);
-    const int kt = b % ktiles; b /= ktiles;
-    const int kvh = b % a.KV, i = b / a.KV;
+    // padded rows past k_len get zeros
+    const Place pl = place_of(a, a.sorted, a.KV * ktiles, [](const Sample& x) { return x.ql; }, [&](const Sample& x) {
+        return ((a.k_off ? x.kl : a.lk) + C::BKEY - 1) / C::BKEY * a.KV;
+    });
+    if (pl.i < 0) return;
+    const int i = pl.i;
     const Sample s = sample_of(a, i);
-    const int kall = a.k_off ? s.kl : a.lk;   // padded rows past k_len get zeros
+    const int kall = a.k_off ? s.kl : a.lk;
+    const int ktn = a.sorted ? (kall + C::BKEY - 1) / C::BKEY : ktiles;
+    const int kt = pl.rest % ktn, kvh = pl.rest / ktn;
     if (kt * C::BKEY >= kall) return;
     const int key = kt * C::BKEY + 32 * kwv + (lane & 31);
     const bool kin = key < kall;
@@ -892,8 +924,8 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
         for (int j = 0; j < QT / 32; ++j) {
             const int qr = qs * QT + 32 * j;
             if (t * C::BQ + qr >= rows) break;
-            floatx16 p = mma_rows<T, DH, St::PS>(Qs + qr * DH, kfr, lane);
-            floatx16 d = mma_rows<T, DH, St::PS>(Ds + qr * DH, vfr, lane);
+            floatx16 p = mma_rows<T, DH, St::PS>(Qs + qr * row_st<DH>(), kfr, lane);
+            floatx16 d = mma_rows<T, DH, St::PS>(Ds + qr * row_st<DH>(), vfr, lane);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float4 lf = *reinterpret_cast<const float4*>(ls + qr + 8 * e + 4 * h);
@@ -907,8 +939,8 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
                     d[4 * e + x] = pe * (d[4 * e + x] - dv4[x]);
                 }
             }
-            mma_tr<T, DH, St::PS>(Ds + qr * DH, p, gv, lane);
-            mma_tr<T, DH, St::PS>(Qs + qr * DH, d, gk, lane);
+            mma_tr<T, DH, St::PS>(Ds + qr * row_st<DH>(), p, gv, lane);
+            mma_tr<T, DH, St::PS>(Qs + qr * row_st<DH>(), d, gk, lane);
         }
     };
     if (nt > 0) {
@@ -918,14 +950,9 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
         __syncthreads();
     }
     for (int t = 0; t < nt; ++t) {
-        const int cur = C::NB == 2 ? t & 1 : 0;
-        if (C::NB == 2 && t + 1 < nt) {
-            store(tiles + (cur ^ 1) * 2 * C::TILE, lss + (cur ^ 1) * 2 * C::BQ);
-            if (t + 2 < nt) fetch(t + 2);
-        }
-        tile(t, tiles + cur * 2 * C::TILE, lss + cur * 2 * C::BQ);
+        tile(t, tiles, lss);
         __syncthreads();
-        if (C::NB == 1 && t + 1 < nt) {
+        if (t + 1 < nt) {
             store(tiles, lss);
             if (t + 2 < nt) fetch(t + 2);
             __syncthreads();
@@ -1066,6 +1093,7 @@ XArgs to_args(const PtcgCrossAttn* d) {
     a.q = d->q; a.k = d->k; a.v = d->v; a.o = d->o;
     a.q_off = d->q_off; a.k_off = d->k_off; a.k_len = d->k_len;
     a.keep = d->keep; a.keep_sn = d->keep_sn;
+    a.sorted = d->n > 1 && d->n <= 64 && (d->q_off || d->k_off || d->k_len);
     return a;
 }
 

@@ -204,29 +204,35 @@ template <typename T, int DH> struct Row {
 
 // LDS rows are ST elements apart and chunk c (8 values) of a row lies at
 // c ^ swz(row).  Both keep the row reads (16 rows' chunk c) and the transposed
-// reads (4 rows' 4 chunks) on 64 different banks.  128 wide: 64 bytes of
+// reads (4 rows' 4 chunks) on 64 different banks.  PAD (128 wide): 64 bytes of
 // padding move 4 successive rows to different quarters of the banks and only
 // the low two bits of c are turned, so that most of an operand's addresses are
-// one register and a constant.
-template <int DH> constexpr int row_st() { return DH == 128 ? 160 : DH; }
-template <int DH> __device__ __forceinline__ int swz(int row) {
-    if constexpr (DH == 64) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
-    else return row >> 2 & 3;
-}
-// element offset of chunk 2 c + h of a row
-template <int DH> __device__ __forceinline__ int chunk_at(int row, int h, int c) {
-    if constexpr (DH == 128) return row * row_st<DH>() + 8 * ((2 * (c & 1) + h) ^ swz<DH>(row)) + 32 * (c >> 1);
-    else return row * DH + (8 * (h ^ swz<DH>(row)) ^ 16 * c);
-}
-// element offset of column group dt (32 columns), chunk ch of it
-template <int DH> __device__ __forceinline__ int group_at(int row, int ch, int dt) {
-    if constexpr (DH == 128) return row * row_st<DH>() + 8 * (ch ^ swz<DH>(row)) + 32 * dt;
-    else return row * DH + (8 * (ch ^ swz<DH>(row)) ^ 32 * dt);
-}
+// one register and a constant (the backward has none to spare); without, a tile
+// of 128 keys and values leaves room for a second workgroup (a token against
+// 50 001 keys: 43 us against 53).
+template <int DH, bool PAD> struct Lds {
+    static_assert(!PAD || DH == 128, "");
+    static constexpr int ST = PAD ? DH + 32 : DH;
+    static __device__ __forceinline__ int swz(int row) {
+        if constexpr (PAD || DH == 32) return row >> 2 & 3;
+        else if constexpr (DH == 64) return (row >> 1 & 1) << 2 | (row >> 2 & 3);
+        else return (row & 3) << 2 | (row >> 2 & 3);
+    }
+    // element offset of chunk 2 c + h of a row
+    static __device__ __forceinline__ int chunk_at(int row, int h, int c) {
+        if constexpr (PAD) return row * ST + 8 * ((2 * (c & 1) + h) ^ swz(row)) + 32 * (c >> 1);
+        else return row * ST + (8 * (h ^ swz(row)) ^ 16 * c);
+    }
+    // element offset of column group dt (32 columns), chunk ch of it
+    static __device__ __forceinline__ int group_at(int row, int ch, int dt) {
+        if constexpr (PAD) return row * ST + 8 * (ch ^ swz(row)) + 32 * dt;
+        else return row * ST + (8 * (ch ^ swz(row)) ^ 32 * dt);
+    }
+};
 
 // S = X Y^T of 32 LDS rows of X (PS elements between its planes) against the
 // lanes' rows
-template <typename T, int DH, int PS>
+template <typename T, int DH, bool PAD, int PS>
 __device__ __forceinline__ floatx16 mma_rows(const __bf16* xs, const Row<T, DH>& y, int lane) {
     floatx16 s;
 #pragma unroll
@@ -235,8 +241,23 @@ __device__ __forceinline__ floatx16 mma_rows(const __bf16* xs, const Row<T, DH>&
     for (int c = 0; c < DH / 16; ++c) {
         bf16x8 a[planes<T>()];
 #pragma unroll
-        for (int p = 0; p < planes<T>(); ++p) a[p] = *reinterpret_cast<const bf16x8*>(xs + p * PS + chunk_at<DH>(lane & 31, lane >> 5, c));
+        for (int p = 0; p < planes<T>(); ++p) a[p] = *reinterpret_cast<const bf16x8*>(xs + p * PS + Lds<DH, PAD>::chunk_at(lane & 31, lane >> 5, c));
         mma(a, y.f[c], s);
+    }
+    return s;
+}
+
+// the same against rows that lie in LDS too (one plane)
+template <int DH, bool PAD>
+__device__ __forceinline__ floatx16 mma_rows_lds(const __bf16* xs, const __bf16* ys, int lane) {
+    floatx16 s;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DH / 16; ++c) {
+        const int at = Lds<DH, PAD>::chunk_at(lane & 31, lane >> 5, c);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(xs + at),
+                                                    *reinterpret_cast<const bf16x8*>(ys + at), s, 0, 0, 0);
     }
     return s;
 }
@@ -245,7 +266,7 @@ __device__ __forceinline__ floatx16 mma_rows(const __bf16* xs, const Row<T, DH>&
 // r stands for row 8 (r / 4) + 4 h + r % 4.  bf16: P is rounded to bf16 for the
 // product (relative 2^-9 each, as the stored operands are); its fp32 values make
 // the softmax's sum.
-template <typename T, int DH, int PS>
+template <typename T, int DH, bool PAD, int PS>
 __device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floatx16 (&c)[DH / 32], int lane) {
     typedef __attribute__((address_space(3))) bf16x4* lds4;
     const int i = lane & 15, r0 = 4 * (lane >> 5) + (i >> 2), ch = 2 * (lane >> 4 & 1) + (i >> 1 & 1);
@@ -261,9 +282,9 @@ __device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floa
             bf16x8 a[planes<T>()];
 #pragma unroll
             for (int pl = 0; pl < planes<T>(); ++pl) {
-                const __bf16* q = xs + pl * PS + 16 * kb * row_st<DH>() + 4 * (i & 1);
-                const bf16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + group_at<DH>(r0, ch, dt)));
-                const bf16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + group_at<DH>(r0 + 8, ch, dt)));
+                const __bf16* q = xs + pl * PS + 16 * kb * Lds<DH, PAD>::ST + 4 * (i & 1);
+                const bf16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + Lds<DH, PAD>::group_at(r0, ch, dt)));
+                const bf16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + Lds<DH, PAD>::group_at(r0 + 8, ch, dt)));
                 a[pl] = bf16x8{u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
             }
             mma(a, b, c[dt]);
@@ -274,8 +295,8 @@ __device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floa
 // A tile of BR rows on its way through registers into LDS: chunks of 8 values,
 // thread t takes chunks t, t + NTH, ...  Loads are issued well before the
 // barrier that publishes them.
-template <typename T, int DH, int BR, int NTH> struct Stage {
-    static constexpr int CPR = DH / 8, NCH = BR * CPR / NTH, RPP = NTH / CPR, PS = BR * row_st<DH>();
+template <typename T, int DH, bool PAD, int BR, int NTH> struct Stage {
+    static constexpr int CPR = DH / 8, NCH = BR * CPR / NTH, RPP = NTH / CPR, PS = BR * Lds<DH, PAD>::ST;
     static_assert(BR * CPR % NTH == 0 && NTH % CPR == 0 && RPP % 16 == 0, "whole chunks per thread, one swizzle");
     Chunk<T> r[NCH];
     // byte offset of the thread's first chunk; chunk i is i * RPP rows on
@@ -301,7 +322,7 @@ template <typename T, int DH, int BR, int NTH> struct Stage {
         r[i].terms(t);
 #pragma unroll
         for (int p = 0; p < planes<T>(); ++p)
-            *reinterpret_cast<pt_uintx4*>(s + p * PS + row * row_st<DH>() + 8 * (tid % CPR ^ swz<DH>(row))) =
+            *reinterpret_cast<pt_uintx4*>(s + p * PS + row * Lds<DH, PAD>::ST + 8 * (tid % CPR ^ Lds<DH, PAD>::swz(row))) =
                 ok ? __builtin_bit_cast(pt_uintx4, t[p]) : pt_uintx4{0, 0, 0, 0};
     }
     __device__ __forceinline__ void store(__bf16* s, int tid) const {
@@ -317,8 +338,8 @@ template <typename T, int DH, int BR, int NTH> struct Stage {
 
 // A tile of keys and values on its way: masked rows enter LDS as zeros, so that
 // what they hold, NaN too, reaches no product; kf holds 0 or -inf per key.
-template <typename T, int DH, int BK, int NTH> struct KvTile {
-    typedef Stage<T, DH, BK, NTH> St;
+template <typename T, int DH, bool PAD, int BK, int NTH> struct KvTile {
+    typedef Stage<T, DH, PAD, BK, NTH> St;
     static_assert(BK <= NTH, "a thread per key flag");
     St k, v;
     float kp[St::NCH], kfr;
@@ -434,7 +455,9 @@ template <typename T, int DH> struct Out {
 
 constexpr size_t max3(size_t a, size_t b, size_t c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
 // elements (bf16) of a tile of BR rows
-template <typename T, int DH, int BR> constexpr int tile_elems() { return planes<T>() * BR * row_st<DH>(); }
+template <typename T, int DH, bool PAD, int BR> constexpr int tile_elems() {
+    return planes<T>() * BR * Lds<DH, PAD>::ST;
+}
 
 // ---------------------------------------------------------------- forward
 // A workgroup owns 32 NW query rows; KS waves share a row block and split each
@@ -443,7 +466,7 @@ template <typename T, int DH, int BR> constexpr int tile_elems() { return planes
 // partial with its maximum and sum for xattn_join_kernel.
 template <typename T, int DH, int NW, int KS, int KT> struct FwdCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
-    static constexpr int TILE = tile_elems<T, DH, BK>();
+    static constexpr int TILE = tile_elems<T, DH, false, BK>();
     // One buffer: what a second one saves in barriers it costs in workgroups a CU
     // holds (8 192 x 64 x 97, 64 wide: 293 us against 333; a token against 50 001
     // keys 39 against 46).
@@ -456,13 +479,18 @@ template <typename T, int DH, int NW, int KS, int KT> struct FwdCfg {
 // Waves a SIMD holds, for the register allocator: two (of 256 registers each)
 // let one wave's softmax run beside the other's products.
 template <typename T, int DH> constexpr int min_waves() { return sizeof(T) == 2 || DH <= 64 ? 2 : 1; }
+// the backward holds two operands' rows; with a tile four times a wave's part
+// (SPLIT waves along it) also on its way, one wave's registers
+template <typename T, int DH, int SPLIT> constexpr int bwd_waves() {
+    return DH * planes<T>() <= 64 || (SPLIT <= 2 && min_waves<T, DH>() == 2) ? 2 : 1;
+}
 
 template <typename T, int DH, int NW, int KS, int KT>
 __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_kernel(const XArgs a,
         const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,
         float* __restrict__ lse, float* __restrict__ part, int qtiles, int nsplit, int split_keys) {
     typedef FwdCfg<T, DH, NW, KS, KT> C;
-    typedef KvTile<T, DH, C::BK, C::NTH> Kv;
+    typedef KvTile<T, DH, false, C::BK, C::NTH> Kv;
     constexpr int PS = Kv::St::PS;
     extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
@@ -518,7 +546,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
         floatx16 sc[KT / 32];
         float mt = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < KT / 32; ++j) sc[j] = mma_rows<T, DH, PS>(Ks + (kw * KT + 32 * j) * row_st<DH>(), qf, lane);
+        for (int j = 0; j < KT / 32; ++j) sc[j] = mma_rows<T, DH, false, PS>(Ks + (kw * KT + 32 * j) * Lds<DH, false>::ST, qf, lane);
         if (masked) {
 #pragma unroll
             for (int j = 0; j < KT / 32; ++j)
@@ -551,7 +579,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
                 sc[j][e] = __builtin_amdgcn_exp2f(fmaf(sc[j][e], a.scale2, -ms));
                 l += sc[j][e];
             }
-            mma_tr<T, DH, PS>(Vs + (kw * KT + 32 * j) * row_st<DH>(), sc[j], o, lane);
+            mma_tr<T, DH, false, PS>(Vs + (kw * KT + 32 * j) * Lds<DH, false>::ST, sc[j], o, lane);
         }
     };
     if (nt > 0) {
@@ -690,7 +718,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(const XArgs a, const fl
 // for the dK / dV kernel, in row order of lse.
 template <typename T, int DH, int NW, int KS, int KT> struct DqCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
-    static constexpr int TILE = tile_elems<T, DH, BK>();
+    static constexpr int TILE = tile_elems<T, DH, DH == 128, BK>();
     static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * DH * 32 * sizeof(float);
     static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);   // the rows' way out
@@ -699,12 +727,12 @@ template <typename T, int DH, int NW, int KS, int KT> struct DqCfg {
 };
 
 template <typename T, int DH, int NW, int KS, int KT>
-__global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_kernel(const XArgs a,
+__global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_dq_kernel(const XArgs a,
         const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ out,
         const float* __restrict__ lse, const T* __restrict__ dout, T* __restrict__ dq,
         float* __restrict__ delta, int qtiles) {
     typedef DqCfg<T, DH, NW, KS, KT> C;
-    typedef KvTile<T, DH, C::BK, C::NTH> Kv;
+    typedef KvTile<T, DH, DH == 128, C::BK, C::NTH> Kv;
     constexpr int PS = Kv::St::PS;
     extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
@@ -778,8 +806,8 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
             const int kr = kw * KT + 32 * j, row0 = t * C::BK + kr;
             if (row0 >= kend) break;
             const bool masked = a.keep || row0 + 32 > kend;
-            floatx16 sc = mma_rows<T, DH, PS>(Ks + kr * row_st<DH>(), qf, lane);
-            const floatx16 dp = mma_rows<T, DH, PS>(Vs + kr * row_st<DH>(), df, lane);
+            floatx16 sc = mma_rows<T, DH, DH == 128, PS>(Ks + kr * Lds<DH, DH == 128>::ST, qf, lane);
+            const floatx16 dp = mma_rows<T, DH, DH == 128, PS>(Vs + kr * Lds<DH, DH == 128>::ST, df, lane);
             if (masked) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -790,7 +818,7 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -l2)) * (dp[e] - D);
-            mma_tr<T, DH, PS>(Ks + kr * row_st<DH>(), sc, g, lane);
+            mma_tr<T, DH, DH == 128, PS>(Ks + kr * Lds<DH, DH == 128>::ST, sc, g, lane);
         }
     };
     if (nt > 0) {
@@ -843,24 +871,28 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_dq_k
 // dV^T += dO^T P and dK^T += Q^T dS read dO and Q transposed from LDS.
 template <typename T, int DH, int NK, int QS, int QT> struct DkvCfg {
     static constexpr int NTH = 64 * NK * QS, BKEY = 32 * NK, BQ = QT * QS;
-    static constexpr int TILE = tile_elems<T, DH, BQ>();
+    static constexpr int TILE = tile_elems<T, DH, DH == 128, BQ>();
     static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
     static constexpr size_t JOIN = (size_t)NK * (QS - 1) * 2 * DH * 32 * sizeof(float);
     static constexpr size_t OUT = (size_t)NK * Out<T, DH>::WAVE * sizeof(T);   // the rows' way out
     static constexpr size_t BUFS = max3(PAIR, JOIN, OUT);
-    static constexpr size_t LDS = BUFS + 2 * BQ * sizeof(float) + 16;
+    // 128 wide in bf16, the values' rows stay in LDS: with them, dK and dV in
+    // registers two waves a SIMD would spill (558 us against 460, 16 packed samples of up to 1 501 x 4 003)
+    static constexpr bool VLDS = sizeof(T) == 2 && DH == 128 && QS == 1;
+    static constexpr size_t VROWS = VLDS ? (size_t)BKEY * Lds<DH, DH == 128>::ST * 2 : 0;
+    static constexpr size_t LDS = BUFS + VROWS + 2 * BQ * sizeof(float) + 16;
 };
 
 template <typename T, int DH, int NK, int QS, int QT>
-__global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_kernel(const XArgs a,
+__global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_dkv_kernel(const XArgs a,
         const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ lse,
         const T* __restrict__ dout, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
         int ktiles) {
     typedef DkvCfg<T, DH, NK, QS, QT> C;
-    typedef Stage<T, DH, C::BQ, C::NTH> St;
+    typedef Stage<T, DH, DH == 128, C::BQ, C::NTH> St;
     extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
-    float* lss = reinterpret_cast<float*>(smem + C::BUFS);   // log-sum-exp and D of each buffer's rows
+    float* lss = reinterpret_cast<float*>(smem + C::BUFS + C::VROWS);   // log-sum-exp and D of each buffer's rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int kwv = wave % NK, qs = wave / NK;
     // padded rows past k_len get zeros
@@ -878,11 +910,19 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
     const bool kin = key < kall;
     const bool kok = key < s.kl && (!a.keep || a.keep[s.keep + key] != 0.f);
 
+    typedef Lds<DH, DH == 128> L;
     Row<T, DH> kfr, vfr;
+    __bf16* Vl = reinterpret_cast<__bf16*>(smem + C::BUFS) + 32 * kwv * L::ST;
     const long ko = s.k + (kin ? (long)key * a.k.sl + (long)kvh * a.k.sh : 0);
     const long vo = s.v + (kin ? (long)key * a.v.sl + (long)kvh * a.v.sh : 0);
     kfr.load(k + ko, kok, a.dh, h);
     vfr.load(v + vo, kok, a.dh, h);
+    if constexpr (C::VLDS) {     // this wave's 32 rows, read by itself alone
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c)
+            *reinterpret_cast<bf16x8*>(Vl + L::chunk_at(lane & 31, h, c)) = vfr.f[c][0];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
     floatx16 gk[DH / 32], gv[DH / 32];
 #pragma unroll
     for (int dt = 0; dt < DH / 32; ++dt)
@@ -924,8 +964,10 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
         for (int j = 0; j < QT / 32; ++j) {
             const int qr = qs * QT + 32 * j;
             if (t * C::BQ + qr >= rows) break;
-            floatx16 p = mma_rows<T, DH, St::PS>(Qs + qr * row_st<DH>(), kfr, lane);
-            floatx16 d = mma_rows<T, DH, St::PS>(Ds + qr * row_st<DH>(), vfr, lane);
+            floatx16 p = mma_rows<T, DH, DH == 128, St::PS>(Qs + qr * Lds<DH, DH == 128>::ST, kfr, lane);
+            floatx16 d;
+            if constexpr (C::VLDS) d = mma_rows_lds<DH, DH == 128>(Ds + qr * L::ST, Vl, lane);
+            else d = mma_rows<T, DH, DH == 128, St::PS>(Ds + qr * L::ST, vfr, lane);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float4 lf = *reinterpret_cast<const float4*>(ls + qr + 8 * e + 4 * h);
@@ -939,8 +981,8 @@ __global__ __launch_bounds__(64 * NK * QS, (min_waves<T, DH>())) void xattn_dkv_
                     d[4 * e + x] = pe * (d[4 * e + x] - dv4[x]);
                 }
             }
-            mma_tr<T, DH, St::PS>(Ds + qr * row_st<DH>(), p, gv, lane);
-            mma_tr<T, DH, St::PS>(Qs + qr * row_st<DH>(), d, gk, lane);
+            mma_tr<T, DH, DH == 128, St::PS>(Ds + qr * Lds<DH, DH == 128>::ST, p, gv, lane);
+            mma_tr<T, DH, DH == 128, St::PS>(Qs + qr * Lds<DH, DH == 128>::ST, d, gk, lane);
         }
     };
     if (nt > 0) {

@@ -730,7 +730,7 @@ template <typename T, int DH, int NW, int KS, int KT>
 __global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_dq_kernel(const XArgs a,
         const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ out,
         const float* __restrict__ lse, const T* __restrict__ dout, T* __restrict__ dq,
-        float* __restrict__ delta, int qtiles) {
+        float* __restrict__ delta, float* __restrict__ part, int qtiles, int nsplit, int split_keys) {
     typedef DqCfg<T, DH, NW, KS, KT> C;
     typedef KvTile<T, DH, DH == 128, C::BK, C::NTH> Kv;
     constexpr int PS = Kv::St::PS;
@@ -740,22 +740,23 @@ __global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_
     int* sh = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int qw = wave % NW, kw = wave / NW;
-    const Place pl = place_of(a, a.sorted, a.KV * qtiles, [](const Sample& x) { return x.kl; },
+    const Place pl = place_of(a, a.sorted && nsplit == 1, a.KV * qtiles * nsplit, [](const Sample& x) { return x.kl; },
                               [&](const Sample& x) { return (x.ql * a.G + C::BQ - 1) / C::BQ * a.KV; });
     if (pl.i < 0) return;
     const int i = pl.i;
     const Sample s = sample_of(a, i);
-    const int qtn = a.sorted ? (s.ql * a.G + C::BQ - 1) / C::BQ : qtiles;
-    const int qt = pl.rest % qtn, kvh = pl.rest / qtn;
+    const int qtn = a.sorted && nsplit == 1 ? (s.ql * a.G + C::BQ - 1) / C::BQ : qtiles;
+    const int qt = pl.rest % qtn, sp = pl.rest / qtn % nsplit, kvh = pl.rest / qtn / nsplit;
     const int rows = s.ql * a.G;
     if (qt * C::BQ >= rows) return;
     const int r = qt * C::BQ + 32 * qw + (lane & 31);
     const bool rok = r < rows;
 
-    int kend = s.kl;
+    const int k0 = sp * split_keys;
+    int kend = min(s.kl, k0 + split_keys);
     Kv kv;
     kv.init(a, s, k, v, kvh, kend, tid);
-    if (kend > 0) kv.fetch(0, tid);
+    if (k0 < kend) kv.fetch(k0, tid);
 
     Row<T, DH> qf, df;
     qf.load(q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
@@ -780,19 +781,19 @@ __global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_
     const float lr = rok ? lse[lrow] : -INFINITY;
     const bool none = lr == -INFINITY;
     const float l2 = none ? INFINITY : lr * LOG2E;
-    if (rok && kw == 0 && h == 0) delta[lrow] = D;
+    if (rok && kw == 0 && h == 0 && sp == 0) delta[lrow] = D;
 
-    if (a.keep && kend > 0) {
-        const int last = last_kept(a.keep + s.keep, 0, kend, C::NTH);
+    if (a.keep && k0 < kend) {
+        const int last = last_kept(a.keep + s.keep, k0, kend, C::NTH);
         if (lane == 0) sh[wave] = last;
         __syncthreads();
-        kend = 0;
+        kend = k0;
 #pragma unroll
         for (int w = 0; w < NW * KS; ++w) kend = max(kend, sh[w]);
         kend = __builtin_amdgcn_readfirstlane(kend);
         kv.kend = kend;
     }
-    const int nt = (kend + C::BK - 1) / C::BK;
+    const int nt = kend > k0 ? (kend - k0 + C::BK - 1) / C::BK : 0;
 
     floatx16 g[DH / 32];
 #pragma unroll
@@ -803,7 +804,7 @@ __global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_
         const __bf16* Vs = Ks + C::TILE;
 #pragma unroll 1
         for (int j = 0; j < KT / 32; ++j) {
-            const int kr = kw * KT + 32 * j, row0 = t * C::BK + kr;
+            const int kr = kw * KT + 32 * j, row0 = k0 + t * C::BK + kr;
             if (row0 >= kend) break;
             const bool masked = a.keep || row0 + 32 > kend;
             floatx16 sc = mma_rows<T, DH, DH == 128, PS>(Ks + kr * Lds<DH, DH == 128>::ST, qf, lane);
@@ -823,7 +824,7 @@ __global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_
     };
     if (nt > 0) {
         kv.store(tiles, tiles + C::TILE, kfs, tid);
-        if (nt > 1) kv.fetch(C::BK, tid);
+        if (nt > 1) kv.fetch(k0 + C::BK, tid);
         __syncthreads();
     }
     for (int t = 0; t < nt; ++t) {
@@ -831,7 +832,7 @@ __global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_
         __syncthreads();
         if (t + 1 < nt) {
             kv.store(tiles, tiles + C::TILE, kfs, tid);
-            if (t + 2 < nt) kv.fetch((t + 2) * C::BK, tid);
+            if (t + 2 < nt) kv.fetch(k0 + (t + 2) * C::BK, tid);
             __syncthreads();
         }
     }
@@ -861,6 +862,10 @@ __global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_
 #pragma unroll
             for (int e = 0; e < 16; ++e) g[dt][e] = 0.f;
     }
+    if (nsplit > 1) {
+        if (rok) store_row<float, DH>(part + ((long)sp * a.n * a.H * a.lq + lrow) * a.dh, g, 1.f, a.dh, h);
+        return;
+    }
     Out<T, DH>::query_rows(a, a.q, dq + s.q, kvh, qt * C::BQ + 32 * qw, rows, g, a.scale,
                            reinterpret_cast<T*>(smem) + qw * Out<T, DH>::WAVE, lane);
 }
@@ -887,7 +892,7 @@ template <typename T, int DH, int NK, int QS, int QT>
 __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_dkv_kernel(const XArgs a,
         const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ lse,
         const T* __restrict__ dout, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
-        int ktiles) {
+        float* __restrict__ part, int ktiles, int nsplit, int split_rows) {
     typedef DkvCfg<T, DH, NK, QS, QT> C;
     typedef Stage<T, DH, DH == 128, C::BQ, C::NTH> St;
     extern __shared__ __align__(256) char smem[];
@@ -896,15 +901,16 @@ __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int kwv = wave % NK, qs = wave / NK;
     // padded rows past k_len get zeros
-    const Place pl = place_of(a, a.sorted, a.KV * ktiles, [](const Sample& x) { return x.ql; }, [&](const Sample& x) {
-        return ((a.k_off ? x.kl : a.lk) + C::BKEY - 1) / C::BKEY * a.KV;
-    });
+    const Place pl = place_of(a, a.sorted && nsplit == 1, a.KV * ktiles * nsplit,
+                              [](const Sample& x) { return x.ql; }, [&](const Sample& x) {
+                                  return ((a.k_off ? x.kl : a.lk) + C::BKEY - 1) / C::BKEY * a.KV;
+                              });
     if (pl.i < 0) return;
     const int i = pl.i;
     const Sample s = sample_of(a, i);
     const int kall = a.k_off ? s.kl : a.lk;
-    const int ktn = a.sorted ? (kall + C::BKEY - 1) / C::BKEY : ktiles;
-    const int kt = pl.rest % ktn, kvh = pl.rest / ktn;
+    const int ktn = a.sorted && nsplit == 1 ? (kall + C::BKEY - 1) / C::BKEY : ktiles;
+    const int kt = pl.rest % ktn, sp = pl.rest / ktn % nsplit, kvh = pl.rest / ktn / nsplit;
     if (kt * C::BKEY >= kall) return;
     const int key = kt * C::BKEY + 32 * kwv + (lane & 31);
     const bool kin = key < kall;
@@ -929,13 +935,15 @@ __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_
 #pragma unroll
         for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
 
-    const int rows = __syncthreads_or(kok) ? s.ql * a.G : 0;   // a block that keeps no key has no gradient
-    const int nt = (rows + C::BQ - 1) / C::BQ;
+    // rows [r0, rows) of this split; a block that keeps no key has no gradient
+    const int r0 = sp * split_rows;
+    const int rows = __syncthreads_or(kok) ? min(s.ql * a.G, r0 + split_rows) : 0;
+    const int nt = rows > r0 ? (rows - r0 + C::BQ - 1) / C::BQ : 0;
     St qs_, ds_;
     float lr = 0.f, dr = 0.f;
     int rown = 0;     // rows of the fetched tile
     auto fetch = [&](int t) {
-        const int row0 = t * C::BQ;
+        const int row0 = r0 + t * C::BQ;
         rown = rows - row0;
         qs_.load_q(a, a.q, q + s.q, kvh, row0, rows, tid);
         ds_.load_q(a, a.o, dout + s.o, kvh, row0, rows, tid);
@@ -963,7 +971,7 @@ __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_
 #pragma unroll 1
         for (int j = 0; j < QT / 32; ++j) {
             const int qr = qs * QT + 32 * j;
-            if (t * C::BQ + qr >= rows) break;
+            if (r0 + t * C::BQ + qr >= rows) break;
             floatx16 p = mma_rows<T, DH, DH == 128, St::PS>(Qs + qr * Lds<DH, DH == 128>::ST, kfr, lane);
             floatx16 d;
             if constexpr (C::VLDS) d = mma_rows_lds<DH, DH == 128>(Ds + qr * L::ST, Vl, lane);
@@ -1033,10 +1041,62 @@ __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_
 #pragma unroll
             for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
     }
+    if (nsplit > 1) {
+        const long R = (long)a.n * a.KV * a.lk, row = ((long)i * a.KV + kvh) * a.lk + key;
+        if (kin) {
+            store_row<float, DH>(part + ((long)sp * 2 * R + row) * a.dh, gk, 1.f, a.dh, h);
+            store_row<float, DH>(part + ((long)sp * 2 * R + R + row) * a.dh, gv, 1.f, a.dh, h);
+        }
+        return;
+    }
     const int key0 = kt * C::BKEY + 32 * kwv;
     T* ws = reinterpret_cast<T*>(smem) + kwv * Out<T, DH>::WAVE;
     Out<T, DH>::key_rows(dk + s.k + (long)kvh * a.k.sh, a.k.sl, key0, kall, a.dh, gk, a.scale, ws, lane);
     Out<T, DH>::key_rows(dv + s.v + (long)kvh * a.v.sh, a.v.sl, key0, kall, a.dh, gv, 1.f, ws, lane);
+}
+
+// adds the splits' parts of dq, or of dk and dv, in split order: 4 columns a thread
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_sum_q_kernel(const XArgs a, const float* __restrict__ part,
+        T* __restrict__ dq, int nsplit) {
+    const int c4 = a.dh / 4;
+    const long R = (long)a.n * a.H * a.lq, at = (long)blockIdx.x * 256 + threadIdx.x, row = at / c4;
+    if (row >= R) return;
+    const int c = (int)(at - row * c4) * 4;
+    const int qi = (int)(row % a.lq), head = (int)(row / a.lq % a.H), i = (int)(row / a.lq / a.H);
+    const Sample s = sample_of(a, i);
+    if (qi >= s.ql) return;
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int p = 0; p < nsplit; ++p) {
+        const float4 x = *reinterpret_cast<const float4*>(part + (p * R + row) * a.dh + c);
+        g.x += x.x; g.y += x.y; g.z += x.z; g.w += x.w;
+    }
+    st4(dq + s.q + (long)qi * a.q.sl + (long)head * a.q.sh + c, g.x * a.scale, g.y * a.scale, g.z * a.scale,
+        g.w * a.scale);
+}
+template <typename T>
+__global__ __launch_bounds__(256) void xattn_sum_kv_kernel(const XArgs a, const float* __restrict__ part,
+        T* __restrict__ dk, T* __restrict__ dv, int nsplit) {
+    const int c4 = a.dh / 4;
+    const long R = (long)a.n * a.KV * a.lk, at = (long)blockIdx.x * 256 + threadIdx.x, both = at / c4;
+    if (both >= 2 * R) return;
+    const bool isv = both >= R;
+    const long row = isv ? both - R : both;
+    const int c = (int)(at - both * c4) * 4;
+    const int key = (int)(row % a.lk), kvh = (int)(row / a.lk % a.KV), i = (int)(row / a.lk / a.KV);
+    const Sample s = sample_of(a, i);
+    if (key >= (a.k_off ? s.kl : a.lk)) return;
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int p = 0; p < nsplit; ++p) {
+        const float4 x = *reinterpret_cast<const float4*>(part + (2 * p * R + both) * a.dh + c);
+        g.x += x.x; g.y += x.y; g.z += x.z; g.w += x.w;
+    }
+    if (isv) st4(dv + s.v + (long)key * a.v.sl + (long)kvh * a.v.sh + c, g.x, g.y, g.z, g.w);
+    else
+        st4(dk + s.k + (long)key * a.k.sl + (long)kvh * a.k.sh + c, g.x * a.scale, g.y * a.scale, g.z * a.scale,
+            g.w * a.scale);
 }
 
 // ------------------------------------------------------------------- host
@@ -1053,29 +1113,46 @@ int cu_count() {
 // planes) fits LDS up to 64 wide.
 int waves_for(long rows, bool bf16, int dh) { return rows <= 32 && (bf16 || dh <= 64) ? 1 : rows <= 64 ? 2 : 4; }
 
-struct Plan { int nw, qtiles, nsplit, split_keys; };
+// Splits of a long axis (keys; rows for dk and dv), where the other axis' work-
+// groups leave CUs idle: `per_cu` workgroups a CU, at least two tiles each, and
+// only from so many tiles on that the joining launch costs less than it saves
+// (an fp32 tile takes twice a bf16 one's time).
+struct Split { int n, len; };
+Split split_of(long blocks, int len, int tile, int per_cu, bool bf16) {
+    Split p = {1, len > 0 ? len : 1};
+    const int cu = cu_count(), tiles = pt_cdiv(len, tile);
+    if (blocks >= cu || blocks <= 0 || tiles < (bf16 ? 6 : 4)) return p;
+    const long want = (per_cu * (long)cu + blocks - 1) / blocks;
+    const int per = pt_cdiv(tiles, want < tiles / 2 ? want : tiles / 2);
+    p.len = per * tile;
+    p.n = pt_cdiv(len, p.len);
+    return p;
+}
 
-// Key splits (forward), where the rows' workgroups leave CUs idle: four
-// workgroups a CU (samples differ in length; the shorter ones' last splits have
-// nothing to do), at least two tiles of keys in each.
+// The forward takes four workgroups a CU: samples differ in length, and the
+// shorter ones' last splits have nothing to do.
+struct Plan { int nw, qtiles; Split s; };
 Plan fwd_plan(const PtcgCrossAttn* d) {
     Plan p;
     const long rows = (long)d->lq * (d->heads / d->kv_heads);
     p.nw = waves_for(rows, d->bf16, d->dh);
     p.qtiles = pt_cdiv(rows, 32 * p.nw);
-    const int bk = p.nw == 1 ? 128 : 64;
-    const long blocks = (long)d->n * d->kv_heads * p.qtiles;
-    const int cu = cu_count();
-    p.nsplit = 1;
-    p.split_keys = d->lk;
-    if (blocks < cu && d->lk >= 8 * bk) {
-        const long want = (4 * cu + blocks - 1) / blocks, most = d->lk / (2 * bk);
-        const int tiles = pt_cdiv(d->lk, bk);
-        const int sp = (int)(want < most ? want : most);
-        const int per = pt_cdiv(tiles, sp);
-        p.split_keys = per * bk;
-        p.nsplit = pt_cdiv(d->lk, p.split_keys);
-    }
+    p.s = split_of((long)d->n * d->kv_heads * p.qtiles, d->lk, p.nw == 1 ? 128 : 64, 4, d->bf16);
+    return p;
+}
+// backward: keys split for dq, rows for dk and dv
+struct BwdPlan { int nw, nk; Split q, k; int64_t delta, part; };   // workspace floats
+BwdPlan bwd_plan(const PtcgCrossAttn* d) {
+    BwdPlan p;
+    const long G = d->heads / d->kv_heads, rows = d->lq * G, pairs = (long)d->n * d->kv_heads;
+    p.nw = waves_for(rows, d->bf16, d->dh);
+    p.nk = waves_for(d->lk, d->bf16, d->dh);
+    p.q = split_of(pairs * pt_cdiv(rows, 32 * p.nw), d->lk, p.nw == 1 ? 128 : 64, 2, d->bf16);
+    p.k = split_of(pairs * pt_cdiv(d->lk, 32 * p.nk), (int)rows, p.nk == 1 ? 128 : 64, 2, d->bf16);
+    const int64_t R = (int64_t)d->n * d->heads * d->lq, RK = pairs * d->lk;
+    p.delta = (R + 3) / 4 * 4;
+    const int64_t q = p.q.n > 1 ? p.q.n * R * d->dh : 0, k = p.k.n > 1 ? p.k.n * 2 * RK * d->dh : 0;
+    p.part = q > k ? q : k;      // dq's are added up before dk's and dv's are made
     return p;
 }
 
@@ -1153,13 +1230,13 @@ int launch_fwd(const XArgs& a, const Plan& p, const void* q, const void* k, cons
     typedef FwdCfg<T, DH, NW, KS, KT> C;
     auto kern = xattn_fwd_kernel<T, DH, NW, KS, KT>;
     PT_TRY(lds_attr(kern, C::LDS));
-    hipLaunchKernelGGL(kern, dim3((unsigned)(a.n * a.KV * (long)p.qtiles * p.nsplit)), dim3(C::NTH), C::LDS, s, a,
+    hipLaunchKernelGGL(kern, dim3((unsigned)(a.n * a.KV * (long)p.qtiles * p.s.n)), dim3(C::NTH), C::LDS, s, a,
                        static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                       static_cast<T*>(out), lse, part, p.qtiles, p.nsplit, p.split_keys);
+                       static_cast<T*>(out), lse, part, p.qtiles, p.s.n, p.s.len);
     PT_LAUNCH_CHECK();
-    if (p.nsplit > 1) {
+    if (p.s.n > 1) {
         hipLaunchKernelGGL(xattn_join_kernel<T>, dim3((unsigned)((long)a.n * a.H * a.lq)), dim3(256), 0, s, a, part,
-                           static_cast<T*>(out), lse, p.nsplit);
+                           static_cast<T*>(out), lse, p.s.n);
         PT_LAUNCH_CHECK();
     }
     return PTCG_OK;
@@ -1175,61 +1252,77 @@ int fwd_nw(const XArgs& a, const Plan& p, const void* q, const void* k, const vo
 }
 
 template <typename T, int DH, int NW, int KS, int KT>
-int launch_dq(const XArgs& a, const void* q, const void* k, const void* v, const void* out, const float* lse,
-              const void* dout, void* dq, float* delta, hipStream_t s) {
+int launch_dq(const XArgs& a, const BwdPlan& p, const void* q, const void* k, const void* v, const void* out,
+              const float* lse, const void* dout, void* dq, float* ws, hipStream_t s) {
     typedef DqCfg<T, DH, NW, KS, KT> C;
     auto kern = xattn_dq_kernel<T, DH, NW, KS, KT>;
     PT_TRY(lds_attr(kern, C::LDS));
     const int qtiles = pt_cdiv((long)a.lq * a.G, C::BQ);
-    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * qtiles)), dim3(C::NTH), C::LDS, s, a,
+    float* part = ws + p.delta;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * qtiles * p.q.n)), dim3(C::NTH), C::LDS, s, a,
                        static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                       static_cast<const T*>(out), lse, static_cast<const T*>(dout), static_cast<T*>(dq), delta,
-                       qtiles);
+                       static_cast<const T*>(out), lse, static_cast<const T*>(dout), static_cast<T*>(dq), ws, part,
+                       qtiles, p.q.n, p.q.len);
     PT_LAUNCH_CHECK();
+    if (p.q.n > 1) {
+        hipLaunchKernelGGL(xattn_sum_q_kernel<T>, dim3(pt_cdiv((long)a.n * a.H * a.lq * (a.dh / 4), 256)), dim3(256),
+                           0, s, a, part, static_cast<T*>(dq), p.q.n);
+        PT_LAUNCH_CHECK();
+    }
     return PTCG_OK;
 }
 
 template <typename T, int DH, int NK, int QS, int QT>
-int launch_dkv(const XArgs& a, const void* q, const void* k, const void* v, const float* lse, const void* dout,
-               const float* delta, void* dk, void* dv, hipStream_t s) {
+int launch_dkv(const XArgs& a, const BwdPlan& p, const void* q, const void* k, const void* v, const float* lse,
+               const void* dout, void* dk, void* dv, float* ws, hipStream_t s) {
     typedef DkvCfg<T, DH, NK, QS, QT> C;
     auto kern = xattn_dkv_kernel<T, DH, NK, QS, QT>;
     PT_TRY(lds_attr(kern, C::LDS));
     const int ktiles = pt_cdiv(a.lk, C::BKEY);
-    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * ktiles)), dim3(C::NTH), C::LDS, s, a,
+    float* part = ws + p.delta;
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * ktiles * p.k.n)), dim3(C::NTH), C::LDS, s, a,
                        static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), lse,
-                       static_cast<const T*>(dout), delta, static_cast<T*>(dk), static_cast<T*>(dv), ktiles);
+                       static_cast<const T*>(dout), ws, static_cast<T*>(dk), static_cast<T*>(dv), part, ktiles,
+                       p.k.n, p.k.len);
     PT_LAUNCH_CHECK();
+    if (p.k.n > 1) {
+        hipLaunchKernelGGL(xattn_sum_kv_kernel<T>, dim3(pt_cdiv(2L * a.n * a.KV * a.lk * (a.dh / 4), 256)), dim3(256),
+                           0, s, a, part, static_cast<T*>(dk), static_cast<T*>(dv), p.k.n);
+        PT_LAUNCH_CHECK();
+    }
     return PTCG_OK;
 }
 
 template <typename T, int DH>
-int bwd(const XArgs& a, const void* q, const void* k, const void* v, const void* out, const float* lse,
-        const void* dout, void* dq, void* dk, void* dv, float* delta, hipStream_t s) {
-    constexpr bool ONE = sizeof(T) == 2 || DH <= 64;
+int bwd(const XArgs& a, const BwdPlan& p, const void* q, const void* k, const void* v, const void* out,
+        const float* lse, const void* dout, void* dq, void* dk, void* dv, float* ws, hipStream_t s) {
+    constexpr bool ONE = sizeof(T) == 2 || DH <= 64;      // waves_for
+    // the rows of a step of dk / dv: 32 where the registers hold no more on their way
+    constexpr int QT = DH * planes<T>() >= 128 ? 32 : 64;
     if (a.lq > 0) {
-        const int nw = waves_for((long)a.lq * a.G, sizeof(T) == 2, DH);
         if constexpr (ONE)
-            if (nw == 1) PT_TRY((launch_dq<T, DH, 1, 4, 32>(a, q, k, v, out, lse, dout, dq, delta, s)));
-        if (nw == 2) PT_TRY((launch_dq<T, DH, 2, 2, 32>(a, q, k, v, out, lse, dout, dq, delta, s)));
-        if (nw == 4) PT_TRY((launch_dq<T, DH, 4, 1, 64>(a, q, k, v, out, lse, dout, dq, delta, s)));
+            if (p.nw == 1) PT_TRY((launch_dq<T, DH, 1, 4, 32>(a, p, q, k, v, out, lse, dout, dq, ws, s)));
+        if (p.nw == 2) PT_TRY((launch_dq<T, DH, 2, 2, 32>(a, p, q, k, v, out, lse, dout, dq, ws, s)));
+        if (p.nw == 4) PT_TRY((launch_dq<T, DH, 4, 1, 64>(a, p, q, k, v, out, lse, dout, dq, ws, s)));
     }
     if (a.lk > 0) {
-        const int nk = waves_for(a.lk, sizeof(T) == 2, DH);
         if constexpr (ONE)
-            if (nk == 1) return launch_dkv<T, DH, 1, 4, 32>(a, q, k, v, lse, dout, delta, dk, dv, s);
-        if (nk == 2) return launch_dkv<T, DH, 2, 2, 32>(a, q, k, v, lse, dout, delta, dk, dv, s);
-        return launch_dkv<T, DH, 4, 1, DH == 128 || (DH == 64 && sizeof(T) == 4) ? 32 : 64>(a, q, k, v, lse, dout, delta, dk, dv, s);
+            if (p.nk == 1) return launch_dkv<T, DH, 1, 4, 32>(a, p, q, k, v, lse, dout, dk, dv, ws, s);
+        if (p.nk == 2) return launch_dkv<T, DH, 2, 2, 32>(a, p, q, k, v, lse, dout, dk, dv, ws, s);
+        return launch_dkv<T, DH, 4, 1, QT>(a, p, q, k, v, lse, dout, dk, dv, ws, s);
     }
     return PTCG_OK;
 }
 
 int64_t ws_need(const PtcgCrossAttn* d, int backward) {
     const int64_t R = (int64_t)d->n * d->heads * d->lq;
-    if (backward) return R * 4;
+    if (backward) {
+        const BwdPlan p = bwd_plan(d);
+        return (p.delta + p.part) * 4;
+    }
     if (R == 0) return 0;
     const Plan p = fwd_plan(d);
-    return p.nsplit > 1 ? (int64_t)p.nsplit * R * (d->dh + 2) * 4 : 0;
+    return p.s.n > 1 ? (int64_t)p.s.n * R * (d->dh + 2) * 4 : 0;
 }
 
 }  // namespace
@@ -1285,13 +1378,14 @@ extern "C" int ptcg_kernel_cross_attention_bwd(const PtcgCrossAttn* d, const voi
                "cross_attention_bwd: workspace of %lld bytes, need %lld (16 B aligned)", (long long)workspace_bytes,
                (long long)need);
     const XArgs a = to_args(d);
-    float* delta = static_cast<float*>(workspace);
+    const BwdPlan p = bwd_plan(d);
+    float* ws = static_cast<float*>(workspace);
     const hipStream_t s = (hipStream_t)stream;
     if (d->bf16)
-        return d->dh <= 32   ? bwd<__bf16, 32>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s)
-               : d->dh <= 64 ? bwd<__bf16, 64>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s)
-                             : bwd<__bf16, 128>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s);
-    return d->dh <= 32   ? bwd<float, 32>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s)
-           : d->dh <= 64 ? bwd<float, 64>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s)
-                         : bwd<float, 128>(a, q, k, v, out, lse, dout, dq, dk, dv, delta, s);
+        return d->dh <= 32   ? bwd<__bf16, 32>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
+               : d->dh <= 64 ? bwd<__bf16, 64>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
+                             : bwd<__bf16, 128>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s);
+    return d->dh <= 32   ? bwd<float, 32>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
+           : d->dh <= 64 ? bwd<float, 64>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
+                         : bwd<float, 128>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s);
 }

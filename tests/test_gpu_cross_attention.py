@@ -258,6 +258,31 @@ def test_few_rows_against_many_keys(lq, lk, H, KV, dh, mask, bf16, cuda):
     op.check()
 
 
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("lq,lk,H,KV,dh,order,packed", [
+    (700, 40, 4, 2, 64, "lhd", False), (600, 130, 6, 2, 128, "kv", True), (20, 900, 8, 2, 32, "hld", False),
+    (513, 520, 2, 1, 40, "lhd", True), (40, 1200, 4, 4, 96, "kv", True)])
+def test_backward_split_over_a_long_axis(lq, lk, H, KV, dh, order, packed, bf16, cuda):
+    """Few workgroups along one axis: keys (for dq) or rows (for dk, dv) are split
+    and added; masks and lengths cut through the splits."""
+    if packed:
+        op = Op(3, lq, lk, H, KV, dh, bf16, q_len=[lq, 0, lq // 3], k_off_len=[lk // 2, 7, lk], order=order, slack=3)
+    else:
+        op = Op(2, lq, lk, H, KV, dh, bf16, order=order, k_len=[lk, lk // 3])
+        op.keep = _holes(2, lk, 2)
+        op.a.keep = op.keep.data_ptr()
+    n, R = op.n, op.n * H * lq
+    assert native.lib().ptcg_kernel_cross_attention_ws_bytes(ctypes.byref(op.a), 1) > 4 * R + 16    # the split form
+    op.fwd()
+    op.bwd()
+    op.check()
+    a = [x.clone() for x in (op.dq, op.dk, op.dv)]
+    op.ws.fill_(0xff)
+    op.bwd()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(a, (op.dq, op.dk, op.dv)))
+
+
 def test_broadcast_keys_and_queries_in_the_forward(cuda):
     op = Op(6, 10, 50, 4, 2, 32, 0, share_kv=True)
     op.fwd()

@@ -498,7 +498,7 @@ int cu_count() {
 // step) gains 14% of the products and costs another 33 MB of partials: from
 // rows * in * out = 4e10 on (65 539 x 4 096 x 1 024: 537 us against 625;
 // 20 000 x 1 024 x 1 024: 70 against 63).  In fp32 its accumulators leave too
-// few registers for the three terms.  At least 8 steps a split.
+// few registers for the three terms.  At least 4 steps a split.
 struct DwPlan { int big_m, big_n, tm, tn, splits, chunk; long pstride; };
 DwPlan dw_plan(int rows, int k, int n, int bf16) {
     DwPlan p;
@@ -508,7 +508,7 @@ DwPlan dw_plan(int rows, int k, int n, int bf16) {
     p.tn = pt_cdiv(k, p.big_n ? 256 : 128);
     const long tiles = (long)p.tm * p.tn;
     long sp = cu_count() / tiles;
-    const long most = rows / (8 * TK);
+    const long most = rows / (4 * TK);
     if (sp > most) sp = most;
     if (sp < 1) sp = 1;
     p.chunk = rows > 0 ? pt_cdiv(pt_cdiv(rows, sp), TK) * TK : TK;

@@ -17,10 +17,12 @@
 // vocabulary fits, else digits of up to 9 bits; per digit a count per
 // workgroup, a scan over the workgroups, and a placement whose ranks within a
 // wave come from ballots.
+// Up to RANK_ROWS tokens each token counts the tokens before it instead (one
+// launch for the three of every digit).
 // Runs longer than CHUNK tokens (frequent ids) are added in CHUNK-aligned
 // pieces of the sorted list by groups of lanes of their own and folded in order,
 // so one frequent id does not hold a single group for its whole run.
-#include "common.h"
+#include "model.h"
 #include "../../include/ptcg_amd_kernels.h"
 
 namespace {
@@ -31,6 +33,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 constexpr int CHUNK = 64;        // tokens a group adds on its own
 constexpr int MAXB = 1024;        // workgroups of a sort pass (tiles grow past it)
 constexpr int BITS1 = 11, BITS2 = 9;
+constexpr int RANK_ROWS = 4096;  // 16 KB of keys in LDS; 4 096 compares a token
 
 // VW values of a row, as floats
 template <int VW> struct Vals { float v[VW]; };
@@ -305,7 +308,52 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
     }
 }
 
-// sorts of several digits: first sorted position of each id, by binary search
+// A token's place is the number of tokens with a smaller id, or with its id and
+// a smaller position; padding goes last.  A workgroup places 64 tokens, each of
+// its waves counting over a quarter of all of them.
+__global__ __launch_bounds__(256) void sort_rank_kernel(const int* __restrict__ ids, int rows, int vocab,
+        int* __restrict__ out_keys, int* __restrict__ out_pos, int* __restrict__ live) {
+    __shared__ __align__(16) unsigned keys[RANK_ROWS];
+    __shared__ int part[4][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, t0 = blockIdx.x * 64, t = t0 + lane;
+    const int all = (rows + 15) / 16 * 16;
+    constexpr unsigned PAD = 0x80000000u, NONE = 0xffffffffu;   // above every id; past the end
+    int kept = 0;
+    for (int j = tid; j < all; j += 256) {
+        const int id = j < rows ? ids[j] : 0;
+        const bool ok = j < rows && (unsigned)id < (unsigned)vocab;
+        keys[j] = ok ? (unsigned)id : j < rows ? PAD : NONE;
+        kept += ok;
+    }
+    if (blockIdx.x == 0) {
+        for (int o = 32; o > 0; o >>= 1) kept += __shfl_xor(kept, o, 64);
+        if (lane == 0) part[wave][0] = kept;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0 && tid == 0) *live = part[0][0] + part[1][0] + part[2][0] + part[3][0];
+    const unsigned mine = keys[min(t, rows - 1)];
+    const int j0 = wave * (all / 4), j1 = j0 + all / 4;
+    int n = 0;
+    for (int j = j0; j < j1; j += 4) {
+        const uint4 k = *reinterpret_cast<const uint4*>(keys + j);
+        // tokens before this workgroup's win ties, those after it lose them
+        const unsigned m = j < t0 ? mine + 1 : mine;
+        n += (k.x < m) + (k.y < m) + (k.z < m) + (k.w < m);
+        if (j >= t0 && j < t0 + 64)
+            n += (k.x == mine && j < t) + (k.y == mine && j + 1 < t) + (k.z == mine && j + 2 < t) +
+                 (k.w == mine && j + 3 < t);
+    }
+    __syncthreads();
+    part[wave][lane] = n;
+    __syncthreads();
+    if (wave > 0 || t >= rows) return;
+    const int at = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+    out_keys[at] = (int)mine;
+    out_pos[at] = t;
+}
+
+// first sorted position of each id, by binary search (a sort of one digit leaves
+// them itself)
 __global__ __launch_bounds__(256) void sort_starts_kernel(const int* __restrict__ keys,
         const int* __restrict__ live, int vocab, int* __restrict__ starts) {
     const int v = blockIdx.x * 256 + threadIdx.x;
@@ -457,16 +505,20 @@ int bits_for(int vocab) {
     return b;
 }
 
-struct SortPlan { int passes, bits, tile, nb, bins; };
+struct SortPlan { int passes, bits, tile, nb, bins; };   // passes 0: by rank
 SortPlan sort_plan(long rows, int vocab) {
     SortPlan p;
     const int nb = bits_for(vocab);
     p.passes = nb <= BITS1 ? 1 : (nb + BITS2 - 1) / BITS2;
+    if (rows <= RANK_ROWS) {
+        p = SortPlan{0, 0, 0, 0, 0};
+        return p;
+    }
     p.bits = (nb + p.passes - 1) / p.passes;
     p.bins = 1 << p.bits;
     p.tile = 1024;
     if (rows > (long)MAXB * 1024) p.tile = pt_cdiv(pt_cdiv(rows, MAXB), 1024) * 1024;
-    p.nb = rows > 0 ? pt_cdiv(rows, p.tile) : 1;
+    p.nb = pt_cdiv(rows, p.tile);
     return p;
 }
 
@@ -484,7 +536,7 @@ Ws ws_layout(long rows, int vocab, int d) {
     w.cnt = take((long)p.bins * p.nb);
     w.tot = take(p.bins);
     w.starts = take((long)vocab + 1);
-    w.live = take(1);
+    w.live = take(4);
     w.part = take(rows > CHUNK ? (long)pt_cdiv(rows, CHUNK) * 2 * d : 0);
     w.total = at;
     return w;
@@ -599,6 +651,12 @@ extern "C" int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const
     const hipStream_t s = (hipStream_t)stream;
     int* ws = static_cast<int*>(workspace);
     const SortPlan p = sort_plan(rows, vocab);
+    if (p.passes == 0 && rows > 0) {
+        hipLaunchKernelGGL(sort_rank_kernel, dim3(pt_cdiv(rows, 64)), dim3(256), 0, s, ids, (int)rows, vocab,
+                           ws + w.keys, ws + w.pos, ws + w.live);
+        PT_LAUNCH_CHECK();
+    }
+    if (rows == 0) PT_TRY(pt_fill_zero(reinterpret_cast<float*>(ws + w.live), 4, s));
     SortPass a{};
     a.keys = ids; a.pos = nullptr; a.n_dev = nullptr;
     a.n = (int)rows; a.vocab = vocab; a.bits = p.bits; a.tile = p.tile; a.nb = p.nb;
@@ -619,7 +677,7 @@ extern "C" int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const
         PT_LAUNCH_CHECK();
         a.keys = a.out_keys; a.pos = a.out_pos; a.n_dev = ws + w.live;
     }
-    if (p.passes > 1) {
+    if (p.passes != 1) {
         hipLaunchKernelGGL(sort_starts_kernel, dim3(pt_cdiv((long)vocab + 1, 256)), dim3(256), 0, s, ws + w.keys,
                            ws + w.live, vocab, ws + w.starts);
         PT_LAUNCH_CHECK();

@@ -73,7 +73,8 @@ CASES = [
     (1000, 50, 77, "uniform"), (1024, 2048, 256, "skewed"), (1025, 2049, 256, "skewed"), (5000, 300, 300, "skewed"),
     (3000, 100003, 40, "uniform"), (20000, 2048, 128, "one"), (30011, 9000, 136, "skewed"), (4096, 16, 1024, "uniform"),
     (777, 513, 1500, "ascending"), (5003, 1 << 20, 12, "skewed"), (270000, 700, 16, "skewed"),
-    (300000, 5000, 8, "uniform"),
+    (300000, 5000, 8, "uniform"), (4095, 3000, 20, "skewed"), (4097, 3000, 20, "skewed"), (63, 64, 4, "ascending"),
+    (2000, (1 << 31) - 1 >> 9, 4, "uniform"),
 ]
 
 

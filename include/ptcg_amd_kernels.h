@@ -282,9 +282,8 @@ int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const void* dout
  * stride lds >= ceil(d / 32)): x8 = code 2^(byte - 127), the scale the least
  * power of two that keeps the group's largest value within 448 of it
  * (bytes 17 .. 246), codes rounded to nearest even; values past 448 2^119
- * saturate, NaN and infinities are kept as NaN.  Any d and strides; 8-value
- * pieces move as vectors where d and the code stride are multiples of 8 and
- * rows are 16 B (codes 8 B) aligned.
+ * saturate, NaN and infinities are kept as NaN.  Any d, strides and
+ * alignment (of the element type).
  * pack: x (fp32, or bf16 where bf16 = 1) to codes and scales; unpack: x8 back.
  * gelu_bwd: the backward of a GELU layer from its pre-activation z8: dz = dy
  * gelu'(z8) and, where act is given, act = gelu(z8) (the next layer's input);

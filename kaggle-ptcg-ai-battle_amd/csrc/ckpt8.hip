@@ -23,57 +23,68 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 constexpr int GRP = 32;
 
-// 8 consecutive values of a row; VEC: 16 B (fp32: 2 x 16 B) aligned and whole,
-// else single loads of those below `left`
-template <bool VEC> __device__ __forceinline__ void ld8(const float* p, int left, float (&x)[8]) {
-    if constexpr (VEC) {
-        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+// 8 consecutive values of a row, as one access of any alignment (the hardware
+// takes dword and wider accesses at any byte), or, past `left` of a row's last
+// piece (TAIL), singly
+template <typename T, int N> struct Packed { T v[N]; } __attribute__((packed));
+template <bool TAIL> __device__ __forceinline__ void ld8(const float* p, int left, float (&x)[8]) {
+    if (!TAIL || left >= 8) {
+        const Packed<float, 8> a = *reinterpret_cast<const Packed<float, 8>*>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = a.v[i];
     } else
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = i < left ? p[i] : 0.f;
 }
-template <bool VEC> __device__ __forceinline__ void ld8(const __bf16* p, int left, float (&x)[8]) {
-    if constexpr (VEC) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
+template <bool TAIL> __device__ __forceinline__ void ld8(const __bf16* p, int left, float (&x)[8]) {
+    if (!TAIL || left >= 8) {
+        const Packed<unsigned, 4> a = *reinterpret_cast<const Packed<unsigned, 4>*>(p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (float)a[i];
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(i % 2 ? a.v[i / 2] & 0xffff0000u : a.v[i / 2] << 16);
     } else
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = i < left ? (float)p[i] : 0.f;
 }
-template <bool VEC> __device__ __forceinline__ void st8(float* p, int left, const float (&x)[8]) {
-    if constexpr (VEC) {
-        *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(p + 4) = make_float4(x[4], x[5], x[6], x[7]);
+template <bool TAIL> __device__ __forceinline__ void st8(float* p, int left, const float (&x)[8]) {
+    if (!TAIL || left >= 8) {
+        Packed<float, 8> a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a.v[i] = x[i];
+        *reinterpret_cast<Packed<float, 8>*>(p) = a;
     } else
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < left) p[i] = x[i];
 }
-template <bool VEC> __device__ __forceinline__ void st8(__bf16* p, int left, const float (&x)[8]) {
-    if constexpr (VEC) {
-        bf16x8 a;
+template <bool TAIL> __device__ __forceinline__ void st8(__bf16* p, int left, const float (&x)[8]) {
+    if (!TAIL || left >= 8) {
+        Packed<unsigned, 4> a;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] = (__bf16)x[i];
-        *reinterpret_cast<bf16x8*>(p) = a;
+        for (int i = 0; i < 4; ++i) a.v[i] = __builtin_bit_cast(unsigned, bf16x2{(__bf16)x[2 * i], (__bf16)x[2 * i + 1]});
+        *reinterpret_cast<Packed<unsigned, 4>*>(p) = a;
     } else
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < left) p[i] = (__bf16)x[i];
 }
-template <bool VEC> __device__ __forceinline__ uint2 ldq8(const uint8_t* p, int left) {
-    if constexpr (VEC) return *reinterpret_cast<const uint2*>(p);
+template <bool TAIL> __device__ __forceinline__ uint2 ldq8(const uint8_t* p, int left) {
+    if (!TAIL || left >= 8) {
+        const Packed<unsigned, 2> a = *reinterpret_cast<const Packed<unsigned, 2>*>(p);
+        return make_uint2(a.v[0], a.v[1]);
+    }
     uint2 r = make_uint2(0u, 0u);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (i < left) (i < 4 ? r.x : r.y) |= (unsigned)p[i] << (8 * (i & 3));
     return r;
 }
-template <bool VEC> __device__ __forceinline__ void stq8(uint8_t* p, int left, uint2 v) {
-    if constexpr (VEC) *reinterpret_cast<uint2*>(p) = v;
-    else
+template <bool TAIL> __device__ __forceinline__ void stq8(uint8_t* p, int left, uint2 v) {
+    if (!TAIL || left >= 8) {
+        Packed<unsigned, 2> a;
+        a.v[0] = v.x;
+        a.v[1] = v.y;
+        *reinterpret_cast<Packed<unsigned, 2>*>(p) = a;
+    } else
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (i < left) p[i] = (uint8_t)((i < 4 ? v.x : v.y) >> (8 * (i & 3)));
@@ -104,14 +115,14 @@ __device__ __forceinline__ Piece piece_of(long rows, int d, int cpr) {
     return r;
 }
 
-template <typename T, bool VEC>
+template <typename T, bool TAIL>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, long ldx, long rows, int d, int cpr,
         uint8_t* __restrict__ q, long ldq, uint8_t* __restrict__ sc, long lds) {
     const Piece p = piece_of(rows, d, cpr);
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = 0.f;
-    if (p.ok) ld8<VEC>(x + p.row * ldx + p.col, p.left, v);
+    if (p.ok) ld8<TAIL>(x + p.row * ldx + p.col, p.left, v);
     unsigned top = 0;    // bits of max |x| over finite values: integer order is float order
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -139,39 +150,39 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ x, long
     hi = __builtin_amdgcn_cvt_pk_fp8_f32(__uint_as_float(h[6]), __uint_as_float(h[7]), hi, true);
     r.x = (unsigned)lo; r.y = (unsigned)hi;
     if (!p.ok) return;
-    stq8<VEC>(q + p.row * ldq + p.col, p.left, r);
+    stq8<TAIL>(q + p.row * ldq + p.col, p.left, r);
     if ((p.col & (GRP - 1)) == 0) sc[p.row * lds + p.col / GRP] = (uint8_t)(e + 127);
 }
 
-template <typename T, bool VEC>
+template <typename T, bool TAIL>
 __global__ __launch_bounds__(256) void unpack_kernel(const uint8_t* __restrict__ q, long ldq,
         const uint8_t* __restrict__ sc, long lds, long rows, int d, int cpr, T* __restrict__ x, long ldx) {
     const Piece p = piece_of(rows, d, cpr);
     if (!p.ok) return;
     float v[8];
-    values8(ldq8<VEC>(q + p.row * ldq + p.col, p.left), scale_of((int)sc[p.row * lds + p.col / GRP] - 127), v);
-    st8<VEC>(x + p.row * ldx + p.col, p.left, v);
+    values8(ldq8<TAIL>(q + p.row * ldq + p.col, p.left), scale_of((int)sc[p.row * lds + p.col / GRP] - 127), v);
+    st8<TAIL>(x + p.row * ldx + p.col, p.left, v);
 }
 
 // z8 -> dz = dy gelu'(z8) and, where asked, a = gelu(z8): the byte stands in for
 // the two activations a GELU layer's backward reads
-template <typename T, bool VEC>
+template <typename T, bool TAIL>
 __global__ __launch_bounds__(256) void gelu_bwd_kernel(const uint8_t* __restrict__ q, long ldq,
         const uint8_t* __restrict__ sc, long lds, long rows, int d, int cpr, const T* dy, long lddy, T* dz,
         long lddz, T* __restrict__ act, long lda) {
     const Piece p = piece_of(rows, d, cpr);
     if (!p.ok) return;
     float g[8], z[8], a[8];
-    ld8<VEC>(dy + p.row * lddy + p.col, p.left, g);
-    values8(ldq8<VEC>(q + p.row * ldq + p.col, p.left), scale_of((int)sc[p.row * lds + p.col / GRP] - 127), z);
+    ld8<TAIL>(dy + p.row * lddy + p.col, p.left, g);
+    values8(ldq8<TAIL>(q + p.row * ldq + p.col, p.left), scale_of((int)sc[p.row * lds + p.col / GRP] - 127), z);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         float gd;
         pt_gelu_both(z[i], a[i], gd);
         g[i] *= gd;
     }
-    st8<VEC>(dz + p.row * lddz + p.col, p.left, g);
-    if (act) st8<VEC>(act + p.row * lda + p.col, p.left, a);
+    st8<TAIL>(dz + p.row * lddz + p.col, p.left, g);
+    if (act) st8<TAIL>(act + p.row * lda + p.col, p.left, a);
 }
 
 // ------------------------------------------------------- weight gradient
@@ -211,25 +222,22 @@ __device__ __forceinline__ bf16x8 frag_tr(const __bf16* s, int st, int lane) {
 
 __device__ __forceinline__ float trunc_bf16(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 
-// 8 values of dY as they were loaded, 8 codes; single values where rows are not
-// aligned
+// 8 values of dY as they were loaded, 8 codes.  Bounds hold per dword: a row
+// whose bytes are no whole dwords loses its last ones where the descriptor
+// ends, so the matrix's last rows come singly then (ONE).
 template <typename T> struct Raw8;
 template <> struct Raw8<float> {
     pt_uintx4 w[2];
-    template <bool VEC> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off) {
-        if constexpr (VEC) {
-            w[0] = ld_buf16(rs, off);
-            w[1] = ld_buf16(rs, off + 16);
-        } else
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i / 4][i % 4] = ld_buf4(rs, off + 4 * i);
+    template <bool ONE> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off) {
+        w[0] = ld_buf16(rs, off);
+        w[1] = ld_buf16(rs, off + 16);
     }
     __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i / 4][i % 4]); }
 };
 template <> struct Raw8<__bf16> {
     pt_uintx4 w;
-    template <bool VEC> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off) {
-        if constexpr (VEC) w = ld_buf16(rs, off);
+    template <bool ONE> __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off) {
+        if constexpr (!ONE) w = ld_buf16(rs, off);
         else
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = ld_buf2(rs, off + 4 * i) | ld_buf2(rs, off + 4 * i + 2) << 16;
@@ -238,8 +246,8 @@ template <> struct Raw8<__bf16> {
         return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     }
 };
-template <bool VEC> __device__ __forceinline__ pt_uintx2 codes8(__amdgpu_buffer_rsrc_t rs, int off) {
-    if constexpr (VEC) return ld_buf8(rs, off);
+template <bool ONE> __device__ __forceinline__ pt_uintx2 codes8(__amdgpu_buffer_rsrc_t rs, int off) {
+    if constexpr (!ONE) return ld_buf8(rs, off);
     pt_uintx2 r = {0u, 0u};
 #pragma unroll
     for (int i = 0; i < 8; ++i) r[i / 4] |= ld_buf1(rs, off + i) << (8 * (i % 4));
@@ -257,8 +265,8 @@ template <typename T, int TM, int TN> struct DwCfg {
     static_assert(TK % RA == 0 && TK % RB == 0 && LDS >= (size_t)RA * TM * 4, "staging passes, column sums");
 };
 
-// VEC: rows of dy and q are 16 / 8 B aligned with n, k multiples of 8
-template <typename T, bool VEC, int TM, int TN>
+// WHOLE: rows of dy and q are whole dwords
+template <typename T, bool WHOLE, int TM, int TN>
 __global__ __launch_bounds__(2 * TN) void dw_kernel(const DwArgs g) {
     typedef DwCfg<T, TM, TN> C;
     constexpr int NP = C::NP, SA = C::SA, SB = C::SB, MT = TM / 64;
@@ -301,14 +309,21 @@ __global__ __launch_bounds__(2 * TN) void dw_kernel(const DwArgs g) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) csum[i] = 0.f;
     auto fetch = [&](int r, Set& f) {
-        const auto ry = ya.rows(r, r1, TK), rq = xq.rows(r, r1, TK), rs = xs.rows(r, r1, TK);
+        // a row more than the step has: its last row's end is inside
+        const auto ry = ya.rows(r, r1, TK + 1), rq = xq.rows(r, r1, TK + 1), rs = xs.rows(r, r1, TK + 1);
+        if (WHOLE || r + TK < r1) {
 #pragma unroll
-        for (int u = 0; u < C::PA; ++u) f.a[u].template load<VEC>(ry, offa[u]);
+            for (int u = 0; u < C::PA; ++u) f.a[u].template load<false>(ry, offa[u]);
 #pragma unroll
-        for (int u = 0; u < C::PB; ++u) {
-            f.xb[u] = codes8<VEC>(rq, offq[u]);
-            f.xe[u] = ld_buf1(rs, offs[u]);
+            for (int u = 0; u < C::PB; ++u) f.xb[u] = codes8<false>(rq, offq[u]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < C::PA; ++u) f.a[u].template load<true>(ry, offa[u]);
+#pragma unroll
+            for (int u = 0; u < C::PB; ++u) f.xb[u] = codes8<true>(rq, offq[u]);
         }
+#pragma unroll
+        for (int u = 0; u < C::PB; ++u) f.xe[u] = ld_buf1(rs, offs[u]);
     };
     auto put = [&](auto sum, __bf16* As, const Set& f) {
         __bf16* Bs = As + NP * TK * SA;
@@ -530,15 +545,12 @@ int grid_for(int rows, int d, int* cpr) {
     *cpr = pt_cdiv(d, GRP) * (GRP / 8);
     return pt_cdiv((long)rows * *cpr, 256);
 }
-// whether 8 values can move as 16 bytes of T (fp32: twice)
-template <typename T> bool vec8(const void* p, long ld) { return al(p, 16) && ld % (16 / (int)sizeof(T)) == 0; }
-bool vecq(const void* q, long ldq, int d) { return al(q, 8) && ldq % 8 == 0 && d % 8 == 0; }
 
 template <typename T>
 int pack(const void* x, long ldx, int rows, int d, uint8_t* q, long ldq, uint8_t* sc, long lds, hipStream_t s) {
     int cpr;
     const int grid = grid_for(rows, d, &cpr);
-    auto kern = vecq(q, ldq, d) && vec8<T>(x, ldx) ? pack_kernel<T, true> : pack_kernel<T, false>;
+    auto kern = d % 8 ? pack_kernel<T, true> : pack_kernel<T, false>;
     hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, s, static_cast<const T*>(x), ldx, (long)rows, d, cpr, q, ldq,
                        sc, lds);
     PT_LAUNCH_CHECK();
@@ -549,7 +561,7 @@ int unpack(const uint8_t* q, long ldq, const uint8_t* sc, long lds, int rows, in
            hipStream_t s) {
     int cpr;
     const int grid = grid_for(rows, d, &cpr);
-    auto kern = vecq(q, ldq, d) && vec8<T>(x, ldx) ? unpack_kernel<T, true> : unpack_kernel<T, false>;
+    auto kern = d % 8 ? unpack_kernel<T, true> : unpack_kernel<T, false>;
     hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, s, q, ldq, sc, lds, (long)rows, d, cpr, static_cast<T*>(x),
                        ldx);
     PT_LAUNCH_CHECK();
@@ -560,30 +572,29 @@ int gelu(const uint8_t* q, long ldq, const uint8_t* sc, long lds, int rows, int 
          void* dz, long lddz, void* act, long lda, hipStream_t s) {
     int cpr;
     const int grid = grid_for(rows, d, &cpr);
-    const bool vec = vecq(q, ldq, d) && vec8<T>(dy, lddy) && vec8<T>(dz, lddz) && (!act || vec8<T>(act, lda));
-    auto kern = vec ? gelu_bwd_kernel<T, true> : gelu_bwd_kernel<T, false>;
+    auto kern = d % 8 ? gelu_bwd_kernel<T, true> : gelu_bwd_kernel<T, false>;
     hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, s, q, ldq, sc, lds, (long)rows, d, cpr,
                        static_cast<const T*>(dy), lddy, static_cast<T*>(dz), lddz, static_cast<T*>(act), lda);
     PT_LAUNCH_CHECK();
     return PTCG_OK;
 }
-template <typename T, bool VEC, int TM, int TN> int launch_dw(const DwArgs& g, hipStream_t s) {
+template <typename T, bool WHOLE, int TM, int TN> int launch_dw(const DwArgs& g, hipStream_t s) {
     typedef DwCfg<T, TM, TN> C;
-    auto kern = dw_kernel<T, VEC, TM, TN>;
+    auto kern = dw_kernel<T, WHOLE, TM, TN>;
     if (C::LDS > 64 * 1024)
         PT_HIP(hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)C::LDS));
     hipLaunchKernelGGL(kern, dim3((unsigned)((long)g.tm * g.tn * g.splits)), dim3(C::NTH), C::LDS, s, g);
     PT_LAUNCH_CHECK();
     return PTCG_OK;
 }
-template <typename T, bool VEC> int dw_tiles(const DwArgs& g, const DwPlan& p, hipStream_t s) {
+template <typename T, bool WHOLE> int dw_tiles(const DwArgs& g, const DwPlan& p, hipStream_t s) {
     if constexpr (sizeof(T) == 2)
-        if (p.big_m) return launch_dw<T, VEC, 256, 256>(g, s);
-    return p.big_n ? launch_dw<T, VEC, 128, 256>(g, s) : launch_dw<T, VEC, 128, 128>(g, s);
+        if (p.big_m) return launch_dw<T, WHOLE, 256, 256>(g, s);
+    return p.big_n ? launch_dw<T, WHOLE, 128, 256>(g, s) : launch_dw<T, WHOLE, 128, 128>(g, s);
 }
 template <typename T> int dw(const DwArgs& g, const DwPlan& p, hipStream_t s) {
-    const bool vec = vecq(g.q, g.ldq, g.k) && vec8<T>(g.dy, g.lddy) && g.n % 8 == 0;
-    PT_TRY(vec ? (dw_tiles<T, true>(g, p, s)) : (dw_tiles<T, false>(g, p, s)));
+    const bool whole = g.k % 4 == 0 && (sizeof(T) == 4 || g.n % 2 == 0);
+    PT_TRY(whole ? (dw_tiles<T, true>(g, p, s)) : (dw_tiles<T, false>(g, p, s)));
     if (p.splits > 1) {
         // enough workgroups for two per CU or so
         const long quads = g.pstride / 4;

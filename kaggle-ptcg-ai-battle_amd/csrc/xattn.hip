@@ -87,9 +87,9 @@ __device__ __forceinline__ long row_off(const XArgs& a, const PtcgHeadLayout& l,
 
 // Workgroups go to the 8 XCDs in turn; consecutive logical indexes on one XCD
 // share a sample's keys in its L2.
-__device__ __forceinline__ int xcd_block(int nblk) {
-    const int x = blockIdx.x & 7, per = nblk >> 3, rem = nblk & 7;
-    return x * per + min(x, rem) + (blockIdx.x >> 3);
+__device__ __forceinline__ int xcd_block(int b, int nblk) {
+    const int x = b & 7, per = nblk >> 3, rem = nblk & 7;
+    return x * per + min(x, rem) + (b >> 3);
 }
 
 // Which (sample, rest) a workgroup works on.  Samples whose lengths only the
@@ -99,15 +99,16 @@ __device__ __forceinline__ int xcd_block(int nblk) {
 // 1 001 .. 4 003 keys on 512 places).  Indexes past the last tile: i = -1.
 struct Place { int i, rest; };
 template <class Cost, class Tiles>
-__device__ __forceinline__ Place place_of(const XArgs& a, bool sorted, int per_sample, Cost cost, Tiles tiles) {
+__device__ __forceinline__ Place place_of(const XArgs& a, bool sorted, int b, int nblk, int per_sample, Cost cost,
+                                          Tiles tiles) {
     Place p;
     if (!sorted) {
-        const int b = xcd_block(gridDim.x);
-        p.i = b / per_sample;
-        p.rest = b - p.i * per_sample;
+        const int l = xcd_block(b, nblk);
+        p.i = l / per_sample;
+        p.rest = l - p.i * per_sample;
         return p;
     }
-    const int lane = threadIdx.x & 63, b = blockIdx.x;
+    const int lane = threadIdx.x & 63;
     const Sample s = sample_of(a, min(lane, a.n - 1));
     const int c = lane < a.n ? cost(s) : -1, t = lane < a.n ? tiles(s) : 0;
     int first = 0;
@@ -498,7 +499,8 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
     int* sh = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int qw = wave % NW, kw = wave / NW;
-    const Place pl = place_of(a, a.sorted && nsplit == 1, a.KV * qtiles * nsplit, [](const Sample& x) { return x.kl; },
+    const Place pl = place_of(a, a.sorted && nsplit == 1, blockIdx.x, gridDim.x, a.KV * qtiles * nsplit,
+                              [](const Sample& x) { return x.kl; },
                               [&](const Sample& x) { return (x.ql * a.G + C::BQ - 1) / C::BQ * a.KV; });
     if (pl.i < 0) return;
     const int i = pl.i;
@@ -659,49 +661,51 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
                            reinterpret_cast<T*>(smem) + qw * Out<T, DH>::WAVE, lane);
 }
 
-// Joins the key splits: a workgroup per row; groups of 32 lanes take every 8th
-// split, 4 columns a lane, and meet in LDS in group order (one wave walking 56
-// splits waits them in line: 13.6 us for 32 rows of 128).
-template <typename T>
-__global__ __launch_bounds__(256) void xattn_join_kernel(const XArgs a, const float* __restrict__ part,
-        T* __restrict__ out, float* __restrict__ lse, int nsplit) {
-    __shared__ float4 sh[256];
-    __shared__ float shl[8], shm[4];
-    const int tid = threadIdx.x, lane = tid & 63, grp = tid >> 5, c = tid & 31;
-    const long R = (long)a.n * a.H * a.lq, row = blockIdx.x;
-    const int qi = (int)(row % a.lq), head = (int)(row / a.lq % a.H), i = (int)(row / a.lq / a.H);
+// Joins the key splits.  Groups of LG lanes (4 columns each) take a row's splits
+// in turn, `per_row` groups a row, and meet in LDS in group order (one wave
+// walking 56 splits waits them in line: 13.6 us for 32 rows of 128; one row a
+// workgroup whatever its splits: 17 us more for 17 208 rows of 8 splits).
+constexpr int JOIN_NTH = 512;
+template <typename T, int LG>
+__global__ __launch_bounds__(JOIN_NTH) void xattn_join_kernel(const XArgs a, const float* __restrict__ part,
+        T* __restrict__ out, float* __restrict__ lse, int nsplit, int per_row) {
+    constexpr int NG = JOIN_NTH / LG;
+    __shared__ float4 sh[JOIN_NTH];
+    __shared__ float2 shm[NG];
+    const int tid = threadIdx.x, grp = tid / LG, c = tid % LG, g0 = grp & (per_row - 1);
+    const long R = (long)a.n * a.H * a.lq, row = (long)blockIdx.x * (NG / per_row) + grp / per_row;
+    const bool live = row < R;
+    const int qi = live ? (int)(row % a.lq) : 0, head = live ? (int)(row / a.lq % a.H) : 0;
+    const int i = live ? (int)(row / a.lq / a.H) : 0;
     const Sample s = sample_of(a, i);
-    if (qi >= s.ql) return;
     const float2* ml = reinterpret_cast<const float2*>(part + (long)nsplit * R * a.dh);
-    float m = -INFINITY;
-    for (int p = tid; p < nsplit; p += 256) m = fmaxf(m, ml[p * R + row].x);
-    m = wave_max(m);
-    if (lane == 0) shm[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(shm[0], shm[1]), fmaxf(shm[2], shm[3]));
-    const float ms = m == -INFINITY ? 0.f : m;
-    float l = 0.f;
+    float m = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    // one more split, or one more group: maximum em, sum el, values x
+    auto add = [&](float em, float el, const float4& x) {
+        const float mn = fmaxf(m, em), ms = mn == -INFINITY ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - ms), f1 = __builtin_amdgcn_exp2f(em - ms);
+        m = mn;
+        l = l * f0 + el * f1;
+        acc.x = acc.x * f0 + x.x * f1; acc.y = acc.y * f0 + x.y * f1;
+        acc.z = acc.z * f0 + x.z * f1; acc.w = acc.w * f0 + x.w * f1;
+    };
+    if (live && qi < s.ql) {
 #pragma unroll 4
-    for (int p = grp; p < nsplit; p += 8) {
-        const float2 e = ml[p * R + row];
-        const float w = __builtin_amdgcn_exp2f(e.x - ms);
-        l += e.y * w;
-        // a split without a kept key left zeros (its w is 0 as well)
-        if (4 * c < a.dh) {
-            const float4 x = *reinterpret_cast<const float4*>(part + (p * R + row) * a.dh + 4 * c);
-            acc.x += x.x * w; acc.y += x.y * w; acc.z += x.z * w; acc.w += x.w * w;
+        for (int p = g0; p < nsplit; p += per_row) {
+            const float2 e = ml[p * R + row];
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (4 * c < a.dh) x = *reinterpret_cast<const float4*>(part + (p * R + row) * a.dh + 4 * c);
+            add(e.x, e.y, x);
         }
     }
     sh[tid] = acc;
-    if (c == 0) shl[grp] = l;
+    if (c == 0) shm[grp] = make_float2(m, l);
     __syncthreads();
-    if (grp > 0) return;
-#pragma unroll
-    for (int g = 1; g < 8; ++g) {
-        const float4 x = sh[g * 32 + c];
-        acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
-        l += shl[g];
+    if (g0 > 0 || !live || qi >= s.ql) return;
+    for (int g = 1; g < per_row; ++g) {
+        const float2 e = shm[grp + g];
+        add(e.x, e.y, sh[(grp + g) * LG + c]);
     }
     const bool none = m == -INFINITY && l == 0.f;
     const float f = none ? 0.f : 1.f / l;
@@ -726,27 +730,33 @@ template <typename T, int DH, int NW, int KS, int KT> struct DqCfg {
     static constexpr size_t LDS = BUFS + BK * sizeof(float) + 64;
 };
 
+// what the backward reads and writes; part: the splits' (nsplit > 1)
+template <typename T> struct Grads {
+    const T *q, *k, *v, *out, *dout;
+    const float* lse;
+    T *dq, *dk, *dv;
+    float *delta, *part;
+};
+// one workgroup's share of a sample: its tile, split and kv head
+struct Share { int i, tile, sp, kvh; };
+
 template <typename T, int DH, int NW, int KS, int KT>
-__global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_dq_kernel(const XArgs a,
-        const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const T* __restrict__ out,
-        const float* __restrict__ lse, const T* __restrict__ dout, T* __restrict__ dq,
-        float* __restrict__ delta, float* __restrict__ part, int qtiles, int nsplit, int split_keys) {
+__device__ __forceinline__ void dq_body(const XArgs& a, const Grads<T>& p, const Share& w, int nsplit,
+                                        int split_keys, char* smem) {
     typedef DqCfg<T, DH, NW, KS, KT> C;
     typedef KvTile<T, DH, DH == 128, C::BK, C::NTH> Kv;
     constexpr int PS = Kv::St::PS;
-    extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     float* kfs = reinterpret_cast<float*>(smem + C::BUFS);
     int* sh = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int qw = wave % NW, kw = wave / NW;
-    const Place pl = place_of(a, a.sorted && nsplit == 1, a.KV * qtiles * nsplit, [](const Sample& x) { return x.kl; },
-                              [&](const Sample& x) { return (x.ql * a.G + C::BQ - 1) / C::BQ * a.KV; });
-    if (pl.i < 0) return;
-    const int i = pl.i;
+    const int i = w.i, qt = w.tile, sp = w.sp, kvh = w.kvh;
     const Sample s = sample_of(a, i);
-    const int qtn = a.sorted && nsplit == 1 ? (s.ql * a.G + C::BQ - 1) / C::BQ : qtiles;
-    const int qt = pl.rest % qtn, sp = pl.rest / qtn % nsplit, kvh = pl.rest / qtn / nsplit;
+    const T *q = p.q, *k = p.k, *v = p.v, *out = p.out, *dout = p.dout;
+    const float* lse = p.lse;
+    T* dq = p.dq;
+    float *delta = p.delta, *part = p.part;
     const int rows = s.ql * a.G;
     if (qt * C::BQ >= rows) return;
     const int r = qt * C::BQ + 32 * qw + (lane & 31);
@@ -888,29 +898,23 @@ template <typename T, int DH, int NK, int QS, int QT> struct DkvCfg {
     static constexpr size_t LDS = BUFS + VROWS + 2 * BQ * sizeof(float) + 16;
 };
 
-template <typename T, int DH, int NK, int QS, int QT>
-__global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_dkv_kernel(const XArgs a,
-        const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, const float* __restrict__ lse,
-        const T* __restrict__ dout, const float* __restrict__ delta, T* __restrict__ dk, T* __restrict__ dv,
-        float* __restrict__ part, int ktiles, int nsplit, int split_rows) {
+// OWN: D_i made here from o and do (nothing of the dQ kernel's is read)
+template <typename T, int DH, int NK, int QS, int QT, bool OWN>
+__device__ __forceinline__ void dkv_body(const XArgs& a, const Grads<T>& g, const Share& w, int nsplit,
+                                         int split_rows, char* smem) {
     typedef DkvCfg<T, DH, NK, QS, QT> C;
     typedef Stage<T, DH, DH == 128, C::BQ, C::NTH> St;
-    extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
-    float* lss = reinterpret_cast<float*>(smem + C::BUFS + C::VROWS);   // log-sum-exp and D of each buffer's rows
+    float* lss = reinterpret_cast<float*>(smem + C::BUFS + C::VROWS);   // log-sum-exp and D of the buffer's rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int kwv = wave % NK, qs = wave / NK;
-    // padded rows past k_len get zeros
-    const Place pl = place_of(a, a.sorted && nsplit == 1, a.KV * ktiles * nsplit,
-                              [](const Sample& x) { return x.ql; }, [&](const Sample& x) {
-                                  return ((a.k_off ? x.kl : a.lk) + C::BKEY - 1) / C::BKEY * a.KV;
-                              });
-    if (pl.i < 0) return;
-    const int i = pl.i;
+    const int i = w.i, kt = w.tile, sp = w.sp, kvh = w.kvh;
     const Sample s = sample_of(a, i);
-    const int kall = a.k_off ? s.kl : a.lk;
-    const int ktn = a.sorted && nsplit == 1 ? (kall + C::BKEY - 1) / C::BKEY : ktiles;
-    const int kt = pl.rest % ktn, sp = pl.rest / ktn % nsplit, kvh = pl.rest / ktn / nsplit;
+    const T *q = g.q, *k = g.k, *v = g.v, *out = g.out, *dout = g.dout;
+    const float *lse = g.lse, *delta = g.delta;
+    T *dk = g.dk, *dv = g.dv;
+    float* part = g.part;
+    const int kall = a.k_off ? s.kl : a.lk;     // padded rows past k_len get zeros
     if (kt * C::BKEY >= kall) return;
     const int key = kt * C::BKEY + 32 * kwv + (lane & 31);
     const bool kin = key < kall;
@@ -939,7 +943,7 @@ __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_
     const int r0 = sp * split_rows;
     const int rows = __syncthreads_or(kok) ? min(s.ql * a.G, r0 + split_rows) : 0;
     const int nt = rows > r0 ? (rows - r0 + C::BQ - 1) / C::BQ : 0;
-    St qs_, ds_;
+    St qs_, ds_, os_;
     float lr = 0.f, dr = 0.f;
     int rown = 0;     // rows of the fetched tile
     auto fetch = [&](int t) {
@@ -947,12 +951,13 @@ __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_
         rown = rows - row0;
         qs_.load_q(a, a.q, q + s.q, kvh, row0, rows, tid);
         ds_.load_q(a, a.o, dout + s.o, kvh, row0, rows, tid);
+        if constexpr (OWN) os_.load_q(a, a.o, out + s.o, kvh, row0, rows, tid);
         if (tid < C::BQ) {
             const int r = min(row0 + tid, rows - 1);
             const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
             const long lrow = ((long)i * a.H + head) * a.lq + qi;
             lr = lse[lrow];
-            dr = delta[lrow];
+            if constexpr (!OWN) dr = delta[lrow];
         }
     };
     auto store = [&](__bf16* Qs, float* ls) {
@@ -962,7 +967,21 @@ __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_
             // exp2(s - inf) = 0: rows past the end, and rows that keep no key, add nothing
             const bool live = tid < rown;
             ls[tid] = live && lr != -INFINITY ? lr * LOG2E : INFINITY;
-            ls[C::BQ + tid] = live ? dr : 0.f;
+            if constexpr (!OWN) ls[C::BQ + tid] = live ? dr : 0.f;
+        }
+        if constexpr (OWN) {
+            // a row's chunks lie in CPR neighbouring lanes
+#pragma unroll
+            for (int c = 0; c < St::NCH; ++c) {
+                float D = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) D += ds_.r[c].at(e) * os_.r[c].at(e);
+                if (tid % St::CPR * 8 >= a.dh) D = 0.f;
+#pragma unroll
+                for (int o = 1; o < St::CPR; o <<= 1) D += __shfl_xor(D, o, 64);
+                const int row = tid / St::CPR + c * St::RPP;
+                if (tid % St::CPR == 0) ls[C::BQ + row] = row < rown ? D : 0.f;
+            }
         }
     };
     auto tile = [&](int t, const __bf16* Qs, const float* ls) {
@@ -1055,6 +1074,51 @@ __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_
     Out<T, DH>::key_rows(dv + s.v + (long)kvh * a.v.sh, a.v.sl, key0, kall, a.dh, gv, 1.f, ws, lane);
 }
 
+template <typename T, int DH, int NW, int KS, int KT>
+__global__ __launch_bounds__(64 * NW * KS, (bwd_waves<T, DH, KS>())) void xattn_dq_kernel(const XArgs a,
+        const Grads<T> p, int qtiles, int nsplit, int split_keys) {
+    typedef DqCfg<T, DH, NW, KS, KT> C;
+    extern __shared__ __align__(256) char smem[];
+    const bool sorted = a.sorted && nsplit == 1;
+    const auto tiles = [&](const Sample& x) { return (x.ql * a.G + C::BQ - 1) / C::BQ; };
+    const Place pl = place_of(a, sorted, blockIdx.x, gridDim.x, a.KV * qtiles * nsplit,
+                              [](const Sample& x) { return x.kl; }, [&](const Sample& x) { return tiles(x) * a.KV; });
+    if (pl.i < 0) return;
+    const int qtn = sorted ? tiles(sample_of(a, pl.i)) : qtiles;
+    dq_body<T, DH, NW, KS, KT>(a, p, {pl.i, pl.rest % qtn, pl.rest / qtn % nsplit, pl.rest / qtn / nsplit}, nsplit,
+                               split_keys, smem);
+}
+
+template <typename T, int DH, int NK, int QS, int QT>
+__global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_dkv_kernel(const XArgs a,
+        const Grads<T> p, int ktiles, int nsplit, int split_rows) {
+    typedef DkvCfg<T, DH, NK, QS, QT> C;
+    extern __shared__ __align__(256) char smem[];
+    const bool sorted = a.sorted && nsplit == 1;
+    const auto tiles = [&](const Sample& x) { return ((a.k_off ? x.kl : a.lk) + C::BKEY - 1) / C::BKEY; };
+    const Place pl = place_of(a, sorted, blockIdx.x, gridDim.x, a.KV * ktiles * nsplit,
+                              [](const Sample& x) { return x.ql; }, [&](const Sample& x) { return tiles(x) * a.KV; });
+    if (pl.i < 0) return;
+    const int ktn = sorted ? tiles(sample_of(a, pl.i)) : ktiles;
+    dkv_body<T, DH, NK, QS, QT, false>(a, p, {pl.i, pl.rest % ktn, pl.rest / ktn % nsplit, pl.rest / ktn / nsplit},
+                                       nsplit, split_rows, smem);
+}
+
+// Both in one launch, a sample's head's workgroups of either kind next to each
+// other: what one reads the other finds in the caches, and a small problem's two
+// halves run side by side (512 x 64 x 97 fp32: 142 us against 144 of the two; 43
+// samples of 78 x 151, 40 wide, bf16, forward and backward: 19 against 24).
+template <typename T, int DH, int NW, int KS, int KT, int NK, int QS, int QT>
+__global__ __launch_bounds__(256, (bwd_waves<T, DH, (KS > QS ? KS : QS)>())) void xattn_bwd_kernel(const XArgs a,
+        const Grads<T> p, int qtiles, int ktiles) {
+    static_assert(NW * KS == 4 && NK * QS == 4, "256 threads");
+    extern __shared__ __align__(256) char smem[];
+    const int per = qtiles + ktiles, l = xcd_block(blockIdx.x, gridDim.x), u = l / per, t = l - u * per;
+    const int i = u / a.KV, kvh = u - i * a.KV;
+    if (t < qtiles) dq_body<T, DH, NW, KS, KT>(a, p, {i, t, 0, kvh}, 1, 1 << 30, smem);
+    else dkv_body<T, DH, NK, QS, QT, true>(a, p, {i, t - qtiles, 0, kvh}, 1, 1 << 30, smem);
+}
+
 // adds the splits' parts of dq, or of dk and dv, in split order: 4 columns a thread
 template <typename T>
 __global__ __launch_bounds__(256) void xattn_sum_q_kernel(const XArgs a, const float* __restrict__ part,
@@ -1113,6 +1177,12 @@ int cu_count() {
 // planes) fits LDS up to 64 wide.
 int waves_for(long rows, bool bf16, int dh) { return rows <= 32 && (bf16 || dh <= 64) ? 1 : rows <= 64 ? 2 : 4; }
 
+// whether workgroups go by place_of's order: more of them than run at once
+bool sorted_places(const PtcgCrossAttn* d, long blocks) {
+    const int at_once = (d->bf16 || d->dh <= 64 ? 2 : 1) * cu_count();
+    return d->n > 1 && d->n <= 64 && (d->q_off || d->k_off || d->k_len) && blocks > at_once;
+}
+
 // Splits of a long axis (keys; rows for dk and dv), where the other axis' work-
 // groups leave CUs idle: `per_cu` workgroups a CU, at least two tiles each, and
 // only from so many tiles on that the joining launch costs less than it saves
@@ -1131,24 +1201,38 @@ Split split_of(long blocks, int len, int tile, int per_cu, bool bf16) {
 
 // The forward takes four workgroups a CU: samples differ in length, and the
 // shorter ones' last splits have nothing to do.
-struct Plan { int nw, qtiles; Split s; };
+struct Plan { int nw, qtiles; Split s; bool sorted; };
 Plan fwd_plan(const PtcgCrossAttn* d) {
     Plan p;
     const long rows = (long)d->lq * (d->heads / d->kv_heads);
     p.nw = waves_for(rows, d->bf16, d->dh);
     p.qtiles = pt_cdiv(rows, 32 * p.nw);
-    p.s = split_of((long)d->n * d->kv_heads * p.qtiles, d->lk, p.nw == 1 ? 128 : 64, 4, d->bf16);
+    const long blocks = (long)d->n * d->kv_heads * p.qtiles;
+    p.s = split_of(blocks, d->lk, p.nw == 1 ? 128 : 64, 4, d->bf16);
+    p.sorted = sorted_places(d, blocks);
     return p;
 }
 // backward: keys split for dq, rows for dk and dv
-struct BwdPlan { int nw, nk; Split q, k; int64_t delta, part; };   // workspace floats
+struct BwdPlan {
+    int nw, nk;
+    bool both;              // one launch for both
+    bool sorted;
+    Split q, k;
+    int64_t delta, part;    // workspace floats
+};
 BwdPlan bwd_plan(const PtcgCrossAttn* d) {
     BwdPlan p;
     const long G = d->heads / d->kv_heads, rows = d->lq * G, pairs = (long)d->n * d->kv_heads;
     p.nw = waves_for(rows, d->bf16, d->dh);
     p.nk = waves_for(d->lk, d->bf16, d->dh);
-    p.q = split_of(pairs * pt_cdiv(rows, 32 * p.nw), d->lk, p.nw == 1 ? 128 : 64, 2, d->bf16);
-    p.k = split_of(pairs * pt_cdiv(d->lk, 32 * p.nk), (int)rows, p.nk == 1 ? 128 : 64, 2, d->bf16);
+    const long qb = pairs * pt_cdiv(rows, 32 * p.nw), kb = pairs * pt_cdiv(d->lk, 32 * p.nk);
+    p.q = split_of(qb, d->lk, p.nw == 1 ? 128 : 64, 2, d->bf16);
+    p.k = split_of(kb, (int)rows, p.nk == 1 ? 128 : 64, 2, d->bf16);
+    p.sorted = sorted_places(d, qb > kb ? qb : kb);
+    // 128 wide in bf16 the pair spills (150 samples of 39 x 78, 8 heads on one kv
+    // head, forward and backward: 69 us against 46)
+    p.both = rows > 0 && d->lk > 0 && p.q.n == 1 && p.k.n == 1 && p.nw > 1 && p.nk > 1 && !p.sorted &&
+             !(d->bf16 && d->dh > 64);
     const int64_t R = (int64_t)d->n * d->heads * d->lq, RK = pairs * d->lk;
     p.delta = (R + 3) / 4 * 4;
     const int64_t q = p.q.n > 1 ? p.q.n * R * d->dh : 0, k = p.k.n > 1 ? p.k.n * 2 * RK * d->dh : 0;
@@ -1203,7 +1287,7 @@ int check_desc(const PtcgCrossAttn* d, const char* who) {
     return PTCG_OK;
 }
 
-XArgs to_args(const PtcgCrossAttn* d) {
+XArgs to_args(const PtcgCrossAttn* d, bool sorted) {
     XArgs a;
     a.n = d->n; a.lq = d->lq; a.lk = d->lk; a.H = d->heads; a.KV = d->kv_heads;
     a.G = d->heads / d->kv_heads; a.dh = d->dh;
@@ -1212,7 +1296,7 @@ XArgs to_args(const PtcgCrossAttn* d) {
     a.q = d->q; a.k = d->k; a.v = d->v; a.o = d->o;
     a.q_off = d->q_off; a.k_off = d->k_off; a.k_len = d->k_len;
     a.keep = d->keep; a.keep_sn = d->keep_sn;
-    a.sorted = d->n > 1 && d->n <= 64 && (d->q_off || d->k_off || d->k_len);
+    a.sorted = sorted;
     return a;
 }
 
@@ -1235,8 +1319,11 @@ int launch_fwd(const XArgs& a, const Plan& p, const void* q, const void* k, cons
                        static_cast<T*>(out), lse, part, p.qtiles, p.s.n, p.s.len);
     PT_LAUNCH_CHECK();
     if (p.s.n > 1) {
-        hipLaunchKernelGGL(xattn_join_kernel<T>, dim3((unsigned)((long)a.n * a.H * a.lq)), dim3(256), 0, s, a, part,
-                           static_cast<T*>(out), lse, p.s.n);
+        constexpr int NG = JOIN_NTH / (DH / 4);
+        int per_row = 1;
+        while (per_row < NG && per_row * 4 < p.s.n) per_row *= 2;     // four splits a group
+        hipLaunchKernelGGL((xattn_join_kernel<T, DH / 4>), dim3(pt_cdiv((long)a.n * a.H * a.lq, NG / per_row)),
+                           dim3(JOIN_NTH), 0, s, a, part, static_cast<T*>(out), lse, p.s.n, per_row);
         PT_LAUNCH_CHECK();
     }
     return PTCG_OK;
@@ -1252,66 +1339,87 @@ int fwd_nw(const XArgs& a, const Plan& p, const void* q, const void* k, const vo
 }
 
 template <typename T, int DH, int NW, int KS, int KT>
-int launch_dq(const XArgs& a, const BwdPlan& p, const void* q, const void* k, const void* v, const void* out,
-              const float* lse, const void* dout, void* dq, float* ws, hipStream_t s) {
+int launch_dq(const XArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
     typedef DqCfg<T, DH, NW, KS, KT> C;
     auto kern = xattn_dq_kernel<T, DH, NW, KS, KT>;
     PT_TRY(lds_attr(kern, C::LDS));
     const int qtiles = pt_cdiv((long)a.lq * a.G, C::BQ);
-    float* part = ws + p.delta;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * qtiles * p.q.n)), dim3(C::NTH), C::LDS, s, a,
-                       static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
-                       static_cast<const T*>(out), lse, static_cast<const T*>(dout), static_cast<T*>(dq), ws, part,
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * qtiles * p.q.n)), dim3(C::NTH), C::LDS, s, a, g,
                        qtiles, p.q.n, p.q.len);
     PT_LAUNCH_CHECK();
     if (p.q.n > 1) {
         hipLaunchKernelGGL(xattn_sum_q_kernel<T>, dim3(pt_cdiv((long)a.n * a.H * a.lq * (a.dh / 4), 256)), dim3(256),
-                           0, s, a, part, static_cast<T*>(dq), p.q.n);
+                           0, s, a, g.part, g.dq, p.q.n);
         PT_LAUNCH_CHECK();
     }
     return PTCG_OK;
 }
 
 template <typename T, int DH, int NK, int QS, int QT>
-int launch_dkv(const XArgs& a, const BwdPlan& p, const void* q, const void* k, const void* v, const float* lse,
-               const void* dout, void* dk, void* dv, float* ws, hipStream_t s) {
+int launch_dkv(const XArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
     typedef DkvCfg<T, DH, NK, QS, QT> C;
     auto kern = xattn_dkv_kernel<T, DH, NK, QS, QT>;
     PT_TRY(lds_attr(kern, C::LDS));
     const int ktiles = pt_cdiv(a.lk, C::BKEY);
-    float* part = ws + p.delta;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * ktiles * p.k.n)), dim3(C::NTH), C::LDS, s, a,
-                       static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), lse,
-                       static_cast<const T*>(dout), ws, static_cast<T*>(dk), static_cast<T*>(dv), part, ktiles,
-                       p.k.n, p.k.len);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * ktiles * p.k.n)), dim3(C::NTH), C::LDS, s, a, g,
+                       ktiles, p.k.n, p.k.len);
     PT_LAUNCH_CHECK();
     if (p.k.n > 1) {
         hipLaunchKernelGGL(xattn_sum_kv_kernel<T>, dim3(pt_cdiv(2L * a.n * a.KV * a.lk * (a.dh / 4), 256)), dim3(256),
-                           0, s, a, part, static_cast<T*>(dk), static_cast<T*>(dv), p.k.n);
+                           0, s, a, g.part, g.dk, g.dv, p.k.n);
         PT_LAUNCH_CHECK();
     }
     return PTCG_OK;
 }
 
+template <typename T, int DH, int NW, int KS, int KT, int NK, int QS, int QT>
+int launch_bwd(const XArgs& a, const Grads<T>& g, hipStream_t s) {
+    typedef DqCfg<T, DH, NW, KS, KT> CQ;
+    typedef DkvCfg<T, DH, NK, QS, QT> CK;
+    constexpr size_t LDS = CQ::LDS > CK::LDS ? CQ::LDS : CK::LDS;
+    auto kern = xattn_bwd_kernel<T, DH, NW, KS, KT, NK, QS, QT>;
+    PT_TRY(lds_attr(kern, LDS));
+    const int qtiles = pt_cdiv((long)a.lq * a.G, CQ::BQ), ktiles = pt_cdiv(a.lk, CK::BKEY);
+    hipLaunchKernelGGL(kern, dim3((unsigned)((long)a.n * a.KV * (qtiles + ktiles))), dim3(256), LDS, s, a, g, qtiles,
+                       ktiles);
+    PT_LAUNCH_CHECK();
+    return PTCG_OK;
+}
+
 template <typename T, int DH>
-int bwd(const XArgs& a, const BwdPlan& p, const void* q, const void* k, const void* v, const void* out,
-        const float* lse, const void* dout, void* dq, void* dk, void* dv, float* ws, hipStream_t s) {
+int bwd(const XArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
     constexpr bool ONE = sizeof(T) == 2 || DH <= 64;      // waves_for
     // the rows of a step of dk / dv: 32 where the registers hold no more on their way
     constexpr int QT = DH * planes<T>() >= 128 ? 32 : 64;
+    if constexpr (sizeof(T) == 4 || DH <= 64)
+        if (p.both) {
+            if (p.nw == 2)
+                return p.nk == 2 ? launch_bwd<T, DH, 2, 2, 32, 2, 2, 32>(a, g, s)
+                                 : launch_bwd<T, DH, 2, 2, 32, 4, 1, QT>(a, g, s);
+            return p.nk == 2 ? launch_bwd<T, DH, 4, 1, 64, 2, 2, 32>(a, g, s)
+                             : launch_bwd<T, DH, 4, 1, 64, 4, 1, QT>(a, g, s);
+        }
     if (a.lq > 0) {
         if constexpr (ONE)
-            if (p.nw == 1) PT_TRY((launch_dq<T, DH, 1, 4, 32>(a, p, q, k, v, out, lse, dout, dq, ws, s)));
-        if (p.nw == 2) PT_TRY((launch_dq<T, DH, 2, 2, 32>(a, p, q, k, v, out, lse, dout, dq, ws, s)));
-        if (p.nw == 4) PT_TRY((launch_dq<T, DH, 4, 1, 64>(a, p, q, k, v, out, lse, dout, dq, ws, s)));
+            if (p.nw == 1) PT_TRY((launch_dq<T, DH, 1, 4, 32>(a, p, g, s)));
+        if (p.nw == 2) PT_TRY((launch_dq<T, DH, 2, 2, 32>(a, p, g, s)));
+        if (p.nw == 4) PT_TRY((launch_dq<T, DH, 4, 1, 64>(a, p, g, s)));
     }
     if (a.lk > 0) {
         if constexpr (ONE)
-            if (p.nk == 1) return launch_dkv<T, DH, 1, 4, 32>(a, p, q, k, v, lse, dout, dk, dv, ws, s);
-        if (p.nk == 2) return launch_dkv<T, DH, 2, 2, 32>(a, p, q, k, v, lse, dout, dk, dv, ws, s);
-        return launch_dkv<T, DH, 4, 1, QT>(a, p, q, k, v, lse, dout, dk, dv, ws, s);
+            if (p.nk == 1) return launch_dkv<T, DH, 1, 4, 32>(a, p, g, s);
+        if (p.nk == 2) return launch_dkv<T, DH, 2, 2, 32>(a, p, g, s);
+        return launch_dkv<T, DH, 4, 1, QT>(a, p, g, s);
     }
     return PTCG_OK;
+}
+template <typename T>
+int bwd_dh(int dh, const XArgs& a, const BwdPlan& p, const void* q, const void* k, const void* v, const void* out,
+           const float* lse, const void* dout, void* dq, void* dk, void* dv, float* ws, hipStream_t s) {
+    const Grads<T> g = {static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                        static_cast<const T*>(out), static_cast<const T*>(dout), lse, static_cast<T*>(dq),
+                        static_cast<T*>(dk), static_cast<T*>(dv), ws, ws + p.delta};
+    return dh <= 32 ? bwd<T, 32>(a, p, g, s) : dh <= 64 ? bwd<T, 64>(a, p, g, s) : bwd<T, 128>(a, p, g, s);
 }
 
 int64_t ws_need(const PtcgCrossAttn* d, int backward) {
@@ -1345,8 +1453,8 @@ extern "C" int ptcg_kernel_cross_attention_fwd(const PtcgCrossAttn* d, const voi
     PT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && al16(workspace)),
                "cross_attention_fwd: workspace of %lld bytes, need %lld (16 B aligned)", (long long)workspace_bytes,
                (long long)need);
-    const XArgs a = to_args(d);
     const Plan p = fwd_plan(d);
+    const XArgs a = to_args(d, p.sorted);
     float* part = static_cast<float*>(workspace);
     const hipStream_t s = (hipStream_t)stream;
     if (d->bf16)
@@ -1377,15 +1485,10 @@ extern "C" int ptcg_kernel_cross_attention_bwd(const PtcgCrossAttn* d, const voi
     PT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && al16(workspace)),
                "cross_attention_bwd: workspace of %lld bytes, need %lld (16 B aligned)", (long long)workspace_bytes,
                (long long)need);
-    const XArgs a = to_args(d);
     const BwdPlan p = bwd_plan(d);
+    const XArgs a = to_args(d, p.sorted);
     float* ws = static_cast<float*>(workspace);
     const hipStream_t s = (hipStream_t)stream;
-    if (d->bf16)
-        return d->dh <= 32   ? bwd<__bf16, 32>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
-               : d->dh <= 64 ? bwd<__bf16, 64>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
-                             : bwd<__bf16, 128>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s);
-    return d->dh <= 32   ? bwd<float, 32>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
-           : d->dh <= 64 ? bwd<float, 64>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
-                         : bwd<float, 128>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s);
+    return d->bf16 ? bwd_dh<__bf16>(d->dh, a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
+                   : bwd_dh<float>(d->dh, a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s);
 }

@@ -217,18 +217,20 @@ int ptcg_kernel_attention_path(int L, int Dh);
  *   out_i = sum_j P_ij v_j, lse_i = log sum_j exp(s_ij).
  * Element (sample, row, head, e) of q lies at q[sn sample + sl row + sh head +
  * e]; the same for k, v and o (strides in elements, multiples of 16 bytes, 0
- * allowed in inputs: a broadcast; buffers 16 B aligned).  Gradients lie as
- * their tensors do, dout as out.
+ * allowed in inputs: a broadcast; buffers 16 B aligned; rows of k and v apart or
+ * the same one, less than 2^22 elements from one to the next).  Gradients lie
+ * as their tensors do, dout as out.  Outputs overlap no input.
  * q_off (device, n + 1 ascending ints): packed queries, sample i owns rows
  * q_off[i] .. q_off[i + 1] - 1 of one long matrix (sn unused), at most lq of
  * them; k_off the same for k, v and keep.  k_len (device, n ints, padded keys
  * only): rows past k_len[i] are not read.  keep: 0 masks the key, padded at
  * keep[keep_sn sample + row], packed at keep[row].  NULL each: all rows, all
  * kept.  Masked rows may hold anything, NaN too; their dk and dv are zeros.
- * Rows outside every packed sample stay as they were.
+ * Rows outside every packed sample stay as they were, in lse too.
  * A query that keeps no key gives out = 0, lse = -inf and no gradient.
  * bf16: products of bf16 operands (P and dS rounded to bf16 for them),
- * softmax, statistics and sums fp32.                                        */
+ * softmax, statistics and sums fp32.  fp32: operands as three bf16 terms, so an
+ * infinity among them becomes NaN.                                          */
 typedef struct PtcgHeadLayout {
     int64_t sn, sl, sh;   /* strides of sample, row, head */
 } PtcgHeadLayout;
@@ -287,11 +289,11 @@ int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const void* dout
  * pack: x (fp32, or bf16 where bf16 = 1) to codes and scales; unpack: x8 back.
  * gelu_bwd: the backward of a GELU layer from its pre-activation z8: dz = dy
  * gelu'(z8) and, where act is given, act = gelu(z8) (the next layer's input);
- * dy, dz, act fp32 or bf16; dz may be dy.
+ * dy, dz, act fp32 or bf16; dz may be dy (with its stride).
  * dw: a linear layer's dW (out, in) = dY^T x8 and db = column sums of dY
  * (nullable), fp32, overwritten, summed in a fixed order; dY (rows, out) fp32
- * (split into three bf16 terms: fp32 products; an infinity becomes NaN) or bf16; workspace of
- * _dw_ws_bytes (0: none, -1: refused), 16 B aligned.
+ * (split into three bf16 terms: fp32 products; an infinity becomes NaN) or bf16;
+ * workspace of _dw_ws_bytes (0: none, -1: refused), 16 B aligned.
  * No reference counterpart: it keeps activations in fp32 or bf16.            */
 int ptcg_kernel_ckpt8_pack(const void* x, int64_t ldx, int bf16, int rows, int d, uint8_t* q, int64_t ldq,
                            uint8_t* scales, int64_t lds, void* stream);

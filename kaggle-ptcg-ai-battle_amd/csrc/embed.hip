@@ -378,8 +378,7 @@ struct GradArgs {
 };
 
 // sums of dout rows of sorted tokens [a, b) at CB column pieces `step` apart, in
-// order; several rows in flight (past the end the last one again, not added),
-// as many as leave eight waves a SIMD
+// order; several rows in flight (past the end the last one again, not added)
 template <typename TO, int VW, int CB>
 __device__ __forceinline__ void run_sum(const TO* __restrict__ dout, const GradArgs& g, int a, int b,
                                         const int (&col)[CB], Vals<VW> (&s)[CB]) {
@@ -410,7 +409,7 @@ __device__ __forceinline__ void run_sum(const TO* __restrict__ dout, const GradA
 // (chunk, column block); rows whose run is longer than CHUNK are left to the
 // chunks.  Wide rows take two pieces a lane (CB = 2): a row of few tokens is a
 // chain of dependent loads, and half as many groups walk it (300 007 tokens of
-// 1 024 bf16 values, 100 003 ids: 269 us with one piece).
+// 1 024 bf16 values, 100 003 ids: 250 us against 269 with one piece).
 template <typename TO, int VW, int CB>
 __global__ __launch_bounds__(256) void embed_grad_kernel(const TO* __restrict__ dout, const GradArgs g) {
     const int gl = threadIdx.x & (g.lpr - 1);
@@ -551,7 +550,7 @@ int launch_fwd(const int* ids, long rows, const void* table, long ldt, int vocab
                long ldo, hipStream_t s) {
     const int cpr = d / VW;
     const long blocks = (rows * cpr + 256 * FWD_U - 1) / (256 * FWD_U);
-    PT_REQUIRE(blocks < (1LL << 31), "embedding_fwd: %ld rows of %d are too many", rows, d);
+    PT_REQUIRE(blocks < (1LL << 24), "embedding_fwd: %ld rows of %d are too many", rows, d);   // 2^32 threads
     hipLaunchKernelGGL((embed_fwd_kernel<TT, TO, VW>), dim3((unsigned)blocks), dim3(256), 0, s, ids, rows,
                        static_cast<const TT*>(table), ldt, vocab, cpr, scale, static_cast<TO*>(out), ldo);
     PT_LAUNCH_CHECK();
@@ -571,41 +570,48 @@ int fwd(const int* ids, long rows, const void* table, long ldt, int vocab, int d
     return launch_fwd<TT, TO, 1>(ids, rows, table, ldt, vocab, d, scale, out, ldo, s);
 }
 
-template <typename TO, int VW>
-int launch_grad(const TO* dout, GradArgs g, long rows, hipStream_t s) {
-    const int cpr = g.d / VW;
-    g.lpr = 1;
-    g.lpr_shift = 0;
-    while (g.lpr < 64 && g.lpr < cpr) {
-        g.lpr <<= 1;
-        ++g.lpr_shift;
+// A group's lanes and the launches over a table's rows and the sorted list's chunks
+struct GradPlan { int vw, lpr, lpr_shift, cb, ncc, fold_ncc, nchunks; long blocks; };
+GradPlan grad_plan(const void* dout, long ldo, int bf16, int vocab, int d, const float* dtable, long ldt, long rows) {
+    GradPlan p;
+    const int e = bf16 ? 2 : 4;
+    p.vw = d % 4 || !fits(dout, ldo, e, 4) || !fits(dtable, ldt, 4, 4) ? 1
+           : bf16 && d % 8 == 0 && fits(dout, ldo, e, 8)               ? 8
+                                                                        : 4;
+    const int cpr = d / p.vw;
+    p.lpr = 1;
+    p.lpr_shift = 0;
+    while (p.lpr < 64 && p.lpr < cpr) {
+        p.lpr <<= 1;
+        ++p.lpr_shift;
     }
-    g.ncc = pt_cdiv(cpr, g.lpr);      // the fold's column blocks; the sums' are cb times as wide
-    g.nchunks = rows > CHUNK ? pt_cdiv(rows, CHUNK) : 0;
-    const int cb = g.ncc > 1 ? 2 : 1, fold_ncc = g.ncc;
-    g.ncc = pt_cdiv(g.ncc, cb);
-    const long items = ((long)g.vocab + g.nchunks) * g.ncc, per = 256 >> g.lpr_shift;
-    PT_REQUIRE((items + per - 1) / per < (1LL << 31) && (long)g.nchunks * fold_ncc < (1LL << 31),
-               "embedding_bwd: %d rows of %d are too many", g.vocab, g.d);
-    auto kern = cb == 2 ? embed_grad_kernel<TO, VW, 2> : embed_grad_kernel<TO, VW, 1>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)((items + per - 1) / per)), dim3(256), 0, s, dout, g);
+    p.fold_ncc = pt_cdiv(cpr, p.lpr);      // the fold's column blocks; the sums' are cb times as wide
+    p.cb = p.fold_ncc > 1 ? 2 : 1;
+    p.ncc = pt_cdiv(p.fold_ncc, p.cb);
+    p.nchunks = rows > CHUNK ? pt_cdiv(rows, CHUNK) : 0;
+    const long items = ((long)vocab + p.nchunks) * p.ncc, per = 256 >> p.lpr_shift;
+    p.blocks = (items + per - 1) / per;
+    return p;
+}
+
+template <typename TO, int VW> int launch_grad(const TO* dout, GradArgs g, const GradPlan& p, hipStream_t s) {
+    auto kern = p.cb == 2 ? embed_grad_kernel<TO, VW, 2> : embed_grad_kernel<TO, VW, 1>;
+    g.lpr = p.lpr; g.lpr_shift = p.lpr_shift; g.ncc = p.ncc; g.nchunks = p.nchunks;
+    hipLaunchKernelGGL(kern, dim3((unsigned)p.blocks), dim3(256), 0, s, dout, g);
     PT_LAUNCH_CHECK();
     if (g.nchunks) {
-        g.ncc = fold_ncc;
+        g.ncc = p.fold_ncc;
         hipLaunchKernelGGL(embed_fold_kernel<VW>, dim3((unsigned)(g.nchunks * g.ncc)), dim3(FOLD), 0, s, g);
         PT_LAUNCH_CHECK();
     }
     return PTCG_OK;
 }
 
-template <typename TO>
-int grad(const void* dout, const GradArgs& g, long rows, hipStream_t s) {
+template <typename TO> int grad(const void* dout, const GradArgs& g, const GradPlan& p, hipStream_t s) {
     const TO* x = static_cast<const TO*>(dout);
-    if (sizeof(TO) == 2 && g.d % 8 == 0 && fits(x, g.ldo, 2, 8) && fits(g.dtable, g.ldt, 4, 4))
-        return launch_grad<TO, 8>(x, g, rows, s);
-    if (g.d % 4 == 0 && fits(x, g.ldo, sizeof(TO), 4) && fits(g.dtable, g.ldt, 4, 4))
-        return launch_grad<TO, 4>(x, g, rows, s);
-    return launch_grad<TO, 1>(x, g, rows, s);
+    if constexpr (sizeof(TO) == 2)
+        if (p.vw == 8) return launch_grad<TO, 8>(x, g, p, s);
+    return p.vw == 4 ? launch_grad<TO, 4>(x, g, p, s) : launch_grad<TO, 1>(x, g, p, s);
 }
 
 int check_sizes(const char* who, int64_t rows, int vocab, int d) {
@@ -648,6 +654,10 @@ extern "C" int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const
     PT_REQUIRE(workspace && workspace_bytes >= w.total * 4 && ((uintptr_t)workspace & 15) == 0,
                "embedding_bwd: workspace of %lld bytes, need %lld (16 B aligned)", (long long)workspace_bytes,
                (long long)(w.total * 4));
+    // a launch holds fewer than 2^32 threads
+    const GradPlan gp = grad_plan(dout, ldo, bf16, vocab, d, dtable, ldt, rows);
+    PT_REQUIRE(gp.blocks < (1LL << 24) && (long)gp.nchunks * gp.fold_ncc < (1LL << 32) / FOLD,
+               "embedding_bwd: %lld tokens and a table of %d rows of %d are too many", (long long)rows, vocab, d);
     const hipStream_t s = (hipStream_t)stream;
     int* ws = static_cast<int*>(workspace);
     const SortPlan p = sort_plan(rows, vocab);
@@ -686,5 +696,5 @@ extern "C" int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const
     g.keys = ws + w.keys; g.pos = ws + w.pos; g.starts = ws + w.starts; g.live = ws + w.live;
     g.ldo = ldo; g.ldt = ldt; g.vocab = vocab; g.d = d; g.scale = scale; g.dtable = dtable;
     g.part = reinterpret_cast<float*>(ws + w.part);
-    return bf16 ? grad<__bf16>(dout, g, rows, s) : grad<float>(dout, g, rows, s);
+    return bf16 ? grad<__bf16>(dout, g, gp, s) : grad<float>(dout, g, gp, s);
 }

@@ -1,6 +1,8 @@
 """What the cross-attention, embedding and 8-bit checkpoint entry points refuse
 before anything reaches a device (the checks run on the host alone)."""
 import ctypes
+import os
+import subprocess
 
 import pytest
 
@@ -151,3 +153,51 @@ def test_ckpt8_refuses():
                       (dict(k=1 << 20, n=1 << 20, ldq=1 << 20, lds=1 << 15, lddy=1 << 20), "too large")):
         with bad(match):
             dw(**kw)
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(k=LAY(sn=1024, sl=16, sh=32)), "key rows overlap"), (dict(v=LAY(sn=1024, sl=24, sh=512)), "key rows overlap"),
+    (dict(lk=1, k_off=P, v=LAY(sn=0, sl=16, sh=32)), "key rows overlap"),
+    (dict(n=1 << 22, kv_heads=4), "too many"), (dict(n=1 << 16, lq=1 << 15, q=LAY(sl=128, sh=32)), "too many"),
+    (dict(o=LAY(sn=1 << 60, sl=128, sh=32), n=100), "overlap"),
+])
+def test_cross_attention_refuses_what_a_launch_cannot_hold(kw, match):
+    with pytest.raises(native.PtcgError, match=match):
+        _fwd(_desc(**kw))
+
+
+def test_operators_refuse_more_than_a_launch_holds():
+    bad = lambda match: pytest.raises(native.PtcgError, match=match)
+    L, check = native.lib(), native.check
+    with bad("too many"):
+        _emb_fwd(rows=(1 << 30) - 1, d=4096, ldt=4096, ldo=4096)
+    with bad("too many"):
+        _emb_bwd(rows=100, vocab=1 << 30, d=64, ldt=64, ldo=64, nb=1 << 60)
+    with bad("too many"):
+        _emb_bwd(rows=(1 << 30) - 1, d=1024, ldt=1024, ldo=1024, nb=1 << 60)
+    with bad("too many"):
+        check(L.ptcg_kernel_ckpt8_pack(P, 1024, 0, 1 << 26, 1024, P, 1024, P, 32, None))
+    with bad("stride"):
+        check(L.ptcg_kernel_ckpt8_gelu_bwd(P, 8, P, 1, 4, 8, P, 8, P, 16, None, 0, 0, None))
+    for dz, act in ((P, P + 64), (P + 64, P + 64)):      # act over dy, over dz
+        with bad("act is"):
+            check(L.ptcg_kernel_ckpt8_gelu_bwd(P, 8, P, 1, 4, 8, P + 64, 8, dz, 8, act, 8, 0, None))
+
+
+def test_cross_attention_struct_matches_the_header(tmp_path):
+    """Sizes and field offsets from the C header (compiled with gcc) equal the
+    ctypes declarations."""
+    for name, ct in (("PtcgHeadLayout", native.CPtcgHeadLayout), ("PtcgCrossAttn", native.CPtcgCrossAttn)):
+        fields = [f for f, _ in ct._fields_]
+        src, exe = tmp_path / (name + ".c"), tmp_path / name
+        src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "ptcg_amd_kernels.h"\nint main(void) {\n'
+                       f'  printf("size %zu\\n", sizeof({name}));\n'
+                       + "".join(f'  printf("{f} %zu\\n", offsetof({name}, {f}));\n' for f in fields)
+                       + "  return 0;\n}\n")
+        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+        subprocess.run(["gcc", "-std=c99", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
+        got = dict(l.split() for l in subprocess.run([str(exe)], capture_output=True, text=True,
+                                                     check=True).stdout.splitlines())
+        assert int(got["size"]) == ctypes.sizeof(ct)
+        for f in fields:
+            assert int(got[f]) == getattr(ct, f).offset, f

@@ -266,7 +266,10 @@ __device__ __forceinline__ floatx16 mma_rows_lds(const __bf16* xs, const __bf16*
 // c += X^T P over 32 LDS rows of X: c[dt] is columns 32 dt .. of X; P's register
 // r stands for row 8 (r / 4) + 4 h + r % 4.  bf16: P is rounded to bf16 for the
 // product (relative 2^-9 each, as the stored operands are); its fp32 values make
-// the softmax's sum.
+// the softmax's sum.  Gradients are then off by 2.3e-3 to 2.5e-3 (relative L2),
+// where rounding an exact one to bf16 gives 1.65e-3; a second term of P for
+// samples of up to 64 keys took 1% off that and cost 12% (8 192 x 64 x 97: 277 us
+// against 247, by its registers).
 template <typename T, int DH, bool PAD, int PS>
 __device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floatx16 (&c)[DH / 32], int lane) {
     typedef __attribute__((address_space(3))) bf16x4* lds4;
@@ -298,7 +301,7 @@ __device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floa
 // barrier that publishes them.
 template <typename T, int DH, bool PAD, int BR, int NTH> struct Stage {
     static constexpr int CPR = DH / 8, NCH = BR * CPR / NTH, RPP = NTH / CPR, PS = BR * Lds<DH, PAD>::ST;
-    static_assert(BR * CPR % NTH == 0 && NTH % CPR == 0 && RPP % 16 == 0, "whole chunks per thread, one swizzle");
+    static_assert(BR * CPR % NTH == 0 && NTH % CPR == 0, "whole chunks per thread");
     Chunk<T> r[NCH];
     // byte offset of the thread's first chunk; chunk i is i * RPP rows on
     static __device__ __forceinline__ int first(int ld, int dh, int tid) {
@@ -469,8 +472,8 @@ template <typename T, int DH, int NW, int KS, int KT> struct FwdCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;
     static constexpr int TILE = tile_elems<T, DH, false, BK>();
     // One buffer: what a second one saves in barriers it costs in workgroups a CU
-    // holds (8 192 x 64 x 97, 64 wide: 293 us against 333; a token against 50 001
-    // keys 39 against 46).
+    // holds (with tiles of 64 keys, 8 192 x 64 x 97, 64 wide: 293 us against 333; a
+    // token against 50 001 keys 39 against 46).
     static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
     static constexpr size_t JOIN = (size_t)NW * (KS - 1) * (DH * 32 + 64) * sizeof(float);
     static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);   // the rows' way out
@@ -1106,8 +1109,8 @@ __global__ __launch_bounds__(64 * NK * QS, (bwd_waves<T, DH, QS>())) void xattn_
 
 // Both in one launch, a sample's head's workgroups of either kind next to each
 // other: what one reads the other finds in the caches, and a small problem's two
-// halves run side by side (512 x 64 x 97 fp32: 142 us against 144 of the two; 43
-// samples of 78 x 151, 40 wide, bf16, forward and backward: 19 against 24).
+// halves run side by side (43 samples of 78 x 151, 40 wide, bf16, forward and
+// backward: 19 us against 24).
 template <typename T, int DH, int NW, int KS, int KT, int NK, int QS, int QT>
 __global__ __launch_bounds__(256, (bwd_waves<T, DH, (KS > QS ? KS : QS)>())) void xattn_bwd_kernel(const XArgs a,
         const Grads<T> p, int qtiles, int ktiles) {
@@ -1177,10 +1180,23 @@ int cu_count() {
 // planes) fits LDS up to 64 wide.
 int waves_for(long rows, bool bf16, int dh) { return rows <= 32 && (bf16 || dh <= 64) ? 1 : rows <= 64 ? 2 : 4; }
 
+// workgroups of four waves that run at once
+long at_once(const PtcgCrossAttn* d) { return (d->bf16 || d->dh <= 64 ? 2L : 1L) * cu_count(); }
+
+// Whether the waves of few rows stay without partners along the keys: with more
+// workgroups than run at once, smaller ones fill the CUs as well, wait for fewer
+// waves at a barrier and join nothing.  Forward: 8 192 x 64 x 97, 64 wide, bf16
+// 223 us against 245; 512 of them fp32 50 against 53, 128 wide 115 against 154;
+// 2 000 x 8 x 150, 8 heads, fp32 264 against 733 (a tile of four waves' keys
+// leaves LDS for one workgroup a CU).  In bf16 a long walk of one wave costs more
+// than that (200 x 8 heads, one row, 1 000 keys: 90 us against 78).
+bool lone_waves(const PtcgCrossAttn* d, int waves, long blocks) {
+    return waves < 4 && blocks > at_once(d) && (!d->bf16 || d->lk <= 512);
+}
+
 // whether workgroups go by place_of's order: more of them than run at once
 bool sorted_places(const PtcgCrossAttn* d, long blocks) {
-    const int at_once = (d->bf16 || d->dh <= 64 ? 2 : 1) * cu_count();
-    return d->n > 1 && d->n <= 64 && (d->q_off || d->k_off || d->k_len) && blocks > at_once;
+    return d->n > 1 && d->n <= 64 && (d->q_off || d->k_off || d->k_len) && blocks > at_once(d);
 }
 
 // Splits of a long axis (keys; rows for dk and dv), where the other axis' work-
@@ -1201,7 +1217,7 @@ Split split_of(long blocks, int len, int tile, int per_cu, bool bf16) {
 
 // The forward takes four workgroups a CU: samples differ in length, and the
 // shorter ones' last splits have nothing to do.
-struct Plan { int nw, qtiles; Split s; bool sorted; };
+struct Plan { int nw, qtiles; Split s; bool sorted, lone; };
 Plan fwd_plan(const PtcgCrossAttn* d) {
     Plan p;
     const long rows = (long)d->lq * (d->heads / d->kv_heads);
@@ -1210,11 +1226,13 @@ Plan fwd_plan(const PtcgCrossAttn* d) {
     const long blocks = (long)d->n * d->kv_heads * p.qtiles;
     p.s = split_of(blocks, d->lk, p.nw == 1 ? 128 : 64, 4, d->bf16);
     p.sorted = sorted_places(d, blocks);
+    p.lone = lone_waves(d, p.nw, blocks);
     return p;
 }
 // backward: keys split for dq, rows for dk and dv
 struct BwdPlan {
     int nw, nk;
+    bool qlone, klone;      // waves without partners along the other axis
     bool both;              // one launch for both
     bool sorted;
     Split q, k;
@@ -1225,14 +1243,27 @@ BwdPlan bwd_plan(const PtcgCrossAttn* d) {
     const long G = d->heads / d->kv_heads, rows = d->lq * G, pairs = (long)d->n * d->kv_heads;
     p.nw = waves_for(rows, d->bf16, d->dh);
     p.nk = waves_for(d->lk, d->bf16, d->dh);
-    const long qb = pairs * pt_cdiv(rows, 32 * p.nw), kb = pairs * pt_cdiv(d->lk, 32 * p.nk);
+    long qb = pairs * pt_cdiv(rows, 32 * p.nw), kb = pairs * pt_cdiv(d->lk, 32 * p.nk);
+    p.qlone = lone_waves(d, p.nw, qb);
+    if (p.qlone) p.nw = 2;      // one of them as in the forward gains nothing: its registers spill
+    // dk and dv with few keys (500 x 64 x 60, 8 heads, 64 wide: bf16 77 us against
+    // 99, both gradients), or rows of one tile, whose staging two waves share as
+    // well as four (2 000 x 8 x 150, bf16: 471 against 608; not 128 wide, where two
+    // waves' spill: 200 samples of 1 x 1 000, 604 against 520)
+    p.klone = kb > at_once(d) && (d->lk <= 64 || (rows <= 32 && d->dh <= 64));
+    if (p.klone) {
+        p.nk = 2;
+        kb = pairs * pt_cdiv(d->lk, 64);
+    }
     p.q = split_of(qb, d->lk, p.nw == 1 ? 128 : 64, 2, d->bf16);
     p.k = split_of(kb, (int)rows, p.nk == 1 ? 128 : 64, 2, d->bf16);
     p.sorted = sorted_places(d, qb > kb ? qb : kb);
-    // 128 wide in bf16 the pair spills (150 samples of 39 x 78, 8 heads on one kv
-    // head, forward and backward: 69 us against 46)
-    p.both = rows > 0 && d->lk > 0 && p.q.n == 1 && p.k.n == 1 && p.nw > 1 && p.nk > 1 && !p.sorted &&
-             !(d->bf16 && d->dh > 64);
+    // One launch up to three rounds of workgroups (128 x 64 x 97, 4 heads, 64 wide,
+    // fp32: 38 us against 43 of two launches); of more, the two kernels' own shapes
+    // win (512 of them: 151 against 133).  128 wide in bf16 the pair spills (150 samples of
+    // 39 x 78, 8 heads on one kv head, forward and backward: 69 us against 46).
+    p.both = rows > 0 && d->lk > 0 && p.q.n == 1 && p.k.n == 1 && p.nw > 1 && p.nk > 1 && !p.sorted && !p.qlone &&
+             !p.klone && qb + kb <= 3 * at_once(d) && !(d->bf16 && d->dh > 64);
     const int64_t R = (int64_t)d->n * d->heads * d->lq, RK = pairs * d->lk;
     p.delta = (R + 3) / 4 * 4;
     const int64_t q = p.q.n > 1 ? p.q.n * R * d->dh : 0, k = p.k.n > 1 ? p.k.n * 2 * RK * d->dh : 0;
@@ -1341,8 +1372,12 @@ template <typename T, int DH>
 int fwd_nw(const XArgs& a, const Plan& p, const void* q, const void* k, const void* v, void* out, float* lse,
            float* part, hipStream_t s) {
     if constexpr (sizeof(T) == 2 || DH <= 64)
-        if (p.nw == 1) return launch_fwd<T, DH, 1, 4, 32>(a, p, q, k, v, out, lse, part, s);
-    if (p.nw == 2) return launch_fwd<T, DH, 2, 2, 32>(a, p, q, k, v, out, lse, part, s);
+        if (p.nw == 1)
+            return p.lone ? launch_fwd<T, DH, 1, 1, 32>(a, p, q, k, v, out, lse, part, s)
+                          : launch_fwd<T, DH, 1, 4, 32>(a, p, q, k, v, out, lse, part, s);
+    if (p.nw == 2)
+        return p.lone ? launch_fwd<T, DH, 2, 1, 32>(a, p, q, k, v, out, lse, part, s)
+                      : launch_fwd<T, DH, 2, 2, 32>(a, p, q, k, v, out, lse, part, s);
     return launch_fwd<T, DH, 4, 1, 64>(a, p, q, k, v, out, lse, part, s);
 }
 
@@ -1410,13 +1445,14 @@ int bwd(const XArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
     if (a.lq > 0) {
         if constexpr (ONE)
             if (p.nw == 1) PT_TRY((launch_dq<T, DH, 1, 4, 32>(a, p, g, s)));
-        if (p.nw == 2) PT_TRY((launch_dq<T, DH, 2, 2, 32>(a, p, g, s)));
+        if (p.nw == 2)
+            PT_TRY(p.qlone ? (launch_dq<T, DH, 2, 1, 32>(a, p, g, s)) : (launch_dq<T, DH, 2, 2, 32>(a, p, g, s)));
         if (p.nw == 4) PT_TRY((launch_dq<T, DH, 4, 1, 64>(a, p, g, s)));
     }
     if (a.lk > 0) {
         if constexpr (ONE)
             if (p.nk == 1) return launch_dkv<T, DH, 1, 4, 32>(a, p, g, s);
-        if (p.nk == 2) return launch_dkv<T, DH, 2, 2, 32>(a, p, g, s);
+        if (p.nk == 2) return p.klone ? launch_dkv<T, DH, 2, 1, 32>(a, p, g, s) : launch_dkv<T, DH, 2, 2, 32>(a, p, g, s);
         return launch_dkv<T, DH, 4, 1, QT>(a, p, g, s);
     }
     return PTCG_OK;

@@ -1216,7 +1216,13 @@ Split split_of(long blocks, int len, int tile, int per_cu, bool bf16) {
 }
 
 // The forward takes four workgroups a CU: samples differ in length, and the
-// shorter ones' last splits have nothing to do.
+// shorter ones' last splits have nothing to do (two in fp32 128 wide, as many as
+// run at once).  Up to 32 rows, in fp32 128 wide 64, against 1 024 keys and more go
+// in lone waves that each walk a split of their own (one row against 50 001 keys,
+// 4 samples, 8 heads on 2: 128 wide bf16 40 us against 43, fp32 123 against 163; 64
+// wide bf16 24 against 28, fp32 49 against 76).  Fewer keys, or more rows, are
+// joined as fast in LDS (6 samples of 8 x 667, 8 heads, fp32 15.0 us against 16.5;
+// 2 of 60 x 8 000, bf16 18.3 against 20.3).
 struct Plan { int nw, qtiles; Split s; bool sorted, lone; };
 Plan fwd_plan(const PtcgCrossAttn* d) {
     Plan p;
@@ -1224,9 +1230,10 @@ Plan fwd_plan(const PtcgCrossAttn* d) {
     p.nw = waves_for(rows, d->bf16, d->dh);
     p.qtiles = pt_cdiv(rows, 32 * p.nw);
     const long blocks = (long)d->n * d->kv_heads * p.qtiles;
-    p.s = split_of(blocks, d->lk, p.nw == 1 ? 128 : 64, 4, d->bf16);
+    p.lone = d->lk >= 1024 && (p.nw == 1 || (p.nw == 2 && !d->bf16 && d->dh > 64));
+    p.s = split_of(blocks, d->lk, p.lone ? 32 : p.nw == 1 ? 128 : 64, d->bf16 || d->dh <= 64 ? 4 : 2, d->bf16);
+    if (p.s.n == 1) p.lone = lone_waves(d, p.nw, blocks);
     p.sorted = sorted_places(d, blocks);
-    p.lone = lone_waves(d, p.nw, blocks);
     return p;
 }
 // backward: keys split for dq, rows for dk and dv

@@ -345,3 +345,57 @@ def test_checkpoints_past_2_to_31_bytes(cuda):
     assert ((x8 - x.double()).abs() <= 2.0 ** -4 * x.double().abs() + 2.0 ** -10 * 0.5).all()
     y = dy.double()
     _close("dW", dW, y.t() @ x8, (3 * rows + 8) * U * (y.abs().t() @ x8.abs()))
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("dh", [32, 64, 96])
+@pytest.mark.parametrize("lq,H,KV,lk,mask", [(3, 8, 8, 60, "keep"), (1, 16, 8, 150, "len"), (7, 32, 8, 33, "keep"),
+                                             (20, 8, 8, 540, "len"), (50, 8, 8, 70, "keep"), (9, 8, 8, 1, None)])
+def test_many_samples_of_few_rows(lq, H, KV, lk, mask, dh, bf16, cuda):
+    """More workgroups than run at once, with up to 64 rows a kv head: waves with no
+    partners along the keys, or for dk and dv along the rows."""
+    n = 70
+    kw = {}
+    if mask == "keep":
+        g = torch.Generator(device="cuda").manual_seed(lk)
+        kw["keep"] = (torch.rand(n, lk, generator=g, device="cuda") < 0.7).float()
+        kw["keep"][5] = 0.0
+    elif mask == "len":
+        kw["k_len"] = [(37 * i) % (lk + 1) for i in range(n)]
+    op = Op(n, lq, lk, H, KV, dh, bf16, seed=lk, **kw)
+    if mask == "keep":
+        dead = (kw["keep"] == 0).reshape(-1)
+        ref = [x.clone() for x in (op.k, op.v)]
+        op.k[dead] = math.nan
+        op.v[dead] = math.inf
+    op.fwd()
+    op.bwd()
+    if mask == "keep":
+        op.k, op.v = ref
+    op.check()
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("lq,lk,H,KV,dh,mask", [(1, 1024, 8, 2, 128, "len"), (1, 1024, 8, 2, 64, "keep"),
+                                                (30, 1500, 2, 2, 32, "keep"), (50, 1100, 2, 2, 96, "len"),
+                                                (4, 2049, 8, 1, 64, "empty")])
+def test_long_keys_split_over_lone_waves(lq, lk, H, KV, dh, mask, bf16, cuda):
+    kw = {}
+    if mask == "len":
+        kw["k_len"] = [lk, 40]
+    else:
+        g = torch.Generator(device="cuda").manual_seed(lk)
+        kw["keep"] = (torch.rand(2, lk, generator=g, device="cuda") < 0.6).float()
+        kw["keep"][1, lk // 3:] = 0.0
+        if mask == "empty":
+            kw["keep"][0] = 0.0
+    op = Op(2, lq, lk, H, KV, dh, bf16, seed=4, **kw)
+    assert native.lib().ptcg_kernel_cross_attention_ws_bytes(ctypes.byref(op.a), 0) > 0     # the split form
+    op.fwd()
+    op.bwd()
+    op.check()
+    first = op.out.clone()
+    op.ws.fill_(0xff)
+    op.fwd(lse=False)
+    torch.cuda.synchronize()
+    assert torch.equal(op.out, first)

@@ -16,10 +16,14 @@
 // Sort: least significant digit first, 1 digit of up to 11 bits where the
 // vocabulary fits, else digits of up to 9 bits; per digit a count per
 // workgroup, a scan over the workgroups, and a placement whose ranks within a
-// wave come from ballots.
+// wave come from ballots.  Where the counts are few the placement scans them (a
+// launch less: 48 107 tokens of 3 606 ids, two digits of 6 bits, 36 us against 40;
+// 90 000 of 50 000, two of 8 bits on 176 workgroups, would take 10 more).  Passes
+// are chains of waits more than work: tiles of 512 tokens take 1.5 us less than
+// 1 024 of them at 49 152.
 // Up to RANK_ROWS tokens each token counts the tokens before it instead (one
 // launch for the three of every digit).
-// Runs longer than CHUNK tokens (frequent ids) are added in CHUNK-aligned
+// Runs longer than LONG tokens (frequent ids) are added in CHUNK-aligned
 // pieces of the sorted list by groups of lanes of their own and folded in order,
 // so one frequent id does not hold a single group for its whole run.
 #include "model.h"
@@ -30,9 +34,14 @@ namespace {
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int CHUNK = 64;        // tokens a group adds on its own
+// Tokens of one id: up to LONG a group of lanes adds in line; more are added in
+// pieces by CHUNK (49 152 tokens, 64 wide, of a Zipf law over 2 048 ids: 34 us
+// against 41 with 64 and 64; with 32 and 32 ids of 24 on average lose 3%)
+constexpr int LONG = 40, CHUNK = 32;
 constexpr int MAXB = 1024;        // workgroups of a sort pass (tiles grow past it)
 constexpr int BITS1 = 11, BITS2 = 9;
+constexpr int SMALL = 100000;    // tokens up to which a sort pass has twice the workgroups
+constexpr int FEW = 8192;        // counts up to which every placing workgroup adds them up itself
 constexpr int RANK_ROWS = 4096;  // 16 KB of keys in LDS; 4 096 compares a token
 
 // VW values of a row, as floats
@@ -194,48 +203,66 @@ __global__ __launch_bounds__(1024) void sort_scan_kernel(const SortPass p) {
     if (w == 0) p.tot[d] = base;
 }
 
-// Placement.  A wave owns a quarter of the workgroup's tile and walks it 64
+// Placement (SCAN: with the scan).  A wave owns a quarter of the workgroup's tile and walks it 64
 // tokens at a time: a token's place is its digit's base, plus the digit's
 // tokens before it in earlier workgroups, waves and batches, plus those in
 // lower lanes of its batch.
-__global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
+template <int U, bool SCAN> __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
     extern __shared__ int sm[];
     const int bins = 1 << p.bits, n = pass_n(p);
     int* cnt = sm;               // [4][bins]
     int* tot = sm + 4 * bins;    // [bins]
-    int* part = tot + bins;      // [4]
+    int* before = tot + bins;    // [bins], SCAN alone
+    int* part = before + (SCAN ? bins : 0);   // [4]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // what the previous launches left, all of it on its way before anything waits
     constexpr int PT = (1 << BITS1) / 256;
     int tv[PT], mv[PT];
     const int* mine = p.cnt + (long)blockIdx.x * bins;
+    if constexpr (!SCAN)
 #pragma unroll
-    for (int i = 0; i < PT; ++i) {
-        const int d = min(tid + 256 * i, bins - 1);
-        tv[i] = p.tot[d];
-        mv[i] = mine[d];
-    }
-    for (int i = tid; i < 4 * bins; i += 256) cnt[i] = 0;
-    // four batches' keys at a time (a wave's quarter is a multiple of 256 tokens)
+        for (int i = 0; i < PT; ++i) {
+            const int d = min(tid + 256 * i, bins - 1);
+            tv[i] = p.tot[d];
+            mv[i] = mine[d];
+        }
+    for (int i = tid; i < (SCAN ? 6 : 4) * bins; i += 256) cnt[i] = 0;
+    // U batches' keys at a time (a wave's quarter is a multiple of 64 U tokens)
     const int per = p.tile / 4, w0 = blockIdx.x * p.tile + wave * per;
-    int key[4], dig[4];
+    int key[U], dig[U];
     auto load = [&](int o) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) dig[u] = digit_of(p, w0 + o + 64 * u + lane, n, key[u]);
+        for (int u = 0; u < U; ++u) dig[u] = digit_of(p, w0 + o + 64 * u + lane, n, key[u]);
     };
     load(0);
     __syncthreads();
-    for (int o = 0; o < per; o += 256) {
+    if constexpr (SCAN) {
+        // each digit's counts of all workgroups and of those before this one
+        const int w = min(bins, 256), g = tid / w, ng = 256 / w;
+        for (int d = tid % w; d < bins; d += w) {
+            int all = 0, pre = 0;
+#pragma unroll 8
+            for (int b = g; b < p.nb; b += ng) {
+                const int c = p.cnt[(long)b * bins + d];
+                all += c;
+                pre += b < (int)blockIdx.x ? c : 0;
+            }
+            atomicAdd(&tot[d], all);
+            atomicAdd(&before[d], pre);
+        }
+    }
+    for (int o = 0; o < per; o += 64 * U) {
         if (o > 0) load(o);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < U; ++u)
             if (dig[u] >= 0) atomicAdd(&cnt[wave * bins + dig[u]], 1);
     }
     // exclusive scan of the digits' totals: thread t adds up bpt consecutive digits
     const int bpt = (bins + 255) / 256, d0 = tid * bpt;
+    if constexpr (!SCAN)
 #pragma unroll
-    for (int i = 0; i < PT; ++i)
-        if (tid + 256 * i < bins) tot[tid + 256 * i] = tv[i];
+        for (int i = 0; i < PT; ++i)
+            if (tid + 256 * i < bins) tot[tid + 256 * i] = tv[i];
     __syncthreads();
     int sum = 0;
     for (int i = 0; i < bpt; ++i)
@@ -271,7 +298,7 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
         if (d >= bins) break;
         const int at = tot[d];
         if (p.starts && blockIdx.x == 0 && d < p.vocab) p.starts[d] = at;
-        int run = at + mv[i];
+        int run = at + (SCAN ? before[d] : mv[i]);
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const int c = cnt[w * bins + d];
@@ -280,11 +307,11 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
         }
     }
     __syncthreads();
-    for (int o = 0; o < per; o += 256) {
-        if (per > 256) load(o);
-        int at[4];
+    for (int o = 0; o < per; o += 64 * U) {
+        if (per > 64 * U) load(o);
+        int at[U];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < U; ++u) {
             const int d = dig[u];
             unsigned long long same = __ballot(d >= 0);
             for (int i = 0; i < p.bits; ++i) {
@@ -299,7 +326,7 @@ __global__ __launch_bounds__(256) void sort_place_kernel(const SortPass p) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < U; ++u)
             if (dig[u] >= 0) {
                 const int t = w0 + o + 64 * u + lane;
                 p.out_keys[at[u]] = key[u];
@@ -406,7 +433,7 @@ __device__ __forceinline__ void run_sum(const TO* __restrict__ dout, const GradA
 }
 
 // One group of lpr lanes per (table row, column block of CB * lpr * VW), then per
-// (chunk, column block); rows whose run is longer than CHUNK are left to the
+// (chunk, column block); rows whose run is longer than LONG are left to the
 // chunks.  Wide rows take two pieces a lane (CB = 2): a row of few tokens is a
 // chain of dependent loads, and half as many groups walk it (300 007 tokens of
 // 1 024 bf16 values, 100 003 ids: 250 us against 269 with one piece).
@@ -429,7 +456,7 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const TO* __restrict__ 
     Vals<VW> s[CB];
     if (item < cold) {
         const int a = g.starts[r], b = g.starts[r + 1];
-        if (b - a > CHUNK) return;
+        if (b - a > LONG) return;
         run_sum<TO, VW, CB>(dout, g, a, b, col, s);
 #pragma unroll
         for (int c = 0; c < CB; ++c) {
@@ -444,14 +471,14 @@ __global__ __launch_bounds__(256) void embed_grad_kernel(const TO* __restrict__ 
     const int a = (int)r * CHUNK, b = min(a + CHUNK, live);
     float* part = g.part + r * 2 * g.d;
     const int v0 = g.keys[a], s0 = g.starts[v0], e0 = g.starts[v0 + 1];
-    if (e0 - s0 > CHUNK && s0 < a) {
+    if (e0 - s0 > LONG && s0 < a) {
         run_sum<TO, VW, CB>(dout, g, a, min(e0, b), col, s);
 #pragma unroll
         for (int c = 0; c < CB; ++c)
             if (ok[c]) st<VW>(part + col[c], s[c]);
     }
     const int v1 = g.keys[b - 1], s1 = g.starts[v1], e1 = g.starts[v1 + 1];
-    if (e1 - s1 > CHUNK && s1 >= a) {
+    if (e1 - s1 > LONG && s1 >= a) {
         run_sum<TO, VW, CB>(dout, g, s1, b, col, s);
 #pragma unroll
         for (int c = 0; c < CB; ++c)
@@ -471,7 +498,7 @@ __global__ __launch_bounds__(FOLD) void embed_fold_kernel(const GradArgs g) {
     if ((long)c * CHUNK >= live) return;
     const int a = c * CHUNK, b = min(a + CHUNK, live);
     const int v = g.keys[b - 1], s0 = g.starts[v], e0 = g.starts[v + 1];
-    if (e0 - s0 <= CHUNK || s0 < a) return;      // the same for the whole workgroup
+    if (e0 - s0 <= LONG || s0 < a) return;      // the same for the whole workgroup
     const int pieces = (e0 - 1) / CHUNK - c + 1;
     const int col = (cc * g.lpr + gl) * VW;
     Vals<VW> s;
@@ -504,20 +531,21 @@ int bits_for(int vocab) {
     return b;
 }
 
-struct SortPlan { int passes, bits, tile, nb, bins; };   // passes 0: by rank
+struct SortPlan { int passes, bits, tile, nb, bins; bool scan; };   // passes 0: by rank
 SortPlan sort_plan(long rows, int vocab) {
     SortPlan p;
     const int nb = bits_for(vocab);
     p.passes = nb <= BITS1 ? 1 : (nb + BITS2 - 1) / BITS2;
     if (rows <= RANK_ROWS) {
-        p = SortPlan{0, 0, 0, 0, 0};
+        p = SortPlan{};
         return p;
     }
     p.bits = (nb + p.passes - 1) / p.passes;
     p.bins = 1 << p.bits;
-    p.tile = 1024;
+    p.tile = rows <= SMALL ? 512 : 1024;
     if (rows > (long)MAXB * 1024) p.tile = pt_cdiv(pt_cdiv(rows, MAXB), 1024) * 1024;
     p.nb = pt_cdiv(rows, p.tile);
+    p.scan = (long)p.bins * p.nb > FEW;
     return p;
 }
 
@@ -536,7 +564,7 @@ Ws ws_layout(long rows, int vocab, int d) {
     w.tot = take(p.bins);
     w.starts = take((long)vocab + 1);
     w.live = take(4);
-    w.part = take(rows > CHUNK ? (long)pt_cdiv(rows, CHUNK) * 2 * d : 0);
+    w.part = take(rows > LONG ? (long)pt_cdiv(rows, CHUNK) * 2 * d : 0);
     w.total = at;
     return w;
 }
@@ -588,7 +616,7 @@ GradPlan grad_plan(const void* dout, long ldo, int bf16, int vocab, int d, const
     p.fold_ncc = pt_cdiv(cpr, p.lpr);      // the fold's column blocks; the sums' are cb times as wide
     p.cb = p.fold_ncc > 1 ? 2 : 1;
     p.ncc = pt_cdiv(p.fold_ncc, p.cb);
-    p.nchunks = rows > CHUNK ? pt_cdiv(rows, CHUNK) : 0;
+    p.nchunks = rows > LONG ? pt_cdiv(rows, CHUNK) : 0;
     const long items = ((long)vocab + p.nchunks) * p.ncc, per = 256 >> p.lpr_shift;
     p.blocks = (items + per - 1) / per;
     return p;
@@ -672,7 +700,7 @@ extern "C" int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const
     a.n = (int)rows; a.vocab = vocab; a.bits = p.bits; a.tile = p.tile; a.nb = p.nb;
     a.cnt = ws + w.cnt; a.tot = ws + w.tot;
     a.starts = p.passes == 1 ? ws + w.starts : nullptr;
-    const size_t place_lds = (5 * (size_t)p.bins + 4) * sizeof(int);
+    const size_t place_lds = ((p.scan ? 5 : 6) * (size_t)p.bins + 4) * sizeof(int);
     for (int k = 0; k < p.passes; ++k) {
         a.shift = k * p.bits;
         a.live = k == 0 ? ws + w.live : nullptr;
@@ -681,9 +709,13 @@ extern "C" int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const
         a.out_pos = ws + (odd ? w.pos2 : w.pos);
         hipLaunchKernelGGL(sort_count_kernel, dim3(a.nb), dim3(256), p.bins * sizeof(int), s, a);
         PT_LAUNCH_CHECK();
-        hipLaunchKernelGGL(sort_scan_kernel, dim3(pt_cdiv(p.bins, 64)), dim3(1024), 0, s, a);
-        PT_LAUNCH_CHECK();
-        hipLaunchKernelGGL(sort_place_kernel, dim3(a.nb), dim3(256), place_lds, s, a);
+        if (p.scan) {
+            hipLaunchKernelGGL(sort_scan_kernel, dim3(pt_cdiv(p.bins, 64)), dim3(1024), 0, s, a);
+            PT_LAUNCH_CHECK();
+        }
+        auto place = p.tile == 512 ? (p.scan ? sort_place_kernel<2, false> : sort_place_kernel<2, true>)
+                                   : (p.scan ? sort_place_kernel<4, false> : sort_place_kernel<4, true>);
+        hipLaunchKernelGGL(place, dim3(a.nb), dim3(256), place_lds, s, a);
         PT_LAUNCH_CHECK();
         a.keys = a.out_keys; a.pos = a.out_pos; a.n_dev = ws + w.live;
     }

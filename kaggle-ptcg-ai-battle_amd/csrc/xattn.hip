@@ -242,7 +242,8 @@ __device__ __forceinline__ floatx16 mma_rows(const __bf16* xs, const Row<T, DH>&
     for (int c = 0; c < DH / 16; ++c) {
         bf16x8 a[planes<T>()];
 #pragma unroll
-        for (int p = 0; p < planes<T>(); ++p) a[p] = *reinterpret_cast<const bf16x8*>(xs + p * PS + Lds<DH, PAD>::chunk_at(lane & 31, lane >> 5, c));
+        for (int p = 0; p < planes<T>(); ++p)
+            a[p] = *reinterpret_cast<const bf16x8*>(xs + p * PS + Lds<DH, PAD>::chunk_at(lane & 31, lane >> 5, c));
         mma(a, y.f[c], s);
     }
     return s;
@@ -287,8 +288,10 @@ __device__ __forceinline__ void mma_tr(const __bf16* xs, const floatx16& p, floa
 #pragma unroll
             for (int pl = 0; pl < planes<T>(); ++pl) {
                 const __bf16* q = xs + pl * PS + 16 * kb * Lds<DH, PAD>::ST + 4 * (i & 1);
-                const bf16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + Lds<DH, PAD>::group_at(r0, ch, dt)));
-                const bf16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + Lds<DH, PAD>::group_at(r0 + 8, ch, dt)));
+                const lds4 p0 = (lds4)(q + Lds<DH, PAD>::group_at(r0, ch, dt));
+                const lds4 p1 = (lds4)(q + Lds<DH, PAD>::group_at(r0 + 8, ch, dt));
+                const bf16x4 u = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(p0);
+                const bf16x4 w = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(p1);
                 a[pl] = bf16x8{u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
             }
             mma(a, b, c[dt]);
@@ -551,7 +554,8 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
         floatx16 sc[KT / 32];
         float mt = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < KT / 32; ++j) sc[j] = mma_rows<T, DH, false, PS>(Ks + (kw * KT + 32 * j) * Lds<DH, false>::ST, qf, lane);
+        for (int j = 0; j < KT / 32; ++j)
+            sc[j] = mma_rows<T, DH, false, PS>(Ks + (kw * KT + 32 * j) * Lds<DH, false>::ST, qf, lane);
         if (masked) {
 #pragma unroll
             for (int j = 0; j < KT / 32; ++j)

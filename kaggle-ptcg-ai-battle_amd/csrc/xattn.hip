@@ -1271,10 +1271,13 @@ BwdPlan bwd_plan(const PtcgCrossAttn* d) {
     p.sorted = sorted_places(d, qb > kb ? qb : kb);
     // One launch up to three rounds of workgroups (128 x 64 x 97, 4 heads, 64 wide,
     // fp32: 38 us against 43 of two launches); of more, the two kernels' own shapes
-    // win (512 of them: 151 against 133).  128 wide in bf16 the pair spills (150 samples of
-    // 39 x 78, 8 heads on one kv head, forward and backward: 69 us against 46).
+    // win (512 of them: 151 against 133).  128 wide the pair's registers do not
+    // suffice: in bf16 it spills (150 samples of 39 x 78, 8 heads on one kv head,
+    // forward and backward: 69 us against 46), in fp32 the compiler moved staging
+    // offsets to accumulation registers where only the lanes with a query row run,
+    // and the other lanes' later tiles were lost.
     p.both = rows > 0 && d->lk > 0 && p.q.n == 1 && p.k.n == 1 && p.nw > 1 && p.nk > 1 && !p.sorted && !p.qlone &&
-             !p.klone && qb + kb <= 3 * at_once(d) && !(d->bf16 && d->dh > 64);
+             !p.klone && qb + kb <= 3 * at_once(d) && d->dh <= 64;
     const int64_t R = (int64_t)d->n * d->heads * d->lq, RK = pairs * d->lk;
     p.delta = (R + 3) / 4 * 4;
     const int64_t q = p.q.n > 1 ? p.q.n * R * d->dh : 0, k = p.k.n > 1 ? p.k.n * 2 * RK * d->dh : 0;
@@ -1286,9 +1289,11 @@ bool layout_ok(const PtcgHeadLayout& l, int e) {
     return l.sn >= 0 && l.sl >= 0 && l.sh >= 0 && l.sn % e == 0 && l.sl % e == 0 && l.sh % e == 0;
 }
 
-// whether no two elements of an output share an address (offsets: the sample
-// stride is unused)
-bool layout_apart(const PtcgHeadLayout& l, int n, int rows, int heads, int dh) {
+// whether no two elements of an output share an address; packed, the host knows
+// no row count (rows only bounds a sample's), and only that rows and heads are not
+// one upon another
+bool layout_apart(const PtcgHeadLayout& l, bool packed, int n, int rows, int heads, int dh) {
+    if (packed) return ((n <= 1 && rows <= 1) || l.sl >= dh) && (heads <= 1 || l.sh >= dh);
     int64_t st[3] = {n > 1 ? l.sn : -1, rows > 1 ? l.sl : -1, heads > 1 ? l.sh : -1};
     int64_t ex[3] = {n, rows, heads};
     for (int i = 0; i < 3; ++i)
@@ -1445,7 +1450,7 @@ int bwd(const XArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
     constexpr bool ONE = sizeof(T) == 2 || DH <= 64;      // waves_for
     // the rows of a step of dk / dv: 32 where the registers hold no more on their way
     constexpr int QT = DH * planes<T>() >= 128 ? 32 : 64;
-    if constexpr (sizeof(T) == 4 || DH <= 64)
+    if constexpr (DH <= 64)
         if (p.both) {
             if (p.nw == 2)
                 return p.nk == 2 ? launch_bwd<T, DH, 2, 2, 32, 2, 2, 32>(a, g, s)
@@ -1502,7 +1507,7 @@ extern "C" int ptcg_kernel_cross_attention_fwd(const PtcgCrossAttn* d, const voi
     if ((int64_t)d->n * d->lq == 0) return PTCG_OK;
     PT_REQUIRE(q && out && (d->lk == 0 || (k && v)), "cross_attention_fwd: null buffer");
     PT_REQUIRE(al16(q) && al16(k) && al16(v) && al16(out), "cross_attention_fwd: buffers must be 16 B aligned");
-    PT_REQUIRE(layout_apart(d->o, d->q_off ? 1 : d->n, d->lq, d->heads, d->dh),
+    PT_REQUIRE(layout_apart(d->o, d->q_off, d->n, d->lq, d->heads, d->dh),
                "cross_attention_fwd: rows of the output overlap");
     const int64_t need = ws_need(d, 0);
     PT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && al16(workspace)),
@@ -1531,10 +1536,10 @@ extern "C" int ptcg_kernel_cross_attention_bwd(const PtcgCrossAttn* d, const voi
     PT_REQUIRE(d->lk == 0 || (k && v && dk && dv), "cross_attention_bwd: null buffer");
     PT_REQUIRE(al16(q) && al16(k) && al16(v) && al16(out) && al16(dout) && al16(dq) && al16(dk) && al16(dv),
                "cross_attention_bwd: buffers must be 16 B aligned");
-    PT_REQUIRE(layout_apart(d->q, d->q_off ? 1 : d->n, d->lq, d->heads, d->dh),
+    PT_REQUIRE(layout_apart(d->q, d->q_off, d->n, d->lq, d->heads, d->dh),
                "cross_attention_bwd: rows of dq overlap (a broadcast q has no gradient layout)");
-    PT_REQUIRE(layout_apart(d->k, d->k_off ? 1 : d->n, d->lk, d->kv_heads, d->dh) &&
-                   layout_apart(d->v, d->k_off ? 1 : d->n, d->lk, d->kv_heads, d->dh),
+    PT_REQUIRE(layout_apart(d->k, d->k_off, d->n, d->lk, d->kv_heads, d->dh) &&
+                   layout_apart(d->v, d->k_off, d->n, d->lk, d->kv_heads, d->dh),
                "cross_attention_bwd: rows of dk or dv overlap (broadcast keys have no gradient layout)");
     const int64_t need = ws_need(d, 1);
     PT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && al16(workspace)),

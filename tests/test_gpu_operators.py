@@ -399,3 +399,24 @@ def test_long_keys_split_over_lone_waves(lq, lk, H, KV, dh, mask, bf16, cuda):
     op.fwd(lse=False)
     torch.cuda.synchronize()
     assert torch.equal(op.out, first)
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+def test_packed_rows_fewer_than_the_bound(bf16, cuda):
+    """The bounds lq and lk of packed samples may pass all rows there are, in
+    matrices of one head after the other too."""
+    op = Op(2, 90, 200, 4, 2, 32, bf16, q_len=[3, 20], k_off_len=[30, 11], order="hld")
+    op.fwd()
+    op.bwd()
+    op.check()
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("dh", [32, 64, 88, 128])
+@pytest.mark.parametrize("lq,lk", [(2, 161), (33, 97), (2, 65), (5, 100), (61, 190)])
+def test_wave_halves_without_rows_against_several_tiles(lq, lk, dh, bf16, cuda):
+    """Lanes without a query row still carry their share of every key tile."""
+    op = Op(3, lq, lk, 2, 2, dh, bf16, seed=30)
+    op.fwd()
+    op.bwd()
+    op.check()

@@ -166,6 +166,13 @@ def test_cross_attention_refuses_what_a_launch_cannot_hold(kw, match):
         _fwd(_desc(**kw))
 
 
+@pytest.mark.parametrize("kw", [dict(o=LAY(sn=0, sl=0, sh=32)), dict(o=LAY(sn=0, sl=128, sh=0)),
+                                dict(o=LAY(sn=0, sl=16, sh=320))])
+def test_packed_cross_attention_refuses_rows_upon_another(kw):
+    with pytest.raises(native.PtcgError, match="overlap"):
+        _fwd(_desc(q_off=P, k_off=P, **kw))
+
+
 def test_operators_refuse_more_than_a_launch_holds():
     bad = lambda match: pytest.raises(native.PtcgError, match=match)
     L, check = native.lib(), native.check

@@ -311,9 +311,10 @@ __global__ __launch_bounds__(2 * TN) void dw_kernel(const DwArgs g) {
     // inlined by order: as a call, the sets lie in scratch (29 777 x 634 x 64 fp32:
     // 688 us against 32)
     auto fetch = [&](int r, Set& f) __attribute__((always_inline)) {
-        // a row more than the step has: its last row's end is inside
-        const auto ry = ya.rows(r, r1, TK + 1), rq = xq.rows(r, r1, TK + 1), rs = xs.rows(r, r1, TK + 1);
-        if (WHOLE || r + TK < r1) {
+        // three rows more than the step has: the last dword of its last row is inside,
+        // for rows of one byte too
+        const auto ry = ya.rows(r, r1, TK + 3), rq = xq.rows(r, r1, TK + 3), rs = xs.rows(r, r1, TK + 3);
+        if (WHOLE || r + TK + 2 < r1) {
 #pragma unroll
             for (int u = 0; u < C::PA; ++u) f.a[u].template load<false>(ry, offa[u]);
 #pragma unroll

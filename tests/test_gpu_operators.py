@@ -9,7 +9,7 @@ import torch
 
 from ptcg_amd import native
 from refxattn import reference, within
-from test_gpu_ckpt8 import values64
+from test_gpu_ckpt8 import test_weight_gradient as check_weight_gradient, values64
 from test_gpu_cross_attention import GUARD, Op
 
 pytestmark = pytest.mark.gpu
@@ -420,3 +420,11 @@ def test_wave_halves_without_rows_against_several_tiles(lq, lk, dh, bf16, cuda):
     op.fwd()
     op.bwd()
     op.check()
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("rows", [32, 33, 34, 35, 36, 65, 3000])
+@pytest.mark.parametrize("k,n,pad", [(1, 4, 0), (1, 4, 1), (2, 1, 0), (3, 3, 0), (5, 1, 1), (9, 7, 0)])
+def test_weight_gradient_of_the_narrowest_rows(k, n, pad, rows, bf16, cuda):
+    """Rows of 1 to 9 bytes, whose last dword ends rows later."""
+    check_weight_gradient(rows, k, n, pad, bf16, cuda)

@@ -219,7 +219,9 @@ int ptcg_kernel_attention_path(int L, int Dh);
  * e]; the same for k, v and o (strides in elements, multiples of 16 bytes, 0
  * allowed in inputs: a broadcast; buffers 16 B aligned; rows of k and v apart or
  * the same one, less than 2^22 elements from one to the next).  Gradients lie
- * as their tensors do, dout as out.  Outputs overlap no input.
+ * as their tensors do, dout as out.  Outputs overlap no input, and no two of an
+ * output's elements share an address: refused where the strides show it (packed,
+ * where two rows or more of them would: the host knows no row count).
  * q_off (device, n + 1 ascending ints): packed queries, sample i owns rows
  * q_off[i] .. q_off[i + 1] - 1 of one long matrix (sn unused), at most lq of
  * them; k_off the same for k, v and keep.  k_len (device, n ints, padded keys

@@ -1289,11 +1289,18 @@ bool layout_ok(const PtcgHeadLayout& l, int e) {
     return l.sn >= 0 && l.sl >= 0 && l.sh >= 0 && l.sn % e == 0 && l.sl % e == 0 && l.sh % e == 0;
 }
 
-// whether no two elements of an output share an address; packed, the host knows
-// no row count (rows only bounds a sample's), and only that rows and heads are not
-// one upon another
+// Whether no two elements of an output share an address.  Packed, the host knows
+// no row count (rows only bounds a sample's): a row's heads have to lie within the
+// row stride, or else two rows, the fewest that a batch of more than one row may
+// hold, within the head stride.
 bool layout_apart(const PtcgHeadLayout& l, bool packed, int n, int rows, int heads, int dh) {
-    if (packed) return ((n <= 1 && rows <= 1) || l.sl >= dh) && (heads <= 1 || l.sh >= dh);
+    if (packed) {
+        const bool many = n > 1 || rows > 1;
+        if (heads <= 1) return !many || l.sl >= dh;
+        if (l.sh < dh) return false;
+        if (!many) return true;
+        return l.sh <= l.sl ? l.sh <= (l.sl - dh) / (heads - 1) : l.sl >= dh && l.sl <= l.sh - dh;
+    }
     int64_t st[3] = {n > 1 ? l.sn : -1, rows > 1 ? l.sl : -1, heads > 1 ? l.sh : -1};
     int64_t ex[3] = {n, rows, heads};
     for (int i = 0; i < 3; ++i)

@@ -208,3 +208,42 @@ def test_cross_attention_struct_matches_the_header(tmp_path):
         assert int(got["size"]) == ctypes.sizeof(ct)
         for f in fields:
             assert int(got[f]) == getattr(ct, f).offset, f
+
+
+@pytest.mark.parametrize("lay", [
+    LAY(sn=0, sl=64, sh=32),      # row r + 1's head 0 on row r's head 2
+    LAY(sn=0, sl=32, sh=32),      # rows and heads at one stride
+    LAY(sn=0, sl=96, sh=32),      # one head too many for a row
+    LAY(sn=0, sl=64, sh=64),
+    LAY(sn=0, sl=128, sh=132),    # heads of rows: the second row reaches into the next head
+    LAY(sn=0, sl=1 << 40, sh=1 << 39),
+    LAY(sn=0, sl=1 << 62, sh=1 << 62),
+])
+def test_packed_outputs_refuse_rows_that_reach_into_heads(lay):
+    """Whatever the packed row counts: from two rows on, two elements share an address."""
+    with pytest.raises(native.PtcgError, match="output overlap"):
+        _fwd(_desc(q_off=P, k_off=P, o=lay))
+    with pytest.raises(native.PtcgError, match="dq overlap"):
+        _bwd(_desc(q_off=P, k_off=P, q=lay))
+    # 4 kv heads: the same layouts for the gradients of k and v
+    for name in ("k", "v") if lay.sl < 1 << 22 else ():
+        with pytest.raises(native.PtcgError, match="dk or dv overlap"):
+            _bwd(_desc(q_off=P, k_off=P, kv_heads=4, **{name: lay}))
+
+
+@pytest.mark.parametrize("lay", [
+    LAY(sn=0, sl=128, sh=32), LAY(sn=0, sl=256, sh=32), LAY(sn=0, sl=512, sh=128), LAY(sn=0, sl=32, sh=64),
+    LAY(sn=0, sl=32, sh=32 * 16), LAY(sn=0, sl=132, sh=164), LAY(sn=0, sl=1 << 40, sh=1 << 38)])
+def test_packed_outputs_that_may_lie_apart_pass_the_layout_check(lay):
+    """They get as far as the workspace (a long sample, whose keys are split)."""
+    with pytest.raises(native.PtcgError, match="workspace"):
+        _fwd(_desc(n=1, lq=3, lk=100000, q_off=P, k_off=P, o=lay))
+    with pytest.raises(native.PtcgError, match="workspace"):
+        _bwd(_desc(q_off=P, k_off=P, q=lay), nb=4)
+
+
+def test_a_lone_row_takes_any_row_stride_and_a_lone_head_any_head_stride():
+    with pytest.raises(native.PtcgError, match="workspace"):
+        _fwd(_desc(n=1, lq=1, lk=100000, q_off=P, k_off=P, o=LAY(sn=0, sl=0, sh=32)))
+    with pytest.raises(native.PtcgError, match="workspace"):
+        _fwd(_desc(n=1, lq=3, lk=100000, heads=1, kv_heads=1, q_off=P, k_off=P, o=LAY(sn=0, sl=32, sh=0)))

@@ -268,12 +268,15 @@ int ptcg_kernel_cross_attention_bwd(const PtcgCrossAttn* desc, const void* q, co
  * their flag is 1 (products and sums fp32).  An id outside [0, vocab) is
  * padding: a row of zeros, and no gradient.
  * bwd: dtable (vocab, d) fp32, overwritten, [v] = scale sum of dout[t] over the
- * tokens of id v in token order (the tokens are sorted: no atomics, the same
- * sums in every run); dout bf16 where bf16 = 1; workspace of _bwd_ws_bytes
- * (-1: refused), 16 B aligned.  rows < 2^30, d <= 65536.
- * Replaces the lookups of the reference's k_tok_cat and their scatter with
- * atomics (native/model/ptcg_model.cu:289, ptcg_model2.cu:36) for tables of
- * any size.                                                                */
+ * tokens of id v; dout bf16 where bf16 = 1; workspace of _bwd_ws_bytes (-1:
+ * refused), 16 B aligned.  The tokens are sorted: no atomics, and a fixed order
+ * of every sum, so equal calls give equal bits.  Up to 40 tokens of an id it is
+ * the tokens' order; more are added in pieces of the sorted list, whose cuts
+ * (and last bits) also depend on the tokens of smaller ids.  rows < 2^30, d <=
+ * 65536.
+ * Reference counterpart: k_tok_cat and its scatter with atomics (native/model/
+ * ptcg_model.cu:289, ptcg_model2.cu:36), in whose place the model here has
+ * kernels of its own; these are for tables of any size.                     */
 int ptcg_kernel_embedding_fwd(const int32_t* ids, int64_t rows, const void* table, int64_t ldt, int table_bf16,
                               int vocab, int d, float scale, void* out, int64_t ldo, int out_bf16, void* stream);
 int64_t ptcg_kernel_embedding_bwd_ws_bytes(int64_t rows, int vocab, int d);

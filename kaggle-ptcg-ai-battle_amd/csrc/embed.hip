@@ -10,7 +10,7 @@
 //
 // Backward.  The tokens are sorted by id (stable: equal ids keep token order),
 // a row of the table then owns a run of the sorted list and adds its tokens in
-// that order, so the sums do not depend on scheduling.  Adding by atomics
+// an order that the list alone gives, not scheduling.  Adding by atomics
 // instead costs a read-modify-write per element and token, in an order that
 // changes; equal ids then queue on the same lines.
 // Sort: least significant digit first, 1 digit of up to 11 bits where the
@@ -24,8 +24,10 @@
 // Up to RANK_ROWS tokens each token counts the tokens before it instead (one
 // launch for the three of every digit).
 // Runs longer than LONG tokens (frequent ids) are added in CHUNK-aligned
-// pieces of the sorted list by groups of lanes of their own and folded in order,
-// so one frequent id does not hold a single group for its whole run.
+// pieces of the sorted list by groups of lanes of their own, and the pieces in a
+// fixed order (embed_fold_kernel), so one frequent id does not hold a single
+// group for its whole run.  Where a run is cut depends on where it lies, that is
+// on the tokens of smaller ids; shorter runs are added in token order.
 #include "model.h"
 #include "../../include/ptcg_amd_kernels.h"
 

@@ -207,3 +207,85 @@ def test_gradient_against_differences(cuda):
     want = float((dtable.double() * dirn.double()).sum())
     slack = float((dtable.double() * dirn.double()).abs().sum())
     assert abs((loss[0] - loss[1]) / (2 * h) - want) <= 2.0 ** -24 * (3 * mag / (2 * h) + rows * slack)
+
+
+def _check_lookup(ids, table, vocab, scale, out):
+    """One product and one rounding: torch's bits, signs among them (zeros of either sign are equal)."""
+    live = (ids >= 0) & (ids < vocab)
+    rows = table.float()[ids.clamp(0, vocab - 1).long()]
+    assert torch.equal(out, torch.where(live[:, None], rows * scale, 0.0).to(out.dtype))
+
+
+@pytest.mark.parametrize("tb,ob", [(0, 0), (0, 1), (1, 0), (1, 1)])
+@pytest.mark.parametrize("d,pad,off", [(1, 0, 0), (64, 0, 0), (64, 3, 0), (77, 0, 0), (256, 8, 1), (1500, 4, 4)])
+def test_lookup_keeps_signs(d, pad, off, tb, ob, cuda):
+    g = torch.Generator(device="cuda").manual_seed(d + pad)
+    rows, vocab = 333, 50
+    ids = _ids(rows, vocab, "uniform", g)
+    table = torch.randn(vocab, d + pad + off, generator=g, device="cuda").to(T[tb])[:, off:off + d]
+    full = torch.full((rows, d + pad + off), GUARD, dtype=T[ob], device="cuda")
+    for scale in (1.5, -0.375):
+        _fwd(ids, table, vocab, d, scale, full[:, off:off + d], full.stride(0))
+        torch.cuda.synchronize()
+        _check_lookup(ids, table, vocab, scale, full[:, off:off + d])
+
+
+@pytest.mark.parametrize("ob", [0, 1])
+@pytest.mark.parametrize("rows,vocab,d,kind", [
+    # few counts, scanned within the placement, with two and with four batches a wave in flight
+    (99999, 40, 16, "skewed"), (100000, 60, 4, "uniform"), (100001, 40, 16, "skewed"), (120001, 3000, 8, "uniform"),
+    (131000, 4096, 4, "skewed"),
+    # tiles of more than 1 024 tokens, whose waves load their keys anew
+    (1048576, 700, 4, "skewed"), (1048577, 700, 4, "skewed"), (1200007, 5, 4, "uniform"), (1200007, 5000, 4, "skewed"),
+    (2100001, 60, 4, "skewed"), (1200007, 100003, 4, "uniform"),
+])
+def test_gradient_of_every_sort_shape(rows, vocab, d, kind, ob, cuda):
+    print(f"embedding gradient {rows} x {d} of {vocab} {kind} bf16={ob}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(rows + d)
+    ids = _ids(rows, vocab, kind, g)
+    dout = torch.randn(rows, d, generator=g, device="cuda").to(T[ob])
+    dtable = torch.full((vocab, d), GUARD, device="cuda")
+    _bwd(ids, dout, vocab, d, 0.5, dtable, _ws(rows, vocab, d))
+    torch.cuda.synchronize()
+    _check_grad(ids, dout, vocab, 0.5, dtable)
+
+
+def _in_token_order(ids, dout, vocab, scale, most):
+    """scale * (((0 + dout[t0]) + dout[t1]) + ...) in fp32 over the first `most` of each id's tokens."""
+    live = torch.nonzero((ids >= 0) & (ids < vocab))[:, 0]
+    order = live[torch.argsort(ids[live].long(), stable=True)]
+    key = ids[order].long()
+    first = torch.searchsorted(key, torch.arange(vocab, device="cuda"))
+    nth = torch.arange(order.numel(), device="cuda") - first[key]
+    s = torch.zeros(vocab, dout.shape[1], device="cuda")
+    for k in range(most):
+        sel = nth == k
+        s[key[sel]] += dout[order[sel]].float()
+    return s * scale
+
+
+COUNTS = [1, 2, 31, 32, 33, 39, 40, 41, 42, 63, 64, 65, 40, 96, 97, 41, 7, 128, 40, 0, 41, 300, 40, 129]
+
+
+@pytest.mark.parametrize("ob", [0, 1])
+@pytest.mark.parametrize("d", [12, 136, 520])
+@pytest.mark.parametrize("stride,fill", [(1, 0), (1, 4500), (4001, 0), (4001, 4500)])   # ids apart; tokens of the last id
+def test_runs_around_the_lengths_that_are_cut(stride, fill, d, ob, cuda):
+    """Ids of 1 to 300 tokens, around 40 (the longest added in line) and multiples
+    of 32 (the pieces of longer ones), at every start within a piece: up to 40
+    tokens the sum is in token order, to the bit, wherever the run lies."""
+    n = len(COUNTS)
+    vocab = (n + 1) * stride + 1
+    for lead in (0, 1, 8, 23, 31, 32):
+        g = torch.Generator(device="cuda").manual_seed(lead + d)
+        counts = [lead] + COUNTS + [fill]
+        ids = torch.cat([torch.full((c,), min(i * stride, vocab - 1), dtype=torch.int32) for i, c in enumerate(counts)])
+        ids = torch.cat([ids, torch.tensor([-1, vocab], dtype=torch.int32)]).cuda()
+        ids = ids[torch.randperm(ids.numel(), generator=g, device="cuda")].contiguous()
+        dout = torch.randn(ids.numel(), d, generator=g, device="cuda").to(T[ob])
+        dtable = torch.full((vocab, d), GUARD, device="cuda")
+        _bwd(ids, dout, vocab, d, 1.25, dtable, _ws(ids.numel(), vocab, d))
+        torch.cuda.synchronize()
+        _check_grad(ids, dout, vocab, 1.25, dtable)
+        short = torch.bincount(ids[(ids >= 0) & (ids < vocab)].long(), minlength=vocab) <= 40
+        assert torch.equal(dtable[short], _in_token_order(ids, dout, vocab, 1.25, 40)[short]), f"lead {lead}"

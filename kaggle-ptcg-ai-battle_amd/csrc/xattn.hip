@@ -23,9 +23,10 @@
 // row-major LDS by ds_read_b64_tr_b16 (4 keys of 16 columns to a lane's 4
 // values).
 // fp32 operands are split into three bf16 terms (x = x0 + x1 + x2, 8 bits each,
-// exact above 2^-102) that lie in LDS as three planes; a product is the six
-// term products down to 2^-26 of it, small ones first: 6 / 16 of the time of
-// v_mfma_f32_32x32x2_f32.  An infinite operand becomes NaN in the products.
+// exact above 2^-102) that lie in LDS as three planes; a product is six term
+// products, small ones first: 6 / 16 of the time of v_mfma_f32_32x32x2_f32.
+// With |x1| <= 2^-8 |x| and |x2| <= 2^-17 |x|, the three left out (x1 y2, x2 y1,
+// x2 y2) come to 2^-24 |x y| at most, one rounding of fp32.  An infinite operand becomes NaN in the products.
 #include "rowbuf.h"
 #include "../../include/ptcg_amd_kernels.h"
 
@@ -266,7 +267,7 @@ __device__ __forceinline__ floatx16 mma_rows_lds(const __bf16* xs, const __bf16*
 
 // c += X^T P over 32 LDS rows of X: c[dt] is columns 32 dt .. of X; P's register
 // r stands for row 8 (r / 4) + 4 h + r % 4.  bf16: P is rounded to bf16 for the
-// product (relative 2^-9 each, as the stored operands are); its fp32 values make
+// product (by up to 2^-8 of each, as the stored operands are); its fp32 values make
 // the softmax's sum.  Gradients are then off by 2.3e-3 to 2.5e-3 (relative L2),
 // where rounding an exact one to bf16 gives 1.65e-3; a second term of P for
 // samples of up to 64 keys took 1% off that and cost 12% (8 192 x 64 x 97: 277 us
@@ -725,7 +726,7 @@ __global__ __launch_bounds__(JOIN_NTH) void xattn_join_kernel(const XArgs a, con
 // --------------------------------------------------------------- backward
 // dQ: the forward's shape.  Per 32 keys S^T and dP^T = V dO^T with queries on
 // lanes, dS^T in registers, dQ^T += K^T dS^T.  Also leaves D_i (from the
-// stored o: in bf16 its rounding moves D by 2^-9 of terms that average out)
+// stored o: in bf16 its rounding moves D by up to 2^-8 of terms that average out)
 // for the dK / dV kernel, in row order of lse.
 template <typename T, int DH, int NW, int KS, int KT> struct DqCfg {
     static constexpr int NTH = 64 * NW * KS, BQ = 32 * NW, BK = KT * KS;

@@ -229,7 +229,8 @@ int ptcg_kernel_attention_path(int L, int Dh);
  * keep[keep_sn sample + row], packed at keep[row].  NULL each: all rows, all
  * kept.  Masked rows may hold anything, NaN too; their dk and dv are zeros.
  * Rows outside every packed sample stay as they were, in lse too.
- * A query that keeps no key gives out = 0, lse = -inf and no gradient.
+ * A query that keeps no key gives out = 0, lse = -inf and no gradient; so does a
+ * finite one whose kept scores are all -inf.
  * bf16: products of bf16 operands (P and dS rounded to bf16 for them),
  * softmax, statistics and sums fp32.  fp32: operands as three bf16 terms, so an
  * infinity among them becomes NaN.                                          */

@@ -9,7 +9,8 @@
 //   dv_j = sum_i P_ij do_i,  dS_ij = P_ij (do_i . v_j - D_i),
 //   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,
 // dk and dv summed over the query heads that share the kv head, in row order.
-// A query that keeps no key: o = 0, lse = -inf, and it adds to no gradient.
+// A query that keeps no key, or whose kept scores are all -inf: o = 0, lse =
+// -inf, and it adds to no gradient.
 //
 // Layout.  The G = heads / kv_heads query heads of a kv head are one matrix of
 // lq * G rows (row r is query r / G, head r % G), so a single token's heads
@@ -316,7 +317,7 @@ template <typename T, int DH, bool PAD, int BR, int NTH> struct Stage {
         for (int i = 0; i < NCH; ++i) r[i].load(rs, off + i * (RPP * ld));
     }
     // rows of the flattened query matrix of kv head kvh, from row0; the last
-    // row stands in for rows past it (zeroed on the way into LDS)
+    // row stands in for rows past it
     __device__ __forceinline__ void load_q(const XArgs& a, const PtcgHeadLayout& l, const T* base, int kvh, int row0,
                                            int len, int tid) {
         const int col = min(tid % CPR * 8, a.dh - 8);
@@ -337,7 +338,7 @@ template <typename T, int DH, bool PAD, int BR, int NTH> struct Stage {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) put(s, tid, i, true);
     }
-    // rows below `rows`, columns below dh
+    // rows below `rows`, columns below dh; zeros besides
     __device__ __forceinline__ void store_q(__bf16* s, int tid, int rows, int dh) const {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) put(s, tid, i, tid / CPR + i * RPP < rows && tid % CPR * 8 < dh);
@@ -655,8 +656,9 @@ __global__ __launch_bounds__(64 * NW * KS, (min_waves<T, DH>())) void xattn_fwd_
         }
         return;
     }
-    // no key kept: no tile was read and the sum is 0 (scores of NaN leave the
-    // maximum at -inf too, but a sum of NaN), whatever the query holds
+    // no key kept, or every kept score -inf: the sum is 0 (scores of NaN leave the
+    // maximum at -inf too, but a sum of NaN); with no key kept no tile was read,
+    // whatever the query holds
     const bool none = m2 == -INFINITY && l == 0.f;
     if (none) {
 #pragma unroll
@@ -969,7 +971,10 @@ __device__ __forceinline__ void dkv_body(const XArgs& a, const Grads<T>& g, cons
         }
     };
     auto store = [&](__bf16* Qs, float* ls) {
-        qs_.store_q(Qs, tid, rown, a.dh);
+        // Past the end q's last row stays, which the log-sum-exp of +inf below takes
+        // out: its scores are infinite only where the row's own are, where zeros
+        // against a key of -inf would make NaN of that key's gradients.
+        qs_.store_q(Qs, tid, C::BQ, a.dh);
         ds_.store_q(Qs + C::TILE, tid, rown, a.dh);
         if (tid < C::BQ) {
             // exp2(s - inf) = 0: rows past the end, and rows that keep no key, add nothing

@@ -372,3 +372,76 @@ def test_gradients_against_differences(cuda):
         want = float((grad * d.double()).sum())
         tol = abs(diff[2.0 ** -5] - diff[2.0 ** -6]) + 4 * noise / 2.0 ** -6
         assert abs(want - diff[2.0 ** -6]) <= tol, (name, want, diff, tol)
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("lq,lk,H,KV,dh", [(1, 2100, 4, 2, 64), (37, 70, 4, 2, 40), (150, 90, 6, 2, 128), (64, 97, 4, 4, 64),
+                                           (20, 700, 8, 1, 96)])
+@pytest.mark.parametrize("packed", ["", "q", "k", "qk"])
+def test_every_tensor_in_a_layout_of_its_own(packed, lq, lk, H, KV, dh, bf16, cuda):
+    """q and k as rows of heads, out (with dout) and v (with dv) as heads of rows
+    with a gap between them, queries and keys packed or padded on their own."""
+    n = 3
+    kw = dict(q_len=[lq, lq // 2, 1]) if "q" in packed else {}
+    if "k" in packed:
+        kw["k_off_len"] = [lk // 3, lk, 2]
+    op = Op(n, lq, lk, H, KV, dh, bf16, slack=2, seed=lq + lk, **kw)
+    if "k" in packed:
+        op.keep = (torch.rand(op.kr, generator=op.g, device="cuda") < 0.7).float()
+    else:
+        op.keep = _holes(n, lk, 7)
+    op.a.keep = op.keep.data_ptr()
+
+    def turned(x, per, heads):
+        """x (rows, heads, dh) in a new memory of (sample, head, row, dh + 8); its strides, and the way back."""
+        m = torch.full((x.shape[0] // per, heads, per, dh + 8), GUARD, dtype=x.dtype, device="cuda")
+        m[..., :dh] = x.view(-1, per, heads, dh).transpose(1, 2)
+        return m, native.CPtcgHeadLayout(heads * per * (dh + 8), dh + 8, per * (dh + 8)), \
+            lambda: m[..., :dh].transpose(1, 2).reshape(x.shape)
+
+    qper, kper = (op.qr if "q" in packed else lq), (op.kr if "k" in packed else lk)
+    flat = dict(do=op.do, v=op.v)
+    op.out, op.a.o, out = turned(op.out, qper, H)
+    op.do = turned(op.do, qper, H)[0]
+    op.v, op.a.v, _ = turned(op.v, kper, KV)
+    op.dv, _, dv = turned(op.dv, kper, KV)
+    op.fwd()
+    op.bwd()
+    torch.cuda.synchronize()
+    for m in (op.out, op.dv):
+        assert (m[..., dh:] == GUARD).all()
+    op.out, op.dv = out(), dv()
+    op.do, op.v = flat["do"], flat["v"]
+    op.check()
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("lq,lk", [(1, 3000), (5, 40), (70, 97), (130, 300)])
+@pytest.mark.parametrize("name", ["k", "v"])
+def test_one_row_for_all_keys_in_the_forward(name, lq, lk, bf16, cuda):
+    """A row stride of 0: every key reads the same row, masked ones aside."""
+    op = Op(2, lq, lk, 4, 2, 64, bf16, keep=_holes(2, lk, 11), seed=8)
+    x = getattr(op, name)
+    x.view(2, lk, -1)[:] = x.view(2, lk, -1)[:, :1].clone()
+    lay = native.CPtcgHeadLayout(lk * 2 * 64, 0, 64)
+    setattr(op.a, name, lay)
+    op.fwd()
+    op.check(bwd=False)
+
+
+@pytest.mark.parametrize("lq,lk", [(1, 2000), (40, 97), (130, 300)])
+def test_bf16_rows_whose_every_kept_score_is_minus_infinity(lq, lk, cuda):
+    """They count as rows that keep no key; a finite score beside the infinite
+    ones gets the whole weight."""
+    op = Op(2, lq, lk, 2, 2, 32, 1, keep=_holes(2, lk, 12), seed=9)
+    op.q.abs_()
+    op.q += 0.125
+    op.k[:, :, 5] = -math.inf
+    j = int(op.keep[1].nonzero()[0, 0])
+    op.k[lk + j] = 0.5
+    op.fwd()
+    op.bwd()
+    torch.cuda.synchronize()
+    assert (op.out[:lq] == 0).all() and (op.lse[0] == -math.inf).all() and (op.dq[:lq] == 0).all()
+    assert (op.dk[:lk] == 0).all() and (op.dv[:lk] == 0).all()
+    assert torch.equal(op.out[lq:], op.v[lk + j].expand(lq, 2, 32)) and op.lse[1].isfinite().all()

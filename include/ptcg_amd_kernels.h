@@ -300,6 +300,8 @@ int ptcg_kernel_embedding_bwd(const int32_t* ids, int64_t rows, const void* dout
  * (nullable), fp32, overwritten, summed in a fixed order; dY (rows, out) fp32
  * (split into three bf16 terms: fp32 products; an infinity becomes NaN) or bf16;
  * workspace of _dw_ws_bytes (0: none, -1: refused), 16 B aligned.
+ * Refused: rows * ceil(d / 32) of 2^30 or more; in dw row strides of 2^23 or more
+ * and in * out of 2^36 or more.
  * No reference counterpart: it keeps activations in fp32 or bf16.            */
 int ptcg_kernel_ckpt8_pack(const void* x, int64_t ldx, int bf16, int rows, int d, uint8_t* q, int64_t ldq,
                            uint8_t* scales, int64_t lds, void* stream);

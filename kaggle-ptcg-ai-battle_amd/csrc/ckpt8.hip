@@ -517,7 +517,8 @@ int cu_count() {
 // step) gains 14% of the products and costs another 33 MB of partials: from
 // rows * in * out = 4e10 on (65 539 x 4 096 x 1 024: 537 us against 625;
 // 20 000 x 1 024 x 1 024: 70 against 63).  In fp32 its accumulators leave too
-// few registers for the three terms.  At least 4 steps a split.
+// few registers for the three terms; in bf16, rows that are no whole dwords make it
+// spill 38 a lane.  At least 4 steps a split.
 struct DwPlan { int big_m, big_n, tm, tn, splits, chunk; long pstride; };
 DwPlan dw_plan(int rows, int k, int n, int bf16) {
     DwPlan p;

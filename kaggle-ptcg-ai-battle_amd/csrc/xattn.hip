@@ -489,7 +489,10 @@ template <typename T, int DH, int NW, int KS, int KT> struct FwdCfg {
 // let one wave's softmax run beside the other's products.
 template <typename T, int DH> constexpr int min_waves() { return sizeof(T) == 2 || DH <= 64 ? 2 : 1; }
 // the backward holds two operands' rows; with a tile four times a wave's part
-// (SPLIT waves along it) also on its way, one wave's registers
+// (SPLIT waves along it) also on its way, one wave's registers.  Some spill all
+// the same (registers a lane, by the compiler): the joint backward in fp32 64 wide
+// 12 to 41, dk and dv in fp32 64 wide 2 to 29 and 128 wide up to 59, in bf16 128
+// wide with two waves along the keys 24 and 68.
 template <typename T, int DH, int SPLIT> constexpr int bwd_waves() {
     return DH * planes<T>() <= 64 || (SPLIT <= 2 && min_waves<T, DH>() == 2) ? 2 : 1;
 }

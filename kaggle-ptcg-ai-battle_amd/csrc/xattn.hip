@@ -1303,6 +1303,7 @@ bool layout_ok(const PtcgHeadLayout& l, int e) {
 // row stride, or else two rows, the fewest that a batch of more than one row may
 // hold, within the head stride.
 bool layout_apart(const PtcgHeadLayout& l, bool packed, int n, int rows, int heads, int dh) {
+    if (n <= 0 || rows <= 0) return true;       // no element
     if (packed) {
         const bool many = n > 1 || rows > 1;
         if (heads <= 1) return !many || l.sl >= dh;

@@ -445,3 +445,15 @@ def test_bf16_rows_whose_every_kept_score_is_minus_infinity(lq, lk, cuda):
     assert (op.out[:lq] == 0).all() and (op.lse[0] == -math.inf).all() and (op.dq[:lq] == 0).all()
     assert (op.dk[:lk] == 0).all() and (op.dv[:lk] == 0).all()
     assert torch.equal(op.out[lq:], op.v[lk + j].expand(lq, 2, 32)) and op.lse[1].isfinite().all()
+
+
+@pytest.mark.parametrize("bf16", [0, 1])
+@pytest.mark.parametrize("lq,lk", [(5, 0), (300, 0), (0, 70), (0, 1)])
+def test_no_keys_and_no_queries(lq, lk, bf16, cuda):
+    """Without keys: out and dq of zeros, lse = -inf; without queries: dk and dv of zeros."""
+    op = Op(2, lq, lk, 4, 2, 40, bf16)
+    op.fwd()
+    op.bwd()
+    torch.cuda.synchronize()
+    assert (op.out == 0).all() and (op.dq == 0).all() and (op.lse == -math.inf).all()
+    assert (op.dk == 0).all() and (op.dv == 0).all()

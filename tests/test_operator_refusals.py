@@ -247,3 +247,11 @@ def test_a_lone_row_takes_any_row_stride_and_a_lone_head_any_head_stride():
         _fwd(_desc(n=1, lq=1, lk=100000, q_off=P, k_off=P, o=LAY(sn=0, sl=0, sh=32)))
     with pytest.raises(native.PtcgError, match="workspace"):
         _fwd(_desc(n=1, lq=3, lk=100000, heads=1, kv_heads=1, q_off=P, k_off=P, o=LAY(sn=0, sl=32, sh=0)))
+
+
+@pytest.mark.parametrize("kw", [dict(lk=0, k=LAY(sn=0, sl=64, sh=32), v=LAY(sn=0, sl=64, sh=32)),
+                                dict(lk=0, k_off=P, k=LAY(sn=0, sl=0, sh=0), v=LAY(sn=0, sl=0, sh=0))])
+def test_gradients_of_no_rows_need_no_layout(kw):
+    """Dense tensors of no keys have a sample stride of 0."""
+    with pytest.raises(native.PtcgError, match="workspace"):
+        _bwd(_desc(**kw), nb=4)

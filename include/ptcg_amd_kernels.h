@@ -315,6 +315,101 @@ int ptcg_kernel_ckpt8_dw(int rows, int in, int out, const void* dY, int64_t lddy
                          int64_t ldq, const uint8_t* scales, int64_t lds, float* dW, float* db, void* workspace,
                          int64_t workspace_bytes, void* stream);
 
+/* Self attention along time: positions, a cache of pages, a causal window.
+ *
+ * Rotation of a head's first `rot` elements (even, 0 to dh; 0: none) to
+ * position p: the pair (a, b) of index i becomes (a c - b s, a s + b c), c =
+ * mag cos(p freq[i]), s = mag sin(p freq[i]).  Pairs are elements (i, i + rot /
+ * 2), or (2 i, 2 i + 1) where interleaved = 1.  freq (device, rot / 2 doubles):
+ * radians per position; products with the position and the reduction are 64 bit,
+ * so far positions lose nothing.  pos (device, one int per row of the matrices):
+ * NULL: the row's index in its sample; in ptcg_kernel_paged_append its place in
+ * its sequence.                                                             */
+typedef struct PtcgRope {
+    int rot, interleaved;
+    float mag;
+    const double* freq;
+    const int32_t* pos;
+} PtcgRope;
+/* freq (host, rot / 2) and mag of base^(-2 i / rot), and of three ways to longer
+ * contexts than the `length` positions trained on, by `factor` >= 1.  scaling: 0
+ * none; 1 positions divided by factor; 2 the base times factor^(rot / (rot - 2));
+ * 3 by parts (Peng, Quesnelle, Fan, Shippole, "YaRN", 2023): pairs of more than
+ * `fast` turns over length kept, of fewer than `slow` divided by factor, linear
+ * in the turns between, mag = 0.1 ln(factor) + 1 (1 in the others).  Host only.
+ * No reference counterpart.                                                 */
+int ptcg_rope_frequencies(int rot, double base, int scaling, double factor, double length, double fast, double slow,
+                          double* freq, float* mag);
+
+/* Norms of queries and keys for each head, then the rotation, in one pass:
+ * y = R(p) (x w / sqrt(mean x^2 + eps)) over a head's dh elements (even, 2 to
+ * 128), w = wq or wk (dh floats; NULL: no norm, R(p) x).  n samples of l rows;
+ * element (sample, row, head, e) of q lies at q[sn sample + sl row + sh head + e],
+ * the same for k (kv_heads heads, 0 for none), qo, ko; any strides >= 0 of the
+ * inputs.  fp32, or bf16 (bf16 = 1; sums, norms and angles fp32 or more, one
+ * rounding at the end).  fwd: qo may be q and ko k, with their layouts.
+ * bwd: gradients dqo, dko (laid out as qo, ko) of the outputs to dq, dk (as q,
+ * k), dwq, dwk (dh floats, where there is a norm; both NULL: not made), all
+ * overwritten, sums in a fixed order.  Without a norm q or k is not read (may be
+ * NULL).  workspace of _bwd_ws_bytes (0: none, -1: refused), 16 B aligned; calls
+ * that may run at the same time need scratch of their own.  Outputs overlap no
+ * input besides the in-place forward, and no two of an output's elements share
+ * an address.
+ * No reference counterpart: its trunk has no positions and one norm a row.  */
+typedef struct PtcgQkRope {
+    int n, l, heads, kv_heads, dh;
+    int bf16;
+    float eps;
+    PtcgHeadLayout q, k, qo, ko;
+    const float *wq, *wk;
+    PtcgRope rope;
+} PtcgQkRope;
+int ptcg_kernel_qk_norm_rope_fwd(const PtcgQkRope* desc, const void* q, const void* k, void* qo, void* ko,
+                                 void* stream);
+int64_t ptcg_kernel_qk_norm_rope_bwd_ws_bytes(const PtcgQkRope* desc);
+int ptcg_kernel_qk_norm_rope_bwd(const PtcgQkRope* desc, const void* q, const void* k, const void* dqo,
+                                 const void* dko, void* dq, void* dk, float* dwq, float* dwk, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
+/* Keys and values of sequences in a pool of `pages` pages of `page` rows each (any
+ * number).  Position p of sequence i lies in row p % page of page
+ * table[table_sn i + p / page] (device ints, per_seq entries a sequence); element
+ * (page, row, kv head, e) of the keys at kp[k.sn page + k.sl row + k.sh head + e],
+ * the same for vp with v.  Sequences may share pages that are only read.  An
+ * entry outside [0, pages) is no page: nothing is written there, and its keys
+ * are masked (pages behind a window may be given back).                      */
+typedef struct PtcgPages {
+    int pages, page, per_seq;
+    PtcgHeadLayout k, v;
+    void *kp, *vp;
+    const int32_t* table;
+    int64_t table_sn;
+} PtcgPages;
+
+/* Appends new rows to the cache: k normed (wk) and rotated, v as it is, and qo =
+ * q normed (wq) and rotated for the attention that follows (q, qo NULL: not made).
+ * Norms and rotation as ptcg_kernel_qk_norm_rope_fwd.  n sequences of lq new rows
+ * each, or packed (q_off, device, n + 1 ascending ints): sequence i owns rows
+ * q_off[i] .. q_off[i + 1] - 1, at most lq of them, of matrices of `rows` rows (sn
+ * unused; rows outside every sequence are neither read nor written).  len
+ * (device, n ints): the sequences' lengths with their new rows, so new row j of
+ * m has place len - m + j; rows of places below 0 or past the table are not
+ * written (their qo is).  A page that new rows lie in belongs to one sequence.
+ * q, k, v and the pool of one type.  qo may be q, with its layout.
+ * No reference counterpart.                                                 */
+typedef struct PtcgPagedAppend {
+    int n, lq, rows, heads, kv_heads, dh;
+    int bf16;
+    float eps;
+    PtcgHeadLayout q, k, v, qo;
+    const int32_t *q_off, *len;
+    const float *wq, *wk;
+    PtcgRope rope;
+    PtcgPages cache;
+} PtcgPagedAppend;
+int ptcg_kernel_paged_append(const PtcgPagedAppend* desc, const void* q, const void* k, const void* v, void* qo,
+                             void* stream);
+
 /* Launch timing: between begin and end, every GEMM, LayerNorm and Adam
  * launch (up to max_launches in all) is bracketed by a HIP event pair on its
  * own stream.  end waits for the events and returns the GEMM launches'

@@ -361,6 +361,19 @@ bool layout_apart(const PtcgHeadLayout& l, bool packed, int n, int rows, int hea
     return true;
 }
 
+// A pool of pages and its table; strides multiples of e elements.
+int check_pages(const PtcgPages& g, int n, int kv_heads, int dh, int e, const char* who) {
+    PT_REQUIRE(g.pages >= 0 && g.page >= 1 && g.per_seq >= 0, "%s: %d pages of %d rows, %d a sequence", who, g.pages,
+               g.page, g.per_seq);
+    PT_REQUIRE((int64_t)g.page * g.per_seq < (1LL << 30), "%s: sequences of 2^30 rows or more", who);
+    PT_REQUIRE(n <= 1 || g.table_sn >= g.per_seq, "%s: page tables overlap", who);
+    PT_REQUIRE(layout_ok(g.k, e) && layout_ok(g.v, e), "%s: page strides must be non-negative multiples of %d elements",
+               who, e);
+    PT_REQUIRE(n == 0 || g.per_seq == 0 || g.table, "%s: no page table", who);
+    PT_REQUIRE(g.pages == 0 || (g.kp && g.vp), "%s: no pool", who);
+    return PTCG_OK;
+}
+
 bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename K> int lds_attr(K kernel, size_t bytes) {

@@ -47,6 +47,33 @@ class CPtcgCrossAttn(ctypes.Structure):
         [(n, c_void_p) for n in ("q_off", "k_off", "k_len", "keep")] + [("keep_sn", ctypes.c_int64)]
 
 
+class CPtcgRope(ctypes.Structure):
+    """struct PtcgRope of include/ptcg_amd_kernels.h."""
+    _fields_ = [("rot", ctypes.c_int), ("interleaved", ctypes.c_int), ("mag", ctypes.c_float), ("freq", c_void_p),
+                ("pos", c_void_p)]
+
+
+class CPtcgQkRope(ctypes.Structure):
+    """struct PtcgQkRope of include/ptcg_amd_kernels.h."""
+    _fields_ = [(n, ctypes.c_int) for n in ("n", "l", "heads", "kv_heads", "dh", "bf16")] + \
+        [("eps", ctypes.c_float)] + [(n, CPtcgHeadLayout) for n in ("q", "k", "qo", "ko")] + \
+        [("wq", c_void_p), ("wk", c_void_p), ("rope", CPtcgRope)]
+
+
+class CPtcgPages(ctypes.Structure):
+    """struct PtcgPages of include/ptcg_amd_kernels.h."""
+    _fields_ = [(n, ctypes.c_int) for n in ("pages", "page", "per_seq")] + \
+        [(n, CPtcgHeadLayout) for n in ("k", "v")] + [(n, c_void_p) for n in ("kp", "vp", "table")] + \
+        [("table_sn", ctypes.c_int64)]
+
+
+class CPtcgPagedAppend(ctypes.Structure):
+    """struct PtcgPagedAppend of include/ptcg_amd_kernels.h."""
+    _fields_ = [(n, ctypes.c_int) for n in ("n", "lq", "rows", "heads", "kv_heads", "dh", "bf16")] + \
+        [("eps", ctypes.c_float)] + [(n, CPtcgHeadLayout) for n in ("q", "k", "v", "qo")] + \
+        [(n, c_void_p) for n in ("q_off", "len", "wq", "wk")] + [("rope", CPtcgRope), ("cache", CPtcgPages)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "ptcg_last_error": (ctypes.c_char_p, []),
@@ -306,6 +333,13 @@ _SIGS = {
     "ptcg_kernel_ckpt8_dw": (ctypes.c_int, [
         ctypes.c_int, ctypes.c_int, ctypes.c_int, c_void_p, ctypes.c_int64, ctypes.c_int, c_void_p, ctypes.c_int64,
         c_void_p, ctypes.c_int64, c_void_p, c_void_p, c_void_p, ctypes.c_int64, c_void_p]),
+    "ptcg_rope_frequencies": (ctypes.c_int, [ctypes.c_int, ctypes.c_double, ctypes.c_int] + [ctypes.c_double] * 4
+                              + [ctypes.POINTER(ctypes.c_double), c_float_p]),
+    "ptcg_kernel_qk_norm_rope_fwd": (ctypes.c_int, [ctypes.POINTER(CPtcgQkRope)] + [c_void_p] * 5),
+    "ptcg_kernel_qk_norm_rope_bwd_ws_bytes": (ctypes.c_int64, [ctypes.POINTER(CPtcgQkRope)]),
+    "ptcg_kernel_qk_norm_rope_bwd": (ctypes.c_int, [ctypes.POINTER(CPtcgQkRope)] + [c_void_p] * 9
+                                     + [ctypes.c_int64, c_void_p]),
+    "ptcg_kernel_paged_append": (ctypes.c_int, [ctypes.POINTER(CPtcgPagedAppend)] + [c_void_p] * 5),
 }
 
 _lib = None

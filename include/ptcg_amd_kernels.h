@@ -410,6 +410,61 @@ typedef struct PtcgPagedAppend {
 int ptcg_kernel_paged_append(const PtcgPagedAppend* desc, const void* q, const void* k, const void* v, void* qo,
                              void* stream);
 
+/* Attention of new rows over a cache of pages: a chunk of each sequence's last
+ * rows, a single token being a chunk of one.  Rows as in ptcg_kernel_paged_append (n
+ * sequences of lq, or packed by q_off within `rows`; len the lengths with the new
+ * rows, whose keys and values are in the cache already).  The row of place p sees
+ * the keys j <= p of its sequence that lie within the window, j > p - window
+ * (window = 0: all), or among the first `sinks`.  Out as PtcgCrossAttn's: query
+ * head h reads kv head h / (heads / kv_heads), dh a multiple of 8 up to 128,
+ * strides multiples of 16 bytes, buffers 16 B aligned.  lse (nullable) (n, heads,
+ * lq) fp32.  A row that sees no key (a place below 0, no pages) gives out = 0, lse =
+ * -inf.  Rows outside every sequence stay as they were.  What unseen places of
+ * the pool hold reaches nothing; NaN and infinities among a call's own new keys and
+ * values may reach rows of that sequence before them.
+ * workspace of _ws_bytes (0: none, -1: refused), 16 B aligned, any contents; calls
+ * that may run at the same time need scratch of their own.
+ * No reference counterpart: its policy has no memory.                       */
+typedef struct PtcgPagedAttn {
+    int n, lq, rows, heads, kv_heads, dh;
+    int bf16;      /* element type of q, out and the pool: 0 fp32, 1 bf16 */
+    float scale;   /* of the scores, positive */
+    int window, sinks;
+    PtcgHeadLayout q, o;
+    const int32_t *q_off, *len;
+    PtcgPages cache;
+} PtcgPagedAttn;
+int64_t ptcg_kernel_paged_attention_ws_bytes(const PtcgPagedAttn* desc);
+int ptcg_kernel_paged_attention(const PtcgPagedAttn* desc, const void* q, void* out, float* lse, void* workspace,
+                                int64_t workspace_bytes, void* stream);
+
+/* The same attention over whole sequences, with its gradient, for training: n
+ * sequences of l rows (len, device, n ints, nullable: rows past len[i] neither
+ * see nor are seen: out = 0, lse = -inf, no gradient, whatever they hold), or packed (off,
+ * device, n + 1 ascending ints: sequence i owns rows off[i] .. off[i + 1] - 1, at
+ * most l of them; rows outside every sequence stay as they were).  The row of place p
+ * sees the keys j <= p with j > p - window (window = 0: all) or j < sinks.  Types,
+ * heads, strides, broadcasts and layouts of gradients as PtcgCrossAttn.  NaN and
+ * infinities may reach other rows of their sequence.  dk and dv are summed over the
+ * heads that share them, every sum in a fixed order: equal calls give equal bits.
+ * lse (n, heads, l) fp32 (nullable in the forward).  workspace of _ws_bytes (backward =
+ * 0 / 1; 0: none, -1: refused), 16 B aligned, any contents.
+ * No reference counterpart: its trunk attends in both directions.           */
+typedef struct PtcgWindowAttn {
+    int n, l, heads, kv_heads, dh;
+    int bf16;
+    float scale;
+    int window, sinks;
+    PtcgHeadLayout q, k, v, o;
+    const int32_t *off, *len;
+} PtcgWindowAttn;
+int64_t ptcg_kernel_window_attention_ws_bytes(const PtcgWindowAttn* desc, int backward);
+int ptcg_kernel_window_attention_fwd(const PtcgWindowAttn* desc, const void* q, const void* k, const void* v, void* out,
+                                     float* lse, void* workspace, int64_t workspace_bytes, void* stream);
+int ptcg_kernel_window_attention_bwd(const PtcgWindowAttn* desc, const void* q, const void* k, const void* v,
+                                     const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                                     void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Launch timing: between begin and end, every GEMM, LayerNorm and Adam
  * launch (up to max_launches in all) is bracketed by a HIP event pair on its
  * own stream.  end waits for the events and returns the GEMM launches'

@@ -1,0 +1,892 @@
+// Causal attention along time, with a window and a few first tokens that stay
+// visible: new rows over a cache of pages (chunks and single tokens), and whole
+// sequences with their gradient.
+//
+// Row i of place p_i sees the keys j <= p_i with p_i - j < window or j < sinks:
+//   s_ij = scale q_i . k_j,  m_i = max_j s_ij,  l_i = sum_j exp(s_ij - m_i),
+//   o_i = sum_j exp(s_ij - m_i) v_j / l_i,  lse_i = m_i + log l_i,
+// in one pass over the keys that any row of a tile sees: tiles of the first tokens,
+// then tiles from the first row's window on to the last row's place.
+// A row that sees no key, or whose seen scores are all -inf: o = 0, lse = -inf.
+//
+// Rows, fragments and products as in the attention to other states (attn_tiles.h):
+// the G = heads / kv_heads query heads of a kv head are one matrix of rows, query r
+// / G and head r % G of row r; S^T = K Q^T leaves a query on a lane and its
+// scores in registers, which are an operand of O^T = V^T P^T as they are.
+#include "attn_tiles.h"
+
+#include <limits.h>
+
+namespace {
+
+// the descriptors as the kernels take them
+struct SArgs {
+    int n, lq, H, KV, G, dh;
+    unsigned gmagic;              // head_div
+    float scale, scale2;          // scale2 = scale * log2(e): exponentials are exp2
+    int window, sinks;            // window: INT_MAX where there is none
+    PtcgHeadLayout q, k, v, o;    // k, v: rows of sequences, or of pages
+    const int *q_off, *len;
+    // pages
+    const int* table;
+    long table_sn;
+    int pages, page, per_seq;
+    int all_rows;                 // rows of the packed matrices
+    double inv_page;
+};
+
+// A sequence: element offsets of row 0, its live rows, the rows that are written (a
+// padded one's dead rows too), its keys, and the place of row 0.
+struct Seq { long q, o, k, v; const int* table; int ql, rows, kl, p0; };
+
+// Counts come from device memory: they are held to the host's bounds.
+template <bool PAGED> __device__ __forceinline__ Seq seq_of(const SArgs& a, int i) {
+    Seq s = {};
+    s.ql = s.rows = a.lq;
+    if (a.q_off) {
+        const int r0 = a.q_off[i];
+        s.ql = s.rows = max(0, min(a.lq, min(a.q_off[i + 1], a.all_rows) - r0));
+        s.q = r0 * a.q.sl; s.o = r0 * a.o.sl;
+        if constexpr (!PAGED) { s.k = r0 * a.k.sl; s.v = r0 * a.v.sl; }
+    } else {
+        s.q = i * a.q.sn; s.o = i * a.o.sn;
+        if constexpr (!PAGED) {
+            s.k = i * a.k.sn; s.v = i * a.v.sn;
+            if (a.len) s.ql = max(0, min(a.lq, a.len[i]));
+        }
+    }
+    s.kl = s.ql;
+    if constexpr (PAGED) {
+        const int n = max(0, a.len[i]);
+        s.p0 = n - s.ql;
+        s.kl = min(n, a.per_seq * a.page);
+        s.table = a.table + i * a.table_sn;
+    }
+    return s;
+}
+
+// Key blocks (of BK keys) that rows of places plo .. phi see: the first hb, then
+// nt - hb from block tw on; keys from kend on are seen by none of them.
+struct Range {
+    int hb, tw, nt, kend;
+    __device__ __forceinline__ int block(int t) const { return t < hb ? t : tw + t - hb; }
+};
+template <int BK> __device__ __forceinline__ Range range_of(const SArgs& a, int plo, int phi, int kl) {
+    Range r = {0, 0, 0, 0};
+    r.kend = min(phi + 1, kl);
+    if (r.kend <= 0) return r;
+    const int te = (r.kend + BK - 1) / BK;
+    r.tw = min(max(0, max(plo, 0) - a.window + 1) / BK, te);
+    r.hb = min((min(a.sinks, r.kend) + BK - 1) / BK, r.tw);
+    r.nt = r.hb + te - r.tw;
+    return r;
+}
+// places of the live rows among flattened rows r0 .. r1 - 1; none: hi < 0
+struct Places { int lo, hi; };
+__device__ __forceinline__ Places places_of(const SArgs& a, const Seq& s, int r0, int r1) {
+    const int q0 = head_div(a, r0), q1 = min(head_div(a, r1 - 1), s.ql - 1);
+    return {s.p0 + q0, q1 < q0 ? -1 : s.p0 + q1};
+}
+
+// What a workgroup works on: sequence, row tile, split of the tile's key blocks
+// (per of them), and the sequence's splits and first slot.
+struct Work { int i, qt, sp, per, splits, first; };
+
+// Slots are handed out on the device, which alone knows the lengths: sequence i has
+// T_i row tiles of at most K_i key blocks; a split takes so many blocks that sum T_i
+// ceil(K_i / per) <= slots, so that every workgroup has one piece of nearly equal
+// length however the sequences differ.  Every wave counts for itself, 64
+// sequences at a time.  by_tile: slot counts tiles, not splits.  i = -1: a slot too many.
+template <bool PAGED, int BQ, int BK>
+__device__ __forceinline__ Work work_of(const SArgs& a, int slot, int slots, int least, bool split, bool by_tile) {
+    const int lane = threadIdx.x & 63;
+    auto shape = [&](int i, int& t, int& k) {
+        t = k = 0;
+        if (i >= a.n) return;
+        const Seq s = seq_of<PAGED>(a, i);
+        t = (s.rows * a.G + BQ - 1) / BQ;
+        const Places p = {s.p0, s.p0 + s.ql - 1};
+        // the blocks of all rows, and of a tile of rows in a window
+        k = range_of<BK>(a, p.lo, p.hi, s.kl).nt;
+        if (a.window < INT_MAX - 4 * BQ)
+            k = min(k, (a.window + (BQ + a.G - 2) / a.G) / BK + 2 + (min(a.sinks, s.kl) + BK - 1) / BK);
+    };
+    int per = INT_MAX;
+    if (split) {
+        int st = 0;
+        float sk = 0.f;      // counts of blocks: only a length that need not be exact comes of them
+        for (int i0 = 0; i0 < a.n; i0 += 64) {
+            int t, k;
+            shape(i0 + lane, t, k);
+            st += t;
+            sk += (float)t * (float)k;
+        }
+        for (int o = 1; o < 64; o <<= 1) {
+            st += __shfl_xor(st, o, 64);
+            sk += __shfl_xor(sk, o, 64);
+        }
+        if (slots > st) per = max(least, (int)fminf(sk * 1.0001f / (float)(slots - st) + 1.f, 1e9f));
+    }
+    int before = 0, pieces = 0;
+    for (int i0 = 0; i0 < a.n; i0 += 64) {
+        int t, k;
+        shape(i0 + lane, t, k);
+        const int s = max(1, (k - 1) / per + 1), c = by_tile ? t : t * s;
+        int to = c, pt = t * s;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(to, o, 64), y = __shfl_up(pt, o, 64);
+            if (lane >= o) {
+                to += x;
+                pt += y;
+            }
+        }
+        const unsigned long long m = __ballot(slot >= before + to - c && slot < before + to);
+        if (m) {
+            const int w = __builtin_ctzll(m);
+            Work r;
+            r.i = i0 + w;
+            r.per = per;
+            r.splits = __builtin_amdgcn_readlane(s, w);
+            const int rest = slot - (before + __builtin_amdgcn_readlane(to - c, w));
+            r.first = pieces + __builtin_amdgcn_readlane(pt - t * s, w);
+            const int tiles = __builtin_amdgcn_readlane(t, w);
+            // the last tile first: its rows see the most
+            r.qt = by_tile ? rest : tiles - 1 - rest / r.splits;
+            r.sp = by_tile ? 0 : rest % r.splits;
+            return r;
+        }
+        before += __builtin_amdgcn_readlane(to, 63);
+        pieces += __builtin_amdgcn_readlane(pt, 63);
+    }
+    return {-1, 0, 0, 0, 0, 0};
+}
+// where a split leaves its part: slot of its piece
+__device__ __forceinline__ int piece_of(const Work& w, int tiles, int qt, int sp) {
+    return w.first + (tiles - 1 - qt) * w.splits + sp;
+}
+
+// Scores of keys that a row of place p does not see become -inf, whatever they are:
+// register e is key k0 + 8 (e / 4) + e % 4.  last: the lesser of p and the last key.
+__device__ __forceinline__ void hide(const SArgs& a, floatx16& s, int k0, int p, int last) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        const int j = k0 + 8 * (e / 4) + e % 4;
+        const bool see = j <= last && (p - j < a.window || j < a.sinks);
+        s[e] = see ? s[e] : -INFINITY;
+    }
+}
+// whether some row of places lo .. hi does not see all of keys k0 .. k0 + nk - 1, or none
+// of them does
+__device__ __forceinline__ bool some_hidden(const SArgs& a, int k0, int nk, int lo, int hi) {
+    return k0 + nk - 1 > lo || (hi - k0 >= a.window && k0 + nk > a.sinks);
+}
+__device__ __forceinline__ bool all_hidden(const SArgs& a, int k0, int nk, int lo, int hi) {
+    return k0 > hi || (lo - (k0 + nk - 1) >= a.window && k0 >= a.sinks);
+}
+
+// Byte-free address of key row `key`: element offset of its row, and whether there
+// is one.  ent: its page-table entry (paged).
+__device__ __forceinline__ int page_of(const SArgs& a, int key) {
+    return (int)(((double)key + 0.5) * a.inv_page);      // exact below 2^30
+}
+__device__ __forceinline__ int entry_of(const SArgs& a, const Seq& s, int key, int kend) {
+    return key < kend ? s.table[page_of(a, key)] : -1;
+}
+
+// A running softmax of the rows on lanes: maximum m2 (of s scale2), this half's sum l.
+template <int DH> struct Soft {
+    float m2, l;
+    floatx16 o[DH / 32];
+    __device__ __forceinline__ void init() {
+        m2 = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
+    }
+    // new scores in: exponentials out, what is summed rescaled to a larger maximum
+    template <int N> __device__ __forceinline__ void step(floatx16 (&sc)[N], float scale2) {
+        float mt = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) mt = fmaxf(mt, sc[j][e]);
+        mt = fmaxf(mt, half_swap(mt));
+        const float mn = fmaxf(m2, mt * scale2);
+        if (__any(mn > m2)) {
+            const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m2 - mn);
+            l *= al;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[dt][e] *= al;
+            m2 = mn;
+        }
+        const float ms = m2 == -INFINITY ? 0.f : m2;
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[j][e] = __builtin_amdgcn_exp2f(fmaf(sc[j][e], scale2, -ms));
+                l += sc[j][e];
+            }
+    }
+};
+
+// What a tile's rows come to: their output, or their split's part for the joining
+// kernel (unnormalised, with maximum and sum).  rows: rows of the sequence.
+template <typename T, int DH, int BQ>
+__device__ __forceinline__ void finish(const SArgs& a, const Seq& s, int i, int kvh, int tile0, int row0, Soft<DH>& f,
+                                       T* out, float* lse, float* part, int prow, T* ws, int lane) {
+    const int rows = s.rows * a.G, r = row0 + (lane & 31), h = lane >> 5;
+    const bool rok = r < rows;
+    if (part) {
+        if (!rok) return;
+        store_row<float, DH>(part + (long)(r - tile0) * a.dh, f.o, 1.f, a.dh, h);
+        if (h == 0) {
+            float* ml = part + (long)prow * a.dh + (r - tile0) * 2;
+            ml[0] = f.m2;
+            ml[1] = f.l;
+        }
+        return;
+    }
+    // nothing seen, or every seen score -inf: the sum is 0 (scores of NaN leave the
+    // maximum at -inf too, but a sum of NaN)
+    const bool none = f.m2 == -INFINITY && f.l == 0.f;
+    if (none) {
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) f.o[dt][e] = 0.f;
+    }
+    if (lse && rok && h == 0) {
+        const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
+        lse[((long)i * a.H + head) * a.lq + qi] = none ? -INFINITY : f.m2 * LN2 + logf(f.l);
+    }
+    Out<T, DH>::query_rows(a, a.o, out + s.o, kvh, row0, rows, f.o, none ? 0.f : 1.f / f.l, ws, lane);
+}
+
+// ---------------------------------------------------------- tiles of many rows
+// A tile of BK keys and values on its way through registers into LDS; keys that
+// are not there (past kend, of no page) enter as zeros and, of no page, with a
+// flag of -inf.
+template <typename T, int DH, int BK, int NTH, bool PAGED> struct KvRegs {
+    typedef Stage<T, DH, false, BK, NTH> St;
+    static_assert(BK <= NTH, "a thread per key flag");
+    St k, v;
+    int ent[St::NCH], entf;
+    float kfr;
+    unsigned ok;
+    // the page-table entries that fetch(block) will need
+    __device__ __forceinline__ void look(const SArgs& a, const Seq& s, int block, int kend, int tid) {
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int i = 0; i < St::NCH; ++i) ent[i] = entry_of(a, s, block * BK + tid / St::CPR + i * St::RPP, kend);
+            entf = tid < BK ? entry_of(a, s, block * BK + tid, kend) : 0;
+        }
+    }
+    __device__ __forceinline__ void fetch(const SArgs& a, const Seq& s, const T* kp, const T* vp, int kvh, int block,
+                                          int kend, int tid) {
+        const int col = tid % St::CPR * 8;
+        ok = 0;
+        kfr = 0.f;
+        if constexpr (PAGED)
+            if (tid < BK && block * BK + tid < kend && (unsigned)entf >= (unsigned)a.pages) kfr = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < St::NCH; ++i) {
+            const int key = block * BK + tid / St::CPR + i * St::RPP;
+            bool there = key < kend && col < a.dh;
+            long ka, va;
+            if constexpr (PAGED) {
+                there = there && (unsigned)ent[i] < (unsigned)a.pages;
+                const int off = key - page_of(a, key) * a.page;
+                ka = (long)ent[i] * a.k.sn + (long)off * a.k.sl;
+                va = (long)ent[i] * a.v.sn + (long)off * a.v.sl;
+            } else {
+                ka = s.k + (long)key * a.k.sl;
+                va = s.v + (long)key * a.v.sl;
+            }
+            if (there) {
+                ok |= 1u << i;
+                k.r[i].load(kp + ka + (long)kvh * a.k.sh + col);
+                v.r[i].load(vp + va + (long)kvh * a.v.sh + col);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(__bf16* Ks, __bf16* Vs, float* kf, int* bad, int tid) const {
+#pragma unroll
+        for (int i = 0; i < St::NCH; ++i) {
+            k.put(Ks, tid, i, ok >> i & 1);
+            v.put(Vs, tid, i, ok >> i & 1);
+        }
+        if constexpr (PAGED)
+            if (tid < BK) {
+                kf[tid] = kfr;
+                if (kfr != 0.f) *bad = 1;      // from this tile on the flags are looked at
+            }
+    }
+};
+
+template <typename T, int DH, int NW> struct TileCfg {
+    static constexpr int NTH = 64 * NW, BQ = 32 * NW, BK = 64;
+    static constexpr int TILE = tile_elems<T, DH, false, BK>();
+    static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
+    static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);
+    static constexpr size_t BUFS = PAIR > OUT ? PAIR : OUT;
+    static constexpr size_t LDS = BUFS + BK * sizeof(float) + 64;
+};
+template <typename T, int DH> constexpr int waves_simd() { return sizeof(T) == 2 || DH <= 64 ? 2 : 1; }
+
+// How slots become work, as the host decided: even: every sequence has qtiles row
+// tiles and nothing is split.
+struct Plan { int slots, tiles, qtiles, least, prow; bool even, split; };
+
+// A workgroup owns 32 NW rows and walks their key blocks (or its split of them).
+template <typename T, int DH, int NW, bool PAGED>
+__global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel(const SArgs a, const T* __restrict__ q,
+        const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
+        float* __restrict__ part, const Plan pl) {
+    typedef TileCfg<T, DH, NW> C;
+    typedef KvRegs<T, DH, C::BK, C::NTH, PAGED> Kv;
+    constexpr int PS = Kv::St::PS, BK = C::BK, BQ = C::BQ;
+    extern __shared__ __align__(256) char smem[];
+    __bf16* Ks = reinterpret_cast<__bf16*>(smem);
+    __bf16* Vs = Ks + C::TILE;
+    float* kf = reinterpret_cast<float*>(smem + C::BUFS);
+    int* bad = reinterpret_cast<int*>(smem + C::LDS - 64);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int l = xcd_block(blockIdx.x, gridDim.x);
+    Work w;
+    int kvh;
+    if (pl.even) {
+        const int u = l / pl.qtiles;
+        kvh = u % a.KV;
+        w = {u / a.KV, pl.qtiles - 1 - l % pl.qtiles, 0, INT_MAX, 1, 0};
+    } else {
+        kvh = l / pl.slots;
+        w = work_of<PAGED, BQ, BK>(a, l % pl.slots, pl.slots, pl.least, pl.split, false);
+    }
+    if (w.i < 0) return;
+    const Seq s = seq_of<PAGED>(a, w.i);
+    const int rows = s.rows * a.G, tile0 = w.qt * BQ;
+    if (tile0 >= rows) return;
+    const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
+    const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
+    const bool joined = rg.nt > w.per;                    // by the joining kernel
+    const int t0 = joined ? w.sp * w.per : 0, t1 = joined ? min(rg.nt, t0 + w.per) : rg.nt;
+    if (joined ? t0 >= rg.nt : w.sp > 0) return;
+    if (tid == 0) *bad = 0;
+
+    const int r0 = tile0 + 32 * wave, r = r0 + (lane & 31);
+    const bool rok = r < rows;
+    // rows past the last stand at its place, dead ones see nothing
+    const int qr = head_div(a, min(r, rows - 1)), p = s.p0 + qr, last = qr < s.ql ? min(p, rg.kend - 1) : -1;
+    const int q0 = __builtin_amdgcn_readfirstlane(qr), q1 = __builtin_amdgcn_readlane(qr, 31);
+    const bool live = r0 < rows, sees = live && q0 < s.ql, dead = q1 >= s.ql;
+    const int wlo = s.p0 + q0, whi = s.p0 + min(q1, s.ql - 1);
+    Row<T, DH> qf;
+    qf.load(q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
+    Soft<DH> f;
+    f.init();
+
+    Kv kv;
+    auto fetch = [&](int t) {
+        kv.fetch(a, s, k, v, kvh, rg.block(t), rg.kend, tid);
+        if (t + 1 < t1) kv.look(a, s, rg.block(t + 1), rg.kend, tid);
+    };
+    if (t0 < t1) {
+        kv.look(a, s, rg.block(t0), rg.kend, tid);
+        fetch(t0);
+        __syncthreads();      // *bad is cleared
+        kv.store(Ks, Vs, kf, bad, tid);
+        if (t0 + 1 < t1) fetch(t0 + 1);
+        __syncthreads();
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int key0 = rg.block(t) * BK;
+        if (sees && !all_hidden(a, key0, BK, wlo, whi)) {
+            floatx16 sc[BK / 32];
+#pragma unroll
+            for (int j = 0; j < BK / 32; ++j)
+                sc[j] = mma_rows<T, DH, false, PS>(Ks + 32 * j * Lds<DH, false>::ST, qf, lane);
+            if (dead || key0 + BK > rg.kend || some_hidden(a, key0, BK, wlo, whi)) {
+#pragma unroll
+                for (int j = 0; j < BK / 32; ++j) hide(a, sc[j], key0 + 32 * j + 4 * h, p, last);
+            }
+            if constexpr (PAGED)
+                if (*bad) {
+#pragma unroll
+                    for (int j = 0; j < BK / 32; ++j)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (kf[32 * j + 8 * (e / 4) + 4 * h + e % 4] != 0.f) sc[j][e] = -INFINITY;
+                }
+            f.step(sc, a.scale2);
+#pragma unroll
+            for (int j = 0; j < BK / 32; ++j)
+                mma_tr<T, DH, false, PS>(Vs + 32 * j * Lds<DH, false>::ST, sc[j], f.o, lane);
+        }
+        __syncthreads();
+        if (t + 1 < t1) {
+            kv.store(Ks, Vs, kf, bad, tid);
+            if (t + 2 < t1) fetch(t + 2);
+            __syncthreads();
+        }
+    }
+    f.l += half_swap(f.l);
+    const int tiles = (rows + BQ - 1) / BQ;
+    float* pp = nullptr;
+    if (joined)
+        pp = part + ((long)piece_of(w, tiles, w.qt, w.sp) * a.KV + kvh) * pl.prow * (a.dh + 2);
+    if (live)
+        finish<T, DH, BQ>(a, s, w.i, kvh, tile0, r0, f, out, lse, pp, pl.prow,
+                          reinterpret_cast<T*>(smem) + wave * Out<T, DH>::WAVE, lane);
+}
+
+// ------------------------------------------------------------ few rows
+// Up to 32 rows (a token's heads) against their keys: bound by reading the keys.
+// Waves of a workgroup take the 32-key blocks in turn and share nothing until the
+// end.  A lane holds a key's row as an operand straight from memory; the values go
+// through the wave's own part of LDS, to be read transposed.  The next block's rows
+// are on their way into the same registers while a block is worked on.
+template <typename T, int DH, int KS> struct TokenCfg {
+    static constexpr int NTH = 64 * KS, BQ = 32, BK = 32;
+    static constexpr int TILE = tile_elems<T, DH, false, BK>();
+    static constexpr size_t VALS = (size_t)KS * TILE * 2;
+    static constexpr int JS = DH * 32 + 64;      // floats of a wave's part
+    static constexpr size_t LDS = max3(VALS, (size_t)(KS - 1) * JS * sizeof(float), Out<T, DH>::WAVE * sizeof(T));
+};
+
+template <typename T, int DH, int KS, bool PAGED>
+__global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kernel(const SArgs a,
+        const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,
+        float* __restrict__ lse, float* __restrict__ part, const Plan pl) {
+    typedef TokenCfg<T, DH, KS> C;
+    typedef Lds<DH, false> L;
+    constexpr int BK = C::BK, BQ = C::BQ, PS = BK * L::ST;
+    extern __shared__ __align__(256) char smem[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    __bf16* Vs = reinterpret_cast<__bf16*>(smem) + wave * C::TILE;
+    const int kvh = blockIdx.x % a.KV, slot = blockIdx.x / a.KV;
+    Work w;
+    if (pl.even) w = {slot / pl.qtiles, pl.qtiles - 1 - slot % pl.qtiles, 0, INT_MAX, 1, 0};
+    else w = work_of<PAGED, BQ, BK>(a, slot, pl.slots, pl.least, pl.split, false);
+    if (w.i < 0) return;
+    const Seq s = seq_of<PAGED>(a, w.i);
+    const int rows = s.rows * a.G, tile0 = w.qt * BQ;
+    if (tile0 >= rows) return;
+    const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
+    const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
+    const bool joined = rg.nt > w.per;
+    const int t0 = joined ? w.sp * w.per : 0, t1 = joined ? min(rg.nt, t0 + w.per) : rg.nt;
+    if (joined ? t0 >= rg.nt : w.sp > 0) return;
+
+    const int r = tile0 + (lane & 31);
+    const bool rok = r < rows;
+    const int qr = head_div(a, min(r, rows - 1)), p = s.p0 + qr, last = qr < s.ql ? min(p, rg.kend - 1) : -1;
+    Row<T, DH> qf;
+    qf.load(q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
+    Soft<DH> f;
+    f.init();
+
+    Chunk<T> kc[DH / 16], vc[DH / 16];
+    int ent = 0;
+    bool nopage = false;
+    auto look = [&](int t) {
+        if constexpr (PAGED) ent = entry_of(a, s, rg.block(t) * BK + (lane & 31), rg.kend);
+    };
+    auto fetch = [&](int t) {
+        const int key = rg.block(t) * BK + (lane & 31);
+        bool there = key < rg.kend;
+        long ka, va;
+        if constexpr (PAGED) {
+            nopage = there && (unsigned)ent >= (unsigned)a.pages;
+            there = there && !nopage;
+            const int off = key - page_of(a, key) * a.page;
+            ka = (long)ent * a.k.sn + (long)off * a.k.sl;
+            va = (long)ent * a.v.sn + (long)off * a.v.sl;
+        } else {
+            ka = s.k + (long)key * a.k.sl;
+            va = s.v + (long)key * a.v.sl;
+        }
+        const T *kr = k + ka + (long)kvh * a.k.sh + 8 * h, *vr = v + va + (long)kvh * a.v.sh + 8 * h;
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) {
+            kc[c].zero();
+            if (there && 16 * c + 8 * h < a.dh) kc[c].load(kr + 16 * c);
+        }
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) {
+            vc[c].zero();
+            if (there && 16 * c + 8 * h < a.dh) vc[c].load(vr + 16 * c);
+        }
+    };
+    int t = t0 + wave;
+    if (t < t1) {
+        look(t);
+        fetch(t);
+        if (t + KS < t1) look(t + KS);
+    }
+    for (; t < t1; t += KS) {
+        const int key0 = rg.block(t) * BK;
+        floatx16 sc[1];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[0][e] = 0.f;
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) {
+            bf16x8 x[planes<T>()];
+            kc[c].terms(x);
+            mma(x, qf.f[c], sc[0]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");     // the last block's values are read
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c) {
+            bf16x8 x[planes<T>()];
+            vc[c].terms(x);
+#pragma unroll
+            for (int pn = 0; pn < planes<T>(); ++pn)
+                *reinterpret_cast<bf16x8*>(Vs + pn * PS + L::chunk_at(lane & 31, h, c)) = x[pn];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const unsigned long long none = PAGED ? __ballot(nopage) : 0;
+        if (t + KS < t1) {
+            fetch(t + KS);
+            if (t + 2 * KS < t1) look(t + 2 * KS);
+        }
+        hide(a, sc[0], key0 + 4 * h, p, last);
+        if (none) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (none >> (8 * (e / 4) + 4 * h + e % 4) & 1) sc[0][e] = -INFINITY;
+        }
+        f.step(sc, a.scale2);
+        mma_tr<T, DH, false, PS>(Vs, sc[0], f.o, lane);
+    }
+    f.l += half_swap(f.l);
+
+    // the waves' parts join in LDS, in wave order
+    if constexpr (KS > 1) {
+        __syncthreads();
+        float* jb = reinterpret_cast<float*>(smem);
+        if (wave > 0) {
+            float* x = jb + (size_t)(wave - 1) * C::JS;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[(dt * 16 + e) * 64 + lane] = f.o[dt][e];
+            if (h == 0) {
+                x[DH * 32 + lane] = f.m2;
+                x[DH * 32 + 32 + lane] = f.l;
+            }
+        }
+        __syncthreads();
+        if (wave > 0) return;
+        for (int u = 1; u < KS; ++u) {
+            const float* x = jb + (size_t)(u - 1) * C::JS;
+            const float mw = x[DH * 32 + (lane & 31)], lw = x[DH * 32 + 32 + (lane & 31)];
+            const float mn = fmaxf(f.m2, mw), ms = mn == -INFINITY ? 0.f : mn;
+            const float f0 = __builtin_amdgcn_exp2f(f.m2 - ms), f1 = __builtin_amdgcn_exp2f(mw - ms);
+            f.l = f.l * f0 + lw * f1;
+            f.m2 = mn;
+#pragma unroll
+            for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) f.o[dt][e] = f.o[dt][e] * f0 + x[(dt * 16 + e) * 64 + lane] * f1;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // before the parts become the rows' way out
+    }
+    float* pp = nullptr;
+    if (joined)
+        pp = part + ((long)piece_of(w, (rows + BQ - 1) / BQ, w.qt, w.sp) * a.KV + kvh) * pl.prow * (a.dh + 2);
+    finish<T, DH, BQ>(a, s, w.i, kvh, tile0, tile0, f, out, lse, pp, pl.prow, reinterpret_cast<T*>(smem), lane);
+}
+
+// ---------------------------------------------------------------- joining
+// Joins the splits of a row tile: a workgroup takes some rows of a (tile, kv head);
+// groups of LG lanes (4 columns each) take a row's splits in turn, per_row groups a
+// row, and meet in LDS in group order.
+constexpr int JOIN_NTH = 512;
+template <typename T, int LG, bool PAGED, int BQ, int BK>
+__global__ __launch_bounds__(JOIN_NTH) void seq_join_kernel(const SArgs a, const float* __restrict__ part,
+        T* __restrict__ out, float* __restrict__ lse, const Plan pl, int per_row, int rgroups) {
+    constexpr int NG = JOIN_NTH / LG;
+    __shared__ float4 sh[JOIN_NTH];
+    __shared__ float2 shm[NG];
+    const int tid = threadIdx.x, grp = tid / LG, c = tid % LG, g0 = grp & (per_row - 1);
+    const int rg_ = blockIdx.x % rgroups, kvh = blockIdx.x / rgroups % a.KV, tile = blockIdx.x / rgroups / a.KV;
+    const Work w = work_of<PAGED, BQ, BK>(a, tile, pl.slots, pl.least, pl.split, true);
+    if (w.i < 0) return;
+    const Seq s = seq_of<PAGED>(a, w.i);
+    const int rows = s.rows * a.G, tile0 = w.qt * BQ, tiles = (rows + BQ - 1) / BQ;
+    const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
+    const int nt = range_of<BK>(a, pt.lo, pt.hi, s.kl).nt;
+    if (nt <= w.per) return;        // made by one workgroup
+    const int nsp = (nt - 1) / w.per + 1;
+    const int row = rg_ * (NG / per_row) + grp / per_row, r = tile0 + row;
+    const bool live = row < BQ && r < rows;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    // one more split, or one more group: maximum em, sum el, values x
+    auto add = [&](float em, float el, const float4& x) {
+        const float mn = fmaxf(m, em), ms = mn == -INFINITY ? 0.f : mn;
+        const float f0 = __builtin_amdgcn_exp2f(m - ms), f1 = __builtin_amdgcn_exp2f(em - ms);
+        m = mn;
+        l = l * f0 + el * f1;
+        acc.x = acc.x * f0 + x.x * f1; acc.y = acc.y * f0 + x.y * f1;
+        acc.z = acc.z * f0 + x.z * f1; acc.w = acc.w * f0 + x.w * f1;
+    };
+    if (live) {
+        const long stride = (long)a.KV * pl.prow * (a.dh + 2);
+        const float* p0 = part + ((long)piece_of(w, tiles, w.qt, 0) * a.KV + kvh) * pl.prow * (a.dh + 2);
+#pragma unroll 4
+        for (int u = g0; u < nsp; u += per_row) {
+            const float* x = p0 + u * stride;
+            const float2 e = *reinterpret_cast<const float2*>(x + (long)pl.prow * a.dh + 2 * row);
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (4 * c < a.dh) y = *reinterpret_cast<const float4*>(x + (long)row * a.dh + 4 * c);
+            add(e.x, e.y, y);
+        }
+    }
+    sh[tid] = acc;
+    if (c == 0) shm[grp] = make_float2(m, l);
+    __syncthreads();
+    if (g0 > 0 || !live) return;
+    for (int g = 1; g < per_row; ++g) {
+        const float2 e = shm[grp + g];
+        add(e.x, e.y, sh[(grp + g) * LG + c]);
+    }
+    const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
+    const bool none = m == -INFINITY && l == 0.f;
+    const float f = none ? 0.f : 1.f / l;
+    if (none) acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (4 * c < a.dh)
+        st4(out + s.o + (long)qi * a.o.sl + (long)head * a.o.sh + 4 * c, acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+    if (lse && c == 0) lse[((long)w.i * a.H + head) * a.lq + qi] = none ? -INFINITY : m * LN2 + logf(l);
+}
+
+// ------------------------------------------------------------------- host
+int check_common(int n, int l, int heads, int kv_heads, int dh, int bf16, float scale, int window, int sinks,
+                 const PtcgHeadLayout& q, const PtcgHeadLayout& o, const char* who) {
+    PT_REQUIRE(n >= 0 && l >= 0, "%s: negative size: %d sequences of %d rows", who, n, l);
+    PT_REQUIRE(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, "%s: %d heads over %d kv heads", who, heads,
+               kv_heads);
+    PT_REQUIRE(dh >= 8 && dh <= 128 && dh % 8 == 0, "%s: head width %d is not a multiple of 8 up to 128", who, dh);
+    PT_REQUIRE(bf16 == 0 || bf16 == 1, "%s: bf16=%d", who, bf16);
+    PT_REQUIRE(scale > 0.f && scale < 1e30f, "%s: scale must be positive and finite", who);
+    PT_REQUIRE(window >= 0 && sinks >= 0, "%s: window=%d sinks=%d", who, window, sinks);
+    const int e = bf16 ? 8 : 4;
+    PT_REQUIRE(layout_ok(q, e) && layout_ok(o, e), "%s: strides must be non-negative multiples of 16 bytes", who);
+    const int64_t G = heads / kv_heads, rows = (int64_t)l * G;
+    PT_REQUIRE(l < (1 << 30) && rows * G < (1LL << 32) && rows < (1LL << 31) - 256,
+               "%s: %d rows of %d heads a kv head are too long", who, l, (int)G);
+    // a launch holds fewer than 2^32 threads, 256 a tile of rows
+    PT_REQUIRE((double)n * kv_heads * (double)(rows / 32 + 2) < (double)(1 << 23) && (double)n * heads * l < 4294967296.0,
+               "%s: too many rows", who);
+    return PTCG_OK;
+}
+int check_paged(const PtcgPagedAttn* d, const char* who) {
+    PT_REQUIRE(d, "%s: null descriptor", who);
+    PT_TRY(check_common(d->n, d->lq, d->heads, d->kv_heads, d->dh, d->bf16, d->scale, d->window, d->sinks, d->q, d->o,
+                        who));
+    PT_REQUIRE(!d->q_off || (d->rows >= 0 && d->rows < (1 << 30)), "%s: rows=%d", who, d->rows);
+    PT_TRY(check_pages(d->cache, d->n, d->kv_heads, d->dh, d->bf16 ? 8 : 4, who));
+    return PTCG_OK;
+}
+int check_window(const PtcgWindowAttn* d, const char* who) {
+    PT_REQUIRE(d, "%s: null descriptor", who);
+    PT_TRY(check_common(d->n, d->l, d->heads, d->kv_heads, d->dh, d->bf16, d->scale, d->window, d->sinks, d->q, d->o,
+                        who));
+    const int e = d->bf16 ? 8 : 4;
+    PT_REQUIRE(layout_ok(d->k, e) && layout_ok(d->v, e), "%s: strides must be non-negative multiples of 16 bytes", who);
+    PT_REQUIRE(!(d->off && d->len), "%s: packed sequences (off) take no len", who);
+    return PTCG_OK;
+}
+
+SArgs base_args(int n, int l, int heads, int kv_heads, int dh, float scale, int window, int sinks) {
+    SArgs a = {};
+    a.n = n; a.lq = l; a.H = heads; a.KV = kv_heads; a.G = heads / kv_heads; a.dh = dh;
+    a.gmagic = (unsigned)((1ULL << 32) / a.G + 1);
+    a.scale = scale; a.scale2 = scale * LOG2E;
+    a.window = window > 0 ? window : INT_MAX;
+    a.sinks = sinks;
+    return a;
+}
+SArgs paged_args(const PtcgPagedAttn* d) {
+    SArgs a = base_args(d->n, d->lq, d->heads, d->kv_heads, d->dh, d->scale, d->window, d->sinks);
+    a.q = d->q; a.o = d->o; a.k = d->cache.k; a.v = d->cache.v;
+    a.q_off = d->q_off; a.len = d->len; a.all_rows = d->rows;
+    a.table = d->cache.table; a.table_sn = d->n > 1 ? d->cache.table_sn : 0;
+    a.pages = d->cache.pages; a.page = d->cache.page; a.per_seq = d->cache.per_seq;
+    a.inv_page = 1.0 / d->cache.page;
+    return a;
+}
+SArgs window_args(const PtcgWindowAttn* d) {
+    SArgs a = base_args(d->n, d->l, d->heads, d->kv_heads, d->dh, d->scale, d->window, d->sinks);
+    a.q = d->q; a.o = d->o; a.k = d->k; a.v = d->v;
+    a.q_off = d->off; a.len = d->len; a.all_rows = INT_MAX;
+    return a;
+}
+
+// Which kernel and how it is split.  Up to 32 rows a (sequence, kv head): the kernel of
+// few rows, its four waves along the keys where a sequence may have more than four blocks
+// of 32.  Else tiles of 64 or 128 rows.
+struct Form {
+    bool token;
+    int waves;       // along the keys (token), along the rows else
+    int bq, bk;
+    Plan p;
+};
+// keys: the most that a row tile may see, as far as the host knows
+Form form_of(const SArgs& a, int64_t packed_rows, int64_t keys, bool bf16, bool may_split) {
+    Form f;
+    const int64_t rows = (int64_t)a.lq * a.G;
+    f.token = rows <= 32;
+    f.waves = f.token ? (keys > 128 ? 4 : 1) : rows <= 64 ? 2 : 4;
+    f.bq = f.token ? 32 : 32 * f.waves;
+    f.bk = f.token ? 32 : 64;
+    const int qtiles = pt_cdiv(rows, f.bq);
+    int64_t tiles = (int64_t)a.n * qtiles;
+    if (a.q_off) {       // no more than the rows there are make
+        const int64_t t = packed_rows * a.G / f.bq + a.n;
+        if (t < tiles) tiles = t;
+    }
+    // Pieces fill the card when row tiles do not: workgroups that run at once.  A split is
+    // two blocks a wave at least, and costs a second launch.
+    const int64_t fill = (f.token ? (bf16 || a.dh <= 64 ? 3 : 1) : (bf16 || a.dh <= 64 ? 2 : 1)) * (int64_t)cu_count();
+    f.p.least = f.token ? 2 * f.waves : 4;
+    f.p.split = may_split && tiles * a.KV < fill && keys >= 4 * f.p.least * f.bk;
+    f.p.tiles = (int)tiles;
+    f.p.slots = (int)(f.p.split ? tiles + pt_cdiv(fill, a.KV) : tiles);
+    f.p.qtiles = qtiles;
+    f.p.even = !a.q_off && !f.p.split;
+    f.p.prow = (int)(rows < f.bq ? rows : f.bq);
+    return f;
+}
+Form paged_form(const PtcgPagedAttn* d, const SArgs& a) {
+    int64_t keys = (int64_t)a.per_seq * a.page;
+    if (d->window > 0 && (int64_t)d->window + d->sinks + d->lq < keys) keys = (int64_t)d->window + d->sinks + d->lq;
+    return form_of(a, d->rows, keys, d->bf16, true);
+}
+Form window_form(const PtcgWindowAttn* d, const SArgs& a) {
+    return form_of(a, (int64_t)d->n * d->l, d->l, d->bf16, true);
+}
+int64_t part_bytes(const Form& f, const SArgs& a) {
+    return f.p.split ? (int64_t)f.p.slots * a.KV * f.p.prow * (a.dh + 2) * 4 : 0;
+}
+
+template <typename T, int DH, bool PAGED, int BQ, int BK>
+int launch_join(const SArgs& a, const Form& f, void* out, float* lse, const float* part, hipStream_t s) {
+    constexpr int LG = DH / 4, NG = JOIN_NTH / LG;
+    // splits a tile may have: those of a lone tile that takes every slot
+    int per_row = 1;
+    while (per_row < NG && per_row * 4 < f.p.slots) per_row *= 2;
+    const int rgroups = pt_cdiv(f.p.prow, NG / per_row);
+    hipLaunchKernelGGL((seq_join_kernel<T, LG, PAGED, BQ, BK>), dim3((unsigned)((int64_t)f.p.tiles * a.KV * rgroups)),
+                       dim3(JOIN_NTH), 0, s, a, part, static_cast<T*>(out), lse, f.p, per_row, rgroups);
+    PT_LAUNCH_CHECK();
+    return PTCG_OK;
+}
+
+template <typename T, int DH, int NW, bool PAGED>
+int launch_tiles(const SArgs& a, const Form& f, const void* q, const void* k, const void* v, void* out, float* lse,
+                 float* part, hipStream_t s) {
+    typedef TileCfg<T, DH, NW> C;
+    auto kern = seq_fwd_kernel<T, DH, NW, PAGED>;
+    PT_TRY(lds_attr(kern, C::LDS));
+    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)f.p.slots * a.KV)), dim3(C::NTH), C::LDS, s, a,
+                       static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                       static_cast<T*>(out), lse, part, f.p);
+    PT_LAUNCH_CHECK();
+    return f.p.split ? launch_join<T, DH, PAGED, C::BQ, C::BK>(a, f, out, lse, part, s) : PTCG_OK;
+}
+template <typename T, int DH, int KS, bool PAGED>
+int launch_token(const SArgs& a, const Form& f, const void* q, const void* k, const void* v, void* out, float* lse,
+                 float* part, hipStream_t s) {
+    typedef TokenCfg<T, DH, KS> C;
+    auto kern = seq_token_kernel<T, DH, KS, PAGED>;
+    PT_TRY(lds_attr(kern, C::LDS));
+    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)f.p.slots * a.KV)), dim3(C::NTH), C::LDS, s, a,
+                       static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                       static_cast<T*>(out), lse, part, f.p);
+    PT_LAUNCH_CHECK();
+    return f.p.split ? launch_join<T, DH, PAGED, C::BQ, C::BK>(a, f, out, lse, part, s) : PTCG_OK;
+}
+template <typename T, int DH, bool PAGED>
+int launch_form(const SArgs& a, const Form& f, const void* q, const void* k, const void* v, void* out, float* lse,
+                float* part, hipStream_t s) {
+    if (f.token)
+        return f.waves == 4 ? launch_token<T, DH, 4, PAGED>(a, f, q, k, v, out, lse, part, s)
+                            : launch_token<T, DH, 1, PAGED>(a, f, q, k, v, out, lse, part, s);
+    return f.waves == 2 ? launch_tiles<T, DH, 2, PAGED>(a, f, q, k, v, out, lse, part, s)
+                        : launch_tiles<T, DH, 4, PAGED>(a, f, q, k, v, out, lse, part, s);
+}
+template <bool PAGED>
+int run_fwd(const SArgs& a, const Form& f, bool bf16, const void* q, const void* k, const void* v, void* out, float* lse,
+            float* part, hipStream_t s) {
+    if (bf16)
+        return a.dh <= 32   ? launch_form<__bf16, 32, PAGED>(a, f, q, k, v, out, lse, part, s)
+               : a.dh <= 64 ? launch_form<__bf16, 64, PAGED>(a, f, q, k, v, out, lse, part, s)
+                            : launch_form<__bf16, 128, PAGED>(a, f, q, k, v, out, lse, part, s);
+    return a.dh <= 32   ? launch_form<float, 32, PAGED>(a, f, q, k, v, out, lse, part, s)
+           : a.dh <= 64 ? launch_form<float, 64, PAGED>(a, f, q, k, v, out, lse, part, s)
+                        : launch_form<float, 128, PAGED>(a, f, q, k, v, out, lse, part, s);
+}
+
+}  // namespace
+
+extern "C" int64_t ptcg_kernel_paged_attention_ws_bytes(const PtcgPagedAttn* d) {
+    if (check_paged(d, "paged_attention_ws_bytes") != PTCG_OK) return -1;
+    if (d->n == 0 || d->lq == 0) return 0;
+    const SArgs a = paged_args(d);
+    return part_bytes(paged_form(d, a), a);
+}
+
+extern "C" int ptcg_kernel_paged_attention(const PtcgPagedAttn* d, const void* q, void* out, float* lse, void* workspace,
+                                           int64_t workspace_bytes, void* stream) {
+    const char* who = "paged_attention";
+    PT_TRY(check_paged(d, who));
+    if (d->n == 0 || d->lq == 0 || (d->q_off && d->rows == 0)) return PTCG_OK;
+    PT_REQUIRE(q && out && d->len, "%s: null buffer", who);
+    PT_REQUIRE(al16(q) && al16(out) && al16(d->cache.kp) && al16(d->cache.vp), "%s: buffers must be 16 B aligned", who);
+    PT_REQUIRE(layout_apart(d->o, d->q_off, d->n, d->lq, d->heads, d->dh), "%s: rows of the output overlap", who);
+    const SArgs a = paged_args(d);
+    const Form f = paged_form(d, a);
+    const int64_t need = part_bytes(f, a);
+    PT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && al16(workspace)),
+               "%s: workspace of %lld bytes, need %lld (16 B aligned)", who, (long long)workspace_bytes,
+               (long long)need);
+    return run_fwd<true>(a, f, d->bf16, q, d->cache.kp, d->cache.vp, out, lse, static_cast<float*>(workspace),
+                         (hipStream_t)stream);
+}
+
+extern "C" int64_t ptcg_kernel_window_attention_ws_bytes(const PtcgWindowAttn* d, int backward) {
+    if (check_window(d, "window_attention_ws_bytes") != PTCG_OK) return -1;
+    if (d->n == 0 || d->l == 0) return 0;
+    const SArgs a = window_args(d);
+    return part_bytes(window_form(d, a), a);
+}
+
+extern "C" int ptcg_kernel_window_attention_fwd(const PtcgWindowAttn* d, const void* q, const void* k, const void* v,
+                                                void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                                                void* stream) {
+    const char* who = "window_attention_fwd";
+    PT_TRY(check_window(d, who));
+    if (d->n == 0 || d->l == 0) return PTCG_OK;
+    PT_REQUIRE(q && k && v && out, "%s: null buffer", who);
+    PT_REQUIRE(al16(q) && al16(k) && al16(v) && al16(out), "%s: buffers must be 16 B aligned", who);
+    PT_REQUIRE(layout_apart(d->o, d->off, d->n, d->l, d->heads, d->dh), "%s: rows of the output overlap", who);
+    const SArgs a = window_args(d);
+    const Form f = window_form(d, a);
+    const int64_t need = part_bytes(f, a);
+    PT_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && al16(workspace)),
+               "%s: workspace of %lld bytes, need %lld (16 B aligned)", who, (long long)workspace_bytes,
+               (long long)need);
+    return run_fwd<false>(a, f, d->bf16, q, k, v, out, lse, static_cast<float*>(workspace), (hipStream_t)stream);
+}
+
+extern "C" int ptcg_kernel_window_attention_bwd(const PtcgWindowAttn* d, const void* q, const void* k, const void* v,
+                                                const void* out, const float* lse, const void* dout, void* dq, void* dk,
+                                                void* dv, void* workspace, int64_t workspace_bytes, void* stream) {
+    PT_REQUIRE(false, "window_attention_bwd: not built yet");
+}

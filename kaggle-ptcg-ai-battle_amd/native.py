@@ -74,6 +74,20 @@ class CPtcgPagedAppend(ctypes.Structure):
         [(n, c_void_p) for n in ("q_off", "len", "wq", "wk")] + [("rope", CPtcgRope), ("cache", CPtcgPages)]
 
 
+class CPtcgPagedAttn(ctypes.Structure):
+    """struct PtcgPagedAttn of include/ptcg_amd_kernels.h."""
+    _fields_ = [(n, ctypes.c_int) for n in ("n", "lq", "rows", "heads", "kv_heads", "dh", "bf16")] + \
+        [("scale", ctypes.c_float), ("window", ctypes.c_int), ("sinks", ctypes.c_int)] + \
+        [(n, CPtcgHeadLayout) for n in ("q", "o")] + [("q_off", c_void_p), ("len", c_void_p), ("cache", CPtcgPages)]
+
+
+class CPtcgWindowAttn(ctypes.Structure):
+    """struct PtcgWindowAttn of include/ptcg_amd_kernels.h."""
+    _fields_ = [(n, ctypes.c_int) for n in ("n", "l", "heads", "kv_heads", "dh", "bf16")] + \
+        [("scale", ctypes.c_float), ("window", ctypes.c_int), ("sinks", ctypes.c_int)] + \
+        [(n, CPtcgHeadLayout) for n in ("q", "k", "v", "o")] + [("off", c_void_p), ("len", c_void_p)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "ptcg_last_error": (ctypes.c_char_p, []),
@@ -340,6 +354,14 @@ _SIGS = {
     "ptcg_kernel_qk_norm_rope_bwd": (ctypes.c_int, [ctypes.POINTER(CPtcgQkRope)] + [c_void_p] * 9
                                      + [ctypes.c_int64, c_void_p]),
     "ptcg_kernel_paged_append": (ctypes.c_int, [ctypes.POINTER(CPtcgPagedAppend)] + [c_void_p] * 5),
+    "ptcg_kernel_paged_attention_ws_bytes": (ctypes.c_int64, [ctypes.POINTER(CPtcgPagedAttn)]),
+    "ptcg_kernel_paged_attention": (ctypes.c_int, [ctypes.POINTER(CPtcgPagedAttn)] + [c_void_p] * 4
+                                    + [ctypes.c_int64, c_void_p]),
+    "ptcg_kernel_window_attention_ws_bytes": (ctypes.c_int64, [ctypes.POINTER(CPtcgWindowAttn), ctypes.c_int]),
+    "ptcg_kernel_window_attention_fwd": (ctypes.c_int, [ctypes.POINTER(CPtcgWindowAttn)] + [c_void_p] * 6
+                                         + [ctypes.c_int64, c_void_p]),
+    "ptcg_kernel_window_attention_bwd": (ctypes.c_int, [ctypes.POINTER(CPtcgWindowAttn)] + [c_void_p] * 10
+                                         + [ctypes.c_int64, c_void_p]),
 }
 
 _lib = None

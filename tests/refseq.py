@@ -11,6 +11,18 @@ Norm and rotation, dh elements a head:
   dx       r (dn w - x m), m = r^2 mean(dn w x): with f = (dh + 12) u,
            r (e |w| + f |dn w|) + r |x| r^2 (mean((e + f |dn|) |w x|) + 2 f mean|dn w x|) + b |dx|
   dw       sum |x r| (e + f |dn|) + terms u sum |dn x r|
+Attention with its gradients, lk keys:
+  scores   |ds| <= (dh + 4) u scale sum|q||k|; an exponential adds 4 u and the
+           shifted argument's rounding |s - m| u: a probability is off by
+           e_i = 2 max_j|ds_ij| + (8 + 4 max|s| + lk) u, relatively
+  out      sum_j P|v| (e + p) + b |out|, p = 2^-8 in bf16 (P rounded for the
+           product), 0 in fp32
+  D        sum_d |do| err(out)_d + dh u sum|do||out|
+  dS       P (err(D) + (dh + 4) u sum|do||v|) + |dS| (e + p + 4 u)
+  dq, dk   scale sum err(dS) |k|, |q| (+ the sum's own u per term) + b |.|
+  dv       sum_i P |do| (e + p + rows u) + b |dv|
+Underflow: an exponential below 2^-126 may come out as 0, so P is off by up to
+2^-126 absolutely as well, and so is every product made from it.
 """
 import math
 
@@ -80,6 +92,65 @@ def norm_rope(x, w, eps, pos, freq, mag, inter, t, dy=None):
     dw = (dn * x * r).sum((0, 1))
     res["dw"] = (dw, (((e + f * dn.abs()) * (x * r).abs()).sum((0, 1)) + terms * U * (dn * x * r).abs().sum((0, 1)))
                  + U * dw.abs() + TINY)
+    return res
+
+
+FLUSH = 2.0 ** -126
+
+
+def sees(qpos, kpos, window, sinks):
+    """(rows, keys): which keys a row sees."""
+    q, k = qpos[:, None], kpos[None]
+    return (k <= q) & ((q - k < (window or 1 << 62)) | (k < sinks))
+
+
+def attention(q, k, v, see, scale, do=None, bf16=False):
+    """One sequence in 64 bits: q (lq, H, d), k, v (lk, KV, d), see (lq, lk) bool.
+    Returns {name: (value, bound)}; lse's bound is absolute too."""
+    t = torch.bfloat16 if bf16 else torch.float32
+    b, p_round = half_step(t), (2.0 ** -8 if bf16 else 0.0)
+    q, k, v = q.double(), k.double(), v.double()
+    unseen = ~see.any(0)
+    k, v = k.masked_fill(unseen[:, None, None], 0.0), v.masked_fill(unseen[:, None, None], 0.0)
+    lq, H, d = q.shape
+    lk, KV = k.shape[0], k.shape[1]
+    G = H // KV
+    live = see.any(1)
+    qh = q.transpose(0, 1).masked_fill(~live[None, :, None], 0.0)
+    kh, vh = (x.transpose(0, 1).repeat_interleave(G, 0) for x in (k, v))
+    s = (scale * qh @ kh.transpose(1, 2)).masked_fill(~see, -math.inf)
+    sabs = (scale * qh.abs() @ kh.abs().transpose(1, 2)).masked_fill(~see, 0.0)
+    lse = torch.logsumexp(s, 2) if lk else torch.full((H, lq), -math.inf, dtype=torch.float64, device=q.device)
+    P = torch.exp(s - torch.where(live, lse, 0.0)[..., None])
+    top = sabs.amax(2, keepdim=True) if lk else torch.zeros(H, lq, 1, dtype=torch.float64, device=q.device)
+    e = (2 * (d + 4) * U * top + (8 + 4 * top + lk) * U) * live[None, :, None]
+    out = P @ vh
+    out_err = (P @ vh.abs()) * (e + p_round) * (1 + p_round) + b * out.abs() + TINY
+    out_err = out_err + FLUSH * (see.double() @ vh.abs())
+    res = {"out": (out.transpose(0, 1), out_err.transpose(0, 1)),
+           "lse": (lse, e[..., 0] + 4 * U * (1 + lse.abs().nan_to_num(posinf=0.0)))}
+    if do is None:
+        return res
+    doh = do.double().transpose(0, 1).masked_fill(~live[None, :, None], 0.0)
+    dP = doh @ vh.transpose(1, 2)
+    D = (doh * out).sum(2, keepdim=True)
+    D_err = (doh.abs() * out_err).sum(2, keepdim=True) + d * U * (doh.abs() * out.abs()).sum(2, keepdim=True)
+    dS = P * (dP - D)
+    dP_err = (d + 4) * U * doh.abs() @ vh.abs().transpose(1, 2)
+    dS_err = P * (D_err + dP_err) * (1 + p_round) + dS.abs() * (e + p_round + 4 * U)
+    dS_err = dS_err + FLUSH * (dP.abs() + D.abs() + 1) * see
+    fold = lambda x: x.unflatten(0, (KV, G)).sum(1)
+    rows = lq * G
+
+    def pair(val, err, terms, absum):
+        return val.transpose(0, 1), (err + terms * U * absum + b * val.abs() + TINY).transpose(0, 1)
+
+    res["dq"] = pair(scale * dS @ kh, scale * dS_err @ kh.abs(), lk + 4, scale * dS.abs() @ kh.abs())
+    res["dk"] = pair(scale * fold(dS.transpose(1, 2) @ qh), scale * fold(dS_err.transpose(1, 2) @ qh.abs()), rows + 4,
+                     scale * fold(dS.abs().transpose(1, 2) @ qh.abs()))
+    res["dv"] = pair(fold(P.transpose(1, 2) @ doh),
+                     fold((P * (e + p_round) + FLUSH * see).transpose(1, 2) @ doh.abs()), rows + 4,
+                     fold(P.transpose(1, 2) @ doh.abs()))
     return res
 
 

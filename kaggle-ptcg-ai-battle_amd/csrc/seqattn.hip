@@ -270,14 +270,26 @@ __device__ __forceinline__ void finish(const SArgs& a, const Seq& s, int i, int 
 // ---------------------------------------------------------- tiles of many rows
 // A tile of BK keys and values on its way through registers into LDS; keys that
 // are not there (past kend, of no page) enter as zeros and, of no page, with a
-// flag of -inf.
-template <typename T, int DH, int BK, int NTH, bool PAGED> struct KvRegs {
-    typedef Stage<T, DH, false, BK, NTH> St;
+// flag of -inf.  Rows of one matrix: bounded loads; of pages: each row by its own
+// page-table entry, looked up a block ahead.
+template <typename T, int DH, bool PAD, int BK, int NTH, bool PAGED> struct KvRegs {
+    typedef Stage<T, DH, PAD, BK, NTH> St;
     static_assert(BK <= NTH, "a thread per key flag");
     St k, v;
+    RowBuf kb, vb;
+    int ko, vo;
     int ent[St::NCH], entf;
     float kfr;
     unsigned ok;
+    __device__ __forceinline__ void init(const SArgs& a, const Seq& s, const T* kp, const T* vp, int kvh, int tid) {
+        if constexpr (!PAGED) {
+            constexpr int es = sizeof(T);
+            kb = {reinterpret_cast<const char*>(kp + s.k + (long)kvh * a.k.sh), (int)a.k.sl * es, a.dh * es};
+            vb = {reinterpret_cast<const char*>(vp + s.v + (long)kvh * a.v.sh), (int)a.v.sl * es, a.dh * es};
+            ko = St::first(kb.ld, a.dh, tid);
+            vo = St::first(vb.ld, a.dh, tid);
+        }
+    }
     // the page-table entries that fetch(block) will need
     __device__ __forceinline__ void look(const SArgs& a, const Seq& s, int block, int kend, int tid) {
         if constexpr (PAGED) {
@@ -288,37 +300,31 @@ template <typename T, int DH, int BK, int NTH, bool PAGED> struct KvRegs {
     }
     __device__ __forceinline__ void fetch(const SArgs& a, const Seq& s, const T* kp, const T* vp, int kvh, int block,
                                           int kend, int tid) {
-        const int col = tid % St::CPR * 8;
-        ok = 0;
-        kfr = 0.f;
-        if constexpr (PAGED)
-            if (tid < BK && block * BK + tid < kend && (unsigned)entf >= (unsigned)a.pages) kfr = -INFINITY;
+        if constexpr (!PAGED) {
+            const auto rk = kb.rows(block * BK, kend, BK), rv = vb.rows(block * BK, kend, BK);
+            k.load(rk, ko, kb.ld);
+            v.load(rv, vo, vb.ld);
+        } else {
+            const int col = tid % St::CPR * 8;
+            ok = 0;
+            kfr = tid < BK && block * BK + tid < kend && (unsigned)entf >= (unsigned)a.pages ? -INFINITY : 0.f;
 #pragma unroll
-        for (int i = 0; i < St::NCH; ++i) {
-            const int key = block * BK + tid / St::CPR + i * St::RPP;
-            bool there = key < kend && col < a.dh;
-            long ka, va;
-            if constexpr (PAGED) {
-                there = there && (unsigned)ent[i] < (unsigned)a.pages;
-                const int off = key - page_of(a, key) * a.page;
-                ka = (long)ent[i] * a.k.sn + (long)off * a.k.sl;
-                va = (long)ent[i] * a.v.sn + (long)off * a.v.sl;
-            } else {
-                ka = s.k + (long)key * a.k.sl;
-                va = s.v + (long)key * a.v.sl;
-            }
-            if (there) {
-                ok |= 1u << i;
-                k.r[i].load(kp + ka + (long)kvh * a.k.sh + col);
-                v.r[i].load(vp + va + (long)kvh * a.v.sh + col);
+            for (int i = 0; i < St::NCH; ++i) {
+                const int key = block * BK + tid / St::CPR + i * St::RPP;
+                if (key < kend && col < a.dh && (unsigned)ent[i] < (unsigned)a.pages) {
+                    const int off = key - page_of(a, key) * a.page;
+                    ok |= 1u << i;
+                    k.r[i].load(kp + (long)ent[i] * a.k.sn + (long)off * a.k.sl + (long)kvh * a.k.sh + col);
+                    v.r[i].load(vp + (long)ent[i] * a.v.sn + (long)off * a.v.sl + (long)kvh * a.v.sh + col);
+                }
             }
         }
     }
     __device__ __forceinline__ void store(__bf16* Ks, __bf16* Vs, float* kf, int* bad, int tid) const {
 #pragma unroll
         for (int i = 0; i < St::NCH; ++i) {
-            k.put(Ks, tid, i, ok >> i & 1);
-            v.put(Vs, tid, i, ok >> i & 1);
+            k.put(Ks, tid, i, !PAGED || (ok >> i & 1));
+            v.put(Vs, tid, i, !PAGED || (ok >> i & 1));
         }
         if constexpr (PAGED)
             if (tid < BK) {
@@ -348,7 +354,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
         float* __restrict__ part, const Plan pl) {
     typedef TileCfg<T, DH, NW> C;
-    typedef KvRegs<T, DH, C::BK, C::NTH, PAGED> Kv;
+    typedef KvRegs<T, DH, false, C::BK, C::NTH, PAGED> Kv;
     constexpr int PS = Kv::St::PS, BK = C::BK, BQ = C::BQ;
     extern __shared__ __align__(256) char smem[];
     __bf16* Ks = reinterpret_cast<__bf16*>(smem);
@@ -391,6 +397,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     f.init();
 
     Kv kv;
+    kv.init(a, s, k, v, kvh, tid);
     auto fetch = [&](int t) {
         kv.fetch(a, s, k, v, kvh, rg.block(t), rg.kend, tid);
         if (t + 1 < t1) kv.look(a, s, rg.block(t + 1), rg.kend, tid);
@@ -665,6 +672,343 @@ __global__ __launch_bounds__(JOIN_NTH) void seq_join_kernel(const SArgs a, const
     if (lse && c == 0) lse[((long)w.i * a.H + head) * a.lq + qi] = none ? -INFINITY : m * LN2 + logf(l);
 }
 
+// --------------------------------------------------------------- backward
+// With P_ij = exp(s_ij - lse_i) and D_i = do_i . o_i over the pairs that see each other:
+//   dv_j = sum_i P_ij do_i,  dS_ij = P_ij (do_i . v_j - D_i),
+//   dq_i = scale sum_j dS_ij k_j,  dk_j = scale sum_i dS_ij q_i,
+// dk and dv summed over the query heads that share the kv head, in row order.
+template <typename T> struct Grads {
+    const T *q, *k, *v, *out, *dout;
+    const float* lse;
+    T *dq, *dk, *dv;
+    float *delta, *part;
+};
+
+// dQ: the forward's shape.  Per 32 keys S^T and dP^T = V dO^T with queries on
+// lanes, dS^T in registers, dQ^T += K^T dS^T.  Also leaves D_i for the dK / dV
+// kernel, in row order of lse.
+template <typename T, int DH, int NW> struct DqCfg {
+    static constexpr bool PAD = DH == 128;
+    static constexpr int NTH = 64 * NW, BQ = 32 * NW, BK = 64;
+    static constexpr int TILE = tile_elems<T, DH, PAD, BK>();
+    static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
+    static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);
+    static constexpr size_t LDS = PAIR > OUT ? PAIR : OUT;
+};
+template <typename T, int DH, int NW>
+__global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(const SArgs a, const Grads<T> g,
+                                                                               const Plan pl) {
+    typedef DqCfg<T, DH, NW> C;
+    typedef KvRegs<T, DH, C::PAD, C::BK, C::NTH, false> Kv;
+    typedef Lds<DH, C::PAD> L;
+    constexpr int PS = Kv::St::PS, BK = C::BK, BQ = C::BQ;
+    extern __shared__ __align__(256) char smem[];
+    __bf16* Ks = reinterpret_cast<__bf16*>(smem);
+    __bf16* Vs = Ks + C::TILE;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    const int l = xcd_block(blockIdx.x, gridDim.x);
+    Work w;
+    int kvh;
+    if (pl.even) {
+        const int u = l / pl.qtiles;
+        kvh = u % a.KV;
+        w = {u / a.KV, pl.qtiles - 1 - l % pl.qtiles, 0, INT_MAX, 1, 0};
+    } else {
+        kvh = l / pl.slots;
+        w = work_of<false, BQ, BK>(a, l % pl.slots, pl.slots, 0, false, false);
+    }
+    if (w.i < 0) return;
+    const Seq s = seq_of<false>(a, w.i);
+    const int rows = s.rows * a.G, tile0 = w.qt * BQ;
+    if (tile0 >= rows) return;
+    const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
+    const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
+
+    const int r0 = tile0 + 32 * wave, r = r0 + (lane & 31);
+    const bool rok = r < rows;
+    const int qr = head_div(a, min(r, rows - 1)), last = qr < s.ql ? min(qr, rg.kend - 1) : -1;
+    const int q0 = __builtin_amdgcn_readfirstlane(qr), q1 = __builtin_amdgcn_readlane(qr, 31);
+    const bool live = r0 < rows, sees = live && q0 < s.ql, dead = q1 >= s.ql;
+    const int wlo = q0, whi = min(q1, s.ql - 1);
+
+    Row<T, DH> qf, df;
+    qf.load(g.q + s.q + (rok ? row_off(a, a.q, kvh, r) : 0), rok, a.dh, h);
+    const long oo = s.o + (rok ? row_off(a, a.o, kvh, r) : 0);
+    float D = 0.f;
+#pragma unroll
+    for (int c = 0; c < DH / 16; ++c) {
+        Chunk<T> x, y;
+        x.zero();
+        y.zero();
+        if (rok && 16 * c + 8 * h < a.dh) {
+            x.load(g.dout + oo + 16 * c + 8 * h);
+            y.load(g.out + oo + 16 * c + 8 * h);
+        }
+        x.terms(df.f[c]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) D += x.at(e) * y.at(e);
+    }
+    D += half_swap(D);
+    const int qi = head_div(a, rok ? r : 0), head = kvh * a.G + (rok ? r : 0) - qi * a.G;
+    const long lrow = ((long)w.i * a.H + head) * a.lq + qi;
+    const float lr = rok && qr < s.ql ? g.lse[lrow] : -INFINITY;
+    const bool none = lr == -INFINITY;
+    const float l2 = none ? INFINITY : lr * LOG2E;
+    if (rok && h == 0) g.delta[lrow] = D;
+
+    floatx16 acc[DH / 32];
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
+    Kv kv;
+    kv.init(a, s, g.k, g.v, kvh, tid);
+    auto fetch = [&](int t) { kv.fetch(a, s, g.k, g.v, kvh, rg.block(t), rg.kend, tid); };
+    if (rg.nt > 0) {
+        fetch(0);
+        kv.store(Ks, Vs, nullptr, nullptr, tid);
+        if (rg.nt > 1) fetch(1);
+        __syncthreads();
+    }
+    for (int t = 0; t < rg.nt; ++t) {
+#pragma unroll 1
+        for (int j = 0; j < BK / 32; ++j) {
+            const int key0 = rg.block(t) * BK + 32 * j;
+            if (!sees || key0 >= rg.kend || all_hidden(a, key0, 32, wlo, whi)) continue;
+            floatx16 sc = mma_rows<T, DH, C::PAD, PS>(Ks + 32 * j * L::ST, qf, lane);
+            const floatx16 dp = mma_rows<T, DH, C::PAD, PS>(Vs + 32 * j * L::ST, df, lane);
+            if (dead || key0 + 32 > rg.kend || some_hidden(a, key0, 32, wlo, whi)) hide(a, sc, key0 + 4 * h, qr, last);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -l2)) * (dp[e] - D);
+            mma_tr<T, DH, C::PAD, PS>(Ks + 32 * j * L::ST, sc, acc, lane);
+        }
+        __syncthreads();
+        if (t + 1 < rg.nt) {
+            kv.store(Ks, Vs, nullptr, nullptr, tid);
+            if (t + 2 < rg.nt) fetch(t + 2);
+            __syncthreads();
+        }
+    }
+    if (!live) return;
+    if (none) {
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
+    }
+    Out<T, DH>::query_rows(a, a.q, g.dq + s.q, kvh, r0, rows, acc, a.scale,
+                           reinterpret_cast<T*>(smem) + wave * Out<T, DH>::WAVE, lane);
+}
+
+// How dK / dV's work is cut.  Key tiles of 32 NK keys; where a window has first tokens,
+// the tiles that hold these (`first` of them) are seen by every later row: the rows
+// past the window's reach (far rows) are cut into `chunks` of `chunk` flattened rows for
+// workgroups of their own, whose parts seq_first_kernel adds up.
+struct DkvPlan { int ktiles, first, chunks, chunk; bool even; };
+
+// rows that see the key tile from key0: near ones up to `far`, far ones from there on
+struct Rows { int lo, far, hi; };
+__device__ __forceinline__ Rows rows_of(const SArgs& a, const Seq& s, int key0, int nk) {
+    Rows r;
+    r.lo = min(key0, s.ql) * a.G;
+    const int reach = a.window > s.ql - key0 - nk ? s.ql : min(s.ql, key0 + nk - 1 + a.window);
+    r.far = reach * a.G;
+    r.hi = key0 < a.sinks ? s.ql * a.G : r.far;
+    return r;
+}
+
+template <typename T, int DH, int NK> struct DkvCfg {
+    static constexpr bool PAD = DH == 128;
+    static constexpr int NTH = 64 * NK, BKEY = 32 * NK;
+    // the rows of a step: 32 where the registers hold no more on their way
+    static constexpr int BQ = DH * planes<T>() >= 128 || NK < 4 ? 32 : 64;
+    static constexpr int TILE = tile_elems<T, DH, PAD, BQ>();
+    static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
+    static constexpr size_t OUT = (size_t)NK * Out<T, DH>::WAVE * sizeof(T);
+    static constexpr size_t BUFS = PAIR > OUT ? PAIR : OUT;
+    // 128 wide in bf16, the values' rows stay in LDS: with them, dK and dV in
+    // registers two waves a SIMD would spill
+    static constexpr bool VLDS = sizeof(T) == 2 && DH == 128;
+    static constexpr size_t VROWS = VLDS ? (size_t)BKEY * Lds<DH, PAD>::ST * 2 : 0;
+    static constexpr size_t LDS = BUFS + VROWS + 3 * BQ * sizeof(float) + 16;
+};
+template <typename T, int DH> constexpr int dkv_waves() {
+    return DH * planes<T>() <= 64 || waves_simd<T, DH>() == 2 ? 2 : 1;
+}
+
+template <typename T, int DH, int NK>
+__global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(const SArgs a, const Grads<T> g,
+                                                                               const DkvPlan pl) {
+    typedef DkvCfg<T, DH, NK> C;
+    typedef Stage<T, DH, C::PAD, C::BQ, C::NTH> St;
+    typedef Lds<DH, C::PAD> L;
+    extern __shared__ __align__(256) char smem[];
+    __bf16* Qs = reinterpret_cast<__bf16*>(smem);
+    __bf16* Ds = Qs + C::TILE;
+    float* ls = reinterpret_cast<float*>(smem + C::BUFS + C::VROWS);   // log-sum-exp, D and place of the rows
+    float* dl = ls + C::BQ;
+    int* ps = reinterpret_cast<int*>(dl + C::BQ);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+    // a (sequence, kv head)'s pieces: near rows of its key tiles, then far chunks of the first ones
+    const int per = pl.ktiles + pl.first * pl.chunks, b = xcd_block(blockIdx.x, gridDim.x);
+    const int u = b / per, x = b - u * per, i = u / a.KV, kvh = u - i * a.KV;
+    const bool isfar = x >= pl.ktiles;
+    const int kt = isfar ? (x - pl.ktiles) / pl.chunks : x, ch = isfar ? (x - pl.ktiles) % pl.chunks : 0;
+    const Seq s = seq_of<false>(a, i);
+    const int kall = s.rows;          // a padded sequence's dead rows get zeros
+    if (kt * C::BKEY >= kall) return;
+    const int key0 = kt * C::BKEY, kw = key0 + 32 * wave, key = kw + (lane & 31);
+    const bool kin = key < kall, kok = key < s.kl;
+    const Rows rr = rows_of(a, s, key0, C::BKEY);
+    const bool cut = kt < pl.first && pl.chunks > 0;
+    int r0 = rr.lo, rows = cut ? rr.far : rr.hi;
+    if (isfar) {
+        r0 = rr.far + ch * pl.chunk;
+        rows = ch + 1 == pl.chunks ? rr.hi : min(rr.hi, r0 + pl.chunk);
+        if (r0 >= rows) return;
+    }
+    if (key0 >= s.kl) rows = r0;
+
+    Row<T, DH> kfr, vfr;
+    __bf16* Vl = reinterpret_cast<__bf16*>(smem + C::BUFS) + 32 * wave * L::ST;
+    const long ko = s.k + (kin ? (long)key * a.k.sl + (long)kvh * a.k.sh : 0);
+    const long vo = s.v + (kin ? (long)key * a.v.sl + (long)kvh * a.v.sh : 0);
+    kfr.load(g.k + ko, kok, a.dh, h);
+    vfr.load(g.v + vo, kok, a.dh, h);
+    if constexpr (C::VLDS) {     // this wave's 32 rows, read by itself alone
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c)
+            *reinterpret_cast<bf16x8*>(Vl + L::chunk_at(lane & 31, h, c)) = vfr.f[c][0];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    floatx16 gk[DH / 32], gv[DH / 32];
+#pragma unroll
+    for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
+
+    const int nt = rows > r0 ? (rows - r0 + C::BQ - 1) / C::BQ : 0;
+    St qs_, ds_;
+    float lr = 0.f, dr = 0.f;
+    int rown = 0, pr = 0;     // rows of the fetched tile; a row's place
+    auto fetch = [&](int t) {
+        const int row0 = r0 + t * C::BQ;
+        rown = rows - row0;
+        qs_.load_q(a, a.q, g.q + s.q, kvh, row0, rows, tid);
+        ds_.load_q(a, a.o, g.dout + s.o, kvh, row0, rows, tid);
+        if (tid < C::BQ) {
+            const int r = min(row0 + tid, rows - 1);
+            const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
+            const long lrow = ((long)i * a.H + head) * a.lq + qi;
+            lr = g.lse[lrow];
+            dr = g.delta[lrow];
+            pr = qi;
+        }
+    };
+    auto store = [&]() {
+        // past the end q's last row stays: its log-sum-exp of +inf takes it out
+        qs_.store_q(Qs, tid, C::BQ, a.dh);
+        ds_.store_q(Ds, tid, rown, a.dh);
+        if (tid < C::BQ) {
+            const bool live = tid < rown;
+            ls[tid] = live && lr != -INFINITY ? lr * LOG2E : INFINITY;
+            dl[tid] = live ? dr : 0.f;
+            ps[tid] = pr;
+        }
+    };
+    if (nt > 0) {
+        fetch(0);
+        store();
+        if (nt > 1) fetch(1);
+        __syncthreads();
+    }
+    for (int t = 0; t < nt; ++t) {
+#pragma unroll 1
+        for (int j = 0; j < C::BQ / 32; ++j) {
+            const int qr = 32 * j, row0 = r0 + t * C::BQ + qr;
+            if (row0 >= rows) break;
+            const int plo = __builtin_amdgcn_readfirstlane(ps[qr]), phi = __builtin_amdgcn_readfirstlane(ps[qr + 31]);
+            if (kw >= s.kl || all_hidden(a, kw, 32, plo, phi)) continue;
+            floatx16 p = mma_rows<T, DH, C::PAD, St::PS>(Qs + qr * L::ST, kfr, lane);
+            floatx16 d;
+            if constexpr (C::VLDS) d = mma_rows_lds<DH, C::PAD>(Ds + qr * L::ST, Vl, lane);
+            else d = mma_rows<T, DH, C::PAD, St::PS>(Ds + qr * L::ST, vfr, lane);
+            if (some_hidden(a, kw, 32, plo, phi)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int at = ps[qr + 8 * (e / 4) + 4 * h + e % 4];
+                    p[e] = key <= at && (at - key < a.window || key < a.sinks) ? p[e] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float4 lf = *reinterpret_cast<const float4*>(ls + qr + 8 * e + 4 * h);
+                const float4 df = *reinterpret_cast<const float4*>(dl + qr + 8 * e + 4 * h);
+                const float lv[4] = {lf.x, lf.y, lf.z, lf.w}, dv4[4] = {df.x, df.y, df.z, df.w};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    // a key that is not there goes along: its columns are cleared at the end
+                    const float pe = __builtin_amdgcn_exp2f(fmaf(p[4 * e + c], a.scale2, -lv[c]));
+                    p[4 * e + c] = pe;
+                    d[4 * e + c] = pe * (d[4 * e + c] - dv4[c]);
+                }
+            }
+            mma_tr<T, DH, C::PAD, St::PS>(Ds + qr * L::ST, p, gv, lane);
+            mma_tr<T, DH, C::PAD, St::PS>(Qs + qr * L::ST, d, gk, lane);
+        }
+        __syncthreads();
+        if (t + 1 < nt) {
+            store();
+            if (t + 2 < nt) fetch(t + 2);
+            __syncthreads();
+        }
+    }
+    if (!kok) {   // a dead key's gradient is zero, whatever the rows hold
+#pragma unroll
+        for (int dt = 0; dt < DH / 32; ++dt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
+    }
+    if (cut) {     // part of the sums over a first tile's rows
+        float* p = g.part + ((((long)u * pl.first + kt) * (pl.chunks + 1) + (isfar ? 1 + ch : 0)) * C::BKEY +
+                             32 * wave + (lane & 31)) * 2 * a.dh;
+        if (kin) {
+            store_row<float, DH>(p, gk, 1.f, a.dh, h);
+            store_row<float, DH>(p + a.dh, gv, 1.f, a.dh, h);
+        }
+        return;
+    }
+    T* ws = reinterpret_cast<T*>(smem) + wave * Out<T, DH>::WAVE;
+    Out<T, DH>::key_rows(g.dk + s.k + (long)kvh * a.k.sh, a.k.sl, kw, kall, a.dh, gk, a.scale, ws, lane);
+    Out<T, DH>::key_rows(g.dv + s.v + (long)kvh * a.v.sh, a.v.sl, kw, kall, a.dh, gv, 1.f, ws, lane);
+}
+
+// the parts of the first tiles' dk and dv, in chunk order: 4 columns a thread
+template <typename T>
+__global__ __launch_bounds__(256) void seq_first_kernel(const SArgs a, const float* __restrict__ part,
+        T* __restrict__ dk, T* __restrict__ dv, const DkvPlan pl, int bkey) {
+    const int c4 = a.dh / 4, per = pl.first * bkey;       // keys a (sequence, kv head)
+    const long at = (long)blockIdx.x * 256 + threadIdx.x, both = at / c4;
+    const int c = (int)(at - both * c4) * 4, isv = (int)(both & 1), u = (int)(both / 2 / per);
+    const int key = (int)(both / 2 - (long)u * per);
+    if (u >= a.n * a.KV) return;
+    const int i = u / a.KV, kvh = u - i * a.KV, kt = key / bkey;
+    const Seq s = seq_of<false>(a, i);
+    if (key >= s.rows) return;
+    const Rows r = rows_of(a, s, kt * bkey, bkey);
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p <= pl.chunks; ++p) {
+        if (p > 0 && (r.far + (p - 1) * pl.chunk >= r.hi || kt * bkey >= s.kl)) break;
+        const float4 x = *reinterpret_cast<const float4*>(
+            part + (((((long)u * pl.first + kt) * (pl.chunks + 1) + p) * bkey + key % bkey) * 2 + isv) * a.dh + c);
+        g.x += x.x; g.y += x.y; g.z += x.z; g.w += x.w;
+    }
+    const float f = isv ? 1.f : a.scale;
+    T* o = isv ? dv + s.v + (long)key * a.v.sl + (long)kvh * a.v.sh : dk + s.k + (long)key * a.k.sl + (long)kvh * a.k.sh;
+    st4(o + c, g.x * f, g.y * f, g.z * f, g.w * f);
+}
+
 // ------------------------------------------------------------------- host
 int check_common(int n, int l, int heads, int kv_heads, int dh, int bf16, float scale, int window, int sinks,
                  const PtcgHeadLayout& q, const PtcgHeadLayout& o, const char* who) {
@@ -700,6 +1044,12 @@ int check_window(const PtcgWindowAttn* d, const char* who) {
     const int e = d->bf16 ? 8 : 4;
     PT_REQUIRE(layout_ok(d->k, e) && layout_ok(d->v, e), "%s: strides must be non-negative multiples of 16 bytes", who);
     PT_REQUIRE(!(d->off && d->len), "%s: packed sequences (off) take no len", who);
+    PT_REQUIRE((d->k.sl | d->v.sl) < (1 << 22), "%s: key rows 2^22 elements apart or more", who);
+    // a bounded tile reads zeros past its rows, which holds for rows that do not
+    // reach into one another
+    PT_REQUIRE((d->l <= 1 && !d->off) ||
+                   ((d->k.sl == 0 || d->k.sl >= d->dh) && (d->v.sl == 0 || d->v.sl >= d->dh)),
+               "%s: key rows overlap", who);
     return PTCG_OK;
 }
 
@@ -724,6 +1074,7 @@ SArgs paged_args(const PtcgPagedAttn* d) {
 SArgs window_args(const PtcgWindowAttn* d) {
     SArgs a = base_args(d->n, d->l, d->heads, d->kv_heads, d->dh, d->scale, d->window, d->sinks);
     a.q = d->q; a.o = d->o; a.k = d->k; a.v = d->v;
+    if (d->l <= 1 && !d->off) a.k.sl = a.v.sl = d->dh;     // one row: any stride was given
     a.q_off = d->off; a.len = d->len; a.all_rows = INT_MAX;
     return a;
 }
@@ -833,6 +1184,80 @@ int run_fwd(const SArgs& a, const Form& f, bool bf16, const void* q, const void*
                         : launch_form<float, 128, PAGED>(a, f, q, k, v, out, lse, part, s);
 }
 
+// The backward's launches: row tiles for dq; key tiles, and chunks of the rows that see
+// first tokens alone, for dk and dv.
+struct BwdPlan {
+    int nw, nk;
+    Plan q;
+    DkvPlan k;
+    int64_t delta, part;     // workspace floats
+};
+BwdPlan bwd_plan(const PtcgWindowAttn* d, const SArgs& a) {
+    BwdPlan p = {};
+    const int64_t rows = (int64_t)a.lq * a.G;
+    p.nw = rows <= 64 ? 2 : 4;
+    p.q.qtiles = pt_cdiv(rows, 32 * p.nw);
+    p.q.tiles = p.q.slots = a.n * p.q.qtiles;
+    p.q.even = !a.q_off;
+    p.nk = a.lq <= 64 && (d->bf16 || a.dh <= 64) ? 2 : 4;
+    const int bkey = 32 * p.nk;
+    p.k.ktiles = pt_cdiv(a.lq, bkey);
+    // Far rows are cut where one tile's would take longer than two key tiles' near ones, in
+    // at most 16 pieces; with more than two such tiles there is work for many workgroups as it is.
+    if (a.sinks > 0 && a.sinks <= 2 * bkey && a.window < a.lq) {
+        const int64_t near = ((int64_t)bkey + a.window) * a.G, far = rows - near;
+        if (far > near) {
+            p.k.first = pt_cdiv(a.sinks, bkey);
+            int64_t chunk = near > far / 16 ? near : far / 16;
+            chunk = (chunk + 63) / 64 * 64;
+            p.k.chunk = (int)chunk;
+            p.k.chunks = pt_cdiv(far, chunk);
+        }
+    }
+    p.delta = ((int64_t)a.n * a.H * a.lq + 3) / 4 * 4;
+    p.part = (int64_t)a.n * a.KV * p.k.first * (p.k.chunks + 1) * bkey * 2 * a.dh;
+    if (p.k.first == 0) p.part = 0;
+    return p;
+}
+
+template <typename T, int DH, int NW> int launch_dq(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
+    typedef DqCfg<T, DH, NW> C;
+    auto kern = seq_dq_kernel<T, DH, NW>;
+    PT_TRY(lds_attr(kern, C::LDS));
+    hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)p.q.slots * a.KV)), dim3(C::NTH), C::LDS, s, a, g, p.q);
+    PT_LAUNCH_CHECK();
+    return PTCG_OK;
+}
+template <typename T, int DH, int NK> int launch_dkv(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
+    typedef DkvCfg<T, DH, NK> C;
+    auto kern = seq_dkv_kernel<T, DH, NK>;
+    PT_TRY(lds_attr(kern, C::LDS));
+    const int64_t pairs = (int64_t)a.n * a.KV;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(pairs * (p.k.ktiles + p.k.first * p.k.chunks))), dim3(C::NTH), C::LDS, s, a,
+                       g, p.k);
+    PT_LAUNCH_CHECK();
+    if (p.k.first) {
+        hipLaunchKernelGGL(seq_first_kernel<T>, dim3(pt_cdiv(pairs * p.k.first * C::BKEY * 2 * (a.dh / 4), 256)), dim3(256),
+                           0, s, a, g.part, g.dk, g.dv, p.k, C::BKEY);
+        PT_LAUNCH_CHECK();
+    }
+    return PTCG_OK;
+}
+template <typename T, int DH> int run_bwd(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
+    PT_TRY(p.nw == 2 ? (launch_dq<T, DH, 2>(a, p, g, s)) : (launch_dq<T, DH, 4>(a, p, g, s)));
+    if constexpr (sizeof(T) == 2 || DH <= 64)
+        if (p.nk == 2) return launch_dkv<T, DH, 2>(a, p, g, s);
+    return launch_dkv<T, DH, 4>(a, p, g, s);
+}
+template <typename T>
+int bwd_dh(const SArgs& a, const BwdPlan& p, const void* q, const void* k, const void* v, const void* out,
+           const float* lse, const void* dout, void* dq, void* dk, void* dv, float* ws, hipStream_t s) {
+    const Grads<T> g = {static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
+                        static_cast<const T*>(out), static_cast<const T*>(dout), lse, static_cast<T*>(dq),
+                        static_cast<T*>(dk), static_cast<T*>(dv), ws, ws + p.delta};
+    return a.dh <= 32 ? run_bwd<T, 32>(a, p, g, s) : a.dh <= 64 ? run_bwd<T, 64>(a, p, g, s) : run_bwd<T, 128>(a, p, g, s);
+}
+
 }  // namespace
 
 extern "C" int64_t ptcg_kernel_paged_attention_ws_bytes(const PtcgPagedAttn* d) {
@@ -864,6 +1289,10 @@ extern "C" int64_t ptcg_kernel_window_attention_ws_bytes(const PtcgWindowAttn* d
     if (check_window(d, "window_attention_ws_bytes") != PTCG_OK) return -1;
     if (d->n == 0 || d->l == 0) return 0;
     const SArgs a = window_args(d);
+    if (backward) {
+        const BwdPlan p = bwd_plan(d, a);
+        return (p.delta + p.part) * 4;
+    }
     return part_bytes(window_form(d, a), a);
 }
 
@@ -888,5 +1317,25 @@ extern "C" int ptcg_kernel_window_attention_fwd(const PtcgWindowAttn* d, const v
 extern "C" int ptcg_kernel_window_attention_bwd(const PtcgWindowAttn* d, const void* q, const void* k, const void* v,
                                                 const void* out, const float* lse, const void* dout, void* dq, void* dk,
                                                 void* dv, void* workspace, int64_t workspace_bytes, void* stream) {
-    PT_REQUIRE(false, "window_attention_bwd: not built yet");
+    const char* who = "window_attention_bwd";
+    PT_TRY(check_window(d, who));
+    if (d->n == 0 || d->l == 0) return PTCG_OK;
+    PT_REQUIRE(q && k && v && out && lse && dout && dq && dk && dv, "%s: null buffer", who);
+    PT_REQUIRE(al16(q) && al16(k) && al16(v) && al16(out) && al16(dout) && al16(dq) && al16(dk) && al16(dv),
+               "%s: buffers must be 16 B aligned", who);
+    PT_REQUIRE(layout_apart(d->q, d->off, d->n, d->l, d->heads, d->dh),
+               "%s: rows of dq overlap (a broadcast q has no gradient layout)", who);
+    PT_REQUIRE(layout_apart(d->k, d->off, d->n, d->l, d->kv_heads, d->dh) &&
+                   layout_apart(d->v, d->off, d->n, d->l, d->kv_heads, d->dh),
+               "%s: rows of dk or dv overlap (broadcast keys have no gradient layout)", who);
+    const SArgs a = window_args(d);
+    const BwdPlan p = bwd_plan(d, a);
+    const int64_t need = (p.delta + p.part) * 4;
+    PT_REQUIRE(workspace && workspace_bytes >= need && al16(workspace),
+               "%s: workspace of %lld bytes, need %lld (16 B aligned)", who, (long long)workspace_bytes,
+               (long long)need);
+    float* ws = static_cast<float*>(workspace);
+    const hipStream_t s = (hipStream_t)stream;
+    return d->bf16 ? bwd_dh<__bf16>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s)
+                   : bwd_dh<float>(a, p, q, k, v, out, lse, dout, dq, dk, dv, ws, s);
 }

@@ -111,6 +111,14 @@ template <typename T, int DH> struct Row {
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c) x[c].terms(f[c]);
     }
+    // the loads end here: in a loop that first uses them the compiler would wait for
+    // everything on its way, each time round
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int c = 0; c < DH / 16; ++c)
+#pragma unroll
+            for (int p = 0; p < planes<T>(); ++p) asm volatile("" : "+v"(f[c][p]));
+    }
 };
 
 // LDS rows are ST elements apart and chunk c (8 values) of a row lies at

@@ -32,7 +32,8 @@ struct SArgs {
     long table_sn;
     int pages, page, per_seq;
     int all_rows;                 // rows of the packed matrices
-    double inv_page;
+    unsigned pmagic;              // key / page = umulhi(key, pmagic) >> pshift (page > 1)
+    int pshift;
 };
 
 // A sequence: element offsets of row 0, its live rows, the rows that are written (a
@@ -88,17 +89,19 @@ __device__ __forceinline__ Places places_of(const SArgs& a, const Seq& s, int r0
     return {s.p0 + q0, q1 < q0 ? -1 : s.p0 + q1};
 }
 
-// What a workgroup works on: sequence, row tile, split of the tile's key blocks
-// (per of them), and the sequence's splits and first slot.
-struct Work { int i, qt, sp, per, splits, first; };
+// What a workgroup works on: sequence, row tile, split of the tile's key blocks (per of
+// them a split), the sequence's splits and first slot; the tile's number among all
+// (tiles of them, where there are splits).
+struct Work { int i, qt, sp, per, splits, first, tile, tiles; };
 
 // Slots are handed out on the device, which alone knows the lengths: sequence i has
 // T_i row tiles of at most K_i key blocks; a split takes so many blocks that sum T_i
-// ceil(K_i / per) <= slots, so that every workgroup has one piece of nearly equal
-// length however the sequences differ.  Every wave counts for itself, 64
-// sequences at a time.  by_tile: slot counts tiles, not splits.  i = -1: a slot too many.
+// ceil(K_i / per) <= slots, the fewest such (searched for up to 64 sequences), and a
+// sequence's splits are made equal: every workgroup has one piece of nearly the same
+// length however the sequences differ.  Every wave counts for itself, 64 sequences at
+// a time.  i = -1: a slot too many.
 template <bool PAGED, int BQ, int BK>
-__device__ __forceinline__ Work work_of(const SArgs& a, int slot, int slots, int least, bool split, bool by_tile) {
+__device__ __forceinline__ Work work_of(const SArgs& a, int slot, int slots, int least, bool split) {
     const int lane = threadIdx.x & 63;
     auto shape = [&](int i, int& t, int& k) {
         t = k = 0;
@@ -111,33 +114,44 @@ __device__ __forceinline__ Work work_of(const SArgs& a, int slot, int slots, int
         if (a.window < INT_MAX - 4 * BQ)
             k = min(k, (a.window + (BQ + a.G - 2) / a.G) / BK + 2 + (min(a.sinks, s.kl) + BK - 1) / BK);
     };
-    int per = INT_MAX;
+    auto sum = [](int x) {
+        for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+        return x;
+    };
+    auto over = [](int k, int per) { return max(1, (k - 1) / per + 1); };      // splits
+    int per = INT_MAX, st = 0, t, k;
     if (split) {
-        int st = 0;
-        float sk = 0.f;      // counts of blocks: only a length that need not be exact comes of them
+        float sk = 0.f;      // counts of blocks: only bounds of the search come of them
         for (int i0 = 0; i0 < a.n; i0 += 64) {
-            int t, k;
             shape(i0 + lane, t, k);
             st += t;
             sk += (float)t * (float)k;
         }
-        for (int o = 1; o < 64; o <<= 1) {
-            st += __shfl_xor(st, o, 64);
-            sk += __shfl_xor(sk, o, 64);
+        st = sum(st);
+        for (int o = 1; o < 64; o <<= 1) sk += __shfl_xor(sk, o, 64);
+        if (slots > st) {
+            per = (int)fminf(sk * 1.0001f / (float)(slots - st) + 1.f, 1e9f);
+            if (a.n <= 64) {
+                int lo = max(1, (int)(sk * 0.9999f / (float)slots));      // too few, or just enough
+                while (per - lo > 1 + lo / 32) {
+                    const int mid = lo + (per - lo) / 2;
+                    if (sum(t * over(k, mid)) <= slots) per = mid;
+                    else lo = mid;
+                }
+            }
+            per = max(per, least);
         }
-        if (slots > st) per = max(least, (int)fminf(sk * 1.0001f / (float)(slots - st) + 1.f, 1e9f));
     }
-    int before = 0, pieces = 0;
+    int before = 0, tiles = 0;
     for (int i0 = 0; i0 < a.n; i0 += 64) {
-        int t, k;
-        shape(i0 + lane, t, k);
-        const int s = max(1, (k - 1) / per + 1), c = by_tile ? t : t * s;
-        int to = c, pt = t * s;
+        if (!split || a.n > 64) shape(i0 + lane, t, k);
+        const int s = over(k, per), c = t * s;
+        int to = c, tt = t;
         for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(to, o, 64), y = __shfl_up(pt, o, 64);
+            const int x = __shfl_up(to, o, 64), y = __shfl_up(tt, o, 64);
             if (lane >= o) {
                 to += x;
-                pt += y;
+                tt += y;
             }
         }
         const unsigned long long m = __ballot(slot >= before + to - c && slot < before + to);
@@ -145,25 +159,36 @@ __device__ __forceinline__ Work work_of(const SArgs& a, int slot, int slots, int
             const int w = __builtin_ctzll(m);
             Work r;
             r.i = i0 + w;
-            r.per = per;
             r.splits = __builtin_amdgcn_readlane(s, w);
-            const int rest = slot - (before + __builtin_amdgcn_readlane(to - c, w));
-            r.first = pieces + __builtin_amdgcn_readlane(pt - t * s, w);
-            const int tiles = __builtin_amdgcn_readlane(t, w);
+            r.first = before + __builtin_amdgcn_readlane(to - c, w);
+            const int nt = __builtin_amdgcn_readlane(t, w), rest = slot - r.first;
+            r.per = r.splits > 1 ? (__builtin_amdgcn_readlane(k, w) - 1) / r.splits + 1 : INT_MAX;
             // the last tile first: its rows see the most
-            r.qt = by_tile ? rest : tiles - 1 - rest / r.splits;
-            r.sp = by_tile ? 0 : rest % r.splits;
+            r.qt = nt - 1 - rest / r.splits;
+            r.sp = rest % r.splits;
+            r.tile = tiles + __builtin_amdgcn_readlane(tt - t, w) + r.qt;
+            r.tiles = st;
             return r;
         }
         before += __builtin_amdgcn_readlane(to, 63);
-        pieces += __builtin_amdgcn_readlane(pt, 63);
+        tiles += __builtin_amdgcn_readlane(tt, 63);
     }
-    return {-1, 0, 0, 0, 0, 0};
+    return {-1, 0, 0, 0, 0, 0, 0, st};
+}
+// the same in scalar registers, as it is one for all lanes
+__device__ __forceinline__ Work uniform(const Work& w) {
+    auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    return {u(w.i), u(w.qt), u(w.sp), u(w.per), u(w.splits), u(w.first), u(w.tile), u(w.tiles)};
 }
 // where a split leaves its part: slot of its piece
 __device__ __forceinline__ int piece_of(const Work& w, int tiles, int qt, int sp) {
     return w.first + (tiles - 1 - qt) * w.splits + sp;
 }
+// What the joining kernel is told: a tile's sequence, number in it, first piece and splits
+// (1: nothing to join); before the first, how many tiles there are.
+struct Joint { int i, qt, piece, splits; };
+// a piece's rows, unnormalised, then their maxima and sums
+__host__ __device__ constexpr long piece_floats(int prow, int dh) { return ((long)prow * (dh + 2) + 3) / 4 * 4; }
 
 // Scores of keys that a row of place p does not see become -inf, whatever they are:
 // register e is key k0 + 8 (e / 4) + e % 4.  last: the lesser of p and the last key.
@@ -187,13 +212,18 @@ __device__ __forceinline__ bool all_hidden(const SArgs& a, int k0, int nk, int l
 // Byte-free address of key row `key`: element offset of its row, and whether there
 // is one.  ent: its page-table entry (paged).
 __device__ __forceinline__ int page_of(const SArgs& a, int key) {
-    return (int)(((double)key + 0.5) * a.inv_page);      // exact below 2^30
+    return a.page == 1 ? key : (int)(__umulhi((unsigned)key, a.pmagic) >> a.pshift);      // exact below 2^31
 }
 __device__ __forceinline__ int entry_of(const SArgs& a, const Seq& s, int key, int kend) {
     return key < kend ? s.table[page_of(a, key)] : -1;
 }
 
-// A running softmax of the rows on lanes: maximum m2 (of s scale2), this half's sum l.
+// A running softmax of the rows on lanes: m2, a bound of the scores (s scale2) so far
+// that was their maximum when it was last set, and this half's sum l of exp2(s scale2 -
+// m2).  Where a score passes m2 by 8 or more, m2 moves up and what is summed is
+// rescaled; below, exponentials reach 2^8, which costs fp32 sums and bf16 products
+// nothing, and the rescaling (a multiplication per output) falls away in most tiles.
+constexpr float SLACK = 8.f;
 template <int DH> struct Soft {
     float m2, l;
     floatx16 o[DH / 32];
@@ -214,7 +244,7 @@ template <int DH> struct Soft {
             for (int e = 0; e < 16; ++e) mt = fmaxf(mt, sc[j][e]);
         mt = fmaxf(mt, half_swap(mt));
         const float mn = fmaxf(m2, mt * scale2);
-        if (__any(mn > m2)) {
+        if (__any(mn > m2 + SLACK)) {
             const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m2 - mn);
             l *= al;
 #pragma unroll
@@ -233,6 +263,32 @@ template <int DH> struct Soft {
             }
     }
 };
+
+// S^T of 64 keys in LDS (bf16).  Operands are asked for four products ahead: left to
+// itself the compiler reads each one just before its product and waits.
+template <int DH>
+__device__ __forceinline__ void scores(const __bf16* ks, const Row<__bf16, DH>& q, floatx16 (&sc)[2], int lane) {
+    typedef Lds<DH, false> L;
+    constexpr int N = DH / 8, AHEAD = N < 4 ? N : 4;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[j][e] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DH / 16; ++c)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const bf16x8 x = *reinterpret_cast<const bf16x8*>(ks + 32 * j * L::ST + L::chunk_at(lane & 31, lane >> 5, c));
+            sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q.f[c][0], sc[j], 0, 0, 0);
+        }
+    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
 
 // What a tile's rows come to: their output, or their split's part for the joining
 // kernel (unnormalised, with maximum and sum).  rows: rows of the sequence.
@@ -334,10 +390,81 @@ template <typename T, int DH, bool PAD, int BK, int NTH, bool PAGED> struct KvRe
     }
 };
 
-template <typename T, int DH, int NW> struct TileCfg {
+// 16 bytes a lane from memory into LDS, lane L's to base + 16 L; zeros past the
+// descriptor's end.  Issued from assembly so that the compiler does not tie LDS reads
+// to loads on their way; who reads waits (arrived) and meets the others at a barrier.
+typedef int intx4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void to_lds(intx4 rs, const __bf16* base, int off) {
+    const unsigned at = (unsigned)(uintptr_t)base;      // LDS offset: low bits of the generic address
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(rs) : "memory");
+}
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// A tile of BK keys and values by 16-byte pieces straight into LDS (bf16): every wave
+// brings BK / NW rows that lie in one matrix, or in one page (whose size is a multiple
+// of them).  A piece's place in LDS is its lane's, so the lane chooses the chunk that
+// belongs there.
+template <int DH, int BK, int NW, bool PAGED> struct KvDma {
+    typedef Lds<DH, false> L;
+    static constexpr int CPR = DH / 8, WR = BK / NW, RPI = 64 / CPR, NI = WR / RPI;   // rows a wave, an instruction
+    static_assert(WR % RPI == 0, "whole instructions");
+    int ko[NI], vo[NI], kld, vld, kw, vw, row;
+    const char *kb, *vb;
+    int ent;
+    __device__ __forceinline__ void init(const SArgs& a, const Seq& s, const __bf16* k, const __bf16* v, int kvh,
+                                         int tid) {
+        const int lane = tid & 63;
+        row = __builtin_amdgcn_readfirstlane(tid >> 6) * WR;
+        kld = (int)a.k.sl * 2;
+        vld = (int)a.v.sl * 2;
+        kb = reinterpret_cast<const char*>(k + (PAGED ? 0 : s.k) + (long)kvh * a.k.sh);
+        vb = reinterpret_cast<const char*>(v + (PAGED ? 0 : s.v) + (long)kvh * a.v.sh);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int r = i * RPI + lane / CPR, c = (lane % CPR) ^ L::swz(row + r);
+            const bool in = 8 * c < a.dh;
+            ko[i] = in ? r * kld + 16 * c : PT_NOWHERE;
+            vo[i] = in ? r * vld + 16 * c : PT_NOWHERE;
+        }
+        kw = vw = 2 * a.dh;
+    }
+    // the page-table entry that fetch(block) will need
+    __device__ __forceinline__ void look(const SArgs& a, const Seq& s, int block, int kend) {
+        if constexpr (PAGED) ent = entry_of(a, s, block * BK + row, kend);
+    }
+    static __device__ __forceinline__ intx4 rsrc(const char* p, int bytes) {
+        const unsigned long long x = (unsigned long long)p;
+        return intx4{__builtin_amdgcn_readfirstlane((int)(unsigned)x),
+                     __builtin_amdgcn_readfirstlane((int)(unsigned)(x >> 32)), __builtin_amdgcn_readfirstlane(bytes),
+                     0x00020000};
+    }
+    __device__ __forceinline__ void fetch(const SArgs& a, int block, int kend, __bf16* Ks, __bf16* Vs) const {
+        const int key = block * BK + row;
+        int n = max(0, min(kend - key, WR));
+        const char *kp = kb, *vp = vb;
+        if constexpr (PAGED) {
+            const bool is = (unsigned)ent < (unsigned)a.pages;
+            if (!is) n = 0;
+            const long e = is ? ent : 0, off = is ? key - page_of(a, key) * a.page : 0;
+            kp += (e * a.k.sn + off * a.k.sl) * 2;
+            vp += (e * a.v.sn + off * a.v.sl) * 2;
+        } else {
+            kp += (long)key * kld;
+            vp += (long)key * vld;
+        }
+        const intx4 rk = rsrc(kp, n ? (n - 1) * kld + kw : 0), rv = rsrc(vp, n ? (n - 1) * vld + vw : 0);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) to_lds(rk, Ks + (row + i * RPI) * L::ST, ko[i]);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) to_lds(rv, Vs + (row + i * RPI) * L::ST, vo[i]);
+    }
+};
+
+template <typename T, int DH, int NW, bool DMA> struct TileCfg {
     static constexpr int NTH = 64 * NW, BQ = 32 * NW, BK = 64;
     static constexpr int TILE = tile_elems<T, DH, false, BK>();
-    static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
+    static constexpr size_t PAIR = (DMA ? 2 : 1) * 4 * (size_t)TILE;   // bytes; DMA: two buffers
     static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);
     static constexpr size_t BUFS = PAIR > OUT ? PAIR : OUT;
     static constexpr size_t LDS = BUFS + BK * sizeof(float) + 64;
@@ -349,16 +476,17 @@ template <typename T, int DH> constexpr int waves_simd() { return sizeof(T) == 2
 struct Plan { int slots, tiles, qtiles, least, prow; bool even, split; };
 
 // A workgroup owns 32 NW rows and walks their key blocks (or its split of them).
-template <typename T, int DH, int NW, bool PAGED>
+// DMA: tiles go straight into one of two buffers while the other is worked on, one
+// barrier a tile; else through registers into one buffer.
+template <typename T, int DH, int NW, bool PAGED, bool DMA>
 __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel(const SArgs a, const T* __restrict__ q,
         const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
         float* __restrict__ part, const Plan pl) {
-    typedef TileCfg<T, DH, NW> C;
+    typedef TileCfg<T, DH, NW, DMA> C;
     typedef KvRegs<T, DH, false, C::BK, C::NTH, PAGED> Kv;
     constexpr int PS = Kv::St::PS, BK = C::BK, BQ = C::BQ;
     extern __shared__ __align__(256) char smem[];
-    __bf16* Ks = reinterpret_cast<__bf16*>(smem);
-    __bf16* Vs = Ks + C::TILE;
+    __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     float* kf = reinterpret_cast<float*>(smem + C::BUFS);
     int* bad = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
@@ -368,11 +496,14 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     if (pl.even) {
         const int u = l / pl.qtiles;
         kvh = u % a.KV;
-        w = {u / a.KV, pl.qtiles - 1 - l % pl.qtiles, 0, INT_MAX, 1, 0};
+        w = {u / a.KV, pl.qtiles - 1 - l % pl.qtiles, 0, INT_MAX, 1, 0, 0, 0};
     } else {
         kvh = l / pl.slots;
-        w = work_of<PAGED, BQ, BK>(a, l % pl.slots, pl.slots, pl.least, pl.split, false);
+        w = work_of<PAGED, BQ, BK>(a, l % pl.slots, pl.slots, pl.least, pl.split);
     }
+    w = uniform(w);
+    Joint* const js = reinterpret_cast<Joint*>(part);      // then the parts
+    if (pl.split && blockIdx.x == 0 && tid == 0) js[0].i = w.tiles;
     if (w.i < 0) return;
     const Seq s = seq_of<PAGED>(a, w.i);
     const int rows = s.rows * a.G, tile0 = w.qt * BQ;
@@ -380,9 +511,11 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
     const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
     const bool joined = rg.nt > w.per;                    // by the joining kernel
+    if (pl.split && w.sp == 0 && kvh == 0 && tid == 0)
+        js[1 + w.tile] = {w.i, w.qt, piece_of(w, (rows + BQ - 1) / BQ, w.qt, 0), joined ? (rg.nt - 1) / w.per + 1 : 1};
     const int t0 = joined ? w.sp * w.per : 0, t1 = joined ? min(rg.nt, t0 + w.per) : rg.nt;
     if (joined ? t0 >= rg.nt : w.sp > 0) return;
-    if (tid == 0) *bad = 0;
+    if (PAGED && tid == 0) *bad = 0;
 
     const int r0 = tile0 + 32 * wave, r = r0 + (lane & 31);
     const bool rok = r < rows;
@@ -396,56 +529,100 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     Soft<DH> f;
     f.init();
 
-    Kv kv;
-    kv.init(a, s, k, v, kvh, tid);
-    auto fetch = [&](int t) {
-        kv.fetch(a, s, k, v, kvh, rg.block(t), rg.kend, tid);
-        if (t + 1 < t1) kv.look(a, s, rg.block(t + 1), rg.kend, tid);
-    };
-    if (t0 < t1) {
-        kv.look(a, s, rg.block(t0), rg.kend, tid);
-        fetch(t0);
-        __syncthreads();      // *bad is cleared
-        kv.store(Ks, Vs, kf, bad, tid);
-        if (t0 + 1 < t1) fetch(t0 + 1);
-        __syncthreads();
-    }
-    for (int t = t0; t < t1; ++t) {
+    qf.settle();
+    // tile t's block from Ks on; nopage: its keys of no page, by lanes
+    auto tile = [&](int t, const __bf16* Ks, unsigned long long nopage) {
+        const __bf16* Vs = Ks + C::TILE;
         const int key0 = rg.block(t) * BK;
-        if (sees && !all_hidden(a, key0, BK, wlo, whi)) {
-            floatx16 sc[BK / 32];
+        if (!sees || all_hidden(a, key0, BK, wlo, whi)) return;
+        floatx16 sc[BK / 32];
+        if constexpr (sizeof(T) == 2) {
+            scores<DH>(Ks, qf, sc, lane);
+        } else {
 #pragma unroll
             for (int j = 0; j < BK / 32; ++j)
                 sc[j] = mma_rows<T, DH, false, PS>(Ks + 32 * j * Lds<DH, false>::ST, qf, lane);
-            if (dead || key0 + BK > rg.kend || some_hidden(a, key0, BK, wlo, whi)) {
+        }
+        if (dead || key0 + BK > rg.kend || some_hidden(a, key0, BK, wlo, whi)) {
 #pragma unroll
-                for (int j = 0; j < BK / 32; ++j) hide(a, sc[j], key0 + 32 * j + 4 * h, p, last);
-            }
-            if constexpr (PAGED)
-                if (*bad) {
-#pragma unroll
-                    for (int j = 0; j < BK / 32; ++j)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            if (kf[32 * j + 8 * (e / 4) + 4 * h + e % 4] != 0.f) sc[j][e] = -INFINITY;
-                }
-            f.step(sc, a.scale2);
+            for (int j = 0; j < BK / 32; ++j) hide(a, sc[j], key0 + 32 * j + 4 * h, p, last);
+        }
+        if (PAGED && nopage) {
 #pragma unroll
             for (int j = 0; j < BK / 32; ++j)
-                mma_tr<T, DH, false, PS>(Vs + 32 * j * Lds<DH, false>::ST, sc[j], f.o, lane);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (nopage >> (32 * j + 8 * (e / 4) + 4 * h + e % 4) & 1) sc[j][e] = -INFINITY;
         }
-        __syncthreads();
-        if (t + 1 < t1) {
+        f.step(sc, a.scale2);
+#pragma unroll
+        for (int j = 0; j < BK / 32; ++j)
+            mma_tr<T, DH, false, PS>(Vs + 32 * j * Lds<DH, false>::ST, sc[j], f.o, lane);
+    };
+    if constexpr (DMA) {
+        static_assert(sizeof(T) == 2 && BK == 64, "");
+        KvDma<DH, BK, NW, PAGED> kv;
+        kv.init(a, s, k, v, kvh, tid);
+        auto fetch = [&](int t) {
+            __bf16* to = tiles + (t - t0 & 1) * 2 * C::TILE;
+            kv.fetch(a, rg.block(t), rg.kend, to, to + C::TILE);
+            if (t + 1 < t1) kv.look(a, s, rg.block(t + 1), rg.kend);
+        };
+        auto lacks = [&](int t) {       // a lane per key
+            const int key = rg.block(t) * BK + lane;
+            return key < rg.kend && (unsigned)s.table[page_of(a, key)] >= (unsigned)a.pages;
+        };
+        if (t0 < t1) {
+            kv.look(a, s, rg.block(t0), rg.kend);
+            fetch(t0);
+        }
+        bool some = false;         // any key of no page: only then tiles look for them
+        if constexpr (PAGED) {
+            for (int t = t0 + wave; t < t1; t += NW) some |= lacks(t);
+            some = __syncthreads_or(some);
+        }
+        for (int t = t0; t < t1; ++t) {
+            arrived();
+            __syncthreads();       // everyone's pieces of tile t are here, and tile t - 1 is done with
+            if (t + 1 < t1) fetch(t + 1);
+            unsigned long long nopage = 0;
+            if (PAGED && some) nopage = __ballot(lacks(t));
+            tile(t, tiles + (t - t0 & 1) * 2 * C::TILE, nopage);
+        }
+        __syncthreads();           // the buffers become the rows' way out
+    } else {
+        __bf16 *Ks = tiles, *Vs = tiles + C::TILE;
+        Kv kv;
+        kv.init(a, s, k, v, kvh, tid);
+        auto fetch = [&](int t) {
+            kv.fetch(a, s, k, v, kvh, rg.block(t), rg.kend, tid);
+            if (t + 1 < t1) kv.look(a, s, rg.block(t + 1), rg.kend, tid);
+        };
+        if (t0 < t1) {
+            kv.look(a, s, rg.block(t0), rg.kend, tid);
+            fetch(t0);
+            __syncthreads();      // *bad is cleared
             kv.store(Ks, Vs, kf, bad, tid);
-            if (t + 2 < t1) fetch(t + 2);
+            if (t0 + 1 < t1) fetch(t0 + 1);
             __syncthreads();
+        }
+        for (int t = t0; t < t1; ++t) {
+            unsigned long long nopage = 0;
+            if (PAGED && *bad) nopage = __ballot(kf[lane] != 0.f);
+            tile(t, Ks, nopage);
+            __syncthreads();
+            if (t + 1 < t1) {
+                kv.store(Ks, Vs, kf, bad, tid);
+                if (t + 2 < t1) fetch(t + 2);
+                __syncthreads();
+            }
         }
     }
     f.l += half_swap(f.l);
-    const int tiles = (rows + BQ - 1) / BQ;
+    const int tiles_ = (rows + BQ - 1) / BQ;
     float* pp = nullptr;
     if (joined)
-        pp = part + ((long)piece_of(w, tiles, w.qt, w.sp) * a.KV + kvh) * pl.prow * (a.dh + 2);
+        pp = part + 4 * (1 + pl.tiles) + ((long)piece_of(w, tiles_, w.qt, w.sp) * a.KV + kvh) * piece_floats(pl.prow, a.dh);
     if (live)
         finish<T, DH, BQ>(a, s, w.i, kvh, tile0, r0, f, out, lse, pp, pl.prow,
                           reinterpret_cast<T*>(smem) + wave * Out<T, DH>::WAVE, lane);
@@ -477,8 +654,11 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
     __bf16* Vs = reinterpret_cast<__bf16*>(smem) + wave * C::TILE;
     const int kvh = blockIdx.x % a.KV, slot = blockIdx.x / a.KV;
     Work w;
-    if (pl.even) w = {slot / pl.qtiles, pl.qtiles - 1 - slot % pl.qtiles, 0, INT_MAX, 1, 0};
-    else w = work_of<PAGED, BQ, BK>(a, slot, pl.slots, pl.least, pl.split, false);
+    if (pl.even) w = {slot / pl.qtiles, pl.qtiles - 1 - slot % pl.qtiles, 0, INT_MAX, 1, 0, 0, 0};
+    else w = work_of<PAGED, BQ, BK>(a, slot, pl.slots, pl.least, pl.split);
+    w = uniform(w);
+    Joint* const js = reinterpret_cast<Joint*>(part);      // then the parts
+    if (pl.split && blockIdx.x == 0 && tid == 0) js[0].i = w.tiles;
     if (w.i < 0) return;
     const Seq s = seq_of<PAGED>(a, w.i);
     const int rows = s.rows * a.G, tile0 = w.qt * BQ;
@@ -486,6 +666,8 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
     const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
     const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
     const bool joined = rg.nt > w.per;
+    if (pl.split && w.sp == 0 && kvh == 0 && tid == 0)
+        js[1 + w.tile] = {w.i, w.qt, piece_of(w, (rows + BQ - 1) / BQ, w.qt, 0), joined ? (rg.nt - 1) / w.per + 1 : 1};
     const int t0 = joined ? w.sp * w.per : 0, t1 = joined ? min(rg.nt, t0 + w.per) : rg.nt;
     if (joined ? t0 >= rg.nt : w.sp > 0) return;
 
@@ -605,7 +787,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
     }
     float* pp = nullptr;
     if (joined)
-        pp = part + ((long)piece_of(w, (rows + BQ - 1) / BQ, w.qt, w.sp) * a.KV + kvh) * pl.prow * (a.dh + 2);
+        pp = part + 4 * (1 + pl.tiles) + ((long)piece_of(w, (rows + BQ - 1) / BQ, w.qt, w.sp) * a.KV + kvh) * piece_floats(pl.prow, a.dh);
     finish<T, DH, BQ>(a, s, w.i, kvh, tile0, tile0, f, out, lse, pp, pl.prow, reinterpret_cast<T*>(smem), lane);
 }
 
@@ -614,7 +796,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
 // groups of LG lanes (4 columns each) take a row's splits in turn, per_row groups a
 // row, and meet in LDS in group order.
 constexpr int JOIN_NTH = 512;
-template <typename T, int LG, bool PAGED, int BQ, int BK>
+template <typename T, int LG, bool PAGED, int BQ>
 __global__ __launch_bounds__(JOIN_NTH) void seq_join_kernel(const SArgs a, const float* __restrict__ part,
         T* __restrict__ out, float* __restrict__ lse, const Plan pl, int per_row, int rgroups) {
     constexpr int NG = JOIN_NTH / LG;
@@ -622,14 +804,13 @@ __global__ __launch_bounds__(JOIN_NTH) void seq_join_kernel(const SArgs a, const
     __shared__ float2 shm[NG];
     const int tid = threadIdx.x, grp = tid / LG, c = tid % LG, g0 = grp & (per_row - 1);
     const int rg_ = blockIdx.x % rgroups, kvh = blockIdx.x / rgroups % a.KV, tile = blockIdx.x / rgroups / a.KV;
-    const Work w = work_of<PAGED, BQ, BK>(a, tile, pl.slots, pl.least, pl.split, true);
-    if (w.i < 0) return;
+    const Joint* js = reinterpret_cast<const Joint*>(part);
+    if (tile >= js[0].i) return;
+    const Joint w = js[1 + tile];
+    const int nsp = w.splits;
+    if (nsp <= 1) return;        // made by one workgroup
     const Seq s = seq_of<PAGED>(a, w.i);
-    const int rows = s.rows * a.G, tile0 = w.qt * BQ, tiles = (rows + BQ - 1) / BQ;
-    const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
-    const int nt = range_of<BK>(a, pt.lo, pt.hi, s.kl).nt;
-    if (nt <= w.per) return;        // made by one workgroup
-    const int nsp = (nt - 1) / w.per + 1;
+    const int rows = s.rows * a.G, tile0 = w.qt * BQ;
     const int row = rg_ * (NG / per_row) + grp / per_row, r = tile0 + row;
     const bool live = row < BQ && r < rows;
     float m = -INFINITY, l = 0.f;
@@ -644,8 +825,8 @@ __global__ __launch_bounds__(JOIN_NTH) void seq_join_kernel(const SArgs a, const
         acc.z = acc.z * f0 + x.z * f1; acc.w = acc.w * f0 + x.w * f1;
     };
     if (live) {
-        const long stride = (long)a.KV * pl.prow * (a.dh + 2);
-        const float* p0 = part + ((long)piece_of(w, tiles, w.qt, 0) * a.KV + kvh) * pl.prow * (a.dh + 2);
+        const long stride = (long)a.KV * piece_floats(pl.prow, a.dh);
+        const float* p0 = part + 4 * (1 + pl.tiles) + ((long)w.piece * a.KV + kvh) * piece_floats(pl.prow, a.dh);
 #pragma unroll 4
         for (int u = g0; u < nsp; u += per_row) {
             const float* x = p0 + u * stride;
@@ -712,11 +893,12 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     if (pl.even) {
         const int u = l / pl.qtiles;
         kvh = u % a.KV;
-        w = {u / a.KV, pl.qtiles - 1 - l % pl.qtiles, 0, INT_MAX, 1, 0};
+        w = {u / a.KV, pl.qtiles - 1 - l % pl.qtiles, 0, INT_MAX, 1, 0, 0, 0};
     } else {
         kvh = l / pl.slots;
-        w = work_of<false, BQ, BK>(a, l % pl.slots, pl.slots, 0, false, false);
+        w = work_of<false, BQ, BK>(a, l % pl.slots, pl.slots, 0, false);
     }
+    w = uniform(w);
     if (w.i < 0) return;
     const Seq s = seq_of<false>(a, w.i);
     const int rows = s.rows * a.G, tile0 = w.qt * BQ;
@@ -1068,7 +1250,12 @@ SArgs paged_args(const PtcgPagedAttn* d) {
     a.q_off = d->q_off; a.len = d->len; a.all_rows = d->rows;
     a.table = d->cache.table; a.table_sn = d->n > 1 ? d->cache.table_sn : 0;
     a.pages = d->cache.pages; a.page = d->cache.page; a.per_seq = d->cache.per_seq;
-    a.inv_page = 1.0 / d->cache.page;
+    // m = ceil(2^(31 + b) / page) with 2^(b - 1) < page <= 2^b: m < 2^32, and key m / 2^(31 +
+    // b) is above key / page by less than key / 2^31 / page < 1 / page
+    int b = 1;
+    while ((1LL << b) < a.page) ++b;
+    a.pmagic = (unsigned)(((1ULL << (31 + b)) + a.page - 1) / a.page);
+    a.pshift = b - 1;
     return a;
 }
 SArgs window_args(const PtcgWindowAttn* d) {
@@ -1084,6 +1271,7 @@ SArgs window_args(const PtcgWindowAttn* d) {
 // of 32.  Else tiles of 64 or 128 rows.
 struct Form {
     bool token;
+    bool dma;        // tiles straight into LDS: bf16 rows of one matrix, or of pages that a wave's rows never leave
     int waves;       // along the keys (token), along the rows else
     int bq, bk;
     Plan p;
@@ -1096,19 +1284,30 @@ Form form_of(const SArgs& a, int64_t packed_rows, int64_t keys, bool bf16, bool 
     f.waves = f.token ? (keys > 128 ? 4 : 1) : rows <= 64 ? 2 : 4;
     f.bq = f.token ? 32 : 32 * f.waves;
     f.bk = f.token ? 32 : 64;
+    f.dma = bf16;
+    if (a.page) {
+        auto fits = [&](const PtcgHeadLayout& l) { return l.sl < (1 << 22) && (l.sl == 0 || l.sl >= a.dh || a.page == 1); };
+        f.dma = f.dma && a.page % (f.bk / f.waves) == 0 && fits(a.k) && fits(a.v);
+    }
     const int qtiles = pt_cdiv(rows, f.bq);
     int64_t tiles = (int64_t)a.n * qtiles;
     if (a.q_off) {       // no more than the rows there are make
         const int64_t t = packed_rows * a.G / f.bq + a.n;
         if (t < tiles) tiles = t;
     }
-    // Pieces fill the card when row tiles do not: workgroups that run at once.  A split is
+    // Where row tiles do not fill the card, pieces do: as many workgroups as run at once, twice
+    // as many where few splits a tile would leave much of a round idle.  A split is
     // two blocks a wave at least, and costs a second launch.
-    const int64_t fill = (f.token ? (bf16 || a.dh <= 64 ? 3 : 1) : (bf16 || a.dh <= 64 ? 2 : 1)) * (int64_t)cu_count();
+    const int64_t fill = (bf16 || a.dh <= 64 ? 2 : 1) * (int64_t)cu_count();
     f.p.least = f.token ? 2 * f.waves : 4;
     f.p.split = may_split && tiles * a.KV < fill && keys >= 4 * f.p.least * f.bk;
     f.p.tiles = (int)tiles;
-    f.p.slots = (int)(f.p.split ? tiles + pt_cdiv(fill, a.KV) : tiles);
+    int64_t slots = tiles;
+    if (f.p.split) {
+        const int64_t most = (tiles * a.KV * 4 > fill ? 2 * fill : fill) / a.KV;
+        if (most > slots) slots = most;
+    }
+    f.p.slots = (int)slots;
     f.p.qtiles = qtiles;
     f.p.even = !a.q_off && !f.p.split;
     f.p.prow = (int)(rows < f.bq ? rows : f.bq);
@@ -1123,33 +1322,33 @@ Form window_form(const PtcgWindowAttn* d, const SArgs& a) {
     return form_of(a, (int64_t)d->n * d->l, d->l, d->bf16, true);
 }
 int64_t part_bytes(const Form& f, const SArgs& a) {
-    return f.p.split ? (int64_t)f.p.slots * a.KV * f.p.prow * (a.dh + 2) * 4 : 0;
+    return f.p.split ? 16 * (1 + (int64_t)f.p.tiles) + (int64_t)f.p.slots * a.KV * piece_floats(f.p.prow, a.dh) * 4 : 0;
 }
 
-template <typename T, int DH, bool PAGED, int BQ, int BK>
+template <typename T, int DH, bool PAGED, int BQ>
 int launch_join(const SArgs& a, const Form& f, void* out, float* lse, const float* part, hipStream_t s) {
     constexpr int LG = DH / 4, NG = JOIN_NTH / LG;
-    // splits a tile may have: those of a lone tile that takes every slot
+    // four splits a group of lanes, as many as tiles have if they are alike
     int per_row = 1;
-    while (per_row < NG && per_row * 4 < f.p.slots) per_row *= 2;
+    while (per_row < NG && (int64_t)per_row * 4 * f.p.tiles < f.p.slots) per_row *= 2;
     const int rgroups = pt_cdiv(f.p.prow, NG / per_row);
-    hipLaunchKernelGGL((seq_join_kernel<T, LG, PAGED, BQ, BK>), dim3((unsigned)((int64_t)f.p.tiles * a.KV * rgroups)),
+    hipLaunchKernelGGL((seq_join_kernel<T, LG, PAGED, BQ>), dim3((unsigned)((int64_t)f.p.tiles * a.KV * rgroups)),
                        dim3(JOIN_NTH), 0, s, a, part, static_cast<T*>(out), lse, f.p, per_row, rgroups);
     PT_LAUNCH_CHECK();
     return PTCG_OK;
 }
 
-template <typename T, int DH, int NW, bool PAGED>
+template <typename T, int DH, int NW, bool PAGED, bool DMA>
 int launch_tiles(const SArgs& a, const Form& f, const void* q, const void* k, const void* v, void* out, float* lse,
                  float* part, hipStream_t s) {
-    typedef TileCfg<T, DH, NW> C;
-    auto kern = seq_fwd_kernel<T, DH, NW, PAGED>;
+    typedef TileCfg<T, DH, NW, DMA> C;
+    auto kern = seq_fwd_kernel<T, DH, NW, PAGED, DMA>;
     PT_TRY(lds_attr(kern, C::LDS));
     hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)f.p.slots * a.KV)), dim3(C::NTH), C::LDS, s, a,
                        static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
                        static_cast<T*>(out), lse, part, f.p);
     PT_LAUNCH_CHECK();
-    return f.p.split ? launch_join<T, DH, PAGED, C::BQ, C::BK>(a, f, out, lse, part, s) : PTCG_OK;
+    return f.p.split ? launch_join<T, DH, PAGED, C::BQ>(a, f, out, lse, part, s) : PTCG_OK;
 }
 template <typename T, int DH, int KS, bool PAGED>
 int launch_token(const SArgs& a, const Form& f, const void* q, const void* k, const void* v, void* out, float* lse,
@@ -1161,7 +1360,7 @@ int launch_token(const SArgs& a, const Form& f, const void* q, const void* k, co
                        static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
                        static_cast<T*>(out), lse, part, f.p);
     PT_LAUNCH_CHECK();
-    return f.p.split ? launch_join<T, DH, PAGED, C::BQ, C::BK>(a, f, out, lse, part, s) : PTCG_OK;
+    return f.p.split ? launch_join<T, DH, PAGED, C::BQ>(a, f, out, lse, part, s) : PTCG_OK;
 }
 template <typename T, int DH, bool PAGED>
 int launch_form(const SArgs& a, const Form& f, const void* q, const void* k, const void* v, void* out, float* lse,
@@ -1169,8 +1368,14 @@ int launch_form(const SArgs& a, const Form& f, const void* q, const void* k, con
     if (f.token)
         return f.waves == 4 ? launch_token<T, DH, 4, PAGED>(a, f, q, k, v, out, lse, part, s)
                             : launch_token<T, DH, 1, PAGED>(a, f, q, k, v, out, lse, part, s);
-    return f.waves == 2 ? launch_tiles<T, DH, 2, PAGED>(a, f, q, k, v, out, lse, part, s)
-                        : launch_tiles<T, DH, 4, PAGED>(a, f, q, k, v, out, lse, part, s);
+    if constexpr (sizeof(T) == 2)
+        if (f.dma)
+            return f.waves == 2 ? launch_tiles<T, DH, 2, PAGED, true>(a, f, q, k, v, out, lse, part, s)
+                                : launch_tiles<T, DH, 4, PAGED, true>(a, f, q, k, v, out, lse, part, s);
+    if constexpr (sizeof(T) == 4 || PAGED)
+        return f.waves == 2 ? launch_tiles<T, DH, 2, PAGED, false>(a, f, q, k, v, out, lse, part, s)
+                            : launch_tiles<T, DH, 4, PAGED, false>(a, f, q, k, v, out, lse, part, s);
+    return PTCG_OK;
 }
 template <bool PAGED>
 int run_fwd(const SArgs& a, const Form& f, bool bf16, const void* q, const void* k, const void* v, void* out, float* lse,

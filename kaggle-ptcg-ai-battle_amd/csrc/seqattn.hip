@@ -862,17 +862,49 @@ template <typename T> struct Grads {
     const T *q, *k, *v, *out, *dout;
     const float* lse;
     T *dq, *dk, *dv;
-    float *delta, *part;
+    float2* stats;
+    float* part;
 };
 
+// Both products of 32 LDS rows that a tile begins with (bf16): s0 = X0 Y0^T, s1 = X1
+// Y1^T; operands asked for ahead as in scores.  Y1 are a lane's rows in registers or
+// (yl) in LDS.
+template <int DH, bool YLDS>
+__device__ __forceinline__ void products(const __bf16* x0, const __bf16* x1, const Row<__bf16, DH>& y0,
+                                         const Row<__bf16, DH>& y1, const __bf16* yl, floatx16& s0, floatx16& s1,
+                                         int lane) {
+    typedef Lds<DH, false> L;
+    constexpr int N = DH / 16, R = YLDS ? 3 : 2, AHEAD = N < 2 ? N : 2;      // reads a step of two products
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s0[e] = s1[e] = 0.f;
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+        const int at = L::chunk_at(lane & 31, lane >> 5, c);
+        const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(x0 + at), a1 = *reinterpret_cast<const bf16x8*>(x1 + at);
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, y0.f[c][0], s0, 0, 0, 0);
+        if constexpr (YLDS)
+            s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, *reinterpret_cast<const bf16x8*>(yl + at), s1, 0, 0, 0);
+        else
+            s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, y1.f[c][0], s1, 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x100, R * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2 * AHEAD, 0);
+}
+
 // dQ: the forward's shape.  Per 32 keys S^T and dP^T = V dO^T with queries on
-// lanes, dS^T in registers, dQ^T += K^T dS^T.  Also leaves D_i for the dK / dV
-// kernel, in row order of lse.
+// lanes, dS^T in registers, dQ^T += K^T dS^T.  Also leaves each row's log-sum-exp (in
+// units of exp2; +inf for a row that sees nothing) and D_i for the dK / dV kernel, in
+// the order of its rows.
 template <typename T, int DH, int NW> struct DqCfg {
-    static constexpr bool PAD = DH == 128;
+    static constexpr bool DMA = sizeof(T) == 2, PAD = DH == 128 && !DMA;
     static constexpr int NTH = 64 * NW, BQ = 32 * NW, BK = 64;
     static constexpr int TILE = tile_elems<T, DH, PAD, BK>();
-    static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
+    static constexpr size_t PAIR = (DMA ? 2 : 1) * 4 * (size_t)TILE;   // bytes
     static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);
     static constexpr size_t LDS = PAIR > OUT ? PAIR : OUT;
 };
@@ -884,8 +916,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     typedef Lds<DH, C::PAD> L;
     constexpr int PS = Kv::St::PS, BK = C::BK, BQ = C::BQ;
     extern __shared__ __align__(256) char smem[];
-    __bf16* Ks = reinterpret_cast<__bf16*>(smem);
-    __bf16* Vs = Ks + C::TILE;
+    __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     const int l = xcd_block(blockIdx.x, gridDim.x);
     Work w;
@@ -936,40 +967,68 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     const float lr = rok && qr < s.ql ? g.lse[lrow] : -INFINITY;
     const bool none = lr == -INFINITY;
     const float l2 = none ? INFINITY : lr * LOG2E;
-    if (rok && h == 0) g.delta[lrow] = D;
+    if (rok && h == 0) g.stats[((long)w.i * a.KV + kvh) * a.lq * a.G + r] = make_float2(l2, D);
 
     floatx16 acc[DH / 32];
 #pragma unroll
     for (int dt = 0; dt < DH / 32; ++dt)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
-    Kv kv;
-    kv.init(a, s, g.k, g.v, kvh, tid);
-    auto fetch = [&](int t) { kv.fetch(a, s, g.k, g.v, kvh, rg.block(t), rg.kend, tid); };
-    if (rg.nt > 0) {
-        fetch(0);
-        kv.store(Ks, Vs, nullptr, nullptr, tid);
-        if (rg.nt > 1) fetch(1);
-        __syncthreads();
-    }
-    for (int t = 0; t < rg.nt; ++t) {
+    qf.settle();
+    df.settle();
+    auto tile = [&](int t, const __bf16* Ks) {
+        const __bf16* Vs = Ks + C::TILE;
 #pragma unroll 1
         for (int j = 0; j < BK / 32; ++j) {
             const int key0 = rg.block(t) * BK + 32 * j;
             if (!sees || key0 >= rg.kend || all_hidden(a, key0, 32, wlo, whi)) continue;
-            floatx16 sc = mma_rows<T, DH, C::PAD, PS>(Ks + 32 * j * L::ST, qf, lane);
-            const floatx16 dp = mma_rows<T, DH, C::PAD, PS>(Vs + 32 * j * L::ST, df, lane);
+            floatx16 sc, dp;
+            if constexpr (C::DMA) {
+                products<DH, false>(Ks + 32 * j * L::ST, Vs + 32 * j * L::ST, qf, df, nullptr, sc, dp, lane);
+            } else {
+                sc = mma_rows<T, DH, C::PAD, PS>(Ks + 32 * j * L::ST, qf, lane);
+                dp = mma_rows<T, DH, C::PAD, PS>(Vs + 32 * j * L::ST, df, lane);
+            }
             if (dead || key0 + 32 > rg.kend || some_hidden(a, key0, 32, wlo, whi)) hide(a, sc, key0 + 4 * h, qr, last);
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -l2)) * (dp[e] - D);
             mma_tr<T, DH, C::PAD, PS>(Ks + 32 * j * L::ST, sc, acc, lane);
         }
-        __syncthreads();
-        if (t + 1 < rg.nt) {
-            kv.store(Ks, Vs, nullptr, nullptr, tid);
-            if (t + 2 < rg.nt) fetch(t + 2);
+    };
+    if constexpr (C::DMA) {
+        KvDma<DH, BK, NW, false> kv;
+        kv.init(a, s, g.k, g.v, kvh, tid);
+        auto fetch = [&](int t) {
+            __bf16* to = tiles + (t & 1) * 2 * C::TILE;
+            kv.fetch(a, rg.block(t), rg.kend, to, to + C::TILE);
+        };
+        if (rg.nt > 0) fetch(0);
+        for (int t = 0; t < rg.nt; ++t) {
+            arrived();
+            __syncthreads();       // everyone's pieces of tile t are here, and tile t - 1 is done with
+            if (t + 1 < rg.nt) fetch(t + 1);
+            tile(t, tiles + (t & 1) * 2 * C::TILE);
+        }
+        __syncthreads();           // the buffers become the rows' way out
+    } else {
+        Kv kv;
+        kv.init(a, s, g.k, g.v, kvh, tid);
+        auto fetch = [&](int t) { kv.fetch(a, s, g.k, g.v, kvh, rg.block(t), rg.kend, tid); };
+        if (rg.nt > 0) {
+            fetch(0);
+            kv.store(tiles, tiles + C::TILE, nullptr, nullptr, tid);
+            if (rg.nt > 1) fetch(1);
             __syncthreads();
+        }
+        for (int t = 0; t < rg.nt; ++t) {
+            tile(t, tiles);
+            __syncthreads();
+            if (t + 1 < rg.nt) {
+                kv.store(tiles, tiles + C::TILE, nullptr, nullptr, tid);
+                if (t + 2 < rg.nt) fetch(t + 2);
+                __syncthreads();
+            }
         }
     }
     if (!live) return;
@@ -987,7 +1046,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
 // the tiles that hold these (`first` of them) are seen by every later row: the rows
 // past the window's reach (far rows) are cut into `chunks` of `chunk` flattened rows for
 // workgroups of their own, whose parts seq_first_kernel adds up.
-struct DkvPlan { int ktiles, first, chunks, chunk; bool even; };
+struct DkvPlan { int ktiles, first, chunks, chunk; };
 
 // rows that see the key tile from key0: near ones up to `far`, far ones from there on
 struct Rows { int lo, far, hi; };
@@ -1000,37 +1059,85 @@ __device__ __forceinline__ Rows rows_of(const SArgs& a, const Seq& s, int key0, 
     return r;
 }
 
-template <typename T, int DH, int NK> struct DkvCfg {
-    static constexpr bool PAD = DH == 128;
+// A tile of BQ query rows with their dO rows and statistics straight into LDS (bf16):
+// pieces of both operands are dealt out to the waves.  Past the last row the last one
+// stands in; its scores are masked.
+template <int DH, int BQ, int NW> struct QDma {
+    typedef Lds<DH, false> L;
+    static constexpr int CPR = DH / 8, RPI = 64 / CPR, PER = BQ / RPI, NI = 2 * PER / NW;   // pieces an operand, a wave
+    static_assert(2 * PER % NW == 0 && PER % NI == 0, "a wave's pieces are of one operand");
+    static constexpr int FULL = 0x7fffffe0;      // the host has seen that offsets stay below
+    intx4 rs, st;
+    int wave, sl, sh, rows, row[NI], col[NI];
+    bool isd;
+    __device__ __forceinline__ void init(const SArgs& a, const Seq& s, const __bf16* q, const __bf16* d,
+                                         const float2* stats, int kvh, int rows_, int tid) {
+        const int lane = tid & 63;
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        isd = wave * NI >= PER;
+        const PtcgHeadLayout& l = isd ? a.o : a.q;
+        sl = (int)l.sl * 2;
+        sh = (int)l.sh * 2;
+        rows = rows_;
+        const __bf16* p = isd ? d + s.o : q + s.q;
+        rs = KvDma<DH, 64, 4, false>::rsrc(reinterpret_cast<const char*>(p + (long)kvh * a.G * l.sh), FULL);
+        st = KvDma<DH, 64, 4, false>::rsrc(reinterpret_cast<const char*>(stats), rows * 8);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            row[i] = (wave * NI + i) % PER * RPI + lane / CPR;
+            const int c = (lane % CPR) ^ L::swz(row[i]);
+            col[i] = 8 * c < a.dh ? 16 * c : PT_NOWHERE;
+        }
+    }
+    __device__ __forceinline__ void fetch(const SArgs& a, int row0, __bf16* Qs, __bf16* Ds, float* ls, int lane) const {
+        __bf16* to = isd ? Ds : Qs;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int r = min(row0 + row[i], rows - 1), qi = head_div(a, r);
+            const int off = col[i] == PT_NOWHERE ? PT_NOWHERE : qi * sl + (r - qi * a.G) * sh + col[i];
+            to_lds(rs, to + (wave * NI + i) % PER * RPI * L::ST, off);
+        }
+        if (wave < BQ / 32) {     // 32 rows' two numbers
+            const unsigned at = (unsigned)(uintptr_t)(ls + wave * 64);
+            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                         :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"((row0 + wave * 32) * 8 + lane * 4), "s"(st)
+                         : "memory");
+        }
+    }
+};
+
+template <typename T, int DH, int NK, bool DMA> struct DkvCfg {
+    static constexpr bool PAD = DH == 128 && !DMA;
     static constexpr int NTH = 64 * NK, BKEY = 32 * NK;
     // the rows of a step: 32 where the registers hold no more on their way
     static constexpr int BQ = DH * planes<T>() >= 128 || NK < 4 ? 32 : 64;
     static constexpr int TILE = tile_elems<T, DH, PAD, BQ>();
-    static constexpr size_t PAIR = 4 * (size_t)TILE;   // bytes
+    static constexpr size_t PAIR = (DMA ? 2 : 1) * 4 * (size_t)TILE;   // bytes
     static constexpr size_t OUT = (size_t)NK * Out<T, DH>::WAVE * sizeof(T);
     static constexpr size_t BUFS = PAIR > OUT ? PAIR : OUT;
     // 128 wide in bf16, the values' rows stay in LDS: with them, dK and dV in
     // registers two waves a SIMD would spill
     static constexpr bool VLDS = sizeof(T) == 2 && DH == 128;
     static constexpr size_t VROWS = VLDS ? (size_t)BKEY * Lds<DH, PAD>::ST * 2 : 0;
-    static constexpr size_t LDS = BUFS + VROWS + 3 * BQ * sizeof(float) + 16;
+    static constexpr size_t LDS = BUFS + VROWS + 2 * 2 * BQ * sizeof(float);
 };
 template <typename T, int DH> constexpr int dkv_waves() {
     return DH * planes<T>() <= 64 || waves_simd<T, DH>() == 2 ? 2 : 1;
 }
 
-template <typename T, int DH, int NK>
+// dK and dV: a workgroup owns 32 NK keys of one kv head, a wave 32 of them, and
+// walks the flattened query rows that see them.  S = Q K^T and dP = dO V^T with
+// keys on lanes; dV^T += dO^T P and dK^T += Q^T dS read dO and Q transposed from LDS.
+template <typename T, int DH, int NK, bool DMA>
 __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(const SArgs a, const Grads<T> g,
                                                                                const DkvPlan pl) {
-    typedef DkvCfg<T, DH, NK> C;
+    typedef DkvCfg<T, DH, NK, DMA> C;
     typedef Stage<T, DH, C::PAD, C::BQ, C::NTH> St;
     typedef Lds<DH, C::PAD> L;
+    constexpr int BQ = C::BQ;
     extern __shared__ __align__(256) char smem[];
-    __bf16* Qs = reinterpret_cast<__bf16*>(smem);
-    __bf16* Ds = Qs + C::TILE;
-    float* ls = reinterpret_cast<float*>(smem + C::BUFS + C::VROWS);   // log-sum-exp, D and place of the rows
-    float* dl = ls + C::BQ;
-    int* ps = reinterpret_cast<int*>(dl + C::BQ);
+    __bf16* tiles = reinterpret_cast<__bf16*>(smem);
+    float* stats = reinterpret_cast<float*>(smem + C::BUFS + C::VROWS);   // log-sum-exp and D of the rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     // a (sequence, kv head)'s pieces: near rows of its key tiles, then far chunks of the first ones
     const int per = pl.ktiles + pl.first * pl.chunks, b = xcd_block(blockIdx.x, gridDim.x);
@@ -1040,7 +1147,7 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
     const Seq s = seq_of<false>(a, i);
     const int kall = s.rows;          // a padded sequence's dead rows get zeros
     if (kt * C::BKEY >= kall) return;
-    const int key0 = kt * C::BKEY, kw = key0 + 32 * wave, key = kw + (lane & 31);
+    const int key0 = kt * C::BKEY, kw = key0 + 32 * __builtin_amdgcn_readfirstlane(wave), key = kw + (lane & 31);
     const bool kin = key < kall, kok = key < s.kl;
     const Rows rr = rows_of(a, s, key0, C::BKEY);
     const bool cut = kt < pl.first && pl.chunks > 0;
@@ -1070,64 +1177,38 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
 #pragma unroll
         for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
 
-    const int nt = rows > r0 ? (rows - r0 + C::BQ - 1) / C::BQ : 0;
-    St qs_, ds_;
-    float lr = 0.f, dr = 0.f;
-    int rown = 0, pr = 0;     // rows of the fetched tile; a row's place
-    auto fetch = [&](int t) {
-        const int row0 = r0 + t * C::BQ;
-        rown = rows - row0;
-        qs_.load_q(a, a.q, g.q + s.q, kvh, row0, rows, tid);
-        ds_.load_q(a, a.o, g.dout + s.o, kvh, row0, rows, tid);
-        if (tid < C::BQ) {
-            const int r = min(row0 + tid, rows - 1);
-            const int qi = head_div(a, r), head = kvh * a.G + r - qi * a.G;
-            const long lrow = ((long)i * a.H + head) * a.lq + qi;
-            lr = g.lse[lrow];
-            dr = g.delta[lrow];
-            pr = qi;
-        }
-    };
-    auto store = [&]() {
-        // past the end q's last row stays: its log-sum-exp of +inf takes it out
-        qs_.store_q(Qs, tid, C::BQ, a.dh);
-        ds_.store_q(Ds, tid, rown, a.dh);
-        if (tid < C::BQ) {
-            const bool live = tid < rown;
-            ls[tid] = live && lr != -INFINITY ? lr * LOG2E : INFINITY;
-            dl[tid] = live ? dr : 0.f;
-            ps[tid] = pr;
-        }
-    };
-    if (nt > 0) {
-        fetch(0);
-        store();
-        if (nt > 1) fetch(1);
-        __syncthreads();
-    }
-    for (int t = 0; t < nt; ++t) {
+    const int nt = rows > r0 ? (rows - r0 + BQ - 1) / BQ : 0;
+    const float2* sg = g.stats + (long)u * a.lq * a.G;
+    kfr.settle();
+    if constexpr (!C::VLDS) vfr.settle();
+    auto tile = [&](int t, const __bf16* Qs, const __bf16* Ds, const float* ls) {
 #pragma unroll 1
-        for (int j = 0; j < C::BQ / 32; ++j) {
-            const int qr = 32 * j, row0 = r0 + t * C::BQ + qr;
+        for (int j = 0; j < BQ / 32; ++j) {
+            const int qr = 32 * j, row0 = r0 + t * BQ + qr;
             if (row0 >= rows) break;
-            const int plo = __builtin_amdgcn_readfirstlane(ps[qr]), phi = __builtin_amdgcn_readfirstlane(ps[qr + 31]);
+            const int plo = head_div(a, row0), phi = head_div(a, min(row0 + 31, rows - 1));
             if (kw >= s.kl || all_hidden(a, kw, 32, plo, phi)) continue;
-            floatx16 p = mma_rows<T, DH, C::PAD, St::PS>(Qs + qr * L::ST, kfr, lane);
-            floatx16 d;
-            if constexpr (C::VLDS) d = mma_rows_lds<DH, C::PAD>(Ds + qr * L::ST, Vl, lane);
-            else d = mma_rows<T, DH, C::PAD, St::PS>(Ds + qr * L::ST, vfr, lane);
-            if (some_hidden(a, kw, 32, plo, phi)) {
+            floatx16 p, d;
+            if constexpr (DMA) {
+                products<DH, C::VLDS>(Qs + qr * L::ST, Ds + qr * L::ST, kfr, vfr, Vl, p, d, lane);
+            } else {
+                p = mma_rows<T, DH, C::PAD, St::PS>(Qs + qr * L::ST, kfr, lane);
+                if constexpr (C::VLDS) d = mma_rows_lds<DH, C::PAD>(Ds + qr * L::ST, Vl, lane);
+                else d = mma_rows<T, DH, C::PAD, St::PS>(Ds + qr * L::ST, vfr, lane);
+            }
+            if (row0 + 32 > rows || some_hidden(a, kw, 32, plo, phi)) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int at = ps[qr + 8 * (e / 4) + 4 * h + e % 4];
-                    p[e] = key <= at && (at - key < a.window || key < a.sinks) ? p[e] : -INFINITY;
+                    const int r = row0 + 8 * (e / 4) + 4 * h + e % 4, at = head_div(a, r);
+                    const bool see = r < rows && key <= at && (at - key < a.window || key < a.sinks);
+                    p[e] = see ? p[e] : -INFINITY;
                 }
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float4 lf = *reinterpret_cast<const float4*>(ls + qr + 8 * e + 4 * h);
-                const float4 df = *reinterpret_cast<const float4*>(dl + qr + 8 * e + 4 * h);
-                const float lv[4] = {lf.x, lf.y, lf.z, lf.w}, dv4[4] = {df.x, df.y, df.z, df.w};
+                const float* x4 = ls + 2 * (qr + 8 * e + 4 * h);
+                const float4 x0 = *reinterpret_cast<const float4*>(x4), x1 = *reinterpret_cast<const float4*>(x4 + 4);
+                const float lv[4] = {x0.x, x0.z, x1.x, x1.z}, dv4[4] = {x0.y, x0.w, x1.y, x1.w};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     // a key that is not there goes along: its columns are cleared at the end
@@ -1139,11 +1220,51 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
             mma_tr<T, DH, C::PAD, St::PS>(Ds + qr * L::ST, p, gv, lane);
             mma_tr<T, DH, C::PAD, St::PS>(Qs + qr * L::ST, d, gk, lane);
         }
-        __syncthreads();
-        if (t + 1 < nt) {
+    };
+    if constexpr (DMA) {
+        QDma<DH, BQ, NK> qd;
+        if (nt > 0) qd.init(a, s, g.q, g.dout, sg, kvh, rows, tid);
+        auto fetch = [&](int t) {
+            __bf16* to = tiles + (t & 1) * 2 * C::TILE;
+            qd.fetch(a, r0 + t * BQ, to, to + C::TILE, stats + (t & 1) * 2 * BQ, lane);
+        };
+        if (nt > 0) fetch(0);
+        for (int t = 0; t < nt; ++t) {
+            arrived();
+            __syncthreads();       // everyone's pieces of tile t are here, and tile t - 1 is done with
+            if (t + 1 < nt) fetch(t + 1);
+            const __bf16* from = tiles + (t & 1) * 2 * C::TILE;
+            tile(t, from, from + C::TILE, stats + (t & 1) * 2 * BQ);
+        }
+        __syncthreads();           // the buffers become the rows' way out
+    } else {
+        St qs_, ds_;
+        float2 lr = make_float2(0.f, 0.f);
+        auto fetch = [&](int t) {
+            const int row0 = r0 + t * BQ;
+            qs_.load_q(a, a.q, g.q + s.q, kvh, row0, rows, tid);
+            ds_.load_q(a, a.o, g.dout + s.o, kvh, row0, rows, tid);
+            if (tid < BQ) lr = sg[min(row0 + tid, rows - 1)];
+        };
+        auto store = [&]() {
+            qs_.store_q(tiles, tid, BQ, a.dh);
+            ds_.store_q(tiles + C::TILE, tid, BQ, a.dh);
+            if (tid < BQ) reinterpret_cast<float2*>(stats)[tid] = lr;
+        };
+        if (nt > 0) {
+            fetch(0);
             store();
-            if (t + 2 < nt) fetch(t + 2);
+            if (nt > 1) fetch(1);
             __syncthreads();
+        }
+        for (int t = 0; t < nt; ++t) {
+            tile(t, tiles, tiles + C::TILE, stats);
+            __syncthreads();
+            if (t + 1 < nt) {
+                store();
+                if (t + 2 < nt) fetch(t + 2);
+                __syncthreads();
+            }
         }
     }
     if (!kok) {   // a dead key's gradient is zero, whatever the rows hold
@@ -1395,7 +1516,8 @@ struct BwdPlan {
     int nw, nk;
     Plan q;
     DkvPlan k;
-    int64_t delta, part;     // workspace floats
+    bool dma;                // dk / dv's tiles straight into LDS
+    int64_t stats, part;     // workspace floats
 };
 BwdPlan bwd_plan(const PtcgWindowAttn* d, const SArgs& a) {
     BwdPlan p = {};
@@ -1419,7 +1541,11 @@ BwdPlan bwd_plan(const PtcgWindowAttn* d, const SArgs& a) {
             p.k.chunks = pt_cdiv(far, chunk);
         }
     }
-    p.delta = ((int64_t)a.n * a.H * a.lq + 3) / 4 * 4;
+    p.stats = ((int64_t)a.n * a.H * a.lq * 2 + 3) / 4 * 4;
+    auto near31 = [&](const PtcgHeadLayout& l) {     // a kv head's rows of a sequence within 2^31 bytes
+        return l.sl < (1LL << 30) && l.sh < (1LL << 30) && ((int64_t)a.lq * l.sl + (int64_t)a.G * l.sh) * 2 < 0x7fffff00LL;
+    };
+    p.dma = d->bf16 && near31(a.q) && near31(a.o);
     p.part = (int64_t)a.n * a.KV * p.k.first * (p.k.chunks + 1) * bkey * 2 * a.dh;
     if (p.k.first == 0) p.part = 0;
     return p;
@@ -1433,9 +1559,10 @@ template <typename T, int DH, int NW> int launch_dq(const SArgs& a, const BwdPla
     PT_LAUNCH_CHECK();
     return PTCG_OK;
 }
-template <typename T, int DH, int NK> int launch_dkv(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
-    typedef DkvCfg<T, DH, NK> C;
-    auto kern = seq_dkv_kernel<T, DH, NK>;
+template <typename T, int DH, int NK, bool DMA>
+int launch_dkv(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
+    typedef DkvCfg<T, DH, NK, DMA> C;
+    auto kern = seq_dkv_kernel<T, DH, NK, DMA>;
     PT_TRY(lds_attr(kern, C::LDS));
     const int64_t pairs = (int64_t)a.n * a.KV;
     hipLaunchKernelGGL(kern, dim3((unsigned)(pairs * (p.k.ktiles + p.k.first * p.k.chunks))), dim3(C::NTH), C::LDS, s, a,
@@ -1450,16 +1577,19 @@ template <typename T, int DH, int NK> int launch_dkv(const SArgs& a, const BwdPl
 }
 template <typename T, int DH> int run_bwd(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
     PT_TRY(p.nw == 2 ? (launch_dq<T, DH, 2>(a, p, g, s)) : (launch_dq<T, DH, 4>(a, p, g, s)));
+    if constexpr (sizeof(T) == 2)
+        if (p.dma)
+            return p.nk == 2 ? launch_dkv<T, DH, 2, true>(a, p, g, s) : launch_dkv<T, DH, 4, true>(a, p, g, s);
     if constexpr (sizeof(T) == 2 || DH <= 64)
-        if (p.nk == 2) return launch_dkv<T, DH, 2>(a, p, g, s);
-    return launch_dkv<T, DH, 4>(a, p, g, s);
+        if (p.nk == 2) return launch_dkv<T, DH, 2, false>(a, p, g, s);
+    return launch_dkv<T, DH, 4, false>(a, p, g, s);
 }
 template <typename T>
 int bwd_dh(const SArgs& a, const BwdPlan& p, const void* q, const void* k, const void* v, const void* out,
            const float* lse, const void* dout, void* dq, void* dk, void* dv, float* ws, hipStream_t s) {
     const Grads<T> g = {static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v),
                         static_cast<const T*>(out), static_cast<const T*>(dout), lse, static_cast<T*>(dq),
-                        static_cast<T*>(dk), static_cast<T*>(dv), ws, ws + p.delta};
+                        static_cast<T*>(dk), static_cast<T*>(dv), reinterpret_cast<float2*>(ws), ws + p.stats};
     return a.dh <= 32 ? run_bwd<T, 32>(a, p, g, s) : a.dh <= 64 ? run_bwd<T, 64>(a, p, g, s) : run_bwd<T, 128>(a, p, g, s);
 }
 
@@ -1496,7 +1626,7 @@ extern "C" int64_t ptcg_kernel_window_attention_ws_bytes(const PtcgWindowAttn* d
     const SArgs a = window_args(d);
     if (backward) {
         const BwdPlan p = bwd_plan(d, a);
-        return (p.delta + p.part) * 4;
+        return (p.stats + p.part) * 4;
     }
     return part_bytes(window_form(d, a), a);
 }
@@ -1535,7 +1665,7 @@ extern "C" int ptcg_kernel_window_attention_bwd(const PtcgWindowAttn* d, const v
                "%s: rows of dk or dv overlap (broadcast keys have no gradient layout)", who);
     const SArgs a = window_args(d);
     const BwdPlan p = bwd_plan(d, a);
-    const int64_t need = (p.delta + p.part) * 4;
+    const int64_t need = (p.stats + p.part) * 4;
     PT_REQUIRE(workspace && workspace_bytes >= need && al16(workspace),
                "%s: workspace of %lld bytes, need %lld (16 B aligned)", who, (long long)workspace_bytes,
                (long long)need);

@@ -17,6 +17,8 @@
 
 #include <limits.h>
 
+#include <type_traits>
+
 namespace {
 
 // the descriptors as the kernels take them
@@ -200,6 +202,12 @@ __device__ __forceinline__ void hide(const SArgs& a, floatx16& s, int k0, int p,
         s[e] = see ? s[e] : -INFINITY;
     }
 }
+// the same of keys of no page: 32 keys' bits
+__device__ __forceinline__ void hide_bits(floatx16& s, unsigned none, int h) {
+    const unsigned mine = none >> 4 * h;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = mine & 1u << (8 * (e / 4) + e % 4) ? -INFINITY : s[e];
+}
 // whether some row of places lo .. hi does not see all of keys k0 .. k0 + nk - 1, or none
 // of them does
 __device__ __forceinline__ bool some_hidden(const SArgs& a, int k0, int nk, int lo, int hi) {
@@ -216,6 +224,12 @@ __device__ __forceinline__ int page_of(const SArgs& a, int key) {
 }
 __device__ __forceinline__ int entry_of(const SArgs& a, const Seq& s, int key, int kend) {
     return key < kend ? s.table[page_of(a, key)] : -1;
+}
+
+// the larger of both halves' values
+__device__ __forceinline__ float half_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // A running softmax of the rows on lanes: m2, a bound of the scores (s scale2) so far
@@ -235,14 +249,18 @@ template <int DH> struct Soft {
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[dt][e] = 0.f;
     }
-    // new scores in: exponentials out, what is summed rescaled to a larger maximum
-    template <int N> __device__ __forceinline__ void step(floatx16 (&sc)[N], float scale2) {
+    // a lane's largest score
+    template <int N> static __device__ __forceinline__ float top(const floatx16 (&sc)[N]) {
         float mt = -INFINITY;
 #pragma unroll
         for (int j = 0; j < N; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) mt = fmaxf(mt, sc[j][e]);
-        mt = fmaxf(mt, half_swap(mt));
+        return mt;
+    }
+    // what is summed is rescaled where new scores, at most mt on this lane, pass the bound
+    __device__ __forceinline__ void raise(float mt, float scale2) {
+        mt = half_max(mt);
         const float mn = fmaxf(m2, mt * scale2);
         if (__any(mn > m2 + SLACK)) {
             const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m2 - mn);
@@ -253,41 +271,89 @@ template <int DH> struct Soft {
                 for (int e = 0; e < 16; ++e) o[dt][e] *= al;
             m2 = mn;
         }
+    }
+    // scores to exponentials
+    __device__ __forceinline__ void exps(floatx16& sc, float scale2) {
         const float ms = m2 == -INFINITY ? 0.f : m2;
 #pragma unroll
-        for (int j = 0; j < N; ++j)
+        for (int e = 0; e < 16; ++e) {
+            sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], scale2, -ms));
+            l += sc[e];
+        }
+    }
+    template <int N> __device__ __forceinline__ void step(floatx16 (&sc)[N], float scale2) {
+        raise(top(sc), scale2);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                sc[j][e] = __builtin_amdgcn_exp2f(fmaf(sc[j][e], scale2, -ms));
-                l += sc[j][e];
-            }
+        for (int j = 0; j < N; ++j) exps(sc[j], scale2);
+    }
+    // elements e0 .. e0 + n - 1 of 32 keys' scores to exponentials, and those to the values'
+    // operand
+    __device__ __forceinline__ void exps_of(floatx16& sc, bf16x8 (&p)[2], float scale2, float ms, int e0, int n) {
+#pragma unroll
+        for (int e = e0; e < e0 + n; ++e) {
+            sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], scale2, -ms));
+            l += sc[e];
+            p[e / 8][e % 8] = (__bf16)sc[e];
+        }
     }
 };
 
-// S^T of 64 keys in LDS (bf16).  Operands are asked for four products ahead: left to
-// itself the compiler reads each one just before its product and waits.
-template <int DH>
-__device__ __forceinline__ void scores(const __bf16* ks, const Row<__bf16, DH>& q, floatx16 (&sc)[2], int lane) {
+// The order of instructions is the source's from here to the next such line: left to
+// itself the compiler reads an operand just before its product and waits, or keeps so
+// many on their way that registers spill.
+__device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
+
+// S^T of 64 keys in LDS (bf16), a product at a time; side(i) goes into product i's shadow.
+template <int DH, class Side>
+__device__ __forceinline__ void scores(const __bf16* ks, const Row<__bf16, DH>& q, floatx16 (&sc)[2], int lane,
+                                       Side side) {
     typedef Lds<DH, false> L;
-    constexpr int N = DH / 8, AHEAD = N < 4 ? N : 4;
+    constexpr int N = DH / 8, AHEAD = 4;       // operands on their way
+    bf16x8 x[N];
+    auto read = [&](int i) {
+        x[i] = *reinterpret_cast<const bf16x8*>(ks + 32 * (i & 1) * L::ST + L::chunk_at(lane & 31, lane >> 5, i >> 1));
+    };
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int e = 0; e < 16; ++e) sc[j][e] = 0.f;
 #pragma unroll
-    for (int c = 0; c < DH / 16; ++c)
+    for (int i = 0; i < AHEAD; ++i) read(i);
+    pin();
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const bf16x8 x = *reinterpret_cast<const bf16x8*>(ks + 32 * j * L::ST + L::chunk_at(lane & 31, lane >> 5, c));
-            sc[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, q.f[c][0], sc[j], 0, 0, 0);
-        }
-    __builtin_amdgcn_sched_group_barrier(0x100, AHEAD, 0);
-#pragma unroll
-    for (int i = 0; i < N - AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    for (int i = 0; i < N; ++i) {
+        sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[i], q.f[i >> 1][0], sc[i & 1], 0, 0, 0);
+        if (i + AHEAD < N) read(i + AHEAD);
+        side(i);
+        pin();
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, AHEAD, 0);
+}
+
+// o^T += V^T P of 32 keys in LDS (bf16) and their exponentials p, in the same way
+template <int DH, class Side>
+__device__ __forceinline__ void values(const __bf16* vs, const bf16x8 (&p)[2], floatx16 (&o)[DH / 32], int lane,
+                                       Side side) {
+    typedef __attribute__((address_space(3))) bf16x4* lds4;
+    typedef Lds<DH, false> L;
+    constexpr int N = DH / 16, DT = DH / 32, AHEAD = 2;
+    const int i15 = lane & 15, r0 = 4 * (lane >> 5) + (i15 >> 2), ch = 2 * (lane >> 4 & 1) + (i15 >> 1 & 1);
+    bf16x4 u[N], w[N];
+    auto read = [&](int i) {
+        const __bf16* q = vs + 16 * (i / DT) * L::ST + 4 * (i15 & 1);
+        u[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + L::group_at(r0, ch, i % DT)));
+        w[i] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds4)(q + L::group_at(r0 + 8, ch, i % DT)));
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) read(i);
+    pin();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const bf16x8 x = bf16x8{u[i][0], u[i][1], u[i][2], u[i][3], w[i][0], w[i][1], w[i][2], w[i][3]};
+        o[i % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, p[i / DT], o[i % DT], 0, 0, 0);
+        if (i + AHEAD < N) read(i + AHEAD);
+        side(i);
+        pin();
+    }
 }
 
 // What a tile's rows come to: their output, or their split's part for the joining
@@ -401,7 +467,7 @@ __device__ __forceinline__ void to_lds(intx4 rs, const __bf16* base, int off) {
 }
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// A tile of BK keys and values by 16-byte pieces straight into LDS (bf16): every wave
+// A tile of BK key or value rows by 16-byte pieces straight into LDS (bf16): every wave
 // brings BK / NW rows that lie in one matrix, or in one page (whose size is a multiple
 // of them).  A piece's place in LDS is its lane's, so the lane chooses the chunk that
 // belongs there.
@@ -409,25 +475,21 @@ template <int DH, int BK, int NW, bool PAGED> struct KvDma {
     typedef Lds<DH, false> L;
     static constexpr int CPR = DH / 8, WR = BK / NW, RPI = 64 / CPR, NI = WR / RPI;   // rows a wave, an instruction
     static_assert(WR % RPI == 0, "whole instructions");
-    int ko[NI], vo[NI], kld, vld, kw, vw, row;
-    const char *kb, *vb;
-    int ent;
-    __device__ __forceinline__ void init(const SArgs& a, const Seq& s, const __bf16* k, const __bf16* v, int kvh,
-                                         int tid) {
+    int off[NI], ld, width, row, ent;
+    const char* base;
+    // rows of layout l; row0: the sequence's first (one matrix)
+    __device__ __forceinline__ void init(const SArgs& a, const Seq& s, const __bf16* x, int kvh, const PtcgHeadLayout& l,
+                                         long row0, int tid) {
         const int lane = tid & 63;
         row = __builtin_amdgcn_readfirstlane(tid >> 6) * WR;
-        kld = (int)a.k.sl * 2;
-        vld = (int)a.v.sl * 2;
-        kb = reinterpret_cast<const char*>(k + (PAGED ? 0 : s.k) + (long)kvh * a.k.sh);
-        vb = reinterpret_cast<const char*>(v + (PAGED ? 0 : s.v) + (long)kvh * a.v.sh);
+        ld = (int)l.sl * 2;
+        width = 2 * a.dh;
+        base = reinterpret_cast<const char*>(x + (PAGED ? 0 : row0) + (long)kvh * l.sh);
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
             const int r = i * RPI + lane / CPR, c = (lane % CPR) ^ L::swz(row + r);
-            const bool in = 8 * c < a.dh;
-            ko[i] = in ? r * kld + 16 * c : PT_NOWHERE;
-            vo[i] = in ? r * vld + 16 * c : PT_NOWHERE;
+            off[i] = 8 * c < a.dh ? r * ld + 16 * c : PT_NOWHERE;
         }
-        kw = vw = 2 * a.dh;
     }
     // the page-table entry that fetch(block) will need
     __device__ __forceinline__ void look(const SArgs& a, const Seq& s, int block, int kend) {
@@ -439,25 +501,22 @@ template <int DH, int BK, int NW, bool PAGED> struct KvDma {
                      __builtin_amdgcn_readfirstlane((int)(unsigned)(x >> 32)), __builtin_amdgcn_readfirstlane(bytes),
                      0x00020000};
     }
-    __device__ __forceinline__ void fetch(const SArgs& a, int block, int kend, __bf16* Ks, __bf16* Vs) const {
+    __device__ __forceinline__ void fetch(const SArgs& a, const PtcgHeadLayout& l, int block, int kend,
+                                          __bf16* to) const {
         const int key = block * BK + row;
         int n = max(0, min(kend - key, WR));
-        const char *kp = kb, *vp = vb;
+        const char* p = base;
         if constexpr (PAGED) {
             const bool is = (unsigned)ent < (unsigned)a.pages;
             if (!is) n = 0;
-            const long e = is ? ent : 0, off = is ? key - page_of(a, key) * a.page : 0;
-            kp += (e * a.k.sn + off * a.k.sl) * 2;
-            vp += (e * a.v.sn + off * a.v.sl) * 2;
+            const long e = is ? ent : 0, at = is ? key - page_of(a, key) * a.page : 0;
+            p += (e * l.sn + at * l.sl) * 2;
         } else {
-            kp += (long)key * kld;
-            vp += (long)key * vld;
+            p += (long)key * ld;
         }
-        const intx4 rk = rsrc(kp, n ? (n - 1) * kld + kw : 0), rv = rsrc(vp, n ? (n - 1) * vld + vw : 0);
+        const intx4 rs = rsrc(p, n ? (n - 1) * ld + width : 0);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) to_lds(rk, Ks + (row + i * RPI) * L::ST, ko[i]);
-#pragma unroll
-        for (int i = 0; i < NI; ++i) to_lds(rv, Vs + (row + i * RPI) * L::ST, vo[i]);
+        for (int i = 0; i < NI; ++i) to_lds(rs, to + (row + i * RPI) * L::ST, off[i]);
     }
 };
 
@@ -470,6 +529,22 @@ template <typename T, int DH, int NW, bool DMA> struct TileCfg {
     static constexpr size_t LDS = BUFS + BK * sizeof(float) + 64;
 };
 template <typename T, int DH> constexpr int waves_simd() { return sizeof(T) == 2 || DH <= 64 ? 2 : 1; }
+
+// Workgroup b of `pairs` (sequence, kv head) pairs with `per` pieces each, the longest
+// first.  Workgroups go to the 8 XCDs in turn: a pair's pieces stay on one XCD, whose L2
+// then holds their keys, pairs are dealt out to the XCDs one by one (sequences
+// differ in length: with neighbours on one XCD a third of the CUs' time was idle), and an XCD
+// takes so many pairs at once that their long pieces come before their short ones.
+struct Share { int pair, piece; };
+__device__ __forceinline__ Share share_of(int b, int pairs, int per) {
+    const int full = pairs >> 3, x = b & 7, idx = b >> 3;
+    if (idx < full * per) {
+        const int most = (127 + per) / per, g = idx / (most * per), n = min(most, full - g * most), r = idx - g * most * per;
+        return {(g * most + r % n) * 8 + x, r / n};
+    }
+    const int rest = pairs - 8 * full, r = b - 8 * full * per;     // the last few: over all XCDs
+    return {8 * full + r % rest, r / rest};
+}
 
 // How slots become work, as the host decided: even: every sequence has qtiles row
 // tiles and nothing is split.
@@ -490,16 +565,15 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     float* kf = reinterpret_cast<float*>(smem + C::BUFS);
     int* bad = reinterpret_cast<int*>(smem + C::LDS - 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const int l = xcd_block(blockIdx.x, gridDim.x);
     Work w;
     int kvh;
     if (pl.even) {
-        const int u = l / pl.qtiles;
-        kvh = u % a.KV;
-        w = {u / a.KV, pl.qtiles - 1 - l % pl.qtiles, 0, INT_MAX, 1, 0, 0, 0};
+        const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.qtiles);
+        kvh = sh.pair % a.KV;
+        w = {sh.pair / a.KV, pl.qtiles - 1 - sh.piece, 0, INT_MAX, 1, 0, 0, 0};
     } else {
-        kvh = l / pl.slots;
-        w = work_of<PAGED, BQ, BK>(a, l % pl.slots, pl.slots, pl.least, pl.split);
+        kvh = blockIdx.x % a.KV;
+        w = work_of<PAGED, BQ, BK>(a, blockIdx.x / a.KV, pl.slots, pl.least, pl.split);
     }
     w = uniform(w);
     Joint* const js = reinterpret_cast<Joint*>(part);      // then the parts
@@ -536,23 +610,16 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         const int key0 = rg.block(t) * BK;
         if (!sees || all_hidden(a, key0, BK, wlo, whi)) return;
         floatx16 sc[BK / 32];
-        if constexpr (sizeof(T) == 2) {
-            scores<DH>(Ks, qf, sc, lane);
-        } else {
 #pragma unroll
-            for (int j = 0; j < BK / 32; ++j)
-                sc[j] = mma_rows<T, DH, false, PS>(Ks + 32 * j * Lds<DH, false>::ST, qf, lane);
-        }
+        for (int j = 0; j < BK / 32; ++j)
+            sc[j] = mma_rows<T, DH, false, PS>(Ks + 32 * j * Lds<DH, false>::ST, qf, lane);
         if (dead || key0 + BK > rg.kend || some_hidden(a, key0, BK, wlo, whi)) {
 #pragma unroll
             for (int j = 0; j < BK / 32; ++j) hide(a, sc[j], key0 + 32 * j + 4 * h, p, last);
         }
         if (PAGED && nopage) {
 #pragma unroll
-            for (int j = 0; j < BK / 32; ++j)
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (nopage >> (32 * j + 8 * (e / 4) + 4 * h + e % 4) & 1) sc[j][e] = -INFINITY;
+            for (int j = 0; j < BK / 32; ++j) hide_bits(sc[j], (unsigned)(nopage >> 32 * j), h);
         }
         f.step(sc, a.scale2);
 #pragma unroll
@@ -561,33 +628,92 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     };
     if constexpr (DMA) {
         static_assert(sizeof(T) == 2 && BK == 64, "");
-        KvDma<DH, BK, NW, PAGED> kv;
-        kv.init(a, s, k, v, kvh, tid);
-        auto fetch = [&](int t) {
-            __bf16* to = tiles + (t - t0 & 1) * 2 * C::TILE;
-            kv.fetch(a, rg.block(t), rg.kend, to, to + C::TILE);
+        // A tile's scores are made while the last one's exponentials are taken and its
+        // values summed, so that matrix and vector instructions run side by side within a
+        // wave: keys come a tile before values.
+        KvDma<DH, BK, NW, PAGED> kk, kv;
+        kk.init(a, s, k, kvh, a.k, s.k, tid);
+        kv.init(a, s, v, kvh, a.v, s.v, tid);
+        __bf16 *kbuf = tiles, *vbuf = tiles + 2 * C::TILE;
+        auto fetch_k = [&](int t) {
+            kk.fetch(a, a.k, rg.block(t), rg.kend, kbuf + (t - t0 & 1) * C::TILE);
+            if (t + 1 < t1) kk.look(a, s, rg.block(t + 1), rg.kend);
+        };
+        auto fetch_v = [&](int t) {
+            kv.fetch(a, a.v, rg.block(t), rg.kend, vbuf + (t - t0 & 1) * C::TILE);
             if (t + 1 < t1) kv.look(a, s, rg.block(t + 1), rg.kend);
         };
         auto lacks = [&](int t) {       // a lane per key
             const int key = rg.block(t) * BK + lane;
             return key < rg.kend && (unsigned)s.table[page_of(a, key)] >= (unsigned)a.pages;
         };
-        if (t0 < t1) {
-            kv.look(a, s, rg.block(t0), rg.kend);
-            fetch(t0);
-        }
         bool some = false;         // any key of no page: only then tiles look for them
-        if constexpr (PAGED) {
-            for (int t = t0 + wave; t < t1; t += NW) some |= lacks(t);
-            some = __syncthreads_or(some);
-        }
-        for (int t = t0; t < t1; ++t) {
+        auto cover = [&](int t, floatx16 (&sc)[2]) {
+            const int key0 = rg.block(t) * BK;
+            if (!sees || dead || key0 + BK > rg.kend || some_hidden(a, key0, BK, wlo, whi)) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) hide(a, sc[j], key0 + 32 * j + 4 * h, p, last);
+            }
+            if (PAGED && some) {
+                const unsigned long long nopage = __ballot(lacks(t));
+                if (nopage) {
+                    hide_bits(sc[0], (unsigned)nopage, h);
+                    hide_bits(sc[1], (unsigned)(nopage >> 32), h);
+                }
+            }
+        };
+        constexpr int ES = 16 / (DH / 8) , EV = 16 / (DH / 16);     // elements in a product's shadow
+        if (t0 < t1) {
+            kk.look(a, s, rg.block(t0), rg.kend);
+            kv.look(a, s, rg.block(t0), rg.kend);
+            fetch_k(t0);
+            if (t0 + 1 < t1) fetch_k(t0 + 1);
+            fetch_v(t0);
+            if constexpr (PAGED) {
+                for (int t = t0 + wave; t < t1; t += NW) some |= lacks(t);
+                some = __syncthreads_or(some);
+            }
+            floatx16 sa[2], sb[2];
             arrived();
-            __syncthreads();       // everyone's pieces of tile t are here, and tile t - 1 is done with
-            if (t + 1 < t1) fetch(t + 1);
-            unsigned long long nopage = 0;
-            if (PAGED && some) nopage = __ballot(lacks(t));
-            tile(t, tiles + (t - t0 & 1) * 2 * C::TILE, nopage);
+            __syncthreads();
+            scores<DH>(kbuf, qf, sa, lane, [](int) {});
+            cover(t0, sa);
+            f.raise(f.top(sa), a.scale2);
+            if (t0 + 2 < t1) __syncthreads();     // keys of the first tile are done with
+            // scores of tile t + 1 from its keys (of the last tile's successor from what lies
+            // there, for nothing), exponentials and values of tile t, whose place in the
+            // buffers is `at`
+            auto turn = [&](int t, auto at, floatx16 (&now)[2], floatx16 (&next)[2]) {
+                if (t > t0) {
+                    arrived();
+                    __syncthreads();   // everyone's pieces are here; keys of tile t and values of t - 1 are done with
+                }
+                if (t + 1 < t1) fetch_v(t + 1);
+                if (t + 2 < t1) fetch_k(t + 2);
+                const __bf16* Vs = vbuf + at * C::TILE;
+                const float ms = f.m2 == -INFINITY ? 0.f : f.m2;
+                bf16x8 pa[2], pb[2];
+                pin();
+                scores<DH>(kbuf + (1 - at) * C::TILE, qf, next, lane,
+                           [&](int i) { f.exps_of(now[0], pa, a.scale2, ms, i * ES, ES); });
+                asm volatile("" : "+v"(pa[0]), "+v"(pa[1]), "+v"(f.l));     // made here, not past the branch
+                if (t + 1 < t1) cover(t + 1, next);
+                pin();
+                values<DH>(Vs, pa, f.o, lane, [&](int i) { f.exps_of(now[1], pb, a.scale2, ms, i * EV, EV); });
+                float mt = -INFINITY;
+                values<DH>(Vs + 32 * Lds<DH, false>::ST, pb, f.o, lane, [&](int i) {
+#pragma unroll
+                    for (int e = i * EV; e < (i + 1) * EV; ++e) {
+                        mt = fmaxf(mt, next[0][e]);
+                        mt = fmaxf(mt, next[1][e]);
+                    }
+                });
+                if (t + 1 < t1) f.raise(mt, a.scale2);
+            };
+            for (int t = t0; t < t1; t += 2) {
+                turn(t, std::integral_constant<int, 0>(), sa, sb);
+                if (t + 1 < t1) turn(t + 1, std::integral_constant<int, 1>(), sb, sa);
+            }
         }
         __syncthreads();           // the buffers become the rows' way out
     } else {
@@ -738,17 +864,13 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
                 *reinterpret_cast<bf16x8*>(Vs + pn * PS + L::chunk_at(lane & 31, h, c)) = x[pn];
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        const unsigned long long none = PAGED ? __ballot(nopage) : 0;
+        const unsigned none = PAGED ? (unsigned)__ballot(nopage) : 0;
         if (t + KS < t1) {
             fetch(t + KS);
             if (t + 2 * KS < t1) look(t + 2 * KS);
         }
         hide(a, sc[0], key0 + 4 * h, p, last);
-        if (none) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (none >> (8 * (e / 4) + 4 * h + e % 4) & 1) sc[0][e] = -INFINITY;
-        }
+        if (none) hide_bits(sc[0], none, h);
         f.step(sc, a.scale2);
         mma_tr<T, DH, false, PS>(Vs, sc[0], f.o, lane);
     }
@@ -867,33 +989,32 @@ template <typename T> struct Grads {
 };
 
 // Both products of 32 LDS rows that a tile begins with (bf16): s0 = X0 Y0^T, s1 = X1
-// Y1^T; operands asked for ahead as in scores.  Y1 are a lane's rows in registers or
-// (yl) in LDS.
+// Y1^T, Y1 a lane's rows in registers or (YLDS) in LDS.
 template <int DH, bool YLDS>
 __device__ __forceinline__ void products(const __bf16* x0, const __bf16* x1, const Row<__bf16, DH>& y0,
                                          const Row<__bf16, DH>& y1, const __bf16* yl, floatx16& s0, floatx16& s1,
                                          int lane) {
     typedef Lds<DH, false> L;
-    constexpr int N = DH / 16, R = YLDS ? 3 : 2, AHEAD = N < 2 ? N : 2;      // reads a step of two products
+    constexpr int N = DH / 16, AHEAD = 2;
+    bf16x8 a0[N], a1[N], b1[N];
+    auto read = [&](int c) {
+        const int at = L::chunk_at(lane & 31, lane >> 5, c);
+        a0[c] = *reinterpret_cast<const bf16x8*>(x0 + at);
+        a1[c] = *reinterpret_cast<const bf16x8*>(x1 + at);
+        if constexpr (YLDS) b1[c] = *reinterpret_cast<const bf16x8*>(yl + at);
+    };
 #pragma unroll
     for (int e = 0; e < 16; ++e) s0[e] = s1[e] = 0.f;
 #pragma unroll
-    for (int c = 0; c < N; ++c) {
-        const int at = L::chunk_at(lane & 31, lane >> 5, c);
-        const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(x0 + at), a1 = *reinterpret_cast<const bf16x8*>(x1 + at);
-        s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, y0.f[c][0], s0, 0, 0, 0);
-        if constexpr (YLDS)
-            s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, *reinterpret_cast<const bf16x8*>(yl + at), s1, 0, 0, 0);
-        else
-            s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, y1.f[c][0], s1, 0, 0, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x100, R * AHEAD, 0);
+    for (int c = 0; c < AHEAD; ++c) read(c);
+    pin();
 #pragma unroll
-    for (int i = 0; i < N - AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    for (int c = 0; c < N; ++c) {
+        s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0[c], y0.f[c][0], s0, 0, 0, 0);
+        s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1[c], YLDS ? b1[c] : y1.f[c][0], s1, 0, 0, 0);
+        if (c + AHEAD < N) read(c + AHEAD);
+        pin();
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2 * AHEAD, 0);
 }
 
 // dQ: the forward's shape.  Per 32 keys S^T and dP^T = V dO^T with queries on
@@ -918,16 +1039,15 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const int l = xcd_block(blockIdx.x, gridDim.x);
     Work w;
     int kvh;
     if (pl.even) {
-        const int u = l / pl.qtiles;
-        kvh = u % a.KV;
-        w = {u / a.KV, pl.qtiles - 1 - l % pl.qtiles, 0, INT_MAX, 1, 0, 0, 0};
+        const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.qtiles);
+        kvh = sh.pair % a.KV;
+        w = {sh.pair / a.KV, pl.qtiles - 1 - sh.piece, 0, INT_MAX, 1, 0, 0, 0};
     } else {
-        kvh = l / pl.slots;
-        w = work_of<false, BQ, BK>(a, l % pl.slots, pl.slots, 0, false);
+        kvh = blockIdx.x % a.KV;
+        w = work_of<false, BQ, BK>(a, blockIdx.x / a.KV, pl.slots, 0, false);
     }
     w = uniform(w);
     if (w.i < 0) return;
@@ -997,11 +1117,13 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
         }
     };
     if constexpr (C::DMA) {
-        KvDma<DH, BK, NW, false> kv;
-        kv.init(a, s, g.k, g.v, kvh, tid);
+        KvDma<DH, BK, NW, false> kk, kv;
+        kk.init(a, s, g.k, kvh, a.k, s.k, tid);
+        kv.init(a, s, g.v, kvh, a.v, s.v, tid);
         auto fetch = [&](int t) {
             __bf16* to = tiles + (t & 1) * 2 * C::TILE;
-            kv.fetch(a, rg.block(t), rg.kend, to, to + C::TILE);
+            kk.fetch(a, a.k, rg.block(t), rg.kend, to);
+            kv.fetch(a, a.v, rg.block(t), rg.kend, to + C::TILE);
         };
         if (rg.nt > 0) fetch(0);
         for (int t = 0; t < rg.nt; ++t) {
@@ -1139,11 +1261,11 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     float* stats = reinterpret_cast<float*>(smem + C::BUFS + C::VROWS);   // log-sum-exp and D of the rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    // a (sequence, kv head)'s pieces: near rows of its key tiles, then far chunks of the first ones
-    const int per = pl.ktiles + pl.first * pl.chunks, b = xcd_block(blockIdx.x, gridDim.x);
-    const int u = b / per, x = b - u * per, i = u / a.KV, kvh = u - i * a.KV;
-    const bool isfar = x >= pl.ktiles;
-    const int kt = isfar ? (x - pl.ktiles) / pl.chunks : x, ch = isfar ? (x - pl.ktiles) % pl.chunks : 0;
+    // a (sequence, kv head)'s pieces: far chunks of its first key tiles, then near rows of all
+    const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.ktiles + pl.first * pl.chunks);
+    const int u = sh.pair, i = u / a.KV, kvh = u - i * a.KV, x = sh.piece - pl.first * pl.chunks;
+    const bool isfar = x < 0;
+    const int kt = isfar ? sh.piece / pl.chunks : x, ch = isfar ? sh.piece % pl.chunks : 0;
     const Seq s = seq_of<false>(a, i);
     const int kall = s.rows;          // a padded sequence's dead rows get zeros
     if (kt * C::BKEY >= kall) return;

@@ -182,4 +182,5 @@ def test_no_register_is_copied_before_the_lanes_return(name):
     assert r.returncode == 0, r.stderr[-2000:]
     assert r.stdout.count("s_or_b64 exec, exec") > 10
     lines = r.stdout.split("\n")
-    assert [x for x in stray_copies(r.stdout) if not _stored_behind(lines, int(x[1].split()[-1]) - 1, x[2])] == []
+    # v_writelane writes its lane whatever the mask
+    assert [x for x in stray_copies(r.stdout) if not x[2].startswith("v_writelane") and not _stored_behind(lines, int(x[1].split()[-1]) - 1, x[2])] == []

@@ -73,6 +73,7 @@ template <> struct Chunk<__bf16> {
     __device__ __forceinline__ void load(const __bf16* p) { w = *reinterpret_cast<const pt_uintx4*>(p); }
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rs, int off) { w = ld_buf16(rs, off); }
     __device__ __forceinline__ void zero() { w = pt_uintx4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void keep(bool ok) { w = ok ? w : pt_uintx4{0, 0, 0, 0}; }
     __device__ __forceinline__ float at(int i) const {
         return __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
     }
@@ -94,6 +95,10 @@ template <> struct Chunk<float> {
         w[1] = ld_buf16(rs, off + 16);
     }
     __device__ __forceinline__ void zero() { w[0] = w[1] = pt_uintx4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void keep(bool ok) {
+        w[0] = ok ? w[0] : pt_uintx4{0, 0, 0, 0};
+        w[1] = ok ? w[1] : pt_uintx4{0, 0, 0, 0};
+    }
     __device__ __forceinline__ float at(int i) const { return __uint_as_float(w[i / 4][i % 4]); }
 };
 

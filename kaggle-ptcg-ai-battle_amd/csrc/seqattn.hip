@@ -91,106 +91,108 @@ __device__ __forceinline__ Places places_of(const SArgs& a, const Seq& s, int r0
     return {s.p0 + q0, q1 < q0 ? -1 : s.p0 + q1};
 }
 
-// What a workgroup works on: sequence, row tile, split of the tile's key blocks (per of
-// them a split), the sequence's splits and first slot; the tile's number among all
-// (tiles of them, where there are splits).
-struct Work { int i, qt, sp, per, splits, first, tile, tiles; };
+// A workgroup's piece of work: key blocks t0 .. t1 - 1 (of those the tile has) of a row
+// tile of a sequence; where the tile is shared with other workgroups, the place of this
+// piece among the parts, its tile's number among all and, with the tile's first piece,
+// the shared ones' count.
+struct Work { int i, qt, t0, t1, part, tile; long next; };
 
-// Slots are handed out on the device, which alone knows the lengths: sequence i has
-// T_i row tiles of at most K_i key blocks; a split takes so many blocks that sum T_i
-// ceil(K_i / per) <= slots, the fewest such (searched for up to 64 sequences), and a
-// sequence's splits are made equal: every workgroup has one piece of nearly the same
-// length however the sequences differ.  Every wave counts for itself, 64 sequences at
-// a time.  i = -1: a slot too many.
-template <bool PAGED, int BQ, int BK>
-__device__ __forceinline__ Work work_of(const SArgs& a, int slot, int slots, int least, bool split) {
-    const int lane = threadIdx.x & 63;
-    auto shape = [&](int i, int& t, int& k) {
+// Splitting.  Row tiles, each as long as its sequence's longest (K_i key blocks of T_i
+// tiles), are laid end to end and cut into `slots` stretches of `per` blocks, one for
+// each workgroup that runs at once: however many tiles there are and however they
+// differ, all workgroups read the same number of keys.  A stretch may hold the end of a
+// tile, whole tiles, and the beginning of one; a tile that is cut leaves a part in each
+// of its stretches for the joining kernel: the stretch's first part, or its second
+// where the tile begins within the stretch.  The lengths are on the device
+// alone: every wave counts for itself, 64 sequences at a time.
+struct Cut { long all; int per, tiles; };
+template <bool PAGED, int BQ, int BK> struct Deal {
+    static __device__ __forceinline__ void shape(const SArgs& a, int i, int& t, int& k) {
         t = k = 0;
         if (i >= a.n) return;
         const Seq s = seq_of<PAGED>(a, i);
         t = (s.rows * a.G + BQ - 1) / BQ;
         const Places p = {s.p0, s.p0 + s.ql - 1};
-        // the blocks of all rows, and of a tile of rows in a window
+        // the blocks of all rows, and of a tile of rows in a window; a tile that sees nothing is one too
         k = range_of<BK>(a, p.lo, p.hi, s.kl).nt;
         if (a.window < INT_MAX - 4 * BQ)
             k = min(k, (a.window + (BQ + a.G - 2) / a.G) / BK + 2 + (min(a.sinks, s.kl) + BK - 1) / BK);
-    };
-    auto sum = [](int x) {
-        for (int o = 1; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-        return x;
-    };
-    auto over = [](int k, int per) { return max(1, (k - 1) / per + 1); };      // splits
-    int per = INT_MAX, st = 0, t, k;
-    if (split) {
-        float sk = 0.f;      // counts of blocks: only bounds of the search come of them
+        k = max(k, 1);
+    }
+    static __device__ __forceinline__ Cut cut(const SArgs& a, int slots, int least) {
+        const int lane = threadIdx.x & 63;
+        long all = 0;
+        int tiles = 0, t, k;
         for (int i0 = 0; i0 < a.n; i0 += 64) {
-            shape(i0 + lane, t, k);
-            st += t;
-            sk += (float)t * (float)k;
+            shape(a, i0 + lane, t, k);
+            all += (long)t * k;
+            tiles += t;
         }
-        st = sum(st);
-        for (int o = 1; o < 64; o <<= 1) sk += __shfl_xor(sk, o, 64);
-        if (slots > st) {
-            per = (int)fminf(sk * 1.0001f / (float)(slots - st) + 1.f, 1e9f);
-            if (a.n <= 64) {
-                int lo = max(1, (int)(sk * 0.9999f / (float)slots));      // too few, or just enough
-                while (per - lo > 1 + lo / 32) {
-                    const int mid = lo + (per - lo) / 2;
-                    if (sum(t * over(k, mid)) <= slots) per = mid;
-                    else lo = mid;
+        for (int o = 1; o < 64; o <<= 1) {
+            all += __shfl_xor(all, o, 64);
+            tiles += __shfl_xor(tiles, o, 64);
+        }
+        return {all, max(least, (int)((all + slots - 1) / slots)), tiles};
+    }
+    // the work from block b on, up to block end; per: of the cut (0: b counts tiles, nothing is shared)
+    static __device__ __forceinline__ Work at(const SArgs& a, long b, long end, int per) {
+        const int lane = threadIdx.x & 63;
+        long before = 0;
+        int tiles = 0, t, k;
+        for (int i0 = 0; i0 < a.n; i0 += 64) {
+            shape(a, i0 + lane, t, k);
+            if (per == 0) k = 1;
+            const long c = (long)t * k;
+            long to = c;
+            int tt = t;
+            for (int o = 1; o < 64; o <<= 1) {
+                const long x = __shfl_up(to, o, 64);
+                const int y = __shfl_up(tt, o, 64);
+                if (lane >= o) {
+                    to += x;
+                    tt += y;
                 }
             }
-            per = max(per, least);
-        }
-    }
-    int before = 0, tiles = 0;
-    for (int i0 = 0; i0 < a.n; i0 += 64) {
-        if (!split || a.n > 64) shape(i0 + lane, t, k);
-        const int s = over(k, per), c = t * s;
-        int to = c, tt = t;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(to, o, 64), y = __shfl_up(tt, o, 64);
-            if (lane >= o) {
-                to += x;
-                tt += y;
+            to += before;
+            const unsigned long long m = __ballot(b >= to - c && b < to);
+            if (m) {
+                const int w = __builtin_ctzll(m);
+                const int kw = __builtin_amdgcn_readlane(k, w), nt = __builtin_amdgcn_readlane(t, w);
+                const long off = b - __shfl(to - c, w, 64);
+                const int q = (int)(off / kw);
+                Work r;
+                r.i = i0 + w;
+                r.qt = nt - 1 - q;                          // the last tile first: its rows see the most
+                r.tile = tiles + __builtin_amdgcn_readlane(tt, w) - nt + q;
+                r.t0 = (int)(off - (long)q * kw);
+                r.t1 = per == 0 ? INT_MAX : (int)(kw - r.t0 < end - b ? kw : r.t0 + (end - b));
+                r.next = b + (r.t1 - r.t0);
+                const long first = b - r.t0;                 // the tile's first block
+                r.part = -1;
+                if (per > 0 && first / per != (first + kw - 1) / per)
+                    r.part = (int)(b / per) * 2 + (b % per != 0);
+                return r;
             }
+            before = __shfl(to, 63, 64);
+            tiles += __builtin_amdgcn_readlane(tt, 63);
         }
-        const unsigned long long m = __ballot(slot >= before + to - c && slot < before + to);
-        if (m) {
-            const int w = __builtin_ctzll(m);
-            Work r;
-            r.i = i0 + w;
-            r.splits = __builtin_amdgcn_readlane(s, w);
-            r.first = before + __builtin_amdgcn_readlane(to - c, w);
-            const int nt = __builtin_amdgcn_readlane(t, w), rest = slot - r.first;
-            r.per = r.splits > 1 ? (__builtin_amdgcn_readlane(k, w) - 1) / r.splits + 1 : INT_MAX;
-            // the last tile first: its rows see the most
-            r.qt = nt - 1 - rest / r.splits;
-            r.sp = rest % r.splits;
-            r.tile = tiles + __builtin_amdgcn_readlane(tt - t, w) + r.qt;
-            r.tiles = st;
-            return r;
-        }
-        before += __builtin_amdgcn_readlane(to, 63);
-        tiles += __builtin_amdgcn_readlane(tt, 63);
+        return {-1, 0, 0, 0, -1, 0, end};
     }
-    return {-1, 0, 0, 0, 0, 0, 0, st};
-}
+};
 // the same in scalar registers, as it is one for all lanes
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long uniform(long x) {
+    return (long)(unsigned)uniform((int)x) | (long)uniform((int)(x >> 32)) << 32;
+}
 __device__ __forceinline__ Work uniform(const Work& w) {
-    auto u = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-    return {u(w.i), u(w.qt), u(w.sp), u(w.per), u(w.splits), u(w.first), u(w.tile), u(w.tiles)};
+    return {uniform(w.i), uniform(w.qt), uniform(w.t0), uniform(w.t1), uniform(w.part), uniform(w.tile), uniform(w.next)};
 }
-// where a split leaves its part: slot of its piece
-__device__ __forceinline__ int piece_of(const Work& w, int tiles, int qt, int sp) {
-    return w.first + (tiles - 1 - qt) * w.splits + sp;
-}
-// What the joining kernel is told: a tile's sequence, number in it, first piece and splits
+__device__ __forceinline__ Cut uniform(const Cut& c) { return {uniform(c.all), uniform(c.per), uniform(c.tiles)}; }
+// What the joining kernel is told: a tile's sequence, number in it, first part and how many
 // (1: nothing to join); before the first, how many tiles there are.
-struct Joint { int i, qt, piece, splits; };
-// a piece's rows, unnormalised, then their maxima and sums
-__host__ __device__ constexpr long piece_floats(int prow, int dh) { return ((long)prow * (dh + 2) + 3) / 4 * 4; }
+struct Joint { int i, qt, part, parts; };
+// a part's rows, unnormalised, then their maxima and sums
+__host__ __device__ constexpr long part_floats(int prow, int dh) { return ((long)prow * (dh + 2) + 3) / 4 * 4; }
 
 // Scores of keys that a row of place p does not see become -inf, whatever they are:
 // register e is key k0 + 8 (e / 4) + e % 4.  last: the lesser of p and the last key.
@@ -222,14 +224,38 @@ __device__ __forceinline__ bool all_hidden(const SArgs& a, int k0, int nk, int l
 __device__ __forceinline__ int page_of(const SArgs& a, int key) {
     return a.page == 1 ? key : (int)(__umulhi((unsigned)key, a.pmagic) >> a.pshift);      // exact below 2^31
 }
+// (kend > 0: the table's first entry is read for keys that are not there; without
+// branches, as regions of some lanes in loops that fill the registers cost more)
 __device__ __forceinline__ int entry_of(const SArgs& a, const Seq& s, int key, int kend) {
-    return key < kend ? s.table[page_of(a, key)] : -1;
+    const int e = s.table[key < kend ? page_of(a, key) : 0];
+    return key < kend ? e : -1;
+}
+// p where ok, else an address that can be read
+template <typename T> __device__ __forceinline__ const T* where(bool ok, const T* p, const T* other) {
+    return ok ? p : other;
+}
+// The kernel's first argument, read again from memory where this is called: around a loop
+// over pieces of work the compiler would hold all of it in scalar registers, which do
+// not suffice.
+__device__ __forceinline__ const SArgs& args_again() {
+    typedef const __attribute__((address_space(4))) SArgs* ArgP;
+    ArgP p = (ArgP)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const SArgs*)p;
 }
 
 // the larger of both halves' values
 __device__ __forceinline__ float half_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// the thread's number, for the compiler not the same each time: nothing made from it is
+// held in registers around the pieces of work
+__device__ __forceinline__ int thread_again() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
 }
 
 // A running softmax of the rows on lanes: m2, a bound of the scores (s scale2) so far
@@ -420,8 +446,9 @@ template <typename T, int DH, bool PAD, int BK, int NTH, bool PAGED> struct KvRe
             entf = tid < BK ? entry_of(a, s, block * BK + tid, kend) : 0;
         }
     }
-    __device__ __forceinline__ void fetch(const SArgs& a, const Seq& s, const T* kp, const T* vp, int kvh, int block,
-                                          int kend, int tid) {
+    // q: an address that can be read
+    __device__ __forceinline__ void fetch(const SArgs& a, const Seq& s, const T* kp, const T* vp, const T* q, int kvh,
+                                          int block, int kend, int tid) {
         if constexpr (!PAGED) {
             const auto rk = kb.rows(block * BK, kend, BK), rv = vb.rows(block * BK, kend, BK);
             k.load(rk, ko, kb.ld);
@@ -433,12 +460,12 @@ template <typename T, int DH, bool PAD, int BK, int NTH, bool PAGED> struct KvRe
 #pragma unroll
             for (int i = 0; i < St::NCH; ++i) {
                 const int key = block * BK + tid / St::CPR + i * St::RPP;
-                if (key < kend && col < a.dh && (unsigned)ent[i] < (unsigned)a.pages) {
-                    const int off = key - page_of(a, key) * a.page;
-                    ok |= 1u << i;
-                    k.r[i].load(kp + (long)ent[i] * a.k.sn + (long)off * a.k.sl + (long)kvh * a.k.sh + col);
-                    v.r[i].load(vp + (long)ent[i] * a.v.sn + (long)off * a.v.sl + (long)kvh * a.v.sh + col);
-                }
+                // what is not there: any address that can be read, dropped in store
+                const bool there = key < kend && col < a.dh && (unsigned)ent[i] < (unsigned)a.pages;
+                const int off = key - page_of(a, key) * a.page;
+                ok |= there ? 1u << i : 0u;
+                k.r[i].load(where(there, kp + (long)ent[i] * a.k.sn + (long)off * a.k.sl + (long)kvh * a.k.sh + col, q));
+                v.r[i].load(where(there, vp + (long)ent[i] * a.v.sn + (long)off * a.v.sl + (long)kvh * a.v.sh + col, q));
             }
         }
     }
@@ -475,7 +502,7 @@ template <int DH, int BK, int NW, bool PAGED> struct KvDma {
     typedef Lds<DH, false> L;
     static constexpr int CPR = DH / 8, WR = BK / NW, RPI = 64 / CPR, NI = WR / RPI;   // rows a wave, an instruction
     static_assert(WR % RPI == 0, "whole instructions");
-    int off[NI], ld, width, row, ent;
+    int off[NI], ld, width, row;
     const char* base;
     // rows of layout l; row0: the sequence's first (one matrix)
     __device__ __forceinline__ void init(const SArgs& a, const Seq& s, const __bf16* x, int kvh, const PtcgHeadLayout& l,
@@ -491,17 +518,14 @@ template <int DH, int BK, int NW, bool PAGED> struct KvDma {
             off[i] = 8 * c < a.dh ? r * ld + 16 * c : PT_NOWHERE;
         }
     }
-    // the page-table entry that fetch(block) will need
-    __device__ __forceinline__ void look(const SArgs& a, const Seq& s, int block, int kend) {
-        if constexpr (PAGED) ent = entry_of(a, s, block * BK + row, kend);
-    }
     static __device__ __forceinline__ intx4 rsrc(const char* p, int bytes) {
         const unsigned long long x = (unsigned long long)p;
         return intx4{__builtin_amdgcn_readfirstlane((int)(unsigned)x),
                      __builtin_amdgcn_readfirstlane((int)(unsigned)(x >> 32)), __builtin_amdgcn_readfirstlane(bytes),
                      0x00020000};
     }
-    __device__ __forceinline__ void fetch(const SArgs& a, const PtcgHeadLayout& l, int block, int kend,
+    // ent: the page that the wave's rows lie in
+    __device__ __forceinline__ void fetch(const SArgs& a, const PtcgHeadLayout& l, int block, int kend, int ent,
                                           __bf16* to) const {
         const int key = block * BK + row;
         int n = max(0, min(kend - key, WR));
@@ -546,15 +570,57 @@ __device__ __forceinline__ Share share_of(int b, int pairs, int per) {
     return {8 * full + r % rest, r / rest};
 }
 
-// How slots become work, as the host decided: even: every sequence has qtiles row
-// tiles and nothing is split.
+// How workgroups get their work, as the host decided: even: every sequence has qtiles row
+// tiles and nothing is split; split: `slots` stretches a kv head; else a row tile each
+// (tiles: at most so many).
 struct Plan { int slots, tiles, qtiles, least, prow; bool even, split; };
+
+// A workgroup's work, one call of f after the other; js: what the joining kernel is told.
+template <bool PAGED, int BQ, int BK, class F>
+__device__ __forceinline__ void work_through(const SArgs& a, const Plan& pl, Joint* js, F f) {
+    typedef Deal<PAGED, BQ, BK> D;
+    Work w;
+    int kvh, per = 0;
+    long b = 0, end = 1;
+    if (pl.even) {
+        const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.qtiles);
+        kvh = sh.pair % a.KV;
+        w = {sh.pair / a.KV, pl.qtiles - 1 - sh.piece, 0, INT_MAX, -1, 0, 1};
+    } else if (!pl.split) {
+        kvh = blockIdx.x % a.KV;             // unequal tiles are spread over the XCDs
+        b = blockIdx.x / a.KV;
+        end = b + 1;
+    } else {
+        const int l = xcd_block(blockIdx.x, gridDim.x);
+        kvh = l / pl.slots;
+        const Cut c = uniform(D::cut(a, pl.slots, pl.least));
+        if (l == 0 && threadIdx.x == 0) js[0].i = c.tiles;
+        per = c.per;
+        b = (long)(l - kvh * pl.slots) * per;
+        end = b + per < c.all ? b + per : c.all;
+    }
+    while (b < end) {
+        if (!pl.even) w = uniform(D::at(a, b, end, per));
+        if (w.i < 0) break;
+        f(w, kvh, per);
+        b = w.next;
+        if (b < end) __syncthreads();        // the next one's tiles take the place of these rows' way out
+    }
+}
+// whether a piece of a tile of nt key blocks leaves a part; the tile's first piece notes
+// what there is to join
+__device__ __forceinline__ bool shared_tile(Joint* js, const Work& w, int kvh, int per, int nt) {
+    const bool cut = w.part >= 0 && (w.t0 > 0 || nt > w.t1);
+    if (per > 0 && w.t0 == 0 && kvh == 0 && threadIdx.x == 0)
+        js[1 + w.tile] = {w.i, w.qt, w.part, cut ? 1 + (nt - w.t1 + per - 1) / per : 1};
+    return cut;
+}
 
 // A workgroup owns 32 NW rows and walks their key blocks (or its split of them).
 // DMA: tiles go straight into one of two buffers while the other is worked on, one
 // barrier a tile; else through registers into one buffer.
 template <typename T, int DH, int NW, bool PAGED, bool DMA>
-__global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel(const SArgs a, const T* __restrict__ q,
+__global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel(const SArgs a_, const T* __restrict__ q,
         const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
         float* __restrict__ part, const Plan pl) {
     typedef TileCfg<T, DH, NW, DMA> C;
@@ -564,31 +630,17 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     float* kf = reinterpret_cast<float*>(smem + C::BUFS);
     int* bad = reinterpret_cast<int*>(smem + C::LDS - 64);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    Work w;
-    int kvh;
-    if (pl.even) {
-        const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.qtiles);
-        kvh = sh.pair % a.KV;
-        w = {sh.pair / a.KV, pl.qtiles - 1 - sh.piece, 0, INT_MAX, 1, 0, 0, 0};
-    } else {
-        kvh = blockIdx.x % a.KV;
-        w = work_of<PAGED, BQ, BK>(a, blockIdx.x / a.KV, pl.slots, pl.least, pl.split);
-    }
-    w = uniform(w);
     Joint* const js = reinterpret_cast<Joint*>(part);      // then the parts
-    if (pl.split && blockIdx.x == 0 && tid == 0) js[0].i = w.tiles;
-    if (w.i < 0) return;
+    work_through<PAGED, BQ, BK>(a_, pl, js, [&](const Work& w, int kvh, int per) {
+    const SArgs& a = args_again();
+    const int tid = thread_again(), lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
     const Seq s = seq_of<PAGED>(a, w.i);
     const int rows = s.rows * a.G, tile0 = w.qt * BQ;
-    if (tile0 >= rows) return;
     const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
     const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
-    const bool joined = rg.nt > w.per;                    // by the joining kernel
-    if (pl.split && w.sp == 0 && kvh == 0 && tid == 0)
-        js[1 + w.tile] = {w.i, w.qt, piece_of(w, (rows + BQ - 1) / BQ, w.qt, 0), joined ? (rg.nt - 1) / w.per + 1 : 1};
-    const int t0 = joined ? w.sp * w.per : 0, t1 = joined ? min(rg.nt, t0 + w.per) : rg.nt;
-    if (joined ? t0 >= rg.nt : w.sp > 0) return;
+    const int t0 = w.t0, t1 = min(rg.nt, w.t1);
+    const bool joined = shared_tile(js, w, kvh, per, rg.nt);
+    if (t0 > 0 && t0 >= rg.nt) return;
     if (PAGED && tid == 0) *bad = 0;
 
     const int r0 = tile0 + 32 * wave, r = r0 + (lane & 31);
@@ -635,14 +687,27 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         kk.init(a, s, k, kvh, a.k, s.k, tid);
         kv.init(a, s, v, kvh, a.v, s.v, tid);
         __bf16 *kbuf = tiles, *vbuf = tiles + 2 * C::TILE;
-        auto fetch_k = [&](int t) {
-            kk.fetch(a, a.k, rg.block(t), rg.kend, kbuf + (t - t0 & 1) * C::TILE);
-            if (t + 1 < t1) kk.look(a, s, rg.block(t + 1), rg.kend);
+        auto fetch_k = [&](int t, int ent) {
+            kk.fetch(a, a.k, rg.block(t), rg.kend, ent, kbuf + (t - t0 & 1) * C::TILE);
         };
-        auto fetch_v = [&](int t) {
-            kv.fetch(a, a.v, rg.block(t), rg.kend, vbuf + (t - t0 & 1) * C::TILE);
-            if (t + 1 < t1) kv.look(a, s, rg.block(t + 1), rg.kend);
+        auto fetch_v = [&](int t, int ent) {
+            kv.fetch(a, a.v, rg.block(t), rg.kend, ent, vbuf + (t - t0 & 1) * C::TILE);
         };
+        // the page of the wave's rows of tile t: 64 tiles' on the lanes, looked up at once (a
+        // scalar load a tile would make every LDS read behind it wait for it)
+        int ents = 0, ents0 = t0 - 64;
+        auto entry = [&](int t) {
+            if constexpr (PAGED) {
+                if (t - ents0 >= 64) {
+                    ents0 = t;
+                    const int key = rg.block(t + lane) * BK + kk.row;
+                    ents = t + lane < t1 && key < rg.kend ? s.table[page_of(a, key)] : -1;
+                }
+                return __builtin_amdgcn_readlane(ents, t - ents0);
+            }
+            return 0;
+        };
+        int e1 = 0;      // that of the tile whose values come next
         auto lacks = [&](int t) {       // a lane per key
             const int key = rg.block(t) * BK + lane;
             return key < rg.kend && (unsigned)s.table[page_of(a, key)] >= (unsigned)a.pages;
@@ -664,11 +729,11 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         };
         constexpr int ES = 16 / (DH / 8) , EV = 16 / (DH / 16);     // elements in a product's shadow
         if (t0 < t1) {
-            kk.look(a, s, rg.block(t0), rg.kend);
-            kv.look(a, s, rg.block(t0), rg.kend);
-            fetch_k(t0);
-            if (t0 + 1 < t1) fetch_k(t0 + 1);
-            fetch_v(t0);
+            const int e0 = entry(t0);
+            e1 = entry(t0 + 1 < t1 ? t0 + 1 : t0);
+            fetch_k(t0, e0);
+            if (t0 + 1 < t1) fetch_k(t0 + 1, e1);
+            fetch_v(t0, e0);
             if constexpr (PAGED) {
                 for (int t = t0 + wave; t < t1; t += NW) some |= lacks(t);
                 some = __syncthreads_or(some);
@@ -688,8 +753,11 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
                     arrived();
                     __syncthreads();   // everyone's pieces are here; keys of tile t and values of t - 1 are done with
                 }
-                if (t + 1 < t1) fetch_v(t + 1);
-                if (t + 2 < t1) fetch_k(t + 2);
+                if (t + 1 < t1) fetch_v(t + 1, e1);
+                if (t + 2 < t1) {
+                    e1 = entry(t + 2);
+                    fetch_k(t + 2, e1);
+                }
                 const __bf16* Vs = vbuf + at * C::TILE;
                 const float ms = f.m2 == -INFINITY ? 0.f : f.m2;
                 bf16x8 pa[2], pb[2];
@@ -721,7 +789,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         Kv kv;
         kv.init(a, s, k, v, kvh, tid);
         auto fetch = [&](int t) {
-            kv.fetch(a, s, k, v, kvh, rg.block(t), rg.kend, tid);
+            kv.fetch(a, s, k, v, q, kvh, rg.block(t), rg.kend, tid);
             if (t + 1 < t1) kv.look(a, s, rg.block(t + 1), rg.kend, tid);
         };
         if (t0 < t1) {
@@ -745,13 +813,11 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         }
     }
     f.l += half_swap(f.l);
-    const int tiles_ = (rows + BQ - 1) / BQ;
-    float* pp = nullptr;
-    if (joined)
-        pp = part + 4 * (1 + pl.tiles) + ((long)piece_of(w, tiles_, w.qt, w.sp) * a.KV + kvh) * piece_floats(pl.prow, a.dh);
+    float* pp = joined ? part + 4 * (1 + pl.tiles) + ((long)w.part * a.KV + kvh) * part_floats(pl.prow, a.dh) : nullptr;
     if (live)
         finish<T, DH, BQ>(a, s, w.i, kvh, tile0, r0, f, out, lse, pp, pl.prow,
                           reinterpret_cast<T*>(smem) + wave * Out<T, DH>::WAVE, lane);
+    });
 }
 
 // ------------------------------------------------------------ few rows
@@ -769,33 +835,25 @@ template <typename T, int DH, int KS> struct TokenCfg {
 };
 
 template <typename T, int DH, int KS, bool PAGED>
-__global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kernel(const SArgs a,
+__global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kernel(const SArgs a_,
         const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out,
         float* __restrict__ lse, float* __restrict__ part, const Plan pl) {
     typedef TokenCfg<T, DH, KS> C;
     typedef Lds<DH, false> L;
     constexpr int BK = C::BK, BQ = C::BQ, PS = BK * L::ST;
     extern __shared__ __align__(256) char smem[];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    __bf16* Vs = reinterpret_cast<__bf16*>(smem) + wave * C::TILE;
-    const int kvh = blockIdx.x % a.KV, slot = blockIdx.x / a.KV;
-    Work w;
-    if (pl.even) w = {slot / pl.qtiles, pl.qtiles - 1 - slot % pl.qtiles, 0, INT_MAX, 1, 0, 0, 0};
-    else w = work_of<PAGED, BQ, BK>(a, slot, pl.slots, pl.least, pl.split);
-    w = uniform(w);
     Joint* const js = reinterpret_cast<Joint*>(part);      // then the parts
-    if (pl.split && blockIdx.x == 0 && tid == 0) js[0].i = w.tiles;
-    if (w.i < 0) return;
+    work_through<PAGED, BQ, BK>(a_, pl, js, [&](const Work& w, int kvh, int per) {
+    const SArgs& a = args_again();
+    const int tid = thread_again(), lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
+    __bf16* Vs = reinterpret_cast<__bf16*>(smem) + wave * C::TILE;
     const Seq s = seq_of<PAGED>(a, w.i);
     const int rows = s.rows * a.G, tile0 = w.qt * BQ;
-    if (tile0 >= rows) return;
     const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
     const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
-    const bool joined = rg.nt > w.per;
-    if (pl.split && w.sp == 0 && kvh == 0 && tid == 0)
-        js[1 + w.tile] = {w.i, w.qt, piece_of(w, (rows + BQ - 1) / BQ, w.qt, 0), joined ? (rg.nt - 1) / w.per + 1 : 1};
-    const int t0 = joined ? w.sp * w.per : 0, t1 = joined ? min(rg.nt, t0 + w.per) : rg.nt;
-    if (joined ? t0 >= rg.nt : w.sp > 0) return;
+    const int t0 = w.t0, t1 = min(rg.nt, w.t1);
+    const bool joined = shared_tile(js, w, kvh, per, rg.nt);
+    if (t0 > 0 && t0 >= rg.nt) return;
 
     const int r = tile0 + (lane & 31);
     const bool rok = r < rows;
@@ -807,7 +865,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
 
     Chunk<T> kc[DH / 16], vc[DH / 16];
     int ent = 0;
-    bool nopage = false;
+    bool nopage = false, here = false;
     auto look = [&](int t) {
         if constexpr (PAGED) ent = entry_of(a, s, rg.block(t) * BK + (lane & 31), rg.kend);
     };
@@ -825,17 +883,15 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
             ka = s.k + (long)key * a.k.sl;
             va = s.v + (long)key * a.v.sl;
         }
+        // rows and columns that are not there: any address that can be read, then zeros
         const T *kr = k + ka + (long)kvh * a.k.sh + 8 * h, *vr = v + va + (long)kvh * a.v.sh + 8 * h;
 #pragma unroll
-        for (int c = 0; c < DH / 16; ++c) {
-            kc[c].zero();
-            if (there && 16 * c + 8 * h < a.dh) kc[c].load(kr + 16 * c);
-        }
+        for (int c = 0; c < DH / 16; ++c)
+            kc[c].load(where(there && 16 * c + 8 * h < a.dh, kr + 16 * c, q));
 #pragma unroll
-        for (int c = 0; c < DH / 16; ++c) {
-            vc[c].zero();
-            if (there && 16 * c + 8 * h < a.dh) vc[c].load(vr + 16 * c);
-        }
+        for (int c = 0; c < DH / 16; ++c)
+            vc[c].load(where(there && 16 * c + 8 * h < a.dh, vr + 16 * c, q));
+        here = there;
     };
     int t = t0 + wave;
     if (t < t1) {
@@ -851,6 +907,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c) {
             bf16x8 x[planes<T>()];
+            kc[c].keep(here && 16 * c + 8 * h < a.dh);
             kc[c].terms(x);
             mma(x, qf.f[c], sc[0]);
         }
@@ -858,6 +915,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c) {
             bf16x8 x[planes<T>()];
+            vc[c].keep(here && 16 * c + 8 * h < a.dh);
             vc[c].terms(x);
 #pragma unroll
             for (int pn = 0; pn < planes<T>(); ++pn)
@@ -901,16 +959,17 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
             f.l = f.l * f0 + lw * f1;
             f.m2 = mn;
 #pragma unroll
-            for (int dt = 0; dt < DH / 32; ++dt)
+            for (int dt = 0; dt < DH / 32; ++dt) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) f.o[dt][e] = f.o[dt][e] * f0 + x[(dt * 16 + e) * 64 + lane] * f1;
+                pin();      // not all the reads at once, whose registers would spill
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");      // before the parts become the rows' way out
     }
-    float* pp = nullptr;
-    if (joined)
-        pp = part + 4 * (1 + pl.tiles) + ((long)piece_of(w, (rows + BQ - 1) / BQ, w.qt, w.sp) * a.KV + kvh) * piece_floats(pl.prow, a.dh);
+    float* pp = joined ? part + 4 * (1 + pl.tiles) + ((long)w.part * a.KV + kvh) * part_floats(pl.prow, a.dh) : nullptr;
     finish<T, DH, BQ>(a, s, w.i, kvh, tile0, tile0, f, out, lse, pp, pl.prow, reinterpret_cast<T*>(smem), lane);
+    });
 }
 
 // ---------------------------------------------------------------- joining
@@ -929,8 +988,7 @@ __global__ __launch_bounds__(JOIN_NTH) void seq_join_kernel(const SArgs a, const
     const Joint* js = reinterpret_cast<const Joint*>(part);
     if (tile >= js[0].i) return;
     const Joint w = js[1 + tile];
-    const int nsp = w.splits;
-    if (nsp <= 1) return;        // made by one workgroup
+    if (w.parts <= 1) return;        // made by one workgroup
     const Seq s = seq_of<PAGED>(a, w.i);
     const int rows = s.rows * a.G, tile0 = w.qt * BQ;
     const int row = rg_ * (NG / per_row) + grp / per_row, r = tile0 + row;
@@ -947,11 +1005,12 @@ __global__ __launch_bounds__(JOIN_NTH) void seq_join_kernel(const SArgs a, const
         acc.z = acc.z * f0 + x.z * f1; acc.w = acc.w * f0 + x.w * f1;
     };
     if (live) {
-        const long stride = (long)a.KV * piece_floats(pl.prow, a.dh);
-        const float* p0 = part + 4 * (1 + pl.tiles) + ((long)w.piece * a.KV + kvh) * piece_floats(pl.prow, a.dh);
+        // the first part's place, then the first places of the stretches after it
+        const float* p0 = part + 4 * (1 + pl.tiles);
 #pragma unroll 4
-        for (int u = g0; u < nsp; u += per_row) {
-            const float* x = p0 + u * stride;
+        for (int u = g0; u < w.parts; u += per_row) {
+            const long at = u == 0 ? w.part : ((w.part >> 1) + u) * 2;
+            const float* x = p0 + (at * a.KV + kvh) * part_floats(pl.prow, a.dh);
             const float2 e = *reinterpret_cast<const float2*>(x + (long)pl.prow * a.dh + 2 * row);
             float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
             if (4 * c < a.dh) y = *reinterpret_cast<const float4*>(x + (long)row * a.dh + 4 * c);
@@ -1039,18 +1098,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    Work w;
-    int kvh;
-    if (pl.even) {
-        const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.qtiles);
-        kvh = sh.pair % a.KV;
-        w = {sh.pair / a.KV, pl.qtiles - 1 - sh.piece, 0, INT_MAX, 1, 0, 0, 0};
-    } else {
-        kvh = blockIdx.x % a.KV;
-        w = work_of<false, BQ, BK>(a, blockIdx.x / a.KV, pl.slots, 0, false);
-    }
-    w = uniform(w);
-    if (w.i < 0) return;
+    work_through<false, BQ, BK>(a, pl, nullptr, [&](const Work& w, int kvh, int) {
     const Seq s = seq_of<false>(a, w.i);
     const int rows = s.rows * a.G, tile0 = w.qt * BQ;
     if (tile0 >= rows) return;
@@ -1122,8 +1170,8 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
         kv.init(a, s, g.v, kvh, a.v, s.v, tid);
         auto fetch = [&](int t) {
             __bf16* to = tiles + (t & 1) * 2 * C::TILE;
-            kk.fetch(a, a.k, rg.block(t), rg.kend, to);
-            kv.fetch(a, a.v, rg.block(t), rg.kend, to + C::TILE);
+            kk.fetch(a, a.k, rg.block(t), rg.kend, 0, to);
+            kv.fetch(a, a.v, rg.block(t), rg.kend, 0, to + C::TILE);
         };
         if (rg.nt > 0) fetch(0);
         for (int t = 0; t < rg.nt; ++t) {
@@ -1136,7 +1184,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     } else {
         Kv kv;
         kv.init(a, s, g.k, g.v, kvh, tid);
-        auto fetch = [&](int t) { kv.fetch(a, s, g.k, g.v, kvh, rg.block(t), rg.kend, tid); };
+        auto fetch = [&](int t) { kv.fetch(a, s, g.k, g.v, g.q, kvh, rg.block(t), rg.kend, tid); };
         if (rg.nt > 0) {
             fetch(0);
             kv.store(tiles, tiles + C::TILE, nullptr, nullptr, tid);
@@ -1162,6 +1210,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     }
     Out<T, DH>::query_rows(a, a.q, g.dq + s.q, kvh, r0, rows, acc, a.scale,
                            reinterpret_cast<T*>(smem) + wave * Out<T, DH>::WAVE, lane);
+    });
 }
 
 // How dK / dV's work is cut.  Key tiles of 32 NK keys; where a window has first tokens,
@@ -1538,19 +1587,13 @@ Form form_of(const SArgs& a, int64_t packed_rows, int64_t keys, bool bf16, bool 
         const int64_t t = packed_rows * a.G / f.bq + a.n;
         if (t < tiles) tiles = t;
     }
-    // Where row tiles do not fill the card, pieces do: as many workgroups as run at once, twice
-    // as many where few splits a tile would leave much of a round idle.  A split is
-    // two blocks a wave at least, and costs a second launch.
+    // Where row tiles do not fill the card, stretches of keys do, one for each workgroup that
+    // runs at once.  A stretch is two blocks a wave at least, and costs a second launch.
     const int64_t fill = (bf16 || a.dh <= 64 ? 2 : 1) * (int64_t)cu_count();
     f.p.least = f.token ? 2 * f.waves : 4;
     f.p.split = may_split && tiles * a.KV < fill && keys >= 4 * f.p.least * f.bk;
     f.p.tiles = (int)tiles;
-    int64_t slots = tiles;
-    if (f.p.split) {
-        const int64_t most = (tiles * a.KV * 4 > fill ? 2 * fill : fill) / a.KV;
-        if (most > slots) slots = most;
-    }
-    f.p.slots = (int)slots;
+    f.p.slots = (int)(f.p.split ? (fill / a.KV > 1 ? fill / a.KV : 1) : tiles);
     f.p.qtiles = qtiles;
     f.p.even = !a.q_off && !f.p.split;
     f.p.prow = (int)(rows < f.bq ? rows : f.bq);
@@ -1565,7 +1608,7 @@ Form window_form(const PtcgWindowAttn* d, const SArgs& a) {
     return form_of(a, (int64_t)d->n * d->l, d->l, d->bf16, true);
 }
 int64_t part_bytes(const Form& f, const SArgs& a) {
-    return f.p.split ? 16 * (1 + (int64_t)f.p.tiles) + (int64_t)f.p.slots * a.KV * piece_floats(f.p.prow, a.dh) * 4 : 0;
+    return f.p.split ? 16 * (1 + (int64_t)f.p.tiles) + 2 * (int64_t)f.p.slots * a.KV * part_floats(f.p.prow, a.dh) * 4 : 0;
 }
 
 template <typename T, int DH, bool PAGED, int BQ>

@@ -329,10 +329,9 @@ template <int DH> struct Soft {
 // many on their way that registers spill.
 __device__ __forceinline__ void pin() { __builtin_amdgcn_sched_barrier(0); }
 
-// S^T of 64 keys in LDS (bf16), a product at a time; side(i) goes into product i's shadow.
-template <int DH, class Side>
-__device__ __forceinline__ void scores(const __bf16* ks, const Row<__bf16, DH>& q, floatx16 (&sc)[2], int lane,
-                                       Side side) {
+// S^T of 64 keys in LDS (bf16), a product at a time
+template <int DH>
+__device__ __forceinline__ void scores(const __bf16* ks, const Row<__bf16, DH>& q, floatx16 (&sc)[2], int lane) {
     typedef Lds<DH, false> L;
     constexpr int N = DH / 8, AHEAD = 4;       // operands on their way
     bf16x8 x[N];
@@ -350,7 +349,6 @@ __device__ __forceinline__ void scores(const __bf16* ks, const Row<__bf16, DH>& 
     for (int i = 0; i < N; ++i) {
         sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x[i], q.f[i >> 1][0], sc[i & 1], 0, 0, 0);
         if (i + AHEAD < N) read(i + AHEAD);
-        side(i);
         pin();
     }
 }
@@ -492,23 +490,25 @@ __device__ __forceinline__ void to_lds(intx4 rs, const __bf16* base, int off) {
     asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(rs) : "memory");
 }
-__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// all but the last N instructions' pieces have arrived
+template <int N = 0> __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// A tile of BK key or value rows by 16-byte pieces straight into LDS (bf16): every wave
-// brings BK / NW rows that lie in one matrix, or in one page (whose size is a multiple
-// of them).  A piece's place in LDS is its lane's, so the lane chooses the chunk that
+// A tile of BK key or value rows by 16-byte pieces straight into LDS (bf16): waves bring WR
+// rows each that lie in one matrix, or in one page (whose size is a multiple of
+// them).  A piece's place in LDS is its lane's, so the lane chooses the chunk that
 // belongs there.
 template <int DH, int BK, int NW, bool PAGED> struct KvDma {
     typedef Lds<DH, false> L;
-    static constexpr int CPR = DH / 8, WR = BK / NW, RPI = 64 / CPR, NI = WR / RPI;   // rows a wave, an instruction
-    static_assert(WR % RPI == 0, "whole instructions");
+    static constexpr int CPR = DH / 8, RPI = 64 / CPR;                     // rows an instruction
+    static constexpr int WR = BK / NW > RPI ? BK / NW : RPI, NI = WR / RPI;     // rows, instructions a wave
+    static_assert(BK % WR == 0, "whole waves");
     int off[NI], ld, width, row;
     const char* base;
     // rows of layout l; row0: the sequence's first (one matrix)
     __device__ __forceinline__ void init(const SArgs& a, const Seq& s, const __bf16* x, int kvh, const PtcgHeadLayout& l,
                                          long row0, int tid) {
         const int lane = tid & 63;
-        row = __builtin_amdgcn_readfirstlane(tid >> 6) * WR;
+        row = __builtin_amdgcn_readfirstlane(tid >> 6) * WR;      // BK and up: nothing to bring
         ld = (int)l.sl * 2;
         width = 2 * a.dh;
         base = reinterpret_cast<const char*>(x + (PAGED ? 0 : row0) + (long)kvh * l.sh);
@@ -527,6 +527,7 @@ template <int DH, int BK, int NW, bool PAGED> struct KvDma {
     // ent: the page that the wave's rows lie in
     __device__ __forceinline__ void fetch(const SArgs& a, const PtcgHeadLayout& l, int block, int kend, int ent,
                                           __bf16* to) const {
+        if (BK < WR * NW && row >= BK) return;
         const int key = block * BK + row;
         int n = max(0, min(kend - key, WR));
         const char* p = base;
@@ -546,8 +547,9 @@ template <int DH, int BK, int NW, bool PAGED> struct KvDma {
 
 template <typename T, int DH, int NW, bool DMA> struct TileCfg {
     static constexpr int NTH = 64 * NW, BQ = 32 * NW, BK = 64;
+    static constexpr int RING = 2;       // DMA: tiles of keys and values in LDS
     static constexpr int TILE = tile_elems<T, DH, false, BK>();
-    static constexpr size_t PAIR = (DMA ? 2 : 1) * 4 * (size_t)TILE;   // bytes; DMA: two buffers
+    static constexpr size_t PAIR = (DMA ? RING : 1) * 4 * (size_t)TILE;   // bytes
     static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);
     static constexpr size_t BUFS = PAIR > OUT ? PAIR : OUT;
     static constexpr size_t LDS = BUFS + BK * sizeof(float) + 64;
@@ -624,8 +626,8 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
         float* __restrict__ part, const Plan pl) {
     typedef TileCfg<T, DH, NW, DMA> C;
-    typedef KvRegs<T, DH, false, C::BK, C::NTH, PAGED> Kv;
-    constexpr int PS = Kv::St::PS, BK = C::BK, BQ = C::BQ;
+    typedef KvRegs<T, DH, false, 64, C::NTH, PAGED> Kv;
+    constexpr int BK = C::BK, BQ = C::BQ, PS = BK * Lds<DH, false>::ST;
     extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     float* kf = reinterpret_cast<float*>(smem + C::BUFS);
@@ -680,19 +682,10 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     };
     if constexpr (DMA) {
         static_assert(sizeof(T) == 2 && BK == 64, "");
-        // A tile's scores are made while the last one's exponentials are taken and its
-        // values summed, so that matrix and vector instructions run side by side within a
-        // wave: keys come a tile before values.
-        KvDma<DH, BK, NW, PAGED> kk, kv;
+        typedef KvDma<DH, BK, NW, PAGED> Dma;
+        Dma kk, kv;
         kk.init(a, s, k, kvh, a.k, s.k, tid);
         kv.init(a, s, v, kvh, a.v, s.v, tid);
-        __bf16 *kbuf = tiles, *vbuf = tiles + 2 * C::TILE;
-        auto fetch_k = [&](int t, int ent) {
-            kk.fetch(a, a.k, rg.block(t), rg.kend, ent, kbuf + (t - t0 & 1) * C::TILE);
-        };
-        auto fetch_v = [&](int t, int ent) {
-            kv.fetch(a, a.v, rg.block(t), rg.kend, ent, vbuf + (t - t0 & 1) * C::TILE);
-        };
         // the page of the wave's rows of tile t: 64 tiles' on the lanes, looked up at once (a
         // scalar load a tile would make every LDS read behind it wait for it)
         int ents = 0, ents0 = t0 - 64;
@@ -700,87 +693,63 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
             if constexpr (PAGED) {
                 if (t - ents0 >= 64) {
                     ents0 = t;
-                    const int key = rg.block(t + lane) * BK + kk.row;
-                    ents = t + lane < t1 && key < rg.kend ? s.table[page_of(a, key)] : -1;
+                    const int key = rg.block(t + lane) * BK + min(kk.row, BK - 1);
+                    ents = entry_of(a, s, t + lane < t1 ? key : rg.kend, rg.kend);
                 }
                 return __builtin_amdgcn_readlane(ents, t - ents0);
             }
             return 0;
         };
-        int e1 = 0;      // that of the tile whose values come next
+        auto fetch = [&](int t, __bf16* to) {
+            const int e = entry(t);
+            kk.fetch(a, a.k, rg.block(t), rg.kend, e, to);
+            kv.fetch(a, a.v, rg.block(t), rg.kend, e, to + C::TILE);
+        };
         auto lacks = [&](int t) {       // a lane per key
             const int key = rg.block(t) * BK + lane;
             return key < rg.kend && (unsigned)s.table[page_of(a, key)] >= (unsigned)a.pages;
         };
-        bool some = false;         // any key of no page: only then tiles look for them
-        auto cover = [&](int t, floatx16 (&sc)[2]) {
-            const int key0 = rg.block(t) * BK;
-            if (!sees || dead || key0 + BK > rg.kend || some_hidden(a, key0, BK, wlo, whi)) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) hide(a, sc[j], key0 + 32 * j + 4 * h, p, last);
-            }
-            if (PAGED && some) {
-                const unsigned long long nopage = __ballot(lacks(t));
-                if (nopage) {
-                    hide_bits(sc[0], (unsigned)nopage, h);
-                    hide_bits(sc[1], (unsigned)(nopage >> 32), h);
-                }
-            }
-        };
-        constexpr int ES = 16 / (DH / 8) , EV = 16 / (DH / 16);     // elements in a product's shadow
         if (t0 < t1) {
-            const int e0 = entry(t0);
-            e1 = entry(t0 + 1 < t1 ? t0 + 1 : t0);
-            fetch_k(t0, e0);
-            if (t0 + 1 < t1) fetch_k(t0 + 1, e1);
-            fetch_v(t0, e0);
+            fetch(t0, tiles);
+            bool some = false;         // any key of no page: only then tiles look for them
             if constexpr (PAGED) {
                 for (int t = t0 + wave; t < t1; t += NW) some |= lacks(t);
                 some = __syncthreads_or(some);
             }
-            floatx16 sa[2], sb[2];
-            arrived();
-            __syncthreads();
-            scores<DH>(kbuf, qf, sa, lane, [](int) {});
-            cover(t0, sa);
-            f.raise(f.top(sa), a.scale2);
-            if (t0 + 2 < t1) __syncthreads();     // keys of the first tile are done with
-            // scores of tile t + 1 from its keys (of the last tile's successor from what lies
-            // there, for nothing), exponentials and values of tile t, whose place in the
-            // buffers is `at`
-            auto turn = [&](int t, auto at, floatx16 (&now)[2], floatx16 (&next)[2]) {
-                if (t > t0) {
-                    arrived();
-                    __syncthreads();   // everyone's pieces are here; keys of tile t and values of t - 1 are done with
+            constexpr int E = 16 / (DH / 16);       // elements in a product's shadow
+            // tile t, at `at` of the two places
+            auto turn = [&](int t, auto at) {
+                constexpr int AT = decltype(at)::value;
+                arrived();
+                __syncthreads();       // everyone's pieces of tile t are here, and tile t - 1 is done with
+                if (t + 1 < t1) fetch(t + 1, tiles + (1 - AT) * 2 * C::TILE);
+                const int key0 = rg.block(t) * BK;
+                if (!sees || all_hidden(a, key0, BK, wlo, whi)) return;
+                const __bf16 *Ks = tiles + AT * 2 * C::TILE, *Vs = Ks + C::TILE;
+                floatx16 sc[2];
+                scores<DH>(Ks, qf, sc, lane);
+                if (dead || key0 + BK > rg.kend || some_hidden(a, key0, BK, wlo, whi)) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) hide(a, sc[j], key0 + 32 * j + 4 * h, p, last);
                 }
-                if (t + 1 < t1) fetch_v(t + 1, e1);
-                if (t + 2 < t1) {
-                    e1 = entry(t + 2);
-                    fetch_k(t + 2, e1);
+                if (PAGED && some) {
+                    const unsigned long long nopage = __ballot(lacks(t));
+                    if (nopage) {
+                        hide_bits(sc[0], (unsigned)nopage, h);
+                        hide_bits(sc[1], (unsigned)(nopage >> 32), h);
+                    }
                 }
-                const __bf16* Vs = vbuf + at * C::TILE;
+                f.raise(f.top(sc), a.scale2);
                 const float ms = f.m2 == -INFINITY ? 0.f : f.m2;
                 bf16x8 pa[2], pb[2];
-                pin();
-                scores<DH>(kbuf + (1 - at) * C::TILE, qf, next, lane,
-                           [&](int i) { f.exps_of(now[0], pa, a.scale2, ms, i * ES, ES); });
-                asm volatile("" : "+v"(pa[0]), "+v"(pa[1]), "+v"(f.l));     // made here, not past the branch
-                if (t + 1 < t1) cover(t + 1, next);
-                pin();
-                values<DH>(Vs, pa, f.o, lane, [&](int i) { f.exps_of(now[1], pb, a.scale2, ms, i * EV, EV); });
-                float mt = -INFINITY;
-                values<DH>(Vs + 32 * Lds<DH, false>::ST, pb, f.o, lane, [&](int i) {
-#pragma unroll
-                    for (int e = i * EV; e < (i + 1) * EV; ++e) {
-                        mt = fmaxf(mt, next[0][e]);
-                        mt = fmaxf(mt, next[1][e]);
-                    }
-                });
-                if (t + 1 < t1) f.raise(mt, a.scale2);
+                f.exps_of(sc[0], pa, a.scale2, ms, 0, 16);
+                // the second half's exponentials in the shadow of the first half's products
+                values<DH>(Vs, pa, f.o, lane, [&](int i) { f.exps_of(sc[1], pb, a.scale2, ms, i * E, E); });
+                values<DH>(Vs + 32 * Lds<DH, false>::ST, pb, f.o, lane, [](int) {});
             };
             for (int t = t0; t < t1; t += 2) {
-                turn(t, std::integral_constant<int, 0>(), sa, sb);
-                if (t + 1 < t1) turn(t + 1, std::integral_constant<int, 1>(), sb, sa);
+                turn(t, std::integral_constant<int, 0>());
+                if (t + 1 < t1) turn(t + 1, std::integral_constant<int, 1>());
             }
         }
         __syncthreads();           // the buffers become the rows' way out
@@ -1575,12 +1544,13 @@ Form form_of(const SArgs& a, int64_t packed_rows, int64_t keys, bool bf16, bool 
     f.token = rows <= 32;
     f.waves = f.token ? (keys > 128 ? 4 : 1) : rows <= 64 ? 2 : 4;
     f.bq = f.token ? 32 : 32 * f.waves;
-    f.bk = f.token ? 32 : 64;
     f.dma = bf16;
     if (a.page) {
         auto fits = [&](const PtcgHeadLayout& l) { return l.sl < (1 << 22) && (l.sl == 0 || l.sl >= a.dh || a.page == 1); };
-        f.dma = f.dma && a.page % (f.bk / f.waves) == 0 && fits(a.k) && fits(a.v);
+        const int rows = f.waves == 2 ? 32 : 16;      // a wave's of 64 keys
+        f.dma = f.dma && a.page % rows == 0 && fits(a.k) && fits(a.v);
     }
+    f.bk = f.token ? 32 : 64;
     const int qtiles = pt_cdiv(rows, f.bq);
     int64_t tiles = (int64_t)a.n * qtiles;
     if (a.q_off) {       // no more than the rows there are make

@@ -95,7 +95,7 @@ __device__ __forceinline__ Places places_of(const SArgs& a, const Seq& s, int r0
 // tile of a sequence; where the tile is shared with other workgroups, the place of this
 // piece among the parts, its tile's number among all and, with the tile's first piece,
 // the shared ones' count.
-struct Work { int i, qt, t0, t1, part, tile; long next; };
+struct Work { int i, qt, t0, t1, part, tile, per, next; };
 
 // Splitting.  Row tiles, each as long as its sequence's longest (K_i key blocks of T_i
 // tiles), are laid end to end and cut into `slots` stretches of `per` blocks, one for
@@ -105,87 +105,122 @@ struct Work { int i, qt, t0, t1, part, tile; long next; };
 // of its stretches for the joining kernel: the stretch's first part, or its second
 // where the tile begins within the stretch.  The lengths are on the device
 // alone: every wave counts for itself, 64 sequences at a time.
-struct Cut { long all; int per, tiles; };
-template <bool PAGED, int BQ, int BK> struct Deal {
-    static __device__ __forceinline__ void shape(const SArgs& a, int i, int& t, int& k) {
-        t = k = 0;
-        if (i >= a.n) return;
-        const Seq s = seq_of<PAGED>(a, i);
-        t = (s.rows * a.G + BQ - 1) / BQ;
-        const Places p = {s.p0, s.p0 + s.ql - 1};
-        // the blocks of all rows, and of a tile of rows in a window; a tile that sees nothing is one too
-        k = range_of<BK>(a, p.lo, p.hi, s.kl).nt;
-        if (a.window < INT_MAX - 4 * BQ)
-            k = min(k, (a.window + (BQ + a.G - 2) / a.G) / BK + 2 + (min(a.sinks, s.kl) + BK - 1) / BK);
-        k = max(k, 1);
-    }
-    static __device__ __forceinline__ Cut cut(const SArgs& a, int slots, int least) {
-        const int lane = threadIdx.x & 63;
-        long all = 0;
-        int tiles = 0, t, k;
-        for (int i0 = 0; i0 < a.n; i0 += 64) {
-            shape(a, i0 + lane, t, k);
-            all += (long)t * k;
-            tiles += t;
+// (Counts of blocks fit 32 bits: the host splits nothing else.)
+struct Cut { int all, per, tiles; };
+
+// inclusive sum over the lanes, in the vector unit alone (by way of LDS the planning took 2 us
+// of a token's call)
+__device__ __forceinline__ int lane_sum(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);      // 1, 2, 4, 8 lanes up in rows of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // lane 15 to row 1, 47 to row 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // lane 31 to rows 2 and 3
+    return x;
+}
+
+template <bool PAGED, int BQ, int BK, bool ALIGNED> struct Deal {
+    int t, k, to, tt;      // of 64 sequences on the lanes: tiles, blocks; pieces and tiles up to and with it
+    int per;               // blocks a stretch, or a piece at most; 0: a piece is a tile
+    // pieces of a tile, or blocks where tiles are laid end to end
+    __device__ __forceinline__ int units() const { return per == 0 ? 1 : ALIGNED ? (k + per - 1) / per : k; }
+    __device__ __forceinline__ void load(const SArgs& a, int i0) {
+        const int i = i0 + (threadIdx.x & 63);
+        t = 0;
+        k = 1;
+        if (i < a.n) {
+            const Seq s = seq_of<PAGED>(a, i);
+            t = (s.rows * a.G + BQ - 1) / BQ;
+            const Places p = {s.p0, s.p0 + s.ql - 1};
+            // the blocks of all rows, and of a tile of rows in a window; a tile that sees nothing is one too
+            k = range_of<BK>(a, p.lo, p.hi, s.kl).nt;
+            if (a.window < INT_MAX - 4 * BQ)
+                k = min(k, (a.window + (BQ + a.G - 2) / a.G) / BK + 2 + (min(a.sinks, s.kl) + BK - 1) / BK);
+            k = max(k, 1);
         }
-        for (int o = 1; o < 64; o <<= 1) {
-            all += __shfl_xor(all, o, 64);
-            tiles += __shfl_xor(tiles, o, 64);
-        }
-        return {all, max(least, (int)((all + slots - 1) / slots)), tiles};
     }
-    // the work from block b on, up to block end; per: of the cut (0: b counts tiles, nothing is shared)
-    static __device__ __forceinline__ Work at(const SArgs& a, long b, long end, int per) {
-        const int lane = threadIdx.x & 63;
-        long before = 0;
-        int tiles = 0, t, k;
+    __device__ __forceinline__ void place() {
+        to = lane_sum(t * units());
+        tt = lane_sum(t);
+    }
+    // up to 64 sequences stay on the lanes
+    __device__ __forceinline__ Cut cut(const SArgs& a, int slots, int least) {
+        int all = 0, tiles = 0;
         for (int i0 = 0; i0 < a.n; i0 += 64) {
-            shape(a, i0 + lane, t, k);
-            if (per == 0) k = 1;
-            const long c = (long)t * k;
-            long to = c;
-            int tt = t;
-            for (int o = 1; o < 64; o <<= 1) {
-                const long x = __shfl_up(to, o, 64);
-                const int y = __shfl_up(tt, o, 64);
-                if (lane >= o) {
-                    to += x;
-                    tt += y;
+            load(a, i0);
+            all += __builtin_amdgcn_readlane(lane_sum(t * k), 63);
+            tiles += __builtin_amdgcn_readlane(lane_sum(t), 63);
+        }
+        if constexpr (ALIGNED) {
+            // sum t ceil(k / per) <= slots for certain from here on (slots > tiles); fewer by search
+            per = max(1, (int)((long)all / max(1, slots - tiles)) + 1);
+            if (a.n <= 64) {
+                int lo = max(1, all / slots);
+                while (per - lo > 1 + lo / 16) {
+                    const int mid = lo + (per - lo) / 2;
+                    if (__builtin_amdgcn_readlane(lane_sum(t * ((k + mid - 1) / mid)), 63) <= slots) per = mid;
+                    else lo = mid;
                 }
             }
-            to += before;
-            const unsigned long long m = __ballot(b >= to - c && b < to);
+            per = max(per, least);
+            all = slots;
+        } else {
+            per = max(least, (int)(((long)all + slots - 1) / slots));
+        }
+        if (a.n <= 64) place();
+        return {all, per, tiles};
+    }
+    // the work from b on, up to end
+    __device__ __forceinline__ Work at(const SArgs& a, int b, int end) {
+        int before = 0, tiles = 0;
+        for (int i0 = 0; i0 < a.n; i0 += 64) {
+            if (per == 0 || a.n > 64) {
+                load(a, i0);
+                place();
+            }
+            const int hi = before + to;
+            const unsigned long long m = __ballot(b >= hi - t * units() && b < hi);
             if (m) {
                 const int w = __builtin_ctzll(m);
-                const int kw = __builtin_amdgcn_readlane(k, w), nt = __builtin_amdgcn_readlane(t, w);
-                const long off = b - __shfl(to - c, w, 64);
-                const int q = (int)(off / kw);
+                const int uw = __builtin_amdgcn_readlane(units(), w), nt = __builtin_amdgcn_readlane(t, w);
+                const int kw = __builtin_amdgcn_readlane(k, w);
+                const int off = b - (__builtin_amdgcn_readlane(hi, w) - nt * uw), q = off / uw, u = off - q * uw;
                 Work r;
                 r.i = i0 + w;
                 r.qt = nt - 1 - q;                          // the last tile first: its rows see the most
                 r.tile = tiles + __builtin_amdgcn_readlane(tt, w) - nt + q;
-                r.t0 = (int)(off - (long)q * kw);
-                r.t1 = per == 0 ? INT_MAX : (int)(kw - r.t0 < end - b ? kw : r.t0 + (end - b));
-                r.next = b + (r.t1 - r.t0);
-                const long first = b - r.t0;                 // the tile's first block
                 r.part = -1;
-                if (per > 0 && first / per != (first + kw - 1) / per)
-                    r.part = (int)(b / per) * 2 + (b % per != 0);
+                r.per = per;
+                r.next = end;
+                if (per == 0) {
+                    r.t0 = 0;
+                    r.t1 = INT_MAX;
+                } else if constexpr (ALIGNED) {
+                    r.per = (kw + uw - 1) / uw;
+                    r.t0 = u * r.per;
+                    r.t1 = r.t0 + r.per;
+                    if (uw > 1) r.part = 2 * b;
+                } else {
+                    r.t0 = u;
+                    r.t1 = min(kw, u + (end - b));
+                    r.next = b + (r.t1 - u);
+                    const int first = b - u;                 // the tile's first block
+                    if (first / per != (first + kw - 1) / per) r.part = b / per * 2 + (b % per != 0);
+                }
                 return r;
             }
-            before = __shfl(to, 63, 64);
+            before += __builtin_amdgcn_readlane(to, 63);
             tiles += __builtin_amdgcn_readlane(tt, 63);
         }
-        return {-1, 0, 0, 0, -1, 0, end};
+        return {-1, 0, 0, 0, -1, 0, 0, end};
     }
 };
 // the same in scalar registers, as it is one for all lanes
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long uniform(long x) {
-    return (long)(unsigned)uniform((int)x) | (long)uniform((int)(x >> 32)) << 32;
-}
 __device__ __forceinline__ Work uniform(const Work& w) {
-    return {uniform(w.i), uniform(w.qt), uniform(w.t0), uniform(w.t1), uniform(w.part), uniform(w.tile), uniform(w.next)};
+    return {uniform(w.i), uniform(w.qt), uniform(w.t0), uniform(w.t1), uniform(w.part), uniform(w.tile), uniform(w.per),
+            uniform(w.next)};
 }
 __device__ __forceinline__ Cut uniform(const Cut& c) { return {uniform(c.all), uniform(c.per), uniform(c.tiles)}; }
 // What the joining kernel is told: a tile's sequence, number in it, first part and how many
@@ -224,11 +259,11 @@ __device__ __forceinline__ bool all_hidden(const SArgs& a, int k0, int nk, int l
 __device__ __forceinline__ int page_of(const SArgs& a, int key) {
     return a.page == 1 ? key : (int)(__umulhi((unsigned)key, a.pmagic) >> a.pshift);      // exact below 2^31
 }
-// (kend > 0: the table's first entry is read for keys that are not there; without
-// branches, as regions of some lanes in loops that fill the registers cost more)
+// (kend > 0.  For keys that are not there the last one's entry is read; no branches, here
+// and around loads: regions of some lanes in loops that fill the registers cost more, and
+// the compiler has lost registers at their ends.)
 __device__ __forceinline__ int entry_of(const SArgs& a, const Seq& s, int key, int kend) {
-    const int e = s.table[key < kend ? page_of(a, key) : 0];
-    return key < kend ? e : -1;
+    return s.table[page_of(a, min(key, kend - 1))];
 }
 // p where ok, else an address that can be read
 template <typename T> __device__ __forceinline__ const T* where(bool ok, const T* p, const T* other) {
@@ -441,7 +476,7 @@ template <typename T, int DH, bool PAD, int BK, int NTH, bool PAGED> struct KvRe
         if constexpr (PAGED) {
 #pragma unroll
             for (int i = 0; i < St::NCH; ++i) ent[i] = entry_of(a, s, block * BK + tid / St::CPR + i * St::RPP, kend);
-            entf = tid < BK ? entry_of(a, s, block * BK + tid, kend) : 0;
+            entf = entry_of(a, s, block * BK + tid, kend);
         }
     }
     // q: an address that can be read
@@ -454,12 +489,12 @@ template <typename T, int DH, bool PAD, int BK, int NTH, bool PAGED> struct KvRe
         } else {
             const int col = tid % St::CPR * 8;
             ok = 0;
-            kfr = tid < BK && block * BK + tid < kend && (unsigned)entf >= (unsigned)a.pages ? -INFINITY : 0.f;
+            kfr = ((tid < BK) & (block * BK + tid < kend) & ((unsigned)entf >= (unsigned)a.pages)) ? -INFINITY : 0.f;
 #pragma unroll
             for (int i = 0; i < St::NCH; ++i) {
                 const int key = block * BK + tid / St::CPR + i * St::RPP;
                 // what is not there: any address that can be read, dropped in store
-                const bool there = key < kend && col < a.dh && (unsigned)ent[i] < (unsigned)a.pages;
+                const bool there = (key < kend) & (col < a.dh) & ((unsigned)ent[i] < (unsigned)a.pages);
                 const int off = key - page_of(a, key) * a.page;
                 ok |= there ? 1u << i : 0u;
                 k.r[i].load(where(there, kp + (long)ent[i] * a.k.sn + (long)off * a.k.sl + (long)kvh * a.k.sh + col, q));
@@ -578,16 +613,16 @@ __device__ __forceinline__ Share share_of(int b, int pairs, int per) {
 struct Plan { int slots, tiles, qtiles, least, prow; bool even, split; };
 
 // A workgroup's work, one call of f after the other; js: what the joining kernel is told.
-template <bool PAGED, int BQ, int BK, class F>
+template <bool PAGED, int BQ, int BK, bool ALIGNED, class F>
 __device__ __forceinline__ void work_through(const SArgs& a, const Plan& pl, Joint* js, F f) {
-    typedef Deal<PAGED, BQ, BK> D;
+    Deal<PAGED, BQ, BK, ALIGNED> d;
+    d.per = 0;
     Work w;
-    int kvh, per = 0;
-    long b = 0, end = 1;
+    int kvh, b = 0, end = 1;
     if (pl.even) {
         const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.qtiles);
         kvh = sh.pair % a.KV;
-        w = {sh.pair / a.KV, pl.qtiles - 1 - sh.piece, 0, INT_MAX, -1, 0, 1};
+        w = {sh.pair / a.KV, pl.qtiles - 1 - sh.piece, 0, INT_MAX, -1, 0, 0, 1};
     } else if (!pl.split) {
         kvh = blockIdx.x % a.KV;             // unequal tiles are spread over the XCDs
         b = blockIdx.x / a.KV;
@@ -595,26 +630,26 @@ __device__ __forceinline__ void work_through(const SArgs& a, const Plan& pl, Joi
     } else {
         const int l = xcd_block(blockIdx.x, gridDim.x);
         kvh = l / pl.slots;
-        const Cut c = uniform(D::cut(a, pl.slots, pl.least));
+        const Cut c = uniform(d.cut(a, pl.slots, pl.least));
         if (l == 0 && threadIdx.x == 0) js[0].i = c.tiles;
-        per = c.per;
-        b = (long)(l - kvh * pl.slots) * per;
-        end = b + per < c.all ? b + per : c.all;
+        const long first = (long)(l - kvh * pl.slots) * (ALIGNED ? 1 : c.per);      // past the end: no work
+        b = first < c.all ? (int)first : c.all;
+        end = min(c.all - b, ALIGNED ? 1 : c.per) + b;
     }
     while (b < end) {
-        if (!pl.even) w = uniform(D::at(a, b, end, per));
+        if (!pl.even) w = uniform(d.at(a, b, end));
         if (w.i < 0) break;
-        f(w, kvh, per);
+        f(w, kvh);
         b = w.next;
         if (b < end) __syncthreads();        // the next one's tiles take the place of these rows' way out
     }
 }
 // whether a piece of a tile of nt key blocks leaves a part; the tile's first piece notes
 // what there is to join
-__device__ __forceinline__ bool shared_tile(Joint* js, const Work& w, int kvh, int per, int nt) {
+__device__ __forceinline__ bool shared_tile(Joint* js, const Work& w, int kvh, int nt) {
     const bool cut = w.part >= 0 && (w.t0 > 0 || nt > w.t1);
-    if (per > 0 && w.t0 == 0 && kvh == 0 && threadIdx.x == 0)
-        js[1 + w.tile] = {w.i, w.qt, w.part, cut ? 1 + (nt - w.t1 + per - 1) / per : 1};
+    if (w.per > 0 && w.t0 == 0 && kvh == 0 && threadIdx.x == 0)
+        js[1 + w.tile] = {w.i, w.qt, w.part, cut ? 1 + (nt - w.t1 + w.per - 1) / w.per : 1};
     return cut;
 }
 
@@ -633,7 +668,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     float* kf = reinterpret_cast<float*>(smem + C::BUFS);
     int* bad = reinterpret_cast<int*>(smem + C::LDS - 64);
     Joint* const js = reinterpret_cast<Joint*>(part);      // then the parts
-    work_through<PAGED, BQ, BK>(a_, pl, js, [&](const Work& w, int kvh, int per) {
+    work_through<PAGED, BQ, BK, false>(a_, pl, js, [&](const Work& w, int kvh) {
     const SArgs& a = args_again();
     const int tid = thread_again(), lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
     const Seq s = seq_of<PAGED>(a, w.i);
@@ -641,7 +676,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
     const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
     const int t0 = w.t0, t1 = min(rg.nt, w.t1);
-    const bool joined = shared_tile(js, w, kvh, per, rg.nt);
+    const bool joined = shared_tile(js, w, kvh, rg.nt);
     if (t0 > 0 && t0 >= rg.nt) return;
     if (PAGED && tid == 0) *bad = 0;
 
@@ -693,8 +728,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
             if constexpr (PAGED) {
                 if (t - ents0 >= 64) {
                     ents0 = t;
-                    const int key = rg.block(t + lane) * BK + min(kk.row, BK - 1);
-                    ents = entry_of(a, s, t + lane < t1 ? key : rg.kend, rg.kend);
+                    ents = entry_of(a, s, rg.block(min(t + lane, t1 - 1)) * BK + kk.row, rg.kend);
                 }
                 return __builtin_amdgcn_readlane(ents, t - ents0);
             }
@@ -707,7 +741,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         };
         auto lacks = [&](int t) {       // a lane per key
             const int key = rg.block(t) * BK + lane;
-            return key < rg.kend && (unsigned)s.table[page_of(a, key)] >= (unsigned)a.pages;
+            return (key < rg.kend) & ((unsigned)entry_of(a, s, key, rg.kend) >= (unsigned)a.pages);
         };
         if (t0 < t1) {
             fetch(t0, tiles);
@@ -812,7 +846,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
     constexpr int BK = C::BK, BQ = C::BQ, PS = BK * L::ST;
     extern __shared__ __align__(256) char smem[];
     Joint* const js = reinterpret_cast<Joint*>(part);      // then the parts
-    work_through<PAGED, BQ, BK>(a_, pl, js, [&](const Work& w, int kvh, int per) {
+    work_through<PAGED, BQ, BK, true>(a_, pl, js, [&](const Work& w, int kvh) {
     const SArgs& a = args_again();
     const int tid = thread_again(), lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
     __bf16* Vs = reinterpret_cast<__bf16*>(smem) + wave * C::TILE;
@@ -821,7 +855,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
     const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
     const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
     const int t0 = w.t0, t1 = min(rg.nt, w.t1);
-    const bool joined = shared_tile(js, w, kvh, per, rg.nt);
+    const bool joined = shared_tile(js, w, kvh, rg.nt);
     if (t0 > 0 && t0 >= rg.nt) return;
 
     const int r = tile0 + (lane & 31);
@@ -843,8 +877,8 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
         bool there = key < rg.kend;
         long ka, va;
         if constexpr (PAGED) {
-            nopage = there && (unsigned)ent >= (unsigned)a.pages;
-            there = there && !nopage;
+            nopage = there & ((unsigned)ent >= (unsigned)a.pages);
+            there = there & ((unsigned)ent < (unsigned)a.pages);
             const int off = key - page_of(a, key) * a.page;
             ka = (long)ent * a.k.sn + (long)off * a.k.sl;
             va = (long)ent * a.v.sn + (long)off * a.v.sl;
@@ -856,10 +890,10 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
         const T *kr = k + ka + (long)kvh * a.k.sh + 8 * h, *vr = v + va + (long)kvh * a.v.sh + 8 * h;
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c)
-            kc[c].load(where(there && 16 * c + 8 * h < a.dh, kr + 16 * c, q));
+            kc[c].load(where(there & (16 * c + 8 * h < a.dh), kr + 16 * c, q));
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c)
-            vc[c].load(where(there && 16 * c + 8 * h < a.dh, vr + 16 * c, q));
+            vc[c].load(where(there & (16 * c + 8 * h < a.dh), vr + 16 * c, q));
         here = there;
     };
     int t = t0 + wave;
@@ -876,7 +910,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c) {
             bf16x8 x[planes<T>()];
-            kc[c].keep(here && 16 * c + 8 * h < a.dh);
+            kc[c].keep(here & (16 * c + 8 * h < a.dh));
             kc[c].terms(x);
             mma(x, qf.f[c], sc[0]);
         }
@@ -884,7 +918,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
 #pragma unroll
         for (int c = 0; c < DH / 16; ++c) {
             bf16x8 x[planes<T>()];
-            vc[c].keep(here && 16 * c + 8 * h < a.dh);
+            vc[c].keep(here & (16 * c + 8 * h < a.dh));
             vc[c].terms(x);
 #pragma unroll
             for (int pn = 0; pn < planes<T>(); ++pn)
@@ -1067,7 +1101,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    work_through<false, BQ, BK>(a, pl, nullptr, [&](const Work& w, int kvh, int) {
+    work_through<false, BQ, BK, false>(a, pl, nullptr, [&](const Work& w, int kvh) {
     const Seq s = seq_of<false>(a, w.i);
     const int rows = s.rows * a.G, tile0 = w.qt * BQ;
     if (tile0 >= rows) return;
@@ -1542,7 +1576,7 @@ Form form_of(const SArgs& a, int64_t packed_rows, int64_t keys, bool bf16, bool 
     Form f;
     const int64_t rows = (int64_t)a.lq * a.G;
     f.token = rows <= 32;
-    f.waves = f.token ? (keys > 128 ? 4 : 1) : rows <= 64 ? 2 : 4;
+    f.waves = f.token ? (keys > 128 ? 4 : 1) : rows <= 64 && (bf16 || a.dh <= 64) ? 2 : 4;     // two spill in fp32 128 wide
     f.bq = f.token ? 32 : 32 * f.waves;
     f.dma = bf16;
     if (a.page) {
@@ -1558,12 +1592,16 @@ Form form_of(const SArgs& a, int64_t packed_rows, int64_t keys, bool bf16, bool 
         if (t < tiles) tiles = t;
     }
     // Where row tiles do not fill the card, stretches of keys do, one for each workgroup that
-    // runs at once.  A stretch is two blocks a wave at least, and costs a second launch.
+    // runs at once.  A stretch is four blocks at least (a token's: one a
+    // wave), and costs a second launch.
     const int64_t fill = (bf16 || a.dh <= 64 ? 2 : 1) * (int64_t)cu_count();
-    f.p.least = f.token ? 2 * f.waves : 4;
-    f.p.split = may_split && tiles * a.KV < fill && keys >= 4 * f.p.least * f.bk;
+    f.p.least = 4;
+    f.p.split = may_split && tiles * a.KV < fill && keys >= 4 * f.p.least * f.bk &&
+                (tiles + 1) * (keys / f.bk + 8) < (1LL << 30);
     f.p.tiles = (int)tiles;
     f.p.slots = (int)(f.p.split ? (fill / a.KV > 1 ? fill / a.KV : 1) : tiles);
+    // a token's pieces: at least a second one for each tile that is cut
+    if (f.p.split && f.token && f.p.slots < 2 * tiles) f.p.slots = (int)(2 * tiles);
     f.p.qtiles = qtiles;
     f.p.even = !a.q_off && !f.p.split;
     f.p.prow = (int)(rows < f.bq ? rows : f.bq);
@@ -1628,9 +1666,11 @@ int launch_form(const SArgs& a, const Form& f, const void* q, const void* k, con
         if (f.dma)
             return f.waves == 2 ? launch_tiles<T, DH, 2, PAGED, true>(a, f, q, k, v, out, lse, part, s)
                                 : launch_tiles<T, DH, 4, PAGED, true>(a, f, q, k, v, out, lse, part, s);
-    if constexpr (sizeof(T) == 4 || PAGED)
-        return f.waves == 2 ? launch_tiles<T, DH, 2, PAGED, false>(a, f, q, k, v, out, lse, part, s)
-                            : launch_tiles<T, DH, 4, PAGED, false>(a, f, q, k, v, out, lse, part, s);
+    if constexpr (sizeof(T) == 4 || PAGED) {
+        if constexpr (sizeof(T) == 2 || DH <= 64)
+            if (f.waves == 2) return launch_tiles<T, DH, 2, PAGED, false>(a, f, q, k, v, out, lse, part, s);
+        return launch_tiles<T, DH, 4, PAGED, false>(a, f, q, k, v, out, lse, part, s);
+    }
     return PTCG_OK;
 }
 template <bool PAGED>

@@ -379,7 +379,7 @@ int vector_width(const RopeArgs& a, int es, const PtcgHeadLayout* const* lays, i
 // and a group that walks several heads has their loads on their way together.
 void set_groups(RopeArgs& a, int vw, int heads) {
     a.lps = ilog2_up((a.dh + 2 * vw - 1) / (2 * vw));
-    const long want = (long)cu_count() * 1024;     // threads
+    const long want = (long)cu_count() * 4096;     // threads
     a.hgs = 0;
     while (a.lps + a.hgs < 8 && (1 << a.hgs) < heads && ((long)a.rows << (a.lps + a.hgs)) < want) ++a.hgs;
 }

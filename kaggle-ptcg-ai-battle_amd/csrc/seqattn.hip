@@ -596,15 +596,18 @@ template <typename T, int DH> constexpr int waves_simd() { return sizeof(T) == 2
 // then holds their keys, pairs are dealt out to the XCDs one by one (sequences
 // differ in length: with neighbours on one XCD a third of the CUs' time was idle), and an XCD
 // takes so many pairs at once that their long pieces come before their short ones.
+// Where pairs are few or of lengths that only the device knows (spread), a pair's pieces go
+// to all XCDs instead (8 packed sequences of 2 heads, one pair or two an XCD: dk and dv
+// 756 us against 440).
 struct Share { int pair, piece; };
-__device__ __forceinline__ Share share_of(int b, int pairs, int per) {
-    const int full = pairs >> 3, x = b & 7, idx = b >> 3;
+__device__ __forceinline__ Share share_of(int b, int pairs, int per, bool spread) {
+    const int full = spread || pairs < 32 ? 0 : pairs >> 3, x = b & 7, idx = b >> 3;
     if (idx < full * per) {
         const int most = (127 + per) / per, g = idx / (most * per), n = min(most, full - g * most), r = idx - g * most * per;
         return {(g * most + r % n) * 8 + x, r / n};
     }
-    const int rest = pairs - 8 * full, r = b - 8 * full * per;     // the last few: over all XCDs
-    return {8 * full + r % rest, r / rest};
+    const int r = b - 8 * full * per, pair = r / per;     // one after the other, over all XCDs
+    return {8 * full + pair, r - pair * per};
 }
 
 // How workgroups get their work, as the host decided: even: every sequence has qtiles row
@@ -620,7 +623,7 @@ __device__ __forceinline__ void work_through(const SArgs& a, const Plan& pl, Joi
     Work w;
     int kvh, b = 0, end = 1;
     if (pl.even) {
-        const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.qtiles);
+        const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.qtiles, false);
         kvh = sh.pair % a.KV;
         w = {sh.pair / a.KV, pl.qtiles - 1 - sh.piece, 0, INT_MAX, -1, 0, 0, 1};
     } else if (!pl.split) {
@@ -698,10 +701,19 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         const __bf16* Vs = Ks + C::TILE;
         const int key0 = rg.block(t) * BK;
         if (!sees || all_hidden(a, key0, BK, wlo, whi)) return;
+        // a half that is not seen costs no products
+        bool half[BK / 32];
         floatx16 sc[BK / 32];
 #pragma unroll
-        for (int j = 0; j < BK / 32; ++j)
-            sc[j] = mma_rows<T, DH, false, PS>(Ks + 32 * j * Lds<DH, false>::ST, qf, lane);
+        for (int j = 0; j < BK / 32; ++j) {
+            half[j] = !all_hidden(a, key0 + 32 * j, 32, wlo, whi);
+            if (half[j]) {
+                sc[j] = mma_rows<T, DH, false, PS>(Ks + 32 * j * Lds<DH, false>::ST, qf, lane);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[j][e] = -INFINITY;
+            }
+        }
         if (dead || key0 + BK > rg.kend || some_hidden(a, key0, BK, wlo, whi)) {
 #pragma unroll
             for (int j = 0; j < BK / 32; ++j) hide(a, sc[j], key0 + 32 * j + 4 * h, p, last);
@@ -713,7 +725,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
         f.step(sc, a.scale2);
 #pragma unroll
         for (int j = 0; j < BK / 32; ++j)
-            mma_tr<T, DH, false, PS>(Vs + 32 * j * Lds<DH, false>::ST, sc[j], f.o, lane);
+            if (half[j]) mma_tr<T, DH, false, PS>(Vs + 32 * j * Lds<DH, false>::ST, sc[j], f.o, lane);
     };
     if constexpr (DMA) {
         static_assert(sizeof(T) == 2 && BK == 64, "");
@@ -1051,11 +1063,11 @@ template <typename T> struct Grads {
 };
 
 // Both products of 32 LDS rows that a tile begins with (bf16): s0 = X0 Y0^T, s1 = X1
-// Y1^T, Y1 a lane's rows in registers or (YLDS) in LDS.
-template <int DH, bool YLDS>
+// Y1^T, Y1 a lane's rows in registers or (YLDS) in LDS; side(c) goes into step c's shadow.
+template <int DH, bool YLDS, class Side>
 __device__ __forceinline__ void products(const __bf16* x0, const __bf16* x1, const Row<__bf16, DH>& y0,
                                          const Row<__bf16, DH>& y1, const __bf16* yl, floatx16& s0, floatx16& s1,
-                                         int lane) {
+                                         int lane, Side side) {
     typedef Lds<DH, false> L;
     constexpr int N = DH / 16, AHEAD = 2;
     bf16x8 a0[N], a1[N], b1[N];
@@ -1075,6 +1087,7 @@ __device__ __forceinline__ void products(const __bf16* x0, const __bf16* x1, con
         s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0[c], y0.f[c][0], s0, 0, 0, 0);
         s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1[c], YLDS ? b1[c] : y1.f[c][0], s1, 0, 0, 0);
         if (c + AHEAD < N) read(c + AHEAD);
+        side(c);
         pin();
     }
 }
@@ -1092,7 +1105,7 @@ template <typename T, int DH, int NW> struct DqCfg {
     static constexpr size_t LDS = PAIR > OUT ? PAIR : OUT;
 };
 template <typename T, int DH, int NW>
-__global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(const SArgs a, const Grads<T> g,
+__global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(const SArgs a_, const Grads<T> g,
                                                                                const Plan pl) {
     typedef DqCfg<T, DH, NW> C;
     typedef KvRegs<T, DH, C::PAD, C::BK, C::NTH, false> Kv;
@@ -1100,8 +1113,9 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     constexpr int PS = Kv::St::PS, BK = C::BK, BQ = C::BQ;
     extern __shared__ __align__(256) char smem[];
     __bf16* tiles = reinterpret_cast<__bf16*>(smem);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    work_through<false, BQ, BK, false>(a, pl, nullptr, [&](const Work& w, int kvh) {
+    work_through<false, BQ, BK, false>(a_, pl, nullptr, [&](const Work& w, int kvh) {
+    const SArgs& a = args_again();
+    const int tid = thread_again(), lane = tid & 63, wave = uniform(tid >> 6), h = lane >> 5;
     const Seq s = seq_of<false>(a, w.i);
     const int rows = s.rows * a.G, tile0 = w.qt * BQ;
     if (tile0 >= rows) return;
@@ -1149,13 +1163,15 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     df.settle();
     auto tile = [&](int t, const __bf16* Ks) {
         const __bf16* Vs = Ks + C::TILE;
+        // half a tile at a time: with both halves' dS on their way the kernel spills 128 wide
+        // (251 us against 204 over 4 x 4 096)
 #pragma unroll 1
         for (int j = 0; j < BK / 32; ++j) {
             const int key0 = rg.block(t) * BK + 32 * j;
             if (!sees || key0 >= rg.kend || all_hidden(a, key0, 32, wlo, whi)) continue;
             floatx16 sc, dp;
             if constexpr (C::DMA) {
-                products<DH, false>(Ks + 32 * j * L::ST, Vs + 32 * j * L::ST, qf, df, nullptr, sc, dp, lane);
+                products<DH, false>(Ks + 32 * j * L::ST, Vs + 32 * j * L::ST, qf, df, nullptr, sc, dp, lane, [](int) {});
             } else {
                 sc = mma_rows<T, DH, C::PAD, PS>(Ks + 32 * j * L::ST, qf, lane);
                 dp = mma_rows<T, DH, C::PAD, PS>(Vs + 32 * j * L::ST, df, lane);
@@ -1314,7 +1330,7 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
     float* stats = reinterpret_cast<float*>(smem + C::BUFS + C::VROWS);   // log-sum-exp and D of the rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     // a (sequence, kv head)'s pieces: far chunks of its first key tiles, then near rows of all
-    const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.ktiles + pl.first * pl.chunks);
+    const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.ktiles + pl.first * pl.chunks, a.q_off != nullptr);
     const int u = sh.pair, i = u / a.KV, kvh = u - i * a.KV, x = sh.piece - pl.first * pl.chunks;
     const bool isfar = x < 0;
     const int kt = isfar ? sh.piece / pl.chunks : x, ch = isfar ? sh.piece % pl.chunks : 0;
@@ -1364,7 +1380,7 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
             if (kw >= s.kl || all_hidden(a, kw, 32, plo, phi)) continue;
             floatx16 p, d;
             if constexpr (DMA) {
-                products<DH, C::VLDS>(Qs + qr * L::ST, Ds + qr * L::ST, kfr, vfr, Vl, p, d, lane);
+                products<DH, C::VLDS>(Qs + qr * L::ST, Ds + qr * L::ST, kfr, vfr, Vl, p, d, lane, [](int) {});
             } else {
                 p = mma_rows<T, DH, C::PAD, St::PS>(Qs + qr * L::ST, kfr, lane);
                 if constexpr (C::VLDS) d = mma_rows_lds<DH, C::PAD>(Ds + qr * L::ST, Vl, lane);
@@ -1378,21 +1394,34 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
                     p[e] = see ? p[e] : -INFINITY;
                 }
             }
+            // a key that is not there goes along: its columns are cleared at the end
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float* x4 = ls + 2 * (qr + 8 * e + 4 * h);
                 const float4 x0 = *reinterpret_cast<const float4*>(x4), x1 = *reinterpret_cast<const float4*>(x4 + 4);
-                const float lv[4] = {x0.x, x0.z, x1.x, x1.z}, dv4[4] = {x0.y, x0.w, x1.y, x1.w};
+                const float lv[4] = {x0.x, x0.z, x1.x, x1.z}, dv[4] = {x0.y, x0.w, x1.y, x1.w};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    // a key that is not there goes along: its columns are cleared at the end
-                    const float pe = __builtin_amdgcn_exp2f(fmaf(p[4 * e + c], a.scale2, -lv[c]));
-                    p[4 * e + c] = pe;
-                    d[4 * e + c] = pe * (d[4 * e + c] - dv4[c]);
+                    p[4 * e + c] = __builtin_amdgcn_exp2f(fmaf(p[4 * e + c], a.scale2, -lv[c]));
+                    d[4 * e + c] -= dv[c];
                 }
             }
-            mma_tr<T, DH, C::PAD, St::PS>(Ds + qr * L::ST, p, gv, lane);
-            mma_tr<T, DH, C::PAD, St::PS>(Qs + qr * L::ST, d, gk, lane);
+            if constexpr (DMA) {
+                constexpr int E = 16 / (DH / 16);       // elements in a product's shadow
+                bf16x8 pb[2], db[2];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) pb[e / 8][e % 8] = (__bf16)p[e];
+                values<DH>(Ds + qr * L::ST, pb, gv, lane, [&](int c) {
+#pragma unroll
+                    for (int e = c * E; e < (c + 1) * E; ++e) db[e / 8][e % 8] = (__bf16)(p[e] * d[e]);
+                });
+                values<DH>(Qs + qr * L::ST, db, gk, lane, [](int) {});
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) d[e] *= p[e];
+                mma_tr<T, DH, C::PAD, St::PS>(Ds + qr * L::ST, p, gv, lane);
+                mma_tr<T, DH, C::PAD, St::PS>(Qs + qr * L::ST, d, gk, lane);
+            }
         }
     };
     if constexpr (DMA) {
@@ -1701,7 +1730,9 @@ BwdPlan bwd_plan(const PtcgWindowAttn* d, const SArgs& a) {
     p.q.qtiles = pt_cdiv(rows, 32 * p.nw);
     p.q.tiles = p.q.slots = a.n * p.q.qtiles;
     p.q.even = !a.q_off;
-    p.nk = a.lq <= 64 && (d->bf16 || a.dh <= 64) ? 2 : 4;
+    // short fp32 sequences, more of them than run at once: two waves wait for less (512 x 97, 4 heads,
+    // 64 wide: 87 us against 97; of row tiles the same costs 8 to 30% more)
+    p.nk = (a.lq <= 64 || (!d->bf16 && a.lq <= 128 && a.n * a.KV > 2 * cu_count())) && (d->bf16 || a.dh <= 64) ? 2 : 4;
     const int bkey = 32 * p.nk;
     p.k.ktiles = pt_cdiv(a.lq, bkey);
     // Far rows are cut where one tile's would take longer than two key tiles' near ones, in

@@ -139,9 +139,23 @@ __device__ __forceinline__ void turn(float (&x)[2 * VW], const float (&c)[VW], c
     }
 }
 
+// sum over a group of 2^lps lanes; up to 16 of them within the vector unit
+template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
+    return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float group_sum(float v, int lps) {
-    for (int o = 1; o < 1 << lps; o <<= 1) v += __shfl_xor(v, o, 64);
+    if (lps > 0) v = dpp_add<0xb1>(v);      // neighbours
+    if (lps > 1) v = dpp_add<0x4e>(v);      // pairs of a quad
+    if (lps > 2) v = dpp_add<0x141>(v);     // the other quad of 8, mirrored: its lanes are alike by now
+    if (lps > 3) v = dpp_add<0x140>(v);     // the other 8 of 16
+    for (int o = 16; o < 1 << lps; o <<= 1) v += __shfl_xor(v, o, 64);
     return v;
+}
+// 1 / sqrt(v) to an ulp, of values whose root the instruction flushes too
+__device__ __forceinline__ float rsqrt_of(float v) {
+    const bool tiny = v < 1.1754944e-38f;
+    const float r = __builtin_amdgcn_rsqf(tiny ? v * 0x1p64f : v);
+    return tiny ? r * 0x1p32f : r;
 }
 
 // Which sample a row of packed matrices belongs to: the last whose first row is
@@ -235,7 +249,7 @@ __global__ __launch_bounds__(NTH) void rope_fwd_kernel(const RopeArgs a, const T
                     float ss = 0.f;
 #pragma unroll
                     for (int e = 0; e < 2 * VW; ++e) ss = fmaf(y[e], y[e], ss);
-                    const float r = 1.f / sqrtf(group_sum(ss, a.lps) * a.inv_dh + a.eps);
+                    const float r = rsqrt_of(group_sum(ss, a.lps) * a.inv_dh + a.eps);
 #pragma unroll
                     for (int e = 0; e < 2 * VW; ++e) y[e] *= r * (isq ? wq[e] : wk[e]);
                 }
@@ -306,7 +320,7 @@ __global__ __launch_bounds__(NTH) void rope_bwd_kernel(const RopeArgs a, const T
                     }
                     ss = group_sum(ss, a.lps);
                     sd = group_sum(sd, a.lps);
-                    const float r = 1.f / sqrtf(ss * a.inv_dh + a.eps), m = r * r * (sd * a.inv_dh);
+                    const float r = rsqrt_of(ss * a.inv_dh + a.eps), m = r * r * (sd * a.inv_dh);
 #pragma unroll
                     for (int e = 0; e < 2 * VW; ++e) {
                         const float gw = y[e] * (xv[e] * r);
@@ -342,9 +356,9 @@ __global__ __launch_bounds__(NTH) void rope_bwd_kernel(const RopeArgs a, const T
 // dw from the workgroups' parts: 16 columns a workgroup, 64 threads down a column
 __global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__ part, int nblk, int dh,
                                                        float* __restrict__ dwq, float* __restrict__ dwk) {
-    __shared__ float sh[64][17];
+    __shared__ double sh[64][17];
     const int c = threadIdx.x & 15, r = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
-    float t = 0.f;
+    double t = 0;       // the parts' sums are long and of both signs
     if (col < 2 * dh)
 #pragma unroll 4
         for (int b = r; b < nblk; b += 64) t += part[(long)b * 2 * dh + col];
@@ -353,7 +367,7 @@ __global__ __launch_bounds__(1024) void rope_dw_kernel(const float* __restrict__
     if (r > 0 || col >= 2 * dh) return;
     for (int x = 1; x < 64; ++x) t += sh[x][c];
     float* out = col < dh ? dwq : dwk;
-    if (out) out[col < dh ? col : col - dh] = t;
+    if (out) out[col < dh ? col : col - dh] = (float)t;
 }
 
 // ------------------------------------------------------------------- host
@@ -377,9 +391,9 @@ int vector_width(const RopeArgs& a, int es, const PtcgHeadLayout* const* lays, i
 
 // Groups a row: as few as fill the card, since each makes the row's angles anew
 // and a group that walks several heads has their loads on their way together.
-void set_groups(RopeArgs& a, int vw, int heads) {
+void set_groups(RopeArgs& a, int vw, int heads, int per_cu) {
     a.lps = ilog2_up((a.dh + 2 * vw - 1) / (2 * vw));
-    const long want = (long)cu_count() * 4096;     // threads
+    const long want = (long)cu_count() * per_cu;     // threads
     a.hgs = 0;
     while (a.lps + a.hgs < 8 && (1 << a.hgs) < heads && ((long)a.rows << (a.lps + a.hgs)) < want) ++a.hgs;
 }
@@ -521,7 +535,7 @@ extern "C" int ptcg_kernel_qk_norm_rope_fwd(const PtcgQkRope* d, const void* q, 
     const PtcgHeadLayout* lays[] = {&a.q, &a.k, &a.qo, &a.ko};
     const void* ptrs[] = {q, k, qo, ko};
     const int vw = vector_width(a, es, lays, 4, ptrs, 4);
-    set_groups(a, vw, a.H + a.KV);
+    set_groups(a, vw, a.H + a.KV, 1024);
     const hipStream_t s = (hipStream_t)stream;
     return d->bf16 ? rope_vw<__bf16, false>(a, vw, d->rope.interleaved, q, k, nullptr, qo, ko, s)
                    : rope_vw<float, false>(a, vw, d->rope.interleaved, q, k, nullptr, qo, ko, s);
@@ -559,7 +573,7 @@ extern "C" int ptcg_kernel_qk_norm_rope_bwd(const PtcgQkRope* d, const void* q, 
         const PtcgHeadLayout* lays[] = {&a.q, &a.k, &a.qo, &a.ko};
         const void* ptrs[] = {q, k, dqo, dko, dq, dk};
         const int vw = vector_width(a, es, lays, 4, ptrs, 6);
-        set_groups(a, vw, a.H + a.KV);
+        set_groups(a, vw, a.H + a.KV, 4096);
         const long full = pt_cdiv((long)a.rows << (a.lps + a.hgs), NTH);
         const int nblk = (int)(full < bwd_blocks(d) ? full : bwd_blocks(d));
         float* part = dw ? static_cast<float*>(workspace) : nullptr;
@@ -616,7 +630,7 @@ extern "C" int ptcg_kernel_paged_append(const PtcgPagedAppend* d, const void* q,
     const PtcgHeadLayout* lays[] = {&a.q, &a.k, &a.v, &a.qo, &a.pg.k, &a.pg.v};
     const void* ptrs[] = {q, k, v, qo, a.pg.kp, a.pg.vp};
     const int vw = vector_width(a, es, lays, 6, ptrs, 6);
-    set_groups(a, vw, a.H + 2 * a.KV);
+    set_groups(a, vw, a.H + 2 * a.KV, 1024);
     const hipStream_t s = (hipStream_t)stream;
     return d->bf16 ? rope_vw<__bf16, true>(a, vw, d->rope.interleaved, q, k, v, qo, nullptr, s)
                    : rope_vw<float, true>(a, vw, d->rope.interleaved, q, k, v, qo, nullptr, s);

@@ -21,6 +21,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace {
 
 constexpr int NTH = 256;
@@ -199,66 +201,53 @@ __global__ __launch_bounds__(NTH) void rope_fwd_kernel(const RopeArgs a, const T
     if (a.pos) p = a.pos[row];
     const bool packed = CACHE && a.q_off;
     auto at = [&](const PtcgHeadLayout& l) { return packed ? row * l.sl : i * l.sn + j * l.sl; };
-    // heads of q, then of k, then of v
-    const int HK = a.H + a.KV, HT = CACHE ? (page >= 0 ? HK + a.KV : a.H) : HK;
-    const long qi = at(a.q), ki = at(a.k), qj = at(a.qo);
-    const long vi = CACHE ? at(a.v) : 0;
-    const long kj = CACHE ? page * a.pg.k.sn + pr * a.pg.k.sl : at(a.ko), vj = page * a.pg.v.sn + pr * a.pg.v.sl;
-    const long ksh = CACHE ? a.pg.k.sh : a.ko.sh;
-    T* const kd = CACHE ? static_cast<T*>(a.pg.kp) : ko;
-    T* const vd = static_cast<T*>(a.pg.vp);
-    auto from = [&](int h) -> const T* {
-        if (h < a.H) return q + qi + h * a.q.sh;
-        if (!CACHE || h < HK) return k + ki + (h - a.H) * a.k.sh;
-        return v + vi + (h - HK) * a.v.sh;
-    };
-    auto to = [&](int h) -> T* {
-        if (h < a.H) return qo + qj + h * a.qo.sh;
-        if (!CACHE || h < HK) return kd + kj + (h - a.H) * ksh;
-        return vd + vj + (h - HK) * a.pg.v.sh;
-    };
-
-    float c[VW], s[VW], wq[2 * VW], wk[2 * VW];
+    const long kj = CACHE ? page * a.pg.k.sn + pr * a.pg.k.sl : at(a.ko);
+    float c[VW], s[VW];
     angles<VW, INTER>(a, u, p, c, s);
+    // The heads of q, of k, and (copied) of v, groups of the row in turn from head h0 on.
+    const int HG = 1 << a.hgs;
+    auto heads = [&](const T* src, long ssh, T* dst, long dsh, int n, int h0, const float* w, auto turns) {
+        float wv[2 * VW];
 #pragma unroll
-    for (int e = 0; e < VW; ++e) {
-        wq[e] = u.live && a.wq ? a.wq[u.oa + e] : 1.f;
-        wq[VW + e] = u.live && a.wq ? a.wq[u.ob + e] : 1.f;
-        wk[e] = u.live && a.wk ? a.wk[u.oa + e] : 1.f;
-        wk[VW + e] = u.live && a.wk ? a.wk[u.ob + e] : 1.f;
-    }
-    for (int h0 = hg; h0 < HT; h0 += U << a.hgs) {
-        Pairs<T, VW> x[U];
+        for (int e = 0; e < 2 * VW; ++e)
+            wv[e] = decltype(turns)::value && u.live && w ? w[e < VW ? u.oa + e : u.ob + e - VW] : 1.f;
+        for (int h = h0; h < n; h += U << a.hgs) {
+            Pairs<T, VW> x[U];
 #pragma unroll
-        for (int t = 0; t < U; ++t) {
-            const int h = h0 + (t << a.hgs);
-            if (!u.live || h >= HT) continue;
-            x[t].load(from(h), u.oa, u.ob);
-        }
+            for (int t = 0; t < U; ++t)
+                if (u.live && h + (t << a.hgs) < n) x[t].load(src + (h + (t << a.hgs)) * ssh, u.oa, u.ob);
 #pragma unroll
-        for (int t = 0; t < U; ++t) {
-            const int h = h0 + (t << a.hgs);
-            if (h >= HT) break;
-            if (!CACHE || h < HK) {
-                float y[2 * VW];
+            for (int t = 0; t < U; ++t) {
+                if (h + (t << a.hgs) >= n) break;
+                if constexpr (decltype(turns)::value) {
+                    float y[2 * VW];
 #pragma unroll
-                for (int e = 0; e < 2 * VW; ++e) y[e] = 0.f;
-                if (u.live) x[t].get(y);
-                const bool isq = h < a.H;
-                if (isq ? a.wq : a.wk) {
-                    float ss = 0.f;
+                    for (int e = 0; e < 2 * VW; ++e) y[e] = 0.f;
+                    if (u.live) x[t].get(y);
+                    if (w) {
+                        float ss = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 2 * VW; ++e) ss = fmaf(y[e], y[e], ss);
-                    const float r = rsqrt_of(group_sum(ss, a.lps) * a.inv_dh + a.eps);
+                        for (int e = 0; e < 2 * VW; ++e) ss = fmaf(y[e], y[e], ss);
+                        const float r = rsqrt_of(group_sum(ss, a.lps) * a.inv_dh + a.eps);
 #pragma unroll
-                    for (int e = 0; e < 2 * VW; ++e) y[e] *= r * (isq ? wq[e] : wk[e]);
+                        for (int e = 0; e < 2 * VW; ++e) y[e] *= r * wv[e];
+                    }
+                    turn<VW, INTER>(y, c, s, u.turns, 1.f);
+                    x[t].set(y);
                 }
-                turn<VW, INTER>(y, c, s, u.turns, 1.f);
-                x[t].set(y);
+                if (u.live) x[t].store(dst + (h + (t << a.hgs)) * dsh, u.oa, u.ob);
             }
-            if (u.live) x[t].store(to(h), u.oa, u.ob);
         }
-    }
+    };
+    auto from = [&](int before) { return (hg - before) & (HG - 1); };
+    heads(q + at(a.q), a.q.sh, qo + at(a.qo), a.qo.sh, a.H, hg, a.wq, std::true_type());
+    if (!CACHE || page >= 0)
+        heads(k + at(a.k), a.k.sh, (CACHE ? static_cast<T*>(a.pg.kp) : ko) + kj, CACHE ? a.pg.k.sh : a.ko.sh, a.KV,
+              from(a.H), a.wk, std::true_type());
+    if constexpr (CACHE)
+        if (page >= 0)
+            heads(v + at(a.v), a.v.sh, static_cast<T*>(a.pg.vp) + page * a.pg.v.sn + pr * a.pg.v.sl, a.pg.v.sh, a.KV,
+                  from(a.H + a.KV), nullptr, std::false_type());
 }
 
 // Backward.  Workgroups walk the rows with a stride, so that a thread's part of
@@ -272,67 +261,62 @@ __global__ __launch_bounds__(NTH) void rope_bwd_kernel(const RopeArgs a, const T
     __shared__ float acc[NTH * 4 * VW];
     const int tid = threadIdx.x, g = tid >> a.lps, hg = g & ((1 << a.hgs) - 1), lane = tid & ((1 << a.lps) - 1);
     const Unit<VW, INTER> u(lane, a.dh, a.rot);
-    const int per = NTH >> (a.lps + a.hgs), HT = a.H + a.KV;
-    float gq[2 * VW], gk[2 * VW], wq[2 * VW], wk[2 * VW];
+    const int per = NTH >> (a.lps + a.hgs), HG = 1 << a.hgs;
+    float gq[2 * VW], gk[2 * VW];
 #pragma unroll
-    for (int e = 0; e < 2 * VW; ++e) {
-        gq[e] = gk[e] = 0.f;
-        const int at = e < VW ? u.oa + e : u.ob + e - VW;
-        wq[e] = u.live && a.wq ? a.wq[at] : 1.f;
-        wk[e] = u.live && a.wk ? a.wk[at] : 1.f;
-    }
+    for (int e = 0; e < 2 * VW; ++e) gq[e] = gk[e] = 0.f;
     for (int row = blockIdx.x * per + (g >> a.hgs); row < a.rows; row += gridDim.x * per) {
         const int i = row / a.l, j = row - i * a.l, p = a.pos ? a.pos[row] : j;
         float c[VW], s[VW];
         angles<VW, INTER>(a, u, p, c, s);
         auto at = [&](const PtcgHeadLayout& l) { return i * l.sn + j * l.sl; };
-        const long qa = at(a.q), ka = at(a.k), qoa = at(a.qo), koa = at(a.ko);
-        for (int h0 = hg; h0 < HT; h0 += U << a.hgs) {
-            Pairs<T, VW> x[U], d[U];
+        auto heads = [&](const T* xs, T* dx, long xsh, const T* dy, long ysh, int n, int h0, const float* w,
+                         float (&gw)[2 * VW]) {
+            float wv[2 * VW];
 #pragma unroll
-            for (int t = 0; t < U; ++t) {
-                const int h = h0 + (t << a.hgs);
-                if (!u.live || h >= HT) continue;
-                const bool isq = h < a.H;
-                d[t].load(isq ? dqo + qoa + h * a.qo.sh : dko + koa + (h - a.H) * a.ko.sh, u.oa, u.ob);
-                if (isq ? a.wq : a.wk) x[t].load(isq ? q + qa + h * a.q.sh : k + ka + (h - a.H) * a.k.sh, u.oa, u.ob);
-            }
+            for (int e = 0; e < 2 * VW; ++e) wv[e] = u.live && w ? w[e < VW ? u.oa + e : u.ob + e - VW] : 1.f;
+            for (int h = h0; h < n; h += U << a.hgs) {
+                Pairs<T, VW> x[U], d[U];
 #pragma unroll
-            for (int t = 0; t < U; ++t) {
-                const int h = h0 + (t << a.hgs);
-                if (h >= HT) break;
-                const bool isq = h < a.H;
-                float y[2 * VW];
-#pragma unroll
-                for (int e = 0; e < 2 * VW; ++e) y[e] = 0.f;
-                if (u.live) d[t].get(y);
-                turn<VW, INTER>(y, c, s, u.turns, -1.f);
-                if (isq ? a.wq : a.wk) {
-                    float xv[2 * VW], ss = 0.f, sd = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 2 * VW; ++e) xv[e] = 0.f;
-                    if (u.live) x[t].get(xv);
-#pragma unroll
-                    for (int e = 0; e < 2 * VW; ++e) {
-                        const float w = isq ? wq[e] : wk[e];
-                        ss = fmaf(xv[e], xv[e], ss);
-                        sd = fmaf(y[e] * w, xv[e], sd);
-                    }
-                    ss = group_sum(ss, a.lps);
-                    sd = group_sum(sd, a.lps);
-                    const float r = rsqrt_of(ss * a.inv_dh + a.eps), m = r * r * (sd * a.inv_dh);
-#pragma unroll
-                    for (int e = 0; e < 2 * VW; ++e) {
-                        const float gw = y[e] * (xv[e] * r);
-                        if (isq) gq[e] += gw;
-                        else gk[e] += gw;
-                        y[e] = r * (y[e] * (isq ? wq[e] : wk[e]) - xv[e] * m);
-                    }
+                for (int t = 0; t < U; ++t) {
+                    if (!u.live || h + (t << a.hgs) >= n) continue;
+                    d[t].load(dy + (h + (t << a.hgs)) * ysh, u.oa, u.ob);
+                    if (w) x[t].load(xs + (h + (t << a.hgs)) * xsh, u.oa, u.ob);
                 }
-                d[t].set(y);
-                if (u.live) d[t].store(isq ? dq + qa + h * a.q.sh : dk + ka + (h - a.H) * a.k.sh, u.oa, u.ob);
+#pragma unroll
+                for (int t = 0; t < U; ++t) {
+                    if (h + (t << a.hgs) >= n) break;
+                    float y[2 * VW];
+#pragma unroll
+                    for (int e = 0; e < 2 * VW; ++e) y[e] = 0.f;
+                    if (u.live) d[t].get(y);
+                    turn<VW, INTER>(y, c, s, u.turns, -1.f);
+                    if (w) {
+                        float xv[2 * VW], ss = 0.f, sd = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 2 * VW; ++e) xv[e] = 0.f;
+                        if (u.live) x[t].get(xv);
+#pragma unroll
+                        for (int e = 0; e < 2 * VW; ++e) {
+                            ss = fmaf(xv[e], xv[e], ss);
+                            sd = fmaf(y[e] * wv[e], xv[e], sd);
+                        }
+                        ss = group_sum(ss, a.lps);
+                        sd = group_sum(sd, a.lps);
+                        const float r = rsqrt_of(ss * a.inv_dh + a.eps), m = r * r * (sd * a.inv_dh);
+#pragma unroll
+                        for (int e = 0; e < 2 * VW; ++e) {
+                            gw[e] += y[e] * (xv[e] * r);
+                            y[e] = r * (y[e] * wv[e] - xv[e] * m);
+                        }
+                    }
+                    d[t].set(y);
+                    if (u.live) d[t].store(dx + (h + (t << a.hgs)) * xsh, u.oa, u.ob);
+                }
             }
-        }
+        };
+        heads(q + at(a.q), dq + at(a.q), a.q.sh, dqo + at(a.qo), a.qo.sh, a.H, hg, a.wq, gq);
+        heads(k + at(a.k), dk + at(a.k), a.k.sh, dko + at(a.ko), a.ko.sh, a.KV, (hg - a.H) & (HG - 1), a.wk, gk);
     }
     if (!part) return;
     // column e of q (then of k) over the groups

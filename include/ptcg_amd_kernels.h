@@ -419,9 +419,9 @@ int ptcg_kernel_paged_append(const PtcgPagedAppend* desc, const void* q, const v
  * head h reads kv head h / (heads / kv_heads), dh a multiple of 8 up to 128,
  * strides multiples of 16 bytes, buffers 16 B aligned.  lse (nullable) (n, heads,
  * lq) fp32.  A row that sees no key (a place below 0, no pages) gives out = 0, lse =
- * -inf.  Rows outside every sequence stay as they were.  What unseen places of
- * the pool hold reaches nothing; NaN and infinities among a call's own new keys and
- * values may reach rows of that sequence before them.
+ * -inf.  Rows outside every sequence stay as they were.  What the pool holds past a
+ * sequence's length or where it has no page reaches nothing; NaN and infinities among the
+ * values that it holds may reach those of its rows in the call that do not see them.
  * workspace of _ws_bytes (0: none, -1: refused), 16 B aligned, any contents; calls
  * that may run at the same time need scratch of their own.
  * No reference counterpart: its policy has no memory.                       */

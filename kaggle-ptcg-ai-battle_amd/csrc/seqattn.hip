@@ -47,7 +47,7 @@ template <bool PAGED> __device__ __forceinline__ Seq seq_of(const SArgs& a, int 
     Seq s = {};
     s.ql = s.rows = a.lq;
     if (a.q_off) {
-        const int r0 = a.q_off[i];
+        const int r0 = max(0, a.q_off[i]);
         s.ql = s.rows = max(0, min(a.lq, min(a.q_off[i + 1], a.all_rows) - r0));
         s.q = r0 * a.q.sl; s.o = r0 * a.o.sl;
         if constexpr (!PAGED) { s.k = r0 * a.k.sl; s.v = r0 * a.v.sl; }
@@ -254,8 +254,7 @@ __device__ __forceinline__ bool all_hidden(const SArgs& a, int k0, int nk, int l
     return k0 > hi || (lo - (k0 + nk - 1) >= a.window && k0 >= a.sinks);
 }
 
-// Byte-free address of key row `key`: element offset of its row, and whether there
-// is one.  ent: its page-table entry (paged).
+// the page of a sequence that key lies in
 __device__ __forceinline__ int page_of(const SArgs& a, int key) {
     return a.page == 1 ? key : (int)(__umulhi((unsigned)key, a.pmagic) >> a.pshift);      // exact below 2^31
 }
@@ -525,8 +524,8 @@ __device__ __forceinline__ void to_lds(intx4 rs, const __bf16* base, int off) {
     asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(rs) : "memory");
 }
-// all but the last N instructions' pieces have arrived
-template <int N = 0> __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+// this wave's pieces have arrived
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // A tile of BK key or value rows by 16-byte pieces straight into LDS (bf16): waves bring WR
 // rows each that lie in one matrix, or in one page (whose size is a multiple of
@@ -535,15 +534,15 @@ template <int N = 0> __device__ __forceinline__ void arrived() { asm volatile("s
 template <int DH, int BK, int NW, bool PAGED> struct KvDma {
     typedef Lds<DH, false> L;
     static constexpr int CPR = DH / 8, RPI = 64 / CPR;                     // rows an instruction
-    static constexpr int WR = BK / NW > RPI ? BK / NW : RPI, NI = WR / RPI;     // rows, instructions a wave
-    static_assert(BK % WR == 0, "whole waves");
+    static constexpr int WR = BK / NW, NI = WR / RPI;      // rows, instructions a wave
+    static_assert(BK % NW == 0 && WR % RPI == 0, "whole instructions");
     int off[NI], ld, width, row;
     const char* base;
     // rows of layout l; row0: the sequence's first (one matrix)
     __device__ __forceinline__ void init(const SArgs& a, const Seq& s, const __bf16* x, int kvh, const PtcgHeadLayout& l,
                                          long row0, int tid) {
         const int lane = tid & 63;
-        row = __builtin_amdgcn_readfirstlane(tid >> 6) * WR;      // BK and up: nothing to bring
+        row = __builtin_amdgcn_readfirstlane(tid >> 6) * WR;
         ld = (int)l.sl * 2;
         width = 2 * a.dh;
         base = reinterpret_cast<const char*>(x + (PAGED ? 0 : row0) + (long)kvh * l.sh);
@@ -562,7 +561,6 @@ template <int DH, int BK, int NW, bool PAGED> struct KvDma {
     // ent: the page that the wave's rows lie in
     __device__ __forceinline__ void fetch(const SArgs& a, const PtcgHeadLayout& l, int block, int kend, int ent,
                                           __bf16* to) const {
-        if (BK < WR * NW && row >= BK) return;
         const int key = block * BK + row;
         int n = max(0, min(kend - key, WR));
         const char* p = base;
@@ -582,9 +580,8 @@ template <int DH, int BK, int NW, bool PAGED> struct KvDma {
 
 template <typename T, int DH, int NW, bool DMA> struct TileCfg {
     static constexpr int NTH = 64 * NW, BQ = 32 * NW, BK = 64;
-    static constexpr int RING = 2;       // DMA: tiles of keys and values in LDS
     static constexpr int TILE = tile_elems<T, DH, false, BK>();
-    static constexpr size_t PAIR = (DMA ? RING : 1) * 4 * (size_t)TILE;   // bytes
+    static constexpr size_t PAIR = (DMA ? 2 : 1) * 4 * (size_t)TILE;   // bytes
     static constexpr size_t OUT = (size_t)NW * Out<T, DH>::WAVE * sizeof(T);
     static constexpr size_t BUFS = PAIR > OUT ? PAIR : OUT;
     static constexpr size_t LDS = BUFS + BK * sizeof(float) + 64;
@@ -598,7 +595,7 @@ template <typename T, int DH> constexpr int waves_simd() { return sizeof(T) == 2
 // takes so many pairs at once that their long pieces come before their short ones.
 // Where pairs are few or of lengths that only the device knows (spread), a pair's pieces go
 // to all XCDs instead (8 packed sequences of 2 heads, one pair or two an XCD: dk and dv
-// 756 us against 440).
+// 756 us against 570).
 struct Share { int pair, piece; };
 __device__ __forceinline__ Share share_of(int b, int pairs, int per, bool spread) {
     const int full = spread || pairs < 32 ? 0 : pairs >> 3, x = b & 7, idx = b >> 3;
@@ -634,7 +631,7 @@ __device__ __forceinline__ void work_through(const SArgs& a, const Plan& pl, Joi
         const int l = xcd_block(blockIdx.x, gridDim.x);
         kvh = l / pl.slots;
         const Cut c = uniform(d.cut(a, pl.slots, pl.least));
-        if (l == 0 && threadIdx.x == 0) js[0].i = c.tiles;
+        if (l == 0 && threadIdx.x == 0) js[0].i = c.tiles <= pl.tiles ? c.tiles : 0;     // more: q_off does not ascend
         const long first = (long)(l - kvh * pl.slots) * (ALIGNED ? 1 : c.per);      // past the end: no work
         b = first < c.all ? (int)first : c.all;
         end = min(c.all - b, ALIGNED ? 1 : c.per) + b;
@@ -649,9 +646,9 @@ __device__ __forceinline__ void work_through(const SArgs& a, const Plan& pl, Joi
 }
 // whether a piece of a tile of nt key blocks leaves a part; the tile's first piece notes
 // what there is to join
-__device__ __forceinline__ bool shared_tile(Joint* js, const Work& w, int kvh, int nt) {
+__device__ __forceinline__ bool shared_tile(Joint* js, const Work& w, int kvh, int nt, int tiles) {
     const bool cut = w.part >= 0 && (w.t0 > 0 || nt > w.t1);
-    if (w.per > 0 && w.t0 == 0 && kvh == 0 && threadIdx.x == 0)
+    if (w.per > 0 && w.t0 == 0 && w.tile < tiles && kvh == 0 && threadIdx.x == 0)
         js[1 + w.tile] = {w.i, w.qt, w.part, cut ? 1 + (nt - w.t1 + w.per - 1) / w.per : 1};
     return cut;
 }
@@ -679,7 +676,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
     const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
     const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
     const int t0 = w.t0, t1 = min(rg.nt, w.t1);
-    const bool joined = shared_tile(js, w, kvh, rg.nt);
+    const bool joined = shared_tile(js, w, kvh, rg.nt, pl.tiles);
     if (t0 > 0 && t0 >= rg.nt) return;
     if (PAGED && tid == 0) *bad = 0;
 
@@ -867,7 +864,7 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
     const Places pt = places_of(a, s, tile0, min(tile0 + BQ, rows));
     const Range rg = range_of<BK>(a, pt.lo, pt.hi, s.kl);
     const int t0 = w.t0, t1 = min(rg.nt, w.t1);
-    const bool joined = shared_tile(js, w, kvh, rg.nt);
+    const bool joined = shared_tile(js, w, kvh, rg.nt, pl.tiles);
     if (t0 > 0 && t0 >= rg.nt) return;
 
     const int r = tile0 + (lane & 31);

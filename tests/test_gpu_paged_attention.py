@@ -149,6 +149,39 @@ def test_chunks(cuda, kw):
     Op(**kw).run().check()
 
 
+@pytest.mark.parametrize("kw", [
+    # more sequences than lanes, whose tiles are cut by keys
+    dict(lens=[2000 - 13 * i for i in range(100)], new=[1 + i % 50 for i in range(100)], H=2, KV=1, dh=64, page=16),
+    dict(lens=[2000 - 13 * i for i in range(100)], new=40, H=1, KV=1, dh=32, page=64, window=900, sinks=5),
+    dict(lens=[2000 - 13 * i for i in range(100)], new=1, H=2, KV=1, dh=64, page=16),
+    # up to 64 rows, in pages of one and two waves' rows
+    dict(lens=[6000, 900, 300], new=9, H=5, KV=1, dh=128, page=32),
+    dict(lens=[6000, 900, 300], new=[9, 0, 3], H=5, KV=1, dh=64, page=64, window=700, sinks=40),
+    dict(lens=[600, 900, 300], new=33, H=1, KV=1, dh=32, page=96, order="heads"),
+    dict(lens=[600, 900, 300], new=12, H=4, KV=1, dh=48, page=8),
+], ids=str)
+@pytest.mark.parametrize("bf16", [True, False])
+def test_plans_over_lanes_and_waves(cuda, kw, bf16):
+    Op(bf16=bf16, **kw).run().check()
+
+
+@pytest.mark.parametrize("bf16", [True, False])
+def test_a_window_of_every_int(cuda, bf16):
+    for window in (2 ** 31 - 1, 2 ** 31 - 200, 2 ** 30):
+        Op(lens=[2100, 300], new=[70, 300], H=2, KV=1, dh=64, bf16=bf16, page=16, window=window, sinks=2 ** 31 - 1).run().check()
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_no_page_in_a_pool_of_nan(cuda, new):
+    """Rows that no page is left for, next to places that hold NaN: zeros and -inf."""
+    op = Op(lens=[900, 400, 77], new=new, H=4, KV=2, dh=64, bf16=True, page=32)
+    op.table[1] = -1
+    op.table[2] = op.kp.shape[0]
+    op.kp[op.table[0, -1].long(), 900 % 32:] = float("nan")
+    op.run().check()
+    assert (op.qv(op.out)[new:] == 0).all() and (op.lse[1:] == -math.inf).all()
+
+
 def test_many_sequences_of_one_chunk_size(cuda):
     Op(lens=[130 + 3 * i for i in range(90)], new=33, H=4, KV=2, dh=64, bf16=True, page=16).run().check()
     Op(lens=[130 + 3 * i for i in range(90)], new=[1 + i % 40 for i in range(90)], H=4, KV=2, dh=64, bf16=True,

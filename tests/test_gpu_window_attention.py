@@ -162,6 +162,43 @@ def test_windows_around_tiles(cuda, window):
     Op(lens=[200, 77], l=200, H=3, KV=1, dh=64, bf16=True, window=window, packed=True).fwd().bwd().check()
 
 
+@pytest.mark.parametrize("l, dh", [(33, 64), (35, 128), (65, 32), (97, 128)])
+def test_rows_so_far_apart_that_a_sequence_passes_31_bits(cuda, l, dh):
+    """The queries' rows 2^31 bytes apart in all (bf16), the outputs' beside each other, and the other way round."""
+    g = torch.Generator(device="cuda").manual_seed(l)
+    H, KV, st = 2, 1, (2 ** 31 // 2 // l // 64 + 1) * 64
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda").bfloat16()
+    near, apart = LAY(sn=0, sl=H * dh, sh=dh), LAY(sn=0, sl=st, sh=dh)
+    at = torch.arange(l, device="cuda")
+    k, v, vals, grads = rnd(l, KV, dh), rnd(l, KV, dh), rnd(l, H, dh), rnd(l, H, dh)
+    ref = attention(vals, k, v, sees(at, at, 20, 2), dh ** -0.5, grads, True)
+    wide = lambda: torch.empty(l * st, dtype=torch.bfloat16, device="cuda").as_strided((l, H, dh), (st, dh, 1))
+    dense = lambda: torch.empty(l, H, dh, dtype=torch.bfloat16, device="cuda")
+    for lq, lo in ((apart, near), (near, apart)):
+        q, dq = (wide() if lq is apart else dense() for _ in range(2))
+        out, do = (wide() if lo is apart else dense() for _ in range(2))
+        dk, dv = torch.empty_like(k), torch.empty_like(v)
+        q.copy_(vals)
+        do.copy_(grads)
+        lse = torch.empty(H, l, device="cuda")
+        lk = LAY(sn=0, sl=KV * dh, sh=dh)
+        a = native.CPtcgWindowAttn(n=1, l=l, heads=H, kv_heads=KV, dh=dh, bf16=1, scale=dh ** -0.5, window=20, sinks=2,
+                                   q=lq, k=lk, v=lk, o=lo)
+        lib = native.lib()
+        nb = max(lib.ptcg_kernel_window_attention_ws_bytes(ctypes.byref(a), x) for x in (0, 1))
+        ws = torch.full((nb,), 0xff, dtype=torch.uint8, device="cuda")
+        native.check(lib.ptcg_kernel_window_attention_fwd(
+            ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), ws.data_ptr(), nb,
+            None))
+        native.check(lib.ptcg_kernel_window_attention_bwd(
+            ctypes.byref(a), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), do.data_ptr(),
+            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nb, None))
+        torch.cuda.synchronize()
+        for name, x in (("out", out), ("dq", dq), ("dk", dk), ("dv", dv)):
+            within(name, x, *ref[name])
+        within("lse", lse, *ref["lse"])
+
+
 def test_forward_alone_and_large_scores(cuda):
     Op(lens=[500, 130], l=500, H=4, KV=2, dh=64, bf16=True, packed=True).fwd(lse=False).check(bwd=False, lse=False)
     Op(lens=[150, 130], l=150, H=4, KV=2, dh=64, bf16=False, scale=6.0, window=40).fwd().bwd().check()

@@ -1229,20 +1229,29 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     });
 }
 
-// How dK / dV's work is cut.  Key tiles of 32 NK keys; where a window has first tokens,
-// the tiles that hold these (`first` of them) are seen by every later row: the rows
-// past the window's reach (far rows) are cut into `chunks` of `chunk` flattened rows for
-// workgroups of their own, whose parts seq_first_kernel adds up.
-struct DkvPlan { int ktiles, first, chunks, chunk; };
+// How dK / dV's work is cut.  Key tiles of 32 NK keys; the rows that see one are cut into
+// pieces where the tiles alone do not fill the card (`nears` pieces of `near` rows), and
+// where a window has first tokens the rows past its reach (far rows), which
+// see none but the tiles that hold these (`first` of them), are `chunks` more
+// pieces of `chunk` rows.  A tile in pieces leaves a part of each, `nears` of every tile
+// that is cut (`cut` of them, from the first on), then the far ones; seq_sum_kernel adds
+// them up in that order.
+struct DkvPlan {
+    int ktiles, first, chunks, chunk, nears, near, cut;
+    __host__ __device__ __forceinline__ int pieces() const { return ktiles * nears + first * chunks; }
+    __host__ __device__ __forceinline__ int parts() const { return cut * nears + first * chunks; }
+};
 
-// rows that see the key tile from key0: near ones up to `far`, far ones from there on
+// rows that see the key tile from key0: near ones up to `far`, far ones from there on (where
+// these are cut off: else all are near)
 struct Rows { int lo, far, hi; };
-__device__ __forceinline__ Rows rows_of(const SArgs& a, const Seq& s, int key0, int nk) {
+__device__ __forceinline__ Rows rows_of(const SArgs& a, const Seq& s, int key0, int nk, bool off) {
     Rows r;
     r.lo = min(key0, s.ql) * a.G;
     const int reach = a.window > s.ql - key0 - nk ? s.ql : min(s.ql, key0 + nk - 1 + a.window);
     r.far = reach * a.G;
     r.hi = key0 < a.sinks ? s.ql * a.G : r.far;
+    if (!off) r.far = r.hi;
     return r;
 }
 
@@ -1327,23 +1336,22 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
     float* stats = reinterpret_cast<float*>(smem + C::BUFS + C::VROWS);   // log-sum-exp and D of the rows
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     // a (sequence, kv head)'s pieces: far chunks of its first key tiles, then near rows of all
-    const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.ktiles + pl.first * pl.chunks, a.q_off != nullptr);
-    const int u = sh.pair, i = u / a.KV, kvh = u - i * a.KV, x = sh.piece - pl.first * pl.chunks;
+    const int fars = pl.first * pl.chunks;
+    const Share sh = share_of(blockIdx.x, a.n * a.KV, pl.pieces(), a.q_off != nullptr);
+    const int u = sh.pair, i = u / a.KV, kvh = u - i * a.KV, x = sh.piece - fars;
     const bool isfar = x < 0;
-    const int kt = isfar ? sh.piece / pl.chunks : x, ch = isfar ? sh.piece % pl.chunks : 0;
+    const int kt = isfar ? sh.piece / pl.chunks : x / pl.nears, ch = isfar ? sh.piece % pl.chunks : x % pl.nears;
     const Seq s = seq_of<false>(a, i);
     const int kall = s.rows;          // a padded sequence's dead rows get zeros
     if (kt * C::BKEY >= kall) return;
     const int key0 = kt * C::BKEY, kw = key0 + 32 * __builtin_amdgcn_readfirstlane(wave), key = kw + (lane & 31);
     const bool kin = key < kall, kok = key < s.kl;
-    const Rows rr = rows_of(a, s, key0, C::BKEY);
-    const bool cut = kt < pl.first && pl.chunks > 0;
-    int r0 = rr.lo, rows = cut ? rr.far : rr.hi;
-    if (isfar) {
-        r0 = rr.far + ch * pl.chunk;
-        rows = ch + 1 == pl.chunks ? rr.hi : min(rr.hi, r0 + pl.chunk);
-        if (r0 >= rows) return;
-    }
+    const Rows rr = rows_of(a, s, key0, C::BKEY, kt < pl.first);
+    // this piece's rows; a tile's first piece is there even without rows
+    const int r0 = isfar ? rr.far + ch * pl.chunk : rr.lo + ch * pl.near, end = isfar ? rr.hi : rr.far;
+    int rows = isfar ? (ch + 1 == pl.chunks ? end : min(end, r0 + pl.chunk))
+                     : (ch + 1 == pl.nears ? end : min(end, r0 + pl.near));
+    if (r0 >= rows && (isfar || ch > 0)) return;
     if (key0 >= s.kl) rows = r0;
 
     Row<T, DH> kfr, vfr;
@@ -1473,9 +1481,9 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
 #pragma unroll
             for (int e = 0; e < 16; ++e) gk[dt][e] = gv[dt][e] = 0.f;
     }
-    if (cut) {     // part of the sums over a first tile's rows
-        float* p = g.part + ((((long)u * pl.first + kt) * (pl.chunks + 1) + (isfar ? 1 + ch : 0)) * C::BKEY +
-                             32 * wave + (lane & 31)) * 2 * a.dh;
+    if (kt < pl.cut) {
+        const int at = isfar ? pl.cut * pl.nears + kt * pl.chunks + ch : kt * pl.nears + ch;
+        float* p = g.part + (((long)u * pl.parts() + at) * C::BKEY + 32 * wave + (lane & 31)) * 2 * a.dh;
         if (kin) {
             store_row<float, DH>(p, gk, 1.f, a.dh, h);
             store_row<float, DH>(p + a.dh, gv, 1.f, a.dh, h);
@@ -1487,11 +1495,11 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
     Out<T, DH>::key_rows(g.dv + s.v + (long)kvh * a.v.sh, a.v.sl, kw, kall, a.dh, gv, 1.f, ws, lane);
 }
 
-// the parts of the first tiles' dk and dv, in chunk order: 4 columns a thread
+// the parts of the cut tiles' dk and dv, in order of their rows: 4 columns a thread
 template <typename T>
-__global__ __launch_bounds__(256) void seq_first_kernel(const SArgs a, const float* __restrict__ part,
+__global__ __launch_bounds__(256) void seq_sum_kernel(const SArgs a, const float* __restrict__ part,
         T* __restrict__ dk, T* __restrict__ dv, const DkvPlan pl, int bkey) {
-    const int c4 = a.dh / 4, per = pl.first * bkey;       // keys a (sequence, kv head)
+    const int c4 = a.dh / 4, per = pl.cut * bkey;       // keys a (sequence, kv head)
     const long at = (long)blockIdx.x * 256 + threadIdx.x, both = at / c4;
     const int c = (int)(at - both * c4) * 4, isv = (int)(both & 1), u = (int)(both / 2 / per);
     const int key = (int)(both / 2 - (long)u * per);
@@ -1499,14 +1507,23 @@ __global__ __launch_bounds__(256) void seq_first_kernel(const SArgs a, const flo
     const int i = u / a.KV, kvh = u - i * a.KV, kt = key / bkey;
     const Seq s = seq_of<false>(a, i);
     if (key >= s.rows) return;
-    const Rows r = rows_of(a, s, kt * bkey, bkey);
+    const Rows r = rows_of(a, s, kt * bkey, bkey, kt < pl.first);
+    // the pieces that have rows
+    const bool dead = kt * bkey >= s.kl;
+    const int nn = dead || pl.nears == 1 ? 1 : max(1, min(pl.nears, (r.far - r.lo + pl.near - 1) / pl.near));
+    const int nf = dead || kt >= pl.first ? 0 : min(pl.chunks, (r.hi - r.far + pl.chunk - 1) / pl.chunk);
+    const float* p = part + (((long)u * pl.parts() * bkey + key % bkey) * 2 + isv) * a.dh + c;
+    const long one = (long)bkey * 2 * a.dh;
     float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = 0; p <= pl.chunks; ++p) {
-        if (p > 0 && (r.far + (p - 1) * pl.chunk >= r.hi || kt * bkey >= s.kl)) break;
-        const float4 x = *reinterpret_cast<const float4*>(
-            part + (((((long)u * pl.first + kt) * (pl.chunks + 1) + p) * bkey + key % bkey) * 2 + isv) * a.dh + c);
-        g.x += x.x; g.y += x.y; g.z += x.z; g.w += x.w;
-    }
+    auto add = [&](int first, int n) {
+#pragma unroll 4
+        for (int x = 0; x < n; ++x) {
+            const float4 y = *reinterpret_cast<const float4*>(p + (first + x) * one);
+            g.x += y.x; g.y += y.y; g.z += y.z; g.w += y.w;
+        }
+    };
+    add(kt * pl.nears, nn);
+    add(pl.cut * pl.nears + kt * pl.chunks, nf);
     const float f = isv ? 1.f : a.scale;
     T* o = isv ? dv + s.v + (long)key * a.v.sl + (long)kvh * a.v.sh : dk + s.k + (long)key * a.k.sl + (long)kvh * a.k.sh;
     st4(o + c, g.x * f, g.y * f, g.z * f, g.w * f);
@@ -1732,25 +1749,49 @@ BwdPlan bwd_plan(const PtcgWindowAttn* d, const SArgs& a) {
     p.nk = (a.lq <= 64 || (!d->bf16 && a.lq <= 128 && a.n * a.KV > 2 * cu_count())) && (d->bf16 || a.dh <= 64) ? 2 : 4;
     const int bkey = 32 * p.nk;
     p.k.ktiles = pt_cdiv(a.lq, bkey);
-    // Far rows are cut where one tile's would take longer than two key tiles' near ones, in
+    // Far rows are cut off where one tile's would take longer than two key tiles' near ones, in
     // at most 16 pieces; with more than two such tiles there is work for many workgroups as it is.
-    if (a.sinks > 0 && a.sinks <= 2 * bkey && a.window < a.lq) {
-        const int64_t near = ((int64_t)bkey + a.window) * a.G, far = rows - near;
-        if (far > near) {
-            p.k.first = pt_cdiv(a.sinks, bkey);
-            int64_t chunk = near > far / 16 ? near : far / 16;
-            chunk = (chunk + 63) / 64 * 64;
-            p.k.chunk = (int)chunk;
-            p.k.chunks = pt_cdiv(far, chunk);
+    const int64_t reach = ((int64_t)bkey + a.window) * a.G, far = rows - reach;
+    const bool firsts = a.sinks > 0 && a.window < a.lq;
+    if (firsts && a.sinks <= 2 * bkey && far > reach) p.k.first = pt_cdiv(a.sinks, bkey);
+    // Where key tiles are fewer than the workgroups that run at once, their near rows are
+    // cut as well, so that the pieces are about as many; of 256 rows at least, and no
+    // more parts than four times the workgroups.  (1 500 rows of 8 heads on one, 128 wide, 12 tiles: dk
+    // and dv 2 446 us uncut, 173 cut in fp32, 438 and 44 in bf16; 4 x 1 000 rows of 8 heads, 64 wide,
+    // 256 tiles: 116 and 75 in fp32, 34 and 38 in bf16, which is left whole from a tile a CU on.)
+    const int64_t span = rows < reach || (firsts && !p.k.first) ? rows : reach, pairs = (int64_t)a.n * a.KV;
+    const int64_t fill = (d->bf16 || a.dh <= 64 ? 2 : 1) * (int64_t)cu_count();
+    p.k.nears = 1;
+    p.k.near = INT_MAX;
+    if (pairs * p.k.ktiles < (d->bf16 ? cu_count() : fill)) {
+        int64_t all = 0;
+        for (int t = 0; t < p.k.ktiles; ++t) {
+            const int64_t left = rows - (int64_t)t * bkey * a.G;
+            all += left < span ? left : span;
+        }
+        int64_t near = all * pairs / fill;
+        if (near < span * pairs * p.k.ktiles / (4 * fill)) near = span * pairs * p.k.ktiles / (4 * fill);
+        if (near < 256) near = 256;
+        near = (near + 63) / 64 * 64;
+        if (near < span) {
+            p.k.near = (int)near;
+            p.k.nears = pt_cdiv(span, near);
         }
     }
+    if (p.k.first) {
+        int64_t chunk = p.k.nears > 1 ? p.k.near : reach;
+        if (chunk < far / 16) chunk = far / 16;
+        chunk = (chunk + 63) / 64 * 64;
+        p.k.chunk = (int)chunk;
+        p.k.chunks = pt_cdiv(far, chunk);
+    }
+    p.k.cut = p.k.nears > 1 ? p.k.ktiles : p.k.first;
     p.stats = ((int64_t)a.n * a.H * a.lq * 2 + 3) / 4 * 4;
     auto near31 = [&](const PtcgHeadLayout& l) {     // a kv head's rows of a sequence within 2^31 bytes
         return l.sl < (1LL << 30) && l.sh < (1LL << 30) && ((int64_t)a.lq * l.sl + (int64_t)a.G * l.sh) * 2 < 0x7fffff00LL;
     };
     p.dma = d->bf16 && near31(a.q) && near31(a.o);
-    p.part = (int64_t)a.n * a.KV * p.k.first * (p.k.chunks + 1) * bkey * 2 * a.dh;
-    if (p.k.first == 0) p.part = 0;
+    p.part = pairs * p.k.parts() * bkey * 2 * a.dh;
     return p;
 }
 
@@ -1768,11 +1809,11 @@ int launch_dkv(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t 
     auto kern = seq_dkv_kernel<T, DH, NK, DMA>;
     PT_TRY(lds_attr(kern, C::LDS));
     const int64_t pairs = (int64_t)a.n * a.KV;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(pairs * (p.k.ktiles + p.k.first * p.k.chunks))), dim3(C::NTH), C::LDS, s, a,
+    hipLaunchKernelGGL(kern, dim3((unsigned)(pairs * p.k.pieces())), dim3(C::NTH), C::LDS, s, a,
                        g, p.k);
     PT_LAUNCH_CHECK();
-    if (p.k.first) {
-        hipLaunchKernelGGL(seq_first_kernel<T>, dim3(pt_cdiv(pairs * p.k.first * C::BKEY * 2 * (a.dh / 4), 256)), dim3(256),
+    if (p.k.cut) {
+        hipLaunchKernelGGL(seq_sum_kernel<T>, dim3(pt_cdiv(pairs * p.k.cut * C::BKEY * 2 * (a.dh / 4), 256)), dim3(256),
                            0, s, a, g.part, g.dk, g.dv, p.k, C::BKEY);
         PT_LAUNCH_CHECK();
     }

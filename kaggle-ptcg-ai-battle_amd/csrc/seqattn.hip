@@ -1092,7 +1092,10 @@ __device__ __forceinline__ void products(const __bf16* x0, const __bf16* x1, con
 // dQ: the forward's shape.  Per 32 keys S^T and dP^T = V dO^T with queries on
 // lanes, dS^T in registers, dQ^T += K^T dS^T.  Also leaves each row's log-sum-exp (in
 // units of exp2; +inf for a row that sees nothing) and D_i for the dK / dV kernel, in
-// the order of its rows.
+// the order of its rows.  D_i is do_i . o_i of the output as it was stored; in bf16 its
+// rounding is the largest error of short rows' gradients (9 keys: 3.3e-3 in relative L2, 2.4e-3
+// without it), so there D_i is summed along the keys as well, for dK / dV, and for dQ too
+// where one tile holds all keys of the rows.
 template <typename T, int DH, int NW> struct DqCfg {
     static constexpr bool DMA = sizeof(T) == 2, PAD = DH == 128 && !DMA;
     static constexpr int NTH = 64 * NW, BQ = 32 * NW, BK = 64;
@@ -1149,7 +1152,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
     const float lr = rok && qr < s.ql ? g.lse[lrow] : -INFINITY;
     const bool none = lr == -INFINITY;
     const float l2 = none ? INFINITY : lr * LOG2E;
-    if (rok && h == 0) g.stats[((long)w.i * a.KV + kvh) * a.lq * a.G + r] = make_float2(l2, D);
+    float Dx = 0.f;      // bf16: D_i again, as sum_j P_ij (do_i . v_j)
 
     floatx16 acc[DH / 32];
 #pragma unroll
@@ -1158,7 +1161,9 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
         for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
     qf.settle();
     df.settle();
-    auto tile = [&](int t, const __bf16* Ks) {
+    // sums: Dx alone
+    auto tile = [&](int t, const __bf16* Ks, auto only) {
+        constexpr bool sums = decltype(only)::value;
         const __bf16* Vs = Ks + C::TILE;
         // half a tile at a time: with both halves' dS on their way the kernel spills 128 wide
         // (251 us against 204 over 4 x 4 096)
@@ -1175,9 +1180,13 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
             }
             if (dead || key0 + 32 > rg.kend || some_hidden(a, key0, 32, wlo, whi)) hide(a, sc, key0 + 4 * h, qr, last);
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -l2)) * (dp[e] - D);
-            mma_tr<T, DH, C::PAD, PS>(Ks + 32 * j * L::ST, sc, acc, lane);
+            for (int e = 0; e < 16; ++e) {
+                sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale2, -l2));
+                if constexpr (C::DMA) Dx = fmaf(sc[e], dp[e], Dx);
+                if (sums) continue;
+                sc[e] *= dp[e] - D;
+            }
+            if (!sums) mma_tr<T, DH, C::PAD, PS>(Ks + 32 * j * L::ST, sc, acc, lane);
         }
     };
     if constexpr (C::DMA) {
@@ -1194,7 +1203,12 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
             arrived();
             __syncthreads();       // everyone's pieces of tile t are here, and tile t - 1 is done with
             if (t + 1 < rg.nt) fetch(t + 1);
-            tile(t, tiles + (t & 1) * 2 * C::TILE);
+            if (rg.nt == 1) {      // all keys are here: dq from the better D as well
+                tile(t, tiles, std::true_type());
+                D = Dx + half_swap(Dx);
+                Dx = 0.f;
+            }
+            tile(t, tiles + (t & 1) * 2 * C::TILE, std::false_type());
         }
         __syncthreads();           // the buffers become the rows' way out
     } else {
@@ -1208,7 +1222,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
             __syncthreads();
         }
         for (int t = 0; t < rg.nt; ++t) {
-            tile(t, tiles);
+            tile(t, tiles, std::false_type());
             __syncthreads();
             if (t + 1 < rg.nt) {
                 kv.store(tiles, tiles + C::TILE, nullptr, nullptr, tid);
@@ -1217,6 +1231,8 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
             }
         }
     }
+    if constexpr (C::DMA) D = Dx + half_swap(Dx);
+    if (rok && h == 0) g.stats[((long)w.i * a.KV + kvh) * a.lq * a.G + r] = make_float2(l2, D);
     if (!live) return;
     if (none) {
 #pragma unroll

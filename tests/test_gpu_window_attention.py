@@ -246,6 +246,29 @@ def test_gradients_against_differences(cuda):
             assert abs((at[0] - at[1]) / (2 * h) - float(dx[row, head, e])) <= 1e-2 * size
 
 
+@pytest.mark.parametrize("l", [3, 9, 18, 64, 200])
+def test_bf16_gradients_are_off_by_two_roundings(cuda, l):
+    """A rounding to bf16 is off by at most 2^-8 / m of a value of mantissa m in [1, 2), evenly: 2^-8 / sqrt(3) sqrt(mean
+    1 / m^2) = 1.66e-3 in relative L2, with m logarithmically spread (mean 1 / m^2 = 3 / (8 ln 2)).  dq and dk are
+    rounded themselves and made from one rounded factor, dS: 2.35e-3, and a tenth for chance.  (dq of keys
+    past one tile has the rounding of the output in it as well.)"""
+    n = max(4, 2000 // l)
+    op = Op(lens=[l] * n, l=l, H=2, KV=2, dh=64, bf16=True, packed=True).fwd().bwd()
+    torch.cuda.synchronize()
+    at = torch.arange(l, device="cuda")
+    got, want = {"dq": [], "dk": []}, {"dq": [], "dk": []}
+    for i in range(n):
+        x = slice(i * l, (i + 1) * l)
+        ref = attention(op.q[x], op.k[x], op.v[x], sees(at, at, 0, 0), op.scale, op.do[x], True)
+        for name in got:
+            got[name].append(getattr(op, name)[x].double())
+            want[name].append(ref[name][0].double())
+    for name in ("dq", "dk") if l <= 64 else ("dk",):
+        a, b = torch.cat(got[name]), torch.cat(want[name])
+        off = float((a - b).norm() / b.norm())
+        assert off < 1.1 * 2.35e-3, (name, off)
+
+
 def test_broadcast_keys_in_the_forward(cuda):
     """One sequence's keys for all (stride 0)."""
     op = Op(lens=[90, 90, 90], l=90, H=4, KV=2, dh=64, bf16=True, window=30, sinks=1)

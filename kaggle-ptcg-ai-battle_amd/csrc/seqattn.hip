@@ -655,7 +655,10 @@ __device__ __forceinline__ bool shared_tile(Joint* js, const Work& w, int kvh, i
 
 // A workgroup owns 32 NW rows and walks their key blocks (or its split of them).
 // DMA: tiles go straight into one of two buffers while the other is worked on, one
-// barrier a tile; else through registers into one buffer.
+// barrier a tile; else through registers into one buffer.  Bound by its products, two
+// workgroups a CU taking turns at them: 4 sequences to 2 048 new rows over 30 000 keys, 8 heads of
+// 128 on 2, bf16, 542 to 563 us (915 to 950 TFLOP/s); 4 x 4 096 rows, 8 heads of 128, 143 us (960).
+// In fp32 the operands' terms and six products a product: 512 x 97 rows, 4 heads of 64, 62 us.
 template <typename T, int DH, int NW, bool PAGED, bool DMA>
 __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel(const SArgs a_, const T* __restrict__ q,
         const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
@@ -837,7 +840,9 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel
 // Waves of a workgroup take the 32-key blocks in turn and share nothing until the
 // end.  A lane holds a key's row as an operand straight from memory; the values go
 // through the wave's own part of LDS, to be read transposed.  The next block's rows
-// are on their way into the same registers while a block is worked on.
+// are on their way into the same registers while a block is worked on.  8 tokens over up to
+// 131 072 keys, 8 heads of 128 on 2, bf16: 156 us, 4.5 TB/s; 256 over up to 8 000, 8 heads of 64: 224
+// us, 4.8 TB/s; 16 over up to 1 000, 4 heads of 64, fp32: 14.4 us, latency.
 template <typename T, int DH, int KS> struct TokenCfg {
     static constexpr int NTH = 64 * KS, BQ = 32, BK = 32;
     static constexpr int TILE = tile_elems<T, DH, false, BK>();
@@ -987,7 +992,8 @@ __global__ __launch_bounds__(64 * KS, (waves_simd<T, DH>())) void seq_token_kern
 // ---------------------------------------------------------------- joining
 // Joins the splits of a row tile: a workgroup takes some rows of a (tile, kv head);
 // groups of LG lanes (4 columns each) take a row's splits in turn, per_row groups a
-// row, and meet in LDS in group order.
+// row, and meet in LDS in group order.  4.0 to 5.5 us for tokens, 16 for a chunk of 8 192 rows
+// 128 wide in 57 MB of parts.
 constexpr int JOIN_NTH = 512;
 template <typename T, int LG, bool PAGED, int BQ>
 __global__ __launch_bounds__(JOIN_NTH) void seq_join_kernel(const SArgs a, const float* __restrict__ part,
@@ -1095,7 +1101,8 @@ __device__ __forceinline__ void products(const __bf16* x0, const __bf16* x1, con
 // the order of its rows.  D_i is do_i . o_i of the output as it was stored; in bf16 its
 // rounding is the largest error of short rows' gradients (9 keys: 3.3e-3 in relative L2, 2.4e-3
 // without it), so there D_i is summed along the keys as well, for dK / dV, and for dQ too
-// where one tile holds all keys of the rows.
+// where one tile holds all keys of the rows.  4 x 4 096 rows, 8 heads of 128, bf16: 200 us (1 030
+// TFLOP/s in three products); 512 x 97, 4 heads of 64, fp32: 81 us.
 template <typename T, int DH, int NW> struct DqCfg {
     static constexpr bool DMA = sizeof(T) == 2, PAD = DH == 128 && !DMA;
     static constexpr int NTH = 64 * NW, BQ = 32 * NW, BK = 64;
@@ -1340,6 +1347,8 @@ template <typename T, int DH> constexpr int dkv_waves() {
 // dK and dV: a workgroup owns 32 NK keys of one kv head, a wave 32 of them, and
 // walks the flattened query rows that see them.  S = Q K^T and dP = dO V^T with
 // keys on lanes; dV^T += dO^T P and dK^T += Q^T dS read dO and Q transposed from LDS.
+// 4 x 4 096 rows, 8 heads of 128, bf16: 251 to 256 us (1 070 TFLOP/s in four products); 512 x 97, 4
+// heads of 64, fp32: 87 us.
 template <typename T, int DH, int NK, bool DMA>
 __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(const SArgs a, const Grads<T> g,
                                                                                const DkvPlan pl) {
@@ -1511,7 +1520,7 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
     Out<T, DH>::key_rows(g.dv + s.v + (long)kvh * a.v.sh, a.v.sl, kw, kall, a.dh, gv, 1.f, ws, lane);
 }
 
-// the parts of the cut tiles' dk and dv, in order of their rows: 4 columns a thread
+// the parts of the cut tiles' dk and dv, in order of their rows: 4 columns a thread.  4 to 13 us
 template <typename T>
 __global__ __launch_bounds__(256) void seq_sum_kernel(const SArgs a, const float* __restrict__ part,
         T* __restrict__ dk, T* __restrict__ dv, const DkvPlan pl, int bkey) {

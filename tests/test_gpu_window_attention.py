@@ -142,6 +142,10 @@ CASES = [
     dict(lens=[2050], l=2050, H=1, KV=1, dh=64, bf16=False, window=1500, sinks=4),
     dict(lens=[20 + 3 * i for i in range(80)], l=260, H=2, KV=1, dh=32, bf16=True, window=50, sinks=2, packed=True),
     dict(lens=[5] * 300, l=5, H=4, KV=4, dh=8, bf16=False, window=2, sinks=1),
+    # few key tiles, cut along their rows; sequences without rows among them
+    dict(lens=[900, 0, 300, 1], l=900, H=8, KV=1, dh=64, bf16=True),
+    dict(lens=[900, 0, 300, 1], l=900, H=8, KV=1, dh=128, bf16=False, window=200, sinks=3),
+    dict(lens=[0, 900, 257, 64], l=900, H=8, KV=1, dh=96, bf16=True, window=90, sinks=150, packed=True, slack=2),
 ]
 
 

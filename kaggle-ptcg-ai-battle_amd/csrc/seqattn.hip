@@ -518,10 +518,13 @@ template <typename T, int DH, bool PAD, int BK, int NTH, bool PAGED> struct KvRe
 // 16 bytes a lane from memory into LDS, lane L's to base + 16 L; zeros past the
 // descriptor's end.  Issued from assembly so that the compiler does not tie LDS reads
 // to loads on their way; who reads waits (arrived) and meets the others at a barrier.
+// The load may not read a descriptor's word within five wait states of its v_readfirstlane,
+// nor M0 within one of its move, and the compiler adds none in here: the move and four more.
+#define PT_WAIT_M0 "s_nop 3\n\t"
 typedef int intx4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void to_lds(intx4 rs, const __bf16* base, int off) {
     const unsigned at = (unsigned)(uintptr_t)base;      // LDS offset: low bits of the generic address
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\t" PT_WAIT_M0 "buffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(rs) : "memory");
 }
 // this wave's pieces have arrived
@@ -1318,7 +1321,7 @@ template <int DH, int BQ, int NW> struct QDma {
         }
         if (wave < BQ / 32) {     // 32 rows' two numbers
             const unsigned at = (unsigned)(uintptr_t)(ls + wave * 64);
-            asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+            asm volatile("s_mov_b32 m0, %0\n\t" PT_WAIT_M0 "buffer_load_dword %1, %2, 0 offen lds"
                          :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"((row0 + wave * 32) * 8 + lane * 4), "s"(st)
                          : "memory");
         }

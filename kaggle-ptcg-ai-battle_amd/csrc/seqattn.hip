@@ -520,12 +520,14 @@ template <typename T, int DH, bool PAD, int BK, int NTH, bool PAGED> struct KvRe
 // to loads on their way; who reads waits (arrived) and meets the others at a barrier.
 // The load may not read a descriptor's word within five wait states of its v_readfirstlane,
 // nor M0 within one of its move, and the compiler adds none in here: the move and four more.
+// (M0 is named as written: the warning that it is a reserved register is what this file means.)
+#pragma clang diagnostic ignored "-Winline-asm"
 #define PT_WAIT_M0 "s_nop 3\n\t"
 typedef int intx4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void to_lds(intx4 rs, const __bf16* base, int off) {
     const unsigned at = (unsigned)(uintptr_t)base;      // LDS offset: low bits of the generic address
     asm volatile("s_mov_b32 m0, %0\n\t" PT_WAIT_M0 "buffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(rs) : "memory");
+                 :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"(off), "s"(rs) : "memory", "m0");
 }
 // this wave's pieces have arrived
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -1323,7 +1325,7 @@ template <int DH, int BQ, int NW> struct QDma {
             const unsigned at = (unsigned)(uintptr_t)(ls + wave * 64);
             asm volatile("s_mov_b32 m0, %0\n\t" PT_WAIT_M0 "buffer_load_dword %1, %2, 0 offen lds"
                          :: "s"(__builtin_amdgcn_readfirstlane(at)), "v"((row0 + wave * 32) * 8 + lane * 4), "s"(st)
-                         : "memory");
+                         : "memory", "m0");
         }
     }
 };

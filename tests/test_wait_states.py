@@ -153,3 +153,10 @@ def test_loads_into_lds_wait_for_what_they_read(name):
     asm = assembly(name)
     assert len(re.findall(r"offen lds$", asm, re.M)) > 100      # the search has something to look at
     assert late_waits(asm) == []
+
+
+@pytest.mark.parametrize("name", sorted(f for f in os.listdir(build.CSRC) if f.endswith((".hip", ".h"))))
+def test_assembly_that_moves_m0_says_so(name):
+    with open(os.path.join(build.CSRC, name)) as f:
+        blocks = re.findall(r"asm volatile\((.*?)\);", f.read(), re.S)
+    assert [b for b in blocks if "m0" in b.split("::")[0] and '"m0"' not in b.split(":")[-1]] == []

@@ -623,7 +623,9 @@ __device__ __forceinline__ int32x4_t buffer_rsrc(const float* p, unsigned bytes)
 }
 __device__ __forceinline__ void dma16(int32x4_t rsrc, const float* lds_base, int voffset_bytes) {
     const unsigned lds = (unsigned)(uintptr_t)lds_base;   // LDS offset (low bits of the generic address)
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+    // a load into LDS may not read M0 within one wait state of its move, and the compiler adds none
+    // in here (descriptors are made well before: tests/test_wait_states.py searches for both)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voffset_bytes), "s"(rsrc) : "memory", "m0");
 }
 template <int N> __device__ __forceinline__ void wait_vm() {

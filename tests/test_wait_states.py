@@ -7,6 +7,7 @@ instruction is one, `s_nop n` is n + 1) along every path:
     buffer descriptor's word) and a memory instruction that reads it, else it may read the
     old one: another bound than the rows have;
   - one between a write of M0 and a load into LDS, whose place M0 is."""
+import concurrent.futures as cf
 import os
 import re
 import subprocess
@@ -15,7 +16,7 @@ import pytest
 
 from ptcg_amd import build
 
-SOURCES = ["seqattn"]
+SOURCES = ["gemm", "seqattn"]
 DESCRIPTOR, PLACE = 5, 1
 
 MEMORY = re.compile(r"(buffer_|global_|flat_|scratch_)")
@@ -140,17 +141,22 @@ def test_the_search_counts_the_instructions_between():
     assert late_waits(scalar) == []
 
 
-def assembly(name):
-    src = os.path.join(build.CSRC, name + ".hip")
-    cmd = [build._hipcc(), *build.CFLAGS, "-w", "--cuda-device-only", "-S", src, "-o", "-"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    assert r.returncode == 0, r.stderr[-2000:]
-    return r.stdout
+@pytest.fixture(scope="module")
+def assembly():
+    def one(name):
+        src = os.path.join(build.CSRC, name + ".hip")
+        cmd = [build._hipcc(), *build.CFLAGS, "-w", "--cuda-device-only", "-S", src, "-o", "-"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr[-2000:]
+        return r.stdout
+
+    with cf.ThreadPoolExecutor(len(SOURCES)) as ex:
+        return dict(zip(SOURCES, ex.map(one, SOURCES)))
 
 
 @pytest.mark.parametrize("name", SOURCES)
-def test_loads_into_lds_wait_for_what_they_read(name):
-    asm = assembly(name)
+def test_loads_into_lds_wait_for_what_they_read(name, assembly):
+    asm = assembly[name]
     assert len(re.findall(r"offen lds$", asm, re.M)) > 100      # the search has something to look at
     assert late_waits(asm) == []
 

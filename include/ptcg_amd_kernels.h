@@ -347,7 +347,10 @@ int ptcg_rope_frequencies(int rot, double base, int scaling, double factor, doub
  * element (sample, row, head, e) of q lies at q[sn sample + sl row + sh head + e],
  * the same for k (kv_heads heads, 0 for none), qo, ko; any strides >= 0 of the
  * inputs.  fp32, or bf16 (bf16 = 1; sums, norms and angles fp32 or more, one
- * rounding at the end).  fwd: qo may be q and ko k, with their layouts.
+ * rounding at the end).  fwd: qo may be q and ko k, with their layouts; rows
+ * whose lanes come to 2^32 are refused (a row has the power of two from dh / (2 e)
+ * on, e the elements of an access: 16 bytes, or as widths, strides and addresses
+ * let it; one element: 64 lanes, so fewer than 2^26 rows).
  * bwd: gradients dqo, dko (laid out as qo, ko) of the outputs to dq, dk (as q,
  * k), dwq, dwk (dh floats, where there is a norm; both NULL: not made), all
  * overwritten, sums in a fixed order.  Without a norm q or k is not read (may be
@@ -395,7 +398,8 @@ typedef struct PtcgPages {
  * (device, n ints): the sequences' lengths with their new rows, so new row j of
  * m has place len - m + j; rows of places below 0 or past the table are not
  * written (their qo is).  A page that new rows lie in belongs to one sequence.
- * q, k, v and the pool of one type.  qo may be q, with its layout.
+ * q, k, v and the pool of one type.  qo may be q, with its layout.  As many rows at
+ * most as ptcg_kernel_qk_norm_rope_fwd takes.
  * No reference counterpart.                                                 */
 typedef struct PtcgPagedAppend {
     int n, lq, rows, heads, kv_heads, dh;

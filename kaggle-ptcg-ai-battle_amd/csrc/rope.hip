@@ -387,6 +387,12 @@ void set_groups(RopeArgs& a, int vw, int heads, int per_cu) {
     while (a.lps + a.hgs < 8 && (1 << a.hgs) < heads && ((long)a.rows << (a.lps + a.hgs)) < want) ++a.hgs;
 }
 
+// A launch holds fewer than 2^32 threads (the backward's grid is bounded as it is).
+int check_launch(const RopeArgs& a, const char* who) {
+    PT_REQUIRE(((int64_t)a.rows << (a.lps + a.hgs)) <= (1LL << 32) - NTH,
+               "%s: too many rows: %d of %d lanes a head", who, a.rows, 1 << a.lps);
+    return PTCG_OK;
+}
 int check_rope(const PtcgRope& r, int dh, const char* who) {
     PT_REQUIRE(r.rot >= 0 && r.rot <= dh && r.rot % 2 == 0, "%s: %d turning elements of a head of %d", who, r.rot, dh);
     PT_REQUIRE(r.interleaved == 0 || r.interleaved == 1, "%s: interleaved=%d", who, r.interleaved);
@@ -525,6 +531,7 @@ extern "C" int ptcg_kernel_qk_norm_rope_fwd(const PtcgQkRope* d, const void* q, 
     const void* ptrs[] = {q, k, qo, ko};
     const int vw = vector_width(a, es, lays, 4, ptrs, 4);
     set_groups(a, vw, a.H + a.KV, 1024);
+    PT_TRY(check_launch(a, who));
     const hipStream_t s = (hipStream_t)stream;
     return d->bf16 ? rope_vw<__bf16, false>(a, vw, d->rope.interleaved, q, k, nullptr, qo, ko, s)
                    : rope_vw<float, false>(a, vw, d->rope.interleaved, q, k, nullptr, qo, ko, s);
@@ -620,6 +627,7 @@ extern "C" int ptcg_kernel_paged_append(const PtcgPagedAppend* d, const void* q,
     const void* ptrs[] = {q, k, v, qo, a.pg.kp, a.pg.vp};
     const int vw = vector_width(a, es, lays, 6, ptrs, 6);
     set_groups(a, vw, a.H + 2 * a.KV, 1024);
+    PT_TRY(check_launch(a, who));
     const hipStream_t s = (hipStream_t)stream;
     return d->bf16 ? rope_vw<__bf16, true>(a, vw, d->rope.interleaved, q, k, v, qo, nullptr, s)
                    : rope_vw<float, true>(a, vw, d->rope.interleaved, q, k, v, qo, nullptr, s);

@@ -1525,38 +1525,42 @@ __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(
     Out<T, DH>::key_rows(g.dv + s.v + (long)kvh * a.v.sh, a.v.sl, kw, kall, a.dh, gv, 1.f, ws, lane);
 }
 
-// the parts of the cut tiles' dk and dv, in order of their rows: 4 columns a thread.  4 to 13 us
+// the parts of the cut tiles' dk and dv, in order of their rows: 4 columns a thread and turn.  4 to 13 us
+constexpr int SUM_BLOCKS = 1 << 16;      // parts may come to 2^32 threads and more: workgroups walk them
 template <typename T>
 __global__ __launch_bounds__(256) void seq_sum_kernel(const SArgs a, const float* __restrict__ part,
         T* __restrict__ dk, T* __restrict__ dv, const DkvPlan pl, int bkey) {
     const int c4 = a.dh / 4, per = pl.cut * bkey;       // keys a (sequence, kv head)
-    const long at = (long)blockIdx.x * 256 + threadIdx.x, both = at / c4;
-    const int c = (int)(at - both * c4) * 4, isv = (int)(both & 1), u = (int)(both / 2 / per);
-    const int key = (int)(both / 2 - (long)u * per);
-    if (u >= a.n * a.KV) return;
-    const int i = u / a.KV, kvh = u - i * a.KV, kt = key / bkey;
-    const Seq s = seq_of<false>(a, i);
-    if (key >= s.rows) return;
-    const Rows r = rows_of(a, s, kt * bkey, bkey, kt < pl.first);
-    // the pieces that have rows
-    const bool dead = kt * bkey >= s.kl;
-    const int nn = dead || pl.nears == 1 ? 1 : max(1, min(pl.nears, (r.far - r.lo + pl.near - 1) / pl.near));
-    const int nf = dead || kt >= pl.first ? 0 : min(pl.chunks, (r.hi - r.far + pl.chunk - 1) / pl.chunk);
-    const float* p = part + (((long)u * pl.parts() * bkey + key % bkey) * 2 + isv) * a.dh + c;
-    const long one = (long)bkey * 2 * a.dh;
-    float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](int first, int n) {
+    const long all = (long)a.n * a.KV * per * 2 * c4;
+    for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < all; at += (long)gridDim.x * 256) {
+        const long both = at / c4;
+        const int c = (int)(at - both * c4) * 4, isv = (int)(both & 1), u = (int)(both / 2 / per);
+        const int key = (int)(both / 2 - (long)u * per);
+        const int i = u / a.KV, kvh = u - i * a.KV, kt = key / bkey;
+        const Seq s = seq_of<false>(a, i);
+        if (key >= s.rows) continue;
+        const Rows r = rows_of(a, s, kt * bkey, bkey, kt < pl.first);
+        // the pieces that have rows
+        const bool dead = kt * bkey >= s.kl;
+        const int nn = dead || pl.nears == 1 ? 1 : max(1, min(pl.nears, (r.far - r.lo + pl.near - 1) / pl.near));
+        const int nf = dead || kt >= pl.first ? 0 : min(pl.chunks, (r.hi - r.far + pl.chunk - 1) / pl.chunk);
+        const float* p = part + (((long)u * pl.parts() * bkey + key % bkey) * 2 + isv) * a.dh + c;
+        const long one = (long)bkey * 2 * a.dh;
+        float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](int first, int n) {
 #pragma unroll 4
-        for (int x = 0; x < n; ++x) {
-            const float4 y = *reinterpret_cast<const float4*>(p + (first + x) * one);
-            g.x += y.x; g.y += y.y; g.z += y.z; g.w += y.w;
-        }
-    };
-    add(kt * pl.nears, nn);
-    add(pl.cut * pl.nears + kt * pl.chunks, nf);
-    const float f = isv ? 1.f : a.scale;
-    T* o = isv ? dv + s.v + (long)key * a.v.sl + (long)kvh * a.v.sh : dk + s.k + (long)key * a.k.sl + (long)kvh * a.k.sh;
-    st4(o + c, g.x * f, g.y * f, g.z * f, g.w * f);
+            for (int x = 0; x < n; ++x) {
+                const float4 y = *reinterpret_cast<const float4*>(p + (first + x) * one);
+                g.x += y.x; g.y += y.y; g.z += y.z; g.w += y.w;
+            }
+        };
+        add(kt * pl.nears, nn);
+        add(pl.cut * pl.nears + kt * pl.chunks, nf);
+        const float f = isv ? 1.f : a.scale;
+        T* o = isv ? dv + s.v + (long)key * a.v.sl + (long)kvh * a.v.sh
+                   : dk + s.k + (long)key * a.k.sl + (long)kvh * a.k.sh;
+        st4(o + c, g.x * f, g.y * f, g.z * f, g.w * f);
+    }
 }
 
 // ------------------------------------------------------------------- host
@@ -1843,8 +1847,9 @@ int launch_dkv(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t 
                        g, p.k);
     PT_LAUNCH_CHECK();
     if (p.k.cut) {
-        hipLaunchKernelGGL(seq_sum_kernel<T>, dim3(pt_cdiv(pairs * p.k.cut * C::BKEY * 2 * (a.dh / 4), 256)), dim3(256),
-                           0, s, a, g.part, g.dk, g.dv, p.k, C::BKEY);
+        const int64_t blocks = (pairs * p.k.cut * C::BKEY * 2 * (a.dh / 4) + 255) / 256;
+        hipLaunchKernelGGL(seq_sum_kernel<T>, dim3((unsigned)(blocks < SUM_BLOCKS ? blocks : SUM_BLOCKS)), dim3(256), 0, s,
+                           a, g.part, g.dk, g.dv, p.k, C::BKEY);
         PT_LAUNCH_CHECK();
     }
     return PTCG_OK;

@@ -293,3 +293,10 @@ def test_two_calls_on_streams_with_scratch_of_their_own(cuda):
         op.fwd(s.cuda_stream).bwd(s.cuda_stream)
     for op in ops:
         op.check()
+
+
+def test_many_sequences_whose_parts_pass_one_round_of_the_sum(cuda):
+    """16 800 (sequence, kv head) pairs with two cut key tiles of 128: 2^24.04 threads' worth of sums, of which a
+    launch has 2^24; the long sequences are the last ones."""
+    Op(lens=[3] * 2060 + [400, 300, 0, 150] * 10, l=400, H=8, KV=8, dh=8, bf16=True, window=1, sinks=200,
+       packed=True).fwd().bwd().check()

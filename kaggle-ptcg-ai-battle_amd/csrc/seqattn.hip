@@ -1564,8 +1564,9 @@ __global__ __launch_bounds__(256) void seq_sum_kernel(const SArgs a, const float
 }
 
 // ------------------------------------------------------------------- host
+// packed_rows: the rows that packed sequences have in all; -1: not known
 int check_common(int n, int l, int heads, int kv_heads, int dh, int bf16, float scale, int window, int sinks,
-                 const PtcgHeadLayout& q, const PtcgHeadLayout& o, const char* who) {
+                 const PtcgHeadLayout& q, const PtcgHeadLayout& o, int64_t packed_rows, const char* who) {
     PT_REQUIRE(n >= 0 && l >= 0, "%s: negative size: %d sequences of %d rows", who, n, l);
     PT_REQUIRE(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, "%s: %d heads over %d kv heads", who, heads,
                kv_heads);
@@ -1575,18 +1576,24 @@ int check_common(int n, int l, int heads, int kv_heads, int dh, int bf16, float 
     PT_REQUIRE(window >= 0 && sinks >= 0, "%s: window=%d sinks=%d", who, window, sinks);
     const int e = bf16 ? 8 : 4;
     PT_REQUIRE(layout_ok(q, e) && layout_ok(o, e), "%s: strides must be non-negative multiples of 16 bytes", who);
+    // (8 bytes of statistics a row within 2^31)
     const int64_t G = heads / kv_heads, rows = (int64_t)l * G;
-    PT_REQUIRE(l < (1 << 30) && rows * G < (1LL << 32) && rows < (1LL << 31) - 256,
+    PT_REQUIRE(l < (1 << 30) && rows * G < (1LL << 32) && rows < (1LL << 28) - 64,
                "%s: %d rows of %d heads a kv head are too long", who, l, (int)G);
-    // a launch holds fewer than 2^32 threads, 256 a tile of rows
-    PT_REQUIRE((double)n * kv_heads * (double)(rows / 32 + 2) < (double)(1 << 23) && (double)n * heads * l < 4294967296.0,
-               "%s: too many rows", who);
+    // A launch holds fewer than 2^32 threads, 256 a tile of rows at most (32 rows or more) and two tiles'
+    // for what of a sequence fills none; dk / dv's pieces, of 64 keys or more, are fewer.
+    double tiles = (double)n * (double)(rows / 32 + 2);
+    if (packed_rows >= 0) {      // no more than the rows there are make
+        const double t = (double)packed_rows * G / 32 + 2.0 * n;
+        if (t < tiles) tiles = t;
+    }
+    PT_REQUIRE(tiles * kv_heads < (double)(1 << 24), "%s: too many rows", who);
     return PTCG_OK;
 }
 int check_paged(const PtcgPagedAttn* d, const char* who) {
     PT_REQUIRE(d, "%s: null descriptor", who);
     PT_TRY(check_common(d->n, d->lq, d->heads, d->kv_heads, d->dh, d->bf16, d->scale, d->window, d->sinks, d->q, d->o,
-                        who));
+                        d->q_off ? d->rows : -1, who));
     PT_REQUIRE(!d->q_off || (d->rows >= 0 && d->rows < (1 << 30)), "%s: rows=%d", who, d->rows);
     PT_TRY(check_pages(d->cache, d->n, d->kv_heads, d->dh, d->bf16 ? 8 : 4, who));
     return PTCG_OK;
@@ -1594,7 +1601,7 @@ int check_paged(const PtcgPagedAttn* d, const char* who) {
 int check_window(const PtcgWindowAttn* d, const char* who) {
     PT_REQUIRE(d, "%s: null descriptor", who);
     PT_TRY(check_common(d->n, d->l, d->heads, d->kv_heads, d->dh, d->bf16, d->scale, d->window, d->sinks, d->q, d->o,
-                        who));
+                        -1, who));
     const int e = d->bf16 ? 8 : 4;
     PT_REQUIRE(layout_ok(d->k, e) && layout_ok(d->v, e), "%s: strides must be non-negative multiples of 16 bytes", who);
     PT_REQUIRE(!(d->off && d->len), "%s: packed sequences (off) take no len", who);

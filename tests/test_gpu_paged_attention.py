@@ -276,3 +276,14 @@ def test_a_cache_past_32_bit_offsets(cuda):
     op2.table, op2.kp, op2.vp = op.table, op.kp, op.vp
     op2.a.cache = c
     op2.run().check()
+
+
+def test_packed_rows_of_sequences_that_could_be_long(cuda):
+    """600 sequences of up to 2^17 new rows of 8 heads on one: only the rows that there are count as launched."""
+    new = [0] * 590 + [1, 40, 0, 300, 7, 0, 65, 2, 129, 33]
+    op = Op(lens=[x + 50 for x in new], new=new, H=8, KV=1, dh=64, bf16=True, page=16, slack=2)
+    op.a.lq = 1 << 17
+    nb = native.lib().ptcg_kernel_paged_attention_ws_bytes(ctypes.byref(op.a))
+    assert nb >= 0
+    op.ws = torch.full((max(16, nb),), 0xff, dtype=torch.uint8, device="cuda")
+    op.run(lse=False).check(lse=False)

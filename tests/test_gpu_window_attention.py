@@ -300,3 +300,9 @@ def test_many_sequences_whose_parts_pass_one_round_of_the_sum(cuda):
     launch has 2^24; the long sequences are the last ones."""
     Op(lens=[3] * 2060 + [400, 300, 0, 150] * 10, l=400, H=8, KV=8, dh=8, bf16=True, window=1, sinks=200,
        packed=True).fwd().bwd().check()
+
+
+def test_packed_sequences_of_as_many_rows_as_a_launch_takes(cuda):
+    """4 096 sequences that might have 8 192 rows each, 8 kv heads: over 2^31 threads of 2^32."""
+    Op(lens=[0] * 4000 + [3] * 60 + [200, 0, 97, 1] * 9, l=8192, H=8, KV=8, dh=8, bf16=True, packed=True,
+       slack=1).fwd().bwd().check()

@@ -376,13 +376,13 @@ int vector_width(const RopeArgs& a, int es, const PtcgHeadLayout* const* lays, i
     return 1;
 }
 
-// Groups a row: as few as fill the card (per_cu threads a CU), since each makes the row's angles anew
-// and a group that walks several heads has their loads on their way together.  The
-// forward takes 1 024 (65 539 bf16 rows of 8 + 2 heads: 84 us, with 4 096 99), the backward, whose
-// rows have twice the loads, 4 096.
-void set_groups(RopeArgs& a, int vw, int heads, int per_cu) {
+// Groups a row: as few as make 1 024 threads a CU, since each makes the row's angles anew
+// and a group that walks several heads has their loads on their way together.  (With groups for 4 096:
+// 65 539 bf16 rows of 8 + 2 heads of 128 forward 74 us for 70, backward 116 for 112; 49 664 of 4 + 4 of
+// 64 42 for 21 and 70 for 37.  The backward launches no more than 1 024 threads a CU, see bwd_blocks.)
+void set_groups(RopeArgs& a, int vw, int heads) {
     a.lps = ilog2_up((a.dh + 2 * vw - 1) / (2 * vw));
-    const long want = (long)cu_count() * per_cu;     // threads
+    const long want = (long)cu_count() * 1024;     // threads
     a.hgs = 0;
     while (a.lps + a.hgs < 8 && (1 << a.hgs) < heads && ((long)a.rows << (a.lps + a.hgs)) < want) ++a.hgs;
 }
@@ -475,7 +475,8 @@ int bwd_vw(const RopeArgs& a, int nblk, int vw, bool inter, const void* q, const
 #undef PT_ROPE_VW
 }
 
-// workgroups of the backward, at most: each leaves a part of dw
+// workgroups of the backward, at most: each leaves a part of dw, and walks its rows (four times as many:
+// 118 us for 113 over the 65 539 rows above, 43 for 37 over the 49 664)
 int bwd_blocks(const PtcgQkRope* d) {
     const long rows = (long)d->n * d->l;
     const long most = 4L * cu_count();
@@ -530,7 +531,7 @@ extern "C" int ptcg_kernel_qk_norm_rope_fwd(const PtcgQkRope* d, const void* q, 
     const PtcgHeadLayout* lays[] = {&a.q, &a.k, &a.qo, &a.ko};
     const void* ptrs[] = {q, k, qo, ko};
     const int vw = vector_width(a, es, lays, 4, ptrs, 4);
-    set_groups(a, vw, a.H + a.KV, 1024);
+    set_groups(a, vw, a.H + a.KV);
     PT_TRY(check_launch(a, who));
     const hipStream_t s = (hipStream_t)stream;
     return d->bf16 ? rope_vw<__bf16, false>(a, vw, d->rope.interleaved, q, k, nullptr, qo, ko, s)
@@ -569,7 +570,7 @@ extern "C" int ptcg_kernel_qk_norm_rope_bwd(const PtcgQkRope* d, const void* q, 
         const PtcgHeadLayout* lays[] = {&a.q, &a.k, &a.qo, &a.ko};
         const void* ptrs[] = {q, k, dqo, dko, dq, dk};
         const int vw = vector_width(a, es, lays, 4, ptrs, 6);
-        set_groups(a, vw, a.H + a.KV, 4096);
+        set_groups(a, vw, a.H + a.KV);
         const long full = pt_cdiv((long)a.rows << (a.lps + a.hgs), NTH);
         const int nblk = (int)(full < bwd_blocks(d) ? full : bwd_blocks(d));
         float* part = dw ? static_cast<float*>(workspace) : nullptr;
@@ -626,7 +627,7 @@ extern "C" int ptcg_kernel_paged_append(const PtcgPagedAppend* d, const void* q,
     const PtcgHeadLayout* lays[] = {&a.q, &a.k, &a.v, &a.qo, &a.pg.k, &a.pg.v};
     const void* ptrs[] = {q, k, v, qo, a.pg.kp, a.pg.vp};
     const int vw = vector_width(a, es, lays, 6, ptrs, 6);
-    set_groups(a, vw, a.H + 2 * a.KV, 1024);
+    set_groups(a, vw, a.H + 2 * a.KV);
     PT_TRY(check_launch(a, who));
     const hipStream_t s = (hipStream_t)stream;
     return d->bf16 ? rope_vw<__bf16, true>(a, vw, d->rope.interleaved, q, k, v, qo, nullptr, s)

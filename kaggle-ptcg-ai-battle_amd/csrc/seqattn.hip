@@ -1781,7 +1781,10 @@ struct BwdPlan {
 BwdPlan bwd_plan(const PtcgWindowAttn* d, const SArgs& a) {
     BwdPlan p = {};
     const int64_t rows = (int64_t)a.lq * a.G;
-    p.nw = rows <= 64 ? 2 : 4;
+    // Two waves for up to 64 rows, as the forward, where their instance holds its registers (512 x 64
+    // rows, 4 heads, both gradients: 32 wide 56 us against 64 in fp32, 32 against 36 in bf16; in fp32 64 and 128
+    // wide it spilled, 111 us against 108 and 404 against 375)
+    p.nw = rows <= 64 && (d->bf16 || a.dh <= 32) ? 2 : 4;
     p.q.qtiles = pt_cdiv(rows, 32 * p.nw);
     p.q.tiles = p.q.slots = a.n * p.q.qtiles;
     p.q.even = !a.q_off;
@@ -1862,7 +1865,9 @@ int launch_dkv(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t 
     return PTCG_OK;
 }
 template <typename T, int DH> int run_bwd(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
-    PT_TRY(p.nw == 2 ? (launch_dq<T, DH, 2>(a, p, g, s)) : (launch_dq<T, DH, 4>(a, p, g, s)));
+    if constexpr (sizeof(T) == 2 || DH <= 32)
+        PT_TRY(p.nw == 2 ? (launch_dq<T, DH, 2>(a, p, g, s)) : (launch_dq<T, DH, 4>(a, p, g, s)));
+    else PT_TRY((launch_dq<T, DH, 4>(a, p, g, s)));
     if constexpr (sizeof(T) == 2)
         if (p.dma)
             return p.nk == 2 ? launch_dkv<T, DH, 2, true>(a, p, g, s) : launch_dkv<T, DH, 4, true>(a, p, g, s);

@@ -427,7 +427,9 @@ int ptcg_kernel_paged_append(const PtcgPagedAppend* desc, const void* q, const v
  * sequence's length or where it has no page reaches nothing; NaN and infinities among the
  * values that it holds may reach those of its rows in the call that do not see them.
  * With G = heads / kv_heads, n (lq G / 32 + 2) kv_heads, or packed, if that is fewer,
- * (rows G / 32 + 2 n) kv_heads, is below 2^24, and lq G below 2^28 - 64.
+ * (rows G / 32 + 2 n) kv_heads, is below 2^24, and lq G below 2^28 - 64.  Packed
+ * sequences are gone through 64 at a time by every workgroup: of many thousand short
+ * ones the time grows with their square.
  * workspace of _ws_bytes (0: none, -1: refused), 16 B aligned, any contents; calls
  * that may run at the same time need scratch of their own.
  * No reference counterpart: its policy has no memory.                       */
@@ -454,7 +456,8 @@ int ptcg_kernel_paged_attention(const PtcgPagedAttn* desc, const void* q, void* 
  * infinities may reach other rows of their sequence.  dk and dv are summed over the
  * heads that share them, every sum in a fixed order: equal calls give equal bits.
  * Sizes as of ptcg_kernel_paged_attention, n (l G / 32 + 2) kv_heads < 2^24, packed
- * sequences too, whose rows the host does not know: l is best their longest.
+ * sequences too, whose rows the host does not know: l is best their longest (and of
+ * many thousand short ones padded sequences are the faster).
  * lse (n, heads, l) fp32 (nullable in the forward).  workspace of _ws_bytes (backward =
  * 0 / 1; 0: none, -1: refused), 16 B aligned, any contents.
  * No reference counterpart: its trunk attends in both directions.           */

@@ -11,8 +11,8 @@
 // where widths, strides and addresses let it.  The statistics are a sum over the
 // group.  An angle's cosine and sine serve a group for all the heads of its row
 // that it walks (hg groups a row share them): no table is read.  512 x 97 rows of 4 + 4
-// heads of 64 in fp32: forward 36 us (5.7 TB/s, read and written), backward 59 (5.2); 65 539 rows
-// of 8 + 2 heads of 128 in bf16: 69 (4.9) and 117 (4.3); 134 MB of new rows into pages and as much
+// heads of 64 in fp32: forward 35 us (5.8 TB/s, read and written), backward 58 (5.2); 65 539 rows
+// of 8 + 2 heads of 128 in bf16: 70 (4.8) and 113 (4.5); 134 MB of new rows into pages and as much
 // written: 58 (4.6).
 //
 // Angles: position times frequency and the reduction to a quarter turn are 64

@@ -104,7 +104,9 @@ struct Work { int i, qt, t0, t1, part, tile, per, next; };
 // tile, whole tiles, and the beginning of one; a tile that is cut leaves a part in each
 // of its stretches for the joining kernel: the stretch's first part, or its second
 // where the tile begins within the stretch.  The lengths are on the device
-// alone: every wave counts for itself, 64 sequences at a time.
+// alone: every wave counts for itself, 64 sequences at a time.  (Packed sequences that are not
+// cut are gone through in the same way to find a tile: 16 384 of up to 12 rows, 4 heads of 64, fp32,
+// take 2.0 ms forward, padded 0.26; 512 of up to 97 67 us and 63.)
 // (Counts of blocks fit 32 bits: the host splits nothing else.)
 struct Cut { int all, per, tiles; };
 
@@ -662,8 +664,10 @@ __device__ __forceinline__ bool shared_tile(Joint* js, const Work& w, int kvh, i
 // DMA: tiles go straight into one of two buffers while the other is worked on, one
 // barrier a tile; else through registers into one buffer.  Bound by its products, two
 // workgroups a CU taking turns at them: 4 sequences to 2 048 new rows over 30 000 keys, 8 heads of
-// 128 on 2, bf16, 542 to 563 us (915 to 950 TFLOP/s); 4 x 4 096 rows, 8 heads of 128, 143 us (960).
-// In fp32 the operands' terms and six products a product: 512 x 97 rows, 4 heads of 64, 62 us.
+// 128 on 2, bf16, 542 to 563 us (915 to 950 TFLOP/s).  Whole sequences of 4 096, 2 198, 3 371 and 1 473
+// rows padded to 4 096, 8 heads of 128: 143 us (503), bound by unequal tiles: these are not cut where there are
+// as many as workgroups run at once, and the longest, of 64 key blocks, takes 1.8 times an XCD's mean load.
+// In fp32 the operands' terms and six products a product: 512 sequences up to 97, 4 heads of 64, 62 us.
 template <typename T, int DH, int NW, bool PAGED, bool DMA>
 __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_fwd_kernel(const SArgs a_, const T* __restrict__ q,
         const T* __restrict__ k, const T* __restrict__ v, T* __restrict__ out, float* __restrict__ lse,
@@ -1106,8 +1110,9 @@ __device__ __forceinline__ void products(const __bf16* x0, const __bf16* x1, con
 // the order of its rows.  D_i is do_i . o_i of the output as it was stored; in bf16 its
 // rounding is the largest error of short rows' gradients (9 keys: 3.3e-3 in relative L2, 2.4e-3
 // without it), so there D_i is summed along the keys as well, for dK / dV, and for dQ too
-// where one tile holds all keys of the rows.  4 x 4 096 rows, 8 heads of 128, bf16: 200 us (1 030
-// TFLOP/s in three products); 512 x 97, 4 heads of 64, fp32: 81 us.
+// where one tile holds all keys of the rows.  The forward's four sequences, 8 heads of 128, bf16:
+// 200 us (540 TFLOP/s in three products; its tiles and their unequal load); 512 sequences up to 97, 4
+// heads of 64, fp32: 81 us.
 template <typename T, int DH, int NW> struct DqCfg {
     static constexpr bool DMA = sizeof(T) == 2, PAD = DH == 128 && !DMA;
     static constexpr int NTH = 64 * NW, BQ = 32 * NW, BK = 64;
@@ -1178,7 +1183,7 @@ __global__ __launch_bounds__(64 * NW, (waves_simd<T, DH>())) void seq_dq_kernel(
         constexpr bool sums = decltype(only)::value;
         const __bf16* Vs = Ks + C::TILE;
         // half a tile at a time: with both halves' dS on their way the kernel spills 128 wide
-        // (251 us against 204 over 4 x 4 096)
+        // (251 us against 204 over the four sequences above)
 #pragma unroll 1
         for (int j = 0; j < BK / 32; ++j) {
             const int key0 = rg.block(t) * BK + 32 * j;
@@ -1352,8 +1357,9 @@ template <typename T, int DH> constexpr int dkv_waves() {
 // dK and dV: a workgroup owns 32 NK keys of one kv head, a wave 32 of them, and
 // walks the flattened query rows that see them.  S = Q K^T and dP = dO V^T with
 // keys on lanes; dV^T += dO^T P and dK^T += Q^T dS read dO and Q transposed from LDS.
-// 4 x 4 096 rows, 8 heads of 128, bf16: 251 to 256 us (1 070 TFLOP/s in four products); 512 x 97, 4
-// heads of 64, fp32: 87 us.
+// The forward's four sequences, 8 heads of 128, bf16: 251 to 256 us (570 TFLOP/s in four products),
+// bound by unequal tiles as well: the first keys' is seen by 128 blocks of rows, where an XCD's mean load
+// is 70; 512 sequences up to 97, 4 heads of 64, fp32: 87 us.
 template <typename T, int DH, int NK, bool DMA>
 __global__ __launch_bounds__(64 * NK, (dkv_waves<T, DH>())) void seq_dkv_kernel(const SArgs a, const Grads<T> g,
                                                                                const DkvPlan pl) {

@@ -35,12 +35,12 @@ def _written(op, rest):
     if not op.startswith("v_"):
         return set()
     dst = rest.split(",")
-    n = 2 if "_co_" in op or "div_scale" in op else 1
+    n = 2 if "_co_" in op or op.startswith(("v_div_scale", "v_mad_u64", "v_mad_i64")) else 1
     return set().union(*(_regs(x) for x in dst[:n])) if op.startswith(("v_cmp", "v_read")) or n == 2 else set()
 
 
 def _blocks(lines):
-    """[(first line, instructions, labels that it may jump to, whether it may fall through)]"""
+    """[(instructions by line, labels that it may jump to, whether it may fall through)], and labels' blocks."""
     blocks, labels, cur = [], {}, []
 
     def close(to=(), falls=True):
@@ -74,10 +74,9 @@ def late_waits(asm):
     it reads."""
     blocks, labels = _blocks(asm.split("\n"))
     start, found = [{} for _ in blocks], {}
-    todo, seen = list(range(len(blocks))), set()
+    todo = list(range(len(blocks)))
     while todo:
         b = todo.pop()
-        seen.add(b)
         ins, to, falls = blocks[b]
         # wait states since a register's last write that matters
         state = dict(start[b])
@@ -103,7 +102,7 @@ def late_waits(asm):
             if new != old:
                 start[nb] = new
                 todo.append(nb)
-    return sorted((n + 1, i, r) for (n, r), i in found.items() for r in [str(r)])
+    return sorted((n + 1, i, str(r)) for (n, r), i in found.items())
 
 
 GOOD = """
@@ -126,6 +125,7 @@ _Z1kv:
     ("s_nop 4", "", "m0"), ("s_nop 4", "", "42"),
     ("s_nop 3", "s_nop 2", "41"),                       # by way of the loop
     ("s_nop 3", "v_cmp_lt_i32_e64 s[42:43], v1, v2", "43"),
+    ("s_nop 3", "v_mad_u64_u32 v[2:3], s[40:41], v4, v5, v[2:3]", "40"),
 ])
 def test_the_search_finds_a_missing_wait(was, put, want):
     assert late_waits(GOOD) == []

@@ -1792,10 +1792,10 @@ struct BwdPlan {
 BwdPlan bwd_plan(const PtcgWindowAttn* d, const SArgs& a) {
     BwdPlan p = {};
     const int64_t rows = (int64_t)a.lq * a.G;
-    // Two waves for up to 64 rows, as the forward, where their instance holds its registers (512 x 64
-    // rows, 4 heads, both gradients: 32 wide 56 us against 64 in fp32, 32 against 36 in bf16; in fp32 64 and 128
-    // wide it spilled, 111 us against 108 and 404 against 375)
-    p.nw = rows <= 64 && (d->bf16 || a.dh <= 32) ? 2 : 4;
+    // Two waves for up to 64 rows as in the forward, but where their instance spills (512 x 64 rows, 4 heads,
+    // both gradients: 32 wide 56 us against 64 in fp32, 32 against 36 in bf16, 64 wide 49 against 52; in fp32
+    // 64 and 128 wide, where it spilled, 111 us against 108 and 404 against 375; 128 wide in bf16 92 against 91)
+    p.nw = rows <= 64 && a.dh <= (d->bf16 ? 64 : 32) ? 2 : 4;
     p.q.qtiles = pt_cdiv(rows, 32 * p.nw);
     p.q.tiles = p.q.slots = a.n * p.q.qtiles;
     p.q.even = !a.q_off;
@@ -1876,7 +1876,7 @@ int launch_dkv(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t 
     return PTCG_OK;
 }
 template <typename T, int DH> int run_bwd(const SArgs& a, const BwdPlan& p, const Grads<T>& g, hipStream_t s) {
-    if constexpr (sizeof(T) == 2 || DH <= 32)
+    if constexpr (DH <= (sizeof(T) == 2 ? 64 : 32))
         PT_TRY(p.nw == 2 ? (launch_dq<T, DH, 2>(a, p, g, s)) : (launch_dq<T, DH, 4>(a, p, g, s)));
     else PT_TRY((launch_dq<T, DH, 4>(a, p, g, s)));
     if constexpr (sizeof(T) == 2)
